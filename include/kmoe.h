@@ -46,6 +46,11 @@ extern "C" {
 #define KMOE_DTYPE_BF16 0
 #define KMOE_DTYPE_F32 1
 #define KMOE_DTYPE_FP8_E4M3 2 /* OCP e4m3fn, saturating at +-448 */
+#define KMOE_DTYPE_FP4_E2M1 3 /* OCP e2m1: 0, .5, 1, 1.5, 2, 3, 4, 6 and their negatives; saturating */
+
+/* scores of kmoe_route_topk */
+#define KMOE_SCORES_SOFTMAX 0
+#define KMOE_SCORES_SIGMOID 1
 
 /* limits */
 #define KMOE_MAX_EXPERTS 64
@@ -535,6 +540,79 @@ int kmoe_combine_residual_dropout(const void* yperm, int d, const int32_t* src_r
                                   const uint8_t* keep, float keep_scale, int64_t T_out, void* y, int y_dtype,
                                   void* stream);
 
+
+/* ------------------------------------------------------------------------ */
+/* Routing of given logits (T, E) f32, E <= 64: for routers whose scores, groups or
+ * balance bias kmoe_router's own top-k does not cover (no counterpart in the
+ * reference, whose router renormalises a plain softmax top-k, moe.py:443-460).
+ *   s = softmax(logits) or sigmoid(logits); an expert whose logit is -inf is masked (s = 0)
+ *   c = s + bias (E f32, nullable), -inf where masked; NaN ranks above everything
+ *   groups: that many equal runs of experts; a group is worth the sum of its best
+ *     group_top (1 or 2) unmasked c; only the best topk_groups stay
+ *   topk_idx (T,k) int64: the k <= 8 largest c of those, equal c lowest index first;
+ *     masked experts come last
+ *   topk_w (T,k) f32: scale s, divided by (sum of the k chosen s + 1e-20) with renorm
+ * c and the group values are computed and compared in 64 bits.
+ * block_counts (nullable): the per-block histograms kmoe_router_hist writes,
+ * (ceil(T / kmoe_router_block_tokens(T)), E) int32, for kmoe_dispatch_counted.      */
+int kmoe_route_topk(const float* logits, int64_t T, int E, int k, int scores, const float* bias, int groups,
+                    int topk_groups, int group_top, int renorm, float scale, int64_t* topk_idx, float* topk_w,
+                    int32_t* block_counts, void* stream);
+/* Its backward from dw (T,k): dlogits (T,E) f32 written, or added to with accumulate.
+ * The choice is piecewise constant, so the bias gets no gradient.                  */
+int kmoe_route_topk_bwd(const float* logits, const int64_t* topk_idx, const float* dw, int64_t T, int E, int k,
+                        int scores, int renorm, float scale, int accumulate, float* dlogits, void* stream);
+
+/* Residual add, RMSNorm and microscaled rows in one pass (T rows of d):
+ *   h = x + delta in x's type, rrms = 1/sqrt(mean(h^2) + eps), n = bf16(weight * (h rrms))
+ *   (delta NULL: h is x and not written)
+ *   fmt fp8_e4m3 / fp4_e2m1: also q, scale = kmoe_quant_rows_mx of n (bf16: neither)
+ * x, delta, weight bf16 or f32; d a multiple of 8 (32 with fmt), <= 8192.  n is that of
+ * kmoe_rmsnorm on h bit for bit; its backward is kmoe_rmsnorm_bwd with dres the
+ * gradient of h: dx is then the gradient of x and of delta.                        */
+int kmoe_add_rmsnorm(const void* x, int x_dtype, const void* delta, int delta_dtype, const void* weight, int w_dtype,
+                     float eps, int64_t T, int d, void* h, void* n, float* rrms, int fmt, void* q, uint8_t* scale,
+                     void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Microscaled (OCP MX) experts: weights in e2m1, activations in e4m3 or e2m1 (`fmt`),
+ * blocks of 32 along K with a power-of-two scale byte (e8m0: 2^(byte - 127), 255 = NaN).
+ *   scale = 2^(floor(log2 amax) - emax), emax 8 (e4m3), 2 (e2m1), at least 2^-127;
+ *   codes: value / scale to nearest even, saturating.  A block with a NaN or an
+ *   infinity has scale 255 and stands for NaN.
+ * A coded row holds K values rounded up to a multiple of 128 (padding: zero codes):
+ * kmoe_mx_row_bytes(K, fmt) bytes of codes (e2m1: two to a byte, the first in the low
+ * half) and kmoe_mx_scale_bytes(K) scale bytes.                                    */
+size_t kmoe_mx_row_bytes(int K, int fmt);
+size_t kmoe_mx_scale_bytes(int K);
+/* Codes of bf16 rows x[row_index ? row_index[r] : r] (K a multiple of 32);
+ * n_rows_dev (nullable, device): rows past *n_rows_dev are left as they are.        */
+int kmoe_quant_rows_mx(const void* x, const int32_t* row_index, int64_t rows, const int32_t* n_rows_dev, int K,
+                       int fmt, void* q, uint8_t* scale, void* stream);
+/* The values (rows, K) bf16 of coded rows row_index[r] (or r); zeros for -1.        */
+int kmoe_dequant_rows_mx(const void* q, const uint8_t* scale, const int32_t* row_index, int64_t rows,
+                         const int32_t* n_rows_dev, int K, int fmt, void* out, void* stream);
+/* w (E, K, N) bf16 or f32 -> bf16 values of its e2m1 blocks along K (any K, a last
+ * block of fewer than 32 values): what kmoe_pack_weights_mx packs.                 */
+int kmoe_fake_quant_mx_cols(const void* w, int w_dtype, int E, int K, int N, void* out, void* stream);
+/* Packed 4-bit weights of w1, w2 (E, d, F), w3 (E, F, d): codes and scales in the
+ * products' operand order.  Sizes: kmoe_packed_mx_bytes, which = 0 w13, 1 its
+ * scales, 2 w3, 3 its scales.  d a multiple of 64, any F.                          */
+size_t kmoe_packed_mx_bytes(int E, int d, int F, int which);
+int kmoe_pack_weights_mx(const void* w1, const void* w2, const void* w3, int w_dtype, int E, int d, int F,
+                         void* w13_packed, uint8_t* w13_scale, void* w3_packed, uint8_t* w3_scale, void* stream);
+/* hq, h_scale = coded rows (K = F, padded columns zero) of silu(x w1) * (x w2) for the
+ * rows of each expert ([offsets[e], offsets[e+1]), device, offsets[E] <= max_rows).
+ * Permuted row r is coded row r of xq, or with row_token (device) row row_token[r] of
+ * its n_x_rows (-1: a zero row).
+ * gu (nullable; training): also the bf16 pre-activation gate / up values, (max_rows,
+ * 2 F_pad) in the order of kmoe_gemm_gate_up_rows_gu.  Rows past offsets[E] are left. */
+int kmoe_gemm_gate_up_mx(const void* xq, const uint8_t* x_scale, int fmt, int64_t n_x_rows, const int32_t* row_token,
+                         const int32_t* offsets, int E, int d, int F, int64_t max_rows, const void* w13_packed,
+                         const uint8_t* w13_scale, void* hq, uint8_t* h_scale, void* gu, void* stream);
+/* y (max_rows, d) bf16 = h w3 of those rows.                                       */
+int kmoe_gemm_down_mx(const void* hq, const uint8_t* h_scale, int fmt, const int32_t* offsets, int E, int d, int F,
+                      int64_t max_rows, const void* w3_packed, const uint8_t* w3_scale, void* y, void* stream);
 
 #ifdef __cplusplus
 }

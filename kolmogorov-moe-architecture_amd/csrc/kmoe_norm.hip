@@ -8,7 +8,9 @@
 // l, l + 64, ... of the row), so each row is read once; HBM-bound.  The training
 // forward materialises n (bf16): the backward's weight gradients need the normalised
 // rows, which the inference path's fold of g into the weights never writes.
-#include "kmoe_common.h"
+#include <type_traits>
+
+#include "kmoe_mx.h"
 
 namespace {
 
@@ -118,6 +120,71 @@ __global__ __launch_bounds__(64 * NORM_FWD_WAVES) void rmsnorm_kernel(const void
     if (lane == 0) mod_logits[t] = ml;
   }
   if (lane == 0) rrms[t] = r;
+}
+
+// h = x + delta rounded to x's type (without delta h is x, not written), n = bf16(g * (h r)), r = 1/sqrt(mean(h^2) + eps), all
+// from the rounded h (what the backward and the next block read), and n's microscaled rows
+// (Q 1: e4m3, 2: e2m1; 0: none).  The rows are those of the bf16 n, so the experts' products
+// see the values that the router sees, and the codes do not depend on the norm being fused.
+// Sums as in rmsnorm_kernel, so n is that of a torch addition followed by kmoe_rmsnorm, bit
+// for bit.  One wave per row.
+template <int NV, bool XF32, int Q>
+__global__ __launch_bounds__(64 * NORM_FWD_WAVES) void add_rmsnorm_kernel(
+    const void* __restrict__ x, const void* __restrict__ delta, bool delta_f32, const void* __restrict__ g, bool g_f32,
+    float eps, int64_t T, int d, void* __restrict__ h, uint16_t* __restrict__ n, float* __restrict__ rrms,
+    uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
+  const int lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * NORM_FWD_WAVES + (threadIdx.x >> 6);
+  if (t >= T) return;
+  const int nvec = d / 8;
+  float hv[NV][8];
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = lane + 64 * i;
+    if (v < nvec) {
+      float dv[8];
+      load8<XF32>(x, t * d + (int64_t)v * 8, hv[i]);
+      if (delta) {
+        load8_any(delta, delta_f32, t * d + (int64_t)v * 8, dv);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) {
+          hv[i][c] += dv[c];
+          if (!XF32) hv[i][c] = bf16_to_f32(f32_to_bf16(hv[i][c]));
+        }
+        store8<XF32>(h, t * d + (int64_t)v * 8, hv[i]);
+      }
+#pragma unroll
+      for (int c = 0; c < 8; ++c) ss = fmaf(hv[i][c], hv[i][c], ss);
+    }
+  }
+  ss = wave_sum(ss);
+  const float r = 1.0f / sqrtf(ss / (float)d + eps);
+  if (lane == 0) rrms[t] = r;
+  const int qvec = Q ? kmoe_mx::round_up(d, kmoe_mx::STEP) / 8 : nvec;  // with the padding of a coded row
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = lane + 64 * i;
+    if (v < qvec) {  // d is a multiple of 32 with Q: the four lanes of a block agree
+      float o[8] = {};
+      if (v < nvec) {
+        float gv[8];
+        load8_any(g, g_f32, (int64_t)v * 8, gv);
+#pragma unroll
+        for (int c = 0; c < 8; ++c) o[c] = bf16_to_f32(f32_to_bf16(gv[c] * (hv[i][c] * r)));
+        store8<false>(n, t * d + (int64_t)v * 8, o);
+      }
+      if constexpr (Q != 0) {
+        uint32_t code;
+        const kmoe_mx::Codes<Q == 2, 8> w = kmoe_mx::encode_quad<Q == 2>(o, code);
+        if constexpr (Q == 2)
+          *reinterpret_cast<uint32_t*>(q + t * (qvec * 4) + v * 4) = w.w[0];
+        else
+          *reinterpret_cast<i32x2_t*>(q + t * (qvec * 8) + v * 8) = i32x2_t{(int)w.w[0], (int)w.w[1]};
+        if ((v & 3) == 0) scale[t * (qvec / 4) + v / 4] = (uint8_t)code;
+      }
+    }
+  }
 }
 
 // One row's inputs as loaded (bf16: one 16-byte vector per 8 elements, f32: two).
@@ -309,6 +376,26 @@ __global__ void zero_words_kernel(uint16_t* __restrict__ p, int64_t n) {
   for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += (int64_t)gridDim.x * blockDim.x) p[i] = 0;
 }
 
+template <bool XF32, int Q>
+int launch_add_norm(const void* x, const void* delta, bool delta_f32, const void* g, bool g_f32, float eps, int64_t T, int d,
+                    void* h, uint16_t* n, float* rrms, uint8_t* q, uint8_t* scale, hipStream_t s) {
+  const dim3 grid((unsigned)kmoe::ceil_div<int64_t>(T, NORM_FWD_WAVES)), block(64 * NORM_FWD_WAVES);
+  const int nv = kmoe::ceil_div((Q ? kmoe_mx::round_up(d, kmoe_mx::STEP) : d) / 8, 64);
+#define KMOE_NORM_CASE(NVV)                                                                                          \
+  if (nv <= NVV) {                                                                                                   \
+    hipLaunchKernelGGL((add_rmsnorm_kernel<NVV, XF32, Q>), grid, block, 0, s, x, delta, delta_f32, g, g_f32, eps, T, \
+                       d, h, n, rrms, q, scale);                                                                     \
+    return KMOE_OK;                                                                                                  \
+  }
+  KMOE_NORM_CASE(1)
+  KMOE_NORM_CASE(2)
+  KMOE_NORM_CASE(4)
+  KMOE_NORM_CASE(8)
+  KMOE_NORM_CASE(16)
+#undef KMOE_NORM_CASE
+  return KMOE_ERR_UNSUPPORTED;
+}
+
 bool is_float_dtype(int dt) { return dt == KMOE_DTYPE_BF16 || dt == KMOE_DTYPE_F32; }
 
 }  // namespace
@@ -333,6 +420,38 @@ extern "C" int kmoe_rmsnorm(const void* x, int x_dtype, const void* weight, int 
           : launch_norm<false>(x, weight, g_f32, eps, T, d, static_cast<uint16_t*>(n), rrms, wm, mod_logits, s);
   if (rc != KMOE_OK) return rc;
   return kmoe::check_launch("kmoe_rmsnorm");
+}
+
+extern "C" int kmoe_add_rmsnorm(const void* x, int x_dtype, const void* delta, int delta_dtype, const void* weight,
+                                int w_dtype, float eps, int64_t T, int d, void* h, void* n, float* rrms, int fmt, void* q,
+                                uint8_t* scale, void* stream) {
+  KMOE_REQUIRE(weight && (T == 0 || (x && n && rrms && (!delta || h))), KMOE_ERR_NULL, "kmoe_add_rmsnorm: null buffer");
+  KMOE_REQUIRE(is_float_dtype(x_dtype) && is_float_dtype(delta_dtype) && is_float_dtype(w_dtype), KMOE_ERR_DTYPE,
+               "kmoe_add_rmsnorm: dtypes %d/%d/%d", x_dtype, delta_dtype, w_dtype);
+  const bool coded = fmt == KMOE_DTYPE_FP8_E4M3 || fmt == KMOE_DTYPE_FP4_E2M1;
+  KMOE_REQUIRE(coded || fmt == KMOE_DTYPE_BF16, KMOE_ERR_DTYPE, "kmoe_add_rmsnorm: element type %d of the coded rows", fmt);
+  KMOE_REQUIRE(!coded || T == 0 || (q && scale), KMOE_ERR_NULL, "kmoe_add_rmsnorm: coded rows need q and scale");
+  KMOE_REQUIRE(T >= 0 && T < (int64_t)1 << 31 && d > 0 && d % 8 == 0 && (!coded || d % kmoe_mx::BLOCK == 0), KMOE_ERR_SHAPE,
+               "kmoe_add_rmsnorm: d=%d must be a positive multiple of %d", d, coded ? kmoe_mx::BLOCK : 8);
+  KMOE_REQUIRE(d <= 8192, KMOE_ERR_UNSUPPORTED, "kmoe_add_rmsnorm: d=%d > 8192", d);
+  KMOE_REQUIRE(eps >= 0.0f, KMOE_ERR_SHAPE, "kmoe_add_rmsnorm: eps must be >= 0");
+  if (T == 0) return KMOE_OK;
+  hipStream_t s = kmoe::as_stream(stream);
+  const bool g_f32 = w_dtype == KMOE_DTYPE_F32, d_f32 = delta_dtype == KMOE_DTYPE_F32;
+  uint16_t* np = static_cast<uint16_t*>(n);
+  uint8_t* qp = static_cast<uint8_t*>(q);
+  auto with = [&](auto xf32, auto qt) {
+    return launch_add_norm<decltype(xf32)::value, decltype(qt)::value>(x, delta, d_f32, weight, g_f32, eps, T, d, h, np, rrms,
+                                                                       qp, scale, s);
+  };
+  auto by_x = [&](auto qt) {
+    return x_dtype == KMOE_DTYPE_F32 ? with(std::true_type{}, qt) : with(std::false_type{}, qt);
+  };
+  const int rc = !coded                       ? by_x(std::integral_constant<int, 0>{})
+                 : fmt == KMOE_DTYPE_FP8_E4M3 ? by_x(std::integral_constant<int, 1>{})
+                                              : by_x(std::integral_constant<int, 2>{});
+  if (rc != KMOE_OK) return rc;
+  return kmoe::check_launch("kmoe_add_rmsnorm");
 }
 
 extern "C" size_t kmoe_rmsnorm_bwd_workspace_bytes(int64_t T, int d) {

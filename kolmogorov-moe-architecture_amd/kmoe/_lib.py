@@ -19,6 +19,8 @@ KMOE_ERR_SHAPE = -2
 DTYPE_BF16 = 0
 DTYPE_F32 = 1
 DTYPE_FP8_E4M3 = 2
+DTYPE_FP4_E2M1 = 3
+SCORES = {"softmax": 0, "sigmoid": 1}
 MAX_EXPERTS = 64
 ROUTER_HIDDEN = 128
 
@@ -107,6 +109,19 @@ _SIGNATURES = {
     "kmoe_router_mlp_bwd": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _sz, _vp]),
     "kmoe_packed_w_in_t_bytes": (_sz, [_i32]),
     "kmoe_pack_w_in_t": (_i32, [_vp, _i32, _i32, _vp, _vp]),
+    # routing of logits, residual add + norm, microscaled experts
+    "kmoe_route_topk": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _i32, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp]),
+    "kmoe_route_topk_bwd": (_i32, [_vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _vp]),
+    "kmoe_add_rmsnorm": (_i32, [_vp, _i32, _vp, _i32, _vp, _i32, _f32, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
+    "kmoe_mx_row_bytes": (_sz, [_i32, _i32]),
+    "kmoe_mx_scale_bytes": (_sz, [_i32]),
+    "kmoe_quant_rows_mx": (_i32, [_vp, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _vp]),
+    "kmoe_dequant_rows_mx": (_i32, [_vp, _vp, _vp, _i64, _vp, _i32, _i32, _vp, _vp]),
+    "kmoe_fake_quant_mx_cols": (_i32, [_vp, _i32, _i32, _i32, _i32, _vp, _vp]),
+    "kmoe_packed_mx_bytes": (_sz, [_i32, _i32, _i32, _i32]),
+    "kmoe_pack_weights_mx": (_i32, [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "kmoe_gemm_gate_up_mx": (_i32, [_vp, _vp, _i32, _i64, _vp, _vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "kmoe_gemm_down_mx": (_i32, [_vp, _vp, _i32, _vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp, _vp]),
 }
 
 

@@ -123,7 +123,8 @@ class Saved(NamedTuple):
     h: torch.Tensor          # (A, F_pad) bf16 (fp8 experts: dequantised from the down GEMM's e4m3 rows)
     gu: torch.Tensor         # (A, 2 F_pad) bf16 pre-activation gate / up
     yperm: torch.Tensor      # (A, d) bf16 expert outputs
-    xperm: torch.Tensor      # (A, d) bf16 permuted input rows (fp8: dequantised e4m3 rows)
+    xperm: torch.Tensor      # (A, d) bf16 permuted input rows (fp8, microscaled: dequantised rows)
+    spec: Optional["ops.RouteSpec"] = None  # of logits that ops.route_topk routed
 
 
 class Grads(NamedTuple):
@@ -311,6 +312,23 @@ def _ones(T, fan, dev):
     return t
 
 
+def _route_dlogits(logits, idx, w, dw, spec, counts=None, ga=None, w_lb=0.0, w_z=0.0):
+    """Logit gradient (T, E) f32 of the routing weights' gradient dw and, with ga, of the aux
+    losses: the router kernel's own top-k (spec None) or ops.route_topk's."""
+    T, E = logits.shape
+    k = idx.shape[1]
+    dl = torch.empty(T, E, device=logits.device, dtype=torch.float32)
+    if spec is not None and ga is None:
+        return ops.route_topk_bwd(logits, idx, dw, spec.scores, spec.renorm, spec.scale) if T else dl
+    with _stage("bwd_router"):
+        # (with a spec only the aux part: zero weights' gradients)
+        _lib.call("kmoe_router_dlogits", ptr(logits), T, E, ptr(idx), ptr(w), ptr(dw if spec is None else torch.zeros_like(dw)),
+                  k, ptr(counts), ptr(ga), float(w_lb), float(w_z), ptr(dl), ops._stream(logits))
+    if spec is not None:
+        ops.route_topk_bwd(logits, idx, dw, spec.scores, spec.renorm, spec.scale, dlogits=dl)
+    return dl
+
+
 def _token_choice_core(sv: Saved, dy, grad_aux, w_out, bw: BwdWeights, E, F, w_lb, w_z, need_weights,
                        extra_rows=0, row_index=None, scale=None):
     """Expert path and router of a token-choice layer backward: dxp (A + T + extra_rows, d)
@@ -327,11 +345,8 @@ def _token_choice_core(sv: Saved, dy, grad_aux, w_out, bw: BwdWeights, E, F, w_l
                                                  disp.offsets, A, bw, E, F, extra_rows=T + extra_rows,
                                                  row_index=row_index, scale=scale)
     # router: logit gradient (top-k renormalisation + aux), MLP backward, dx rows, dW_in
-    dl = torch.empty(T, E, device=dev, dtype=torch.float32)
     ga = None if grad_aux is None else grad_aux.reshape(1).to(torch.float32).contiguous()
-    with _stage("bwd_router"):
-        _lib.call("kmoe_router_dlogits", ptr(sv.logits), T, E, ptr(sv.idx), ptr(sv.w), ptr(dw), k,
-                  ptr(disp.counts), ptr(ga), float(w_lb), float(w_z), ptr(dl), s)
+    dl = _route_dlogits(sv.logits, sv.idx, sv.w, dw, sv.spec, disp.counts, ga, w_lb, w_z)
     dw_in, dw_out = _router_core(x2d, sv.hidden, w_out, bw, dl, dxp[A:A + T], need_weights)
     return dxp, dscale, dw_in, dw_out, dyperm, dgu
 
@@ -481,18 +496,14 @@ def experts_backward(dy, yperm, gu, h, xperm, slot_row, slot_w, offsets, A, bw: 
     return dx, dw, dw1, dw2, dw3
 
 
-def router_backward(x2d, logits, idx, w, hidden, dw, dlogits_in, w_out, bw: BwdWeights, need_weights=True):
+def router_backward(x2d, logits, idx, w, hidden, dw, dlogits_in, w_out, bw: BwdWeights, need_weights=True, spec=None):
     """Backward of Router.forward alone (moe.py:423-462): from the gradients of its top-k
-    weights dw (T, k) and of its logits (T, E, nullable) to (dx, dw_in, dw_out)."""
+    weights dw (T, k) and of its logits (T, E, nullable) to (dx, dw_in, dw_out).  spec: of
+    logits that ops.route_topk routed."""
     T, d = x2d.shape
     E = logits.shape[1]
-    k = idx.shape[1]
     dev = x2d.device
-    s = ops._stream(x2d)
-    dl = torch.empty(T, E, device=dev, dtype=torch.float32)
-    with _stage("bwd_router"):
-        _lib.call("kmoe_router_dlogits", ptr(logits), T, E, ptr(idx), ptr(w), ptr(dw), k, None, None, 0.0, 0.0,
-                  ptr(dl), s)
+    dl = _route_dlogits(logits, idx, w, dw, spec)
     if dlogits_in is not None:
         dl += dlogits_in.reshape(T, E).to(torch.float32)
     dx = torch.empty(T, d, device=dev, dtype=_BF16)

@@ -60,6 +60,35 @@ class RMSNorm(nn.Module):
         return self.weight * (x / rms)
 
 
+class _AddNormFn(torch.autograd.Function):
+    """ops.add_rmsnorm with the norm's HIP backward: the gradient of h plus the norm's goes to
+    x and to delta."""
+
+    @staticmethod
+    def forward(ctx, x, delta, weight, eps):
+        d = x.shape[-1]
+        r = ops.add_rmsnorm(x.detach().reshape(-1, d), delta.detach().reshape(-1, d), weight, eps)
+        ctx.save_for_backward(r.h, r.rrms, weight)
+        ctx.meta = (x.shape, x.dtype, delta.dtype)
+        return r.h.view(x.shape), r.n.view(x.shape)
+
+    @staticmethod
+    def backward(ctx, dh, dn):
+        h, rrms, weight = ctx.saved_tensors
+        shape, x_dtype, delta_dtype = ctx.meta
+        ds, dg = ops.rmsnorm_bwd(dn.reshape(h.shape), h, weight, rrms, dres=dh.reshape(h.shape))
+        ds = ds.view(shape)
+        return ds.to(x_dtype), ds.to(delta_dtype), dg, None
+
+
+def add_rms_norm(x: torch.Tensor, delta: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5):
+    """(h, n): h = x + delta and n = RMSNorm(h) (bf16) in one pass, differentiable in x, delta
+    and weight (bf16 or f32; the residual stream h has x's type, or f32 with an f32 delta)."""
+    if x.shape != delta.shape:
+        raise ValueError(f"kmoe.add_rms_norm: x {tuple(x.shape)}, delta {tuple(delta.shape)}")
+    return _AddNormFn.apply(x, delta, weight, eps)
+
+
 def get_norm_layer(config) -> nn.Module:
     """Norm layer of the config (embeddings.py:196-212)."""
     norm_type = getattr(config, "norm_type", "rmsnorm")
@@ -103,9 +132,24 @@ class MoEFFNBlock(nn.Module):
             return False
         if ffn.grouped_experts.use_fp8 or ffn.router.balanced_routing or not ffn.grouped_experts.gated:
             return False
+        if ffn.grouped_experts.mx is not None or ffn.router.spec is not None:
+            return False
         if torch.is_grad_enabled() and (h.requires_grad or any(p.requires_grad for p in self.parameters())):
             return False
         return torch.promote_types(h.dtype, self.ffn_norm.weight.dtype) in (torch.bfloat16, torch.float32)
+
+    def _mx_fusable(self, h: torch.Tensor) -> bool:
+        """Whether the forward without gradients takes the norm's microscaled rows."""
+        ffn = self.ffn
+        if not isinstance(self.ffn_norm, RMSNorm) or ffn.routing_type == "expert_choice" or ffn.grouped_experts.mx is None:
+            return False
+        if torch.is_grad_enabled() and (h.requires_grad or any(p.requires_grad for p in self.parameters())):
+            return False
+        return self._dropout_off() and h.shape[-1] <= 8192 and torch.promote_types(
+            h.dtype, self.ffn_norm.weight.dtype) in (torch.bfloat16, torch.float32)
+
+    def _dropout_off(self) -> bool:
+        return not self.training or float(self.residual_dropout.p) <= 0.0
 
     def _dropout_keep(self, T, d, device):
         """(keep mask or None, 1/(1-p)) of this forward's residual dropout."""
@@ -150,8 +194,20 @@ class MoEFFNBlock(nn.Module):
         return h.dtype in (torch.bfloat16, torch.float32) and self.ffn_norm.weight.dtype in (torch.bfloat16,
                                                                                                torch.float32)
 
-    def forward(self, hidden_states: torch.Tensor) -> torch.Tensor:
+    def forward(self, hidden_states: torch.Tensor, delta: torch.Tensor = None) -> torch.Tensor:
+        """out = h + residual_dropout(ffn(ffn_norm(h))) with h = hidden_states, or with `delta` (the
+        attention half's output, not yet added to the stream) h = hidden_states + delta."""
         use_mod = self.ffn_mod_router is not None and self.training
+        if delta is not None and delta.shape != hidden_states.shape:
+            raise ValueError(f"kmoe.MoEFFNBlock: hidden_states {tuple(hidden_states.shape)}, delta {tuple(delta.shape)}")
+        if not use_mod and self._mx_fusable(hidden_states) and not (torch.is_grad_enabled() and delta is not None
+                                                                    and delta.requires_grad):
+            out = self._forward_mx(hidden_states, delta)
+            self.last_path = "fused_mx"
+            self.aux_loss = self.ffn.aux_loss if self.training else 0.0
+            return out
+        if delta is not None:
+            hidden_states = hidden_states + delta
         if self._train_fusable(hidden_states):
             ffn, ge = self.ffn, self.ffn.grouped_experts
             w_mod = self.ffn_mod_router.router.weight if use_mod else None
@@ -197,6 +253,21 @@ class MoEFFNBlock(nn.Module):
         y = ops.combine(yperm, disp.slot_row.view(T, k), disp.slot_w.view(T, k), T, out_dtype=out_dtype,
                         residual=x2d, keep_mask=keep, keep_scale=keep_scale)
         ffn._set_token_choice_aux(r, disp, T)
+        return y.view(B, S, d)
+
+
+    def _forward_mx(self, h: torch.Tensor, delta: torch.Tensor) -> torch.Tensor:
+        """Microscaled experts without gradients: one pass adds delta, norms and codes the rows;
+        the router reads the norm's bf16 rows, the experts their codes, the combine adds h."""
+        ffn = self.ffn
+        B, S, d = h.shape
+        T = B * S
+        r = ops.add_rmsnorm(h.reshape(T, d), None if delta is None else delta.reshape(T, d), self.ffn_norm.weight,
+                            self.ffn_norm.eps, quant=ffn.grouped_experts.mx_act)
+        out_dtype = torch.promote_types(r.h.dtype, self.ffn_norm.weight.dtype)
+        y, rt, disp = ffn.forward_rows(r.n, T, out_dtype=out_dtype, residual=r.h,
+                                       coded=ops.MXRows(r.q, r.scale, d, ffn.grouped_experts.mx_act))
+        ffn._set_token_choice_aux(rt, disp, T)
         return y.view(B, S, d)
 
 

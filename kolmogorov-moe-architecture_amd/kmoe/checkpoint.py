@@ -121,8 +121,8 @@ def save_packed(experts, path: str) -> None:
     """Write the experts' packed weights (GroupedExperts / GroupedExpertsExpertChoice,
     bf16 or fp8 with scales), the source fingerprint and the packed layout's version
     and sizes to a safetensors file.  Gated (swiglu) experts only."""
-    if not getattr(experts, "gated", True):
-        raise ValueError("kmoe: packed-weight files hold gated (swiglu) experts only")
+    if not getattr(experts, "gated", True) or experts.mx is not None:
+        raise ValueError("kmoe: packed-weight files hold gated (swiglu) bf16 or fp8 experts only")
     pw = experts.packed()
     tensors = {"w13": pw.w13, "w3": pw.w3}
     if pw.fp8:
@@ -138,8 +138,8 @@ def packed_file_matches(experts, path: str) -> bool:
     (layout and ABI versions, buffer sizes).  Reads the metadata and tensor shapes only."""
     from safetensors import safe_open
 
-    if not getattr(experts, "gated", True):
-        return False  # packed-weight files hold gated (swiglu) experts only
+    if not getattr(experts, "gated", True) or experts.mx is not None:
+        return False  # packed-weight files hold gated (swiglu) bf16 or fp8 experts only
     with safe_open(path, framework="pt") as f:
         meta = f.metadata() or {}
         if meta.get("kmoe_packed") != "1":

@@ -50,6 +50,21 @@ class AdvancedMoEConfig:
     # Expert GEMMs on fp8 e4m3 with per-token activation scales and
     # per-expert per-output-row weight scales.
     moe_fp8: bool = False
+    # Expert GEMMs on microscaled 4-bit weights (blocks of 32 along K, power-of-two scales):
+    # "w4a8" with e4m3 activations, "w4a4" with e2m1 ones, in such blocks too.
+    moe_mx: Optional[str] = None
+    # Routing (token choice): scores "softmax" or "sigmoid"; moe_router_groups equal runs of
+    # experts, of which the best moe_router_topk_groups stay (a group is worth the sum of its
+    # best moe_router_group_top choices); weights divided by their sum (renorm), times scale.
+    moe_router_scores: str = "softmax"
+    moe_router_groups: int = 1
+    moe_router_topk_groups: int = 1
+    moe_router_group_top: int = 2
+    moe_router_renorm: bool = True
+    moe_router_scale: float = 1.0
+    # A bias for balance: Router.balance_bias (E f32, a buffer that starts at zero and that the
+    # training program moves) is added to the scores for the choice of experts only.
+    moe_balance_bias: bool = False
     # Optional per-expert logit bias added before the softmax (E floats).
     moe_router_bias: Optional[Sequence[float]] = None
 

@@ -99,8 +99,26 @@ class _RouterMLP(nn.Module):
         return self._bf16_cache[1], self._bf16_cache[2]
 
 
+def _route_spec(config) -> Optional[ops.RouteSpec]:
+    """The configuration's RouteSpec, None where it is the plain renormalised softmax top-k."""
+    d = ops.RouteSpec()
+    spec = ops.RouteSpec(*(type(v)(getattr(config, "moe_router_" + n, v)) for n, v in zip(d._fields, d)))
+    if spec._replace(group_top=d.group_top) == d:
+        return None  # one group: its value does not matter
+    ops._scores(spec.scores)
+    E, k = int(config.n_experts), int(config.moe_top_k)
+    if spec.groups < 1 or E % spec.groups or not 1 <= spec.topk_groups <= spec.groups or spec.group_top not in (1, 2):
+        raise ValueError(f"kmoe.Router: {spec.groups} groups of {E} experts, {spec.topk_groups} kept, by their best "
+                         f"{spec.group_top}: groups must divide the experts, the kept ones lie in 1..groups, and the "
+                         f"best be 1 or 2")
+    if k > spec.topk_groups * (E // spec.groups):
+        raise ValueError(f"kmoe.Router: moe_top_k={k} exceeds the experts of {spec.topk_groups} kept groups")
+    return spec
+
+
 class Router(_RouterMLP):
-    """Token-choice top-k router (moe.py:327-462)."""
+    """Token-choice top-k router (moe.py:327-462), with the scores, groups and balance bias of
+    the configuration's moe_router_* fields."""
 
     def __init__(self, config: AdvancedMoEConfig):
         super().__init__(config.d_model, config.n_experts)
@@ -111,6 +129,26 @@ class Router(_RouterMLP):
         bias = getattr(config, "moe_router_bias", None)
         # fp32 per-expert logit bias (kept out of the state dict and of dtype casts)
         self.logit_bias = None if bias is None else torch.tensor(list(bias), dtype=torch.float32)
+        # how logits become experts and weights; None: the router kernel's own top-k
+        self.spec = _route_spec(config)
+        # added to the scores for the choice only; moved by the training program (kept in fp32
+        # by dtype casts, in the state dict)
+        self.register_buffer("balance_bias", torch.zeros(config.n_experts, dtype=torch.float32)
+                             if getattr(config, "moe_balance_bias", False) else None)
+        if self.balance_bias is not None and self.spec is None:
+            self.spec = ops.RouteSpec()
+        if self.spec is not None and self.balanced_routing:
+            raise ValueError("kmoe.Router: moe_balanced_routing has its own assignment; scores, groups, renorm, scale "
+                             "and the balance bias do not apply to it")
+
+    def _apply(self, fn, recurse=True):
+        bias = self.balance_bias
+        super()._apply(fn, recurse)
+        if bias is not None and self.balance_bias.dtype != torch.float32:
+            new = self.balance_bias
+            self.balance_bias = (torch.empty_like(new, dtype=torch.float32) if bias.is_meta or new.is_meta
+                                 else bias.to(new.device))
+        return self
 
     def device_bias(self, x2d: torch.Tensor) -> Optional[torch.Tensor]:
         """The fp32 logit bias on x2d's device, or None."""
@@ -129,6 +167,10 @@ class Router(_RouterMLP):
             r = ops.router(x2d, w_in, w_out, 0, bias=bias, row_index=row_index, T=T, save_hidden=save_hidden)
             idx, w = ops.balanced_topk(r.logits, self.top_k)
             return ops.RouterOut(r.logits, idx, w, r.partials, r.hidden)
+        if self.spec is not None:
+            r = ops.router(x2d, w_in, w_out, 0, bias=bias, row_index=row_index, T=T, save_hidden=save_hidden)
+            rt = ops.route_topk(r.logits, self.top_k, bias=self.balance_bias, hist=hist, **self.spec._asdict())
+            return ops.RouterOut(r.logits, rt.idx, rt.w, r.partials, r.hidden, None, rt.block_counts)
         return ops.router(x2d, w_in, w_out, self.top_k, bias=bias, row_index=row_index, T=T, save_hidden=save_hidden,
                           hist=hist)
 
@@ -198,12 +240,27 @@ class _PackedExperts(nn.Module):
         _init_expert_weights(self.w1, self.w2, self.w3)
         self._packed = None
         self.use_fp8 = False
+        # microscaled experts: "w4a8", "w4a4" or None
+        self.mx = None
 
     def _weights(self):
         return tuple(w for w in (self.w1, self.w2, self.w3) if w is not None)
 
     def _packed_key(self):
-        return tuple((w.data_ptr(), w._version, w.device) for w in self._weights()) + (self.use_fp8,)
+        return tuple((w.data_ptr(), w._version, w.device) for w in self._weights()) + (self.use_fp8, self.mx)
+
+    @property
+    def mx_act(self) -> Optional[str]:
+        """Element type of the microscaled experts' activations, None without them."""
+        if self.mx is None:
+            return None
+        if self.mx not in ops.MX_EXPERTS:
+            raise ValueError(f"kmoe: microscaled experts are one of {sorted(ops.MX_EXPERTS)}, not {self.mx!r}")
+        if self.use_fp8:
+            raise ValueError("kmoe: experts are either fp8 or microscaled, not both")
+        if not self.gated:
+            raise NotImplementedError("kmoe: microscaled experts are implemented for swiglu only")
+        return ops.MX_EXPERTS[self.mx]
 
     def cast_grads(self, dw1, dw2, dw3):
         """The weight gradients in the parameters' dtypes (dw3 None for non-gated experts)."""
@@ -220,6 +277,17 @@ class _PackedExperts(nn.Module):
         with save h and the input rows dequantised (bf16, the values the fp8 GEMMs
         took: the straight-through backward's operands) and the descaled gate/up values."""
         pw = self.packed()
+        if self.mx is not None:
+            # row_token[r] of x2d, quantised once per token; the operands come back dequantised
+            xq = ops.quant_rows_mx(x2d, self.mx_act)
+            if not save:
+                return ops.gemm_down_mx(ops.gemm_gate_up_mx(xq, row_token, offsets, pw, A), offsets, pw, A), None, None, None
+            h, gu = ops.gemm_gate_up_mx(xq, row_token, offsets, pw, A, save_gu=True)
+            n_dev = offsets[self.n_experts:]
+            yperm = ops.gemm_down_mx(h, offsets, pw, A)
+            # (h's padded columns come back too: the weight gradient reads whole rows)
+            hv = ops.dequant_rows_mx(h._replace(K=gu.shape[1] // 2), n_rows_dev=n_dev)
+            return yperm, hv, gu, ops.dequant_rows_mx(xq, row_token[:A], n_rows_dev=n_dev)
         if self.use_fp8:
             if not save:
                 return ops.grouped_ffn(xperm, xscale, offsets, pw, A), None, None, None
@@ -240,6 +308,8 @@ class _PackedExperts(nn.Module):
         """The expert weights the backward multiplies by: the parameters, or for fp8
         experts the fake-quantised ones the fp8 GEMMs used (straight-through: their
         gradients go to the parameters unchanged)."""
+        if self.mx is not None:
+            return tuple(ops.fake_quant_mx_cols(w) for w in (self.w1, self.w2, self.w3))
         if not self.use_fp8:
             return self.w1, self.w2, self.w3
         return tuple(ops.fake_quant_cols_e4m3(w) for w in (self.w1, self.w2, self.w3))
@@ -247,15 +317,15 @@ class _PackedExperts(nn.Module):
     def install_packed(self, pw: ops.PackedWeights) -> None:
         """Use `pw` (packed from exactly the current w1/w2/w3, e.g. read back from disk)
         until a parameter changes."""
-        if not self.gated:
-            raise ValueError("kmoe: packed-weight files hold gated (swiglu) experts only")
+        if not self.gated or self.mx is not None:
+            raise ValueError("kmoe: packed-weight files hold gated (swiglu) bf16 or fp8 experts only")
         if (pw.E, pw.d, pw.F, pw.fp8) != (self.n_experts, self.d_model, self.d_ff, self.use_fp8):
             raise ValueError("kmoe: packed weights do not match the experts' shapes / fp8 mode")
         self._packed = (self._packed_key(), pw)
 
     def bwd_packed(self) -> _bwd.BwdWeights:
         """Backward packed weights (no router part), rebuilt only when a parameter changed."""
-        key = tuple((w.data_ptr(), w._version) for w in self._weights()) + (self.use_fp8,)
+        key = tuple((w.data_ptr(), w._version) for w in self._weights()) + (self.use_fp8, self.mx)
         cache = getattr(self, "_bwd_cache", None)
         if cache is None or cache[0] != key:
             with torch.no_grad():
@@ -276,7 +346,9 @@ class _PackedExperts(nn.Module):
         key = self._packed_key()
         if self._packed is None or self._packed[0] != key:
             with torch.no_grad():
-                if not self.gated:
+                if self.mx_act is not None:
+                    pw = ops.pack_weights_mx(self.w1.detach(), self.w2.detach(), self.w3.detach())
+                elif not self.gated:
                     if self.use_fp8:
                         raise NotImplementedError("kmoe: fp8 non-gated experts are not implemented")
                     pw = ops.pack_weights_plain(self.w1.detach(), self.w2.detach())
@@ -290,18 +362,26 @@ class GroupedExperts(_PackedExperts):
     """Token-choice grouped SwiGLU experts (moe.py:161-294)."""
 
     def run(self, x2d, expert_indices, expert_weights, row_index=None, T_out=None, out_map=None, scale=None,
-            out_dtype=torch.bfloat16, residual=None, capacity=0, block_counts=None, aux=None):
+            out_dtype=torch.bfloat16, residual=None, capacity=0, block_counts=None, aux=None, coded=None):
         """dispatch -> grouped GEMMs -> combine (+ residual, added in the combine); returns (y, DispatchOut).
         capacity > 0 drops each expert's assignments past the first `capacity` (MoELayer's
         drop_overflow rule); 0, the default and what forward() uses, drops nothing (the
         reference's GroupedExperts never drops).  block_counts: the router's per-block
         histograms of expert_indices (RouterOut.block_counts), if it wrote them.
         aux = (partials, w_lb, w_z): the dispatch also computes the aux losses
-        (DispatchOut.aux; needs block_counts)."""
+        (DispatchOut.aux; needs block_counts).  coded (microscaled experts): the rows' codes,
+        quant_rows_mx(x2d), if the caller has them (the norm's)."""
         E = self.n_experts
         pw = self.packed()
         T, k = expert_indices.shape
-        if pw.fp8:
+        if self.mx is not None:
+            disp = ops.dispatch(x2d, expert_indices, expert_weights, E, capacity=capacity, row_index=row_index,
+                                materialize=False, block_counts=block_counts, aux=aux)
+            if coded is None:
+                coded = ops.quant_rows_mx(x2d, self.mx_act, row_index=row_index)
+            h = ops.gemm_gate_up_mx(coded, disp.row_token, disp.offsets, pw, T * k)
+            yperm = ops.gemm_down_mx(h, disp.offsets, pw, T * k)
+        elif pw.fp8:
             disp = ops.dispatch(x2d, expert_indices, expert_weights, E, capacity=capacity, fp8=True,
                                 row_index=row_index, block_counts=block_counts, aux=aux)
             yperm = ops.grouped_ffn(disp.xperm, disp.xscale, disp.offsets, pw, T * k)
@@ -325,6 +405,8 @@ class GroupedExperts(_PackedExperts):
         if self._trainable(x, expert_weights):
             return _ExpertsFn.apply(x, expert_weights, self.w1, self.w2, self.w3, self, expert_indices)
         out_dtype = torch.float32 if x.dtype == torch.float32 else torch.bfloat16
+        if self.mx is not None and x.shape[0] == 0:
+            return x.new_empty(0, self.d_model)
         y, _ = self.run(x, expert_indices, expert_weights, out_dtype=out_dtype)
         return _forward_only(y.to(x.dtype), x, self.w1, self.w2, self.w3, expert_weights)
 
@@ -335,7 +417,9 @@ class GroupedExpertsExpertChoice(_PackedExperts):
     def run(self, x2d, sel: ops.ECSelectOut, B, S, C, out_dtype=torch.bfloat16):
         pw = self.packed()
         n_rows = self.n_experts * B * C
-        if isinstance(pw, ops.PackedWeights) and not pw.fp8:
+        if self.mx is not None:
+            yperm = self.expert_rows(x2d, sel.row_token, sel.offsets, n_rows)[0]
+        elif isinstance(pw, ops.PackedWeights) and not pw.fp8:
             # bf16 SwiGLU: the gate/up GEMM gathers the selected token rows itself (no
             # permuted copy of x; a -1 entry of row_token reads as a zero row, as gather_rows
             # writes it)
@@ -375,6 +459,31 @@ class GroupedExpertsExpertChoice(_PackedExperts):
         src_w[toks, ee] = expert_weights.detach().reshape(-1).float()
         offsets = (torch.arange(E + 1, device=dev, dtype=torch.int32) * (B * C))
         return ops.ECSelectOut(token_indices, expert_weights, row_token, offsets, src_row, src_w)
+
+
+class _RouteFn(torch.autograd.Function):
+    """ops.route_topk with its backward on the HIP kernel."""
+
+    @staticmethod
+    def forward(ctx, logits, k, bias, spec):
+        r = ops.route_topk(logits.detach(), k, bias=bias, **spec._asdict())
+        ctx.save_for_backward(logits, r.idx)
+        ctx.spec = spec
+        ctx.mark_non_differentiable(r.idx)
+        return r.w, r.idx
+
+    @staticmethod
+    def backward(ctx, dw, didx):
+        logits, idx = ctx.saved_tensors
+        s = ctx.spec
+        dl = ops.route_topk_bwd(logits, idx, dw, scores=s.scores, renorm=s.renorm, scale=s.scale)
+        return dl.to(logits.dtype), None, None, None
+
+
+def route_topk(logits, k, scores="softmax", bias=None, groups=1, topk_groups=1, group_top=2, renorm=True, scale=1.0):
+    """(w (T, k) f32, idx (T, k) int64) of ops.route_topk, differentiable in the logits (the
+    choice is piecewise constant: the bias gets no gradient)."""
+    return _RouteFn.apply(logits, k, bias, ops.RouteSpec(scores, groups, topk_groups, group_top, renorm, scale))
 
 
 class _MoETrainFn(torch.autograd.Function):
@@ -441,7 +550,8 @@ class _RouterFn(torch.autograd.Function):
         dw = torch.zeros(T, router.top_k, device=xb.device) if dw is None else dw.float().contiguous()
         need_w = any(ctx.needs_input_grad[1:3])
         dx, dw_in, dw_out = _bwd.router_backward(xb, r.logits, r.idx, r.w, r.hidden, dw, dlogits,
-                                                 router.router[2].weight, router._bwd_weights(), need_weights=need_w)
+                                                 router.router[2].weight, router._bwd_weights(), need_weights=need_w,
+                                                 spec=router.spec)
         w_in, w_out = router.router[0].weight, router.router[2].weight
         return (dx.to(x2d.dtype), None if dw_in is None else dw_in.to(w_in.dtype), dw_out.to(w_out.dtype), None)
 
@@ -494,7 +604,7 @@ class _ExpertsFn(torch.autograd.Function):
         T, k = idx.shape
         E = experts.n_experts
         xb = x2d.detach().to(torch.bfloat16).contiguous()
-        disp = ops.dispatch(xb, idx, w.detach(), E, materialize=True, fp8=experts.use_fp8)
+        disp = ops.dispatch(xb, idx, w.detach(), E, materialize=experts.mx is None, fp8=experts.use_fp8)
         yperm, h, gu, xrows = experts.expert_rows(xb, disp.row_token, disp.offsets, T * k, xperm=disp.xperm,
                                                   xscale=disp.xscale, save=True)
         out_dtype = torch.float32 if x2d.dtype == torch.float32 else torch.bfloat16
@@ -529,7 +639,8 @@ class _ExpertsECFn(torch.autograd.Function):
         sel = experts.tables(token_indices, w, S)
         xb = x3d.detach().reshape(B * S, d).to(torch.bfloat16).contiguous()
         A = E * B * C
-        xperm, xscale = ops.gather_rows(xb, sel.row_token, A, fp8=experts.use_fp8)
+        xperm, xscale = ((None, None) if experts.mx is not None
+                         else ops.gather_rows(xb, sel.row_token, A, fp8=experts.use_fp8))
         yperm, h, gu, xperm = experts.expert_rows(xb, sel.row_token, sel.offsets, A, xperm=xperm, xscale=xscale,
                                                   save=True)
         out_dtype = torch.float32 if x3d.dtype == torch.float32 else torch.bfloat16
@@ -570,7 +681,8 @@ class _MoEECTrainFn(torch.autograd.Function):
         r, sel, C = layer.router.route(xb, descending=False, save_hidden=True)
         x2d = xb.reshape(T, d)
         A = E * B * C
-        xperm, xscale = ops.gather_rows(x2d, sel.row_token, A, fp8=ge.use_fp8)
+        xperm, xscale = ((None, None) if ge.mx is not None
+                         else ops.gather_rows(x2d, sel.row_token, A, fp8=ge.use_fp8))
         yperm, h, gu, xperm = ge.expert_rows(x2d, sel.row_token, sel.offsets, A, xperm=xperm, xscale=xscale,
                                              save=True)
         y = ops.combine(yperm, sel.src_row, sel.src_w, T, out_dtype=layer._out_dtype(x))
@@ -640,19 +752,30 @@ class MoELayer(nn.Module):
         use_fp8 = bool(getattr(config, "moe_fp8", False))
         if use_fp8 and getattr(config, "ffn_activation", "swiglu") != "swiglu":
             raise NotImplementedError("kmoe: fp8 experts are implemented for swiglu only")
+        mx = getattr(config, "moe_mx", None)
+        if mx is not None and mx not in ops.MX_EXPERTS:
+            raise ValueError(f"kmoe.MoELayer: moe_mx={mx!r} is none of {sorted(ops.MX_EXPERTS)}")
+        if mx is not None and use_fp8:
+            raise ValueError("kmoe.MoELayer: moe_fp8 and moe_mx exclude each other")
+        if mx is not None and getattr(config, "ffn_activation", "swiglu") != "swiglu":
+            raise NotImplementedError("kmoe: microscaled experts are implemented for swiglu only")
         check_supported(config)
         if self.routing_type == "expert_choice":
+            if _route_spec(config) is not None or getattr(config, "moe_balance_bias", False):
+                raise ValueError("kmoe.MoELayer: router scores, groups, renorm, scale and balance bias are for token choice")
             self.router = ExpertChoiceRouter(config)
             self.grouped_experts = None
             self.grouped_experts_ec = GroupedExpertsExpertChoice(config.n_experts, config.d_model,
                                                                  config.d_ff_expert, config.ffn_activation)
             self.grouped_experts_ec.use_fp8 = use_fp8
+            self.grouped_experts_ec.mx = mx
         else:
             self.router = Router(config)
             self.grouped_experts_ec = None
             self.grouped_experts = GroupedExperts(config.n_experts, config.d_model, config.d_ff_expert,
                                                  config.ffn_activation)
             self.grouped_experts.use_fp8 = use_fp8
+            self.grouped_experts.mx = mx
         self.experts = None
         self.load_balance_loss_weight = config.moe_load_balance_loss_weight
         self.router_z_loss_weight = config.moe_router_z_loss_weight
@@ -691,7 +814,7 @@ class MoELayer(nn.Module):
         """Backward packed weights, rebuilt only when a parameter changed."""
         ge = self.grouped_experts if self.grouped_experts is not None else self.grouped_experts_ec
         w_in = self.router.router[0].weight
-        key = tuple((w.data_ptr(), w._version) for w in ge._weights() + (w_in,)) + (ge.use_fp8,)
+        key = tuple((w.data_ptr(), w._version) for w in ge._weights() + (w_in,)) + (ge.use_fp8, ge.mx)
         cache = getattr(self, "_bwd_cache", None)
         if cache is None or cache[0] != key:
             with torch.no_grad():
@@ -713,7 +836,7 @@ class MoELayer(nn.Module):
         # gathers its own A rows from x; fp8: the rows are the dispatch's e4m3 codes, kept
         # dequantised)
         aux_in = self._aux_args(r, T)
-        disp = ops.dispatch(x2d, r.idx, r.w, E, capacity=cap, materialize=True, fp8=ge.use_fp8,
+        disp = ops.dispatch(x2d, r.idx, r.w, E, capacity=cap, materialize=ge.mx is None, fp8=ge.use_fp8,
                             block_counts=r.block_counts, aux=aux_in)
         yperm, h, gu, xrows = ge.expert_rows(x2d, disp.row_token, disp.offsets, T * k, xperm=disp.xperm,
                                              xscale=disp.xscale, save=True)
@@ -726,7 +849,7 @@ class MoELayer(nn.Module):
             aux = (disp.aux if disp.aux is not None else
                    ops.aux_loss(r.partials, T, E, disp.counts, k, self.load_balance_loss_weight,
                                 self.router_z_loss_weight))[0]
-        sv = _bwd.Saved(x2d, r.logits, r.idx, r.w, r.hidden, disp, h, gu, yperm, xrows)
+        sv = _bwd.Saved(x2d, r.logits, r.idx, r.w, r.hidden, disp, h, gu, yperm, xrows, self.router.spec)
         return y, aux, sv
 
     def _forward_token_choice(self, hidden_states: torch.Tensor) -> torch.Tensor:
@@ -750,7 +873,8 @@ class MoELayer(nn.Module):
         """Whether a token-choice forward of T tokens without gradients runs as one native
         call: gated bf16 experts and plain top-k routing, no per-stage timing."""
         ge = self.grouped_experts
-        return T > 0 and ge.gated and not ge.use_fp8 and not self.router.balanced_routing and not ops.stage_timing()
+        return (T > 0 and ge.gated and not ge.use_fp8 and ge.mx is None and not self.router.balanced_routing
+                and self.router.spec is None and not ops.stage_timing())
 
     def forward_one_call(self, x2d, w_in, w_out, pw, out_dtype, residual=None, rms_eps=None):
         """ops.moe_forward with this layer's settings; sets last_expert_counts and aux_loss."""
@@ -763,16 +887,17 @@ class MoELayer(nn.Module):
         return y
 
     def forward_rows(self, x2d, T, row_index=None, T_out=None, out_map=None, scale=None,
-                     out_dtype=torch.bfloat16, residual=None):
+                     out_dtype=torch.bfloat16, residual=None, coded=None):
         """Token-choice MoE over rows row_index[t] (t < T) of x2d; kernel-level entry
-        used by the MoD composition.  Returns (y, RouterOut, DispatchOut)."""
+        used by the MoD composition.  Returns (y, RouterOut, DispatchOut).  coded: as in
+        GroupedExperts.run."""
         if x2d.dtype != torch.bfloat16:
             x2d = x2d.to(torch.bfloat16)
         r = self.router.route(x2d, row_index=row_index, T=T)
         cap = ops.capacity_of(self.capacity_factor, T, self.top_k, self.n_experts) if self.drop_overflow else 0
         y, disp = self.grouped_experts.run(x2d, r.idx, r.w, row_index=row_index, T_out=T_out, out_map=out_map,
                                            scale=scale, out_dtype=out_dtype, residual=residual, capacity=cap,
-                                           block_counts=r.block_counts, aux=self._aux_args(r, T))
+                                           block_counts=r.block_counts, aux=self._aux_args(r, T), coded=coded)
         return y, r, disp
 
     def _aux_args(self, r, T):

@@ -702,3 +702,261 @@ def rmsnorm_bwd(dn, x2d, weight, rrms, dres=None, dw_dtype=None):
         _lib.call("kmoe_rmsnorm_bwd", ptr(dn), ptr(x2d), _fdt(x2d), ptr(weight), _fdt(weight), ptr(rrms), ptr(dres), T,
                   d, ptr(dx), ptr(dwt), _fdt(dwt), ptr(ws), wsb, _stream(x2d))
     return dx, dwt
+
+# ---------------------------------------------------------------- routing of logits
+class RouteSpec(NamedTuple):
+    """How logits become experts and weights (kmoe_route_topk): `scores` "softmax" or
+    "sigmoid"; `groups` equal runs of experts of which the best `topk_groups` stay, a group
+    being worth the sum of its best `group_top` (1 or 2) choices; `renorm` divides the
+    weights by their sum; `scale` multiplies them."""
+    scores: str = "softmax"
+    groups: int = 1
+    topk_groups: int = 1
+    group_top: int = 2
+    renorm: bool = True
+    scale: float = 1.0
+
+
+class RouteOut(NamedTuple):
+    idx: torch.Tensor                        # (T, k) int64
+    w: torch.Tensor                          # (T, k) f32
+    block_counts: Optional[torch.Tensor] = None  # router-block histograms of idx (hist=True)
+
+
+def _scores(name) -> int:
+    try:
+        return _lib.SCORES[name]
+    except (KeyError, TypeError):
+        raise ValueError(f"kmoe.route_topk: scores {name!r} is none of {sorted(_lib.SCORES)}") from None
+
+
+def _route_logits(logits, who):
+    _need_gpu(logits)
+    if logits.dim() != 2:
+        raise ValueError(f"kmoe.{who}: logits must be (tokens, experts), got {tuple(logits.shape)}")
+    return _contig(logits, torch.float32)
+
+
+def route_topk(logits, k, scores="softmax", bias=None, groups=1, topk_groups=1, group_top=2, renorm=True, scale=1.0,
+               hist=False) -> RouteOut:
+    """Experts and weights of logits (T, E): the k largest scores + bias (E,) among the
+    experts of the best topk_groups of `groups` groups, and those experts' scores (without
+    the bias), renormalised and times `scale`.  A logit of -inf masks its expert: it is
+    picked only when too few others are left, with weight 0.  Equal choices: lowest index
+    first; choices are compared in 64 bits.  hist: also the histograms that
+    dispatch(block_counts=...) takes.  Not differentiable: kmoe.route_topk is."""
+    sc = _scores(scores)
+    logits = _route_logits(logits, "route_topk")
+    T, E = logits.shape
+    if bias is not None:
+        if bias.shape != (E,) or bias.device != logits.device:
+            raise ValueError(f"kmoe.route_topk: bias must be ({E},) on {logits.device}, got {tuple(bias.shape)} on "
+                             f"{bias.device}")
+        bias = _contig(bias.detach(), torch.float32)
+    dev = logits.device
+    idx = torch.empty(T, int(k), device=dev, dtype=torch.int64)
+    w = torch.empty(T, int(k), device=dev, dtype=torch.float32)
+    with torch.cuda.device(dev), _Stage("route"):
+        bc = torch.empty(-(-T // router_block_tokens(T)), E, device=dev, dtype=torch.int32) if hist and T > 0 else None
+        _lib.call("kmoe_route_topk", ptr(logits), T, E, int(k), sc, ptr(bias), int(groups), int(topk_groups),
+                  int(group_top), int(bool(renorm)), float(scale), ptr(idx), ptr(w), ptr(bc), _stream(logits))
+    return RouteOut(idx, w, bc)
+
+
+def route_topk_bwd(logits, idx, dw, scores="softmax", renorm=True, scale=1.0, dlogits=None):
+    """Gradient of route_topk's weights: dw (T, k) to the logits' (T, E) f32, added to
+    `dlogits` when given."""
+    sc = _scores(scores)
+    logits = _route_logits(logits, "route_topk_bwd")
+    T, E = logits.shape
+    _need_gpu(idx, dw)
+    k = idx.shape[-1]
+    if idx.shape != (T, k) or dw.shape != (T, k):
+        raise ValueError(f"kmoe.route_topk_bwd: idx and dw must be ({T}, k), got {tuple(idx.shape)}, {tuple(dw.shape)}")
+    add = dlogits is not None
+    if add and (dlogits.shape != (T, E) or dlogits.dtype != torch.float32 or not dlogits.is_contiguous()):
+        raise ValueError(f"kmoe.route_topk_bwd: dlogits must be contiguous f32 ({T}, {E})")
+    if not add:
+        dlogits = torch.empty(T, E, device=logits.device, dtype=torch.float32)
+    with torch.cuda.device(logits.device), _Stage("bwd_router"):
+        _lib.call("kmoe_route_topk_bwd", ptr(logits), ptr(_contig(idx, torch.int64)), ptr(_contig(dw, torch.float32)), T, E,
+                  k, sc, int(bool(renorm)), float(scale), int(add), ptr(dlogits), _stream(logits))
+    return dlogits
+
+
+# ---------------------------------------------------------------- microscaled rows and experts
+MX_FORMATS = {"e4m3": _lib.DTYPE_FP8_E4M3, "e2m1": _lib.DTYPE_FP4_E2M1}
+# activation format of each kind of 4-bit experts
+MX_EXPERTS = {"w4a8": "e4m3", "w4a4": "e2m1"}
+
+
+def _mx_fmt(fmt) -> int:
+    try:
+        return MX_FORMATS[fmt]
+    except (KeyError, TypeError):
+        raise ValueError(f"kmoe: microscaled element type {fmt!r} is none of {sorted(MX_FORMATS)}") from None
+
+
+class MXRows(NamedTuple):
+    """Rows in blocks of 32 values that share a power-of-two scale.  q (rows, Kp) e4m3 codes
+    or (rows, Kp / 2) e2m1 pairs, the first in the low half, Kp = K rounded up to 128;
+    scale (rows, Kp / 32), byte c for 2^(c - 127), 255 for a block of NaN."""
+    q: torch.Tensor
+    scale: torch.Tensor
+    K: int
+    fmt: str
+
+
+def _mx_rows(rows, K, fmt, dev) -> MXRows:
+    kp = (K + 127) // 128 * 128
+    return MXRows(torch.empty(rows, kp if fmt == "e4m3" else kp // 2, device=dev, dtype=torch.uint8),
+                  torch.empty(rows, kp // 32, device=dev, dtype=torch.uint8), K, fmt)
+
+
+def quant_rows_mx(m, fmt="e4m3", row_index=None, n_rows_dev=None) -> MXRows:
+    """Microscaled codes of the bf16 rows of m (n, K), K a multiple of 32, or of its rows
+    row_index (int32).  Rows past *n_rows_dev (int32, on the GPU) are left unwritten."""
+    code = _mx_fmt(fmt)
+    _need_gpu(m, row_index, n_rows_dev)
+    if m.dim() != 2:
+        raise ValueError(f"kmoe.quant_rows_mx: a matrix is needed, got {tuple(m.shape)}")
+    m = _contig(m, _BF16)
+    if row_index is not None:
+        row_index = _contig(row_index, torch.int32)
+    rows = m.shape[0] if row_index is None else row_index.numel()
+    out = _mx_rows(rows, m.shape[1], fmt, m.device)
+    with torch.cuda.device(m.device), _Stage("quant_x"):
+        _lib.call("kmoe_quant_rows_mx", ptr(m), ptr(row_index), rows, ptr(n_rows_dev), m.shape[1], code, ptr(out.q),
+                  ptr(out.scale), _stream(m))
+    return out
+
+
+def dequant_rows_mx(r: MXRows, row_index=None, n_rows_dev=None):
+    """The values (n, K) bf16 of coded rows, or of rows row_index (int32; -1: zeros)."""
+    code = _mx_fmt(r.fmt)
+    _need_gpu(r.q, r.scale, row_index, n_rows_dev)
+    if row_index is not None:
+        row_index = _contig(row_index, torch.int32)
+    rows = r.q.shape[0] if row_index is None else row_index.numel()
+    out = torch.empty(rows, r.K, device=r.q.device, dtype=_BF16)
+    with torch.cuda.device(r.q.device), _Stage("mx_dequant"):
+        _lib.call("kmoe_dequant_rows_mx", ptr(r.q), ptr(r.scale), ptr(row_index), rows, ptr(n_rows_dev), r.K, code,
+                  ptr(out), _stream(r.q))
+    return out
+
+
+def fake_quant_mx_cols(w):
+    """The bf16 values that w (E, K, N) stands for in e2m1 blocks of 32 along K, as
+    pack_weights_mx packs it."""
+    _need_gpu(w)
+    if w.dtype not in (torch.float32, _BF16) or w.dim() != 3:
+        raise ValueError(f"kmoe.fake_quant_mx_cols: bf16 or f32 (E, K, N) weights are needed, got {w.dtype} "
+                         f"{tuple(w.shape)}")
+    w = _contig(w.detach(), w.dtype)
+    E, K, N = w.shape
+    out = torch.empty(E, K, N, device=w.device, dtype=_BF16)
+    with torch.cuda.device(w.device):
+        _lib.call("kmoe_fake_quant_mx_cols", ptr(w), _fdt(w), E, K, N, ptr(out), _stream(w))
+    return out
+
+
+class PackedWeightsMX(NamedTuple):
+    """4-bit expert weights in the products' operand order (kmoe_pack_weights_mx)."""
+    w13: torch.Tensor
+    s13: torch.Tensor
+    w3: torch.Tensor
+    s3: torch.Tensor
+    E: int
+    d: int
+    F: int
+
+
+def pack_weights_mx(w1, w2, w3) -> PackedWeightsMX:
+    """e2m1 blocks along K of the expert weights w1, w2 (E,d,F), w3 (E,F,d), packed."""
+    _need_gpu(w1, w2, w3)
+    E, d, F = w1.shape
+    if w2.shape != (E, d, F) or w3.shape != (E, F, d):
+        raise ValueError("kmoe.pack_weights_mx: w1/w2 must be (E,d,F) and w3 (E,F,d)")
+    dt = w1.dtype
+    if dt not in (torch.float32, _BF16):
+        raise ValueError(f"kmoe.pack_weights_mx: unsupported weight dtype {dt}")
+    w1, w2, w3 = (_contig(w, dt) for w in (w1, w2, w3))
+    lib = _lib.load()
+    dev = w1.device
+    bufs = [torch.empty(lib.kmoe_packed_mx_bytes(E, d, F, i), device=dev, dtype=torch.uint8) for i in range(4)]
+    with torch.cuda.device(dev):
+        _lib.call("kmoe_pack_weights_mx", ptr(w1), ptr(w2), ptr(w3), _fdt(w1), E, d, F, *(ptr(b) for b in bufs), _stream(w1))
+    return PackedWeightsMX(*bufs, E, d, F)
+
+
+def gemm_gate_up_mx(x: MXRows, row_token, offsets, pw: PackedWeightsMX, max_rows, save_gu=False):
+    """Coded rows of silu(x w1) * (x w2) in x's format: permuted row r is x's row
+    row_token[r] (row r without row_token).  save_gu (training): (h, gu), gu the bf16
+    pre-activation gate / up values (max_rows, 2 F_pad) in the backward's column order."""
+    _need_gpu(x.q, row_token, offsets)
+    if x.K != pw.d:
+        raise ValueError(f"kmoe.gemm_gate_up_mx: rows of {x.K} values for weights of d={pw.d}")
+    if row_token is None and x.q.shape[0] < max_rows:
+        raise ValueError(f"kmoe.gemm_gate_up_mx: {x.q.shape[0]} permuted rows, max_rows {max_rows}")
+    fp = (pw.F + 127) // 128 * 128
+    h = _mx_rows(max(max_rows, 1), pw.F, x.fmt, x.q.device)
+    gu = torch.empty(max(max_rows, 1), 2 * fp, device=x.q.device, dtype=_BF16) if save_gu else None
+    with torch.cuda.device(x.q.device), _Stage("gemm_gate_up"):
+        _lib.call("kmoe_gemm_gate_up_mx", ptr(x.q), ptr(x.scale), _mx_fmt(x.fmt), x.q.shape[0], ptr(row_token),
+                  ptr(offsets), pw.E, pw.d, pw.F, max_rows, ptr(pw.w13), ptr(pw.s13), ptr(h.q), ptr(h.scale), ptr(gu),
+                  _stream(x.q))
+    return (h, gu) if save_gu else h
+
+
+def gemm_down_mx(h: MXRows, offsets, pw: PackedWeightsMX, max_rows):
+    """y (max_rows, d) bf16 = h w3 of the coded rows of each expert."""
+    _need_gpu(h.q, offsets)
+    if h.K != pw.F or h.q.shape[0] < max_rows:
+        raise ValueError(f"kmoe.gemm_down_mx: rows {tuple(h.q.shape)} of {h.K} values, F={pw.F}, max_rows {max_rows}")
+    y = torch.empty(max(max_rows, 1), pw.d, device=h.q.device, dtype=_BF16)
+    with torch.cuda.device(h.q.device), _Stage("gemm_down"):
+        _lib.call("kmoe_gemm_down_mx", ptr(h.q), ptr(h.scale), _mx_fmt(h.fmt), ptr(offsets), pw.E, pw.d, pw.F, max_rows,
+                  ptr(pw.w3), ptr(pw.s3), ptr(y), _stream(h.q))
+    return y
+
+
+class AddNormOut(NamedTuple):
+    h: torch.Tensor                # (T, d) x + delta, in x's type
+    n: torch.Tensor                # (T, d) bf16 RMSNorm of h
+    rrms: torch.Tensor             # (T,) f32 1/sqrt(mean(h^2) + eps)
+    q: Optional[torch.Tensor]      # codes and scales of n (quant), as MXRows has them
+    scale: Optional[torch.Tensor]
+
+
+def add_rmsnorm(x2d, delta, weight, eps, quant=None) -> AddNormOut:
+    """Residual add and RMSNorm in one pass: h = x + delta (delta None: x itself),
+    n = bf16(weight * h / sqrt(mean(h^2) + eps)) and, with quant "e4m3" / "e2m1", n's
+    microscaled rows (those of quant_rows_mx(n)).  x2d, delta (T, d) bf16 or f32; an f32
+    delta makes h f32.  Not differentiable: kmoe.add_rms_norm is."""
+    code = _lib.DTYPE_BF16 if quant is None else _mx_fmt(quant)
+    _need_gpu(x2d, delta, weight)
+    T, d = x2d.shape
+    if weight.shape != (d,) or (delta is not None and delta.shape != (T, d)):
+        raise ValueError(f"kmoe.add_rmsnorm: x {(T, d)}, delta {None if delta is None else tuple(delta.shape)}, weight "
+                         f"{tuple(weight.shape)}")
+    dt = x2d.dtype if x2d.dtype in (torch.float32, _BF16) else torch.float32
+    if delta is not None:
+        if delta.dtype != _BF16:
+            dt = torch.float32
+            delta = _contig(delta, torch.float32)
+        else:
+            delta = delta.contiguous()
+    x2d = _contig(x2d, dt)
+    weight = weight.detach()
+    weight = _contig(weight, weight.dtype if weight.dtype in (torch.float32, _BF16) else torch.float32)
+    dev = x2d.device
+    h = x2d if delta is None else torch.empty(T, d, device=dev, dtype=dt)
+    n = torch.empty(T, d, device=dev, dtype=_BF16)
+    rrms = torch.empty(T, device=dev, dtype=torch.float32)
+    rows = _mx_rows(T, d, quant, dev) if quant is not None else None
+    q, scale = (None, None) if rows is None else rows[:2]
+    with torch.cuda.device(dev), _Stage("rmsnorm"):
+        _lib.call("kmoe_add_rmsnorm", ptr(x2d), _fdt(x2d), ptr(delta), _lib.DTYPE_BF16 if delta is None else _fdt(delta),
+                  ptr(weight), _fdt(weight), float(eps), T, d, ptr(h), ptr(n), ptr(rrms), code, ptr(q), ptr(scale),
+                  _stream(x2d))
+    return AddNormOut(h, n, rrms, q, scale)

@@ -1,0 +1,252 @@
+"""Routing of logits (scores, balance bias, groups, renormalisation) and its backward against
+64-bit restatements."""
+import pytest
+import torch
+
+import kmoe
+from kmoe import ops
+from oracle import mx_oracle as M
+
+pytestmark = pytest.mark.gpu
+F32 = torch.float32
+HALF_F32 = torch.finfo(F32).eps / 2
+INF = float("inf")
+
+
+def logits_of(dev, T, E, seed=0, std=1.5):
+    g = torch.Generator().manual_seed(seed)
+    return (std * torch.randn(T, E, generator=g)).to(dev)
+
+
+def bias_of(dev, E, seed=1):
+    return (0.1 * torch.randn(E, generator=torch.Generator().manual_seed(seed))).to(dev)
+
+
+CASES = [
+    # T, E, k, scores, bias, groups, topk_groups, group_top, renorm, scale
+    (1, 1, 1, "softmax", False, 1, 1, 2, True, 1.0),
+    (1, 16, 2, "softmax", False, 1, 1, 2, True, 1.0),
+    (3, 5, 5, "sigmoid", True, 1, 1, 2, False, 0.5),
+    (33, 13, 3, "softmax", True, 1, 1, 2, True, 2.5),
+    (129, 64, 8, "sigmoid", True, 8, 4, 2, True, 2.5),
+    (70, 63, 7, "softmax", True, 7, 1, 1, False, 1.0),
+    (65, 24, 4, "sigmoid", False, 12, 2, 2, True, 1.0),
+    (40, 32, 2, "softmax", False, 32, 3, 2, True, 1.0),   # groups of one expert
+    (513, 48, 6, "softmax", True, 2, 1, 2, True, 1.0),
+]
+
+
+def kwargs(dev, c):
+    _, E, _, scores, bias, groups, keep, top, renorm, scale = c
+    return dict(scores=scores, bias=bias_of(dev, E) if bias else None, groups=groups, topk_groups=keep, group_top=top,
+                renorm=renorm, scale=scale)
+
+
+@pytest.mark.parametrize("c", CASES)
+def test_forward(dev, c):
+    T, E, k = c[:3]
+    lg = logits_of(dev, T, E, seed=T + E)
+    kw = kwargs(dev, c)
+    r = ops.route_topk(lg, k, hist=True, **kw)
+    cpu = {**kw, "bias": None if kw["bias"] is None else kw["bias"].cpu()}
+    idx, w = M.route(lg.cpu(), k, kind=cpu.pop("scores"), **cpu)
+    assert torch.equal(r.idx.cpu(), idx)
+    # rounded once from 64 bits (1e-13: the two 64-bit computations)
+    assert bool(((r.w.double().cpu() - w).abs() <= (HALF_F32 + 1e-13) * w.abs()).all())
+    hb = ops.router_block_tokens(T)
+    want = torch.stack([torch.bincount(b.reshape(-1), minlength=E) for b in r.idx.cpu().split(hb)])
+    assert torch.equal(r.block_counts.cpu().long(), want)
+
+
+def test_near_ties_are_told_apart(dev):
+    """Choices that differ by less than 32 bits resolve, and equal ones: lowest index first."""
+    T, E = 64, 16
+    base = torch.zeros(T, E, dtype=F32)
+    base[:, 5] = 2.0
+    base[:, 9] = 2.0                      # tie of 5 and 9
+    base[:, 3] = 2.0 + 2.0 ** -22         # one step of a float above
+    bias = torch.zeros(E)
+    r = ops.route_topk(base.to(dev), 3, scores="sigmoid", bias=bias.to(dev))
+    assert r.idx.cpu().tolist() == [[3, 5, 9]] * T
+    # a bias that closes the gap of two scores but for 1e-12
+    s = torch.sigmoid(torch.tensor([0.3, -0.7], dtype=F32).double())
+    b = float((s[0] - s[1]).float())
+    lg = torch.full((T, E), -5.0)
+    lg[:, 2], lg[:, 11] = 0.3, -0.7
+    bias[11] = b
+    exact = float(s[1]) + float(bias[11].double()) > float(s[0])
+    r = ops.route_topk(lg.to(dev), 1, scores="sigmoid", bias=bias.to(dev))
+    assert r.idx.cpu().flatten().tolist() == [11 if exact else 2] * T
+
+
+@pytest.mark.parametrize("scores", ["softmax", "sigmoid"])
+@pytest.mark.parametrize("groups,keep", [(1, 1), (4, 2)])
+def test_masked_rows_infinities_and_nan(dev, scores, groups, keep):
+    E, k = 16, 3
+    lg = logits_of(dev, 8, E).cpu()
+    lg[0] = -INF                       # nothing left
+    lg[1, 2:] = -INF                   # fewer experts than k
+    lg[2, 4:12] = torch.finfo(F32).min
+    lg[3] = torch.finfo(F32).min
+    lg[4, 3] = INF
+    lg[5, 7] = float("nan")
+    lg[6, ::2] = -INF
+    bias = bias_of("cpu", E)
+    bias[:] += 1.0
+    kw = dict(groups=groups, topk_groups=keep)
+    r = ops.route_topk(lg.to(dev), k, scores=scores, bias=bias.to(dev), **kw)
+    idx, w = M.route(lg, k, kind=scores, bias=bias, **kw)
+    got = r.idx.cpu()
+    assert int(got.min()) >= 0 and int(got.max()) < E
+    assert all(len(set(row)) == k for row in got.tolist())
+    assert torch.equal(got, idx)
+    wd = r.w.double().cpu()
+    assert torch.equal(wd.isnan(), w.isnan())
+    assert bool(((wd - w).abs().nan_to_num() <= (HALF_F32 + 1e-13) * w.abs().nan_to_num() + 1e-45).all())
+    assert not wd[0].any()
+    dl = ops.route_topk_bwd(lg.to(dev), r.idx, torch.ones(8, k, device=dev), scores=scores)
+    assert bool(dl[:4].isfinite().all()) and not dl[0].any()
+
+
+@pytest.mark.parametrize("c", CASES)
+def test_backward(dev, c):
+    T, E, k, scores, _, _, _, _, renorm, scale = c
+    lg = logits_of(dev, T, E, seed=T)
+    kw = kwargs(dev, c)
+    x = lg.clone().requires_grad_(True)
+    w, idx = kmoe.route_topk(x, k, **kw)
+    dw = logits_of(dev, T, k, seed=7)
+    (dl,) = torch.autograd.grad(w, x, dw)
+    x64 = lg.double().cpu().requires_grad_(True)
+    w64 = M.route_weights(x64, idx.cpu(), scores, renorm, scale)
+    (want,) = torch.autograd.grad(w64, x64, dw.double().cpu())
+    # f32 sums over the token's experts and k weights: exp and quotient (8 steps of 2^-24), sums
+    # of E and of k terms; the terms of a row, before they cancel, are at most scale max|dw|
+    # (without renorm times s <= 1)
+    bound = (16 + E + 3 * k) * 2.0 ** -24 * 4 * abs(scale) * dw.double().cpu().abs().amax(1, keepdim=True)
+    assert bool(((dl.double().cpu() - want).abs() <= bound).all())
+    add = torch.ones(T, E, device=dev)
+    ops.route_topk_bwd(lg, idx, dw, scores, renorm, scale, dlogits=add)
+    assert bool(((add - 1) - dl).abs().max() <= 2.0 ** -22 * (1 + float(dl.abs().max())))
+
+
+@pytest.mark.parametrize("scores,renorm", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+def test_backward_against_differences(dev, scores, renorm):
+    T, E, k, h = 6, 12, 3, 2.0 ** -7
+    lg = logits_of(dev, T, E, std=1.0)
+    _, idx = kmoe.route_topk(lg, k, scores=scores, renorm=renorm)
+    dw = logits_of(dev, T, k, seed=3)
+    dl = ops.route_topk_bwd(lg, idx, dw, scores, renorm).double().cpu()
+    f = lambda l: (M.route_weights(l, idx.cpu(), scores, renorm, 1.0) * dw.double().cpu()).sum()  # noqa: E731
+    x = lg.double().cpu()
+    for t in range(T):
+        for e in range(E):
+            d = torch.zeros_like(x)
+            d[t, e] = h
+            num = float(f(x + d) - f(x - d)) / (2 * h)
+            # central difference: h^2 / 6 of the third derivative, below 8 max|dw| k here
+            assert abs(num - float(dl[t, e])) <= h * h / 6 * 8 * k * float(dw.abs().max()) + 1e-5
+
+
+def test_strides_types_streams_and_graph(dev):
+    lg = logits_of(dev, 100, 32)
+    want = ops.route_topk(lg, 4, scores="sigmoid", groups=4, topk_groups=2)
+    wide = torch.randn(100, 64, device=dev)
+    wide[:, 16:48] = lg
+    got = ops.route_topk(wide[:, 16:48], 4, scores="sigmoid", groups=4, topk_groups=2)
+    assert torch.equal(got.idx, want.idx) and torch.equal(got.w, want.w)
+    lb = lg.to(torch.bfloat16)
+    a, b = ops.route_topk(lb, 4), ops.route_topk(lb.float(), 4)
+    assert torch.equal(a.idx, b.idx) and torch.equal(a.w, b.w)
+    buf = lg.clone()
+    g = torch.cuda.CUDAGraph()
+    s = torch.cuda.Stream()
+    with torch.cuda.graph(g, stream=s):
+        r = ops.route_topk(buf, 4, scores="sigmoid", groups=4, topk_groups=2, hist=True)
+    for seed in (1, 2, 3):
+        new = logits_of(dev, 100, 32, seed=seed)
+        eager = ops.route_topk(new, 4, scores="sigmoid", groups=4, topk_groups=2, hist=True)
+        buf.copy_(new)
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(r.idx, eager.idx) and torch.equal(r.w, eager.w)
+        assert torch.equal(r.block_counts, eager.block_counts)
+
+
+def test_large_and_empty(dev):
+    lg = logits_of(dev, 20001, 64)
+    bias = bias_of(dev, 64)
+    r = ops.route_topk(lg, 8, scores="sigmoid", bias=bias, groups=8, topk_groups=4, hist=True)
+    s = torch.sigmoid(lg.double())
+    c = (s + bias.double()).view(-1, 8, 8)
+    keep = c.topk(2, -1).values.sum(-1).topk(4, -1).indices
+    on = torch.zeros(20001, 8, dtype=torch.bool, device=dev).scatter_(1, keep, True)
+    idx = torch.where(on[:, :, None], c, -INF).view(-1, 64).topk(8, -1).indices
+    assert torch.equal(r.idx, idx)
+    assert int(r.block_counts.sum()) == 20001 * 8
+    e = ops.route_topk(lg[:0], 4, hist=True)
+    assert e.idx.shape == (0, 4) and e.block_counts is None
+    assert ops.route_topk_bwd(lg[:0], e.idx, e.w).shape == (0, 64)
+
+
+def test_router_module(dev):
+    """The layer's router with grouped sigmoid scores and a balance bias: forward and gradients
+    against 64-bit autograd at the kernel's choice."""
+    cfg = kmoe.AdvancedMoEConfig(d_model=128, n_experts=16, moe_top_k=4, d_ff_expert=64, moe_router_scores="sigmoid",
+                                 moe_router_groups=4, moe_router_topk_groups=2, moe_router_scale=2.5, moe_balance_bias=True)
+    router = kmoe.Router(cfg).to(dev).to(torch.bfloat16)
+    assert router.balance_bias.dtype == F32 and router.balance_bias.is_cuda
+    assert "balance_bias" in router.state_dict()
+    with torch.no_grad():
+        router.balance_bias.copy_(bias_of("cpu", 16))
+    x = torch.randn(2, 30, 128, device=dev, dtype=torch.bfloat16)
+    with torch.no_grad():
+        w0, idx0, lg0 = router(x)
+    xg = x.clone().requires_grad_(True)
+    w, idx, lg = router(xg)
+    assert torch.equal(idx, idx0) and torch.equal(w, w0)
+    dw = torch.randn_like(w)
+    got = torch.autograd.grad(w, (xg, router.router[0].weight, router.router[2].weight), dw)
+    d64 = lambda t: t.detach().double().cpu().requires_grad_(True)  # noqa: E731
+    leaves = [d64(x), d64(router.router[0].weight), d64(router.router[2].weight)]
+    l64 = torch.nn.functional.silu(leaves[0].reshape(60, 128) @ leaves[1].t()) @ leaves[2].t()
+    w64 = M.route_weights(l64, idx.reshape(60, 4).cpu(), "sigmoid", True, 2.5)
+    want = torch.autograd.grad(w64, leaves, dw.reshape(60, 4).double().cpu())
+    for a, b in zip(got, want):
+        # bf16 roundings: the hidden gradient and the result
+        assert float((a.double().cpu() - b).norm() / b.norm()) <= 4 * torch.finfo(torch.bfloat16).eps / 2
+    plain = kmoe.Router(kmoe.AdvancedMoEConfig(d_model=128, n_experts=16, d_ff_expert=64))
+    assert plain.spec is None and "balance_bias" not in plain.state_dict()
+
+
+def test_layer_with_aux_losses(dev):
+    """Aux losses and routed gradients meet in the logit gradient: the sum of both parts."""
+    kw = dict(d_model=128, n_experts=8, moe_top_k=2, d_ff_expert=64, moe_router_scores="sigmoid", moe_router_groups=2)
+    layer = kmoe.MoELayer(kmoe.AdvancedMoEConfig(**kw)).to(dev).to(torch.bfloat16).train()
+    x = torch.randn(1, 70, 128, device=dev, dtype=torch.bfloat16)
+    dy = torch.randn_like(x)
+    w_out = layer.router.router[2].weight
+
+    def grad(with_y, with_aux):
+        y = layer(x)
+        loss = (y * dy).sum().float() * with_y + layer.aux_loss * with_aux
+        return torch.autograd.grad(loss, w_out)[0].double()
+    both, a, b = grad(1.0, 1.0), grad(1.0, 0.0), grad(0.0, 1.0)
+    assert float(a.norm()) > 0 and float(b.norm()) > 0
+    assert float((both - a - b).norm()) <= 4 * torch.finfo(torch.bfloat16).eps / 2 * float(a.norm() + b.norm())
+
+
+def test_refusals(dev):
+    lg = logits_of(dev, 4, 16)
+    for kw, err in ((dict(k=0), kmoe.KmoeError), (dict(k=9), kmoe.KmoeError), (dict(k=2, groups=3), kmoe.KmoeError),
+                    (dict(k=5, groups=4, topk_groups=1), kmoe.KmoeError), (dict(k=2, groups=4, topk_groups=5), kmoe.KmoeError),
+                    (dict(k=2, groups=2, group_top=3), kmoe.KmoeError), (dict(k=2, scores="tanh"), ValueError),
+                    (dict(k=2, bias=torch.zeros(3, device=dev)), ValueError), (dict(k=2, bias=torch.zeros(16)), ValueError)):
+        with pytest.raises(err):
+            ops.route_topk(lg, **kw)
+    with pytest.raises(kmoe.KmoeError):
+        ops.route_topk(logits_of(dev, 2, 65), 2)
+    with pytest.raises(ValueError):
+        ops.route_topk(lg[0], 2)
+    with pytest.raises(ValueError):
+        ops.route_topk_bwd(lg, torch.zeros(4, 2, dtype=torch.int64, device=dev), torch.zeros(4, 3, device=dev))
