@@ -335,6 +335,7 @@ class _PackedExperts(nn.Module):
 
     def _trainable(self, *inputs) -> bool:
         """Whether a direct call records a backward through the HIP kernels."""
+        _ = self.mx_act  # refuses a mode that does not exist
         if not torch.is_grad_enabled():
             return False
         if not any(isinstance(t, torch.Tensor) and t.requires_grad for t in inputs + tuple(self.parameters())):

@@ -343,7 +343,7 @@ def test_layer_forward_and_training(dev, mx, routing):
         aux0 = layer.aux_loss
     xg = x.clone().requires_grad_(True)
     y1 = layer(xg)
-    assert torch.equal(y0, y1) and float(aux0) == float(layer.aux_loss)
+    assert torch.equal(y0, y1) and float(aux0) == float(layer.aux_loss.detach())
     (y1.float().square().sum() + layer.aux_loss).backward()
     for n, p in layer.named_parameters():
         assert p.grad is not None and bool(p.grad.isfinite().all()) and float(p.grad.abs().sum()) > 0, n
