@@ -32,11 +32,11 @@ __host__ __device__ inline int round_up(int a, int b) { return (a + b - 1) / b *
 __host__ __device__ inline int64_t row_bytes(bool fp4, int K) { return round_up(K, STEP) / (fp4 ? 2 : 1); }
 __host__ __device__ inline int64_t scale_bytes(int K) { return round_up(K, STEP) / BLOCK; }
 
-// Scale byte of a block whose largest magnitude is amax (not negative; NaN or infinity: 255).
+// Scale byte of a block whose largest magnitude has the bits amax (NaN or infinity: 255).
 // The exponent bits of a float are floor(log2) + 127; subnormal floats count as 2^-127.
 template <bool FP4>
-__device__ __forceinline__ uint32_t scale_code(float amax) {
-  const uint32_t ef = __float_as_uint(amax) >> 23;
+__device__ __forceinline__ uint32_t scale_code(uint32_t amax) {
+  const uint32_t ef = amax >> 23;
   constexpr uint32_t EMAX = FP4 ? 2 : 8;
   return ef >= 255u ? 255u : (ef > EMAX ? ef - EMAX : 0u);
 }
@@ -47,26 +47,23 @@ __device__ __forceinline__ float scale_value(uint32_t c) {
   return c == 255u ? __uint_as_float(0x7fc00000u) : c == 0u ? __uint_as_float(0x00400000u) : __uint_as_float(c << 23);
 }
 
-// Largest magnitude, with every NaN counted as an infinity (fmaxf would drop it).
-__device__ __forceinline__ float amax_nan(float m, float v) {
-  const float a = fabsf(v);
-  return fmaxf(m, a != a ? __uint_as_float(0x7f800000u) : a);
-}
+// Largest magnitude as float bits, which order as integers do; a NaN's are above infinity's.
+__device__ __forceinline__ uint32_t amax_bits(uint32_t m, float v) { return max(m, __float_as_uint(v) & 0x7fffffffu); }
 
-// e2m1 code of v (finite): thresholds are the midpoints of 0, .5, 1, 1.5, 2, 3, 4, 6, a tie
-// goes to the even code.
-__device__ __forceinline__ uint32_t e2m1(float v) {
-  const float a = fabsf(v);
-  const uint32_t c = (uint32_t)(a > 0.25f) + (uint32_t)(a >= 0.75f) + (uint32_t)(a > 1.25f) + (uint32_t)(a >= 1.75f) +
-                     (uint32_t)(a > 2.5f) + (uint32_t)(a >= 3.5f) + (uint32_t)(a > 5.0f);
-  return c | (__float_as_uint(v) >> 31 << 3);
+// Two finite values as e2m1 codes (a in bits 0 .. 3): the hardware converter, whose rounding
+// (nearest, ties to the even code, 6 from above 5) equals the thresholds .25 .75 1.25 1.75 2.5
+// 3.5 5 on every finite float (checked exhaustively on gfx950).  SEL: byte of `old` to write.
+template <int SEL>
+__device__ __forceinline__ uint32_t e2m1x2(uint32_t old, float a, float b) {
+  return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(old, a, b, 1.0f, SEL);
 }
-__device__ __forceinline__ float e2m1_value(uint32_t c) {
-  const uint32_t m = c & 7u;
-  // exponent field m / 2, mantissa m % 2; field 0 is 0 and 0.5
-  const float v = m < 2u ? 0.5f * (float)m : __uint_as_float(((m >> 1) + 126u) << 23 | (m & 1u) << 22);
-  return c & 8u ? -v : v;
+// The values of the two codes in byte SEL of w
+template <int SEL>
+__device__ __forceinline__ f32x2_t e2m1x2_values(uint32_t w) {
+  const auto v = __builtin_amdgcn_cvt_scalef32_pk_f32_fp4(w, 1.0f, SEL);
+  return f32x2_t{v[0], v[1]};
 }
+__device__ __forceinline__ float clamp448(float v) { return __builtin_amdgcn_fmed3f(v, -448.0f, 448.0f); }
 
 // Codes of v[0 .. N) / scale: N bytes (e4m3) or N / 2 (e2m1, the first value in the low nibble).
 template <bool FP4, int N>
@@ -77,20 +74,21 @@ template <bool FP4, int N>
 __device__ __forceinline__ Codes<FP4, N> encode(const float (&v)[N], uint32_t code) {
   Codes<FP4, N> out;
   const float inv = inv_scale(code);
-  const bool none = code == 255u;
+  const bool none = code == 255u;  // inv 0: NaN and infinity times 0 are NaN, replaced below
   if constexpr (FP4) {
 #pragma unroll
     for (int i = 0; i < N / 8; ++i) {
-      uint32_t w = 0;
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w |= e2m1(v[8 * i + j] * inv) << (4 * j);
+      uint32_t w = e2m1x2<0>(0u, v[8 * i] * inv, v[8 * i + 1] * inv);
+      w = e2m1x2<1>(w, v[8 * i + 2] * inv, v[8 * i + 3] * inv);
+      w = e2m1x2<2>(w, v[8 * i + 4] * inv, v[8 * i + 5] * inv);
+      w = e2m1x2<3>(w, v[8 * i + 6] * inv, v[8 * i + 7] * inv);
       out.w[i] = none ? 0u : w;
     }
   } else {
 #pragma unroll
     for (int i = 0; i < N / 4; ++i) {
-      int r = __builtin_amdgcn_cvt_pk_fp8_f32(sat448(v[4 * i] * inv), sat448(v[4 * i + 1] * inv), 0, false);
-      r = __builtin_amdgcn_cvt_pk_fp8_f32(sat448(v[4 * i + 2] * inv), sat448(v[4 * i + 3] * inv), r, true);
+      int r = __builtin_amdgcn_cvt_pk_fp8_f32(clamp448(v[4 * i] * inv), clamp448(v[4 * i + 1] * inv), 0, false);
+      r = __builtin_amdgcn_cvt_pk_fp8_f32(clamp448(v[4 * i + 2] * inv), clamp448(v[4 * i + 3] * inv), r, true);
       out.w[i] = none ? 0u : (uint32_t)r;
     }
   }
@@ -110,11 +108,11 @@ __device__ __forceinline__ void unpack8(const i32x4_t& a, float (&v)[8]) {
 // and the group's scale byte.
 template <bool FP4>
 __device__ __forceinline__ Codes<FP4, 8> encode_quad(const float (&v)[8], uint32_t& code) {
-  float m = 0.0f;
+  uint32_t m = 0;
 #pragma unroll
-  for (int q = 0; q < 8; ++q) m = amax_nan(m, v[q]);
-  m = fmaxf(m, quad_xor<1>(m));
-  m = fmaxf(m, quad_xor<2>(m));
+  for (int q = 0; q < 8; ++q) m = amax_bits(m, v[q]);
+  m = max(m, (uint32_t)quad_xor<1>((int)m));
+  m = max(m, (uint32_t)quad_xor<2>((int)m));
   code = scale_code<FP4>(m);
   return encode<FP4, 8>(v, code);
 }

@@ -45,8 +45,14 @@ template <bool FP4>
 __device__ __forceinline__ void decode8(const uint8_t* p, float s, float (&v)[8]) {
   if constexpr (FP4) {
     const uint32_t w = *reinterpret_cast<const uint32_t*>(p);
+    const f32x2_t a = e2m1x2_values<0>(w), b = e2m1x2_values<1>(w), c = e2m1x2_values<2>(w), d = e2m1x2_values<3>(w);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = e2m1_value((w >> (4 * j)) & 15u) * s;
+    for (int j = 0; j < 2; ++j) {
+      v[j] = a[j] * s;
+      v[2 + j] = b[j] * s;
+      v[4 + j] = c[j] * s;
+      v[6 + j] = d[j] * s;
+    }
   } else {
     const i32x2_t w = *reinterpret_cast<const i32x2_t*>(p);
 #pragma unroll
@@ -101,17 +107,22 @@ __global__ __launch_bounds__(256) void fake_quant_kernel(const void* __restrict_
     const int64_t e = eb / nb;
     const int k0 = (int)(eb - e * nb) * BLOCK;
     const int64_t base = (e * K + k0) * N + n;
-    float v[BLOCK], m = 0.0f;
+    float v[BLOCK];
+    uint32_t m = 0;
 #pragma unroll
     for (int j = 0; j < BLOCK; ++j) {
       v[j] = k0 + j < K ? load1<F32>(w, base + (int64_t)j * N) : 0.0f;
-      m = amax_nan(m, v[j]);
+      m = amax_bits(m, v[j]);
     }
     const uint32_t code = scale_code<true>(m);
     const float inv = inv_scale(code), s = scale_value(code);
 #pragma unroll
-    for (int j = 0; j < BLOCK; ++j)
-      if (k0 + j < K) out[base + (int64_t)j * N] = f32_to_bf16(code == 255u ? s : e2m1_value(e2m1(v[j] * inv)) * s);
+    for (int j = 0; j < BLOCK; j += 2) {
+      const f32x2_t q = e2m1x2_values<0>(e2m1x2<0>(0u, v[j] * inv, v[j + 1] * inv));
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (k0 + j + u < K) out[base + (int64_t)(j + u) * N] = f32_to_bf16(code == 255u ? s : q[u] * s);
+    }
   }
 }
 
@@ -130,11 +141,12 @@ __global__ __launch_bounds__(256) void pack_mx_kernel(const void* __restrict__ w
     const int n = (int)(i - eb * Np);
     const int64_t e = eb / nb;
     const int b = (int)(eb - e * nb), k0 = b * BLOCK;
-    float v[BLOCK], m = 0.0f;
+    float v[BLOCK];
+    uint32_t m = 0;
 #pragma unroll
     for (int j = 0; j < BLOCK; ++j) {
       v[j] = n < N && k0 + j < K ? load1<F32>(w, (e * K + k0 + j) * N + n) : 0.0f;
-      m = amax_nan(m, v[j]);
+      m = amax_bits(m, v[j]);
     }
     const uint32_t code = scale_code<true>(m);
     const Codes<true, BLOCK> o = encode<true, BLOCK>(v, code);

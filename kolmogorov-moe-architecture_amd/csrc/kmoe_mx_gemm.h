@@ -24,7 +24,6 @@
 namespace kmoe_mx {
 
 constexpr int GEMM_THREADS = 256;
-constexpr int NST = 3;  // LDS stages
 
 struct MxGemmArgs {
   const uint8_t* a;        // activation rows
@@ -100,6 +99,15 @@ __device__ __forceinline__ void slot_rows(const SlotScan& s, int slot, int& e, i
   m_end = __builtin_amdgcn_readlane(s.hi, e);
 }
 
+// Compile-time loop: f(std::integral_constant<int, I>) for I in [I0, N).
+template <int I0, int N, class Fn>
+__device__ __forceinline__ void static_for(Fn&& f) {
+  if constexpr (I0 < N) {
+    f(std::integral_constant<int, I0>{});
+    static_for<I0 + 1, N>(f);
+  }
+}
+
 // Four values as bf16.
 __device__ __forceinline__ i32x2_t pack4_bf16(float a, float b, float c, float d) {
   const uint32_t lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
@@ -124,13 +132,11 @@ __device__ __forceinline__ i32x4_t merge_runs(i32x2_t x, i32x2_t y) {
 // q: the block's codes, scale: its byte; nothing is stored where !on.  All lanes take part.
 template <bool FP4>
 __device__ __forceinline__ void store_block(const float (&v)[16], int half, bool on, uint8_t* q, uint8_t* scale) {
-  float m = 0.0f;
+  uint32_t m = 0, o0, o1;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) m = amax_nan(m, v[i]);
-  uint32_t o0, o1;
-  swap_halves(__float_as_uint(m), __float_as_uint(m), o0, o1);  // (own or partner's, the other)
-  m = fmaxf(__uint_as_float(o0), __uint_as_float(o1));
-  const uint32_t code = scale_code<FP4>(m);
+  for (int i = 0; i < 16; ++i) m = amax_bits(m, v[i]);
+  swap_halves(m, m, o0, o1);  // its own and its partner's
+  const uint32_t code = scale_code<FP4>(max(o0, o1));
   const Codes<FP4, 16> d = encode<FP4, 16>(v, code);
   if constexpr (FP4) {
     // d.w[p]: runs 2 p (low 16 bits) and 2 p + 1
@@ -149,6 +155,7 @@ __device__ __forceinline__ void store_block(const float (&v)[16], int half, bool
 template <bool GATE_UP, bool FP4, int MI, int NJ, bool SAVE_GU>
 struct MxTile {
   static constexpr int BM = 64 * MI;
+  static constexpr int NST = MI == 2 ? 2 : 3;  // LDS stages
   static constexpr int AB = BM * (FP4 ? 64 : 128), BB = NJ * 4096, AS = BM * 4, BS = NJ * 256;
   static constexpr int STAGE = AB + BB + AS + BS;
   static constexpr int NA = AB / 4096, NB = NJ, NL = NA + NB + 2;  // loads per wave and step
@@ -159,6 +166,7 @@ template <bool GATE_UP, bool FP4, int MI, int NJ, bool SAVE_GU>
 __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) {
   using T = MxTile<GATE_UP, FP4, MI, NJ, SAVE_GU>;
   static_assert(!SAVE_GU || GATE_UP, "gate / up values are the first product's");
+  constexpr int NST = T::NST;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[NST * T::STAGE];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -217,23 +225,25 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   }
   const uint32_t ssrc = source_row((wave % MI) * 64 + lane);
   const uint32_t soff = ssrc == NONE ? NONE : ssrc * (uint32_t)lds_a;
+  const uint32_t boff = wave * T::NB * 1024 + lane * 16, toff = (wave % NJ) * 256 + lane * 4;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(KMOE_LDS uint8_t*)lds;
 
-  auto load_step = [&](int kt) {
-    const uint32_t base = lds0 + (uint32_t)(kt % NST) * T::STAGE;
-    const int k = __builtin_amdgcn_readfirstlane(kt);
-#pragma unroll
-    for (int q = 0; q < T::NA; ++q)
+  // load `q` of step k into the stage at byte offset st: A rows, weights, then the scales (64
+  // rows, or 128 bytes of two column blocks, a load; with fewer loads than waves two waves
+  // write the same values)
+  auto load_one = [&](auto q_tag, int k, uint32_t st) {
+    constexpr int q = decltype(q_tag)::value;
+    const uint32_t base = lds0 + st;
+    if constexpr (q < T::NA)
       buffer_to_lds16(ar, aoff[q], k * (FP4 ? 64 : 128), __builtin_amdgcn_readfirstlane(base + (wave * T::NA + q) * 1024));
-#pragma unroll
-    for (int q = 0; q < T::NB; ++q)
-      buffer_to_lds16(br, (wave * T::NB + q) * 1024 + lane * 16, k * TILE_STEP,
-                      __builtin_amdgcn_readfirstlane(base + T::AB + (wave * T::NB + q) * 1024));
-    // scales: 64 rows (128-byte halves of the column blocks) a load; with fewer loads than
-    // waves two waves write the same values
-    buffer_to_lds4(sr, soff, k * 4, __builtin_amdgcn_readfirstlane(base + T::AB + T::BB + (wave % MI) * 256));
-    buffer_to_lds4(tr, (wave % NJ) * 256 + lane * 4, k * SCALE_STEP,
-                   __builtin_amdgcn_readfirstlane(base + T::AB + T::BB + T::AS + (wave % NJ) * 256));
+    else if constexpr (q < T::NA + T::NB)
+      buffer_to_lds16(br, boff + (q - T::NA) * 1024, k * TILE_STEP,
+                      __builtin_amdgcn_readfirstlane(base + T::AB + (wave * T::NB + q - T::NA) * 1024));
+    else if constexpr (q == T::NA + T::NB)
+      buffer_to_lds4(sr, soff, k * 4, __builtin_amdgcn_readfirstlane(base + T::AB + T::BB + (wave % MI) * 256));
+    else
+      buffer_to_lds4(tr, toff, k * SCALE_STEP,
+                     __builtin_amdgcn_readfirstlane(base + T::AB + T::BB + T::AS + (wave % NJ) * 256));
   };
 
   f32x16_t acc[MI][NJ];
@@ -244,89 +254,112 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
 
-  i32x8_t fa[2][MI];
-  i32x4_t fb[2][NJ];
-  int sa[2][MI], sb[2][NJ];  // scales of a step (both substeps), double buffered
-  auto read_sub = [&](int kt, int i, int set) {
-    const uint8_t* const st = lds + (kt % NST) * T::STAGE;
-#pragma unroll
-    for (int mi = 0; mi < MI; ++mi) {
-      const int r = wm * 32 * MI + mi * 32 + lr;
-      if constexpr (FP4) {
-        const i32x4_t v = *reinterpret_cast<const i32x4_t*>(st + a_lds<true>(r, 2 * i + lh));
-        fa[set][mi] = i32x8_t{v[0], v[1], v[2], v[3], 0, 0, 0, 0};
-      } else {
-        const i32x4_t v = *reinterpret_cast<const i32x4_t*>(st + a_lds<false>(r, 4 * i + lh));
-        const i32x4_t u = *reinterpret_cast<const i32x4_t*>(st + a_lds<false>(r, 4 * i + 2 + lh));
-        fa[set][mi] = i32x8_t{v[0], v[1], v[2], v[3], u[0], u[1], u[2], u[3]};
-      }
+  // Operands of the two K halves of a step, and the step's scales (s: of the half about to be
+  // multiplied first, s2 their copy for the second)
+  constexpr int PER_A = FP4 ? 1 : 2;                // LDS reads of an A fragment
+  constexpr int NR = NJ + MI * PER_A, NS = NJ + MI;  // reads of a half's operands, of the scales
+  i32x4_t fa[2][MI][PER_A], fb[2][NJ];
+  int sa[MI], sb[NJ], sa2[MI], sb2[NJ];
+  auto read_one = [&](auto r_tag, auto half_tag, uint32_t st) {  // operand read r of half i
+    constexpr int r = decltype(r_tag)::value, i = decltype(half_tag)::value;
+    if constexpr (r < NJ) {
+      fb[i][r] = *reinterpret_cast<const i32x4_t*>(lds + st + T::AB + (wn * NJ + r) * 2048 + i * 1024 + lane * 16);
+    } else {
+      constexpr int mi = (r - NJ) / PER_A, part = (r - NJ) % PER_A;
+      const int row = wm * 32 * MI + mi * 32 + lr;
+      fa[i][mi][part] = *reinterpret_cast<const i32x4_t*>(lds + st + a_lds<FP4>(row, FP4 ? 2 * i + lh : 4 * i + 2 * part + lh));
     }
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      fb[set][j] = *reinterpret_cast<const i32x4_t*>(st + T::AB + (wn * NJ + j) * 2048 + i * 1024 + lane * 16);
   };
-  auto read_scales = [&](int kt, int set) {
-    const uint8_t* const sp = lds + (kt % NST) * T::STAGE + T::AB + T::BB;
-#pragma unroll
-    for (int mi = 0; mi < MI; ++mi)
-      sa[set][mi] = (int)(*reinterpret_cast<const uint32_t*>(sp + (wm * 32 * MI + mi * 32 + lr) * 4) >> (8 * lh));
-#pragma unroll
-    for (int j = 0; j < NJ; ++j)
-      sb[set][j] = *reinterpret_cast<const uint16_t*>(sp + T::AS + (wn * NJ + j) * 128 + lane * 2);
+  auto read_scale = [&](auto r_tag, uint32_t st) {
+    constexpr int r = decltype(r_tag)::value;
+    const uint8_t* const sp = lds + st + T::AB + T::BB;
+    if constexpr (r < NJ)
+      sb[r] = *reinterpret_cast<const uint16_t*>(sp + T::AS + (wn * NJ + r) * 128 + lane * 2);
+    else
+      sa[r - NJ] = (int)(*reinterpret_cast<const uint32_t*>(sp + (wm * 32 * MI + (r - NJ) * 32 + lr) * 4) >> (8 * lh));
   };
-  auto mma = [&](auto i_tag, int set) {
-    constexpr int i = decltype(i_tag)::value;
-#pragma unroll
-    for (int mi = 0; mi < MI; ++mi)
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) {
-        const i32x4_t b = fb[i][j];
-        acc[mi][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(i32x8_t{b[0], b[1], b[2], b[3], 0, 0, 0, 0}, fa[i][mi],
-                                                                      acc[mi][j], 4, FP4 ? 4 : 0, i, sb[set][j], 2 * i,
-                                                                      sa[set][mi]);
-      }
+  auto mma_one = [&](auto g_tag, auto half_tag) {
+    constexpr int g = decltype(g_tag)::value, i = decltype(half_tag)::value, mi = g / NJ, j = g % NJ;
+    const i32x4_t b = fb[i][j], a0 = fa[i][mi][0], a1 = FP4 ? i32x4_t{0, 0, 0, 0} : fa[i][mi][PER_A - 1];
+    acc[mi][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+        i32x8_t{b[0], b[1], b[2], b[3], 0, 0, 0, 0}, i32x8_t{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]},
+        acc[mi][j], 4, FP4 ? 4 : 0, i, i ? sb2[j] : sb[j], 2 * i, i ? sa2[mi] : sa[mi]);
   };
+  // The K loop is emitted in program order: each MFMA with the LDS reads and loads assigned to
+  // it, fenced with sched_barrier (left alone, the compiler moves the MFMAs of two steps
+  // behind all their reads and spills).  op(n): operation n of `count`, spread over the MFMAs
+  // [0, last).
+  constexpr int NM = MI * NJ;
+  auto spread = [&](auto g_tag, auto count_tag, auto last_tag, auto&& op) {
+    constexpr int g = decltype(g_tag)::value, count = decltype(count_tag)::value, last = decltype(last_tag)::value;
+    if constexpr (g < last)
+      static_for<(count * g + last - 1) / last, (count * (g + 1) + last - 1) / last>([&](auto n) { op(n); });
+  };
+  using H0 = std::integral_constant<int, 0>;
+  using H1 = std::integral_constant<int, 1>;
 
   const int nk = g.k_steps;
-#pragma unroll
-  for (int s = 0; s < NST; ++s)
-    if (s < nk) load_step(s);
-  if (nk >= 3)
-    wait_vmcnt<2 * T::NL>();
-  else if (nk == 2)
+  static_for<0, NST>([&](auto s) {
+    if (s < nk) static_for<0, T::NL>([&](auto q) { load_one(q, s, s * T::STAGE); });
+  });
+  if (NST == 3 && nk >= 3)
+    wait_vmcnt<(NST - 1) * T::NL>();
+  else if (nk >= 2)
     wait_vmcnt<T::NL>();
   else
     wait_vmcnt<0>();
   barrier_nofence();
-  read_sub(0, 0, 0);
-  read_scales(0, 0);
+  static_for<0, NR>([&](auto r) { read_one(r, H0{}, 0); });
+  static_for<0, NS>([&](auto r) { read_scale(r, 0); });
+  uint32_t cur = 0;  // byte offset of the step's stage
   // Step kt: its first half is in registers.  Its second half is read under the first half's
   // products; then every wave is done with the step's stage, so the barrier that publishes
-  // step kt + 1 also frees it for step kt + 3.
-  auto step = [&](int kt, auto par_tag) {
-    constexpr int par = decltype(par_tag)::value;  // set of the step's scales
-    read_sub(kt, 1, 1);
-    mma(std::integral_constant<int, 0>{}, par);
-    if (kt + 1 < nk) {
+  // step kt + 1 also frees it for step kt + NST (LOAD), whose loads go out under the second
+  // half's products with the reads of step kt + 1.  WAIT: loads that may stay in flight at the
+  // barrier; -1: the last step.
+  auto step = [&](int kt, auto load_tag, auto wait_tag) {
+    constexpr bool LOAD = decltype(load_tag)::value;
+    constexpr int WAIT = decltype(wait_tag)::value;
+    const uint32_t nxt = cur + T::STAGE == NST * T::STAGE ? 0 : cur + T::STAGE;
+    static_for<0, NM>([&](auto gt) {
+      mma_one(gt, H0{});
+      spread(gt, std::integral_constant<int, NR>{}, std::integral_constant<int, (NM * 3 + 3) / 4>{},
+             [&](auto n) { read_one(n, H1{}, cur); });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) sb2[j] = sb[j];
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) sa2[mi] = sa[mi];
+    if constexpr (WAIT >= 0) {
       wait_lgkmcnt0();
-      if (kt + 2 < nk)
-        wait_vmcnt<T::NL>();
-      else
-        wait_vmcnt<0>();
+      wait_vmcnt<(WAIT >= 0 ? WAIT : 0)>();
       barrier_nofence();
-      if (kt + 3 < nk) load_step(kt + 3);
-      read_sub(kt + 1, 0, 0);
-      read_scales(kt + 1, par ^ 1);
     }
-    mma(std::integral_constant<int, 1>{}, par);
+    __builtin_amdgcn_sched_barrier(0);
+    static_for<0, NM>([&](auto gt) {
+      mma_one(gt, H1{});
+      if constexpr (WAIT >= 0)
+        spread(gt, std::integral_constant<int, NR + NS>{}, std::integral_constant<int, (NM * 3 + 3) / 4>{}, [&](auto n) {
+          if constexpr (n < NR)
+            read_one(n, H0{}, nxt);
+          else
+            read_scale(std::integral_constant<int, n - NR>{}, nxt);
+        });
+      if constexpr (LOAD)
+        spread(gt, std::integral_constant<int, T::NL>{}, std::integral_constant<int, NM>{},
+               [&](auto n) { load_one(n, kt + NST, cur); });
+      __builtin_amdgcn_sched_barrier(0);
+    });
+    cur = nxt;
   };
   int kt = 0;
 #pragma unroll 1
-  for (; kt + 1 < nk; kt += 2) {
-    step(kt, std::integral_constant<int, 0>{});
-    step(kt + 1, std::integral_constant<int, 1>{});
-  }
-  if (kt < nk) step(kt, std::integral_constant<int, 0>{});
+  for (; kt + NST < nk; ++kt) step(kt, std::true_type{}, std::integral_constant<int, (NST - 2) * T::NL>{});
+  if constexpr (NST == 3)
+    if (kt + 2 < nk) step(kt++, std::false_type{}, std::integral_constant<int, T::NL>{});
+  if (kt + 1 < nk) step(kt++, std::false_type{}, std::integral_constant<int, 0>{});
+  step(kt, std::false_type{}, std::integral_constant<int, -1>{});
 
   // ---- epilogue: lane's row of block mi, columns 8 c + 4 lh + t of block j
 #pragma unroll

@@ -11,7 +11,7 @@ namespace {
 // Rows of a tile / 64 for max_rows rows over E experts.
 int tile_rows(int64_t max_rows, int E) {
   const int64_t per = max_rows / E;
-  return per > 128 ? 4 : per > 64 ? 2 : 1;
+  return per > 128 ? 2 : per > 64 ? 2 : 1;
 }
 
 int check(const char* who, const void* a, const uint8_t* a_scale, int fmt, const int32_t* offsets, int E, int d, int F,
