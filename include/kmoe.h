@@ -582,7 +582,8 @@ int kmoe_add_rmsnorm(const void* x, int x_dtype, const void* delta, int delta_dt
  *   infinity has scale 255 and stands for NaN.
  * A coded row holds K values rounded up to a multiple of 128 (padding: zero codes):
  * kmoe_mx_row_bytes(K, fmt) bytes of codes (e2m1: two to a byte, the first in the low
- * half) and kmoe_mx_scale_bytes(K) scale bytes.                                    */
+ * half) and kmoe_mx_scale_bytes(K) scale bytes, of which those past the padded values
+ * are not used.                                    */
 size_t kmoe_mx_row_bytes(int K, int fmt);
 size_t kmoe_mx_scale_bytes(int K);
 /* Codes of bf16 rows x[row_index ? row_index[r] : r] (K a multiple of 32);
@@ -613,6 +614,21 @@ int kmoe_gemm_gate_up_mx(const void* xq, const uint8_t* x_scale, int fmt, int64_
 /* y (max_rows, d) bf16 = h w3 of those rows.                                       */
 int kmoe_gemm_down_mx(const void* hq, const uint8_t* h_scale, int fmt, const int32_t* offsets, int E, int d, int F,
                       int64_t max_rows, const void* w3_packed, const uint8_t* w3_scale, void* y, void* stream);
+/* Routed tokens through those experts in one call: kmoe_dispatch (tables only), the rows'
+ * quantisation, the two products and kmoe_combine_residual.  Token t's row is
+ * x[row_index ? row_index[t] : t], or coded row t of xq, x_scale when given (no row_index
+ * then); topk_idx, topk_w (T, k), capacity, counts as for kmoe_dispatch; block_counts
+ * (nullable) as for kmoe_dispatch_counted, with partials, w_lb, w_z, aux_out (nullable) as
+ * for kmoe_dispatch_counted_aux; out_map, out_scale, residual, T_out, y as for
+ * kmoe_combine_residual.  T > 0.                                                   */
+size_t kmoe_mx_experts_workspace_bytes(int64_t T, int d, int E, int k, int F, int fmt, int coded);
+int kmoe_mx_experts(const void* x, const int32_t* row_index, int64_t T, int d, int fmt, const void* xq,
+                    const uint8_t* x_scale, const int64_t* topk_idx, const void* topk_w, int w_dtype, int k, int E,
+                    int64_t capacity, const int32_t* block_counts, const float* partials, float w_lb, float w_z,
+                    float* aux_out, const void* w13_packed, const uint8_t* w13_scale, const void* w3_packed,
+                    const uint8_t* w3_scale, int F, const int32_t* out_map, const float* out_scale,
+                    const void* residual, int64_t T_out, void* y, int y_dtype, int32_t* counts, void* workspace,
+                    size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -28,9 +28,10 @@ constexpr int TILE_STEP = 16 * 1024;   // bytes of a weight tile per step
 constexpr int SCALE_STEP = 1024;       // scale bytes of a weight tile per step
 
 __host__ __device__ inline int round_up(int a, int b) { return (a + b - 1) / b * b; }
-// bytes of a row of K values (K rounded up to the step) and of its scales
+// Bytes of a row of K values (K rounded up to the step) and of its scales (rounded up to 16:
+// four steps, which the products load at once).
 __host__ __device__ inline int64_t row_bytes(bool fp4, int K) { return round_up(K, STEP) / (fp4 ? 2 : 1); }
-__host__ __device__ inline int64_t scale_bytes(int K) { return round_up(K, STEP) / BLOCK; }
+__host__ __device__ inline int64_t scale_bytes(int K) { return round_up(K, 4 * STEP) / BLOCK; }
 
 // Scale byte of a block whose largest magnitude has the bits amax (NaN or infinity: 255).
 // The exponent bits of a float are floor(log2) + 127; subnormal floats count as 2^-127.

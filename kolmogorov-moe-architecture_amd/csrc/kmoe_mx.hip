@@ -20,7 +20,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const uint16_t* __restr
                                                          int64_t rows, const int32_t* __restrict__ n_rows_dev, int K,
                                                          uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
   const int64_t nr = n_rows_dev ? min<int64_t>(rows, (int64_t)*n_rows_dev) : rows;
-  const int Kp = round_up(K, STEP), cpr = Kp / 8;
+  const int Kp = round_up(K, STEP), cpr = Kp / 8, spr = (int)scale_bytes(K);
   const int64_t total = nr * cpr;  // a multiple of 16: the lanes of a block stay together
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / cpr;
@@ -36,7 +36,7 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const uint16_t* __restr
       *reinterpret_cast<uint32_t*>(q + r * (Kp / 2) + c * 4) = o.w[0];
     else
       *reinterpret_cast<i32x2_t*>(q + r * Kp + c * 8) = i32x2_t{(int)o.w[0], (int)o.w[1]};
-    if ((c & 3) == 0) scale[r * (Kp / BLOCK) + c / 4] = (uint8_t)code;
+    if ((c & 3) == 0) scale[r * spr + c / 4] = (uint8_t)code;
   }
 }
 
@@ -74,7 +74,7 @@ __global__ __launch_bounds__(256) void dequant_rows_kernel(const uint8_t* __rest
                                                            const int32_t* __restrict__ n_rows_dev, int K,
                                                            uint16_t* __restrict__ out) {
   const int64_t nr = n_rows_dev ? min<int64_t>(rows, (int64_t)*n_rows_dev) : rows;
-  const int Kp = round_up(K, STEP), cpr = K / 8;
+  const int Kp = round_up(K, STEP), cpr = K / 8, spr = (int)scale_bytes(K);
   const int64_t total = nr * cpr;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
     const int64_t r = i / cpr;
@@ -82,7 +82,7 @@ __global__ __launch_bounds__(256) void dequant_rows_kernel(const uint8_t* __rest
     const int64_t src = row_index ? (int64_t)row_index[r] : r;
     float v[8] = {};
     if (src >= 0) {
-      const float s = scale_value(scale[src * (Kp / BLOCK) + c / 4]);
+      const float s = scale_value(scale[src * spr + c / 4]);
       decode8<FP4>(q + (FP4 ? src * (Kp / 2) + c * 4 : src * Kp + c * 8), s, v);
     }
     *reinterpret_cast<i32x4_t*>(out + r * K + c * 8) = pack8(v);

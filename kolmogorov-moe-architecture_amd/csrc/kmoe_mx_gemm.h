@@ -155,11 +155,13 @@ __device__ __forceinline__ void store_block(const float (&v)[16], int half, bool
 template <bool GATE_UP, bool FP4, int MI, int NJ, bool SAVE_GU>
 struct MxTile {
   static constexpr int BM = 64 * MI;
-  static constexpr int NST = MI == 2 ? 2 : 3;  // LDS stages
-  static constexpr int AB = BM * (FP4 ? 64 : 128), BB = NJ * 4096, AS = BM * 4, BS = NJ * 256;
-  static constexpr int STAGE = AB + BB + AS + BS;
-  static constexpr int NA = AB / 4096, NB = NJ, NL = NA + NB + 2;  // loads per wave and step
-  static_assert(NST * STAGE <= 160 * 1024, "LDS");
+  static constexpr int NST = MI == 2 && !FP4 ? 2 : 3;  // LDS stages: two workgroups fit a CU at MI 2
+  static constexpr int AB = BM * (FP4 ? 64 : 128), BB = NJ * 4096, BS = NJ * 256;
+  static constexpr int STAGE = AB + BB + BS;
+  static constexpr int AS = BM * 16;  // the rows' scales of four steps, two sets behind the stages
+  static constexpr int LDS = NST * STAGE + 2 * AS;
+  static constexpr int NA = AB / 4096, NB = NJ, NL = NA + NB + 1;  // loads per wave and step, without those scales
+  static_assert(LDS <= 160 * 1024, "LDS");
 };
 
 template <bool GATE_UP, bool FP4, int MI, int NJ, bool SAVE_GU>
@@ -167,7 +169,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   using T = MxTile<GATE_UP, FP4, MI, NJ, SAVE_GU>;
   static_assert(!SAVE_GU || GATE_UP, "gate / up values are the first product's");
   constexpr int NST = T::NST;
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[NST * T::STAGE];
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lr = lane & 31, lh = lane >> 5;
@@ -198,7 +200,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   const int rows = m_end - m0;
 
   // operand windows and per-lane offsets of a step's loads
-  const int64_t lda = (int64_t)g.k_steps * (FP4 ? 64 : 128), lds_a = (int64_t)g.k_steps * 4;
+  const int64_t lda = (int64_t)g.k_steps * (FP4 ? 64 : 128), lds_a = (int64_t)((g.k_steps + 3) / 4) * 16;
   const bool gather = GATE_UP && g.row_token;
   const i32x4_t ar = gather ? buffer_of(g.a, g.a_rows * lda) : buffer_of(g.a + m0 * lda, rows * lda);
   const i32x4_t sr = gather ? buffer_of(g.a_scale, g.a_rows * lds_a) : buffer_of(g.a_scale + m0 * lds_a, rows * lds_a);
@@ -223,14 +225,13 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
     const uint32_t src = source_row(r);
     aoff[q] = src == NONE ? NONE : src * (uint32_t)lda + chunk16;
   }
-  const uint32_t ssrc = source_row((wave % MI) * 64 + lane);
+  const uint32_t ssrc = wave < MI ? source_row(wave * 64 + lane) : NONE;
   const uint32_t soff = ssrc == NONE ? NONE : ssrc * (uint32_t)lds_a;
   const uint32_t boff = wave * T::NB * 1024 + lane * 16, toff = (wave % NJ) * 256 + lane * 4;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(KMOE_LDS uint8_t*)lds;
 
-  // load `q` of step k into the stage at byte offset st: A rows, weights, then the scales (64
-  // rows, or 128 bytes of two column blocks, a load; with fewer loads than waves two waves
-  // write the same values)
+  // load `q` of step k into the stage at byte offset st: A rows, weights, their scales (two
+  // column blocks a load; with fewer loads than waves two waves write the same values)
   auto load_one = [&](auto q_tag, int k, uint32_t st) {
     constexpr int q = decltype(q_tag)::value;
     const uint32_t base = lds0 + st;
@@ -239,11 +240,16 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
     else if constexpr (q < T::NA + T::NB)
       buffer_to_lds16(br, boff + (q - T::NA) * 1024, k * TILE_STEP,
                       __builtin_amdgcn_readfirstlane(base + T::AB + (wave * T::NB + q - T::NA) * 1024));
-    else if constexpr (q == T::NA + T::NB)
-      buffer_to_lds4(sr, soff, k * 4, __builtin_amdgcn_readfirstlane(base + T::AB + T::BB + (wave % MI) * 256));
     else
-      buffer_to_lds4(tr, toff, k * SCALE_STEP,
-                     __builtin_amdgcn_readfirstlane(base + T::AB + T::BB + T::AS + (wave % NJ) * 256));
+      buffer_to_lds4(tr, toff, k * SCALE_STEP, __builtin_amdgcn_readfirstlane(base + T::AB + T::BB + (wave % NJ) * 256));
+  };
+  // The rows' scales come four steps at a time, 16 bytes a row (a dword a step was half of all
+  // L2 requests): 64 rows a wave, by the first MI waves, in front of the loads of a step
+  // that begins four.
+  auto load_row_scales = [&](int k) {
+    if ((k & 3) == 0 && wave < MI)
+      buffer_to_lds16(sr, soff, k * 4,
+                      __builtin_amdgcn_readfirstlane(lds0 + NST * T::STAGE + ((k >> 2) & 1) * T::AS + wave * 1024));
   };
 
   f32x16_t acc[MI][NJ];
@@ -270,13 +276,14 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
       fa[i][mi][part] = *reinterpret_cast<const i32x4_t*>(lds + st + a_lds<FP4>(row, FP4 ? 2 * i + lh : 4 * i + 2 * part + lh));
     }
   };
-  auto read_scale = [&](auto r_tag, uint32_t st) {
+  auto read_scale = [&](auto r_tag, int k, uint32_t st) {
     constexpr int r = decltype(r_tag)::value;
-    const uint8_t* const sp = lds + st + T::AB + T::BB;
-    if constexpr (r < NJ)
-      sb[r] = *reinterpret_cast<const uint16_t*>(sp + T::AS + (wn * NJ + r) * 128 + lane * 2);
-    else
-      sa[r - NJ] = (int)(*reinterpret_cast<const uint32_t*>(sp + (wm * 32 * MI + (r - NJ) * 32 + lr) * 4) >> (8 * lh));
+    if constexpr (r < NJ) {
+      sb[r] = *reinterpret_cast<const uint16_t*>(lds + st + T::AB + T::BB + (wn * NJ + r) * 128 + lane * 2);
+    } else {
+      const uint8_t* const sp = lds + NST * T::STAGE + ((k >> 2) & 1) * T::AS + (k & 3) * 4;
+      sa[r - NJ] = (int)(*reinterpret_cast<const uint32_t*>(sp + (wm * 32 * MI + (r - NJ) * 32 + lr) * 16) >> (8 * lh));
+    }
   };
   auto mma_one = [&](auto g_tag, auto half_tag) {
     constexpr int g = decltype(g_tag)::value, i = decltype(half_tag)::value, mi = g / NJ, j = g % NJ;
@@ -300,7 +307,10 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
 
   const int nk = g.k_steps;
   static_for<0, NST>([&](auto s) {
-    if (s < nk) static_for<0, T::NL>([&](auto q) { load_one(q, s, s * T::STAGE); });
+    if (s < nk) {
+      load_row_scales(s);
+      static_for<0, T::NL>([&](auto q) { load_one(q, s, s * T::STAGE); });
+    }
   });
   if (NST == 3 && nk >= 3)
     wait_vmcnt<(NST - 1) * T::NL>();
@@ -310,7 +320,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
     wait_vmcnt<0>();
   barrier_nofence();
   static_for<0, NR>([&](auto r) { read_one(r, H0{}, 0); });
-  static_for<0, NS>([&](auto r) { read_scale(r, 0); });
+  static_for<0, NS>([&](auto r) { read_scale(r, 0, 0); });
   uint32_t cur = 0;  // byte offset of the step's stage
   // Step kt: its first half is in registers.  Its second half is read under the first half's
   // products; then every wave is done with the step's stage, so the barrier that publishes
@@ -333,9 +343,14 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
     for (int mi = 0; mi < MI; ++mi) sa2[mi] = sa[mi];
     if constexpr (WAIT >= 0) {
       wait_lgkmcnt0();
-      wait_vmcnt<(WAIT >= 0 ? WAIT : 0)>();
+      // (one load more may stay in flight where step kt + 2 began with row scales)
+      if (WAIT > 0 && ((kt + 2) & 3) == 0 && wave < MI)
+        wait_vmcnt<(WAIT > 0 ? WAIT + 1 : 0)>();
+      else
+        wait_vmcnt<(WAIT >= 0 ? WAIT : 0)>();
       barrier_nofence();
     }
+    if constexpr (LOAD) load_row_scales(kt + NST);
     __builtin_amdgcn_sched_barrier(0);
     static_for<0, NM>([&](auto gt) {
       mma_one(gt, H1{});
@@ -344,7 +359,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
           if constexpr (n < NR)
             read_one(n, H0{}, nxt);
           else
-            read_scale(std::integral_constant<int, n - NR>{}, nxt);
+            read_scale(std::integral_constant<int, n - NR>{}, kt + 1, nxt);
         });
       if constexpr (LOAD)
         spread(gt, std::integral_constant<int, T::NL>{}, std::integral_constant<int, NM>{},
@@ -375,7 +390,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
 #pragma unroll
         for (int i = 0; i < 16; ++i) h[i] = silu_fast_f32(acc[mi][2 * p][i]) * acc[mi][2 * p + 1][i];
         store_block<FP4>(h, lh, on, g.q + row * (g.ldc / (FP4 ? 2 : 1)) + f0 / (FP4 ? 2 : 1),
-                         g.q_scale + row * (g.ldc / BLOCK) + f0 / BLOCK);
+                         g.q_scale + row * scale_bytes((int)g.ldc) + f0 / BLOCK);
         if constexpr (SAVE_GU) {
           uint16_t* const gp = g.gu + row * 2 * g.ldc + (f0 >> 7) * 256 + (f0 & 127) + 8 * lh;
 #pragma unroll
@@ -410,6 +425,7 @@ struct MxLaunch {
   int64_t max_rows;
   hipStream_t s;
 };
+constexpr int SMALL_ROWS = 32;  // rows of a slot of the small-row kernel
 template <bool GATE_UP, bool FP4, int MI, int NJ, bool SAVE_GU = false>
 void launch_mx_tile(MxLaunch l) {
   using T = MxTile<GATE_UP, FP4, MI, NJ, SAVE_GU>;
@@ -420,5 +436,6 @@ void launch_mx_tile(MxLaunch l) {
 }
 void launch_mx_gate_up(const MxLaunch& l, bool fp4, int mi);  // with l.g.gu: saving the gate / up values
 void launch_mx_down(const MxLaunch& l, bool fp4, int mi);
+void launch_mx_small(const MxLaunch& l, bool gate_up, bool fp4);
 
 }  // namespace kmoe_mx

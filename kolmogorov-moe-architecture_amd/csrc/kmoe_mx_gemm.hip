@@ -14,6 +14,19 @@ int tile_rows(int64_t max_rows, int E) {
   return per > 128 ? 2 : per > 64 ? 2 : 1;
 }
 
+// Whether a product runs on the small-row kernel (kmoe_mx_gemm_small.hip): where its grid is at
+// most three workgroups per CU, as latency then counts, at few rows per expert.  Kernel times
+// in us, small-row kernel / 64-row tiles, top-2 of 16 experts, d 2048, F 2816, w4a8: 1 token
+// (176 workgroups in gate/up, 128 in down) 6.1 / 11.2 and 5.2 / 12.7; 4 tokens (704, 512) 9.8 /
+// 11.9 and 7.5 / 12.7; 8 tokens (1408, 1024) 19.5 / 12.8 and 10.4 / 12.7; 48 tokens (1672,
+// 1216) 28 / 20 and 15.7 / 13.5; 32 rows of 64 experts, d 1024, F 704 (792, 1056) 12.5 / 8.1
+// and 7.5 / 6.3: each workgroup looks its slot up and reduces, which the tiles do once for
+// eight times the weights.
+bool small_product(bool gate_up, int64_t max_rows, int E, int b_tiles) {
+  const int64_t slots = max_rows / SMALL_ROWS + std::min<int64_t>(max_rows, E);
+  return max_rows <= 32 * (int64_t)E && slots * b_tiles * (gate_up ? 4 : 8) <= 3 * kmoe::cu_count();
+}
+
 int check(const char* who, const void* a, const uint8_t* a_scale, int fmt, const int32_t* offsets, int E, int d, int F,
           int64_t max_rows, const void* w, const uint8_t* ws, int64_t a_rows, int K) {
   KMOE_REQUIRE(a && a_scale && offsets && w && ws, KMOE_ERR_NULL, "%s: null buffer", who);
@@ -28,8 +41,8 @@ int check(const char* who, const void* a, const uint8_t* a_scale, int fmt, const
   KMOE_REQUIRE((a_rows + 1) * lda < (int64_t)1 << 31 && 257 * lda < (int64_t)1 << 31 &&
                    (int64_t)round_up(K, STEP) * 128 < (int64_t)1 << 31,
                KMOE_ERR_SHAPE, "%s: operand too large for 32-bit offsets (%lld rows, K=%d)", who, (long long)a_rows, K);
-  // a launch takes 2^24 workgroups of 256
-  KMOE_REQUIRE((max_rows / 64 + E) * (int64_t)std::max(round_up(F, 128) / 128, round_up(d, 256) / 256) < 1 << 24,
+  // a launch takes 2^24 workgroups of 256, 2^23 of 512
+  KMOE_REQUIRE((max_rows / SMALL_ROWS + E) * (int64_t)std::max(round_up(F, 128) / 32, round_up(d, 256) / 32) < 1 << 23,
                KMOE_ERR_SHAPE, "%s: grid too large", who);
   return KMOE_OK;
 }
@@ -65,7 +78,10 @@ extern "C" int kmoe_gemm_gate_up_mx(const void* xq, const uint8_t* x_scale, int 
   l.g.ldc = Fp;
   l.max_rows = max_rows;
   l.s = kmoe::as_stream(stream);
-  launch_mx_gate_up(l, fmt == KMOE_DTYPE_FP4_E2M1, tile_rows(max_rows, E));
+  if (small_product(true, max_rows, E, l.g.b_tiles))
+    launch_mx_small(l, true, fmt == KMOE_DTYPE_FP4_E2M1);
+  else
+    launch_mx_gate_up(l, fmt == KMOE_DTYPE_FP4_E2M1, tile_rows(max_rows, E));
   return kmoe::check_launch("kmoe_gemm_gate_up_mx");
 }
 
@@ -91,6 +107,9 @@ extern "C" int kmoe_gemm_down_mx(const void* hq, const uint8_t* h_scale, int fmt
   l.g.n_valid = d;
   l.max_rows = max_rows;
   l.s = kmoe::as_stream(stream);
-  launch_mx_down(l, fmt == KMOE_DTYPE_FP4_E2M1, tile_rows(max_rows, E));
+  if (small_product(false, max_rows, E, l.g.b_tiles))
+    launch_mx_small(l, false, fmt == KMOE_DTYPE_FP4_E2M1);
+  else
+    launch_mx_down(l, fmt == KMOE_DTYPE_FP4_E2M1, tile_rows(max_rows, E));
   return kmoe::check_launch("kmoe_gemm_down_mx");
 }

@@ -181,7 +181,7 @@ __global__ __launch_bounds__(64 * NORM_FWD_WAVES) void add_rmsnorm_kernel(
           *reinterpret_cast<uint32_t*>(q + t * (qvec * 4) + v * 4) = w.w[0];
         else
           *reinterpret_cast<i32x2_t*>(q + t * (qvec * 8) + v * 8) = i32x2_t{(int)w.w[0], (int)w.w[1]};
-        if ((v & 3) == 0) scale[t * (qvec / 4) + v / 4] = (uint8_t)code;
+        if ((v & 3) == 0) scale[t * kmoe_mx::scale_bytes(d) + v / 4] = (uint8_t)code;
       }
     }
   }

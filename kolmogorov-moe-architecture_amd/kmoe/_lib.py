@@ -121,6 +121,9 @@ _SIGNATURES = {
     "kmoe_packed_mx_bytes": (_sz, [_i32, _i32, _i32, _i32]),
     "kmoe_pack_weights_mx": (_i32, [_vp, _vp, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _vp, _vp, _vp]),
     "kmoe_gemm_gate_up_mx": (_i32, [_vp, _vp, _i32, _i64, _vp, _vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "kmoe_mx_experts_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32, _i32, _i32]),
+    "kmoe_mx_experts": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i64, _vp, _vp, _f32, _f32,
+                               _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _i32, _vp, _vp, _sz, _vp]),
     "kmoe_gemm_down_mx": (_i32, [_vp, _vp, _i32, _vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp, _vp]),
 }
 

@@ -364,7 +364,8 @@ class GroupedExperts(_PackedExperts):
 
     def run(self, x2d, expert_indices, expert_weights, row_index=None, T_out=None, out_map=None, scale=None,
             out_dtype=torch.bfloat16, residual=None, capacity=0, block_counts=None, aux=None, coded=None):
-        """dispatch -> grouped GEMMs -> combine (+ residual, added in the combine); returns (y, DispatchOut).
+        """dispatch -> grouped GEMMs -> combine (+ residual, added in the combine); returns (y, DispatchOut;
+        for microscaled experts its counts and aux).
         capacity > 0 drops each expert's assignments past the first `capacity` (MoELayer's
         drop_overflow rule); 0, the default and what forward() uses, drops nothing (the
         reference's GroupedExperts never drops).  block_counts: the router's per-block
@@ -376,6 +377,13 @@ class GroupedExperts(_PackedExperts):
         pw = self.packed()
         T, k = expert_indices.shape
         if self.mx is not None:
+            if not ops.stage_timing():
+                y, counts, aux_out = ops.mx_experts(x2d, expert_indices, expert_weights, pw, self.mx_act, capacity=capacity,
+                                                    row_index=row_index, coded=coded, block_counts=block_counts, aux=aux,
+                                                    T_out=T_out, out_map=out_map, scale=scale, out_dtype=out_dtype,
+                                                    residual=residual)
+                return y, ops.RoutedOut(counts, aux_out)
+            # the same, call by call
             disp = ops.dispatch(x2d, expert_indices, expert_weights, E, capacity=capacity, row_index=row_index,
                                 materialize=False, block_counts=block_counts, aux=aux)
             if coded is None:
@@ -406,8 +414,6 @@ class GroupedExperts(_PackedExperts):
         if self._trainable(x, expert_weights):
             return _ExpertsFn.apply(x, expert_weights, self.w1, self.w2, self.w3, self, expert_indices)
         out_dtype = torch.float32 if x.dtype == torch.float32 else torch.bfloat16
-        if self.mx is not None and x.shape[0] == 0:
-            return x.new_empty(0, self.d_model)
         y, _ = self.run(x, expert_indices, expert_weights, out_dtype=out_dtype)
         return _forward_only(y.to(x.dtype), x, self.w1, self.w2, self.w3, expert_weights)
 

@@ -35,6 +35,25 @@ def _stream(t):
     return _lib.stream_ptr(t.device)
 
 
+class _Here:
+    """Context of a call on the current device."""
+
+    def __enter__(self):
+        return self
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def _device(dev):
+    """Context that makes `dev` the current device (the launch's device, and the one whose CU
+    count sizes grids), for nothing where it already is."""
+    return _HERE if dev.index == torch.cuda.current_device() else torch.cuda.device(dev)
+
+
 # ---------------------------------------------------------------- stage timing
 # When a list is installed here (bench.py does), every stage records a pair of
 # HIP events on the launch stream: (name, start, end).  Off by default.
@@ -756,7 +775,7 @@ def route_topk(logits, k, scores="softmax", bias=None, groups=1, topk_groups=1, 
     dev = logits.device
     idx = torch.empty(T, int(k), device=dev, dtype=torch.int64)
     w = torch.empty(T, int(k), device=dev, dtype=torch.float32)
-    with torch.cuda.device(dev), _Stage("route"):
+    with _device(dev), _Stage("route"):
         bc = torch.empty(-(-T // router_block_tokens(T)), E, device=dev, dtype=torch.int32) if hist and T > 0 else None
         _lib.call("kmoe_route_topk", ptr(logits), T, E, int(k), sc, ptr(bias), int(groups), int(topk_groups),
                   int(group_top), int(bool(renorm)), float(scale), ptr(idx), ptr(w), ptr(bc), _stream(logits))
@@ -778,7 +797,7 @@ def route_topk_bwd(logits, idx, dw, scores="softmax", renorm=True, scale=1.0, dl
         raise ValueError(f"kmoe.route_topk_bwd: dlogits must be contiguous f32 ({T}, {E})")
     if not add:
         dlogits = torch.empty(T, E, device=logits.device, dtype=torch.float32)
-    with torch.cuda.device(logits.device), _Stage("bwd_router"):
+    with _device(logits.device), _Stage("bwd_router"):
         _lib.call("kmoe_route_topk_bwd", ptr(logits), ptr(_contig(idx, torch.int64)), ptr(_contig(dw, torch.float32)), T, E,
                   k, sc, int(bool(renorm)), float(scale), int(add), ptr(dlogits), _stream(logits))
     return dlogits
@@ -800,7 +819,8 @@ def _mx_fmt(fmt) -> int:
 class MXRows(NamedTuple):
     """Rows in blocks of 32 values that share a power-of-two scale.  q (rows, Kp) e4m3 codes
     or (rows, Kp / 2) e2m1 pairs, the first in the low half, Kp = K rounded up to 128;
-    scale (rows, Kp / 32), byte c for 2^(c - 127), 255 for a block of NaN."""
+    scale (rows, K rounded up to 512, / 32), byte c for 2^(c - 127), 255 for a block of NaN; bytes
+    past Kp / 32 are not used."""
     q: torch.Tensor
     scale: torch.Tensor
     K: int
@@ -810,7 +830,7 @@ class MXRows(NamedTuple):
 def _mx_rows(rows, K, fmt, dev) -> MXRows:
     kp = (K + 127) // 128 * 128
     return MXRows(torch.empty(rows, kp if fmt == "e4m3" else kp // 2, device=dev, dtype=torch.uint8),
-                  torch.empty(rows, kp // 32, device=dev, dtype=torch.uint8), K, fmt)
+                  torch.empty(rows, (K + 511) // 512 * 16, device=dev, dtype=torch.uint8), K, fmt)
 
 
 def quant_rows_mx(m, fmt="e4m3", row_index=None, n_rows_dev=None) -> MXRows:
@@ -825,7 +845,7 @@ def quant_rows_mx(m, fmt="e4m3", row_index=None, n_rows_dev=None) -> MXRows:
         row_index = _contig(row_index, torch.int32)
     rows = m.shape[0] if row_index is None else row_index.numel()
     out = _mx_rows(rows, m.shape[1], fmt, m.device)
-    with torch.cuda.device(m.device), _Stage("quant_x"):
+    with _device(m.device), _Stage("quant_x"):
         _lib.call("kmoe_quant_rows_mx", ptr(m), ptr(row_index), rows, ptr(n_rows_dev), m.shape[1], code, ptr(out.q),
                   ptr(out.scale), _stream(m))
     return out
@@ -839,7 +859,7 @@ def dequant_rows_mx(r: MXRows, row_index=None, n_rows_dev=None):
         row_index = _contig(row_index, torch.int32)
     rows = r.q.shape[0] if row_index is None else row_index.numel()
     out = torch.empty(rows, r.K, device=r.q.device, dtype=_BF16)
-    with torch.cuda.device(r.q.device), _Stage("mx_dequant"):
+    with _device(r.q.device), _Stage("mx_dequant"):
         _lib.call("kmoe_dequant_rows_mx", ptr(r.q), ptr(r.scale), ptr(row_index), rows, ptr(n_rows_dev), r.K, code,
                   ptr(out), _stream(r.q))
     return out
@@ -855,7 +875,7 @@ def fake_quant_mx_cols(w):
     w = _contig(w.detach(), w.dtype)
     E, K, N = w.shape
     out = torch.empty(E, K, N, device=w.device, dtype=_BF16)
-    with torch.cuda.device(w.device):
+    with _device(w.device):
         _lib.call("kmoe_fake_quant_mx_cols", ptr(w), _fdt(w), E, K, N, ptr(out), _stream(w))
     return out
 
@@ -884,7 +904,7 @@ def pack_weights_mx(w1, w2, w3) -> PackedWeightsMX:
     lib = _lib.load()
     dev = w1.device
     bufs = [torch.empty(lib.kmoe_packed_mx_bytes(E, d, F, i), device=dev, dtype=torch.uint8) for i in range(4)]
-    with torch.cuda.device(dev):
+    with _device(dev):
         _lib.call("kmoe_pack_weights_mx", ptr(w1), ptr(w2), ptr(w3), _fdt(w1), E, d, F, *(ptr(b) for b in bufs), _stream(w1))
     return PackedWeightsMX(*bufs, E, d, F)
 
@@ -901,7 +921,7 @@ def gemm_gate_up_mx(x: MXRows, row_token, offsets, pw: PackedWeightsMX, max_rows
     fp = (pw.F + 127) // 128 * 128
     h = _mx_rows(max(max_rows, 1), pw.F, x.fmt, x.q.device)
     gu = torch.empty(max(max_rows, 1), 2 * fp, device=x.q.device, dtype=_BF16) if save_gu else None
-    with torch.cuda.device(x.q.device), _Stage("gemm_gate_up"):
+    with _device(x.q.device), _Stage("gemm_gate_up"):
         _lib.call("kmoe_gemm_gate_up_mx", ptr(x.q), ptr(x.scale), _mx_fmt(x.fmt), x.q.shape[0], ptr(row_token),
                   ptr(offsets), pw.E, pw.d, pw.F, max_rows, ptr(pw.w13), ptr(pw.s13), ptr(h.q), ptr(h.scale), ptr(gu),
                   _stream(x.q))
@@ -914,10 +934,73 @@ def gemm_down_mx(h: MXRows, offsets, pw: PackedWeightsMX, max_rows):
     if h.K != pw.F or h.q.shape[0] < max_rows:
         raise ValueError(f"kmoe.gemm_down_mx: rows {tuple(h.q.shape)} of {h.K} values, F={pw.F}, max_rows {max_rows}")
     y = torch.empty(max(max_rows, 1), pw.d, device=h.q.device, dtype=_BF16)
-    with torch.cuda.device(h.q.device), _Stage("gemm_down"):
+    with _device(h.q.device), _Stage("gemm_down"):
         _lib.call("kmoe_gemm_down_mx", ptr(h.q), ptr(h.scale), _mx_fmt(h.fmt), ptr(offsets), pw.E, pw.d, pw.F, max_rows,
                   ptr(pw.w3), ptr(pw.s3), ptr(y), _stream(h.q))
     return y
+
+
+class RoutedOut(NamedTuple):
+    """What a one-call pass over routed tokens reports of its dispatch."""
+    counts: torch.Tensor        # (E,) int32 routed counts
+    aux: Optional[torch.Tensor]  # (3,) f32 aux losses, when asked for
+
+
+def mx_experts(x2d, idx, w, pw: PackedWeightsMX, fmt, capacity=0, row_index=None, coded: Optional[MXRows] = None,
+               block_counts=None, aux=None, T_out=None, out_map=None, scale=None, out_dtype=_BF16, residual=None):
+    """Routed tokens through the 4-bit experts in one native call, as dispatch, quant_rows_mx,
+    gemm_gate_up_mx, gemm_down_mx and combine do it: (y (T_out, d), counts (E,) int32, aux
+    (3,) f32 or None).  fmt: element type of the activations; coded: their codes, if the
+    caller has them; aux = (partials, w_lb, w_z): as for dispatch."""
+    code = _mx_fmt(fmt)
+    _need_gpu(x2d, idx, w, row_index, residual)
+    x2d = _contig(x2d, _BF16)
+    idx = _contig(idx, torch.int64)
+    if w.dtype not in (torch.float32, _BF16):
+        w = w.float()
+    w = w.contiguous()
+    T, k = idx.shape
+    d = x2d.shape[1]
+    if w.shape != (T, k) or pw.d != d or (row_index is None and x2d.shape[0] != T):
+        raise ValueError(f"kmoe.mx_experts: x {tuple(x2d.shape)}, idx {(T, k)}, w {tuple(w.shape)}, weights of d={pw.d}")
+    xq = xs = None
+    if coded is not None:
+        if coded.fmt != fmt or coded.K != d or coded.q.shape[0] != T or row_index is not None:
+            raise ValueError(f"kmoe.mx_experts: coded rows {tuple(coded.q.shape)} ({coded.fmt}, K={coded.K}) for T={T}, "
+                             f"d={d}, {fmt}")
+        xq, xs = coded.q, coded.scale
+    if row_index is not None:
+        row_index = _contig(row_index, torch.int32)
+        if row_index.numel() != T:
+            raise ValueError(f"kmoe.mx_experts: row_index of {row_index.numel()} rows for {T} tokens")
+    T_out = T if T_out is None else T_out
+    dev = x2d.device
+    y = torch.empty(T_out, d, device=dev, dtype=out_dtype)
+    if residual is not None:
+        residual = _contig(residual, out_dtype)
+        if residual.shape != (T_out, d):
+            raise ValueError(f"kmoe.mx_experts: residual shape {tuple(residual.shape)} != {(T_out, d)}")
+    if T == 0:
+        y.zero_() if residual is None else y.copy_(residual)
+        return y, torch.zeros(pw.E, device=dev, dtype=torch.int32), None
+    counts = torch.empty(pw.E, device=dev, dtype=torch.int32)
+    partials = aux_out = None
+    w_lb = w_z = 0.0
+    if aux is not None:
+        partials, w_lb, w_z = aux
+        aux_out = torch.empty(3, device=dev, dtype=torch.float32)
+    lib = _lib._LIB or _lib.load()
+    with _device(dev):
+        if block_counts is not None and block_counts.numel() != -(-T // lib.kmoe_router_block_tokens(T)) * pw.E:
+            raise ValueError("kmoe.mx_experts: block_counts must be the router's per-block histograms")
+        wsb = lib.kmoe_mx_experts_workspace_bytes(T, d, pw.E, k, pw.F, code, int(coded is not None))
+        ws = torch.empty(max(wsb, 4), device=dev, dtype=torch.uint8)
+        _lib.call("kmoe_mx_experts", ptr(x2d), ptr(row_index), T, d, code, ptr(xq), ptr(xs), ptr(idx), ptr(w),
+                  _lib.DTYPE_F32 if w.dtype == torch.float32 else _lib.DTYPE_BF16, k, pw.E, int(capacity), ptr(block_counts),
+                  ptr(partials), float(w_lb), float(w_z), ptr(aux_out), ptr(pw.w13), ptr(pw.s13), ptr(pw.w3), ptr(pw.s3),
+                  pw.F, ptr(out_map), ptr(scale), ptr(residual), T_out, ptr(y),
+                  _lib.DTYPE_F32 if out_dtype == torch.float32 else _lib.DTYPE_BF16, ptr(counts), ptr(ws), wsb, _stream(x2d))
+    return y, counts, aux_out
 
 
 class AddNormOut(NamedTuple):
@@ -955,7 +1038,7 @@ def add_rmsnorm(x2d, delta, weight, eps, quant=None) -> AddNormOut:
     rrms = torch.empty(T, device=dev, dtype=torch.float32)
     rows = _mx_rows(T, d, quant, dev) if quant is not None else None
     q, scale = (None, None) if rows is None else rows[:2]
-    with torch.cuda.device(dev), _Stage("rmsnorm"):
+    with _device(dev), _Stage("rmsnorm"):
         _lib.call("kmoe_add_rmsnorm", ptr(x2d), _fdt(x2d), ptr(delta), _lib.DTYPE_BF16 if delta is None else _fdt(delta),
                   ptr(weight), _fdt(weight), float(eps), T, d, ptr(h), ptr(n), ptr(rrms), code, ptr(q), ptr(scale),
                   _stream(x2d))

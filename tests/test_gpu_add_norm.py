@@ -35,7 +35,8 @@ def test_forward(dev, quant, xd, dd, wd, T, d):
     assert bool(((r.n.double() - n64).abs() <= tol * n64.abs()).all())
     if quant:
         want = ops.quant_rows_mx(base.n, quant)
-        assert torch.equal(r.q, want.q) and torch.equal(r.scale, want.scale)
+        n = (d + 127) // 128 * 4  # scale bytes behind are not written
+        assert torch.equal(r.q, want.q) and torch.equal(r.scale[:, :n], want.scale[:, :n])
     else:
         assert r.q is None and r.scale is None
 
@@ -49,7 +50,7 @@ def test_without_delta_zero_rows_and_bad_values(dev):
     r = ops.add_rmsnorm(x, None, w, EPS, quant="e4m3")
     assert r.h.data_ptr() == x.data_ptr()
     assert not r.n[1].any() and not r.q[1].any()
-    assert bool(r.n[2].isnan().all()) and bool((r.scale[2] == 255).all())
+    assert bool(r.n[2].isnan().all()) and bool((r.scale[2, :4] == 255).all())
     good = [0, 1, 4, 5]
     clean = ops.add_rmsnorm(x[good], None, w, EPS, quant="e4m3")
     assert torch.equal(r.q[good], clean.q) and torch.equal(r.n[good], clean.n)
@@ -104,7 +105,9 @@ def test_views_streams_and_graph(dev):
     w = torch.ones(256, device=dev, dtype=BF)
     a = ops.add_rmsnorm(x[:, 128:384], delta[:, :256], w, EPS, quant="e4m3")
     b = ops.add_rmsnorm(x[:, 128:384].contiguous(), delta[:, :256].contiguous(), w, EPS, quant="e4m3")
-    assert all(torch.equal(u, v) for u, v in zip(a, b))
+    def same(a, b):
+        return all(torch.equal(u, v) for u, v in zip((*a[:4], a.scale[:, :8]), (*b[:4], b.scale[:, :8])))
+    assert same(a, b)
     bx, bd = x[:, :256].contiguous(), delta[:, :256].contiguous()
     g = torch.cuda.CUDAGraph()
     with torch.cuda.graph(g):
@@ -115,7 +118,7 @@ def test_views_streams_and_graph(dev):
         bx.copy_(nx)
         g.replay()
         torch.cuda.synchronize()
-        assert all(torch.equal(u, v) for u, v in zip(r, want))
+        assert same(r, want)
 
 
 def test_refusals(dev):

@@ -19,9 +19,14 @@ def rnd(dev, *shape, seed=0, std=1.0, dtype=BF):
     return (std * torch.randn(*shape, generator=g)).to(dtype).to(dev)
 
 
+def used(r: ops.MXRows):
+    """The scale bytes of the padded row (those behind are not written)."""
+    return r.scale[:, :(r.K + 127) // 128 * 4]
+
+
 def decode(r: ops.MXRows):
-    """(elements, scale bytes) of coded rows on the CPU, padding included."""
-    s = r.scale.cpu().long()
+    """(elements, scale bytes) of coded rows on the CPU, K padded to 128 included."""
+    s = used(r).cpu().long()
     if r.fmt == "e4m3":
         return r.q.cpu().view(torch.float8_e4m3fn).double(), s
     grid = torch.tensor([0, .5, 1, 1.5, 2, 3, 4, 6, -0., -.5, -1, -1.5, -2, -3, -4, -6], dtype=torch.float64)
@@ -77,7 +82,7 @@ def test_quant_gathered_rows_and_row_count(dev, fmt):
     index = torch.tensor([49, 0, 0, 7, 31], dtype=torch.int32, device=dev)
     got = ops.quant_rows_mx(x, fmt, row_index=index)
     want = ops.quant_rows_mx(x[index.long()], fmt)
-    assert torch.equal(got.q, want.q) and torch.equal(got.scale, want.scale)
+    assert torch.equal(got.q, want.q) and torch.equal(used(got), used(want))
     # a strided view, as a slice of a wider activation
     wide = rnd(dev, 50, 256, seed=2)
     assert torch.equal(ops.quant_rows_mx(wide[:, 64:192], fmt).q, ops.quant_rows_mx(wide[:, 64:192].contiguous(), fmt).q)
@@ -153,7 +158,7 @@ def test_products(dev, fmt, case):
     # permuted rows give the same bits, and so does the call without the saved values
     perm = ops.MXRows(xq.q[tokens.long()], xq.scale[tokens.long()], d, fmt)
     h2 = ops.gemm_gate_up_mx(perm, None, offsets, pw, A)
-    assert torch.equal(h.q, h2.q) and torch.equal(h.scale, h2.scale)
+    assert torch.equal(h.q, h2.q) and torch.equal(used(h), used(h2))
     y = ops.gemm_down_mx(h, offsets, pw, A)
     xv = M.quant(x.cpu(), fmt)[0][tokens.cpu().long()]
     wv = [M.q_cols(t.cpu()) for t in w]
@@ -440,6 +445,33 @@ def test_other_stream_and_graph(dev):
             assert torch.equal(layer(xs[(i + 1) % 4]), eager[(i + 1) % 4])
 
 
+@pytest.mark.parametrize("mx", ["w4a8", "w4a4"])
+@pytest.mark.parametrize("T,k,E,cap", [(1, 1, 1, 0), (1, 8, 16, 0), (48, 2, 16, 5), (341, 3, 64, 0), (342, 3, 5, 100), (700, 2, 8, 0)])
+def test_one_call_is_the_calls_it_makes(dev, mx, T, k, E, cap):
+    """The native pass against its pieces, bit for bit: at most 1024 assignments go through the
+    one-workgroup dispatch.  Ids out of range and one expert twice included."""
+    d, F = 192, 100
+    ex = kmoe.GroupedExperts(E, d, F).to(dev).to(BF)
+    ex.mx = mx
+    x, res = rnd(dev, T + 9, d), rnd(dev, T, d, seed=8)
+    rows = torch.randperm(T + 9, generator=torch.Generator().manual_seed(1))[:T].to(torch.int32).to(dev)
+    idx = torch.randint(0, E, (T, k), generator=torch.Generator().manual_seed(2)).to(dev)
+    if T > 1:
+        idx[1, 0] = -1
+        idx[0, :] = E - 1
+    for w in (torch.rand(T, k, device=dev), torch.rand(T, k, device=dev).to(BF)):
+        for kw in (dict(), dict(row_index=rows), dict(residual=res), dict(out_dtype=torch.float32),
+                   dict(coded=ops.quant_rows_mx(x[:T], ex.mx_act))):
+            xin = x if "row_index" in kw else x[:T]
+            one, d1 = ex.run(xin, idx, w, capacity=cap, **kw)
+            ops.set_stage_timing([])
+            try:
+                many, d2 = ex.run(xin, idx, w, capacity=cap, **kw)
+            finally:
+                ops.set_stage_timing(None)
+            assert torch.equal(one, many) and torch.equal(d1.counts, d2.counts)
+
+
 def test_empty_calls(dev):
     assert ops.quant_rows_mx(rnd(dev, 0, 64)).q.shape == (0, 128)
     assert ops.dequant_rows_mx(ops.quant_rows_mx(rnd(dev, 0, 64))).shape == (0, 64)
@@ -448,6 +480,11 @@ def test_empty_calls(dev):
     with torch.no_grad():
         y = ex(rnd(dev, 0, 64), torch.zeros(0, 2, dtype=torch.int64, device=dev), torch.zeros(0, 2, device=dev))
     assert y.shape == (0, 64)
+    r = rnd(dev, 0, 64)
+    layer = kmoe.GroupedExperts(2, 64, 64).to(dev).to(BF)
+    layer.mx = "w4a4"
+    got, info = layer.run(r, torch.zeros(0, 2, dtype=torch.int64, device=dev), torch.zeros(0, 2, device=dev), residual=r)
+    assert got.shape == (0, 64) and not info.counts.any()
 
 
 def test_refusals(dev):
@@ -477,6 +514,15 @@ def test_refusals(dev):
     ex.mx, ex.use_fp8 = "w4a8", True
     with pytest.raises(ValueError, match="not both"):
         ex(rnd(dev, 2, 64), torch.zeros(2, 1, dtype=torch.int64, device=dev), torch.ones(2, 1, device=dev))
+    i1, w1 = torch.zeros(2, 1, dtype=torch.int64, device=dev), torch.ones(2, 1, device=dev)
+    x64 = rnd(dev, 2, 64)
+    for bad in (dict(coded=ops.quant_rows_mx(x64, "e2m1")), dict(coded=ops.quant_rows_mx(rnd(dev, 3, 64))),
+                dict(residual=x64[:1]), dict(row_index=torch.zeros(3, dtype=torch.int32, device=dev)),
+                dict(block_counts=torch.zeros(3, dtype=torch.int32, device=dev))):
+        with pytest.raises(ValueError):
+            ops.mx_experts(x64, i1, w1, pw, "e4m3", **bad)
+    with pytest.raises(ValueError):
+        ops.mx_experts(rnd(dev, 3, 64), i1, w1, pw, "e4m3")
     with pytest.raises(ValueError, match="packed-weight files"):
         ex.use_fp8 = False
         kmoe.checkpoint.save_packed(ex, "unused.safetensors")

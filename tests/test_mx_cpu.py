@@ -25,7 +25,7 @@ def rc(lib, name, *args):
 def test_sizes(lib):
     assert lib.kmoe_mx_row_bytes(2048, E4) == 2048 and lib.kmoe_mx_row_bytes(192, E2) == 128
     assert lib.kmoe_mx_row_bytes(64, 0) == 0 and lib.kmoe_mx_row_bytes(0, E4) == 0
-    assert lib.kmoe_mx_scale_bytes(2048) == 64 and lib.kmoe_mx_scale_bytes(96) == 4
+    assert lib.kmoe_mx_scale_bytes(2048) == 64 and lib.kmoe_mx_scale_bytes(96) == 16
     # half a byte a weight, one scale byte for 32
     assert lib.kmoe_packed_mx_bytes(16, 2048, 2816, 0) == 16 * 2 * 2816 * 2048 // 2
     assert lib.kmoe_packed_mx_bytes(16, 2048, 2816, 1) == 16 * 2 * 2816 * 2048 // 32
