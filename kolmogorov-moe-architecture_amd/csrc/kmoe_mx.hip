@@ -89,76 +89,123 @@ __global__ __launch_bounds__(256) void dequant_rows_kernel(const uint8_t* __rest
   }
 }
 
-template <bool F32>
-__device__ __forceinline__ float load1(const void* __restrict__ p, int64_t i) {
-  return F32 ? static_cast<const float*>(p)[i] : bf16_to_f32(static_cast<const uint16_t*>(p)[i]);
+// The 32 values of K from k0 on of C columns n .. of w (K, N) (C a divisor of N with aligned
+// rows, or 1), zeros past K and N: v[j][c].
+template <bool F32, int C>
+struct WBlock {
+  float v[BLOCK][C];
+};
+template <bool F32, int C>
+__device__ __forceinline__ void load_block(const void* __restrict__ w, int64_t base, int k0, int K, int N, bool on,
+                                           WBlock<F32, C>& o) {
+#pragma unroll
+  for (int j = 0; j < BLOCK; ++j) {
+    const bool in = on && k0 + j < K;
+    const int64_t i = base + (int64_t)j * N;
+    if constexpr (C == 1) {
+      o.v[j][0] = !in ? 0.0f : F32 ? static_cast<const float*>(w)[i] : bf16_to_f32(static_cast<const uint16_t*>(w)[i]);
+    } else if constexpr (F32) {
+      const f32x4_t z = {0.0f, 0.0f, 0.0f, 0.0f};
+      const f32x4_t a = in ? *reinterpret_cast<const f32x4_t*>(static_cast<const float*>(w) + i) : z;
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o.v[j][c] = a[c];
+    } else {
+      const i32x2_t a = in ? *reinterpret_cast<const i32x2_t*>(static_cast<const uint16_t*>(w) + i) : i32x2_t{0, 0};
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        o.v[j][2 * c] = __uint_as_float((uint32_t)a[c] << 16);
+        o.v[j][2 * c + 1] = __uint_as_float((uint32_t)a[c] & 0xffff0000u);
+      }
+    }
+  }
+}
+template <bool F32, int C>
+__device__ __forceinline__ uint32_t column_code(const WBlock<F32, C>& o, int c) {
+  uint32_t m = 0;
+#pragma unroll
+  for (int j = 0; j < BLOCK; ++j) m = amax_bits(m, o.v[j][c]);
+  return scale_code<true>(m);
 }
 
-// w (E, K, N) to the values its e2m1 blocks along K stand for, bf16: one thread per column of
-// a block.
-template <bool F32>
+// w (E, K, N) to the values its e2m1 blocks along K stand for, bf16.  A thread takes C columns
+// of a block: with four (8 bytes of a bf16 row a lane) E 16, K 2048, N 2816 take XX us, with
+// one 174.
+template <bool F32, int C>
 __global__ __launch_bounds__(256) void fake_quant_kernel(const void* __restrict__ w, int E, int K, int N,
                                                          uint16_t* __restrict__ out) {
-  const int nb = (K + BLOCK - 1) / BLOCK;
-  const int64_t total = (int64_t)E * nb * N;
+  const int nb = (K + BLOCK - 1) / BLOCK, per = N / C;
+  const int64_t total = (int64_t)E * nb * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t eb = i / N;
-    const int n = (int)(i - eb * N);
+    const int64_t eb = i / per;
+    const int n = (int)(i - eb * per) * C;
     const int64_t e = eb / nb;
     const int k0 = (int)(eb - e * nb) * BLOCK;
     const int64_t base = (e * K + k0) * N + n;
-    float v[BLOCK];
-    uint32_t m = 0;
+    WBlock<F32, C> o;
+    load_block<F32, C>(w, base, k0, K, N, true, o);
 #pragma unroll
-    for (int j = 0; j < BLOCK; ++j) {
-      v[j] = k0 + j < K ? load1<F32>(w, base + (int64_t)j * N) : 0.0f;
-      m = amax_bits(m, v[j]);
+    for (int c = 0; c < C; ++c) {
+      const uint32_t code = column_code<F32, C>(o, c);
+      const float inv = inv_scale(code), s = scale_value(code);
+#pragma unroll
+      for (int j = 0; j < BLOCK; j += 2) {
+        const f32x2_t q = e2m1x2_values<0>(e2m1x2<0>(0u, o.v[j][c] * inv, o.v[j + 1][c] * inv));
+        o.v[j][c] = code == 255u ? s : q[0] * s;
+        o.v[j + 1][c] = code == 255u ? s : q[1] * s;
+      }
     }
-    const uint32_t code = scale_code<true>(m);
-    const float inv = inv_scale(code), s = scale_value(code);
 #pragma unroll
-    for (int j = 0; j < BLOCK; j += 2) {
-      const f32x2_t q = e2m1x2_values<0>(e2m1x2<0>(0u, v[j] * inv, v[j + 1] * inv));
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        if (k0 + j + u < K) out[base + (int64_t)(j + u) * N] = f32_to_bf16(code == 255u ? s : q[u] * s);
-    }
+    for (int j = 0; j < BLOCK; ++j)
+      if (k0 + j < K) {
+        if constexpr (C == 1) {
+          out[base + (int64_t)j * N] = f32_to_bf16(o.v[j][0]);
+        } else {
+          // exact, so the upper halves of the floats are the bf16 values (a NaN's too)
+          auto hi = [&](int c) { return __float_as_uint(o.v[j][c]); };
+          *reinterpret_cast<i32x2_t*>(out + base + (int64_t)j * N) =
+              i32x2_t{(int)(hi(0) >> 16 | (hi(1) & 0xffff0000u)), (int)(hi(2) >> 16 | (hi(3) & 0xffff0000u))};
+        }
+      }
   }
 }
 
 // One matrix w (E, K, N) into a packed weight: output column n of an expert goes to row
 // `row(n)` of its tiles.  gate_up: tile n / 128, 32-row block 2 ((n % 128) / 32) + half; else
-// tile n / 256, block (n % 256) / 32.  A thread quantises one column's 32 values of K (16
-// bytes of one lane of an MFMA block); N and K run over the padded sizes (zeros).
-template <bool F32>
+// tile n / 256, block (n % 256) / 32.  A thread quantises the 32 values of K of C columns
+// (16 bytes of C neighbouring lanes of an MFMA block); N and K run over the padded sizes.
+template <bool F32, int C>
 __global__ __launch_bounds__(256) void pack_mx_kernel(const void* __restrict__ w, int E, int K, int N, int Np, bool gate_up,
                                                       int half, int tiles, uint8_t* __restrict__ q,
                                                       uint8_t* __restrict__ scale) {
-  const int Kp = round_up(K, STEP), nb = Kp / BLOCK;
-  const int64_t total = (int64_t)E * nb * Np;
+  const int Kp = round_up(K, STEP), nb = Kp / BLOCK, per = Np / C;
+  const int64_t total = (int64_t)E * nb * per;
   for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < total; i += (int64_t)gridDim.x * 256) {
-    const int64_t eb = i / Np;
-    const int n = (int)(i - eb * Np);
+    const int64_t eb = i / per;
+    const int n0 = (int)(i - eb * per) * C;
     const int64_t e = eb / nb;
     const int b = (int)(eb - e * nb), k0 = b * BLOCK;
-    float v[BLOCK];
-    uint32_t m = 0;
-#pragma unroll
-    for (int j = 0; j < BLOCK; ++j) {
-      v[j] = n < N && k0 + j < K ? load1<F32>(w, (e * K + k0 + j) * N + n) : 0.0f;
-      m = amax_bits(m, v[j]);
-    }
-    const uint32_t code = scale_code<true>(m);
-    const Codes<true, BLOCK> o = encode<true, BLOCK>(v, code);
-    const int tile = gate_up ? n / 128 : n / 256;
-    const int blk = gate_up ? 2 * ((n & 127) / 32) + half : (n & 255) / 32;
-    const int step = b / 4, sub = (b >> 1) & 1, lane = (b & 1) * 32 + (n & 31);
+    WBlock<F32, C> o;
+    load_block<F32, C>(w, (e * K + k0) * N + n0, k0, K, N, n0 < N, o);
+    const int tile = gate_up ? n0 / 128 : n0 / 256;
+    const int blk = gate_up ? 2 * ((n0 & 127) / 32) + half : (n0 & 255) / 32;
+    const int step = b / 4, sub = (b >> 1) & 1, lane = (b & 1) * 32 + (n0 & 31);
     const int64_t ts = (e * tiles + tile) * (Kp / STEP) + step;
-    *reinterpret_cast<i32x4_t*>(q + ts * TILE_STEP + blk * 2048 + sub * 1024 + lane * 16) =
-        i32x4_t{(int)o.w[0], (int)o.w[1], (int)o.w[2], (int)o.w[3]};
-    scale[ts * SCALE_STEP + blk * 128 + lane * 2 + sub] = (uint8_t)code;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      const uint32_t code = column_code<F32, C>(o, c);
+      float v[BLOCK];
+#pragma unroll
+      for (int j = 0; j < BLOCK; ++j) v[j] = o.v[j][c];
+      const Codes<true, BLOCK> d = encode<true, BLOCK>(v, code);
+      *reinterpret_cast<i32x4_t*>(q + ts * TILE_STEP + blk * 2048 + sub * 1024 + (lane + c) * 16) =
+          i32x4_t{(int)d.w[0], (int)d.w[1], (int)d.w[2], (int)d.w[3]};
+      scale[ts * SCALE_STEP + blk * 128 + (lane + c) * 2 + sub] = (uint8_t)code;
+    }
   }
 }
+
+// Whether four columns at a time can be loaded: rows of whole, aligned quadruples.
+bool four_columns(const void* p, bool f32, int N) { return N % 4 == 0 && reinterpret_cast<uintptr_t>(p) % (f32 ? 16 : 8) == 0; }
 
 bool is_float(int dt) { return dt == KMOE_DTYPE_BF16 || dt == KMOE_DTYPE_F32; }
 bool is_mx(int dt) { return dt == KMOE_DTYPE_FP8_E4M3 || dt == KMOE_DTYPE_FP4_E2M1; }
@@ -211,12 +258,19 @@ extern "C" int kmoe_fake_quant_mx_cols(const void* w, int w_dtype, int E, int K,
   KMOE_REQUIRE(w && out, KMOE_ERR_NULL, "kmoe_fake_quant_mx_cols: null buffer");
   KMOE_REQUIRE(is_float(w_dtype), KMOE_ERR_DTYPE, "kmoe_fake_quant_mx_cols: dtype %d", w_dtype);
   KMOE_REQUIRE(E > 0 && K > 0 && N > 0, KMOE_ERR_SHAPE, "kmoe_fake_quant_mx_cols: E=%d K=%d N=%d", E, K, N);
-  const unsigned grid = grid_of((int64_t)E * kmoe::ceil_div(K, BLOCK) * N, 256);
   hipStream_t s = kmoe::as_stream(stream);
-  if (w_dtype == KMOE_DTYPE_F32)
-    hipLaunchKernelGGL(fake_quant_kernel<true>, dim3(grid), dim3(256), 0, s, w, E, K, N, static_cast<uint16_t*>(out));
+  const bool f32 = w_dtype == KMOE_DTYPE_F32;
+  const int C = four_columns(w, f32, N) && reinterpret_cast<uintptr_t>(out) % 8 == 0 ? 4 : 1;
+  const dim3 grid(grid_of((int64_t)E * kmoe::ceil_div(K, BLOCK) * (N / C), 256));
+  uint16_t* op = static_cast<uint16_t*>(out);
+  if (f32 && C == 4)
+    hipLaunchKernelGGL((fake_quant_kernel<true, 4>), grid, dim3(256), 0, s, w, E, K, N, op);
+  else if (f32)
+    hipLaunchKernelGGL((fake_quant_kernel<true, 1>), grid, dim3(256), 0, s, w, E, K, N, op);
+  else if (C == 4)
+    hipLaunchKernelGGL((fake_quant_kernel<false, 4>), grid, dim3(256), 0, s, w, E, K, N, op);
   else
-    hipLaunchKernelGGL(fake_quant_kernel<false>, dim3(grid), dim3(256), 0, s, w, E, K, N, static_cast<uint16_t*>(out));
+    hipLaunchKernelGGL((fake_quant_kernel<false, 1>), grid, dim3(256), 0, s, w, E, K, N, op);
   return kmoe::check_launch("kmoe_fake_quant_mx_cols");
 }
 
@@ -249,12 +303,18 @@ extern "C" int kmoe_pack_weights_mx(const void* w1, const void* w2, const void* 
   hipStream_t s = kmoe::as_stream(stream);
   const int Fp = round_up(F, 128), dp = round_up(d, 256);
   auto one = [&](const void* w, int K, int N, int Np, bool gate_up, int half, int tiles, void* q, uint8_t* sc) {
-    const unsigned grid = grid_of((int64_t)E * (round_up(K, STEP) / BLOCK) * Np, 256);
+    const bool f32 = w_dtype == KMOE_DTYPE_F32;
+    const int C = four_columns(w, f32, N) ? 4 : 1;
+    const dim3 grid(grid_of((int64_t)E * (round_up(K, STEP) / BLOCK) * (Np / C), 256));
     uint8_t* qp = static_cast<uint8_t*>(q);
-    if (w_dtype == KMOE_DTYPE_F32)
-      hipLaunchKernelGGL(pack_mx_kernel<true>, dim3(grid), dim3(256), 0, s, w, E, K, N, Np, gate_up, half, tiles, qp, sc);
+    if (f32 && C == 4)
+      hipLaunchKernelGGL((pack_mx_kernel<true, 4>), grid, dim3(256), 0, s, w, E, K, N, Np, gate_up, half, tiles, qp, sc);
+    else if (f32)
+      hipLaunchKernelGGL((pack_mx_kernel<true, 1>), grid, dim3(256), 0, s, w, E, K, N, Np, gate_up, half, tiles, qp, sc);
+    else if (C == 4)
+      hipLaunchKernelGGL((pack_mx_kernel<false, 4>), grid, dim3(256), 0, s, w, E, K, N, Np, gate_up, half, tiles, qp, sc);
     else
-      hipLaunchKernelGGL(pack_mx_kernel<false>, dim3(grid), dim3(256), 0, s, w, E, K, N, Np, gate_up, half, tiles, qp, sc);
+      hipLaunchKernelGGL((pack_mx_kernel<false, 1>), grid, dim3(256), 0, s, w, E, K, N, Np, gate_up, half, tiles, qp, sc);
   };
   one(w1, d, F, Fp, true, 0, Fp / 128, w13_packed, w13_scale);
   one(w2, d, F, Fp, true, 1, Fp / 128, w13_packed, w13_scale);

@@ -8,13 +8,16 @@ using namespace kmoe_mx;
 
 namespace {
 
-constexpr int FEW = 1024;  // assignments that one workgroup dispatches
+constexpr int FEW = 1024;  // threads of the workgroup that dispatches
+constexpr int MAX_ROUNDS = 4;
+// Rounds of FEW assignments that one workgroup dispatches: an expert and round cost a ballot.
+int few_rounds(int E) { return 64 / E < 1 ? 1 : 64 / E > MAX_ROUNDS ? MAX_ROUNDS : 64 / E; }
 
-// Dispatch of at most FEW assignments (the tables of kmoe_dispatch, same order) by workgroup
+// Dispatch of at most R FEW assignments (the tables of kmoe_dispatch, same order) by workgroup
 // 0, the quantisation of the T rows x[row_index[t]] by the others: one launch in place of
-// three, whose latencies are the time at these sizes.  A thread holds one assignment; its
-// rank is counted by ballots in its wave and summed over the waves before it.
-template <bool FP4>
+// three, whose latencies are the time at these sizes.  A thread holds assignments tid, FEW +
+// tid, ..; a rank is counted by ballots in its wave and summed over the waves before it.
+template <bool FP4, int R>
 __global__ __launch_bounds__(FEW) void tables_kernel(const int64_t* __restrict__ idx, const void* __restrict__ wsrc,
                                                      bool w_f32, int T, int k, int E, int64_t capacity,
                                                      int32_t* __restrict__ counts, int32_t* __restrict__ offsets,
@@ -41,28 +44,42 @@ __global__ __launch_bounds__(FEW) void tables_kernel(const int64_t* __restrict__
     if ((c & 3) == 0) scale[t * scale_bytes(d) + c / 4] = (uint8_t)code;
     return;
   }
-  __shared__ int cnt[FEW / 64][KMOE_MAX_EXPERTS];
+  constexpr int NW = R * FEW / 64;  // waves' worth of assignments
+  __shared__ int cnt[NW][KMOE_MAX_EXPERTS];
   __shared__ int off[KMOE_MAX_EXPERTS];
   const int lane = tid & 63, wave = tid >> 6, A = T * k;
-  int e = -1;
-  float w = 0.0f;
-  if (tid < A) {
-    const int64_t v = idx[tid];
-    e = v >= 0 && v < E ? (int)v : -1;  // ids out of range are dropped
-    w = w_f32 ? static_cast<const float*>(wsrc)[tid] : bf16_to_f32(static_cast<const uint16_t*>(wsrc)[tid]);
+  int e[R], rank[R];
+  float w[R];
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int a = r * FEW + tid;
+    e[r] = -1;
+    rank[r] = 0;
+    w[r] = 0.0f;
+    if (a < A) {
+      const int64_t v = idx[a];
+      e[r] = v >= 0 && v < E ? (int)v : -1;  // ids out of range are dropped
+      w[r] = w_f32 ? static_cast<const float*>(wsrc)[a] : bf16_to_f32(static_cast<const uint16_t*>(wsrc)[a]);
+    }
   }
   const uint64_t before = lane == 0 ? 0ull : ~0ull >> (64 - lane);
-  int rank = 0;
-  for (int ee = 0; ee < E; ++ee) {
-    const uint64_t m = __ballot(e == ee);
-    if (e == ee) rank = __popcll(m & before);
-    if (lane == 0) cnt[wave][ee] = __popcll(m);
-  }
+  for (int ee = 0; ee < E; ++ee)
+#pragma unroll
+    for (int r = 0; r < R; ++r) {
+      const uint64_t m = __ballot(e[r] == ee);
+      if (e[r] == ee) rank[r] = __popcll(m & before);
+      if (lane == 0) cnt[r * (FEW / 64) + wave][ee] = __popcll(m);
+    }
   __syncthreads();
   if (wave == 0) {
+    // lane: an expert; cnt becomes the count of the waves before
     int c = 0;
     if (lane < E)
-      for (int v = 0; v < FEW / 64; ++v) c += cnt[v][lane];
+      for (int v = 0; v < NW; ++v) {
+        const int n = cnt[v][lane];
+        cnt[v][lane] = c;
+        c += n;
+      }
     const int kept = capacity > 0 && c > capacity ? (int)capacity : c;
     int incl = kept;
 #pragma unroll
@@ -78,17 +95,21 @@ __global__ __launch_bounds__(FEW) void tables_kernel(const int64_t* __restrict__
     if (lane == E - 1) offsets[E] = incl;
   }
   __syncthreads();
-  if (tid < A) {
-    int row = -1;
-    if (e >= 0) {
-      for (int v = 0; v < wave; ++v) rank += cnt[v][e];
-      if (capacity <= 0 || rank < capacity) {
-        row = off[e] + rank;
-        row_token[row] = tid / k;
+#pragma unroll
+  for (int r = 0; r < R; ++r) {
+    const int a = r * FEW + tid;
+    if (a < A) {
+      int row = -1;
+      if (e[r] >= 0) {
+        const int at = rank[r] + cnt[r * (FEW / 64) + wave][e[r]];
+        if (capacity <= 0 || at < capacity) {
+          row = off[e[r]] + at;
+          row_token[row] = a / k;
+        }
       }
+      slot_row[a] = row;
+      slot_w[a] = w[r];
     }
-    slot_row[tid] = row;
-    slot_w[tid] = w;
   }
 }
 
@@ -157,19 +178,25 @@ extern "C" int kmoe_mx_experts(const void* x, const int32_t* row_index, int64_t 
   const int64_t A = T * k;
   const bool quant = !xq;
   int rc;
-  if (A <= FEW && !aux_out) {
+  if (A <= (int64_t)FEW * few_rounds(E) && !aux_out) {
     const int64_t chunks = quant ? T * (round_up(d, STEP) / 8) : 0;
     const dim3 grid((unsigned)(1 + kmoe::ceil_div<int64_t>(chunks, FEW)));
     const uint16_t* xp = static_cast<const uint16_t*>(x);
     hipStream_t s = kmoe::as_stream(stream);
-    if (fp4)
-      hipLaunchKernelGGL(tables_kernel<true>, grid, dim3(FEW), 0, s, topk_idx, topk_w, w_dtype == KMOE_DTYPE_F32, (int)T, k, E,
-                         capacity, counts, i32(b.offsets), i32(b.row_token), i32(b.slot_row), slot_w, xp, row_index, d,
-                         ws + b.xq, ws + b.xs);
+    const int R = A <= FEW ? 1 : MAX_ROUNDS;
+#define KMOE_TABLES(FP4_, R_)                                                                                             \
+  hipLaunchKernelGGL((tables_kernel<FP4_, R_>), grid, dim3(FEW), 0, s, topk_idx, topk_w, w_dtype == KMOE_DTYPE_F32, (int)T, k, \
+                     E, capacity, counts, i32(b.offsets), i32(b.row_token), i32(b.slot_row), slot_w, xp, row_index, d,       \
+                     ws + b.xq, ws + b.xs)
+    if (fp4 && R == 1)
+      KMOE_TABLES(true, 1);
+    else if (fp4)
+      KMOE_TABLES(true, MAX_ROUNDS);
+    else if (R == 1)
+      KMOE_TABLES(false, 1);
     else
-      hipLaunchKernelGGL(tables_kernel<false>, grid, dim3(FEW), 0, s, topk_idx, topk_w, w_dtype == KMOE_DTYPE_F32, (int)T, k,
-                         E, capacity, counts, i32(b.offsets), i32(b.row_token), i32(b.slot_row), slot_w, xp, row_index, d,
-                         ws + b.xq, ws + b.xs);
+      KMOE_TABLES(false, MAX_ROUNDS);
+#undef KMOE_TABLES
     rc = kmoe::check_launch("kmoe_mx_experts");
     if (rc) return rc;
   } else {

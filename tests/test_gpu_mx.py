@@ -99,7 +99,7 @@ def test_quant_gathered_rows_and_row_count(dev, fmt):
 
 
 @pytest.mark.parametrize("dtype", [BF, torch.float32])
-@pytest.mark.parametrize("E,K,N", [(1, 1, 1), (2, 33, 5), (3, 64, 352), (2, 100, 131), (4, 256, 40)])
+@pytest.mark.parametrize("E,K,N", [(1, 1, 1), (2, 33, 5), (3, 64, 352), (2, 100, 131), (2, 100, 132), (4, 256, 40), (1, 31, 4)])
 def test_fake_quant_weights(dev, dtype, E, K, N):
     w = rnd(dev, E, K, N, seed=K, std=0.02, dtype=dtype)
     if K > 1:
@@ -446,10 +446,11 @@ def test_other_stream_and_graph(dev):
 
 
 @pytest.mark.parametrize("mx", ["w4a8", "w4a4"])
-@pytest.mark.parametrize("T,k,E,cap", [(1, 1, 1, 0), (1, 8, 16, 0), (48, 2, 16, 5), (341, 3, 64, 0), (342, 3, 5, 100), (700, 2, 8, 0)])
+@pytest.mark.parametrize("T,k,E,cap", [(1, 1, 1, 0), (1, 8, 16, 0), (48, 2, 16, 5), (341, 3, 64, 0), (342, 3, 5, 100), (700, 2, 8, 0), (2048, 2, 16, 200),
+                                       (2049, 2, 16, 0), (600, 2, 64, 0)])
 def test_one_call_is_the_calls_it_makes(dev, mx, T, k, E, cap):
-    """The native pass against its pieces, bit for bit: at most 1024 assignments go through the
-    one-workgroup dispatch.  Ids out of range and one expert twice included."""
+    """The native pass against its pieces, bit for bit: up to 4096 assignments (fewer over
+    many experts) go through the one-workgroup dispatch.  Ids out of range and one expert twice included."""
     d, F = 192, 100
     ex = kmoe.GroupedExperts(E, d, F).to(dev).to(BF)
     ex.mx = mx
