@@ -568,11 +568,17 @@ int kmoe_route_topk_bwd(const float* logits, const int64_t* topk_idx, const floa
  *   (delta NULL: h is x and not written)
  *   fmt fp8_e4m3 / fp4_e2m1: also q, scale = kmoe_quant_rows_mx of n (bf16: neither)
  * x, delta, weight bf16 or f32; d a multiple of 8 (32 with fmt), <= 8192.  n is that of
- * kmoe_rmsnorm on h bit for bit; its backward is kmoe_rmsnorm_bwd with dres the
- * gradient of h: dx is then the gradient of x and of delta.                        */
+ * kmoe_rmsnorm on h bit for bit.                                                   */
 int kmoe_add_rmsnorm(const void* x, int x_dtype, const void* delta, int delta_dtype, const void* weight, int w_dtype,
                      float eps, int64_t T, int d, void* h, void* n, float* rrms, int fmt, void* q, uint8_t* scale,
                      void* stream);
+
+/* Its backward, kmoe_rmsnorm_bwd with dh (nullable) the gradient of h: dx (h's type) is
+ * the gradient of x and of delta; dx_bf16 (nullable, f32 h only) its rounding, for the
+ * one of them that is bf16.  Workspace: kmoe_rmsnorm_bwd_workspace_bytes.          */
+int kmoe_add_rmsnorm_bwd(const void* dn, const void* h, int h_dtype, const void* weight, int w_dtype, const float* rrms,
+                         const void* dh, int64_t T, int d, void* dx, void* dx_bf16, void* dweight, int dw_dtype,
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* ------------------------------------------------------------------------ */
 /* Microscaled (OCP MX) experts: weights in e2m1, activations in e4m3 or e2m1 (`fmt`),

@@ -222,7 +222,7 @@ struct NormRow {
   float r;
 };
 
-// dx (dtype of x) and the per-segment partial sums of dg.  Workgroup = NORM_WAVES waves
+// dx (dtype of x; with dx16 also rounded to bf16) and the per-segment partial sums of dg.  Workgroup = NORM_WAVES waves
 // over the rows [seg * seg_rows, ...) of its segment, wave w taking every NORM_WAVES-th
 // row (its x, dn and dres loads issued together); the waves' dg sums are then added in
 // wave order through LDS and written as partial[seg][:] (reduced over segments afterwards
@@ -231,7 +231,7 @@ template <int NV, bool XF32>
 __global__ __launch_bounds__(64 * NORM_WAVES) void rmsnorm_bwd_kernel(
     const uint16_t* __restrict__ dn, const void* __restrict__ x, const void* __restrict__ g, bool g_f32,
     const float* __restrict__ rrms, const void* __restrict__ dres, int64_t T, int d, int64_t seg_rows,
-    void* __restrict__ dx, float* __restrict__ partial) {
+    void* __restrict__ dx, uint16_t* __restrict__ dx16, float* __restrict__ partial) {
   __shared__ float red[NORM_WAVES][512];
   const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
   const int nvec = d / 8;
@@ -296,6 +296,7 @@ __global__ __launch_bounds__(64 * NORM_WAVES) void rmsnorm_bwd_kernel(
           acc[i][q] = fmaf(dv[q] * xv[q], r, acc[i][q]);
         }
         store8<XF32>(dx, t * d + (int64_t)v * 8, o);
+        if (XF32 && dx16) store8<false>(dx16, t * d + (int64_t)v * 8, o);
       }
     }
   };
@@ -354,13 +355,13 @@ int launch_norm(const void* x, const void* g, bool g_f32, float eps, int64_t T, 
 
 template <bool XF32>
 int launch_norm_bwd(const uint16_t* dn, const void* x, const void* g, bool g_f32, const float* rrms, const void* dres,
-                    int64_t T, int d, int64_t seg_rows, void* dx, float* partial, hipStream_t s) {
+                    int64_t T, int d, int64_t seg_rows, void* dx, uint16_t* dx16, float* partial, hipStream_t s) {
   const dim3 grid((unsigned)kmoe::ceil_div<int64_t>(T, seg_rows)), block(64 * NORM_WAVES);
   const int nv = kmoe::ceil_div(d / 8, 64);
 #define KMOE_NORM_CASE(NVV)                                                                              \
   if (nv <= NVV) {                                                                                       \
     hipLaunchKernelGGL((rmsnorm_bwd_kernel<NVV, XF32>), grid, block, 0, s, dn, x, g, g_f32, rrms, dres, T, \
-                       d, seg_rows, dx, partial);                                                        \
+                       d, seg_rows, dx, dx16, partial);                                                  \
     return KMOE_OK;                                                                                      \
   }
   KMOE_NORM_CASE(1)
@@ -459,36 +460,54 @@ extern "C" size_t kmoe_rmsnorm_bwd_workspace_bytes(int64_t T, int d) {
   return (size_t)kmoe::ceil_div<int64_t>(T, norm_seg_rows(T)) * (size_t)d * sizeof(float);
 }
 
-extern "C" int kmoe_rmsnorm_bwd(const void* dn, const void* x, int x_dtype, const void* weight, int w_dtype,
-                                const float* rrms, const void* dres, int64_t T, int d, void* dx, void* dweight,
-                                int dw_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+static int norm_bwd(const char* who, const void* dn, const void* x, int x_dtype, const void* weight, int w_dtype,
+                    const float* rrms, const void* dres, int64_t T, int d, void* dx, void* dx16, void* dweight, int dw_dtype,
+                    void* workspace, size_t workspace_bytes, void* stream) {
   // with no rows only the weight gradient (zeros) is written
   KMOE_REQUIRE(weight && dweight && (T == 0 || (dn && x && rrms && dx)), KMOE_ERR_NULL,
-               "kmoe_rmsnorm_bwd: null buffer");
+               "%s: null buffer", who);
   KMOE_REQUIRE(is_float_dtype(x_dtype) && is_float_dtype(w_dtype) && is_float_dtype(dw_dtype), KMOE_ERR_DTYPE,
-               "kmoe_rmsnorm_bwd: dtypes %d/%d/%d", x_dtype, w_dtype, dw_dtype);
+               "%s: dtypes %d/%d/%d", who, x_dtype, w_dtype, dw_dtype);
   KMOE_REQUIRE(T >= 0 && d > 0 && d % 8 == 0, KMOE_ERR_SHAPE,
-               "kmoe_rmsnorm_bwd: d=%d must be a positive multiple of 8", d);
-  KMOE_REQUIRE(d <= 8192, KMOE_ERR_UNSUPPORTED, "kmoe_rmsnorm_bwd: d=%d > 8192", d);
+               "%s: d=%d must be a positive multiple of 8", who, d);
+  KMOE_REQUIRE(d <= 8192, KMOE_ERR_UNSUPPORTED, "%s: d=%d > 8192", who, d);
   hipStream_t s = kmoe::as_stream(stream);
   if (T == 0) {  // no rows: dg = 0 (a fill kernel, so the call stays capturable)
     hipLaunchKernelGGL(zero_words_kernel, dim3((unsigned)kmoe::ceil_div(d, 256)), dim3(256), 0, s,
                        static_cast<uint16_t*>(dweight), (int64_t)d * (dw_dtype == KMOE_DTYPE_F32 ? 2 : 1));
-    return kmoe::check_launch("kmoe_rmsnorm_bwd");
+    return kmoe::check_launch(who);
   }
   const size_t need = kmoe_rmsnorm_bwd_workspace_bytes(T, d);
   KMOE_REQUIRE(workspace && workspace_bytes >= need, KMOE_ERR_WORKSPACE,
-               "kmoe_rmsnorm_bwd: workspace %zu < %zu bytes", workspace_bytes, need);
+               "%s: workspace %zu < %zu bytes", who, workspace_bytes, need);
   const int64_t seg_rows = norm_seg_rows(T);
   const int64_t nseg = kmoe::ceil_div<int64_t>(T, seg_rows);
   float* partial = static_cast<float*>(workspace);
   const bool g_f32 = w_dtype == KMOE_DTYPE_F32;
   const uint16_t* dnp = static_cast<const uint16_t*>(dn);
   const int rc = x_dtype == KMOE_DTYPE_F32
-                     ? launch_norm_bwd<true>(dnp, x, weight, g_f32, rrms, dres, T, d, seg_rows, dx, partial, s)
-                     : launch_norm_bwd<false>(dnp, x, weight, g_f32, rrms, dres, T, d, seg_rows, dx, partial, s);
+                     ? launch_norm_bwd<true>(dnp, x, weight, g_f32, rrms, dres, T, d, seg_rows, dx,
+                                             static_cast<uint16_t*>(dx16), partial, s)
+                     : launch_norm_bwd<false>(dnp, x, weight, g_f32, rrms, dres, T, d, seg_rows, dx,
+                                             static_cast<uint16_t*>(dx16), partial, s);
   if (rc != KMOE_OK) return rc;
-  const int rc2 = kmoe::check_launch("kmoe_rmsnorm_bwd");
+  const int rc2 = kmoe::check_launch(who);
   if (rc2 != KMOE_OK) return rc2;
   return kmoe_reduce_f32(partial, nseg, d, dweight, dw_dtype, stream);
+}
+
+extern "C" int kmoe_rmsnorm_bwd(const void* dn, const void* x, int x_dtype, const void* weight, int w_dtype,
+                                const float* rrms, const void* dres, int64_t T, int d, void* dx, void* dweight,
+                                int dw_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  return norm_bwd("kmoe_rmsnorm_bwd", dn, x, x_dtype, weight, w_dtype, rrms, dres, T, d, dx, nullptr, dweight, dw_dtype,
+                  workspace, workspace_bytes, stream);
+}
+
+extern "C" int kmoe_add_rmsnorm_bwd(const void* dn, const void* h, int h_dtype, const void* weight, int w_dtype,
+                                    const float* rrms, const void* dh, int64_t T, int d, void* dx, void* dx_bf16,
+                                    void* dweight, int dw_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  KMOE_REQUIRE(!dx_bf16 || h_dtype == KMOE_DTYPE_F32, KMOE_ERR_DTYPE,
+               "kmoe_add_rmsnorm_bwd: dx_bf16 is the rounding of an f32 gradient");
+  return norm_bwd("kmoe_add_rmsnorm_bwd", dn, h, h_dtype, weight, w_dtype, rrms, dh, T, d, dx, dx_bf16, dweight, dw_dtype,
+                  workspace, workspace_bytes, stream);
 }

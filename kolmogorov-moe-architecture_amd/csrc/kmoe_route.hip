@@ -9,8 +9,11 @@
 //   ds_j = a / S (dw_j - sum_i dw_i s_i / S), S = sum_i s_i + 1e-20   (or a dw_j)
 //   sigmoid: dl_j = ds_j s_j (1 - s_j);  softmax: dl_e = s_e (ds_e - sum_j ds_j s_j)
 //
-// Two choices may be closer than 32-bit rounding: choices and group values are computed and
-// compared in 64 bits, so the experts picked are those of the definition.
+// Two choices may be closer than 32-bit rounding, and the experts picked are those of the
+// definition: a token is ranked in f32, and again in 64 bits where two neighbours of that
+// order (or the last kept and the first dropped group) are closer than the f32 error.
+#include <type_traits>
+
 #include "kmoe_common.h"
 
 namespace {
@@ -25,31 +28,59 @@ __device__ __forceinline__ int64_t key_of(double v) {
   return b < 0 ? (int64_t)(~(uint64_t)b ^ 0x8000000000000000ull) : b;
 }
 
-template <int L, class V>
-__device__ __forceinline__ V group_sum(V v) {
+// The value of the lane whose place in its group of 2 S lanes is mirrored (S 4, 8) or S lanes
+// away (S 1, 2, 16, 32), by lane moves instead of LDS permutes: in a reduction that has made
+// the groups of S lanes uniform both are the other group's.
+template <int S>
+__device__ __forceinline__ int across(int v) {
+  if constexpr (S == 1)
+    return __builtin_amdgcn_update_dpp(0, v, 0xB1, 0xF, 0xF, false);  // quad_perm 1 0 3 2
+  else if constexpr (S == 2)
+    return __builtin_amdgcn_update_dpp(0, v, 0x4E, 0xF, 0xF, false);  // quad_perm 2 3 0 1
+  else if constexpr (S == 4)
+    return __builtin_amdgcn_update_dpp(0, v, 0x141, 0xF, 0xF, false);  // row_half_mirror
+  else if constexpr (S == 8)
+    return __builtin_amdgcn_update_dpp(0, v, 0x140, 0xF, 0xF, false);  // row_mirror
+  else
+    return __shfl_xor(v, S, 64);
+}
+template <int L, class Op>
+__device__ __forceinline__ float group_reduce(float v, Op op) {
+  auto step = [&](auto s) { v = op(v, __int_as_float(across<decltype(s)::value>(__float_as_int(v)))); };
+  if constexpr (L >= 2) step(std::integral_constant<int, 1>{});
+  if constexpr (L >= 4) step(std::integral_constant<int, 2>{});
+  if constexpr (L >= 8) step(std::integral_constant<int, 4>{});
+  if constexpr (L >= 16) step(std::integral_constant<int, 8>{});
+  if constexpr (L >= 32) step(std::integral_constant<int, 16>{});
+  if constexpr (L >= 64) step(std::integral_constant<int, 32>{});
+  return v;
+}
+template <int L>
+__device__ __forceinline__ float group_sum(float v) {
+  return group_reduce<L>(v, [](float a, float b) { return a + b; });
+}
+template <int L>
+__device__ __forceinline__ double group_sum(double v) {
 #pragma unroll
   for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
   return v;
 }
-// maximum over the L lanes of a token, NaN if there is one
+// Maximum over the L lanes of a token, NaN if there is one.
 template <int L>
 __device__ __forceinline__ float group_max(float v) {
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) {
-    const float u = __shfl_xor(v, o, 64);
-    v = v != v ? v : (u != u || u > v ? u : v);
-  }
-  return v;
+  return group_reduce<L>(v, [](float a, float b) { return a != a ? a : (b != b || b > a ? b : a); });
+}
+// Maximum of numbers.
+template <int L>
+__device__ __forceinline__ float group_top(float v) {
+  return group_reduce<L>(v, [](float a, float b) { return fmaxf(a, b); });
 }
 
-// Score of lane e's logit (64 bits); every lane of the token's L takes part.
-template <int L>
-__device__ __forceinline__ double score(float l, bool on, bool sigmoid) {
-  if (sigmoid) return on ? 1.0 / (1.0 + exp(-(double)l)) : 0.0;
-  const float m = group_max<L>(on ? l : -INFINITY);
-  if (m == -INFINITY) return 0.0;
-  const double p = on ? exp((double)l - (double)m) : 0.0;
-  return p / group_sum<L>(p);
+// LDS written by this wave is read by this wave: no workgroup barrier.
+__device__ __forceinline__ void wave_lds_fence() {
+  __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
 struct RouteArgs {
@@ -60,97 +91,260 @@ struct RouteArgs {
   const float* bias;
   int groups, topk_groups, group_top;
   bool renorm;
-  double scale;
+  float scale;
   int64_t* idx;
   float* w;
   int32_t* block_counts;
   int hb;  // tokens of a workgroup: the histogram's block
 };
 
-// One workgroup per histogram block; L lanes (a power of two >= E) hold a token's experts.
-// Ranks are counted: an expert's place is the number of experts ahead of it, read from LDS
-// as broadcasts, so no step depends on the one before.
-template <int L>
-__global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
-  __shared__ int64_t key[1024];
-  __shared__ int64_t gkey[1024];
-  __shared__ double pick[1024 / L][MAX_K];
-  __shared__ int count[64];
-  const int tid = threadIdx.x, e = tid % L, slot = tid / L, per = blockDim.x / L;
-  const int64_t t_begin = (int64_t)blockIdx.x * a.hb;
-  if (tid < 64) count[tid] = 0;
-  const int gs = a.E / a.groups;
-  for (int p = 0; p < a.hb; p += per) {  // the same trip count for every thread
-    const int64_t t = t_begin + p + slot;
-    const bool live = p + slot < a.hb && t < a.T;
-    const bool on = live && e < a.E;
-    const float l = on ? a.logits[t * a.E + e] : -INFINITY;
-    const double s = score<L>(l, on, a.sigmoid);
-    const bool masked = !on || l == -INFINITY;
-    const double c = masked ? -INFINITY : s + (a.bias ? (double)a.bias[e] : 0.0);
-    int64_t kc = key_of(c);
-    const int64_t none = key_of(-INFINITY);
-    bool in = on;
-    if (a.groups > 1) {
-      __syncthreads();
-      key[tid] = __double_as_longlong(c);
-      __syncthreads();
-      if (e < a.groups) {
-        double b1 = -INFINITY, b2 = -INFINITY;
-        bool nan = false;
-        for (int j = 0; j < gs; ++j) {
-          const double v = __longlong_as_double(key[slot * L + e * gs + j]);
-          nan |= v != v;
-          if (v > b1) {
-            b2 = b1;
-            b1 = v;
-          } else if (v > b2) {
-            b2 = v;
-          }
-        }
-        if (a.group_top == 2 && b2 > -INFINITY) b1 += b2;
-        gkey[tid] = nan ? INT64_MAX : key_of(b1);
-      }
-      __syncthreads();
-      if (on) {
-        const int g = e / gs;
-        const int64_t mine = gkey[slot * L + g];
-        int rank = 0;
-        for (int j = 0; j < a.groups; ++j) {
-          const int64_t o = gkey[slot * L + j];
-          rank += o > mine || (o == mine && j < g);
-        }
-        in = rank < a.topk_groups;
-      }
+constexpr int LANES = 16;         // lanes of a token: its reductions are moves within a row of lanes
+
+// What a token keeps in LDS.
+struct RouteLds {
+  int64_t key[KMOE_MAX_EXPERTS];
+  int64_t gkey[KMOE_MAX_EXPERTS];
+  float pick[MAX_K];  // chosen scores
+};
+
+// Scores of a token's logits l (expert sub EPL + i of the lane), in type V; rel: bounds of their
+// relative errors in f32: exp 2 half steps (2^-24) and, for softmax, the rounding of l - max, |l
+// - max| half steps; the sum of the token's exponentials the same, at most 16 half steps where
+// it matters (smaller ones add less than their error), and its additions 2 + log2 16; the
+// quotient one: (|l - max| + 32) 2^-24.  Sigmoid: exp, sum, quotient, under 8 2^-24.
+template <int EPL, class V>
+__device__ __forceinline__ void scores_of(const float (&l)[EPL], bool sigmoid, V (&s)[EPL], float (&rel)[EPL]) {
+  if (sigmoid) {
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      s[i] = (V)1 / ((V)1 + exp(-(V)l[i]));  // 0 for -inf
+      rel[i] = 0x1p-21f;
     }
-    __syncthreads();
-    // experts of dropped groups rank behind masked ones
-    key[tid] = in ? kc : INT64_MIN;
-    if (!in) kc = INT64_MIN;
-    __syncthreads();
-    if (on && in) {
-      int rank = 0;
-      for (int j = 0; j < a.E; ++j) {
-        const int64_t o = key[slot * L + j];
-        rank += o > kc || (o == kc && j < e);
-      }
-      if (rank < a.k) {
-        pick[slot][rank] = kc == none ? 0.0 : s;
-        a.idx[t * a.k + rank] = e;
-        if (a.block_counts) atomicAdd(&count[e], 1);
-      }
+    return;
+  }
+  float m = l[0];
+#pragma unroll
+  for (int i = 1; i < EPL; ++i) m = m != m ? m : (l[i] != l[i] || l[i] > m ? l[i] : m);
+  m = group_max<LANES>(m);
+  V z = (V)0;
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    s[i] = m == -INFINITY ? (V)0 : exp((V)l[i] - (V)m);
+    rel[i] = (m - l[i] + 32.0f) * 0x1p-24f;
+    z += s[i];
+  }
+  z = group_sum<LANES>(z);
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) s[i] = m == -INFINITY ? (V)0 : s[i] / z;
+}
+
+// Groups kept by their values val[g] in LDS (equal values: lowest group first), as a mask;
+// low and high: the least value kept and the greatest dropped among the lane's groups.
+template <class V>
+__device__ __forceinline__ uint64_t keep_groups(const RouteArgs& a, const V* val, int sub, V& low, V& high) {
+  uint64_t kept = 0;
+  for (int g = sub; g < a.groups; g += LANES) {
+    const V v = val[g];
+    int rank = 0;
+    for (int j = 0; j < a.groups; ++j) {
+      const V o = val[j];
+      rank += o > v || (o == v && j < g);
     }
-    __syncthreads();
-    if (live && e < a.k) {
-      double w = pick[slot][e];
-      if (a.renorm) {
-        double sum = ROUTE_TINY;
-        for (int j = 0; j < a.k; ++j) sum += pick[slot][j];
-        w /= sum;
-      }
-      a.w[t * a.k + e] = (float)(a.scale * w);
+    if (rank < a.topk_groups) {
+      kept |= 1ull << g;
+      low = v < low ? v : low;
+    } else {
+      high = v > high ? v : high;
     }
   }
+#pragma unroll
+  for (int o = 1; o < LANES; o *= 2) kept |= __shfl_xor(kept, o, 64);
+  return kept;
+}
+__device__ __forceinline__ int64_t row_max(int64_t v) {
+  auto step = [&](auto s) {
+    constexpr int S = decltype(s)::value;
+    const uint64_t hi = (uint32_t)across<S>((int)(v >> 32)), lo = (uint32_t)across<S>((int)v);
+    const int64_t u = (int64_t)(hi << 32 | lo);
+    v = u > v ? u : v;
+  };
+  step(std::integral_constant<int, 1>{});
+  step(std::integral_constant<int, 2>{});
+  step(std::integral_constant<int, 4>{});
+  step(std::integral_constant<int, 8>{});
+  return v;
+}
+
+// A token's order in 64 bits.  rank: the place of each of the lane's experts (< k: chosen, its
+// score in pick), or MAX_K.
+template <int EPL>
+__device__ __forceinline__ void rank64(const RouteArgs& a, RouteLds& s, const float (&l)[EPL], const float (&b)[EPL], int sub,
+                                       int gs, int base, int (&rank)[EPL]) {
+  double sc[EPL];
+  float rel[EPL];
+  scores_of<EPL, double>(l, a.sigmoid, sc, rel);
+  int64_t kc[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const double c = l[i] == -INFINITY ? -INFINITY : sc[i] + (double)b[i];
+    kc[i] = sub * EPL + i < a.E ? key_of(c) : INT64_MIN;
+    s.key[sub * EPL + i] = __double_as_longlong(c);
+    rank[i] = MAX_K;
+  }
+  wave_lds_fence();
+  if (a.groups > 1) {
+    for (int g = sub; g < a.groups; g += LANES) {
+      double b1 = -INFINITY, b2 = -INFINITY;
+      bool nan = false;
+      for (int j = 0; j < gs; ++j) {
+        const double v = __longlong_as_double(s.key[g * gs + j]);
+        nan |= v != v;
+        if (v > b1) {
+          b2 = b1;
+          b1 = v;
+        } else if (v > b2) {
+          b2 = v;
+        }
+      }
+      if (a.group_top == 2 && b2 > -INFINITY) b1 += b2;
+      s.gkey[g] = nan ? INT64_MAX : key_of(b1);
+    }
+    wave_lds_fence();
+    int64_t low = INT64_MAX, high = INT64_MIN;
+    const uint64_t kept = keep_groups<int64_t>(a, s.gkey, sub, low, high);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (!((kept >> ((sub * EPL + i) / gs)) & 1)) kc[i] = INT64_MIN;  // behind masked experts
+  }
+  for (int r = 0; r < a.k; ++r) {
+    int64_t m = kc[0];
+#pragma unroll
+    for (int i = 1; i < EPL; ++i) m = kc[i] > m ? kc[i] : m;
+    const int64_t best = row_max(m);
+    const uint32_t at = (uint32_t)(__ballot(m == best) >> base) & 0xffffu;
+    if (sub == __builtin_ctz(at | 0x10000u)) {
+      bool done = false;
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (!done && kc[i] == best) {
+          done = true;
+          kc[i] = INT64_MIN;
+          rank[i] = r;
+          s.pick[r] = l[i] == -INFINITY ? 0.0f : (float)sc[i];
+        }
+    }
+  }
+  wave_lds_fence();
+}
+
+// One workgroup per histogram block, its waves independent of each other; 16 lanes hold a
+// token, EPL experts each.  The time is that of one token's chain of dependent steps, so a
+// wave works on four and a workgroup on 64 at once: 16384 tokens, 64 experts, 8 groups, top-8
+// XX us (64 lanes a token, four tokens a wave one after the other: 27).
+template <int EPL>
+__global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
+  __shared__ RouteLds lds[64];
+  __shared__ int count[64];
+  const int tid = threadIdx.x, sub = tid % LANES, slot = tid / LANES, base = tid & 63 & ~(LANES - 1);
+  if (tid < 64) count[tid] = 0;
+  __syncthreads();
+  RouteLds& s = lds[slot];
+  const int64_t t = (int64_t)blockIdx.x * a.hb + slot;  // blockDim.x = LANES hb
+  const bool live = t < a.T;
+  const int gs = a.E / a.groups;
+  float l[EPL], b[EPL], sc[EPL], x[EPL];
+#pragma unroll
+  for (int i = 0; i < EPL; ++i) {
+    const int e = sub * EPL + i;
+    const bool on = live && e < a.E;
+    l[i] = on ? a.logits[t * a.E + e] : -INFINITY;
+    b[i] = on && a.bias ? a.bias[e] : 0.0f;
+  }
+  if (!__any(live)) goto done;
+  {
+    float rel[EPL];  // more than the scores' relative errors
+    scores_of<EPL, float>(l, a.sigmoid, sc, rel);
+    bool sure = true;
+    float err = 0.0f;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) {
+      x[i] = l[i] == -INFINITY ? -INFINITY : sc[i] + b[i];
+      if (l[i] != -INFINITY) {
+        sure = sure && fabsf(x[i]) < INFINITY;  // NaN and infinities are left to the 64-bit order
+        err = fmaxf(err, sc[i] * rel[i] + fabsf(x[i]) * 0x1p-23f);
+      }
+    }
+    err = group_top<LANES>(err);  // more than the error of any choice of the token
+    if (a.groups > 1) {
+      // (the 64-bit order's keys are not in use yet)
+      float* const cv = reinterpret_cast<float*>(s.key);
+      float* const gv = reinterpret_cast<float*>(s.gkey);
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) cv[sub * EPL + i] = x[i];
+      wave_lds_fence();
+      for (int g = sub; g < a.groups; g += LANES) {
+        float v = -INFINITY, b2 = -INFINITY;
+        for (int j = 0; j < gs; ++j) {
+          const float u = cv[g * gs + j];
+          b2 = fmaxf(b2, fminf(v, u));
+          v = fmaxf(v, u);
+        }
+        if (a.group_top == 2 && b2 > -INFINITY) v += b2;
+        gv[g] = v;
+      }
+      wave_lds_fence();
+      float low = INFINITY, high = -INFINITY;
+      const uint64_t kept = keep_groups<float>(a, gv, sub, low, high);
+      low = -group_top<LANES>(-low);
+      high = group_top<LANES>(high);
+      // a group's value is the sum of up to two choices
+      sure = sure && (a.topk_groups == a.groups || low - high > 4.0f * err);
+#pragma unroll
+      for (int i = 0; i < EPL; ++i)
+        if (!((kept >> ((sub * EPL + i) / gs)) & 1)) x[i] = -INFINITY;
+      wave_lds_fence();
+    }
+    // k rounds of the largest choice, and one more for the gap behind the last
+    int rank[EPL];
+#pragma unroll
+    for (int i = 0; i < EPL; ++i) rank[i] = MAX_K;
+    float last = 0.0f;
+    const int rounds = a.k < a.E ? a.k + 1 : a.k;
+    for (int r = 0; r < rounds; ++r) {
+      float m = x[0];
+#pragma unroll
+      for (int i = 1; i < EPL; ++i) m = fmaxf(m, x[i]);
+      const float best = group_top<LANES>(m);
+      const uint32_t at = (uint32_t)(__ballot(m == best) >> base) & 0xffffu;
+      sure = sure && (r == 0 || last - best > 2.0f * err) && (r == a.k || best > -INFINITY);
+      last = best;
+      if (sub == __builtin_ctz(at | 0x10000u)) {
+        bool done = false;
+#pragma unroll
+        for (int i = 0; i < EPL; ++i)
+          if (!done && x[i] == best) {
+            done = true;
+            x[i] = -INFINITY;
+            if (r < a.k) {
+              rank[i] = r;
+              s.pick[r] = sc[i];
+            }
+          }
+      }
+    }
+    wave_lds_fence();
+    if (__any(live && !sure)) rank64<EPL>(a, s, l, b, sub, gs, base, rank);
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (live && rank[i] < a.k) {
+        a.idx[t * a.k + rank[i]] = sub * EPL + i;
+        if (a.block_counts) atomicAdd(&count[sub * EPL + i], 1);
+      }
+    const float p = sub < a.k ? s.pick[sub] : 0.0f;
+    const float sum = group_sum<LANES>(p) + (float)ROUTE_TINY;
+    if (live && sub < a.k) a.w[t * a.k + sub] = a.scale * (a.renorm ? p / sum : p);
+  }
+done:
   if (a.block_counts) {
     __syncthreads();
     if (tid < a.E) a.block_counts[(int64_t)blockIdx.x * a.E + tid] = count[tid];
@@ -228,16 +422,15 @@ extern "C" int kmoe_route_topk(const float* logits, int64_t T, int E, int k, int
   const int64_t blocks = kmoe::ceil_div<int64_t>(T, hb);
   KMOE_REQUIRE(blocks < 1 << 22, KMOE_ERR_SHAPE, "kmoe_route_topk: T=%lld is too large", (long long)T);
   const RouteArgs a{logits, T,    E,           k,      scores == KMOE_SCORES_SIGMOID, bias, groups, topk_groups, group_top,
-                    renorm != 0, (double)scale, topk_idx, topk_w, block_counts, hb};
+                    renorm != 0, scale, topk_idx, topk_w, block_counts, hb};
   hipStream_t s = kmoe::as_stream(stream);
-  const int L = lanes_of(E);
-  const int threads = hb * L < 1024 ? hb * L : 1024;
-  switch (L) {
-    case 8: hipLaunchKernelGGL(route_kernel<8>, dim3((unsigned)blocks), dim3(threads), 0, s, a); break;
-    case 16: hipLaunchKernelGGL(route_kernel<16>, dim3((unsigned)blocks), dim3(threads), 0, s, a); break;
-    case 32: hipLaunchKernelGGL(route_kernel<32>, dim3((unsigned)blocks), dim3(threads), 0, s, a); break;
-    default: hipLaunchKernelGGL(route_kernel<64>, dim3((unsigned)blocks), dim3(threads), 0, s, a);
-  }
+  const dim3 grid((unsigned)blocks), block(LANES * hb);  // 512 or 1024 threads
+  if (E <= LANES)
+    hipLaunchKernelGGL(route_kernel<1>, grid, block, 0, s, a);
+  else if (E <= 2 * LANES)
+    hipLaunchKernelGGL(route_kernel<2>, grid, block, 0, s, a);
+  else
+    hipLaunchKernelGGL(route_kernel<4>, grid, block, 0, s, a);
   return kmoe::check_launch("kmoe_route_topk");
 }
 

@@ -113,6 +113,7 @@ _SIGNATURES = {
     "kmoe_route_topk": (_i32, [_vp, _i64, _i32, _i32, _i32, _vp, _i32, _i32, _i32, _i32, _f32, _vp, _vp, _vp, _vp]),
     "kmoe_route_topk_bwd": (_i32, [_vp, _vp, _vp, _i64, _i32, _i32, _i32, _i32, _f32, _i32, _vp, _vp]),
     "kmoe_add_rmsnorm": (_i32, [_vp, _i32, _vp, _i32, _vp, _i32, _f32, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _vp, _vp]),
+    "kmoe_add_rmsnorm_bwd": (_i32, [_vp, _vp, _i32, _vp, _i32, _vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _sz, _vp]),
     "kmoe_mx_row_bytes": (_sz, [_i32, _i32]),
     "kmoe_mx_scale_bytes": (_sz, [_i32]),
     "kmoe_quant_rows_mx": (_i32, [_vp, _vp, _i64, _vp, _i32, _i32, _vp, _vp, _vp]),

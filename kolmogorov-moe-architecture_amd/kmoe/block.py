@@ -40,6 +40,7 @@ from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import backward as _bwd
 from . import ops
@@ -70,15 +71,23 @@ class _AddNormFn(torch.autograd.Function):
         r = ops.add_rmsnorm(x.detach().reshape(-1, d), delta.detach().reshape(-1, d), weight, eps)
         ctx.save_for_backward(r.h, r.rrms, weight)
         ctx.meta = (x.shape, x.dtype, delta.dtype)
+        ctx.set_materialize_grads(False)
         return r.h.view(x.shape), r.n.view(x.shape)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dh, dn):
         h, rrms, weight = ctx.saved_tensors
         shape, x_dtype, delta_dtype = ctx.meta
-        ds, dg = ops.rmsnorm_bwd(dn.reshape(h.shape), h, weight, rrms, dres=dh.reshape(h.shape))
-        ds = ds.view(shape)
-        return ds.to(x_dtype), ds.to(delta_dtype), dg, None
+        if dn is None:  # only h went on
+            return (None, None, None, None) if dh is None else (dh.to(x_dtype), dh.to(delta_dtype), None, None)
+        ds, ds16, dg = ops.add_rmsnorm_bwd(dn.reshape(h.shape), h, weight, rrms,
+                                           dh=None if dh is None else dh.reshape(h.shape),
+                                           bf16=torch.bfloat16 in (x_dtype, delta_dtype))
+
+        def grad(dtype):
+            return (ds16 if dtype == torch.bfloat16 and ds16 is not None else ds).view(shape).to(dtype)
+        return grad(x_dtype), grad(delta_dtype), dg, None
 
 
 def add_rms_norm(x: torch.Tensor, delta: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5):

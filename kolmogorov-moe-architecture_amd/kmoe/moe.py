@@ -28,6 +28,7 @@ from typing import Optional, Tuple
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import _lib
 from . import backward as _bwd
@@ -480,6 +481,7 @@ class _RouteFn(torch.autograd.Function):
         return r.w, r.idx
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dw, didx):
         logits, idx = ctx.saved_tensors
         s = ctx.spec

@@ -1043,3 +1043,30 @@ def add_rmsnorm(x2d, delta, weight, eps, quant=None) -> AddNormOut:
                   ptr(weight), _fdt(weight), float(eps), T, d, ptr(h), ptr(n), ptr(rrms), code, ptr(q), ptr(scale),
                   _stream(x2d))
     return AddNormOut(h, n, rrms, q, scale)
+
+
+def add_rmsnorm_bwd(dn, h, weight, rrms, dh=None, bf16=False, dw_dtype=None):
+    """Backward of add_rmsnorm from dn and dh (None: zero), the gradients of n and h (T, d):
+    (dx in h's type, dx rounded to bf16 or None, dweight).  dx is the gradient of x and of
+    delta; bf16 asks for the rounding of an f32 one, for the input that is bf16."""
+    _need_gpu(dn, h, weight, rrms, dh)
+    T, d = h.shape
+    if dn.shape != (T, d) or (dh is not None and dh.shape != (T, d)):
+        raise ValueError(f"kmoe.add_rmsnorm_bwd: h {(T, d)}, dn {tuple(dn.shape)}, dh "
+                         f"{None if dh is None else tuple(dh.shape)}")
+    dn, h = _contig(dn, _BF16), h.contiguous()
+    weight = weight.detach()
+    dw_dtype = weight.dtype if dw_dtype is None else dw_dtype
+    weight = _contig(weight, weight.dtype if weight.dtype in (torch.float32, _BF16) else torch.float32)
+    dh = _contig(dh, h.dtype)
+    dev = h.device
+    dx = torch.empty(T, d, device=dev, dtype=h.dtype)
+    dx16 = torch.empty(T, d, device=dev, dtype=_BF16) if bf16 and h.dtype == torch.float32 else None
+    dwt = torch.empty(d, device=dev, dtype=dw_dtype if dw_dtype in (torch.float32, _BF16) else torch.float32)
+    lib = _lib._LIB or _lib.load()
+    wsb = lib.kmoe_rmsnorm_bwd_workspace_bytes(T, d)
+    ws = torch.empty(max(wsb, 4), device=dev, dtype=torch.uint8)
+    with _device(dev), _Stage("bwd_rmsnorm"):
+        _lib.call("kmoe_add_rmsnorm_bwd", ptr(dn), ptr(h), _fdt(h), ptr(weight), _fdt(weight), ptr(rrms), ptr(dh), T, d,
+                  ptr(dx), ptr(dx16), ptr(dwt), _fdt(dwt), ptr(ws), wsb, _stream(h))
+    return dx, dx16, dwt.to(dw_dtype)

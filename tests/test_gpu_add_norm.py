@@ -77,6 +77,22 @@ def test_backward(dev, xd, dd, T, d):
     assert float((dg.double() - gw).norm() / gw.norm()) <= 2.0 ** -18
 
 
+def test_backward_of_one_output(dev):
+    """Only n, or only h, goes on: the other's gradient is nothing."""
+    x, delta = rnd(dev, 30, 128, dtype=F32).requires_grad_(True), rnd(dev, 30, 128, seed=1).requires_grad_(True)
+    w = torch.ones(128, device=dev).requires_grad_(True)
+    dn, dh = rnd(dev, 30, 128, seed=2), rnd(dev, 30, 128, seed=3, dtype=F32)
+    h, n = kmoe.add_rms_norm(x, delta, w, EPS)
+    a = torch.autograd.grad(n, (x, delta, w), dn, retain_graph=True)
+    b = torch.autograd.grad((h, n), (x, delta, w), (torch.zeros_like(h), dn), retain_graph=True)
+    assert all(torch.equal(u, v) for u, v in zip(a, b))
+    c = torch.autograd.grad(h, (x, delta), dh, retain_graph=True)
+    assert torch.equal(c[0], dh) and torch.equal(c[1], dh.to(BF))
+    with pytest.raises(RuntimeError):  # no second derivative
+        (g,) = torch.autograd.grad(n.float().square().sum(), x, create_graph=True)
+        g.sum().backward()
+
+
 def test_backward_against_differences(dev):
     T, d, h = 3, 64, 2.0 ** -6
     x, delta = rnd(dev, T, d, dtype=F32).requires_grad_(True), rnd(dev, T, d, seed=1, dtype=F32)
@@ -131,6 +147,9 @@ def test_refusals(dev):
         ops.add_rmsnorm(x, x, w, EPS, quant="int8")
     with pytest.raises(ValueError):
         kmoe.add_rms_norm(x, x[:1], w, EPS)
+    r = ops.add_rmsnorm(x, x, w, EPS)
+    with pytest.raises(ValueError):
+        ops.add_rmsnorm_bwd(x[:1], r.h, w, r.rrms)
     y = rnd(dev, 2, 40)
     with pytest.raises(kmoe.KmoeError, match="multiple of 32"):
         ops.add_rmsnorm(y, y, torch.ones(40, device=dev), EPS, quant="e4m3")

@@ -11,6 +11,11 @@ pytestmark = pytest.mark.gpu
 F32 = torch.float32
 HALF_F32 = torch.finfo(F32).eps / 2
 INF = float("inf")
+# weights: scores in f32 (the logit's difference to the largest, at most 16 here, is rounded:
+# 16 half steps of the exponential; exp, six sums of a pair and the quotient: 9 half steps more);
+# the sum they are divided by has the same error and those of four additions, the quotient
+# and the scale round once each
+W_ERR = (2 * 25 + 6) * HALF_F32
 
 
 def logits_of(dev, T, E, seed=0, std=1.5):
@@ -51,8 +56,7 @@ def test_forward(dev, c):
     cpu = {**kw, "bias": None if kw["bias"] is None else kw["bias"].cpu()}
     idx, w = M.route(lg.cpu(), k, kind=cpu.pop("scores"), **cpu)
     assert torch.equal(r.idx.cpu(), idx)
-    # rounded once from 64 bits (1e-13: the two 64-bit computations)
-    assert bool(((r.w.double().cpu() - w).abs() <= (HALF_F32 + 1e-13) * w.abs()).all())
+    assert bool(((r.w.double().cpu() - w).abs() <= W_ERR * w.abs()).all())
     hb = ops.router_block_tokens(T)
     want = torch.stack([torch.bincount(b.reshape(-1), minlength=E) for b in r.idx.cpu().split(hb)])
     assert torch.equal(r.block_counts.cpu().long(), want)
@@ -102,7 +106,7 @@ def test_masked_rows_infinities_and_nan(dev, scores, groups, keep):
     assert torch.equal(got, idx)
     wd = r.w.double().cpu()
     assert torch.equal(wd.isnan(), w.isnan())
-    assert bool(((wd - w).abs().nan_to_num() <= (HALF_F32 + 1e-13) * w.abs().nan_to_num() + 1e-45).all())
+    assert bool(((wd - w).abs().nan_to_num() <= W_ERR * w.abs().nan_to_num() + 1e-45).all())
     assert not wd[0].any()
     dl = ops.route_topk_bwd(lg.to(dev), r.idx, torch.ones(8, k, device=dev), scores=scores)
     assert bool(dl[:4].isfinite().all()) and not dl[0].any()
@@ -171,6 +175,27 @@ def test_strides_types_streams_and_graph(dev):
         torch.cuda.synchronize()
         assert torch.equal(r.idx, eager.idx) and torch.equal(r.w, eager.w)
         assert torch.equal(r.block_counts, eager.block_counts)
+
+
+def test_order_of_close_choices(dev):
+    """Rows whose neighbours differ by parts of an f32 step of the scores, among ordinary rows:
+    the order is that of 64 bits."""
+    T, E, k = 257, 24, 6
+    lg = logits_of("cpu", T, E, seed=5)
+    g = torch.Generator().manual_seed(6)
+    for t in range(0, T, 3):
+        i, j = torch.randperm(E, generator=g)[:2].tolist()
+        lg[t, i] = lg[t].max()
+        lg[t, j] = torch.nextafter(lg[t, i], torch.tensor(INF))
+    # a bias that equals the difference of two scores to f32: 64 bits tell them apart
+    bias = torch.zeros(E)
+    s = torch.sigmoid(lg.double())
+    bias[3] = (s[1, 4] - s[1, 3]).float()
+    for kind in ("softmax", "sigmoid"):
+        for kw in (dict(), dict(bias=bias), dict(groups=4, topk_groups=2), dict(groups=8, topk_groups=3, group_top=1, bias=bias)):
+            dkw = {n: v.to(dev) if isinstance(v, torch.Tensor) else v for n, v in kw.items()}
+            r = ops.route_topk(lg.to(dev), k, scores=kind, **dkw)
+            assert torch.equal(r.idx.cpu(), M.route(lg, k, kind=kind, **kw)[0])
 
 
 def test_large_and_empty(dev):

@@ -54,6 +54,8 @@ def test_add_norm_refusals(lib):
     assert call(x=NULL) == -1 and call(h=NULL) == -1
     assert call(xd=2) == -3 and call(fmt=1) == -3
     assert call(fmt=E4) == -1 and call(d=60) == -2 and call(fmt=E4, q=FAKE, d=40) == -2
+    assert rc(lib, "kmoe_add_rmsnorm_bwd", FAKE, FAKE, 0, FAKE, 0, FAKE, FAKE, 4, 64, FAKE, FAKE, FAKE, 0, FAKE, 1 << 20,
+              NULL)[0] == -3
     assert call(d=8200) == -6 and call(eps=-1.0) == -2 and call(eps=float("nan")) == -2
 
 
