@@ -324,17 +324,23 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   uint32_t cur = 0;  // byte offset of the step's stage
   // Step kt: its first half is in registers.  Its second half is read under the first half's
   // products; then every wave is done with the step's stage, so the barrier that publishes
-  // step kt + 1 also frees it for step kt + NST (LOAD), whose loads go out under the second
-  // half's products with the reads of step kt + 1.  WAIT: loads that may stay in flight at the
-  // barrier; -1: the last step.
-  auto step = [&](int kt, auto load_tag, auto wait_tag) {
-    constexpr bool LOAD = decltype(load_tag)::value;
+  // step kt + 1 also frees it for step kt + NST.  With three stages those loads are spread over
+  // the second half (LOAD2) and the next step's first (LOAD1), with two they all go out in the
+  // second.  WAIT: loads that may stay in flight at the barrier; -1: the last step.
+  constexpr bool SPREAD = NST == 3;
+  constexpr int NL2 = SPREAD ? T::NL / 2 : T::NL;
+  auto step = [&](int kt, auto load1_tag, auto load2_tag, auto wait_tag) {
+    constexpr bool LOAD1 = SPREAD && decltype(load1_tag)::value, LOAD2 = decltype(load2_tag)::value;
     constexpr int WAIT = decltype(wait_tag)::value;
     const uint32_t nxt = cur + T::STAGE == NST * T::STAGE ? 0 : cur + T::STAGE;
+    const uint32_t prv = cur == 0 ? (NST - 1) * T::STAGE : cur - T::STAGE;
     static_for<0, NM>([&](auto gt) {
       mma_one(gt, H0{});
       spread(gt, std::integral_constant<int, NR>{}, std::integral_constant<int, (NM * 3 + 3) / 4>{},
              [&](auto n) { read_one(n, H1{}, cur); });
+      if constexpr (LOAD1)
+        spread(gt, std::integral_constant<int, T::NL - NL2>{}, std::integral_constant<int, NM>{},
+               [&](auto n) { load_one(std::integral_constant<int, n + NL2>{}, kt - 1 + NST, prv); });
       __builtin_amdgcn_sched_barrier(0);
     });
 #pragma unroll
@@ -350,7 +356,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
         wait_vmcnt<(WAIT >= 0 ? WAIT : 0)>();
       barrier_nofence();
     }
-    if constexpr (LOAD) load_row_scales(kt + NST);
+    if constexpr (LOAD2) load_row_scales(kt + NST);
     __builtin_amdgcn_sched_barrier(0);
     static_for<0, NM>([&](auto gt) {
       mma_one(gt, H1{});
@@ -361,20 +367,27 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
           else
             read_scale(std::integral_constant<int, n - NR>{}, kt + 1, nxt);
         });
-      if constexpr (LOAD)
-        spread(gt, std::integral_constant<int, T::NL>{}, std::integral_constant<int, NM>{},
+      if constexpr (LOAD2)
+        spread(gt, std::integral_constant<int, NL2>{}, std::integral_constant<int, NM>{},
                [&](auto n) { load_one(n, kt + NST, cur); });
       __builtin_amdgcn_sched_barrier(0);
     });
     cur = nxt;
   };
+  using Yes = std::true_type;
+  using No = std::false_type;
+  using Late = std::integral_constant<int, (NST - 2) * T::NL>;
   int kt = 0;
+  if (nk > NST) {
+    step(kt++, No{}, Yes{}, Late{});
 #pragma unroll 1
-  for (; kt + NST < nk; ++kt) step(kt, std::true_type{}, std::integral_constant<int, (NST - 2) * T::NL>{});
-  if constexpr (NST == 3)
-    if (kt + 2 < nk) step(kt++, std::false_type{}, std::integral_constant<int, T::NL>{});
-  if (kt + 1 < nk) step(kt++, std::false_type{}, std::integral_constant<int, 0>{});
-  step(kt, std::false_type{}, std::integral_constant<int, -1>{});
+    for (; kt + NST < nk; ++kt) step(kt, Yes{}, Yes{}, Late{});
+    if constexpr (SPREAD) step(kt++, Yes{}, No{}, Late{});
+  } else if (NST == 3 && nk == 3) {
+    step(kt++, No{}, No{}, Late{});
+  }
+  if (kt + 1 < nk) step(kt++, No{}, No{}, std::integral_constant<int, 0>{});
+  step(kt, No{}, No{}, std::integral_constant<int, -1>{});
 
   // ---- epilogue: lane's row of block mi, columns 8 c + 4 lh + t of block j
 #pragma unroll
