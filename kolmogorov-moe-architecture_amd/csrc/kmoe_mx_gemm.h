@@ -12,7 +12,9 @@
 // lane's results are four consecutive output columns 8 c + 4 h .. of one row, c = 0 .. 3: a
 // 32-column MX block of h is the 16 results of a lane and of its partner half.
 //
-// A workgroup of 2 x 2 waves owns 64 MI rows x 64 NJ weight rows, a wave 32 MI x 32 NJ.
+// A workgroup of 2 x 2 waves owns 64 MI rows x 256 weight rows, a wave 32 MI x 128.  (256 rows
+// by 4 x 2 waves load a quarter less, but leave one workgroup a CU: 16384 rows, top-2 of 16
+// experts, d 2048, F 2816, gate/up 340 us in w4a8 against 330, 236 in w4a4 against 227.)
 // Both operands go global -> LDS directly, 128 of K per step, three stages; the K loop has
 // one barrier per step, placed where every wave has the step's last fragments in registers.
 #pragma once
@@ -24,6 +26,8 @@
 namespace kmoe_mx {
 
 constexpr int GEMM_THREADS = 256;
+constexpr int NJ = 4;          // 32-row weight blocks of a wave
+constexpr int SLOT_GROUP = 8;  // slots that share a column tile's weights in an XCD's L2
 
 struct MxGemmArgs {
   const uint8_t* a;        // activation rows
@@ -36,13 +40,13 @@ struct MxGemmArgs {
   const uint8_t* b;        // packed weights and scales
   const uint8_t* b_scale;
   int b_tiles;             // 256-row weight tiles of an expert
+  int n_ct;                // small-row kernel: column tiles of an expert
   uint8_t* q;              // gate_up: h's codes, scales, and (training) gate / up values
   uint8_t* q_scale;
   uint16_t* gu;
   uint16_t* c;             // down: output
   int64_t ldc;             // gate_up: padded columns of h; down: columns of c
   int n_valid;             // down: columns to store
-  int n_ct;                // column tiles of 64 NJ weight rows
 };
 
 __device__ __forceinline__ i32x4_t buffer_of(const void* base, int64_t bytes) {
@@ -152,21 +156,21 @@ __device__ __forceinline__ void store_block(const float (&v)[16], int half, bool
   if (on && half == 0) *scale = (uint8_t)code;
 }
 
-template <bool GATE_UP, bool FP4, int MI, int NJ, bool SAVE_GU>
+template <bool GATE_UP, bool FP4, int MI, bool SAVE_GU>
 struct MxTile {
   static constexpr int BM = 64 * MI;
-  static constexpr int NST = MI == 2 && !FP4 ? 2 : 3;  // LDS stages: two workgroups fit a CU at MI 2
-  static constexpr int AB = BM * (FP4 ? 64 : 128), BB = NJ * 4096, BS = NJ * 256;
+  static constexpr int NST = MI == 2 && !FP4 ? 2 : 3;  // LDS stages: two workgroups of 128 rows fit a CU
+  static constexpr int AB = BM * (FP4 ? 64 : 128), BB = TILE_STEP, BS = SCALE_STEP;
   static constexpr int STAGE = AB + BB + BS;
   static constexpr int AS = BM * 16;  // the rows' scales of four steps, two sets behind the stages
   static constexpr int LDS = NST * STAGE + 2 * AS;
-  static constexpr int NA = AB / 4096, NB = NJ, NL = NA + NB + 1;  // loads per wave and step, without those scales
+  static constexpr int NA = AB / 4096, NB = BB / 4096, NL = NA + NB + 1;  // loads per wave and step, without those scales
   static_assert(LDS <= 160 * 1024, "LDS");
 };
 
-template <bool GATE_UP, bool FP4, int MI, int NJ, bool SAVE_GU>
+template <bool GATE_UP, bool FP4, int MI, bool SAVE_GU>
 __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) {
-  using T = MxTile<GATE_UP, FP4, MI, NJ, SAVE_GU>;
+  using T = MxTile<GATE_UP, FP4, MI, SAVE_GU>;
   static_assert(!SAVE_GU || GATE_UP, "gate / up values are the first product's");
   constexpr int NST = T::NST;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS];
@@ -176,24 +180,21 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   const int wm = wave >> 1, wn = wave & 1;
 
   // tile: each XCD (workgroups go round over the 8) takes a contiguous range of the tiles, in
-  // which four slots share a column tile's weights in its L2
+  // which a group of slots shares a column tile's weights in its L2: the 64 workgroups of 32 CUs
+  // then read eight slots' rows and eight column tiles' weights.  16384 rows, top-2 of 16
+  // experts, d 2048, F 2816, w4a8, down: groups of 4 / 8 / 16 177 / 168 / 171 us; d 4096,
+  // gate/up: 600 / 603 / 615 us.
   const SlotScan st = scan_slots<T::BM>(g.offsets, g.E);
-  const int n_all = st.n_slots * g.n_ct;
+  const int n_all = st.n_slots * g.b_tiles;
   const int chunk = (n_all + 7) / 8, at = blockIdx.x >> 3;
   const int t = (blockIdx.x & 7) * chunk + at;
   if (at >= chunk || t >= n_all) return;
   int slot, ct;
   {
-    const int full = (st.n_slots >> 2) * 4 * g.n_ct;
-    if (t < full) {
-      const int grp = t / (4 * g.n_ct), r = t - grp * 4 * g.n_ct;
-      ct = r >> 2;
-      slot = grp * 4 + (r & 3);
-    } else {
-      const int rem = st.n_slots & 3, u = t - full;
-      ct = u / rem;
-      slot = (st.n_slots & ~3) + (u - ct * rem);
-    }
+    const int grp = t / (SLOT_GROUP * g.b_tiles), r = t - grp * SLOT_GROUP * g.b_tiles;
+    const int n = min(SLOT_GROUP, st.n_slots - grp * SLOT_GROUP);
+    ct = r / n;
+    slot = grp * SLOT_GROUP + (r - ct * n);
   }
   int e, m0, m_end;
   slot_rows<T::BM>(st, slot, e, m0, m_end);
@@ -204,10 +205,9 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   const bool gather = GATE_UP && g.row_token;
   const i32x4_t ar = gather ? buffer_of(g.a, g.a_rows * lda) : buffer_of(g.a + m0 * lda, rows * lda);
   const i32x4_t sr = gather ? buffer_of(g.a_scale, g.a_rows * lds_a) : buffer_of(g.a_scale + m0 * lds_a, rows * lds_a);
-  constexpr int SPLIT = 4 / NJ;  // column tiles of a weight tile
-  const int64_t bt = ((int64_t)e * g.b_tiles + ct / SPLIT) * g.k_steps;
-  const i32x4_t br = buffer_of(g.b + bt * TILE_STEP + (ct % SPLIT) * T::BB, (int64_t)g.k_steps * TILE_STEP - (ct % SPLIT) * T::BB);
-  const i32x4_t tr = buffer_of(g.b_scale + bt * SCALE_STEP + (ct % SPLIT) * T::BS, (int64_t)g.k_steps * SCALE_STEP - (ct % SPLIT) * T::BS);
+  const int64_t bt = ((int64_t)e * g.b_tiles + ct) * g.k_steps;
+  const i32x4_t br = buffer_of(g.b + bt * TILE_STEP, (int64_t)g.k_steps * TILE_STEP);
+  const i32x4_t tr = buffer_of(g.b_scale + bt * SCALE_STEP, (int64_t)g.k_steps * SCALE_STEP);
   constexpr uint32_t NONE = 0x80000000u;  // an offset past every window
   auto source_row = [&](int r) -> uint32_t {  // row of `a` (or of the slot) that tile row r is; NONE without one
     if (r >= rows) return NONE;
@@ -227,11 +227,11 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   }
   const uint32_t ssrc = wave < MI ? source_row(wave * 64 + lane) : NONE;
   const uint32_t soff = ssrc == NONE ? NONE : ssrc * (uint32_t)lds_a;
-  const uint32_t boff = wave * T::NB * 1024 + lane * 16, toff = (wave % NJ) * 256 + lane * 4;
+  const uint32_t boff = wave * T::NB * 1024 + lane * 16, toff = wave * 256 + lane * 4;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(KMOE_LDS uint8_t*)lds;
 
   // load `q` of step k into the stage at byte offset st: A rows, weights, their scales (two
-  // column blocks a load; with fewer loads than waves two waves write the same values)
+  // column blocks a load)
   auto load_one = [&](auto q_tag, int k, uint32_t st) {
     constexpr int q = decltype(q_tag)::value;
     const uint32_t base = lds0 + st;
@@ -241,7 +241,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
       buffer_to_lds16(br, boff + (q - T::NA) * 1024, k * TILE_STEP,
                       __builtin_amdgcn_readfirstlane(base + T::AB + (wave * T::NB + q - T::NA) * 1024));
     else
-      buffer_to_lds4(tr, toff, k * SCALE_STEP, __builtin_amdgcn_readfirstlane(base + T::AB + T::BB + (wave % NJ) * 256));
+      buffer_to_lds4(tr, toff, k * SCALE_STEP, __builtin_amdgcn_readfirstlane(base + T::AB + T::BB + wave * 256));
   };
   // The rows' scales come four steps at a time, 16 bytes a row (a dword a step was half of all
   // L2 requests): 64 rows a wave, by the first MI waves, in front of the loads of a step
@@ -418,16 +418,27 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
         }
       }
     } else {
+      // a wave's 32 x 128 values go through LDS, so that a store instruction writes four rows'
+      // 256 bytes and not 32 rows' 32 bytes
+      uint8_t* const out = lds + wave * 8192;
+      if (mi == 0) barrier_nofence();  // the last step's operands are in registers
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
-        for (int c = 0; c < 4; c += 2) {
+        for (int c = 0; c < 4; ++c) {
           const f32x16_t& a = acc[mi][j];
-          const i32x4_t v = merge_runs(pack4_bf16(a[4 * c], a[4 * c + 1], a[4 * c + 2], a[4 * c + 3]),
-                                       pack4_bf16(a[4 * c + 4], a[4 * c + 5], a[4 * c + 6], a[4 * c + 7]));
-          const int col = (ct * 2 * NJ + wn * NJ + j) * 32 + 8 * (c + lh);
-          if (on && col < g.n_valid) *reinterpret_cast<i32x4_t*>(g.c + row * g.ldc + col) = v;
+          *reinterpret_cast<i32x2_t*>(out + lr * 256 + (((4 * j + c) ^ (lr & 15)) << 4) + 8 * lh) =
+              pack4_bf16(a[4 * c], a[4 * c + 1], a[4 * c + 2], a[4 * c + 3]);
         }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+      const int col = (ct * 2 * NJ + wn * NJ) * 32 + 8 * (lane & 15);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        const int rr = 4 * q + (lane >> 4), ro = wm * 32 * MI + mi * 32 + rr;
+        const i32x4_t v = *reinterpret_cast<const i32x4_t*>(out + rr * 256 + (((lane & 15) ^ (rr & 15)) << 4));
+        if (ro < rows && col < g.n_valid) *reinterpret_cast<i32x4_t*>(g.c + (m0 + ro) * g.ldc + col) = v;
+      }
+      __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     }
   }
 }
@@ -439,16 +450,16 @@ struct MxLaunch {
   hipStream_t s;
 };
 constexpr int SMALL_ROWS = 32;  // rows of a slot of the small-row kernel
-template <bool GATE_UP, bool FP4, int MI, int NJ, bool SAVE_GU = false>
-void launch_mx_tile(MxLaunch l) {
-  using T = MxTile<GATE_UP, FP4, MI, NJ, SAVE_GU>;
-  l.g.n_ct = l.g.b_tiles * (4 / NJ);
+template <bool GATE_UP, bool FP4, int MI, bool SAVE_GU = false>
+void launch_mx_tile(const MxLaunch& l) {
+  using T = MxTile<GATE_UP, FP4, MI, SAVE_GU>;
   const int64_t slots = l.max_rows / T::BM + (l.max_rows < l.g.E ? l.max_rows : l.g.E);
-  const int64_t blocks = (slots * l.g.n_ct + 7) / 8 * 8;
-  hipLaunchKernelGGL((mx_gemm_kernel<GATE_UP, FP4, MI, NJ, SAVE_GU>), dim3((unsigned)blocks), dim3(GEMM_THREADS), 0, l.s, l.g);
+  const int64_t blocks = (slots * l.g.b_tiles + 7) / 8 * 8;
+  hipLaunchKernelGGL((mx_gemm_kernel<GATE_UP, FP4, MI, SAVE_GU>), dim3((unsigned)blocks), dim3(GEMM_THREADS), 0, l.s, l.g);
 }
-void launch_mx_gate_up(const MxLaunch& l, bool fp4, int mi);  // with l.g.gu: saving the gate / up values
-void launch_mx_down(const MxLaunch& l, bool fp4, int mi);
+// rows: of a tile, 64 or 128
+void launch_mx_gate_up(const MxLaunch& l, bool fp4, int rows);  // with l.g.gu: saving the gate / up values
+void launch_mx_down(const MxLaunch& l, bool fp4, int rows);
 void launch_mx_small(const MxLaunch& l, bool gate_up, bool fp4);
 
 }  // namespace kmoe_mx

@@ -8,10 +8,10 @@ using namespace kmoe_mx;
 
 namespace {
 
-// Rows of a tile / 64 for max_rows rows over E experts.
+// Rows of a tile for max_rows rows over E experts.
 int tile_rows(int64_t max_rows, int E) {
   const int64_t per = max_rows / E;
-  return per > 128 ? 2 : per > 64 ? 2 : 1;
+  return per > 64 ? 128 : 64;
 }
 
 // Whether a product runs on the small-row kernel (kmoe_mx_gemm_small.hip): where its grid is at

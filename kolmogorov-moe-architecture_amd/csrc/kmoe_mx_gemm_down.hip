@@ -3,13 +3,11 @@
 
 namespace kmoe_mx {
 template <bool FP4>
-static void by_rows(const MxLaunch& l, int mi) {
-  if (mi == 4)
-    launch_mx_tile<false, FP4, 4, 4>(l);
-  else if (mi == 2)
-    launch_mx_tile<false, FP4, 2, 4>(l);
+static void by_rows(const MxLaunch& l, int rows) {
+  if (rows == 128)
+    launch_mx_tile<false, FP4, 2>(l);
   else
-    launch_mx_tile<false, FP4, 1, 4>(l);
+    launch_mx_tile<false, FP4, 1>(l);
 }
-void launch_mx_down(const MxLaunch& l, bool fp4, int mi) { fp4 ? by_rows<true>(l, mi) : by_rows<false>(l, mi); }
+void launch_mx_down(const MxLaunch& l, bool fp4, int rows) { fp4 ? by_rows<true>(l, rows) : by_rows<false>(l, rows); }
 }  // namespace kmoe_mx
