@@ -12,11 +12,12 @@
 // lane's results are four consecutive output columns 8 c + 4 h .. of one row, c = 0 .. 3: a
 // 32-column MX block of h is the 16 results of a lane and of its partner half.
 //
-// A workgroup of 2 x 2 waves owns 64 MI rows x 256 weight rows, a wave 32 MI x 128.  (256 rows
-// by 4 x 2 waves load a quarter less, but leave one workgroup a CU: 16384 rows, top-2 of 16
-// experts, d 2048, F 2816, gate/up 340 us in w4a8 against 330, 236 in w4a4 against 227.)
-// Both operands go global -> LDS directly, 128 of K per step, three stages; the K loop has
-// one barrier per step, placed where every wave has the step's last fragments in registers.
+// A workgroup of 2 x 2 waves owns 64 MI rows x 64 NJ weight rows, a wave 32 MI x 32 NJ.  (256
+// rows by 4 x 2 waves load a quarter less, but leave one workgroup a CU: 16384 rows, top-2 of 16
+// experts, d 2048, F 2816, gate/up 340 us in w4a8 against 330, 236 in w4a4 against 227.)  Both
+// operands go global -> LDS directly, 128 of K per step, in as many stages up to three as let
+// two workgroups share a CU (with four and five of the small tiles nothing gained); the K loop
+// has one barrier per step, placed where every wave has the step's last fragments in registers.
 #pragma once
 
 #include <type_traits>
@@ -26,7 +27,6 @@
 namespace kmoe_mx {
 
 constexpr int GEMM_THREADS = 256;
-constexpr int NJ = 4;          // 32-row weight blocks of a wave
 constexpr int SLOT_GROUP = 8;  // slots that share a column tile's weights in an XCD's L2
 
 struct MxGemmArgs {
@@ -156,21 +156,22 @@ __device__ __forceinline__ void store_block(const float (&v)[16], int half, bool
   if (on && half == 0) *scale = (uint8_t)code;
 }
 
-template <bool GATE_UP, bool FP4, int MI, bool SAVE_GU>
+template <bool GATE_UP, bool FP4, int MI, int NJ, bool SAVE_GU>
 struct MxTile {
   static constexpr int BM = 64 * MI;
-  static constexpr int NST = MI == 2 && !FP4 ? 2 : 3;  // LDS stages: two workgroups of 128 rows fit a CU
-  static constexpr int AB = BM * (FP4 ? 64 : 128), BB = TILE_STEP, BS = SCALE_STEP;
+  static constexpr int AB = BM * (FP4 ? 64 : 128), BB = NJ * 4096, BS = NJ * 256;
   static constexpr int STAGE = AB + BB + BS;
   static constexpr int AS = BM * 16;  // the rows' scales of four steps, two sets behind the stages
+  static constexpr int FIT = (80 * 1024 - 2 * AS) / STAGE;  // LDS stages: two workgroups fit a CU
+  static constexpr int NST = FIT < 3 ? FIT : 3;
   static constexpr int LDS = NST * STAGE + 2 * AS;
-  static constexpr int NA = AB / 4096, NB = BB / 4096, NL = NA + NB + 1;  // loads per wave and step, without those scales
+  static constexpr int NA = AB / 4096, NB = NJ, NL = NA + NB + 1;  // loads per wave and step, without those scales
   static_assert(LDS <= 160 * 1024, "LDS");
 };
 
-template <bool GATE_UP, bool FP4, int MI, bool SAVE_GU>
+template <bool GATE_UP, bool FP4, int MI, int NJ, bool SAVE_GU>
 __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) {
-  using T = MxTile<GATE_UP, FP4, MI, SAVE_GU>;
+  using T = MxTile<GATE_UP, FP4, MI, NJ, SAVE_GU>;
   static_assert(!SAVE_GU || GATE_UP, "gate / up values are the first product's");
   constexpr int NST = T::NST;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS];
@@ -185,13 +186,15 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   // experts, d 2048, F 2816, w4a8, down: groups of 4 / 8 / 16 177 / 168 / 171 us; d 4096,
   // gate/up: 600 / 603 / 615 us.
   const SlotScan st = scan_slots<T::BM>(g.offsets, g.E);
-  const int n_all = st.n_slots * g.b_tiles;
+  constexpr int SPLIT = 4 / NJ;  // column tiles of a weight tile
+  const int n_ct = g.b_tiles * SPLIT;
+  const int n_all = st.n_slots * n_ct;
   const int chunk = (n_all + 7) / 8, at = blockIdx.x >> 3;
   const int t = (blockIdx.x & 7) * chunk + at;
   if (at >= chunk || t >= n_all) return;
   int slot, ct;
   {
-    const int grp = t / (SLOT_GROUP * g.b_tiles), r = t - grp * SLOT_GROUP * g.b_tiles;
+    const int grp = t / (SLOT_GROUP * n_ct), r = t - grp * SLOT_GROUP * n_ct;
     const int n = min(SLOT_GROUP, st.n_slots - grp * SLOT_GROUP);
     ct = r / n;
     slot = grp * SLOT_GROUP + (r - ct * n);
@@ -205,9 +208,9 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   const bool gather = GATE_UP && g.row_token;
   const i32x4_t ar = gather ? buffer_of(g.a, g.a_rows * lda) : buffer_of(g.a + m0 * lda, rows * lda);
   const i32x4_t sr = gather ? buffer_of(g.a_scale, g.a_rows * lds_a) : buffer_of(g.a_scale + m0 * lds_a, rows * lds_a);
-  const int64_t bt = ((int64_t)e * g.b_tiles + ct) * g.k_steps;
-  const i32x4_t br = buffer_of(g.b + bt * TILE_STEP, (int64_t)g.k_steps * TILE_STEP);
-  const i32x4_t tr = buffer_of(g.b_scale + bt * SCALE_STEP, (int64_t)g.k_steps * SCALE_STEP);
+  const int64_t bt = ((int64_t)e * g.b_tiles + ct / SPLIT) * g.k_steps;
+  const i32x4_t br = buffer_of(g.b + bt * TILE_STEP + (ct % SPLIT) * T::BB, (int64_t)g.k_steps * TILE_STEP - (ct % SPLIT) * T::BB);
+  const i32x4_t tr = buffer_of(g.b_scale + bt * SCALE_STEP + (ct % SPLIT) * T::BS, (int64_t)g.k_steps * SCALE_STEP - (ct % SPLIT) * T::BS);
   constexpr uint32_t NONE = 0x80000000u;  // an offset past every window
   auto source_row = [&](int r) -> uint32_t {  // row of `a` (or of the slot) that tile row r is; NONE without one
     if (r >= rows) return NONE;
@@ -227,7 +230,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   }
   const uint32_t ssrc = wave < MI ? source_row(wave * 64 + lane) : NONE;
   const uint32_t soff = ssrc == NONE ? NONE : ssrc * (uint32_t)lds_a;
-  const uint32_t boff = wave * T::NB * 1024 + lane * 16, toff = wave * 256 + lane * 4;
+  const uint32_t boff = wave * T::NB * 1024 + lane * 16, toff = (wave % NJ) * 256 + lane * 4;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(KMOE_LDS uint8_t*)lds;
 
   // load `q` of step k into the stage at byte offset st: A rows, weights, their scales (two
@@ -241,7 +244,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
       buffer_to_lds16(br, boff + (q - T::NA) * 1024, k * TILE_STEP,
                       __builtin_amdgcn_readfirstlane(base + T::AB + (wave * T::NB + q - T::NA) * 1024));
     else
-      buffer_to_lds4(tr, toff, k * SCALE_STEP, __builtin_amdgcn_readfirstlane(base + T::AB + T::BB + wave * 256));
+      buffer_to_lds4(tr, toff, k * SCALE_STEP, __builtin_amdgcn_readfirstlane(base + T::AB + T::BB + (wave % NJ) * 256));
   };
   // The rows' scales come four steps at a time, 16 bytes a row (a dword a step was half of all
   // L2 requests): 64 rows a wave, by the first MI waves, in front of the loads of a step
@@ -312,12 +315,10 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
       static_for<0, T::NL>([&](auto q) { load_one(q, s, s * T::STAGE); });
     }
   });
-  if (NST == 3 && nk >= 3)
-    wait_vmcnt<(NST - 1) * T::NL>();
-  else if (nk >= 2)
-    wait_vmcnt<T::NL>();
-  else
-    wait_vmcnt<0>();
+  static_for<0, NST>([&](auto i) {
+    constexpr int R = NST - i;  // the first of R steps has landed
+    if (R == NST ? nk >= R : nk == R) wait_vmcnt<(R - 1) * T::NL>();
+  });
   barrier_nofence();
   static_for<0, NR>([&](auto r) { read_one(r, H0{}, 0); });
   static_for<0, NS>([&](auto r) { read_scale(r, 0, 0); });
@@ -326,8 +327,8 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   // products; then every wave is done with the step's stage, so the barrier that publishes
   // step kt + 1 also frees it for step kt + NST.  With three stages those loads are spread over
   // the second half (LOAD2) and the next step's first (LOAD1), with two they all go out in the
-  // second.  WAIT: loads that may stay in flight at the barrier; -1: the last step.
-  constexpr bool SPREAD = NST == 3;
+  // second.  WAIT: steps whose loads may stay in flight at the barrier; -1: the last step.
+  constexpr bool SPREAD = NST >= 3;
   constexpr int NL2 = SPREAD ? T::NL / 2 : T::NL;
   auto step = [&](int kt, auto load1_tag, auto load2_tag, auto wait_tag) {
     constexpr bool LOAD1 = SPREAD && decltype(load1_tag)::value, LOAD2 = decltype(load2_tag)::value;
@@ -349,11 +350,12 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
     for (int mi = 0; mi < MI; ++mi) sa2[mi] = sa[mi];
     if constexpr (WAIT >= 0) {
       wait_lgkmcnt0();
-      // (one load more may stay in flight where step kt + 2 began with row scales)
-      if (WAIT > 0 && ((kt + 2) & 3) == 0 && wave < MI)
-        wait_vmcnt<(WAIT > 0 ? WAIT + 1 : 0)>();
+      // (with one load more where a step of those began with row scales)
+      constexpr int CNT = WAIT >= 0 ? WAIT : 0;
+      if (CNT > 0 && ((kt + 1 + CNT) & ~3) >= kt + 2 && wave < MI)
+        wait_vmcnt<CNT * T::NL + (CNT > 0)>();
       else
-        wait_vmcnt<(WAIT >= 0 ? WAIT : 0)>();
+        wait_vmcnt<CNT * T::NL>();
       barrier_nofence();
     }
     if constexpr (LOAD2) load_row_scales(kt + NST);
@@ -376,17 +378,18 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   };
   using Yes = std::true_type;
   using No = std::false_type;
-  using Late = std::integral_constant<int, (NST - 2) * T::NL>;
+  using Late = std::integral_constant<int, NST - 2>;
   int kt = 0;
   if (nk > NST) {
     step(kt++, No{}, Yes{}, Late{});
 #pragma unroll 1
     for (; kt + NST < nk; ++kt) step(kt, Yes{}, Yes{}, Late{});
     if constexpr (SPREAD) step(kt++, Yes{}, No{}, Late{});
-  } else if (NST == 3 && nk == 3) {
-    step(kt++, No{}, No{}, Late{});
   }
-  if (kt + 1 < nk) step(kt++, No{}, No{}, std::integral_constant<int, 0>{});
+  static_for<0, NST - 1>([&](auto i) {
+    constexpr int R = NST - i;  // steps left
+    if (nk - kt == R) step(kt++, No{}, No{}, std::integral_constant<int, R - 2>{});
+  });
   step(kt, No{}, No{}, std::integral_constant<int, -1>{});
 
   // ---- epilogue: lane's row of block mi, columns 8 c + 4 lh + t of block j
@@ -420,22 +423,23 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
     } else {
       // a wave's 32 x 128 values go through LDS, so that a store instruction writes four rows'
       // 256 bytes and not 32 rows' 32 bytes
-      uint8_t* const out = lds + wave * 8192;
+      constexpr int OC = NJ * 4;  // 16-byte chunks of a row
+      uint8_t* const out = lds + wave * 32 * OC * 16;
       if (mi == 0) barrier_nofence();  // the last step's operands are in registers
 #pragma unroll
       for (int j = 0; j < NJ; ++j)
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           const f32x16_t& a = acc[mi][j];
-          *reinterpret_cast<i32x2_t*>(out + lr * 256 + (((4 * j + c) ^ (lr & 15)) << 4) + 8 * lh) =
+          *reinterpret_cast<i32x2_t*>(out + ((lr * OC + ((4 * j + c) ^ (lr & (OC - 1)))) << 4) + 8 * lh) =
               pack4_bf16(a[4 * c], a[4 * c + 1], a[4 * c + 2], a[4 * c + 3]);
         }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-      const int col = (ct * 2 * NJ + wn * NJ) * 32 + 8 * (lane & 15);
+      const int oc = lane % OC, col = (ct * 2 * NJ + wn * NJ) * 32 + 8 * oc;
 #pragma unroll
-      for (int q = 0; q < 8; ++q) {
-        const int rr = 4 * q + (lane >> 4), ro = wm * 32 * MI + mi * 32 + rr;
-        const i32x4_t v = *reinterpret_cast<const i32x4_t*>(out + rr * 256 + (((lane & 15) ^ (rr & 15)) << 4));
+      for (int q = 0; q < OC / 2; ++q) {
+        const int rr = 64 / OC * q + lane / OC, ro = wm * 32 * MI + mi * 32 + rr;
+        const i32x4_t v = *reinterpret_cast<const i32x4_t*>(out + ((rr * OC + (oc ^ (rr & (OC - 1)))) << 4));
         if (ro < rows && col < g.n_valid) *reinterpret_cast<i32x4_t*>(g.c + (m0 + ro) * g.ldc + col) = v;
       }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -450,16 +454,16 @@ struct MxLaunch {
   hipStream_t s;
 };
 constexpr int SMALL_ROWS = 32;  // rows of a slot of the small-row kernel
-template <bool GATE_UP, bool FP4, int MI, bool SAVE_GU = false>
+template <bool GATE_UP, bool FP4, int MI, int NJ, bool SAVE_GU = false>
 void launch_mx_tile(const MxLaunch& l) {
-  using T = MxTile<GATE_UP, FP4, MI, SAVE_GU>;
+  using T = MxTile<GATE_UP, FP4, MI, NJ, SAVE_GU>;
   const int64_t slots = l.max_rows / T::BM + (l.max_rows < l.g.E ? l.max_rows : l.g.E);
-  const int64_t blocks = (slots * l.g.b_tiles + 7) / 8 * 8;
-  hipLaunchKernelGGL((mx_gemm_kernel<GATE_UP, FP4, MI, SAVE_GU>), dim3((unsigned)blocks), dim3(GEMM_THREADS), 0, l.s, l.g);
+  const int64_t blocks = (slots * l.g.b_tiles * (4 / NJ) + 7) / 8 * 8;
+  hipLaunchKernelGGL((mx_gemm_kernel<GATE_UP, FP4, MI, NJ, SAVE_GU>), dim3((unsigned)blocks), dim3(GEMM_THREADS), 0, l.s, l.g);
 }
-// rows: of a tile, 64 or 128
-void launch_mx_gate_up(const MxLaunch& l, bool fp4, int rows);  // with l.g.gu: saving the gate / up values
-void launch_mx_down(const MxLaunch& l, bool fp4, int rows);
+enum class MxTileSize { R64xC128, R64xC256, R128xC256 };  // rows, weight rows of a workgroup
+void launch_mx_gate_up(const MxLaunch& l, bool fp4, MxTileSize t);  // with l.g.gu: saving the gate / up values
+void launch_mx_down(const MxLaunch& l, bool fp4, MxTileSize t);
 void launch_mx_small(const MxLaunch& l, bool gate_up, bool fp4);
 
 }  // namespace kmoe_mx

@@ -8,23 +8,34 @@ using namespace kmoe_mx;
 
 namespace {
 
-// Rows of a tile for max_rows rows over E experts.
-int tile_rows(int64_t max_rows, int E) {
-  const int64_t per = max_rows / E;
-  return per > 64 ? 128 : 64;
+// Tile of a product of max_rows rows over E experts, by the number of 64 x 256 tiles that they
+// come to where rows spread over the experts.  Up to 1.5 of those a CU, half as wide tiles use
+// the idle CUs; from there on the width halves the reads of rows.  128 rows halve the reads of
+// weights, but need many tiles: with e4m3 rows, of which two workgroups fit a CU with two LDS
+// stages only, from 5 a CU, with e2m1 rows (three stages) from 2.  us for 64x128 / 64x256 /
+// 128x256, weights not in cache, (tiles a CU): top-2 of 16, d 2048, F 2816, e4m3: down, 48
+// tokens (0.5) 10.9 / 13.1 / 22; 777 (1) 18.6 / 20.8 / 23.5; 2042 (2.2) 31.7 / 32.5 / 35;
+// gate/up, 48 (1.4) 19.9 / 20.8 / 29; 1024 (3.5) 42 / 38 / 48; 2042 (6.1) 64 / 61 / 60; 4096
+// (12) 114 / 102 / 101; e2m1: gate/up, 777 (2.8) 32 / 33 / 30; 2042 (6.1) 52 / 50 / 45; down,
+// 1024 (1.3) 17.9 / 17.8 / 16.3.  Top-6 of 64, d 1024, F 704, gate/up: e4m3, 400 (1.7) 14.8 /
+// 13.7 / 16.7; 2000 (5.1) 30 / 32 / 27; e2m1, 400 (1.7) 12.8 / 12.6 / 15.0.
+MxTileSize tile_size(bool fp4, int64_t max_rows, int E, int b_tiles) {
+  const int64_t used = std::min<int64_t>(max_rows, E), tiles = std::max(used, max_rows / 64 + used / 2) * b_tiles;
+  const int64_t cu = kmoe::cu_count();
+  if (2 * tiles <= 3 * cu) return MxTileSize::R64xC128;
+  return tiles <= (fp4 ? 2 : 5) * cu ? MxTileSize::R64xC256 : MxTileSize::R128xC256;
 }
 
 // Whether a product runs on the small-row kernel (kmoe_mx_gemm_small.hip): where its grid is at
-// most three workgroups per CU, as latency then counts, at few rows per expert.  Kernel times
-// in us, small-row kernel / 64-row tiles, top-2 of 16 experts, d 2048, F 2816, w4a8: 1 token
-// (176 workgroups in gate/up, 128 in down) 6.1 / 11.2 and 5.2 / 12.7; 4 tokens (704, 512) 9.8 /
-// 11.9 and 7.5 / 12.7; 8 tokens (1408, 1024) 19.5 / 12.8 and 10.4 / 12.7; 48 tokens (1672,
-// 1216) 28 / 20 and 15.7 / 13.5; 32 rows of 64 experts, d 1024, F 704 (792, 1056) 12.5 / 8.1
-// and 7.5 / 6.3: each workgroup looks its slot up and reduces, which the tiles do once for
-// eight times the weights.
+// most two workgroups per CU, as latency then counts, at few rows per expert.  us, small-row
+// kernel / 64 x 128 tiles, e4m3 (workgroups): top-2 of 16 experts, d 2048, F 2816, down, 1 token
+// (128) 7.3 / 9.8, 4 (512) 7.7 / 9.9, 16 (1088) 12.9 / 10.7; gate/up, 1 (176) 9.3 / 10.1, 4
+// (704) 14.5 / 11.1, 48 (1672) 31 / 19.4; top-2 of 8, d 4096, F 1408, gate/up, 4 (352) 9.9 /
+// 13.5, 48 (484) 15.3 / 14.4: each workgroup looks its slot up and reduces, which the tiles do
+// once for four times the weights.
 bool small_product(bool gate_up, int64_t max_rows, int E, int b_tiles) {
   const int64_t slots = max_rows / SMALL_ROWS + std::min<int64_t>(max_rows, E);
-  return max_rows <= 32 * (int64_t)E && slots * b_tiles * (gate_up ? 4 : 8) <= 3 * kmoe::cu_count();
+  return max_rows <= 32 * (int64_t)E && slots * b_tiles * (gate_up ? 4 : 8) <= 2 * kmoe::cu_count();
 }
 
 int check(const char* who, const void* a, const uint8_t* a_scale, int fmt, const int32_t* offsets, int E, int d, int F,
@@ -81,7 +92,7 @@ extern "C" int kmoe_gemm_gate_up_mx(const void* xq, const uint8_t* x_scale, int 
   if (small_product(true, max_rows, E, l.g.b_tiles))
     launch_mx_small(l, true, fmt == KMOE_DTYPE_FP4_E2M1);
   else
-    launch_mx_gate_up(l, fmt == KMOE_DTYPE_FP4_E2M1, tile_rows(max_rows, E));
+    launch_mx_gate_up(l, fmt == KMOE_DTYPE_FP4_E2M1, tile_size(fmt == KMOE_DTYPE_FP4_E2M1, max_rows, E, l.g.b_tiles));
   return kmoe::check_launch("kmoe_gemm_gate_up_mx");
 }
 
@@ -110,6 +121,6 @@ extern "C" int kmoe_gemm_down_mx(const void* hq, const uint8_t* h_scale, int fmt
   if (small_product(false, max_rows, E, l.g.b_tiles))
     launch_mx_small(l, false, fmt == KMOE_DTYPE_FP4_E2M1);
   else
-    launch_mx_down(l, fmt == KMOE_DTYPE_FP4_E2M1, tile_rows(max_rows, E));
+    launch_mx_down(l, fmt == KMOE_DTYPE_FP4_E2M1, tile_size(fmt == KMOE_DTYPE_FP4_E2M1, max_rows, E, l.g.b_tiles));
   return kmoe::check_launch("kmoe_gemm_down_mx");
 }

@@ -3,11 +3,13 @@
 
 namespace kmoe_mx {
 template <bool FP4>
-static void by_rows(const MxLaunch& l, int rows) {
-  if (rows == 128)
-    launch_mx_tile<false, FP4, 2>(l);
+static void by_tile(const MxLaunch& l, MxTileSize t) {
+  if (t == MxTileSize::R128xC256)
+    launch_mx_tile<false, FP4, 2, 4>(l);
+  else if (t == MxTileSize::R64xC256)
+    launch_mx_tile<false, FP4, 1, 4>(l);
   else
-    launch_mx_tile<false, FP4, 1>(l);
+    launch_mx_tile<false, FP4, 1, 2>(l);
 }
-void launch_mx_down(const MxLaunch& l, bool fp4, int rows) { fp4 ? by_rows<true>(l, rows) : by_rows<false>(l, rows); }
+void launch_mx_down(const MxLaunch& l, bool fp4, MxTileSize t) { fp4 ? by_tile<true>(l, t) : by_tile<false>(l, t); }
 }  // namespace kmoe_mx
