@@ -11,19 +11,20 @@ namespace {
 // Tile of a product of max_rows rows over E experts, by the number of 64 x 256 tiles that they
 // come to where rows spread over the experts.  Up to 1.5 of those a CU, half as wide tiles use
 // the idle CUs; from there on the width halves the reads of rows.  128 rows halve the reads of
-// weights, but need many tiles: with e4m3 rows, of which two workgroups fit a CU with two LDS
-// stages only, from 5 a CU, with e2m1 rows (three stages) from 2.  us for 64x128 / 64x256 /
-// 128x256, weights not in cache, (tiles a CU): top-2 of 16, d 2048, F 2816, e4m3: down, 48
-// tokens (0.5) 10.9 / 13.1 / 22; 777 (1) 18.6 / 20.8 / 23.5; 2042 (2.2) 31.7 / 32.5 / 35;
-// gate/up, 48 (1.4) 19.9 / 20.8 / 29; 1024 (3.5) 42 / 38 / 48; 2042 (6.1) 64 / 61 / 60; 4096
-// (12) 114 / 102 / 101; e2m1: gate/up, 777 (2.8) 32 / 33 / 30; 2042 (6.1) 52 / 50 / 45; down,
-// 1024 (1.3) 17.9 / 17.8 / 16.3.  Top-6 of 64, d 1024, F 704, gate/up: e4m3, 400 (1.7) 14.8 /
-// 13.7 / 16.7; 2000 (5.1) 30 / 32 / 27; e2m1, 400 (1.7) 12.8 / 12.6 / 15.0.
+// weights: with e2m1 rows where the experts have more than 64 and the tiles fill the CUs; with
+// e4m3 rows, of which two workgroups fit a CU with two LDS stages only, from 5 tiles a CU.  us
+// for 64x128 / 64x256 / 128x256, weights from HBM, (tiles a CU): top-2 of 16, d 2048, F 2816,
+// e4m3: down, 48 tokens (0.5) 13.3 / 15.0 / 27; 777 (1) 22 / 24 / 28; 2042 (2.2) 35 / 35 / 38;
+// gate/up, 48 (1.4) 21.7 / 22.3 / 29; 1024 (3.4) 44 / 39 / 49; 2042 (6.2) 66 / 60 / 60; 4096
+// (12) 117 / 103 / 101; e2m1: down, 500 (0.8) 17.1 / 15.0 / 17.7; 777 (1) 20.7 / 22 / 18.3; 2042
+// 33 / 32 / 32; gate/up, 777 (2.8) 33 / 33 / 29; 2042 54 / 52 / 47.  Top-6 of 64, d 1024, F 704,
+// gate/up: e4m3, 400 (1.6) 17.2 / 15.3 / 18.9; 2000 (5.1) 35 / 32 / 31; e2m1, 400 15.1 / 14.4 /
+// 17.4; 1000 (93 rows an expert, 2.9) 19.4 / 19.4 / 18.0.
 MxTileSize tile_size(bool fp4, int64_t max_rows, int E, int b_tiles) {
   const int64_t used = std::min<int64_t>(max_rows, E), tiles = std::max(used, max_rows / 64 + used / 2) * b_tiles;
   const int64_t cu = kmoe::cu_count();
-  if (2 * tiles <= 3 * cu) return MxTileSize::R64xC128;
-  return tiles <= (fp4 ? 2 : 5) * cu ? MxTileSize::R64xC256 : MxTileSize::R128xC256;
+  if (fp4 ? max_rows > 64 * (int64_t)E && tiles >= cu : tiles > 5 * cu) return MxTileSize::R128xC256;
+  return 2 * tiles <= 3 * cu ? MxTileSize::R64xC128 : MxTileSize::R64xC256;
 }
 
 // Whether a product runs on the small-row kernel (kmoe_mx_gemm_small.hip): where its grid is at
