@@ -592,7 +592,7 @@ int kmoe_add_rmsnorm_bwd(const void* dn, const void* h, int h_dtype, const void*
  * are not used.                                    */
 size_t kmoe_mx_row_bytes(int K, int fmt);
 size_t kmoe_mx_scale_bytes(int K);
-/* Codes of bf16 rows x[row_index ? row_index[r] : r] (K a multiple of 32);
+/* Codes of bf16 rows x[row_index ? row_index[r] : r] (-1: zeros; K a multiple of 32);
  * n_rows_dev (nullable, device): rows past *n_rows_dev are left as they are.        */
 int kmoe_quant_rows_mx(const void* x, const int32_t* row_index, int64_t rows, const int32_t* n_rows_dev, int K,
                        int fmt, void* q, uint8_t* scale, void* stream);

@@ -14,7 +14,8 @@ unsigned grid_of(int64_t items, int per_block) {
 }
 
 // Rows of x (bf16, K a multiple of 32) to codes and scales, both padded to the 128-step of
-// K with zeros.  A lane takes 8 values, four lanes a block; row r is x[row_index[r]].
+// K with zeros.  A lane takes 8 values, four lanes a block; row r is x[row_index[r]],
+// zeros for -1.
 template <bool FP4>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const uint16_t* __restrict__ x, const int32_t* __restrict__ row_index,
                                                          int64_t rows, const int32_t* __restrict__ n_rows_dev, int K,
@@ -26,10 +27,8 @@ __global__ __launch_bounds__(256) void quant_rows_kernel(const uint16_t* __restr
     const int64_t r = i / cpr;
     const int c = (int)(i - r * cpr);
     float v[8] = {};
-    if (c * 8 < K) {
-      const int64_t src = row_index ? (int64_t)row_index[r] : r;
-      unpack8(*reinterpret_cast<const i32x4_t*>(x + src * K + c * 8), v);
-    }
+    const int64_t src = row_index ? (int64_t)row_index[r] : r;
+    if (c * 8 < K && src >= 0) unpack8(*reinterpret_cast<const i32x4_t*>(x + src * K + c * 8), v);
     uint32_t code;
     const Codes<FP4, 8> o = encode_quad<FP4>(v, code);
     if constexpr (FP4)

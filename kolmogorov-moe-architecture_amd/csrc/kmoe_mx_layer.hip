@@ -33,8 +33,8 @@ __global__ __launch_bounds__(FEW) void tables_kernel(const int64_t* __restrict__
     const int64_t t = i / cpr;
     const int c = (int)(i - t * cpr);
     float v[8] = {};
-    if (c * 8 < d)
-      unpack8(*reinterpret_cast<const i32x4_t*>(x + (row_index ? (int64_t)row_index[t] : t) * d + c * 8), v);
+    const int64_t src = row_index ? (int64_t)row_index[t] : t;
+    if (c * 8 < d && src >= 0) unpack8(*reinterpret_cast<const i32x4_t*>(x + src * d + c * 8), v);
     uint32_t code;
     const Codes<FP4, 8> o = encode_quad<FP4>(v, code);
     if constexpr (FP4)

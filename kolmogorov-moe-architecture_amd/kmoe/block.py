@@ -209,6 +209,8 @@ class MoEFFNBlock(nn.Module):
         use_mod = self.ffn_mod_router is not None and self.training
         if delta is not None and delta.shape != hidden_states.shape:
             raise ValueError(f"kmoe.MoEFFNBlock: hidden_states {tuple(hidden_states.shape)}, delta {tuple(delta.shape)}")
+        if delta is not None and delta.dtype not in (torch.bfloat16, torch.float32):
+            hidden_states, delta = hidden_states + delta, None
         if not use_mod and self._mx_fusable(hidden_states) and not (torch.is_grad_enabled() and delta is not None
                                                                     and delta.requires_grad):
             out = self._forward_mx(hidden_states, delta)

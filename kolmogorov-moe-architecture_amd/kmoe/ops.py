@@ -784,7 +784,7 @@ def route_topk(logits, k, scores="softmax", bias=None, groups=1, topk_groups=1, 
 
 def route_topk_bwd(logits, idx, dw, scores="softmax", renorm=True, scale=1.0, dlogits=None):
     """Gradient of route_topk's weights: dw (T, k) to the logits' (T, E) f32, added to
-    `dlogits` when given."""
+    `dlogits` when given.  idx: route_topk's, so a token's experts are distinct."""
     sc = _scores(scores)
     logits = _route_logits(logits, "route_topk_bwd")
     T, E = logits.shape
@@ -833,9 +833,27 @@ def _mx_rows(rows, K, fmt, dev) -> MXRows:
                   torch.empty(rows, (K + 511) // 512 * 16, device=dev, dtype=torch.uint8), K, fmt)
 
 
+def _coded(r: MXRows, who) -> int:
+    """The element type code of coded rows that are laid out as the kernels read them."""
+    code = _mx_fmt(r.fmt)
+    kp = (r.K + 127) // 128 * 128
+    if (r.q.dim() != 2 or r.q.shape[1] != (kp if r.fmt == "e4m3" else kp // 2)
+            or r.scale.shape != (r.q.shape[0], (r.K + 511) // 512 * 16) or r.scale.device != r.q.device
+            or any(t.element_size() != 1 or not t.is_contiguous() or t.data_ptr() % 16 for t in r[:2])):
+        raise ValueError(f"kmoe.{who}: q {tuple(r.q.shape)} {r.q.dtype}, scale {tuple(r.scale.shape)} {r.scale.dtype} are "
+                         f"not the contiguous, 16-byte aligned codes and scales of {r.fmt} rows of {r.K} values")
+    return code
+
+
+def _table(t, n, who, name):
+    """An int32 table of at least n entries as the kernels read it."""
+    if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < n:
+        raise ValueError(f"kmoe.{who}: {name} must be contiguous int32 of {n} entries, got {t.dtype} {tuple(t.shape)}")
+
+
 def quant_rows_mx(m, fmt="e4m3", row_index=None, n_rows_dev=None) -> MXRows:
     """Microscaled codes of the bf16 rows of m (n, K), K a multiple of 32, or of its rows
-    row_index (int32).  Rows past *n_rows_dev (int32, on the GPU) are left unwritten."""
+    row_index (int32; -1: zeros).  Rows past *n_rows_dev (int32, on the GPU) are left unwritten."""
     code = _mx_fmt(fmt)
     _need_gpu(m, row_index, n_rows_dev)
     if m.dim() != 2:
@@ -853,7 +871,7 @@ def quant_rows_mx(m, fmt="e4m3", row_index=None, n_rows_dev=None) -> MXRows:
 
 def dequant_rows_mx(r: MXRows, row_index=None, n_rows_dev=None):
     """The values (n, K) bf16 of coded rows, or of rows row_index (int32; -1: zeros)."""
-    code = _mx_fmt(r.fmt)
+    code = _coded(r, "dequant_rows_mx")
     _need_gpu(r.q, r.scale, row_index, n_rows_dev)
     if row_index is not None:
         row_index = _contig(row_index, torch.int32)
@@ -913,6 +931,10 @@ def gemm_gate_up_mx(x: MXRows, row_token, offsets, pw: PackedWeightsMX, max_rows
     """Coded rows of silu(x w1) * (x w2) in x's format: permuted row r is x's row
     row_token[r] (row r without row_token).  save_gu (training): (h, gu), gu the bf16
     pre-activation gate / up values (max_rows, 2 F_pad) in the backward's column order."""
+    code = _coded(x, "gemm_gate_up_mx")
+    _table(offsets, pw.E + 1, "gemm_gate_up_mx", "offsets")
+    if row_token is not None:
+        _table(row_token, max_rows, "gemm_gate_up_mx", "row_token")
     _need_gpu(x.q, row_token, offsets)
     if x.K != pw.d:
         raise ValueError(f"kmoe.gemm_gate_up_mx: rows of {x.K} values for weights of d={pw.d}")
@@ -922,7 +944,7 @@ def gemm_gate_up_mx(x: MXRows, row_token, offsets, pw: PackedWeightsMX, max_rows
     h = _mx_rows(max(max_rows, 1), pw.F, x.fmt, x.q.device)
     gu = torch.empty(max(max_rows, 1), 2 * fp, device=x.q.device, dtype=_BF16) if save_gu else None
     with _device(x.q.device), _Stage("gemm_gate_up"):
-        _lib.call("kmoe_gemm_gate_up_mx", ptr(x.q), ptr(x.scale), _mx_fmt(x.fmt), x.q.shape[0], ptr(row_token),
+        _lib.call("kmoe_gemm_gate_up_mx", ptr(x.q), ptr(x.scale), code, x.q.shape[0], ptr(row_token),
                   ptr(offsets), pw.E, pw.d, pw.F, max_rows, ptr(pw.w13), ptr(pw.s13), ptr(h.q), ptr(h.scale), ptr(gu),
                   _stream(x.q))
     return (h, gu) if save_gu else h
@@ -930,12 +952,14 @@ def gemm_gate_up_mx(x: MXRows, row_token, offsets, pw: PackedWeightsMX, max_rows
 
 def gemm_down_mx(h: MXRows, offsets, pw: PackedWeightsMX, max_rows):
     """y (max_rows, d) bf16 = h w3 of the coded rows of each expert."""
+    code = _coded(h, "gemm_down_mx")
+    _table(offsets, pw.E + 1, "gemm_down_mx", "offsets")
     _need_gpu(h.q, offsets)
     if h.K != pw.F or h.q.shape[0] < max_rows:
         raise ValueError(f"kmoe.gemm_down_mx: rows {tuple(h.q.shape)} of {h.K} values, F={pw.F}, max_rows {max_rows}")
     y = torch.empty(max(max_rows, 1), pw.d, device=h.q.device, dtype=_BF16)
     with _device(h.q.device), _Stage("gemm_down"):
-        _lib.call("kmoe_gemm_down_mx", ptr(h.q), ptr(h.scale), _mx_fmt(h.fmt), ptr(offsets), pw.E, pw.d, pw.F, max_rows,
+        _lib.call("kmoe_gemm_down_mx", ptr(h.q), ptr(h.scale), code, ptr(offsets), pw.E, pw.d, pw.F, max_rows,
                   ptr(pw.w3), ptr(pw.s3), ptr(y), _stream(h.q))
     return y
 
@@ -968,12 +992,18 @@ def mx_experts(x2d, idx, w, pw: PackedWeightsMX, fmt, capacity=0, row_index=None
         if coded.fmt != fmt or coded.K != d or coded.q.shape[0] != T or row_index is not None:
             raise ValueError(f"kmoe.mx_experts: coded rows {tuple(coded.q.shape)} ({coded.fmt}, K={coded.K}) for T={T}, "
                              f"d={d}, {fmt}")
+        _coded(coded, "mx_experts")
         xq, xs = coded.q, coded.scale
     if row_index is not None:
         row_index = _contig(row_index, torch.int32)
         if row_index.numel() != T:
             raise ValueError(f"kmoe.mx_experts: row_index of {row_index.numel()} rows for {T} tokens")
     T_out = T if T_out is None else T_out
+    if out_map is not None:
+        _table(out_map, T_out, "mx_experts", "out_map")
+    if scale is not None and (scale.dtype != torch.float32 or not scale.is_contiguous() or scale.numel() < T):
+        raise ValueError(f"kmoe.mx_experts: scale must be contiguous f32 of {T} tokens, got {scale.dtype} "
+                         f"{tuple(scale.shape)}")
     dev = x2d.device
     y = torch.empty(T_out, d, device=dev, dtype=out_dtype)
     if residual is not None:

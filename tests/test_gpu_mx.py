@@ -488,6 +488,114 @@ def test_empty_calls(dev):
     assert got.shape == (0, 64) and not info.counts.any()
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+def test_missing_rows_are_zeros(dev, fmt):
+    """row_index -1 in the quantisation and in the one-call pass."""
+    x = rnd(dev, 5, 96)
+    rows = torch.tensor([3, -1, 0, -1], dtype=torch.int32, device=dev)
+    q = ops.quant_rows_mx(x, fmt, row_index=rows)
+    want = ops.quant_rows_mx(torch.stack([x[3], torch.zeros_like(x[0]), x[0], torch.zeros_like(x[0])]), fmt)
+    assert torch.equal(q.q, want.q) and torch.equal(used(q), used(want))
+    pw = ops.pack_weights_mx(*weights(dev, 2, 128, 64))
+    x = rnd(dev, 5, 128)
+    idx, w = torch.tensor([[0], [1], [1], [0]], device=dev), torch.ones(4, 1, device=dev)
+    y = ops.mx_experts(x, idx, w, pw, fmt, row_index=rows)[0]
+    assert not y[1].any() and not y[3].any()
+    assert torch.equal(y[[0, 2]], ops.mx_experts(x[[3, 0]], idx[[0, 2]], w[[0, 2]], pw, fmt)[0])
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("d,F", [(128, 2816), (2816, 128)])
+def test_offsets_past_32_bits(dev, fmt, d, F):
+    """The last tokens of a batch whose expert rows (h, or y) hold over 2^31 values: those of
+    the same tokens alone."""
+    E, k, T = 3, 2, 400_003
+    pw = ops.pack_weights_mx(*weights(dev, E, d, F))
+    g = torch.Generator(device=dev).manual_seed(3)
+    x = torch.empty(T, d, device=dev, dtype=BF).normal_(generator=g)
+    idx = torch.randint(0, E, (T, k), device=dev, generator=g)
+    w = torch.ones(T, k, device=dev)
+    y = ops.mx_experts(x, idx, w, pw, fmt)[0]
+    few = [0, 1, T // 2, T - 3, T - 2, T - 1]
+    assert torch.equal(y[few], ops.mx_experts(x[few], idx[few], w[few], pw, fmt)[0])
+
+
+def test_two_streams_at_once(dev):
+    """Two passes of one layer on two streams at once, several times: each its own result."""
+    layer = kmoe.MoELayer(config(E=8, d=256, F=352, moe_mx="w4a4")).to(dev).to(BF).eval()
+    xs = [rnd(dev, 1, T, 256, seed=T) for T in (33, 700)]
+    with torch.no_grad():
+        want = [layer(x) for x in xs]
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        got = []
+        for s in streams:
+            s.wait_stream(torch.cuda.current_stream())
+        for _ in range(8):
+            for s, x in zip(streams, xs):
+                with torch.cuda.stream(s):
+                    got.append(layer(x))
+        torch.cuda.synchronize()
+        for i, y in enumerate(got):
+            assert torch.equal(y, want[i % 2])
+
+
+def test_training_step_in_a_graph(dev):
+    """Forward and gradients of norm, routing and experts captured together and replayed on new
+    inputs, eager passes of other leaves in between."""
+    d, E, k, T = 128, 8, 2, 40
+    ex = kmoe.GroupedExperts(E, d, 96).to(dev).to(BF)
+    ex.mx = "w4a8"
+    wr = rnd(dev, E, d, std=0.1, dtype=torch.float32)
+    dy, dh = rnd(dev, T, d, seed=5), rnd(dev, T, d, seed=6)
+
+    def step(x, delta, gain):
+        leaves = [v.detach().requires_grad_(True) for v in (x, delta, gain)]
+        params = list(ex.parameters())
+        h, n = kmoe.add_rms_norm(*leaves)
+        w, idx = kmoe.route_topk(torch.nn.functional.linear(n.float(), wr), k, scores="sigmoid", groups=2)
+        y = ex(n, idx, w)
+        return [y.detach(), h.detach()] + list(torch.autograd.grad([y, h], leaves + params, [dy, dh]))
+
+    sets = [(rnd(dev, T, d, seed=i), rnd(dev, T, d, seed=10 + i), 1 + rnd(dev, d, seed=20 + i, std=0.1)) for i in range(4)]
+    buf = [v.clone() for v in sets[0]]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*buf)
+    torch.cuda.current_stream().wait_stream(side)
+    eager = [step(*s) for s in sets]
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(*buf)
+    for i in (1, 2, 3, 0):
+        for b, v in zip(buf, sets[i]):
+            b.copy_(v)
+        g.replay()
+        torch.cuda.synchronize()
+        for u, v in zip(out, eager[i]):
+            assert torch.equal(u, v)
+        assert all(torch.equal(u, v) for u, v in zip(step(*sets[(i + 1) % 4]), eager[(i + 1) % 4]))
+
+
+@pytest.mark.parametrize("training", [False, True])
+@pytest.mark.parametrize("dtype", [BF, torch.float32, torch.float16])
+def test_block_edge_calls(dev, training, dtype):
+    """One token, and streams and deltas of other types than the weights'; an empty batch is
+    refused by the router, as in the bf16 block."""
+    cfg = config(E=4, d=128, F=96, moe_mx="w4a8")
+    blk = kmoe.MoEFFNBlock(cfg).to(dev).to(BF).train(training)
+    with torch.no_grad():
+        h = rnd(dev, 1, 1, 128, dtype=dtype)
+        for empty in ((h[:, :0],), (h[:, :0], h[:, :0])):
+            with pytest.raises(kmoe.KmoeError, match="kmoe_router"):
+                blk(*empty)
+        for dd in (BF, torch.float32, torch.float16, torch.float64):
+            delta = rnd(dev, 1, 1, 128, seed=1, dtype=dd)
+            y = blk(h, delta)
+            want = blk(h + delta)
+            assert y.dtype == want.dtype and torch.equal(y, want)
+
+
 def test_refusals(dev):
     with pytest.raises(ValueError, match="element type"):
         ops.quant_rows_mx(rnd(dev, 2, 64), "e5m2")

@@ -129,6 +129,32 @@ def test_cpu_tensors_are_refused():
             call()
 
 
+def test_coded_rows_and_tables_are_checked():
+    """Codes, scales and tables that the kernels would read past: refused by their layout, on
+    any device."""
+    u8 = torch.uint8
+    good = ops.MXRows(torch.zeros(4, 128, dtype=u8), torch.zeros(4, 16, dtype=u8), 64, "e4m3")
+    pw = ops.PackedWeightsMX(*(torch.zeros(1, dtype=u8) for _ in range(4)), 2, 64, 64)
+    off, row = torch.zeros(3, dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    bad = [good._replace(q=torch.zeros(4, 256, dtype=u8)[:, :128]), good._replace(q=torch.zeros(4, 64, dtype=u8)),
+           good._replace(K=192), good._replace(fmt="e2m1"), good._replace(scale=torch.zeros(3, 16, dtype=u8)),
+           good._replace(scale=torch.zeros(4, 4, dtype=u8)), good._replace(scale=torch.zeros(4, 32, dtype=u8)[:, :16]),
+           good._replace(q=good.q.to(torch.int32)), good._replace(q=torch.zeros(128, 4, dtype=u8).t()),
+           good._replace(q=torch.zeros(4 * 128 + 8, dtype=u8)[8:].view(4, 128))]
+    for r in bad:
+        for call in (lambda: ops.dequant_rows_mx(r), lambda: ops.gemm_gate_up_mx(r, None, off, pw, 4),
+                     lambda: ops.gemm_down_mx(r, off, pw, 4)):
+            with pytest.raises(ValueError, match="contiguous, 16-byte aligned codes"):
+                call()
+    for o, r in ((off[:2], row), (off.long(), row), (off, row[:3]), (off, row.long()), (off, row.repeat(2)[::2])):
+        with pytest.raises(ValueError, match="contiguous int32"):
+            ops.gemm_gate_up_mx(good, r, o, pw, 4)
+    with pytest.raises(ValueError, match="contiguous int32"):
+        ops.gemm_down_mx(good, off[:2], pw, 4)
+    with pytest.raises(ValueError, match="GPU"):
+        ops.gemm_down_mx(good, off, pw, 4)
+
+
 # ---- the restatements themselves
 def test_elements_against_torch_casts():
     v = torch.cat([torch.linspace(-500, 500, 20001), torch.logspace(-12, 9, 5000, base=2.0)]).double()
