@@ -116,6 +116,19 @@ def test_backward_against_differences(dev):
             assert abs(num - float(dx[t, c])) <= bound + 1e-4
 
 
+def test_offsets_past_32_bits(dev):
+    """The last rows of 2^31 values, forward and backward: those of the same rows alone."""
+    T, d = 525_003, 4096
+    g = torch.Generator(device=dev).manual_seed(1)
+    x, delta, dn = (torch.empty(T, d, device=dev, dtype=BF).normal_(generator=g) for _ in range(3))
+    w = 1 + rnd(dev, d, std=0.1)
+    few = [0, T // 2, T - 2, T - 1]
+    r, f = ops.add_rmsnorm(x, delta, w, EPS, quant="e4m3"), ops.add_rmsnorm(x[few], delta[few], w, EPS, quant="e4m3")
+    assert all(torch.equal(u[few], v) for u, v in zip(r, f))
+    dx = ops.add_rmsnorm_bwd(dn, r.h, w, r.rrms, dh=delta)[0]
+    assert torch.equal(dx[few], ops.add_rmsnorm_bwd(dn[few], f.h, w, f.rrms, dh=delta[few])[0])
+
+
 def test_views_streams_and_graph(dev):
     x, delta = rnd(dev, 40, 512), rnd(dev, 40, 512, seed=1)
     w = torch.ones(256, device=dev, dtype=BF)

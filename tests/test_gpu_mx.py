@@ -520,6 +520,25 @@ def test_offsets_past_32_bits(dev, fmt, d, F):
     assert torch.equal(y[few], ops.mx_experts(x[few], idx[few], w[few], pw, fmt)[0])
 
 
+def test_weights_past_32_bits(dev):
+    """Experts whose weights and packed codes hold over 2^31 values and bytes: the last ones
+    alone give the same values, packs and products."""
+    E, d, F = 64, 4096, 9216
+    w = [torch.empty(*s, device=dev, dtype=BF) for s in ((E, d, F), (E, d, F), (E, F, d))]
+    for i, v in enumerate(w):
+        v.zero_()
+        v[-1].normal_(std=0.02, generator=torch.Generator(device=dev).manual_seed(i))
+    last = [v[-1:].contiguous() for v in w]
+    assert torch.equal(ops.fake_quant_mx_cols(w[0])[-1:], ops.fake_quant_mx_cols(last[0]))
+    pw, p1 = ops.pack_weights_mx(*w), ops.pack_weights_mx(*last)
+    for u, v in zip(pw[:4], p1[:4]):
+        assert torch.equal(u[-v.numel():], v)
+    x, one = rnd(dev, 40, d), torch.ones(40, 1, device=dev)
+    idx = torch.full((40, 1), E - 1, device=dev)
+    for fmt in ("e4m3", "e2m1"):
+        assert torch.equal(ops.mx_experts(x, idx, one, pw, fmt)[0], ops.mx_experts(x, 0 * idx, one, p1, fmt)[0])
+
+
 def test_two_streams_at_once(dev):
     """Two passes of one layer on two streams at once, several times: each its own result."""
     layer = kmoe.MoELayer(config(E=8, d=256, F=352, moe_mx="w4a4")).to(dev).to(BF).eval()
