@@ -15,8 +15,8 @@ int few_rounds(int E) { return 64 / E < 1 ? 1 : 64 / E > MAX_ROUNDS ? MAX_ROUNDS
 
 // Dispatch of at most R FEW assignments (the tables of kmoe_dispatch, same order) by workgroup
 // 0, the quantisation of the T rows x[row_index[t]] by the others: one launch in place of
-// three, whose latencies are the time at these sizes.  A thread holds assignments tid, FEW +
-// tid, ..; a rank is counted by ballots in its wave and summed over the waves before it.
+// three, whose latencies are the time at these sizes.  A thread holds assignments R tid ..
+// R tid + R - 1; a rank is counted by ballots in its wave and summed over the waves before it.
 template <bool FP4, int R>
 __global__ __launch_bounds__(FEW) void tables_kernel(const int64_t* __restrict__ idx, const void* __restrict__ wsrc,
                                                      bool w_f32, int T, int k, int E, int64_t capacity,
@@ -44,7 +44,7 @@ __global__ __launch_bounds__(FEW) void tables_kernel(const int64_t* __restrict__
     if ((c & 3) == 0) scale[t * scale_bytes(d) + c / 4] = (uint8_t)code;
     return;
   }
-  constexpr int NW = R * FEW / 64;  // waves' worth of assignments
+  constexpr int NW = FEW / 64;
   __shared__ int cnt[NW][KMOE_MAX_EXPERTS];
   __shared__ int off[KMOE_MAX_EXPERTS];
   const int lane = tid & 63, wave = tid >> 6, A = T * k;
@@ -52,7 +52,7 @@ __global__ __launch_bounds__(FEW) void tables_kernel(const int64_t* __restrict__
   float w[R];
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int a = r * FEW + tid;
+    const int a = tid * R + r;
     e[r] = -1;
     rank[r] = 0;
     w[r] = 0.0f;
@@ -63,23 +63,33 @@ __global__ __launch_bounds__(FEW) void tables_kernel(const int64_t* __restrict__
     }
   }
   const uint64_t before = lane == 0 ? 0ull : ~0ull >> (64 - lane);
-  for (int ee = 0; ee < E; ++ee)
+  for (int ee = 0; ee < E; ++ee) {
+    int at = 0, all = 0;  // of the lanes before, of the wave
 #pragma unroll
     for (int r = 0; r < R; ++r) {
       const uint64_t m = __ballot(e[r] == ee);
-      if (e[r] == ee) rank[r] = __popcll(m & before);
-      if (lane == 0) cnt[r * (FEW / 64) + wave][ee] = __popcll(m);
+      at += __popcll(m & before);
+      all += __popcll(m);
     }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (e[r] == ee) rank[r] = at++;
+    if (lane == 0) cnt[wave][ee] = all;
+  }
   __syncthreads();
   if (wave == 0) {
     // lane: an expert; cnt becomes the count of the waves before
     int c = 0;
-    if (lane < E)
+    if (lane < E) {
+      int n[NW];
+#pragma unroll
+      for (int v = 0; v < NW; ++v) n[v] = cnt[v][lane];
+#pragma unroll
       for (int v = 0; v < NW; ++v) {
-        const int n = cnt[v][lane];
         cnt[v][lane] = c;
-        c += n;
+        c += n[v];
       }
+    }
     const int kept = capacity > 0 && c > capacity ? (int)capacity : c;
     int incl = kept;
 #pragma unroll
@@ -97,11 +107,11 @@ __global__ __launch_bounds__(FEW) void tables_kernel(const int64_t* __restrict__
   __syncthreads();
 #pragma unroll
   for (int r = 0; r < R; ++r) {
-    const int a = r * FEW + tid;
+    const int a = tid * R + r;
     if (a < A) {
       int row = -1;
       if (e[r] >= 0) {
-        const int at = rank[r] + cnt[r * (FEW / 64) + wave][e[r]];
+        const int at = rank[r] + cnt[wave][e[r]];
         if (capacity <= 0 || at < capacity) {
           row = off[e[r]] + at;
           row_token[row] = a / k;

@@ -122,71 +122,6 @@ __global__ __launch_bounds__(64 * NORM_FWD_WAVES) void rmsnorm_kernel(const void
   if (lane == 0) rrms[t] = r;
 }
 
-// h = x + delta rounded to x's type (without delta h is x, not written), n = bf16(g * (h r)), r = 1/sqrt(mean(h^2) + eps), all
-// from the rounded h (what the backward and the next block read), and n's microscaled rows
-// (Q 1: e4m3, 2: e2m1; 0: none).  The rows are those of the bf16 n, so the experts' products
-// see the values that the router sees, and the codes do not depend on the norm being fused.
-// Sums as in rmsnorm_kernel, so n is that of a torch addition followed by kmoe_rmsnorm, bit
-// for bit.  One wave per row.
-template <int NV, bool XF32, int Q>
-__global__ __launch_bounds__(64 * NORM_FWD_WAVES) void add_rmsnorm_kernel(
-    const void* __restrict__ x, const void* __restrict__ delta, bool delta_f32, const void* __restrict__ g, bool g_f32,
-    float eps, int64_t T, int d, void* __restrict__ h, uint16_t* __restrict__ n, float* __restrict__ rrms,
-    uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
-  const int lane = threadIdx.x & 63;
-  const int64_t t = (int64_t)blockIdx.x * NORM_FWD_WAVES + (threadIdx.x >> 6);
-  if (t >= T) return;
-  const int nvec = d / 8;
-  float hv[NV][8];
-  float ss = 0.0f;
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = lane + 64 * i;
-    if (v < nvec) {
-      float dv[8];
-      load8<XF32>(x, t * d + (int64_t)v * 8, hv[i]);
-      if (delta) {
-        load8_any(delta, delta_f32, t * d + (int64_t)v * 8, dv);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) {
-          hv[i][c] += dv[c];
-          if (!XF32) hv[i][c] = bf16_to_f32(f32_to_bf16(hv[i][c]));
-        }
-        store8<XF32>(h, t * d + (int64_t)v * 8, hv[i]);
-      }
-#pragma unroll
-      for (int c = 0; c < 8; ++c) ss = fmaf(hv[i][c], hv[i][c], ss);
-    }
-  }
-  ss = wave_sum(ss);
-  const float r = 1.0f / sqrtf(ss / (float)d + eps);
-  if (lane == 0) rrms[t] = r;
-  const int qvec = Q ? kmoe_mx::round_up(d, kmoe_mx::STEP) / 8 : nvec;  // with the padding of a coded row
-#pragma unroll
-  for (int i = 0; i < NV; ++i) {
-    const int v = lane + 64 * i;
-    if (v < qvec) {  // d is a multiple of 32 with Q: the four lanes of a block agree
-      float o[8] = {};
-      if (v < nvec) {
-        float gv[8];
-        load8_any(g, g_f32, (int64_t)v * 8, gv);
-#pragma unroll
-        for (int c = 0; c < 8; ++c) o[c] = bf16_to_f32(f32_to_bf16(gv[c] * (hv[i][c] * r)));
-        store8<false>(n, t * d + (int64_t)v * 8, o);
-      }
-      if constexpr (Q != 0) {
-        uint32_t code;
-        const kmoe_mx::Codes<Q == 2, 8> w = kmoe_mx::encode_quad<Q == 2>(o, code);
-        if constexpr (Q == 2)
-          *reinterpret_cast<uint32_t*>(q + t * (qvec * 4) + v * 4) = w.w[0];
-        else
-          *reinterpret_cast<i32x2_t*>(q + t * (qvec * 8) + v * 8) = i32x2_t{(int)w.w[0], (int)w.w[1]};
-        if ((v & 3) == 0) scale[t * kmoe_mx::scale_bytes(d) + v / 4] = (uint8_t)code;
-      }
-    }
-  }
-}
-
 // One row's inputs as loaded (bf16: one 16-byte vector per 8 elements, f32: two).
 template <bool F32>
 struct Raw8 {
@@ -211,6 +146,111 @@ __device__ __forceinline__ void unpack_raw(const Raw8<F32>& r, float (&v)[8]) {
     for (int q = 0; q < 4; ++q) {
       v[2 * q] = __uint_as_float(((uint32_t)r.v[0][q]) << 16);
       v[2 * q + 1] = __uint_as_float(((uint32_t)r.v[0][q]) & 0xffff0000u);
+    }
+  }
+}
+
+// h = x + delta rounded to x's type (without delta h is x, not written), n = bf16(g * (h r)), r =
+// 1/sqrt(mean(h^2) + eps), all from the rounded h (what the backward and the next block read),
+// and n's microscaled rows (Q 1: e4m3, 2: e2m1; 0: none).  The rows are those of the bf16 n, so
+// the experts' products see the values that the router sees, and the codes do not depend on the
+// norm being fused.  Sums as in rmsnorm_kernel, so n is that of a torch addition followed by
+// kmoe_rmsnorm, bit for bit.  One wave per row.  Memory bounds it, at few rows its latency: a
+// row's loads (up to d 2048 the weight's too) go out before the first is waited for.  bf16 with
+// e4m3 rows, d 2048: 16384 rows 56 us, 5.4 TB/s (each
+// vector waited for on its own 65), 48 rows 7.4 (8.7).
+template <int NV, bool XF32, int Q>
+__global__ __launch_bounds__(64 * NORM_FWD_WAVES) void add_rmsnorm_kernel(
+    const void* __restrict__ x, const void* __restrict__ delta, bool delta_f32, const void* __restrict__ g, bool g_f32,
+    float eps, int64_t T, int d, void* __restrict__ h, uint16_t* __restrict__ n, float* __restrict__ rrms,
+    uint8_t* __restrict__ q, uint8_t* __restrict__ scale) {
+  const int lane = threadIdx.x & 63;
+  const int64_t t = (int64_t)blockIdx.x * NORM_FWD_WAVES + (threadIdx.x >> 6);
+  if (t >= T) return;
+  const int nvec = d / 8;
+  constexpr bool EARLY_G = NV <= 4;
+  auto at = [&](int i) { return (int64_t)min(lane + 64 * i, nvec - 1) * 8; };  // lanes past the row read its end
+  Raw8<XF32> xr[NV];
+#pragma unroll
+  for (int i = 0; i < NV; ++i) load_raw<XF32>(x, t * d + at(i), xr[i]);
+  Raw8<true> gr[EARLY_G ? NV : 1];
+  auto early_g = [&]() {
+    if constexpr (EARLY_G) {
+#pragma unroll
+      for (int i = 0; i < NV; ++i) {
+        const i32x4_t* const p = reinterpret_cast<const i32x4_t*>(static_cast<const uint8_t*>(g) + at(i) * (g_f32 ? 4 : 2));
+        gr[i].v[0] = p[0];
+        gr[i].v[1] = p[g_f32 ? 1 : 0];
+      }
+    }
+  };
+  float hv[NV][8];
+  auto add = [&](auto f32_tag) {
+    constexpr bool F32 = decltype(f32_tag)::value;
+    Raw8<F32> dr[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) load_raw<F32>(delta, t * d + at(i), dr[i]);
+    early_g();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+      float dv[8];
+      unpack_raw<XF32>(xr[i], hv[i]);
+      unpack_raw<F32>(dr[i], dv);
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        hv[i][c] += dv[c];
+        if (!XF32) hv[i][c] = bf16_to_f32(f32_to_bf16(hv[i][c]));
+      }
+      if (lane + 64 * i < nvec) store8<XF32>(h, t * d + at(i), hv[i]);
+    }
+  };
+  if (!delta) {
+    early_g();
+#pragma unroll
+    for (int i = 0; i < NV; ++i) unpack_raw<XF32>(xr[i], hv[i]);
+  } else if (delta_f32) {
+    add(std::true_type{});
+  } else {
+    add(std::false_type{});
+  }
+  float ss = 0.0f;
+#pragma unroll
+  for (int i = 0; i < NV; ++i)
+    if (lane + 64 * i < nvec) {
+#pragma unroll
+      for (int c = 0; c < 8; ++c) ss = fmaf(hv[i][c], hv[i][c], ss);
+    }
+  ss = wave_sum(ss);
+  const float r = 1.0f / sqrtf(ss / (float)d + eps);
+  if (lane == 0) rrms[t] = r;
+  const int qvec = Q ? kmoe_mx::round_up(d, kmoe_mx::STEP) / 8 : nvec;  // with the padding of a coded row
+#pragma unroll
+  for (int i = 0; i < NV; ++i) {
+    const int v = lane + 64 * i;
+    if (v < qvec) {  // d is a multiple of 32 with Q: the four lanes of a block agree
+      float o[8] = {};
+      if (v < nvec) {
+        float gv[8];
+        if constexpr (!EARLY_G) {
+          load8_any(g, g_f32, (int64_t)v * 8, gv);
+        } else if (g_f32) {
+          unpack_raw<true>(gr[i], gv);
+        } else {
+          unpack_raw<false>(Raw8<false>{{gr[i].v[0]}}, gv);
+        }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) o[c] = bf16_to_f32(f32_to_bf16(gv[c] * (hv[i][c] * r)));
+        store8<false>(n, t * d + (int64_t)v * 8, o);
+      }
+      if constexpr (Q != 0) {
+        uint32_t code;
+        const kmoe_mx::Codes<Q == 2, 8> w = kmoe_mx::encode_quad<Q == 2>(o, code);
+        if constexpr (Q == 2)
+          *reinterpret_cast<uint32_t*>(q + t * (qvec * 4) + v * 4) = w.w[0];
+        else
+          *reinterpret_cast<i32x2_t*>(q + t * (qvec * 8) + v * 8) = i32x2_t{(int)w.w[0], (int)w.w[1]};
+        if ((v & 3) == 0) scale[t * kmoe_mx::scale_bytes(d) + v / 4] = (uint8_t)code;
+      }
     }
   }
 }
