@@ -146,6 +146,7 @@ __device__ __forceinline__ uint64_t keep_groups(const RouteArgs& a, const V* val
   for (int g = sub; g < a.groups; g += LANES) {
     const V v = val[g];
     int rank = 0;
+#pragma unroll 8
     for (int j = 0; j < a.groups; ++j) {
       const V o = val[j];
       rank += o > v || (o == v && j < g);
@@ -160,6 +161,14 @@ __device__ __forceinline__ uint64_t keep_groups(const RouteArgs& a, const V* val
 #pragma unroll
   for (int o = 1; o < LANES; o *= 2) kept |= __shfl_xor(kept, o, 64);
   return kept;
+}
+// Order-preserving integer of a float's bits, and back.
+__device__ __forceinline__ int ordered(int b) { return b ^ ((b >> 31) & 0x7fffffff); }
+__device__ __forceinline__ int row_max(int v) {
+  v = max(v, across<1>(v));
+  v = max(v, across<2>(v));
+  v = max(v, across<4>(v));
+  return max(v, across<8>(v));
 }
 __device__ __forceinline__ int64_t row_max(int64_t v) {
   auto step = [&](auto s) {
@@ -196,6 +205,7 @@ __device__ __forceinline__ void rank64(const RouteArgs& a, RouteLds& s, const fl
     for (int g = sub; g < a.groups; g += LANES) {
       double b1 = -INFINITY, b2 = -INFINITY;
       bool nan = false;
+#pragma unroll 4
       for (int j = 0; j < gs; ++j) {
         const double v = __longlong_as_double(s.key[g * gs + j]);
         nan |= v != v;
@@ -240,7 +250,8 @@ __device__ __forceinline__ void rank64(const RouteArgs& a, RouteLds& s, const fl
 // One workgroup per histogram block, its waves independent of each other; 16 lanes hold a
 // token, EPL experts each.  The time is that of one token's chain of dependent steps, so a
 // wave works on four and a workgroup on 64 at once: 16384 tokens, 64 experts, 8 groups, top-8
-// XX us (64 lanes a token, four tokens a wave one after the other: 27).
+// 12.9 us (64 lanes a token, four tokens a wave one after the other: 27), 64 tokens 5.5; with
+// choices so far apart that no token needs the 64-bit order 8.5 and 5.5.
 template <int EPL>
 __global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
   __shared__ RouteLds lds[64];
@@ -284,6 +295,7 @@ __global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
       wave_lds_fence();
       for (int g = sub; g < a.groups; g += LANES) {
         float v = -INFINITY, b2 = -INFINITY;
+#pragma unroll 8
         for (int j = 0; j < gs; ++j) {
           const float u = cv[g * gs + j];
           b2 = fmaxf(b2, fminf(v, u));
@@ -304,34 +316,42 @@ __global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
         if (!((kept >> ((sub * EPL + i) / gs)) & 1)) x[i] = -INFINITY;
       wave_lds_fence();
     }
-    // k rounds of the largest choice, and one more for the gap behind the last
-    int rank[EPL];
+    // k rounds of the largest choice, and one more for the gap behind the last, on integers of
+    // the floats' order.  Equal choices go in one round: more than k are then gone.
+    int rank[EPL], key[EPL];
 #pragma unroll
-    for (int i = 0; i < EPL; ++i) rank[i] = MAX_K;
-    float last = 0.0f;
-    const int rounds = a.k < a.E ? a.k + 1 : a.k;
-    for (int r = 0; r < rounds; ++r) {
-      float m = x[0];
-#pragma unroll
-      for (int i = 1; i < EPL; ++i) m = fmaxf(m, x[i]);
-      const float best = group_top<LANES>(m);
-      const uint32_t at = (uint32_t)(__ballot(m == best) >> base) & 0xffffu;
-      sure = sure && (r == 0 || last - best > 2.0f * err) && (r == a.k || best > -INFINITY);
-      last = best;
-      if (sub == __builtin_ctz(at | 0x10000u)) {
-        bool done = false;
-#pragma unroll
-        for (int i = 0; i < EPL; ++i)
-          if (!done && x[i] == best) {
-            done = true;
-            x[i] = -INFINITY;
-            if (r < a.k) {
-              rank[i] = r;
-              s.pick[r] = sc[i];
-            }
-          }
-      }
+    for (int i = 0; i < EPL; ++i) {
+      rank[i] = MAX_K;
+      key[i] = ordered(__float_as_int(x[i]));
     }
+    float last = INFINITY;
+    auto round = [&](int r, bool take) {
+      int m = key[0];
+#pragma unroll
+      for (int i = 1; i < EPL; ++i) m = max(m, key[i]);
+      m = row_max(m);
+      const float best = __int_as_float(ordered(m));
+      sure = sure && last - best > 2.0f * err && (best > -INFINITY || !take);
+      last = best;
+      if (take) {
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) {
+          const bool hit = key[i] == m;
+          rank[i] = hit ? r : rank[i];
+          key[i] = hit ? INT_MIN : key[i];
+        }
+      }
+    };
+    for (int r = 0; r < a.k; ++r) round(r, true);
+    if (a.k < a.E) round(a.k, false);
+    float gone = 0.0f;
+#pragma unroll
+    for (int i = 0; i < EPL; ++i)
+      if (rank[i] < a.k) {
+        gone += 1.0f;
+        s.pick[rank[i]] = sc[i];
+      }
+    sure = sure && group_sum<LANES>(gone) == (float)a.k;
     wave_lds_fence();
     if (__any(live && !sure)) rank64<EPL>(a, s, l, b, sub, gs, base, rank);
 #pragma unroll
