@@ -10,7 +10,8 @@
 // 32 (l / 32) .. + 31 as 16 bytes at 16 l, the even K in the low nibble.  A weight tile is
 // 256 rows; per 128 of K it holds its eight 32-row blocks, each with its two K halves: 16
 // KiB, and the tile's steps follow each other, so a product streams memory in order.  The
-// scales of the same tile step are 1 KiB: per 32-row block and lane two bytes (the K halves).
+// scales of the same tile step are 1 KiB: 16 bytes, one for each 16 weight rows of the tile, of
+// row r of those and K 32 b .. at 16 (16 b + r), so one load of a lane has all that it needs.
 //   w13: E x Fp/128 tiles x dk/128 steps; block 2 j holds 32 gate columns, 2 j + 1 the up
 //        columns of the same f (so a wave that owns both has h in its registers)
 //   w3:  E x dp/256 tiles x Fp/128 steps; block j holds output columns 32 j ..

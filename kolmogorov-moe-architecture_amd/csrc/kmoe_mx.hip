@@ -198,7 +198,7 @@ __global__ __launch_bounds__(256) void pack_mx_kernel(const void* __restrict__ w
       const Codes<true, BLOCK> d = encode<true, BLOCK>(v, code);
       *reinterpret_cast<i32x4_t*>(q + ts * TILE_STEP + blk * 2048 + sub * 1024 + (lane + c) * 16) =
           i32x4_t{(int)d.w[0], (int)d.w[1], (int)d.w[2], (int)d.w[3]};
-      scale[ts * SCALE_STEP + blk * 128 + (lane + c) * 2 + sub] = (uint8_t)code;
+      scale[ts * SCALE_STEP + ((b & 3) * 16 + (n0 & 15) + c) * 16 + 2 * blk + (n0 >> 4 & 1)] = (uint8_t)code;
     }
   }
 }

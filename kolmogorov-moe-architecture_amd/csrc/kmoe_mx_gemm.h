@@ -132,27 +132,19 @@ __device__ __forceinline__ i32x4_t merge_runs(i32x2_t x, i32x2_t y) {
   return i32x4_t{(int)a0, (int)b0, (int)a1, (int)b1};
 }
 
-// Stores a row's 32 values, 16 a lane (v[4 c + t]: column 8 c + 4 half + t), as an MX block.
+// Stores a row's 32 values, 16 a lane (v[4 c + t]: column 8 c + 4 half + t), as an e2m1 block.
 // q: the block's codes, scale: its byte; nothing is stored where !on.  All lanes take part.
-template <bool FP4>
 __device__ __forceinline__ void store_block(const float (&v)[16], int half, bool on, uint8_t* q, uint8_t* scale) {
   uint32_t m = 0, o0, o1;
 #pragma unroll
   for (int i = 0; i < 16; ++i) m = amax_bits(m, v[i]);
   swap_halves(m, m, o0, o1);  // its own and its partner's
-  const uint32_t code = scale_code<FP4>(max(o0, o1));
-  const Codes<FP4, 16> d = encode<FP4, 16>(v, code);
-  if constexpr (FP4) {
-    // d.w[p]: runs 2 p (low 16 bits) and 2 p + 1
-    uint32_t a, b;
-    swap_halves(d.w[0], d.w[1], a, b);
-    if (on) *reinterpret_cast<i32x2_t*>(q + 8 * half) = i32x2_t{(int)((a & 0xffffu) | (b << 16)), (int)((a >> 16) | (b & 0xffff0000u))};
-  } else {
-    uint32_t a0, a1, b0, b1;
-    swap_halves(d.w[0], d.w[2], a0, a1);
-    swap_halves(d.w[1], d.w[3], b0, b1);
-    if (on) *reinterpret_cast<i32x4_t*>(q + 16 * half) = i32x4_t{(int)a0, (int)a1, (int)b0, (int)b1};
-  }
+  const uint32_t code = scale_code<true>(max(o0, o1));
+  const Codes<true, 16> d = encode<true, 16>(v, code);
+  // d.w[p]: runs 2 p (low 16 bits) and 2 p + 1
+  uint32_t a, b;
+  swap_halves(d.w[0], d.w[1], a, b);
+  if (on) *reinterpret_cast<i32x2_t*>(q + 8 * half) = i32x2_t{(int)((a & 0xffffu) | (b << 16)), (int)((a >> 16) | (b & 0xffff0000u))};
   if (on && half == 0) *scale = (uint8_t)code;
 }
 
@@ -170,14 +162,14 @@ struct MxTile {
 };
 
 template <bool GATE_UP, bool FP4, int MI, int NJ, bool SAVE_GU>
-__global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) {
+__global__ __launch_bounds__(GEMM_THREADS, 2) void mx_gemm_kernel(MxGemmArgs g) {
   using T = MxTile<GATE_UP, FP4, MI, NJ, SAVE_GU>;
   static_assert(!SAVE_GU || GATE_UP, "gate / up values are the first product's");
   constexpr int NST = T::NST;
   __shared__ __attribute__((aligned(1024))) uint8_t lds[T::LDS];
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int lr = lane & 31, lh = lane >> 5;
+  const int lr = lane & 31, lh = lane >> 5, l16 = lane & 15, lq = lane >> 4;
   const int wm = wave >> 1, wn = wave & 1;
 
   // tile: each XCD (workgroups go round over the 8) takes a contiguous range of the tiles, in
@@ -210,7 +202,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   const i32x4_t sr = gather ? buffer_of(g.a_scale, g.a_rows * lds_a) : buffer_of(g.a_scale + m0 * lds_a, rows * lds_a);
   const int64_t bt = ((int64_t)e * g.b_tiles + ct / SPLIT) * g.k_steps;
   const i32x4_t br = buffer_of(g.b + bt * TILE_STEP + (ct % SPLIT) * T::BB, (int64_t)g.k_steps * TILE_STEP - (ct % SPLIT) * T::BB);
-  const i32x4_t tr = buffer_of(g.b_scale + bt * SCALE_STEP + (ct % SPLIT) * T::BS, (int64_t)g.k_steps * SCALE_STEP - (ct % SPLIT) * T::BS);
+  const i32x4_t tr = buffer_of(g.b_scale + bt * SCALE_STEP, (int64_t)g.k_steps * SCALE_STEP);
   constexpr uint32_t NONE = 0x80000000u;  // an offset past every window
   auto source_row = [&](int r) -> uint32_t {  // row of `a` (or of the slot) that tile row r is; NONE without one
     if (r >= rows) return NONE;
@@ -230,7 +222,9 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   }
   const uint32_t ssrc = wave < MI ? source_row(wave * 64 + lane) : NONE;
   const uint32_t soff = ssrc == NONE ? NONE : ssrc * (uint32_t)lds_a;
-  const uint32_t boff = wave * T::NB * 1024 + lane * 16, toff = (wave % NJ) * 256 + lane * 4;
+  const uint32_t boff = wave * T::NB * 1024 + lane * 16;
+  const int ti = (wave % NJ) * 64 + lane;  // dword of the column tile's scales: NJ of each of 64
+  const uint32_t toff = (ti / NJ) * 16 + (ct % SPLIT) * NJ * 4 + (ti % NJ) * 4;
   const uint32_t lds0 = (uint32_t)(uintptr_t)(KMOE_LDS uint8_t*)lds;
 
   // load `q` of step k into the stage at byte offset st: A rows, weights, their scales (two
@@ -255,51 +249,85 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
                       __builtin_amdgcn_readfirstlane(lds0 + NST * T::STAGE + ((k >> 2) & 1) * T::AS + wave * 1024));
   };
 
-  f32x16_t acc[MI][NJ];
+  // e2m1 rows: 32 x 32 results, the operands of the two K halves of a step.  e4m3 rows: 16 x 16
+  // results, all of a step's weights and the rows in two parts.  In both a step has two phases,
+  // and the second one's operands are read under the first one's products.
+  constexpr int RB = 2 * MI, CB = 2 * NJ;            // 16-row blocks of rows and weights of a wave
+  constexpr int NM = FP4 ? MI * NJ : MI * CB;        // products of a phase
+  constexpr int NR = FP4 ? NJ + MI : 2 * MI;         // reads of a phase's operands (e4m3: of its rows)
+  constexpr int NS = FP4 ? 2 + MI : 1 + RB;          // reads of a step's scales
+  constexpr int SW = NJ / 2;                         // scale words of a lane
+  f32x16_t acc[FP4 ? MI : 1][FP4 ? NJ : 1];
+  f32x4_t acc4[FP4 ? 1 : RB][FP4 ? 1 : CB];
+  if constexpr (FP4) {
 #pragma unroll
-  for (int i = 0; i < MI; ++i)
+    for (int i = 0; i < MI; ++i)
 #pragma unroll
-    for (int j = 0; j < NJ; ++j)
+      for (int j = 0; j < NJ; ++j)
 #pragma unroll
-      for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-
-  // Operands of the two K halves of a step, and the step's scales (s: of the half about to be
-  // multiplied first, s2 their copy for the second)
-  constexpr int PER_A = FP4 ? 1 : 2;                // LDS reads of an A fragment
-  constexpr int NR = NJ + MI * PER_A, NS = NJ + MI;  // reads of a half's operands, of the scales
-  i32x4_t fa[2][MI][PER_A], fb[2][NJ];
-  int sa[MI], sb[NJ], sa2[MI], sb2[NJ];
-  auto read_one = [&](auto r_tag, auto half_tag, uint32_t st) {  // operand read r of half i
+        for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+  } else {
+#pragma unroll
+    for (int i = 0; i < RB; ++i)
+#pragma unroll
+      for (int j = 0; j < CB; ++j) acc4[i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
+  }
+  i32x4_t fa[2][FP4 ? MI : 2 * MI];  // [phase]; e4m3: [block 2 i, its K 64 .. 127 at 2 i + 1]
+  i32x4_t fb[FP4 ? 2 : 1][FP4 ? NJ : CB];
+  // scales: of the step about to begin; *2: of the second phase's products, once the first is over
+  uint32_t sb[FP4 ? 2 : 1][SW], sb2[SW];
+  int sa[FP4 ? MI : RB], sa2[MI];
+  auto read_one = [&](auto r_tag, auto half_tag, uint32_t st) {  // operand read r of phase i
     constexpr int r = decltype(r_tag)::value, i = decltype(half_tag)::value;
-    if constexpr (r < NJ) {
+    if constexpr (!FP4) {
+      const int row = wm * 32 * MI + (i * MI + r / 2) * 16 + l16;
+      fa[i][r] = *reinterpret_cast<const i32x4_t*>(lds + st + a_lds<FP4>(row, lq + 4 * (r % 2)));
+    } else if constexpr (r < NJ) {
       fb[i][r] = *reinterpret_cast<const i32x4_t*>(lds + st + T::AB + (wn * NJ + r) * 2048 + i * 1024 + lane * 16);
     } else {
-      constexpr int mi = (r - NJ) / PER_A, part = (r - NJ) % PER_A;
-      const int row = wm * 32 * MI + mi * 32 + lr;
-      fa[i][mi][part] = *reinterpret_cast<const i32x4_t*>(lds + st + a_lds<FP4>(row, FP4 ? 2 * i + lh : 4 * i + 2 * part + lh));
+      const int row = wm * 32 * MI + (r - NJ) * 32 + lr;
+      fa[i][r - NJ] = *reinterpret_cast<const i32x4_t*>(lds + st + a_lds<FP4>(row, 2 * i + lh));
     }
+  };
+  auto read_weights = [&](auto c_tag, uint32_t st) {  // e4m3: the 16 weight rows c
+    constexpr int c = decltype(c_tag)::value;
+    fb[0][c] = *reinterpret_cast<const i32x4_t*>(lds + st + T::AB + (wn * NJ + c / 2) * 2048 + (lq >> 1) * 1024 +
+                                                 ((lq & 1) * 32 + (c % 2) * 16 + l16) * 16);
   };
   auto read_scale = [&](auto r_tag, int k, uint32_t st) {
     constexpr int r = decltype(r_tag)::value;
-    if constexpr (r < NJ) {
-      sb[r] = *reinterpret_cast<const uint16_t*>(lds + st + T::AB + T::BB + (wn * NJ + r) * 128 + lane * 2);
+    const uint8_t* const sp = lds + NST * T::STAGE + ((k >> 2) & 1) * T::AS + (k & 3) * 4 + wm * 512 * MI;
+    if constexpr (r < (FP4 ? 2 : 1)) {
+      // (e2m1: K 32 (2 r + lh) .. of weight row lr of each block, its 16-row half by a shift)
+      const uint8_t* const p = lds + st + T::AB + T::BB + (FP4 ? 32 * r + 16 * lh + (lr & 15) : lane) * 4 * NJ + wn * 2 * NJ;
+#pragma unroll
+      for (int w = 0; w < SW; ++w) sb[r][w] = reinterpret_cast<const uint32_t*>(p)[w] >> (FP4 ? 8 * (lr >> 4) : 0);
+    } else if constexpr (FP4) {
+      sa[r - 2] = (int)(*reinterpret_cast<const uint32_t*>(sp + ((r - 2) * 32 + lr) * 16) >> (8 * lh));
     } else {
-      const uint8_t* const sp = lds + NST * T::STAGE + ((k >> 2) & 1) * T::AS + (k & 3) * 4;
-      sa[r - NJ] = (int)(*reinterpret_cast<const uint32_t*>(sp + (wm * 32 * MI + (r - NJ) * 32 + lr) * 16) >> (8 * lh));
+      sa[r - 1] = sp[((r - 1) * 16 + l16) * 16 + lq];
     }
   };
   auto mma_one = [&](auto g_tag, auto half_tag) {
-    constexpr int g = decltype(g_tag)::value, i = decltype(half_tag)::value, mi = g / NJ, j = g % NJ;
-    const i32x4_t b = fb[i][j], a0 = fa[i][mi][0], a1 = FP4 ? i32x4_t{0, 0, 0, 0} : fa[i][mi][PER_A - 1];
-    acc[mi][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-        i32x8_t{b[0], b[1], b[2], b[3], 0, 0, 0, 0}, i32x8_t{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]},
-        acc[mi][j], 4, FP4 ? 4 : 0, i, i ? sb2[j] : sb[j], 2 * i, i ? sa2[mi] : sa[mi]);
+    constexpr int g = decltype(g_tag)::value, i = decltype(half_tag)::value;
+    if constexpr (FP4) {
+      constexpr int mi = g / NJ, j = g % NJ;
+      const i32x4_t b = fb[i][j], a = fa[i][mi];
+      acc[mi][j] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+          i32x8_t{b[0], b[1], b[2], b[3], 0, 0, 0, 0}, i32x8_t{a[0], a[1], a[2], a[3], 0, 0, 0, 0}, acc[mi][j], 4, 4,
+          2 * (j & 1), i ? sb2[j >> 1] : sb[0][j >> 1], 2 * i, i ? sa2[mi] : sa[mi]);
+    } else {
+      constexpr int c = g / MI, m = g % MI;
+      const i32x4_t b = fb[0][c], a0 = fa[i][2 * m], a1 = fa[i][2 * m + 1];
+      acc4[i * MI + m][c] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
+          i32x8_t{b[0], b[1], b[2], b[3], 0, 0, 0, 0}, i32x8_t{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]},
+          acc4[i * MI + m][c], 4, 0, c & 3, i ? sb2[c >> 2] : sb[0][c >> 2], 0, i ? sa2[m] : sa[m]);
+    }
   };
   // The K loop is emitted in program order: each MFMA with the LDS reads and loads assigned to
   // it, fenced with sched_barrier (left alone, the compiler moves the MFMAs of two steps
   // behind all their reads and spills).  op(n): operation n of `count`, spread over the MFMAs
   // [0, last).
-  constexpr int NM = MI * NJ;
   auto spread = [&](auto g_tag, auto count_tag, auto last_tag, auto&& op) {
     constexpr int g = decltype(g_tag)::value, count = decltype(count_tag)::value, last = decltype(last_tag)::value;
     if constexpr (g < last)
@@ -321,6 +349,7 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   });
   barrier_nofence();
   static_for<0, NR>([&](auto r) { read_one(r, H0{}, 0); });
+  if constexpr (!FP4) static_for<0, CB>([&](auto c) { read_weights(c, 0); });
   static_for<0, NS>([&](auto r) { read_scale(r, 0, 0); });
   uint32_t cur = 0;  // byte offset of the step's stage
   // Step kt: its first half is in registers.  Its second half is read under the first half's
@@ -345,9 +374,9 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
       __builtin_amdgcn_sched_barrier(0);
     });
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) sb2[j] = sb[j];
+    for (int w = 0; w < SW; ++w) sb2[w] = sb[FP4 ? 1 : 0][w];
 #pragma unroll
-    for (int mi = 0; mi < MI; ++mi) sa2[mi] = sa[mi];
+    for (int mi = 0; mi < MI; ++mi) sa2[mi] = sa[FP4 ? mi : MI + mi];
     if constexpr (WAIT >= 0) {
       wait_lgkmcnt0();
       // (with one load more where a step of those began with row scales)
@@ -362,6 +391,9 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
     __builtin_amdgcn_sched_barrier(0);
     static_for<0, NM>([&](auto gt) {
       mma_one(gt, H1{});
+      // (e4m3: weights whose last product this was make room for the next step's)
+      if constexpr (WAIT >= 0 && !FP4 && gt % MI == MI - 1)
+        read_weights(std::integral_constant<int, gt / MI>{}, nxt);
       if constexpr (WAIT >= 0)
         spread(gt, std::integral_constant<int, NR + NS>{}, std::integral_constant<int, (NM * 3 + 3) / 4>{}, [&](auto n) {
           if constexpr (n < NR)
@@ -392,21 +424,23 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
   });
   step(kt, No{}, No{}, std::integral_constant<int, -1>{});
 
-  // ---- epilogue: lane's row of block mi, columns 8 c + 4 lh + t of block j
+  // ---- epilogue.  e2m1 rows: the lane's row of 32-row block mi, columns 8 c + 4 lh + t of
+  // block j.  e4m3 rows: its row of 16-row block rb, columns 4 lq + t of 16-column block c.
+  // Where a wave's 32 rows (e4m3 h: all its rows) go through LDS, a store instruction writes
+  // whole pieces of few rows and not 32 or 8 bytes of each.
+  if constexpr (GATE_UP && FP4) {
 #pragma unroll
-  for (int mi = 0; mi < MI; ++mi) {
-    const int r = wm * 32 * MI + mi * 32 + lr;
-    const bool on = r < rows;
-    const int64_t row = m0 + r;
-    if constexpr (GATE_UP) {
+    for (int mi = 0; mi < MI; ++mi) {
+      const int r = wm * 32 * MI + mi * 32 + lr;
+      const bool on = r < rows;
+      const int64_t row = m0 + r;
 #pragma unroll
       for (int p = 0; p < NJ / 2; ++p) {
         const int f0 = (ct * 2 * NJ + wn * NJ) * 16 + p * 32;  // first of the block's 32 columns
         float h[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) h[i] = silu_fast_f32(acc[mi][2 * p][i]) * acc[mi][2 * p + 1][i];
-        store_block<FP4>(h, lh, on, g.q + row * (g.ldc / (FP4 ? 2 : 1)) + f0 / (FP4 ? 2 : 1),
-                         g.q_scale + row * scale_bytes((int)g.ldc) + f0 / BLOCK);
+        store_block(h, lh, on, g.q + row * (g.ldc / 2) + f0 / 2, g.q_scale + row * scale_bytes((int)g.ldc) + f0 / BLOCK);
         if constexpr (SAVE_GU) {
           uint16_t* const gp = g.gu + row * 2 * g.ldc + (f0 >> 7) * 256 + (f0 & 127) + 8 * lh;
 #pragma unroll
@@ -420,20 +454,81 @@ __global__ __launch_bounds__(GEMM_THREADS, 1) void mx_gemm_kernel(MxGemmArgs g) 
             }
         }
       }
-    } else {
-      // a wave's 32 x 128 values go through LDS, so that a store instruction writes four rows'
-      // 256 bytes and not 32 rows' 32 bytes
-      constexpr int OC = NJ * 4;  // 16-byte chunks of a row
-      uint8_t* const out = lds + wave * 32 * OC * 16;
-      if (mi == 0) barrier_nofence();  // the last step's operands are in registers
+    }
+  } else if constexpr (GATE_UP) {
+    // weight blocks of 32 rows are gate and up in turn: c 4 p, 4 p + 1 and 4 p + 2, 4 p + 3
+    uint8_t* const out = lds + wave * 32 * MI * 16 * NJ;
+    const int f00 = (ct * 2 * NJ + wn * NJ) * 16;  // the wave's first column of h
+    barrier_nofence();                             // the last step's operands are in registers
 #pragma unroll
-      for (int j = 0; j < NJ; ++j)
+    for (int rb = 0; rb < RB; ++rb) {
+      const int rr = rb * 16 + l16, r = wm * 32 * MI + rr;
+      const bool on = r < rows;
+      const int64_t row = m0 + r;
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const f32x16_t& a = acc[mi][j];
-          *reinterpret_cast<i32x2_t*>(out + ((lr * OC + ((4 * j + c) ^ (lr & (OC - 1)))) << 4) + 8 * lh) =
-              pack4_bf16(a[4 * c], a[4 * c + 1], a[4 * c + 2], a[4 * c + 3]);
+      for (int p = 0; p < NJ / 2; ++p) {
+        float h[8];
+        uint32_t m = 0, o0, o1;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          h[i] = silu_fast_f32(acc4[rb][4 * p + i / 4][i % 4]) * acc4[rb][4 * p + 2 + i / 4][i % 4];
+          m = amax_bits(m, h[i]);
         }
+        swap_halves(m, m, o0, o1);  // the block's 32 columns are 8 values in each of the row's four lanes
+        m = max(o0, o1);
+        const auto o = __builtin_amdgcn_permlane16_swap(m, m, false, false);
+        const uint32_t code = scale_code<false>(max((uint32_t)o[0], (uint32_t)o[1]));
+        const Codes<false, 8> d = encode<false, 8>(h, code);
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+          *reinterpret_cast<uint32_t*>(out + rr * 16 * NJ + (((2 * p + b) ^ ((rr >> 2) & (NJ - 1))) << 4) + 4 * lq) = d.w[b];
+        if (on && lq == 0) g.q_scale[row * scale_bytes((int)g.ldc) + f00 / BLOCK + p] = (uint8_t)code;
+        if constexpr (SAVE_GU) {
+          const int f0 = f00 + p * 32;
+          uint16_t* const gp = g.gu + row * 2 * g.ldc + (f0 >> 7) * 256 + (f0 & 127) + 4 * lq;
+          if (on)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const f32x4_t& a = acc4[rb][4 * p + i];
+              *reinterpret_cast<i32x2_t*>(gp + (i / 2) * 128 + (i % 2) * 16) = pack4_bf16(a[0], a[1], a[2], a[3]);
+            }
+        }
+      }
+    }
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    const int oc = lane % NJ;
+#pragma unroll
+    for (int q = 0; q < MI * NJ / 2; ++q) {
+      const int rr = 64 / NJ * q + lane / NJ, r = wm * 32 * MI + rr;
+      const i32x4_t v = *reinterpret_cast<const i32x4_t*>(out + rr * 16 * NJ + ((oc ^ ((rr >> 2) & (NJ - 1))) << 4));
+      if (r < rows) *reinterpret_cast<i32x4_t*>(g.q + (m0 + r) * g.ldc + f00 + 16 * oc) = v;
+    }
+  } else {
+    constexpr int OC = NJ * 4;  // 16-byte chunks of a row
+    uint8_t* const out = lds + wave * 32 * OC * 16;
+    barrier_nofence();  // the last step's operands are in registers
+#pragma unroll
+    for (int mi = 0; mi < MI; ++mi) {
+      auto put = [&](int rr, int c, int part, float a0, float a1, float a2, float a3) {
+        *reinterpret_cast<i32x2_t*>(out + ((rr * OC + (c ^ (rr & (OC - 1)))) << 4) + 8 * part) = pack4_bf16(a0, a1, a2, a3);
+      };
+      if constexpr (FP4) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const f32x16_t& a = acc[mi][j];
+            put(lr, 4 * j + c, lh, a[4 * c], a[4 * c + 1], a[4 * c + 2], a[4 * c + 3]);
+          }
+      } else {
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int c = 0; c < CB; ++c) {
+            const f32x4_t& a = acc4[2 * mi + b][c];
+            put(16 * b + l16, 2 * c + (lq >> 1), lq & 1, a[0], a[1], a[2], a[3]);
+          }
+      }
       __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
       const int oc = lane % OC, col = (ct * 2 * NJ + wn * NJ) * 32 + 8 * oc;
 #pragma unroll

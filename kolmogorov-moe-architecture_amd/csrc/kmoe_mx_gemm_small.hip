@@ -44,9 +44,9 @@ __global__ __launch_bounds__(64 * WAVES) void mx_small_kernel(MxGemmArgs g) {
   constexpr int PER_TILE = GATE_UP ? 4 : 8;  // column blocks of a weight tile
   const int64_t tile = ((int64_t)e * g.b_tiles + ct / PER_TILE) * nk;
   const uint8_t* const wq = g.b + tile * TILE_STEP + (ct % PER_TILE) * (GATE_UP ? 4096 : 2048);
-  const uint8_t* const ws = g.b_scale + tile * SCALE_STEP + (ct % PER_TILE) * (GATE_UP ? 256 : 128);
+  const uint8_t* const ws = g.b_scale + tile * SCALE_STEP + (ct % PER_TILE) * NB;
   const uint32_t woff = (q >> 1) * 1024 + ((q & 1) * 32 + r16) * 16;   // + 256 for the other 16 rows, + 2048 for up
-  const uint32_t soff = ((q & 1) * 32 + r16) * 2 + (q >> 1);           // + 32, + 128
+  const uint32_t soff = lane * 16;
   const int64_t lda = (int64_t)nk * (FP4 ? 64 : 128), lds_a = (int64_t)((nk + 3) / 4) * 16;
   const bool gather = GATE_UP && g.row_token;
   const uint8_t* const abase = gather ? g.a : g.a + m0 * lda;
@@ -62,15 +62,14 @@ __global__ __launch_bounds__(64 * WAVES) void mx_small_kernel(MxGemmArgs g) {
     constexpr int MB = decltype(mb_tag)::value;  // 16-row blocks with rows
     constexpr int PA = FP4 ? 1 : 2;
     i32x4_t w[DEPTH][NB], a[DEPTH][MB][PA];
-    int sw[DEPTH][NB], sa[DEPTH][MB];
+    int sw[DEPTH], sa[DEPTH][MB];
     // step s into ring entry u; steps past the wave's range read nothing (empty windows)
     auto load_w = [&](int u, int s) {
       const __amdgpu_buffer_rsrc_t rw = window(wq, s < s1 ? 0x7fffffff : 0), rs = window(ws, s < s1 ? 0x7fffffff : 0);
 #pragma unroll
-      for (int b = 0; b < NB; ++b) {
-        w[u][b] = load16(rw, woff + (b & 1) * 256 + (b >> 1) * 2048, s * TILE_STEP);
-        sw[u][b] = __builtin_amdgcn_raw_buffer_load_b8(rs, soff + (b & 1) * 32 + (b >> 1) * 128, s * SCALE_STEP, 0);
-      }
+      for (int b = 0; b < NB; ++b) w[u][b] = load16(rw, woff + (b & 1) * 256 + (b >> 1) * 2048, s * TILE_STEP);
+      sw[u] = GATE_UP ? (int)__builtin_amdgcn_raw_buffer_load_b32(rs, soff, s * SCALE_STEP, 0)
+                      : (int)__builtin_amdgcn_raw_buffer_load_b16(rs, soff, s * SCALE_STEP, 0);
     };
     uint32_t aoff[MB], asoff[MB];
     auto load_a = [&](int u, int s) {
@@ -100,13 +99,12 @@ __global__ __launch_bounds__(64 * WAVES) void mx_small_kernel(MxGemmArgs g) {
         // entries past the range hold zeros (codes and scales)
 #pragma unroll
         for (int m = 0; m < MB; ++m)
-#pragma unroll
-          for (int b = 0; b < NB; ++b) {
+          static_for<0, NB>([&](auto b) {
             const i32x4_t wv = w[u][b], a0 = a[u][m][0], a1 = FP4 ? i32x4_t{0, 0, 0, 0} : a[u][m][PA - 1];
             acc[m][b] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(
                 i32x8_t{wv[0], wv[1], wv[2], wv[3], 0, 0, 0, 0}, i32x8_t{a0[0], a0[1], a0[2], a0[3], a1[0], a1[1], a1[2], a1[3]},
-                acc[m][b], 4, FP4 ? 4 : 0, 0, sw[u][b], 0, sa[u][m]);
-          }
+                acc[m][b], 4, FP4 ? 4 : 0, decltype(b)::value, sw[u], 0, sa[u][m]);
+          });
         load_w(u, s + u + DEPTH);
         load_a(u, s + u + DEPTH);
       }
