@@ -5,19 +5,29 @@
 // for the rows r of expert e, [offsets[e], offsets[e+1]).  x and h are e4m3 (w4a8) or e2m1
 // (w4a4) rows with one scale per 32 values, the weights are packed e2m1 (kmoe_mx.h).
 //
-// v_mfma_scale_f32_32x32x64_f8f6f4 takes both operands' codes and their scale bytes, so a
-// block's scales cost no arithmetic.  Operand layout (lane l, row l % 32, half h = l / 32):
-// e2m1 holds K 32 h .. + 31; e4m3 holds K 16 h .. + 15 and 32 + 16 h .. + 15; the scale byte
-// of lane half h is that of K 32 h .. + 31 in both.  Weights are the first operand, so a
-// lane's results are four consecutive output columns 8 c + 4 h .. of one row, c = 0 .. 3: a
-// 32-column MX block of h is the 16 results of a lane and of its partner half.
+// v_mfma_scale_f32_* takes both operands' codes and their scale bytes, so a block's scales cost
+// no arithmetic.  Weights are the first operand.  Operand layouts:
+//   e2m1 rows  32x32x64, the faster shape for two 4-bit operands (6.8 PFLOP/s of products alone,
+//              16x16x128 4.6).  Lane l, row l % 32, half h = l / 32 holds K 32 h .. + 31 and its
+//              scale byte; its results are the output columns 8 c + 4 h .. + 3 of one row, c = 0
+//              .. 3: a 32-column MX block of h is the 16 results of a lane and its partner half.
+//   e4m3 rows  16x16x128 (4.1, 32x32x64 3.6).  Lane l, row l % 16, q = l / 16 holds K 32 q .. +
+//              31 of the weights, K 16 q .. + 15 and 64 + 16 q .. + 15 of the rows, the scale byte
+//              of K 32 q .. of both; its results are columns 4 q .. + 3 of one row.
 //
 // A workgroup of 2 x 2 waves owns 64 MI rows x 64 NJ weight rows, a wave 32 MI x 32 NJ.  (256
 // rows by 4 x 2 waves load a quarter less, but leave one workgroup a CU: 16384 rows, top-2 of 16
-// experts, d 2048, F 2816, gate/up 340 us in w4a8 against 330, 236 in w4a4 against 227.)  Both
-// operands go global -> LDS directly, 128 of K per step, in as many stages up to three as let
-// two workgroups share a CU (with four and five of the small tiles nothing gained); the K loop
-// has one barrier per step, placed where every wave has the step's last fragments in registers.
+// experts, d 2048, F 2816, gate/up 340 us in w4a8 against 330 then, 236 in w4a4 against 227.)
+// Both operands go global -> LDS directly, 128 of K per step, in as many stages up to three as
+// let two workgroups share a CU (with four and five of the small tiles nothing gained); the K
+// loop has one barrier per step, placed where every wave has the step's last fragments in
+// registers.
+//
+// At that size gate/up takes 308 us in w4a8 (2.45 PFLOP/s) and 218 in w4a4 (3.47), down 156 and
+// 111; d 4096 572 and 400, 308 and 228.  In w4a8 with 32 x 32 products, d 4096 (593 and 331
+// then): without the loads in the loop 450 and 181, without the LDS reads 554 and 321, without
+// the epilogue 550 and 264, without all three 401 and 200: the loads cost most, more by the power
+// they draw (the clock falls from 2.4 to 1.8 .. 2.1 GHz) than by waiting.
 #pragma once
 
 #include <type_traits>

@@ -14,12 +14,12 @@ namespace {
 // weights: with e2m1 rows where the experts have more than 64 and the tiles fill the CUs; with
 // e4m3 rows, of which two workgroups fit a CU with two LDS stages only, from 5 tiles a CU.  us
 // for 64x128 / 64x256 / 128x256, weights from HBM, (tiles a CU): top-2 of 16, d 2048, F 2816,
-// e4m3: down, 48 tokens (0.5) 13.3 / 15.0 / 27; 777 (1) 22 / 24 / 28; 2042 (2.2) 35 / 35 / 38;
-// gate/up, 48 (1.4) 21.7 / 22.3 / 29; 1024 (3.4) 44 / 39 / 49; 2042 (6.2) 66 / 60 / 60; 4096
-// (12) 117 / 103 / 101; e2m1: down, 500 (0.8) 17.1 / 15.0 / 17.7; 777 (1) 20.7 / 22 / 18.3; 2042
-// 33 / 32 / 32; gate/up, 777 (2.8) 33 / 33 / 29; 2042 54 / 52 / 47.  Top-6 of 64, d 1024, F 704,
-// gate/up: e4m3, 400 (1.6) 17.2 / 15.3 / 18.9; 2000 (5.1) 35 / 32 / 31; e2m1, 400 15.1 / 14.4 /
-// 17.4; 1000 (93 rows an expert, 2.9) 19.4 / 19.4 / 18.0.
+// e4m3: down, 48 tokens (0.5) 13.8 / 15.6 / 27; 777 (1) 22.5 / 23.5 / 28; 2042 (2.2) 36 / 35 /
+// 37; gate/up, 48 (1.4) 22.6 / 22.3 / 30; 1024 (3.4) 43 / 39 / 48; 2042 (6.2) 63 / 58 / 58; 4096
+// (12) 115 / 97 / 99; e2m1: down, 500 (0.8) 17.4 / 15.3 / 17.5; 777 (1) 21.5 / 22 / 18; 2042 33 /
+// 31 / 32; gate/up, 777 (2.8) 34 / 32 / 27; 2042 55 / 51 / 45.  Top-6 of 64, d 1024, F 704,
+// gate/up: e4m3, 400 (1.6) 17.6 / 15.3 / 19.6; 2000 (5.1) 34 / 31 / 31; e2m1, 400 15.5 / 14.7 /
+// 17.1; 1000 (93 rows an expert, 2.9) 19.1 / 19.2 / 18.8.
 MxTileSize tile_size(bool fp4, int64_t max_rows, int E, int b_tiles) {
   const int64_t used = std::min<int64_t>(max_rows, E), tiles = std::max(used, max_rows / 64 + used / 2) * b_tiles;
   const int64_t cu = kmoe::cu_count();
@@ -29,11 +29,11 @@ MxTileSize tile_size(bool fp4, int64_t max_rows, int E, int b_tiles) {
 
 // Whether a product runs on the small-row kernel (kmoe_mx_gemm_small.hip): where its grid is at
 // most two workgroups per CU, as latency then counts, at few rows per expert.  us, small-row
-// kernel / 64 x 128 tiles, e4m3 (workgroups): top-2 of 16 experts, d 2048, F 2816, down, 1 token
-// (128) 7.3 / 9.8, 4 (512) 7.7 / 9.9, 16 (1088) 12.9 / 10.7; gate/up, 1 (176) 9.3 / 10.1, 4
-// (704) 14.5 / 11.1, 48 (1672) 31 / 19.4; top-2 of 8, d 4096, F 1408, gate/up, 4 (352) 9.9 /
-// 13.5, 48 (484) 15.3 / 14.4: each workgroup looks its slot up and reduces, which the tiles do
-// once for four times the weights.
+// kernel / 64 x 128 tiles, e4m3, weights from HBM (workgroups): top-2 of 16 experts, d 2048, F
+// 2816, down, 1 token (128) 4.9 / 9.8, 4 (512) 8.0 / 10.0, 16 (1088) 14.9 / 13.3; gate/up, 1
+// (176) 6.5 / 9.0, 2 (352) 9.7 / 9.1, 4 (704) 14.1 / 12.6, 48 (1672) 31 / 22; top-2 of 8, d 4096,
+// F 1408, gate/up, 4 (352) 9.5 / 18.3, 48 (484) 18.0 / 20.1, 100 (616) 23.5 / 20.1: each
+// workgroup looks its slot up and reduces, which the tiles do once for four times the weights.
 bool small_product(bool gate_up, int64_t max_rows, int E, int b_tiles) {
   const int64_t slots = max_rows / SMALL_ROWS + std::min<int64_t>(max_rows, E);
   return max_rows <= 32 * (int64_t)E && slots * b_tiles * (gate_up ? 4 : 8) <= 2 * kmoe::cu_count();
