@@ -142,6 +142,14 @@ __device__ __forceinline__ i32x4_t merge_runs(i32x2_t x, i32x2_t y) {
   return i32x4_t{(int)a0, (int)b0, (int)a1, (int)b1};
 }
 
+// Eight consecutive bf16 columns from the lane's four (quarter q of the wave: 4 q ..) of two
+// 16-column blocks: even quarters 4 q .. 4 q + 7 of the first, odd ones 4 (q - 1) .. of the second.
+__device__ __forceinline__ i32x4_t merge_quads(i32x2_t x, i32x2_t y) {
+  const auto a = __builtin_amdgcn_permlane16_swap((uint32_t)x[0], (uint32_t)y[0], false, false);
+  const auto b = __builtin_amdgcn_permlane16_swap((uint32_t)x[1], (uint32_t)y[1], false, false);
+  return i32x4_t{(int)a[0], (int)b[0], (int)a[1], (int)b[1]};
+}
+
 // Stores a row's 32 values, 16 a lane (v[4 c + t]: column 8 c + 4 half + t), as an e2m1 block.
 // q: the block's codes, scale: its byte; nothing is stored where !on.  All lanes take part.
 __device__ __forceinline__ void store_block(const float (&v)[16], int half, bool on, uint8_t* q, uint8_t* scale) {
@@ -495,13 +503,13 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void mx_gemm_kernel(MxGemmArgs g) 
         if (on && lq == 0) g.q_scale[row * scale_bytes((int)g.ldc) + f00 / BLOCK + p] = (uint8_t)code;
         if constexpr (SAVE_GU) {
           const int f0 = f00 + p * 32;
-          uint16_t* const gp = g.gu + row * 2 * g.ldc + (f0 >> 7) * 256 + (f0 & 127) + 4 * lq;
-          if (on)
+          uint16_t* const gp = g.gu + row * 2 * g.ldc + (f0 >> 7) * 256 + (f0 & 127) + (lq & 1) * 16 + (lq >> 1) * 8;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const f32x4_t& a = acc4[rb][4 * p + i];
-              *reinterpret_cast<i32x2_t*>(gp + (i / 2) * 128 + (i % 2) * 16) = pack4_bf16(a[0], a[1], a[2], a[3]);
-            }
+          for (int u = 0; u < 2; ++u) {
+            const f32x4_t &a = acc4[rb][4 * p + 2 * u], &b = acc4[rb][4 * p + 2 * u + 1];
+            const i32x4_t v = merge_quads(pack4_bf16(a[0], a[1], a[2], a[3]), pack4_bf16(b[0], b[1], b[2], b[3]));
+            if (on) *reinterpret_cast<i32x4_t*>(gp + u * 128) = v;
+          }
         }
       }
     }
