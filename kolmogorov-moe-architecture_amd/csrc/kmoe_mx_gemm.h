@@ -26,8 +26,9 @@
 // At that size gate/up takes 308 us in w4a8 (2.45 PFLOP/s) and 218 in w4a4 (3.47), down 156 and
 // 111; d 4096 572 and 400, 308 and 228.  In w4a8 with 32 x 32 products, d 4096 (593 and 331
 // then): without the loads in the loop 450 and 181, without the LDS reads 554 and 321, without
-// the epilogue 550 and 264, without all three 401 and 200: the loads cost most, more by the power
-// they draw (the clock falls from 2.4 to 1.8 .. 2.1 GHz) than by waiting.
+// the epilogue 550 and 264, without all three 401 and 200: the loads cost most, by the power
+// they draw (the clock falls from 2.4 to 1.8 .. 2.1 GHz) and by waves that wait for them (the
+// matrix units are busy for 0.6 of the cycles in w4a8, 0.4 in w4a4).
 #pragma once
 
 #include <type_traits>
