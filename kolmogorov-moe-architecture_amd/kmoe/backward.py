@@ -19,6 +19,7 @@ Data flow (A = routed rows, grouped by expert):
 from __future__ import annotations
 
 import math
+import weakref
 from typing import NamedTuple, Optional
 
 import torch
@@ -44,6 +45,30 @@ def router_wgrad_rows(T: int, d: int, n_cu: int) -> int:
     tokens, d 2048 46.2 / 47.3 / 36.3 (512); at 1.3 to 1.8 rounds a third slower)."""
     segs = max(1, min(n_cu // -(-d // 256), _lib.MAX_EXPERTS))
     return max(64, math.isqrt(T * d // 200) // 64 * 64, _ru(-(-T // segs), 64))
+
+
+class _Live:
+    """Held by the autograd nodes of a leaf's eager graphs."""
+    __slots__ = ("__weakref__",)
+
+
+_LIVE = weakref.WeakValueDictionary()  # id of a leaf (alive as long as its graphs are) -> its _Live
+
+
+def leaves_of(ctx, *inputs):
+    """Called by a forward that records a backward.  A leaf's gradient accumulates on the stream of
+    its first graph, so a capture of a backward while a graph of the same leaf made on the
+    default stream lives would draw that stream into the capture, which ends the process:
+    such a capture is refused here."""
+    leaves = [t for t in inputs if t is not None and t.requires_grad and t.is_leaf and t.is_cuda]
+    if not leaves:
+        return
+    if torch.cuda.is_current_stream_capturing():
+        if any(id(t) in _LIVE for t in leaves):
+            raise RuntimeError("kmoe: a graph of these leaves, recorded on the default stream outside of this capture, is "
+                               "still alive: delete its outputs (or run it on another stream) before capturing a backward")
+    elif ops._stream(leaves[0]) == 0:
+        ctx.live = [_LIVE.setdefault(id(t), _Live()) for t in leaves]
 
 
 class BwdWeights(NamedTuple):

@@ -68,6 +68,7 @@ class _AddNormFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, delta, weight, eps):
         d = x.shape[-1]
+        _bwd.leaves_of(ctx, x, delta, weight)
         r = ops.add_rmsnorm(x.detach().reshape(-1, d), delta.detach().reshape(-1, d), weight, eps)
         ctx.save_for_backward(r.h, r.rrms, weight)
         ctx.meta = (x.shape, x.dtype, delta.dtype)
@@ -288,6 +289,8 @@ class _BlockTrainFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, h, g, w_mod, w_in, w_out, w1, w2, w3, blk, use_mod):
+        if blk.ffn.grouped_experts.mx is not None:
+            _bwd.leaves_of(ctx, h, g, w_mod, w_in, w_out, w1, w2, w3)
         B, S, d = h.shape
         T = B * S
         ffn = blk.ffn

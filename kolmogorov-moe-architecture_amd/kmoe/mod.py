@@ -124,6 +124,8 @@ class _MoDTrainFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, residual, w_mod, w_in, w_out, w1, w2, w3, ffn, mod_router, xb, sel):
+        if ffn.grouped_experts.mx is not None:
+            _bwd.leaves_of(ctx, x, residual, w_mod, w_in, w_out, w1, w2, w3)
         B, S, d = x.shape
         keep = sel.sel_idx.shape[1]
         T = B * keep

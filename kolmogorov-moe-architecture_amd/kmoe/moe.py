@@ -474,6 +474,7 @@ class _RouteFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, k, bias, spec):
+        _bwd.leaves_of(ctx, logits)
         r = ops.route_topk(logits.detach(), k, bias=bias, **spec._asdict())
         ctx.save_for_backward(logits, r.idx)
         ctx.spec = spec
@@ -503,6 +504,8 @@ class _MoETrainFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w_in, w_out, w1, w2, w3, layer):
+        if layer.grouped_experts.mx is not None:
+            _bwd.leaves_of(ctx, x, w_in, w_out, w1, w2, w3)
         B, S, d = x.shape
         T = B * S
         x2d = x.reshape(T, d).to(torch.bfloat16).contiguous()
@@ -610,6 +613,8 @@ class _ExpertsFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x2d, w, w1, w2, w3, experts, idx):
+        if experts.mx is not None:
+            _bwd.leaves_of(ctx, x2d, w, w1, w2, w3)
         T, k = idx.shape
         E = experts.n_experts
         xb = x2d.detach().to(torch.bfloat16).contiguous()
@@ -643,6 +648,8 @@ class _ExpertsECFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x3d, w, w1, w2, w3, experts, token_indices):
+        if experts.mx is not None:
+            _bwd.leaves_of(ctx, x3d, w, w1, w2, w3)
         B, S, d = x3d.shape
         _, E, C = token_indices.shape
         sel = experts.tables(token_indices, w, S)
@@ -682,6 +689,8 @@ class _MoEECTrainFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, x, w_in, w_out, w1, w2, w3, layer):
+        if layer.grouped_experts_ec.mx is not None:
+            _bwd.leaves_of(ctx, x, w_in, w_out, w1, w2, w3)
         B, S, d = x.shape
         T = B * S
         E = layer.n_experts

@@ -596,6 +596,39 @@ def test_training_step_in_a_graph(dev):
         assert all(torch.equal(u, v) for u, v in zip(step(*sets[(i + 1) % 4]), eager[(i + 1) % 4]))
 
 
+@pytest.mark.filterwarnings("ignore:The CUDA Graph is empty")
+def test_capture_beside_an_eager_graph(dev):
+    """Refused before anything is recorded, for each operator; captured once that graph is gone."""
+    ex = kmoe.GroupedExperts(4, 64, 64).to(dev).to(BF)
+    ex.mx = "w4a4"
+    x, gain = rnd(dev, 8, 64), torch.ones(64, device=dev, dtype=BF).requires_grad_(True)
+    logits = rnd(dev, 8, 4, dtype=torch.float32).requires_grad_(True)
+    idx, w = torch.zeros(8, 1, dtype=torch.int64, device=dev), torch.ones(8, 1, device=dev)
+    dy = rnd(dev, 8, 64, seed=1)
+    calls = [(lambda: kmoe.route_topk(logits, 2)[0], logits, torch.ones(8, 2, device=dev)),
+             (lambda: kmoe.add_rms_norm(x, x, gain)[1], gain, dy), (lambda: ex(x, idx, w), ex.w1, dy)]
+    for call, leaf, dout in calls:
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.autograd.grad(call(), leaf, dout)
+        torch.cuda.current_stream().wait_stream(side)
+        alive = call()
+        with pytest.raises(RuntimeError, match="still alive"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                call()
+        want = torch.autograd.grad(alive, leaf, dout)[0]
+        del alive
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            got = torch.autograd.grad(call(), leaf, dout)[0]
+        for _ in range(3):
+            got.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(got, want)
+
+
 @pytest.mark.parametrize("training", [False, True])
 @pytest.mark.parametrize("dtype", [BF, torch.float32, torch.float16])
 def test_block_edge_calls(dev, training, dtype):

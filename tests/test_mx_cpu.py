@@ -155,6 +155,37 @@ def test_coded_rows_and_tables_are_checked():
         ops.gemm_down_mx(good, off, pw, 4)
 
 
+def test_capture_beside_an_eager_graph_is_refused(monkeypatch):
+    """The rule alone, on stand-ins for leaves: refused while a graph recorded on the default
+    stream lives, not for graphs of other leaves, of another stream, or gone."""
+    from types import SimpleNamespace
+
+    from kmoe import backward
+
+    def leaf(**kw):
+        return SimpleNamespace(**{**dict(requires_grad=True, is_leaf=True, is_cuda=True), **kw})
+    state = dict(capturing=False, stream=0)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: state["capturing"])
+    monkeypatch.setattr(ops, "_stream", lambda t: state["stream"])
+
+    def record(*leaves, **kw):
+        state.update(dict(capturing=False, stream=0), **kw)
+        ctx = SimpleNamespace()
+        backward.leaves_of(ctx, *leaves)
+        return ctx
+    a, b, c = leaf(), leaf(), leaf(is_leaf=False)
+    first, second = record(a, None, c), record(a)
+    del first
+    with pytest.raises(RuntimeError, match="still alive"):
+        record(b, a, capturing=True)
+    record(b, c, capturing=True)
+    del second
+    record(a, capturing=True)
+    side = record(b, stream=7)
+    record(b, capturing=True)
+    assert not vars(side)
+
+
 # ---- the restatements themselves
 def test_elements_against_torch_casts():
     v = torch.cat([torch.linspace(-500, 500, 20001), torch.logspace(-12, 9, 5000, base=2.0)]).double()
