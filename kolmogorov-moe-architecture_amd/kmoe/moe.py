@@ -245,10 +245,18 @@ class _PackedExperts(nn.Module):
         self.mx = None
 
     def _weights(self):
-        return tuple(w for w in (self.w1, self.w2, self.w3) if w is not None)
+        p = self._parameters  # (looked up once: a Module's attributes cost half a microsecond each)
+        if "w1" in p and "w2" in p and "w3" in p:
+            ws = p["w1"], p["w2"], p["w3"]
+        else:
+            ws = self.w1, self.w2, self.w3
+        return ws if ws[2] is not None else ws[:2]
 
     def _packed_key(self):
-        return tuple((w.data_ptr(), w._version, w.device) for w in self._weights()) + (self.use_fp8, self.mx)
+        key = [self.use_fp8, self.mx]
+        for w in self._weights():
+            key += (w.data_ptr(), w._version, w.device)
+        return key
 
     @property
     def mx_act(self) -> Optional[str]:

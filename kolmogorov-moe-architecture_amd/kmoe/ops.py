@@ -6,6 +6,7 @@ torch's current HIP stream.  There is no CPU path: inputs must live on a GPU.
 """
 from __future__ import annotations
 
+import functools
 import math
 from typing import NamedTuple, Optional
 
@@ -964,6 +965,11 @@ def gemm_down_mx(h: MXRows, offsets, pw: PackedWeightsMX, max_rows):
     return y
 
 
+@functools.lru_cache(maxsize=1024)
+def _mx_workspace(T, d, E, k, F, fmt, coded) -> int:
+    return _lib.load().kmoe_mx_experts_workspace_bytes(T, d, E, k, F, fmt, int(coded))
+
+
 class RoutedOut(NamedTuple):
     """What a one-call pass over routed tokens reports of its dispatch."""
     counts: torch.Tensor        # (E,) int32 routed counts
@@ -1023,7 +1029,7 @@ def mx_experts(x2d, idx, w, pw: PackedWeightsMX, fmt, capacity=0, row_index=None
     with _device(dev):
         if block_counts is not None and block_counts.numel() != -(-T // lib.kmoe_router_block_tokens(T)) * pw.E:
             raise ValueError("kmoe.mx_experts: block_counts must be the router's per-block histograms")
-        wsb = lib.kmoe_mx_experts_workspace_bytes(T, d, pw.E, k, pw.F, code, int(coded is not None))
+        wsb = _mx_workspace(T, d, pw.E, k, pw.F, code, coded is not None)
         ws = torch.empty(max(wsb, 4), device=dev, dtype=torch.uint8)
         _lib.call("kmoe_mx_experts", ptr(x2d), ptr(row_index), T, d, code, ptr(xq), ptr(xs), ptr(idx), ptr(w),
                   _lib.DTYPE_F32 if w.dtype == torch.float32 else _lib.DTYPE_BF16, k, pw.E, int(capacity), ptr(block_counts),
@@ -1063,7 +1069,7 @@ def add_rmsnorm(x2d, delta, weight, eps, quant=None) -> AddNormOut:
     weight = weight.detach()
     weight = _contig(weight, weight.dtype if weight.dtype in (torch.float32, _BF16) else torch.float32)
     dev = x2d.device
-    h = x2d if delta is None else torch.empty(T, d, device=dev, dtype=dt)
+    h = x2d if delta is None else torch.empty_like(x2d)
     n = torch.empty(T, d, device=dev, dtype=_BF16)
     rrms = torch.empty(T, device=dev, dtype=torch.float32)
     rows = _mx_rows(T, d, quant, dev) if quant is not None else None
