@@ -520,6 +520,28 @@ def test_offsets_past_32_bits(dev, fmt, d, F):
     assert torch.equal(y[few], ops.mx_experts(x[few], idx[few], w[few], pw, fmt)[0])
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+def test_tile_sizes_agree(dev, fmt):
+    """The first tokens of batches that take the different tile sizes of both products (64 x 128,
+    64 x 256, 128 x 256 on 256 CUs), with and without the kept gate / up values: each K sum has one
+    order in all of them, so the same bits."""
+    E, d, F, k = 4, 1024, 2048, 2
+    pw = ops.pack_weights_mx(*weights(dev, E, d, F))
+    T = 8001
+    x = rnd(dev, T, d)
+    idx = torch.rand(T, E, generator=torch.Generator().manual_seed(4)).topk(k, 1).indices.to(dev)
+    w = torch.ones(T, k, device=dev)
+    want = None
+    for t in (100, 1203, T):
+        y = ops.mx_experts(x[:t], idx[:t], w[:t], pw, fmt)[0]
+        disp = ops.dispatch(x[:t], idx[:t], w[:t], E, materialize=False)
+        h, gu = ops.gemm_gate_up_mx(ops.quant_rows_mx(x[:t], fmt), disp.row_token, disp.offsets, pw, t * k, save_gu=True)
+        rows = disp.slot_row.view(t, k)[:100].long().flatten()
+        got = (y[:100], ops.gemm_down_mx(h, disp.offsets, pw, t * k)[rows], h.q[rows], used(h)[rows], gu[rows])
+        want = got if want is None else want
+        assert all(torch.equal(u, v) for u, v in zip(got, want))
+
+
 def test_weights_past_32_bits(dev):
     """Experts whose weights and packed codes hold over 2^31 values and bytes: the last ones
     alone give the same values, packs and products."""
