@@ -10,15 +10,18 @@ namespace {
 
 constexpr int FEW = 1024;  // threads of the workgroup that dispatches
 constexpr int MAX_ROUNDS = 4;
-// Rounds of FEW assignments that one workgroup dispatches: an expert and round cost a ballot.
-int few_rounds(int E) { return 64 / E < 1 ? 1 : 64 / E > MAX_ROUNDS ? MAX_ROUNDS : 64 / E; }
+// Rounds of FEW assignments that one workgroup dispatches: an expert and round cost a ballot.  A
+// whole pass with this dispatch / with kmoe_dispatch and the quantisation, us: 16 experts, 96
+// assignments 18.4 / 23.7, 1536 27.2 / 31.9, 3000 37.7 / 38.9, 4080 47.4 / 46.7; 8 experts, 4080
+// 44.7 / 46.0; 32 experts, 2000 27.8 / 30.4, 3000 33.2 / 31.1; 64 experts, 2000 34.6 / 38.8.
+int few_rounds(int E) { return E <= 16 ? MAX_ROUNDS : 2; }
 
 // Dispatch of at most R FEW assignments (the tables of kmoe_dispatch, same order) by workgroup
 // 0, the quantisation of the T rows x[row_index[t]] by the others: one launch in place of
 // three, whose latencies are the time at these sizes.  A thread holds assignments R tid ..
 // R tid + R - 1; a rank is counted by ballots in its wave and summed over the waves before it.
-// 96 assignments of 16 experts and 48 x 2048 rows 4.0 us, 1554 and 777 8.0 (dispatch in three
-// launches and the quantisation 11 + 9).
+// 96 assignments of 16 experts and 48 x 2048 rows 4.0 us (kmoe_dispatch and the quantisation 8.0),
+// 1554 and 777 6.2 (9.1).
 template <bool FP4, int R>
 __global__ __launch_bounds__(FEW) void tables_kernel(const int64_t* __restrict__ idx, const void* __restrict__ wsrc,
                                                      bool w_f32, int T, int k, int E, int64_t capacity,
@@ -195,19 +198,23 @@ extern "C" int kmoe_mx_experts(const void* x, const int32_t* row_index, int64_t 
     const dim3 grid((unsigned)(1 + kmoe::ceil_div<int64_t>(chunks, FEW)));
     const uint16_t* xp = static_cast<const uint16_t*>(x);
     hipStream_t s = kmoe::as_stream(stream);
-    const int R = A <= FEW ? 1 : MAX_ROUNDS;
 #define KMOE_TABLES(FP4_, R_)                                                                                             \
   hipLaunchKernelGGL((tables_kernel<FP4_, R_>), grid, dim3(FEW), 0, s, topk_idx, topk_w, w_dtype == KMOE_DTYPE_F32, (int)T, k, \
                      E, capacity, counts, i32(b.offsets), i32(b.row_token), i32(b.slot_row), slot_w, xp, row_index, d,       \
                      ws + b.xq, ws + b.xs)
-    if (fp4 && R == 1)
-      KMOE_TABLES(true, 1);
-    else if (fp4)
-      KMOE_TABLES(true, MAX_ROUNDS);
-    else if (R == 1)
-      KMOE_TABLES(false, 1);
-    else
-      KMOE_TABLES(false, MAX_ROUNDS);
+#define KMOE_TABLES_FMT(R_)    \
+  if (fp4)                     \
+    KMOE_TABLES(true, R_);     \
+  else                         \
+    KMOE_TABLES(false, R_)
+    if (A <= FEW) {
+      KMOE_TABLES_FMT(1);
+    } else if (A <= 2 * FEW) {
+      KMOE_TABLES_FMT(2);
+    } else {
+      KMOE_TABLES_FMT(MAX_ROUNDS);
+    }
+#undef KMOE_TABLES_FMT
 #undef KMOE_TABLES
     rc = kmoe::check_launch("kmoe_mx_experts");
     if (rc) return rc;
