@@ -121,6 +121,8 @@ class Router(_RouterMLP):
     """Token-choice top-k router (moe.py:327-462), with the scores, groups and balance bias of
     the configuration's moe_router_* fields."""
 
+    spec: Optional[ops.RouteSpec] = None  # how logits become experts and weights; None: the router kernel's own top-k
+
     def __init__(self, config: AdvancedMoEConfig):
         super().__init__(config.d_model, config.n_experts)
         self.d_model = config.d_model
@@ -130,7 +132,6 @@ class Router(_RouterMLP):
         bias = getattr(config, "moe_router_bias", None)
         # fp32 per-expert logit bias (kept out of the state dict and of dtype casts)
         self.logit_bias = None if bias is None else torch.tensor(list(bias), dtype=torch.float32)
-        # how logits become experts and weights; None: the router kernel's own top-k
         self.spec = _route_spec(config)
         # added to the scores for the choice only; moved by the training program (kept in fp32
         # by dtype casts, in the state dict)
@@ -143,7 +144,7 @@ class Router(_RouterMLP):
                              "and the balance bias do not apply to it")
 
     def _apply(self, fn, recurse=True):
-        bias = self.balance_bias
+        bias = self._buffers.get("balance_bias")
         super()._apply(fn, recurse)
         if bias is not None and self.balance_bias.dtype != torch.float32:
             new = self.balance_bias
@@ -222,6 +223,8 @@ class ExpertChoiceRouter(_RouterMLP):
 class _PackedExperts(nn.Module):
     """Holds w1,w2 (E,d,F), w3 (E,F,d) and their packed kernel layout (derived cache)."""
 
+    mx: Optional[str] = None  # microscaled experts: "w4a8", "w4a4" or None (also of a module pickled without it)
+
     def __init__(self, n_experts: int, d_model: int, d_ff: int, activation: str = "swiglu"):
         super().__init__()
         self.n_experts = n_experts
@@ -241,8 +244,6 @@ class _PackedExperts(nn.Module):
         _init_expert_weights(self.w1, self.w2, self.w3)
         self._packed = None
         self.use_fp8 = False
-        # microscaled experts: "w4a8", "w4a4" or None
-        self.mx = None
 
     def _weights(self):
         p = self._parameters  # (looked up once: a Module's attributes cost half a microsecond each)

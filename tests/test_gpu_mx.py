@@ -562,6 +562,29 @@ def test_weights_past_32_bits(dev):
         assert torch.equal(ops.mx_experts(x, idx, one, pw, fmt)[0], ops.mx_experts(x, 0 * idx, one, p1, fmt)[0])
 
 
+@pytest.mark.parametrize("mx", ["w4a8", "w4a4"])
+def test_capacity_in_training(dev, mx):
+    """Dropped assignments: the training forward gives the inference one's values, a token whose
+    every assignment was dropped gets no output, and no gradient through the experts."""
+    cfg = config(E=4, d=128, F=96, moe_mx=mx, moe_drop_overflow=True, moe_capacity_factor=0.25)
+    layer = kmoe.MoELayer(cfg).to(dev).to(BF).train()
+    x = rnd(dev, 1, 300, 128)
+    with torch.no_grad():
+        want = layer(x)
+    xg = x.clone().requires_grad_(True)
+    y = layer(xg)
+    assert torch.equal(y, want)
+    empty = ~want[0].any(1)
+    assert bool(empty.any()) and not bool(empty.all())
+    ex = layer.grouped_experts
+    dw = torch.autograd.grad(y, [ex.w1, ex.w2, ex.w3], rnd(dev, 1, 300, 128, seed=1), retain_graph=False)
+    assert all(bool(g.isfinite().all()) and bool(g.any()) for g in dw)
+    y2 = layer(xg)
+    dy = rnd(dev, 1, 300, 128, seed=1)
+    dy[0, empty] = 100.0  # (what a token without output gets does not reach the experts)
+    assert all(torch.equal(u, v) for u, v in zip(torch.autograd.grad(y2, [ex.w1, ex.w2, ex.w3], dy), dw))
+
+
 def test_two_streams_at_once(dev):
     """Two passes of one layer on two streams at once, several times: each its own result."""
     layer = kmoe.MoELayer(config(E=8, d=256, F=352, moe_mx="w4a4")).to(dev).to(BF).eval()

@@ -121,6 +121,16 @@ def test_balance_bias_keeps_its_type():
     assert m.balance_bias.dtype == torch.float32 and not m.balance_bias.is_meta
 
 
+def test_modules_without_the_new_attributes():
+    """Modules pickled before these attributes were there act as they did."""
+    ex, router = kmoe.GroupedExperts(2, 64, 64), kmoe.Router(kmoe.AdvancedMoEConfig(d_model=64, n_experts=4))
+    ex.__dict__.pop("mx", None)
+    router.__dict__.pop("spec", None)
+    router._buffers.pop("balance_bias")
+    assert ex.mx is None and ex.mx_act is None and router.spec is None
+    router.to(torch.bfloat16)
+
+
 def test_cpu_tensors_are_refused():
     x = torch.zeros(2, 64, dtype=torch.bfloat16)
     for call in (lambda: ops.route_topk(torch.zeros(2, 4), 1), lambda: ops.quant_rows_mx(x),
