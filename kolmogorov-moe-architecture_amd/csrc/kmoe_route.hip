@@ -59,10 +59,19 @@ template <int L>
 __device__ __forceinline__ float group_sum(float v) {
   return group_reduce<L>(v, [](float a, float b) { return a + b; });
 }
-template <int L>
-__device__ __forceinline__ double group_sum(double v) {
-#pragma unroll
-  for (int o = L / 2; o > 0; o >>= 1) v += __shfl_xor(v, o, 64);
+__device__ __forceinline__ double wave_sum(double v) {
+  auto step = [&](auto s) {
+    constexpr int S = decltype(s)::value;
+    const int64_t b = __double_as_longlong(v);
+    const uint64_t hi = (uint32_t)across<S>((int)(b >> 32)), lo = (uint32_t)across<S>((int)b);
+    v += __longlong_as_double((int64_t)(hi << 32 | lo));
+  };
+  step(std::integral_constant<int, 1>{});
+  step(std::integral_constant<int, 2>{});
+  step(std::integral_constant<int, 4>{});
+  step(std::integral_constant<int, 8>{});
+  step(std::integral_constant<int, 16>{});
+  step(std::integral_constant<int, 32>{});
   return v;
 }
 // Maximum over the L lanes of a token, NaN if there is one.
@@ -102,22 +111,22 @@ constexpr int LANES = 16;         // lanes of a token: its reductions are moves 
 
 // What a token keeps in LDS.
 struct RouteLds {
-  int64_t key[KMOE_MAX_EXPERTS];
+  int64_t key[KMOE_MAX_EXPERTS];   // (64: a lane's place each)
   int64_t gkey[KMOE_MAX_EXPERTS];
   float pick[MAX_K];  // chosen scores
 };
 
-// Scores of a token's logits l (expert sub EPL + i of the lane), in type V; rel: bounds of their
-// relative errors in f32: exp 2 half steps (2^-24) and, for softmax, the rounding of l - max, |l
-// - max| half steps; the sum of the token's exponentials the same, at most 16 half steps where
-// it matters (smaller ones add less than their error), and its additions 2 + log2 16; the
-// quotient one: (|l - max| + 32) 2^-24.  Sigmoid: exp, sum, quotient, under 8 2^-24.
-template <int EPL, class V>
-__device__ __forceinline__ void scores_of(const float (&l)[EPL], bool sigmoid, V (&s)[EPL], float (&rel)[EPL]) {
+// Scores of a token's logits l (expert sub EPL + i of the lane) in f32; rel: bounds of their
+// relative errors: exp 2 half steps (2^-24) and, for softmax, the rounding of l - max, |l - max|
+// half steps; the sum of the token's exponentials the same, at most 16 half steps where it
+// matters (smaller ones add less than their error), and its additions 2 + log2 16; the quotient
+// one: (|l - max| + 32) 2^-24.  Sigmoid: exp, sum, quotient, under 8 2^-24.
+template <int EPL>
+__device__ __forceinline__ void scores_of(const float (&l)[EPL], bool sigmoid, float (&s)[EPL], float (&rel)[EPL]) {
   if (sigmoid) {
 #pragma unroll
     for (int i = 0; i < EPL; ++i) {
-      s[i] = (V)1 / ((V)1 + exp(-(V)l[i]));  // 0 for -inf
+      s[i] = 1.0f / (1.0f + expf(-l[i]));  // 0 for -inf
       rel[i] = 0x1p-21f;
     }
     return;
@@ -126,29 +135,28 @@ __device__ __forceinline__ void scores_of(const float (&l)[EPL], bool sigmoid, V
 #pragma unroll
   for (int i = 1; i < EPL; ++i) m = m != m ? m : (l[i] != l[i] || l[i] > m ? l[i] : m);
   m = group_max<LANES>(m);
-  V z = (V)0;
+  float z = 0.0f;
 #pragma unroll
   for (int i = 0; i < EPL; ++i) {
-    s[i] = m == -INFINITY ? (V)0 : exp((V)l[i] - (V)m);
+    s[i] = m == -INFINITY ? 0.0f : expf(l[i] - m);
     rel[i] = (m - l[i] + 32.0f) * 0x1p-24f;
     z += s[i];
   }
   z = group_sum<LANES>(z);
 #pragma unroll
-  for (int i = 0; i < EPL; ++i) s[i] = m == -INFINITY ? (V)0 : s[i] / z;
+  for (int i = 0; i < EPL; ++i) s[i] = m == -INFINITY ? 0.0f : s[i] / z;
 }
 
 // Groups kept by their values val[g] in LDS (equal values: lowest group first), as a mask;
 // low and high: the least value kept and the greatest dropped among the lane's groups.
-template <class V>
-__device__ __forceinline__ uint64_t keep_groups(const RouteArgs& a, const V* val, int sub, V& low, V& high) {
+__device__ __forceinline__ uint64_t keep_groups(const RouteArgs& a, const float* val, int sub, float& low, float& high) {
   uint64_t kept = 0;
   for (int g = sub; g < a.groups; g += LANES) {
-    const V v = val[g];
+    const float v = val[g];
     int rank = 0;
 #pragma unroll 8
     for (int j = 0; j < a.groups; ++j) {
-      const V o = val[j];
+      const float o = val[j];
       rank += o > v || (o == v && j < g);
     }
     if (rank < a.topk_groups) {
@@ -170,44 +178,31 @@ __device__ __forceinline__ int row_max(int v) {
   v = max(v, across<4>(v));
   return max(v, across<8>(v));
 }
-__device__ __forceinline__ int64_t row_max(int64_t v) {
-  auto step = [&](auto s) {
-    constexpr int S = decltype(s)::value;
-    const uint64_t hi = (uint32_t)across<S>((int)(v >> 32)), lo = (uint32_t)across<S>((int)v);
-    const int64_t u = (int64_t)(hi << 32 | lo);
-    v = u > v ? u : v;
-  };
-  step(std::integral_constant<int, 1>{});
-  step(std::integral_constant<int, 2>{});
-  step(std::integral_constant<int, 4>{});
-  step(std::integral_constant<int, 8>{});
-  return v;
-}
 
-// A token's order in 64 bits.  rank: the place of each of the lane's experts (< k: chosen, its
-// score in pick), or MAX_K.
-template <int EPL>
-__device__ __forceinline__ void rank64(const RouteArgs& a, RouteLds& s, const float (&l)[EPL], const float (&b)[EPL], int sub,
-                                       int gs, int base, int (&rank)[EPL]) {
-  double sc[EPL];
-  float rel[EPL];
-  scores_of<EPL, double>(l, a.sigmoid, sc, rel);
-  int64_t kc[EPL];
-#pragma unroll
-  for (int i = 0; i < EPL; ++i) {
-    const double c = l[i] == -INFINITY ? -INFINITY : sc[i] + (double)b[i];
-    kc[i] = sub * EPL + i < a.E ? key_of(c) : INT64_MIN;
-    s.key[sub * EPL + i] = __double_as_longlong(c);
-    rank[i] = MAX_K;
+// A token's order in 64 bits, by the whole wave: lane e holds expert e, its logit l and bias b
+// (e >= E: l -inf).  The place of the lane's expert; its score in the token's pick if that is < k.
+__device__ __forceinline__ int rank64(const RouteArgs& a, RouteLds& s, float l, float b, int lane, int gs) {
+  double sc;
+  if (a.sigmoid) {
+    sc = 1.0 / (1.0 + exp(-(double)l));  // 0 for -inf
+  } else {
+    const float m = group_max<64>(l);
+    sc = m == -INFINITY ? 0.0 : exp((double)l - (double)m);
+    const double z = wave_sum(sc);
+    sc = m == -INFINITY ? 0.0 : sc / z;
   }
-  wave_lds_fence();
+  const double c = l == -INFINITY ? -INFINITY : sc + (double)b;
+  int64_t key = lane < a.E ? key_of(c) : INT64_MIN;
   if (a.groups > 1) {
-    for (int g = sub; g < a.groups; g += LANES) {
+    s.key[lane] = __double_as_longlong(c);
+    wave_lds_fence();
+    int64_t mine = INT64_MIN;
+    if (lane < a.groups) {
       double b1 = -INFINITY, b2 = -INFINITY;
       bool nan = false;
-#pragma unroll 4
+#pragma unroll 8
       for (int j = 0; j < gs; ++j) {
-        const double v = __longlong_as_double(s.key[g * gs + j]);
+        const double v = __longlong_as_double(s.key[lane * gs + j]);
         nan |= v != v;
         if (v > b1) {
           b2 = b1;
@@ -217,41 +212,37 @@ __device__ __forceinline__ void rank64(const RouteArgs& a, RouteLds& s, const fl
         }
       }
       if (a.group_top == 2 && b2 > -INFINITY) b1 += b2;
-      s.gkey[g] = nan ? INT64_MAX : key_of(b1);
+      mine = nan ? INT64_MAX : key_of(b1);
     }
+    s.gkey[lane] = mine;
     wave_lds_fence();
-    int64_t low = INT64_MAX, high = INT64_MIN;
-    const uint64_t kept = keep_groups<int64_t>(a, s.gkey, sub, low, high);
-#pragma unroll
-    for (int i = 0; i < EPL; ++i)
-      if (!((kept >> ((sub * EPL + i) / gs)) & 1)) kc[i] = INT64_MIN;  // behind masked experts
-  }
-  for (int r = 0; r < a.k; ++r) {
-    int64_t m = kc[0];
-#pragma unroll
-    for (int i = 1; i < EPL; ++i) m = kc[i] > m ? kc[i] : m;
-    const int64_t best = row_max(m);
-    const uint32_t at = (uint32_t)(__ballot(m == best) >> base) & 0xffffu;
-    if (sub == __builtin_ctz(at | 0x10000u)) {
-      bool done = false;
-#pragma unroll
-      for (int i = 0; i < EPL; ++i)
-        if (!done && kc[i] == best) {
-          done = true;
-          kc[i] = INT64_MIN;
-          rank[i] = r;
-          s.pick[r] = l[i] == -INFINITY ? 0.0f : (float)sc[i];
-        }
+    int rank = 0;
+#pragma unroll 8
+    for (int j = 0; j < a.groups; ++j) {
+      const int64_t o = s.gkey[j];
+      rank += o > mine || (o == mine && j < lane);
     }
+    const uint64_t kept = __ballot(lane < a.groups && rank < a.topk_groups);
+    if (!((kept >> (lane / gs)) & 1)) key = INT64_MIN;  // behind masked experts
   }
+  s.key[lane] = key;
   wave_lds_fence();
+  int rank = 0;
+#pragma unroll 8
+  for (int j = 0; j < a.E; ++j) {
+    const int64_t o = s.key[j];
+    rank += o > key || (o == key && j < lane);
+  }
+  if (lane < a.E && rank < a.k) s.pick[rank] = l == -INFINITY ? 0.0f : (float)sc;
+  return lane < a.E ? rank : MAX_K;
 }
 
 // One workgroup per histogram block, its waves independent of each other; 16 lanes hold a
 // token, EPL experts each.  The time is that of one token's chain of dependent steps, so a
 // wave works on four and a workgroup on 64 at once: 16384 tokens, 64 experts, 8 groups, top-8
-// 12.9 us (64 lanes a token, four tokens a wave one after the other: 27), 64 tokens 5.5; with
-// choices so far apart that no token needs the 64-bit order 8.5 and 5.5.
+// 11.9 us (64 lanes a token, four tokens a wave one after the other: 27), 64 tokens 5.5; with
+// choices so far apart that no token needs the 64-bit order 8.6 and 5.5.  That order takes the
+// whole wave for one token (with its 16 lanes, the wave's four tokens together, 12.9).
 template <int EPL>
 __global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
   __shared__ RouteLds lds[64];
@@ -274,7 +265,7 @@ __global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
   if (!__any(live)) goto done;
   {
     float rel[EPL];  // more than the scores' relative errors
-    scores_of<EPL, float>(l, a.sigmoid, sc, rel);
+    scores_of<EPL>(l, a.sigmoid, sc, rel);
     bool sure = true;
     float err = 0.0f;
 #pragma unroll
@@ -306,7 +297,7 @@ __global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
       }
       wave_lds_fence();
       float low = INFINITY, high = -INFINITY;
-      const uint64_t kept = keep_groups<float>(a, gv, sub, low, high);
+      const uint64_t kept = keep_groups(a, gv, sub, low, high);
       low = -group_top<LANES>(-low);
       high = group_top<LANES>(high);
       // a group's value is the sum of up to two choices
@@ -353,7 +344,31 @@ __global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
       }
     sure = sure && group_sum<LANES>(gone) == (float)a.k;
     wave_lds_fence();
-    if (__any(live && !sure)) rank64<EPL>(a, s, l, b, sub, gs, base, rank);
+    const uint64_t open = __ballot(live && !sure);  // lanes of the tokens to order in 64 bits
+    if (open) {
+      float* const lv = reinterpret_cast<float*>(s.key);
+#pragma unroll
+      for (int i = 0; i < EPL; ++i) lv[sub * EPL + i] = l[i];
+      wave_lds_fence();
+      const int lane = tid & 63;
+      for (int j = 0; j < 64 / LANES; ++j)
+        if ((open >> (j * LANES)) & 0xffffu) {
+          const int tok = (tid >> 6) * (64 / LANES) + j;
+          RouteLds& o = lds[tok];
+          const float le = lane < a.E ? reinterpret_cast<const float*>(o.key)[lane] : -INFINITY;
+          const float be = lane < a.E && a.bias ? a.bias[lane] : 0.0f;
+          wave_lds_fence();
+          const int r = rank64(a, o, le, be, lane, gs);
+          if (r < a.k) {
+            a.idx[((int64_t)blockIdx.x * a.hb + tok) * a.k + r] = lane;
+            if (a.block_counts) atomicAdd(&count[lane], 1);
+          }
+        }
+      wave_lds_fence();
+      if ((open >> base) & 0xffffu)
+#pragma unroll
+        for (int i = 0; i < EPL; ++i) rank[i] = MAX_K;  // written above
+    }
 #pragma unroll
     for (int i = 0; i < EPL; ++i)
       if (live && rank[i] < a.k) {
