@@ -88,7 +88,9 @@ class _AddNormFn(torch.autograd.Function):
 
         def grad(dtype):
             return (ds16 if dtype == torch.bfloat16 and ds16 is not None else ds).view(shape).to(dtype)
-        return grad(x_dtype), grad(delta_dtype), dg, None
+        gx = grad(x_dtype)
+        # (of one type the same tensor twice: autograd copies what two leaves would share)
+        return gx, gx if delta_dtype == x_dtype else grad(delta_dtype), dg, None
 
 
 def add_rms_norm(x: torch.Tensor, delta: torch.Tensor, weight: torch.Tensor, eps: float = 1e-5):

@@ -93,6 +93,27 @@ def test_backward_of_one_output(dev):
         g.sum().backward()
 
 
+@pytest.mark.parametrize("xd,dd", [(BF, BF), (F32, F32), (F32, BF), (BF, F32)])
+@pytest.mark.parametrize("both", [False, True])
+def test_gradients_are_not_shared(dev, xd, dd, both):
+    """x and delta leaves of one sum: writing to one's gradient leaves the other's as it was; one
+    tensor as both gets twice the gradient."""
+    x, delta = (rnd(dev, 3, 64, seed=i, dtype=t).requires_grad_(True) for i, t in enumerate((xd, dd)))
+    w = torch.ones(64, device=dev)
+    h, n = kmoe.add_rms_norm(x, delta, w, EPS)
+    torch.autograd.backward([n, h] if both else [h], [torch.ones_like(t) for t in ([n, h] if both else [h])])
+    want = delta.grad.clone()
+    x.grad.mul_(2.0)
+    assert torch.equal(delta.grad, want)
+    y = rnd(dev, 3, 64, dtype=xd).requires_grad_(True)
+    z = y.detach().clone().requires_grad_(True)
+    u = y.detach().clone().requires_grad_(True)
+    for a, b in ((y, y), (z, u)):
+        h, n = kmoe.add_rms_norm(a, b, w, EPS)
+        torch.autograd.backward([n, h], [torch.ones_like(n), torch.ones_like(h)])
+    assert torch.equal(y.grad, z.grad + u.grad)
+
+
 def test_backward_against_differences(dev):
     T, d, h = 3, 64, 2.0 ** -6
     x, delta = rnd(dev, T, d, dtype=F32).requires_grad_(True), rnd(dev, T, d, seed=1, dtype=F32)
