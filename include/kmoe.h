@@ -611,7 +611,7 @@ int kmoe_pack_weights_mx(const void* w1, const void* w2, const void* w3, int w_d
 /* hq, h_scale = coded rows (K = F, padded columns zero) of silu(x w1) * (x w2) for the
  * rows of each expert ([offsets[e], offsets[e+1]), device, offsets[E] <= max_rows).
  * Permuted row r is coded row r of xq, or with row_token (device) row row_token[r] of
- * its n_x_rows (-1: a zero row).
+ * its n_x_rows (-1 or past them: a zero row).
  * gu (nullable; training): also the bf16 pre-activation gate / up values, (max_rows,
  * 2 F_pad) in the order of kmoe_gemm_gate_up_rows_gu.  Rows past offsets[E] are left. */
 int kmoe_gemm_gate_up_mx(const void* xq, const uint8_t* x_scale, int fmt, int64_t n_x_rows, const int32_t* row_token,

@@ -56,6 +56,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_small_kernel(MxGemmArgs g) {
   const bool gather = GATE_UP && g.row_token;
   const uint8_t* const abase = gather ? g.a : g.a + m0 * lda;
   const uint8_t* const sbase = gather ? g.a_scale : g.a_scale + m0 * lds_a;
+  const int64_t a_rows = gather ? g.a_rows : rows;  // rows past these read as zeros
 
   f32x4_t acc[2][NB];
 #pragma unroll
@@ -78,7 +79,7 @@ __global__ __launch_bounds__(64 * WAVES) void mx_small_kernel(MxGemmArgs g) {
     };
     uint32_t aoff[MB], asoff[MB];
     auto load_a = [&](int u, int s) {
-      const __amdgpu_buffer_rsrc_t ra = window(abase, s < s1 ? 0x7fffffff : 0), rs = window(sbase, s < s1 ? 0x7fffffff : 0);
+      const __amdgpu_buffer_rsrc_t ra = window(abase, s < s1 ? a_rows * lda : 0), rs = window(sbase, s < s1 ? a_rows * lds_a : 0);
 #pragma unroll
       for (int m = 0; m < MB; ++m) {
 #pragma unroll

@@ -66,7 +66,8 @@ def leaves_of(ctx, *inputs):
     if torch.cuda.is_current_stream_capturing():
         if any(id(t) in _LIVE for t in leaves):
             raise RuntimeError("kmoe: a graph of these leaves, recorded on the default stream outside of this capture, is "
-                               "still alive: delete its outputs (or run it on another stream) before capturing a backward")
+                               "still alive: delete its outputs (or run it on another stream) before capturing a "
+                               "backward; a forward alone is captured under torch.no_grad()")
     elif ops._stream(leaves[0]) == 0:
         ctx.live = [_LIVE.setdefault(id(t), _Live()) for t in leaves]
 

@@ -245,6 +245,23 @@ def test_nan_rows_and_missing_rows(dev, fmt):
     assert not yt[10].any() and torch.equal(yt[11:], y0[11:])
 
 
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("A", [3, 200])
+def test_rows_past_the_last_are_zeros(dev, fmt, A):
+    """row_token entries outside of the gathered rows, in the small-row kernel and in a tile."""
+    pw = ops.pack_weights_mx(*weights(dev, 1, 128, 64))
+    x = ops.quant_rows_mx(rnd(dev, 5, 128), fmt)
+    token = torch.arange(A, dtype=torch.int32) % 5
+    bad = [1, 2] if A == 3 else [1, 64, 130, 199]
+    token[bad] = torch.tensor([5, 5000, -1, 77777], dtype=torch.int32)[:len(bad)]
+    off = torch.tensor([0, A], dtype=torch.int32, device=dev)
+    h = ops.gemm_gate_up_mx(x, token.to(dev), off, pw, A)
+    good = [i for i in range(A) if i not in bad]
+    assert not h.q[bad].any() and bool(h.q[good].any(1).all())
+    one = ops.gemm_gate_up_mx(x, torch.tensor([0], dtype=torch.int32, device=dev), off.clamp(max=1), pw, 1)
+    assert torch.equal(h.q[0], one.q[0])
+
+
 def test_products_do_not_depend_on_the_run(dev):
     E, d, F, T, k = 4, 256, 352, 300, 2
     ex = kmoe.GroupedExperts(E, d, F).to(dev).to(BF)
