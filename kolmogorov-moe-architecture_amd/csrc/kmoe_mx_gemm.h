@@ -46,7 +46,7 @@ struct MxGemmArgs {
   const uint8_t* a;        // activation rows
   const uint8_t* a_scale;
   int64_t a_rows;          // rows of a (gathered) or max_rows
-  const int32_t* row_token;  // gate_up: permuted row r is a's row row_token[r] (nullable; -1: zeros)
+  const int32_t* row_token;  // gate_up: permuted row r is a's row row_token[r] (nullable; -1 or past a_rows: zeros)
   const int32_t* offsets;
   int E;
   int k_steps;             // K / 128, padded
@@ -228,8 +228,9 @@ __global__ __launch_bounds__(GEMM_THREADS, 2) void mx_gemm_kernel(MxGemmArgs g) 
   auto source_row = [&](int r) -> uint32_t {  // row of `a` (or of the slot) that tile row r is; NONE without one
     if (r >= rows) return NONE;
     if (!gather) return (uint32_t)r;
-    const int src = g.row_token[m0 + r];
-    return src < 0 ? NONE : (uint32_t)src;
+    // compared before it is multiplied: the 32-bit offset of a row past the end could wrap into the window
+    const uint32_t src = (uint32_t)g.row_token[m0 + r];
+    return src < (uint32_t)g.a_rows ? src : NONE;
   };
   constexpr int CPR = FP4 ? 4 : 8, RPB = 64 / CPR;  // 16-byte chunks per row, rows per 1 KiB load
   uint32_t aoff[T::NA];

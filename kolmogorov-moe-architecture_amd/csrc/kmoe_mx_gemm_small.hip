@@ -93,9 +93,11 @@ __global__ __launch_bounds__(64 * WAVES) void mx_small_kernel(MxGemmArgs g) {
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
       const int r = m * 16 + r16;
-      int src = r < rows ? (gather ? g.row_token[m0 + r] : r) : -1;
-      aoff[m] = src < 0 ? 0x80000000u : (uint32_t)src * (uint32_t)lda + q * 16u;
-      asoff[m] = src < 0 ? 0x80000000u : (uint32_t)src * (uint32_t)lds_a + q;
+      const uint32_t src = r < rows ? (gather ? (uint32_t)g.row_token[m0 + r] : (uint32_t)r) : ~0u;
+      // (a missing row's offset is past every window; that of a row past the end could wrap into it)
+      const bool on = src < (uint32_t)a_rows;
+      aoff[m] = on ? src * (uint32_t)lda + q * 16u : 0x80000000u;
+      asoff[m] = on ? src * (uint32_t)lds_a + q : 0x80000000u;
     }
 #pragma unroll
     for (int u = 0; u < DEPTH; ++u) load_a(u, s0 + u);

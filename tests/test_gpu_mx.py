@@ -750,3 +750,21 @@ def test_refusals(dev):
     with pytest.raises(ValueError, match="packed-weight files"):
         ex.use_fp8 = False
         kmoe.checkpoint.save_packed(ex, "unused.safetensors")
+
+
+@pytest.mark.parametrize("fmt", ["e4m3", "e2m1"])
+@pytest.mark.parametrize("A", [5, 200])
+def test_rows_far_past_the_last_are_zeros(dev, fmt, A):
+    """row_token entries whose byte offset is a multiple of 2^32 (of the codes: 2^25 and 2^26 rows of
+    128 and 64 bytes; of the scales: 2^28 of 16), and the largest entry, in the small-row kernel and a
+    tile."""
+    pw = ops.pack_weights_mx(*weights(dev, 1, 128, 64))
+    x = ops.quant_rows_mx(rnd(dev, 5, 128), fmt)
+    far = [1 << 25, (1 << 26) + 1, 1 << 28, 2**31 - 1]
+    token = torch.arange(A, dtype=torch.int32) % 5
+    bad = [1, 2, 3, 4] if A == 5 else [1, 64, 130, 199]
+    token[bad] = torch.tensor(far, dtype=torch.int32)
+    off = torch.tensor([0, A], dtype=torch.int32, device=dev)
+    h = ops.gemm_gate_up_mx(x, token.to(dev), off, pw, A)
+    good = [i for i in range(A) if i not in bad]
+    assert not h.q[bad].any() and bool(h.q[good].any(1).all())
