@@ -571,11 +571,16 @@ struct MxLaunch {
   hipStream_t s;
 };
 constexpr int SMALL_ROWS = 32;  // rows of a slot of the small-row kernel
+// Workgroups of tiles of `rows` rows and a `split`-th of a weight tile: the most slots that max_rows rows of E
+// experts come to, times the column tiles, a multiple of the 8 XCDs.
+inline int64_t mx_workgroups(int64_t max_rows, int E, int b_tiles, int rows, int split) {
+  const int64_t slots = max_rows / rows + (max_rows < E ? max_rows : E);
+  return (slots * b_tiles * split + 7) / 8 * 8;
+}
 template <bool GATE_UP, bool FP4, int MI, int NJ, bool SAVE_GU = false>
 void launch_mx_tile(const MxLaunch& l) {
   using T = MxTile<GATE_UP, FP4, MI, NJ, SAVE_GU>;
-  const int64_t slots = l.max_rows / T::BM + (l.max_rows < l.g.E ? l.max_rows : l.g.E);
-  const int64_t blocks = (slots * l.g.b_tiles * (4 / NJ) + 7) / 8 * 8;
+  const int64_t blocks = mx_workgroups(l.max_rows, l.g.E, l.g.b_tiles, T::BM, 4 / NJ);
   hipLaunchKernelGGL((mx_gemm_kernel<GATE_UP, FP4, MI, NJ, SAVE_GU>), dim3((unsigned)blocks), dim3(GEMM_THREADS), 0, l.s, l.g);
 }
 enum class MxTileSize { R64xC128, R64xC256, R128xC256 };  // rows, weight rows of a workgroup

@@ -53,10 +53,25 @@ int check(const char* who, const void* a, const uint8_t* a_scale, int fmt, const
   KMOE_REQUIRE((a_rows + 1) * lda < (int64_t)1 << 31 && 257 * lda < (int64_t)1 << 31 &&
                    (int64_t)round_up(K, STEP) * 128 < (int64_t)1 << 31,
                KMOE_ERR_SHAPE, "%s: operand too large for 32-bit offsets (%lld rows, K=%d)", who, (long long)a_rows, K);
-  // a launch takes 2^24 workgroups of 256, 2^23 of 512
-  KMOE_REQUIRE((max_rows / SMALL_ROWS + E) * (int64_t)std::max(round_up(F, 128) / 32, round_up(d, 256) / 32) < 1 << 23,
-               KMOE_ERR_SHAPE, "%s: grid too large", who);
   return KMOE_OK;
+}
+
+// Picks a product's kernel and launches it, if its grid is one that a launch takes (fewer than 2^24 workgroups of
+// 256; the small-row kernel's is a few per CU).
+int launch(const char* who, const MxLaunch& l, bool gate_up, bool fp4) {
+  if (small_product(gate_up, l.max_rows, l.g.E, l.g.b_tiles)) {
+    launch_mx_small(l, gate_up, fp4);
+    return kmoe::check_launch(who);
+  }
+  const MxTileSize t = tile_size(fp4, l.max_rows, l.g.E, l.g.b_tiles);
+  const int rows = t == MxTileSize::R128xC256 ? 128 : 64, split = t == MxTileSize::R64xC128 ? 2 : 1;
+  KMOE_REQUIRE(mx_workgroups(l.max_rows, l.g.E, l.g.b_tiles, rows, split) < 1 << 24, KMOE_ERR_SHAPE, "%s: grid too large",
+               who);
+  if (gate_up)
+    launch_mx_gate_up(l, fp4, t);
+  else
+    launch_mx_down(l, fp4, t);
+  return kmoe::check_launch(who);
 }
 
 }  // namespace
@@ -90,11 +105,7 @@ extern "C" int kmoe_gemm_gate_up_mx(const void* xq, const uint8_t* x_scale, int 
   l.g.ldc = Fp;
   l.max_rows = max_rows;
   l.s = kmoe::as_stream(stream);
-  if (small_product(true, max_rows, E, l.g.b_tiles))
-    launch_mx_small(l, true, fmt == KMOE_DTYPE_FP4_E2M1);
-  else
-    launch_mx_gate_up(l, fmt == KMOE_DTYPE_FP4_E2M1, tile_size(fmt == KMOE_DTYPE_FP4_E2M1, max_rows, E, l.g.b_tiles));
-  return kmoe::check_launch("kmoe_gemm_gate_up_mx");
+  return launch("kmoe_gemm_gate_up_mx", l, true, fmt == KMOE_DTYPE_FP4_E2M1);
 }
 
 extern "C" int kmoe_gemm_down_mx(const void* hq, const uint8_t* h_scale, int fmt, const int32_t* offsets, int E, int d,
@@ -119,9 +130,5 @@ extern "C" int kmoe_gemm_down_mx(const void* hq, const uint8_t* h_scale, int fmt
   l.g.n_valid = d;
   l.max_rows = max_rows;
   l.s = kmoe::as_stream(stream);
-  if (small_product(false, max_rows, E, l.g.b_tiles))
-    launch_mx_small(l, false, fmt == KMOE_DTYPE_FP4_E2M1);
-  else
-    launch_mx_down(l, fmt == KMOE_DTYPE_FP4_E2M1, tile_size(fmt == KMOE_DTYPE_FP4_E2M1, max_rows, E, l.g.b_tiles));
-  return kmoe::check_launch("kmoe_gemm_down_mx");
+  return launch("kmoe_gemm_down_mx", l, false, fmt == KMOE_DTYPE_FP4_E2M1);
 }

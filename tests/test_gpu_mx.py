@@ -768,3 +768,21 @@ def test_rows_far_past_the_last_are_zeros(dev, fmt, A):
     h = ops.gemm_gate_up_mx(x, token.to(dev), off, pw, A)
     good = [i for i in range(A) if i not in bad]
     assert not h.q[bad].any() and bool(h.q[good].any(1).all())
+
+
+@pytest.mark.parametrize("mx", ["w4a8", "w4a4"])
+def test_more_rows_than_a_grid_of_small_slots(dev, mx):
+    """400000 tokens of top-8 at F 2816: 3.2 M routed rows, of which 32-row slots of 32 columns would be more
+    workgroups than a launch takes; the kernel that runs needs a sixteenth of them.  Tokens among
+    them are those of a call of their own."""
+    T, k, E, d, F = 400_000, 8, 8, 64, 2816
+    pw = ops.pack_weights_mx(*weights(dev, E, d, F))
+    g = torch.Generator(device=dev).manual_seed(3)
+    x = torch.empty(T, d, device=dev, dtype=BF).normal_(generator=g)
+    idx = torch.argsort(torch.rand(T, E, device=dev, generator=g), 1)
+    w = torch.rand(T, k, device=dev, generator=g)
+    y, counts, _ = ops.mx_experts(x, idx, w, pw, ops.MX_EXPERTS[mx])
+    assert int(counts.sum()) == T * k
+    few = torch.tensor(list(range(0, T, T // 300)) + [T - 1], device=dev)
+    want, _, _ = ops.mx_experts(x[few], idx[few], w[few], pw, ops.MX_EXPERTS[mx])
+    assert torch.equal(y[few], want)
