@@ -387,8 +387,36 @@ done:
   }
 }
 
-// dlogits (accumulate: added to).  L lanes per token; f32 throughout: no comparisons.  4099
-// tokens, 48 experts, top-6 4.8 us: a launch's latency and one chain of reductions.
+// v of lane J of the lane's row of 16 (L 8: of its half row).
+template <int L, int J>
+__device__ __forceinline__ int entry(int v) {
+  const int lo = __builtin_amdgcn_update_dpp(0, v, 0x150 + J, 0xF, 0xF, false);  // row_newbcast
+  if constexpr (L >= 16) return lo;
+  const int hi = __builtin_amdgcn_update_dpp(0, v, 0x150 + J + 8, 0xF, 0xF, false);
+  return threadIdx.x & 8 ? hi : lo;
+}
+// f(j) for the entries j < k, two at a time (with an odd k one past it, an entry without an expert).
+template <int J = 0, class Fn>
+__device__ __forceinline__ void each_entry(int k, Fn&& f) {
+  if constexpr (J < MAX_K) {
+    if (J >= k) return;
+    f(std::integral_constant<int, J>{});
+    f(std::integral_constant<int, J + 1>{});
+    each_entry<J + 2>(k, f);
+  }
+}
+
+// dlogits (accumulate: added to).  L lanes per token; f32 throughout: no comparisons.  Differences of
+// sums that nearly cancel are written as sums of differences, with P = sum of the chosen s, S = P + tiny,
+// D_e = sum_i s_i (dw_e - dw_i) over the chosen i, m = sum_i s_i dw_i / S:
+//   renorm   ds_e = a / S (D_e + tiny dw_e) / S;  sum_i ds_i s_i = a tiny m / S
+//   without  softmax: ds_e - sum_i ds_i s_i = a (D_e + dw_e U), U the sum of the other experts' s
+// so that gradients that vanish (one expert, or equal dw, renormalised) are not the roundings of
+// the terms: sigmoid, 16 experts, top-1 had up to 5e-7 of those.  s (1 - s) of the sigmoid
+// comes from exp(-|l|) for the same reason.  A lane loads one entry of the choice, and the
+// others come by moves within its row of lanes.  A launch's latency and one chain of reductions: 4099
+// tokens, 48 experts, top-6 in a replayed graph 3.5 us (with sums over the lanes in
+// place of the entries 3.8), 16384 tokens, 64 experts, top-8 6.5 (8.3).
 template <int L>
 __global__ __launch_bounds__(256) void route_bwd_kernel(const float* __restrict__ logits, const int64_t* __restrict__ idx,
                                                         const float* __restrict__ dw, int64_t T, int E, int k, bool sigmoid,
@@ -398,36 +426,53 @@ __global__ __launch_bounds__(256) void route_bwd_kernel(const float* __restrict_
   const int64_t t = (int64_t)blockIdx.x * (256 / L) + threadIdx.x / L;
   const bool live = t < T, on = live && e < E;
   const float l = on ? logits[t * E + e] : -INFINITY;
-  float s;
+  // the token's choice, one entry j a lane (copies in each row of 16 lanes): its expert (an id out of
+  // range: none) and the gradient of its weight
+  constexpr int ROW = L < 16 ? L : 16;
+  const int j0 = threadIdx.x % ROW;
+  const int64_t id = live && j0 < k ? idx[t * k + j0] : -1;
+  const int ej = id >= 0 && id < E ? (int)id : -1;
+  const float gj = ej >= 0 ? dw[t * k + j0] : 0.0f;
+  // this lane's own gradient, 0 where it was not chosen
+  float g = 0.0f;
+  bool chosen = false;
+  each_entry(k, [&](auto j) {  // (the broadcasts by all lanes: none under a condition of the lane's own)
+    const int ev = entry<L, decltype(j)::value>(ej);
+    const float gv = __int_as_float(entry<L, decltype(j)::value>(__float_as_int(gj)));
+    g = ev == e ? gv : g;
+    chosen = chosen || ev == e;
+  });
+  float s, ds_dl = 0.0f;  // score; its own derivative (sigmoid)
   if (sigmoid) {
-    s = on ? 1.0f / (1.0f + expf(-l)) : 0.0f;
+    const float q = expf(-fabsf(l)), r = 1.0f / (1.0f + q);
+    s = on ? (l < 0.0f ? q * r : r) : 0.0f;
+    ds_dl = q * r * r;
   } else {
     const float m = group_max<L>(l);
     s = on && m != -INFINITY ? expf(l - m) : 0.0f;
     const float z = group_sum<L>(s);
     s = m == -INFINITY ? 0.0f : s / z;
   }
-  // this lane's gradient of the weight, 0 where it was not chosen
-  float g = 0.0f;
-  bool chosen = false;
-  if (on)
-    for (int j = 0; j < k; ++j)
-      if (idx[t * k + j] == e) {
-        g = dw[t * k + j];
-        chosen = true;
-      }
-  float ds = scale * g;
-  if (renorm) {
-    const float S = group_sum<L>(chosen ? s : 0.0f) + (float)ROUTE_TINY;
-    const float mean = group_sum<L>(chosen ? g * s : 0.0f) / S;
-    ds = chosen ? scale / S * (g - mean) : 0.0f;
-  }
+  const float si = __shfl(s, max(ej, 0), L), sj = ej >= 0 ? si : 0.0f;
+  float S = 0.0f, D = 0.0f, M = 0.0f;
+  each_entry(k, [&](auto j) {  // entries without an expert add zeros
+    const float sv = __int_as_float(entry<L, decltype(j)::value>(__float_as_int(sj)));
+    const float gv = __int_as_float(entry<L, decltype(j)::value>(__float_as_int(gj)));
+    S += sv;
+    D = fmaf(sv, g - gv, D);
+    M = fmaf(sv, gv, M);
+  });
   float dl;
-  if (sigmoid) {
-    dl = chosen ? ds * s * (1.0f - s) : 0.0f;
+  if (renorm) {
+    // (s / S and ds_dl / S are at most 1 for a chosen expert, also where S is tiny)
+    S += (float)ROUTE_TINY;
+    const float c = chosen ? fmaf(g, (float)ROUTE_TINY, D) / S : 0.0f;
+    dl = !sigmoid ? scale * (s / S) * (c - M / S * (float)ROUTE_TINY) : chosen ? scale * (ds_dl / S) * c : 0.0f;
+  } else if (sigmoid) {
+    dl = chosen ? scale * g * ds_dl : 0.0f;
   } else {
-    const float q = group_sum<L>(chosen ? ds * s : 0.0f);
-    dl = s * (ds - q);
+    const float U = group_sum<L>(chosen ? 0.0f : s);
+    dl = scale * s * fmaf(g, U, D);
   }
   if (on) dlogits[t * E + e] = accumulate ? dlogits[t * E + e] + dl : dl;
 }

@@ -275,3 +275,42 @@ def test_refusals(dev):
         ops.route_topk(lg[0], 2)
     with pytest.raises(ValueError):
         ops.route_topk_bwd(lg, torch.zeros(4, 2, dtype=torch.int64, device=dev), torch.zeros(4, 3, device=dev))
+
+
+@pytest.mark.parametrize("scores,renorm", [("softmax", True), ("softmax", False), ("sigmoid", True), ("sigmoid", False)])
+@pytest.mark.parametrize("k,same,std", [(1, False, 1.5), (4, True, 1.5), (4, False, 6.0), (8, False, 1.5)])
+def test_gradients_that_nearly_vanish(dev, scores, renorm, k, same, std):
+    """One expert, or equal gradients of the weights, renormalised: only the 1e-20 is left of the
+    gradient.  Confident scores: 1 - s is small.  Held against the terms that remain when the sums
+    that cancel are taken exactly, not against the largest gradient."""
+    T, E, scale, tiny = 2000, 16, 2.5, 1e-20
+    lg = logits_of(dev, T, E, seed=k, std=std)
+    idx = ops.route_topk(lg, k, scores=scores, renorm=renorm).idx
+    dw = logits_of(dev, T, 1 if same else k, seed=9).expand(T, k).contiguous()
+    got = ops.route_topk_bwd(lg, idx, dw, scores, renorm, scale).double().cpu()
+    l, i, g = lg.double().cpu(), idx.cpu(), dw.double().cpu()
+    s = torch.sigmoid(l) if scores == "sigmoid" else torch.softmax(l, -1)
+    on = torch.zeros(T, E, dtype=torch.bool).scatter_(1, i, True)
+    ge = torch.zeros(T, E, dtype=torch.float64).scatter_(1, i, g)
+    sc = s.gather(1, i)
+    S = sc.sum(1, keepdim=True) + tiny
+    diff = ge[:, :, None] - g[:, None, :]                  # (T, E, k)
+    D, Dabs = (diff * sc[:, None, :]).sum(-1), (diff.abs() * sc[:, None, :]).sum(-1)
+    slope = s * torch.sigmoid(-l)
+    if renorm:
+        c, cabs = torch.where(on, (D + tiny * ge) / S, 0.0), torch.where(on, (Dabs + tiny * ge.abs()) / S, 0.0)
+        m, mabs = (sc * g).sum(1, keepdim=True) / S, (sc * g.abs()).sum(1, keepdim=True) / S
+        want, terms = (slope / S * c, slope / S * cabs) if scores == "sigmoid" else (
+            s / S * (c - tiny * m), s / S * (cabs + tiny * mabs))
+    elif scores == "sigmoid":
+        want = terms = torch.where(on, ge * slope, 0.0)
+    else:
+        U = torch.where(on, 0.0, s).sum(1, keepdim=True)
+        want, terms = s * (D + ge * U), s * (Dabs + ge.abs() * U)
+    # scores: the logit's difference to the largest (below 32 at std 1.5, 64 at 6, asserted) is rounded, the
+    # exponential off by 2 half steps of f32, the sum of E and the quotient: far + E + 4 half steps;
+    # a term has at most three of them (s, S, s_i, or S twice), a difference, sums of E + k and eight products
+    far = 64 if std > 2 else 32
+    assert float((l.amax(1, keepdim=True) - l).max()) < far
+    steps = 3 * (far + E + 4) + E + k + 10
+    assert bool(((got - scale * want).abs() <= steps * HALF_F32 * scale * terms.abs() + 1e-37).all())
