@@ -44,6 +44,7 @@ from torch.autograd.function import once_differentiable
 
 from . import backward as _bwd
 from . import ops
+from .derived import Sources, kept
 from .mod import MoDRouter, mod_ffn
 from .moe import MoELayer, _once
 
@@ -177,8 +178,8 @@ class MoEFFNBlock(nn.Module):
         ge = self.ffn.grouped_experts
         w_in, w_out = self.ffn.router.router[0].weight, self.ffn.router.router[2].weight
         g = self.ffn_norm.weight
-        key = tuple((t.data_ptr(), t._version, t.device) for t in (g, w_in, w_out, ge.w1, ge.w2, ge.w3))
-        if self._fused_cache is None or self._fused_cache[0] != key:
+        ws = (g, w_in, w_out, ge.w1, ge.w2, ge.w3)
+        if not kept(self._fused_cache, ws):
             with torch.no_grad():
                 gf = g.detach().float()
                 w_in_g = (w_in.detach().float() * gf[None, :]).to(torch.bfloat16).contiguous()
@@ -188,7 +189,7 @@ class MoEFFNBlock(nn.Module):
                 w2g = ge.w2.detach().float() * gf[None, :, None]
                 pw = ops.pack_weights(w1g, w2g, ge.w3.detach(), fp8=False)
                 del w1g, w2g
-            self._fused_cache = (key, w_in_g, w_out_b, pw)
+            self._fused_cache = (Sources(ws), w_in_g, w_out_b, pw)
         return self._fused_cache[1:]
 
     def _train_fusable(self, h: torch.Tensor) -> bool:

@@ -1,0 +1,61 @@
+"""Values made from weights (packed copies, casts, folds), kept until a weight changes.
+
+What torch counts is seen: a write by an operation (an optimizer's step, copy_), a parameter that
+is replaced, a .data that is assigned.  What it does not count is not: a write through .data or
+a view of it, by a replayed graph, or by code outside of torch; `weights_changed` is for those.
+"""
+from __future__ import annotations
+
+from torch.multiprocessing.reductions import StorageWeakRef
+
+
+class Sources:
+    """The tensors that a value was made from: their addresses, version counters and storages.  An
+    address and a counter alone say nothing, as the allocator gives a freed weight's place to
+    the next one and counters start at zero; the weak references hold on to no memory, but to the
+    storages' identities.  Equal to nothing once copied or pickled with its module, whose
+    copy has other weights."""
+    __slots__ = ("_flags", "_at", "_refs")
+
+    def __init__(self, tensors, flags=()):
+        self._flags = flags
+        self._refs = tuple(StorageWeakRef(t.untyped_storage()) for t in tensors)
+        self._at = tuple((t.data_ptr(), t._version, r.cdata) for t, r in zip(tensors, self._refs))
+
+    def same(self, tensors, flags=()) -> bool:
+        if flags != self._flags or len(tensors) != len(self._at):
+            return False
+        for t, (ptr, version, storage) in zip(tensors, self._at):
+            if t._version != version or t.data_ptr() != ptr or t.untyped_storage()._cdata != storage:
+                return False
+        return True
+
+    def __reduce__(self):
+        return _gone, ()
+
+    def __deepcopy__(self, memo):
+        return _gone()
+
+
+def _gone() -> Sources:
+    return Sources((), None)
+
+
+def kept(entry, tensors, flags=()) -> bool:
+    """Whether the entry (Sources, value, ...) was made from these tensors as they are."""
+    return entry is not None and isinstance(entry[0], Sources) and entry[0].same(tensors, flags)
+
+
+_ENTRIES = ("_packed", "_bwd_cache", "_bf16_cache", "_fused_cache")
+FREE = {}  # entries of functions that take weights and belong to no module
+
+
+def weights_changed(module) -> None:
+    """Forget what was made from the weights of `module` and the modules in it: its next call makes
+    it again.  For writes that torch does not count: through .data, by replays of a captured
+    optimizer step, by other code on the memory."""
+    FREE.clear()
+    for m in module.modules():
+        for name in _ENTRIES:
+            if m.__dict__.get(name) is not None:
+                setattr(m, name, None)

@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import torch
 
-from . import _lib, ops
+from . import _lib, derived, ops
 
 
 def is_kernel_available() -> bool:
@@ -22,17 +22,13 @@ def is_kernel_available() -> bool:
         return False
 
 
-_PACK_CACHE = {}
-
-
 def _packed(W1, W2, W3):
-    key = tuple((w.data_ptr(), w._version) for w in (W1, W2, W3))
-    pw = _PACK_CACHE.get(key)
-    if pw is None:
-        _PACK_CACHE.clear()
-        pw = ops.pack_weights(W1, W2, W3)
-        _PACK_CACHE[key] = pw
-    return pw
+    ws = (W1, W2, W3)
+    entry = derived.FREE.get("grouped_swiglu_forward")
+    if not derived.kept(entry, ws):
+        derived.FREE.clear()  # (its memory first)
+        entry = derived.FREE["grouped_swiglu_forward"] = (derived.Sources(ws), ops.pack_weights(W1, W2, W3))
+    return entry[1]
 
 
 def grouped_swiglu_forward(sorted_inputs, W1, W2, W3, sorted_expert_ids, seg_starts, seg_ends,

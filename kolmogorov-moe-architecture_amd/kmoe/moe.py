@@ -34,6 +34,7 @@ from . import _lib
 from . import backward as _bwd
 from . import ops
 from .config import AdvancedMoEConfig
+from .derived import Sources, kept
 
 ROUTER_HIDDEN = 128  # moe.py:346
 
@@ -80,10 +81,9 @@ class _RouterMLP(nn.Module):
     def _bwd_weights(self):
         """Backward packed w_in (rebuilt only when it changed)."""
         w_in = self.router[0].weight
-        key = (w_in.data_ptr(), w_in._version)
-        if self._bwd_cache is None or self._bwd_cache[0] != key:
+        if not kept(self._bwd_cache, (w_in,)):
             with torch.no_grad():
-                self._bwd_cache = (key, _bwd.pack_bwd_weights(None, None, None, w_in))
+                self._bwd_cache = (Sources((w_in,)), _bwd.pack_bwd_weights(None, None, None, w_in))
         return self._bwd_cache[1]
 
     def _trainable(self, x) -> bool:
@@ -93,9 +93,8 @@ class _RouterMLP(nn.Module):
         w_in, w_out = self.router[0].weight, self.router[2].weight
         if w_in.dtype == torch.bfloat16:
             return w_in.detach(), w_out.detach()
-        key = (w_in.data_ptr(), w_in._version, w_out.data_ptr(), w_out._version)
-        if self._bf16_cache is None or self._bf16_cache[0] != key:
-            self._bf16_cache = (key, w_in.detach().to(torch.bfloat16).contiguous(),
+        if not kept(self._bf16_cache, (w_in, w_out)):
+            self._bf16_cache = (Sources((w_in, w_out)), w_in.detach().to(torch.bfloat16).contiguous(),
                                 w_out.detach().to(torch.bfloat16).contiguous())
         return self._bf16_cache[1], self._bf16_cache[2]
 
@@ -253,12 +252,6 @@ class _PackedExperts(nn.Module):
             ws = self.w1, self.w2, self.w3
         return ws if ws[2] is not None else ws[:2]
 
-    def _packed_key(self):
-        key = [self.use_fp8, self.mx]
-        for w in self._weights():
-            key += (w.data_ptr(), w._version, w.device)
-        return key
-
     @property
     def mx_act(self) -> Optional[str]:
         """Element type of the microscaled experts' activations, None without them."""
@@ -331,15 +324,15 @@ class _PackedExperts(nn.Module):
             raise ValueError("kmoe: packed-weight files hold gated (swiglu) bf16 or fp8 experts only")
         if (pw.E, pw.d, pw.F, pw.fp8) != (self.n_experts, self.d_model, self.d_ff, self.use_fp8):
             raise ValueError("kmoe: packed weights do not match the experts' shapes / fp8 mode")
-        self._packed = (self._packed_key(), pw)
+        self._packed = (Sources(self._weights(), (self.use_fp8, self.mx)), pw)
 
     def bwd_packed(self) -> _bwd.BwdWeights:
         """Backward packed weights (no router part), rebuilt only when a parameter changed."""
-        key = tuple((w.data_ptr(), w._version) for w in self._weights()) + (self.use_fp8, self.mx)
+        ws, mode = self._weights(), (self.use_fp8, self.mx)
         cache = getattr(self, "_bwd_cache", None)
-        if cache is None or cache[0] != key:
+        if not kept(cache, ws, mode):
             with torch.no_grad():
-                cache = (key, _bwd.pack_bwd_weights(*self.bwd_source_weights(), None))
+                cache = (Sources(ws, mode), _bwd.pack_bwd_weights(*self.bwd_source_weights(), None))
             self._bwd_cache = cache
         return cache[1]
 
@@ -353,9 +346,9 @@ class _PackedExperts(nn.Module):
         return not self.d_ff % 8
 
     def packed(self) -> ops.PackedWeights:
-        """Packed weights, rebuilt only when a parameter changed (version counters)."""
-        key = self._packed_key()
-        if self._packed is None or self._packed[0] != key:
+        """Packed weights, rebuilt only when a parameter changed (see `derived`)."""
+        ws, mode = self._weights(), (self.use_fp8, self.mx)
+        if not kept(self._packed, ws, mode):
             with torch.no_grad():
                 if self.mx_act is not None:
                     pw = ops.pack_weights_mx(self.w1.detach(), self.w2.detach(), self.w3.detach())
@@ -365,7 +358,7 @@ class _PackedExperts(nn.Module):
                     pw = ops.pack_weights_plain(self.w1.detach(), self.w2.detach())
                 else:
                     pw = ops.pack_weights(self.w1.detach(), self.w2.detach(), self.w3.detach(), fp8=self.use_fp8)
-            self._packed = (key, pw)
+            self._packed = (Sources(ws, mode), pw)
         return self._packed[1]
 
 
@@ -841,11 +834,11 @@ class MoELayer(nn.Module):
         """Backward packed weights, rebuilt only when a parameter changed."""
         ge = self.grouped_experts if self.grouped_experts is not None else self.grouped_experts_ec
         w_in = self.router.router[0].weight
-        key = tuple((w.data_ptr(), w._version) for w in ge._weights() + (w_in,)) + (ge.use_fp8, ge.mx)
+        ws, mode = ge._weights() + (w_in,), (ge.use_fp8, ge.mx)
         cache = getattr(self, "_bwd_cache", None)
-        if cache is None or cache[0] != key:
+        if not kept(cache, ws, mode):
             with torch.no_grad():
-                cache = (key, _bwd.pack_bwd_weights(*ge.bwd_source_weights(), w_in))
+                cache = (Sources(ws, mode), _bwd.pack_bwd_weights(*ge.bwd_source_weights(), w_in))
             self._bwd_cache = cache
         return cache[1]
 

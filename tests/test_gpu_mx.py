@@ -786,3 +786,38 @@ def test_more_rows_than_a_grid_of_small_slots(dev, mx):
     few = torch.tensor(list(range(0, T, T // 300)) + [T - 1], device=dev)
     want, _, _ = ops.mx_experts(x[few], idx[few], w[few], pw, ops.MX_EXPERTS[mx])
     assert torch.equal(y[few], want)
+
+
+@pytest.mark.parametrize("mx", [None, "w4a8"])
+@pytest.mark.parametrize("how", ["parameter", "data", "written"])
+def test_outputs_follow_the_weights(dev, mx, how):
+    """Weights that are replaced (the new ones in the freed ones' memory), assigned through .data, or written
+    there and told of: the layer's output, and its gradients, are those of a layer that never had others."""
+    cfg = kmoe.AdvancedMoEConfig(d_model=128, n_experts=4, moe_top_k=2, d_ff_expert=64, moe_mx=mx)
+    torch.manual_seed(1)
+    layer, other = kmoe.MoELayer(cfg).to(dev), kmoe.MoELayer(cfg).to(dev)
+    x, dy = rnd(dev, 1, 30, 128, dtype=torch.float32), rnd(dev, 1, 30, 128, seed=1, dtype=torch.float32)
+
+    def run(m):
+        xg = x.clone().requires_grad_(True)
+        y = m(xg)
+        with torch.no_grad():
+            return [m(x), y.detach()] + list(torch.autograd.grad(y, [xg] + list(m.parameters()), dy))
+    run(layer)
+    for (name, p), q in zip(layer.named_parameters(), other.parameters()):
+        if how == "written":
+            p.data.copy_(q)
+            continue
+        shape = p.shape
+        p.data = torch.empty(0, device=dev)  # its memory is the next one's
+        new = torch.empty(shape, device=dev)
+        new.data.copy_(q)
+        if how == "data":
+            p.data = new
+        else:
+            owner, _, leaf = name.rpartition(".")
+            setattr(layer.get_submodule(owner), leaf, torch.nn.Parameter(new))
+    if how == "written":
+        kmoe.weights_changed(layer)
+    for u, v in zip(run(layer), run(other)):
+        assert torch.equal(u, v)
