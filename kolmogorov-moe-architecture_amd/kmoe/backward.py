@@ -26,6 +26,7 @@ import torch
 
 from . import _lib, ops
 from ._lib import ptr
+from .derived import capturing
 
 _BF16 = torch.bfloat16
 
@@ -332,9 +333,12 @@ def _ones(T, fan, dev):
     key = (T, fan, str(dev))
     t = _ONES.get(key)
     if t is None:
+        t = torch.ones(T, fan, device=dev, dtype=torch.float32)
+        if capturing(t):
+            return t  # without contents before a replay
         if len(_ONES) > 16:
             _ONES.clear()
-        t = _ONES[key] = torch.ones(T, fan, device=dev, dtype=torch.float32)
+        _ONES[key] = t
     return t
 
 

@@ -44,7 +44,7 @@ from torch.autograd.function import once_differentiable
 
 from . import backward as _bwd
 from . import ops
-from .derived import Sources, kept
+from .derived import derived
 from .mod import MoDRouter, mod_ffn
 from .moe import MoELayer, _once
 
@@ -178,19 +178,16 @@ class MoEFFNBlock(nn.Module):
         ge = self.ffn.grouped_experts
         w_in, w_out = self.ffn.router.router[0].weight, self.ffn.router.router[2].weight
         g = self.ffn_norm.weight
-        ws = (g, w_in, w_out, ge.w1, ge.w2, ge.w3)
-        if not kept(self._fused_cache, ws):
-            with torch.no_grad():
-                gf = g.detach().float()
-                w_in_g = (w_in.detach().float() * gf[None, :]).to(torch.bfloat16).contiguous()
-                w_out_b = w_out.detach().to(torch.bfloat16).contiguous()
-                # folded in f32, rounded to bf16 once by the pack
-                w1g = ge.w1.detach().float() * gf[None, :, None]
-                w2g = ge.w2.detach().float() * gf[None, :, None]
-                pw = ops.pack_weights(w1g, w2g, ge.w3.detach(), fp8=False)
-                del w1g, w2g
-            self._fused_cache = (Sources(ws), w_in_g, w_out_b, pw)
-        return self._fused_cache[1:]
+
+        def fold():
+            gf = g.detach().float()
+            w_in_g = (w_in.detach().float() * gf[None, :]).to(torch.bfloat16).contiguous()
+            w_out_b = w_out.detach().to(torch.bfloat16).contiguous()
+            # folded in f32, rounded to bf16 once by the pack
+            w1g = ge.w1.detach().float() * gf[None, :, None]
+            w2g = ge.w2.detach().float() * gf[None, :, None]
+            return w_in_g, w_out_b, ops.pack_weights(w1g, w2g, ge.w3.detach(), fp8=False)
+        return derived(self.__dict__, "_fused_cache", (g, w_in, w_out, ge.w1, ge.w2, ge.w3), fold)
 
     def _train_fusable(self, h: torch.Tensor) -> bool:
         """Whether the forward records the fused training backward (_BlockTrainFn)."""

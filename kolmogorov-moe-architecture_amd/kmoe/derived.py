@@ -3,9 +3,12 @@
 What torch counts is seen: a write by an operation (an optimizer's step, copy_), a parameter that
 is replaced, a .data that is assigned.  What it does not count is not: a write through .data or
 a view of it, by a replayed graph, or by code outside of torch; `weights_changed` is for those.
+
+In a capture nothing runs, so what is made there is not kept: it has no contents before a replay.
 """
 from __future__ import annotations
 
+import torch
 from torch.multiprocessing.reductions import StorageWeakRef
 
 
@@ -41,9 +44,22 @@ def _gone() -> Sources:
     return Sources((), None)
 
 
-def kept(entry, tensors, flags=()) -> bool:
-    """Whether the entry (Sources, value, ...) was made from these tensors as they are."""
-    return entry is not None and isinstance(entry[0], Sources) and entry[0].same(tensors, flags)
+def capturing(t) -> bool:
+    """Whether work on t's device is being captured into a graph."""
+    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+
+
+def derived(owner: dict, name: str, tensors, make, flags=()):
+    """What make() made from the tensors (and the flags), kept in owner[name] (a module's __dict__)
+    until one of them changes."""
+    entry = owner.get(name)
+    if entry is not None and isinstance(entry[0], Sources) and entry[0].same(tensors, flags):
+        return entry[1]
+    with torch.no_grad():
+        value = make()
+    if not capturing(tensors[0]):
+        owner[name] = (Sources(tensors, flags), value)
+    return value
 
 
 _ENTRIES = ("_packed", "_bwd_cache", "_bf16_cache", "_fused_cache")
@@ -54,7 +70,7 @@ def weights_changed(module) -> None:
     """Forget what was made from the weights of `module` and the modules in it: its next call makes
     it again.  For writes that torch does not count: through .data, by replays of a captured
     optimizer step, by other code on the memory."""
-    FREE.clear()
+    FREE.pop("grouped_swiglu_forward", None)
     for m in module.modules():
         for name in _ENTRIES:
             if m.__dict__.get(name) is not None:

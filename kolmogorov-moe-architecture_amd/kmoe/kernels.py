@@ -23,12 +23,7 @@ def is_kernel_available() -> bool:
 
 
 def _packed(W1, W2, W3):
-    ws = (W1, W2, W3)
-    entry = derived.FREE.get("grouped_swiglu_forward")
-    if not derived.kept(entry, ws):
-        derived.FREE.clear()  # (its memory first)
-        entry = derived.FREE["grouped_swiglu_forward"] = (derived.Sources(ws), ops.pack_weights(W1, W2, W3))
-    return entry[1]
+    return derived.derived(derived.FREE, "grouped_swiglu_forward", (W1, W2, W3), lambda: ops.pack_weights(W1, W2, W3))
 
 
 def grouped_swiglu_forward(sorted_inputs, W1, W2, W3, sorted_expert_ids, seg_starts, seg_ends,

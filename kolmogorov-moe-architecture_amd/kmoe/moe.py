@@ -34,7 +34,7 @@ from . import _lib
 from . import backward as _bwd
 from . import ops
 from .config import AdvancedMoEConfig
-from .derived import Sources, kept
+from .derived import Sources, derived
 
 ROUTER_HIDDEN = 128  # moe.py:346
 
@@ -81,10 +81,7 @@ class _RouterMLP(nn.Module):
     def _bwd_weights(self):
         """Backward packed w_in (rebuilt only when it changed)."""
         w_in = self.router[0].weight
-        if not kept(self._bwd_cache, (w_in,)):
-            with torch.no_grad():
-                self._bwd_cache = (Sources((w_in,)), _bwd.pack_bwd_weights(None, None, None, w_in))
-        return self._bwd_cache[1]
+        return derived(self.__dict__, "_bwd_cache", (w_in,), lambda: _bwd.pack_bwd_weights(None, None, None, w_in))
 
     def _trainable(self, x) -> bool:
         return torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters()))
@@ -93,10 +90,8 @@ class _RouterMLP(nn.Module):
         w_in, w_out = self.router[0].weight, self.router[2].weight
         if w_in.dtype == torch.bfloat16:
             return w_in.detach(), w_out.detach()
-        if not kept(self._bf16_cache, (w_in, w_out)):
-            self._bf16_cache = (Sources((w_in, w_out)), w_in.detach().to(torch.bfloat16).contiguous(),
-                                w_out.detach().to(torch.bfloat16).contiguous())
-        return self._bf16_cache[1], self._bf16_cache[2]
+        return derived(self.__dict__, "_bf16_cache", (w_in, w_out),
+                       lambda: tuple(w.detach().to(torch.bfloat16).contiguous() for w in (w_in, w_out)))
 
 
 def _route_spec(config) -> Optional[ops.RouteSpec]:
@@ -328,13 +323,8 @@ class _PackedExperts(nn.Module):
 
     def bwd_packed(self) -> _bwd.BwdWeights:
         """Backward packed weights (no router part), rebuilt only when a parameter changed."""
-        ws, mode = self._weights(), (self.use_fp8, self.mx)
-        cache = getattr(self, "_bwd_cache", None)
-        if not kept(cache, ws, mode):
-            with torch.no_grad():
-                cache = (Sources(ws, mode), _bwd.pack_bwd_weights(*self.bwd_source_weights(), None))
-            self._bwd_cache = cache
-        return cache[1]
+        return derived(self.__dict__, "_bwd_cache", self._weights(),
+                       lambda: _bwd.pack_bwd_weights(*self.bwd_source_weights(), None), (self.use_fp8, self.mx))
 
     def _trainable(self, *inputs) -> bool:
         """Whether a direct call records a backward through the HIP kernels."""
@@ -345,21 +335,18 @@ class _PackedExperts(nn.Module):
             return False
         return not self.d_ff % 8
 
+    def _pack(self):
+        if self.mx_act is not None:
+            return ops.pack_weights_mx(self.w1.detach(), self.w2.detach(), self.w3.detach())
+        if not self.gated:
+            if self.use_fp8:
+                raise NotImplementedError("kmoe: fp8 non-gated experts are not implemented")
+            return ops.pack_weights_plain(self.w1.detach(), self.w2.detach())
+        return ops.pack_weights(self.w1.detach(), self.w2.detach(), self.w3.detach(), fp8=self.use_fp8)
+
     def packed(self) -> ops.PackedWeights:
         """Packed weights, rebuilt only when a parameter changed (see `derived`)."""
-        ws, mode = self._weights(), (self.use_fp8, self.mx)
-        if not kept(self._packed, ws, mode):
-            with torch.no_grad():
-                if self.mx_act is not None:
-                    pw = ops.pack_weights_mx(self.w1.detach(), self.w2.detach(), self.w3.detach())
-                elif not self.gated:
-                    if self.use_fp8:
-                        raise NotImplementedError("kmoe: fp8 non-gated experts are not implemented")
-                    pw = ops.pack_weights_plain(self.w1.detach(), self.w2.detach())
-                else:
-                    pw = ops.pack_weights(self.w1.detach(), self.w2.detach(), self.w3.detach(), fp8=self.use_fp8)
-            self._packed = (Sources(ws, mode), pw)
-        return self._packed[1]
+        return derived(self.__dict__, "_packed", self._weights(), self._pack, (self.use_fp8, self.mx))
 
 
 class GroupedExperts(_PackedExperts):
@@ -834,13 +821,8 @@ class MoELayer(nn.Module):
         """Backward packed weights, rebuilt only when a parameter changed."""
         ge = self.grouped_experts if self.grouped_experts is not None else self.grouped_experts_ec
         w_in = self.router.router[0].weight
-        ws, mode = ge._weights() + (w_in,), (ge.use_fp8, ge.mx)
-        cache = getattr(self, "_bwd_cache", None)
-        if not kept(cache, ws, mode):
-            with torch.no_grad():
-                cache = (Sources(ws, mode), _bwd.pack_bwd_weights(*ge.bwd_source_weights(), w_in))
-            self._bwd_cache = cache
-        return cache[1]
+        return derived(self.__dict__, "_bwd_cache", ge._weights() + (w_in,),
+                       lambda: _bwd.pack_bwd_weights(*ge.bwd_source_weights(), w_in), (ge.use_fp8, ge.mx))
 
     def _train_forward(self, x2d, T, out_dtype, out_map=None, scale=None, residual=None, T_out=None,
                        keep_mask=None, keep_scale=1.0):

@@ -126,3 +126,28 @@ def test_freed_weights_are_not_held():
     assert s.same((t,)) and not storage.expired()
     del t
     assert storage.expired() and not s.same((torch.zeros(1000),))
+
+
+def test_captures(packs, monkeypatch):
+    """What is made in a capture is not kept.  (A capture is a stand-in here.)"""
+    from kmoe import backward, derived
+    state = dict(capturing=False)
+    for m in (derived, backward):
+        monkeypatch.setattr(m, "capturing", lambda t: state["capturing"])
+    ex = kmoe.GroupedExperts(E, D, F)
+    state["capturing"] = True
+    ex.packed()
+    assert ex._packed is None and len(packs) == 1
+    state["capturing"] = False
+    kept = ex.packed()
+    assert ex._packed[1] is kept and len(packs) == 2
+    state["capturing"] = True
+    assert ex.packed() is kept and ex.packed() is kept and len(packs) == 2
+    state["capturing"] = False
+    # constants of shapes
+    monkeypatch.setattr(backward, "_ONES", {})
+    state["capturing"] = True
+    assert backward._ones(3, 2, "cpu") is not backward._ones(3, 2, "cpu")
+    state["capturing"] = False
+    t = backward._ones(3, 2, "cpu")
+    assert backward._ones(3, 2, "cpu") is t

@@ -821,3 +821,25 @@ def test_outputs_follow_the_weights(dev, mx, how):
         kmoe.weights_changed(layer)
     for u, v in zip(run(layer), run(other)):
         assert torch.equal(u, v)
+
+
+@pytest.mark.parametrize("mx", [None, "w4a8"])
+def test_a_captured_forward_packs_nothing_for_others(dev, mx):
+    """The first call of a layer is captured: an eager call before any replay does not take the packed weights
+    that the capture recorded and nothing has written yet.  Replays follow."""
+    cfg = kmoe.AdvancedMoEConfig(d_model=128, n_experts=4, moe_top_k=2, d_ff_expert=64, moe_mx=mx)
+    layer, x = kmoe.MoELayer(cfg).to(dev), rnd(dev, 1, 30, 128, dtype=torch.float32)
+    want = None
+    with torch.no_grad():
+        other = kmoe.MoELayer(cfg).to(dev)
+        other.load_state_dict(layer.state_dict())
+        want = other(x)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = layer(x)
+        assert torch.equal(layer(x), want)
+        for _ in range(3):
+            y.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want) and torch.equal(layer(x), want)
