@@ -168,6 +168,14 @@ def _stage(name):
 
 
 _INDEX_CACHE: dict = {}
+_IN_GRAPHS: set = set()  # keys of constants that captured graphs read
+
+
+def _make_room(cache):
+    """At most 16 shapes at a time, and those that graphs read."""
+    if len(cache) > 16:
+        for key in [key for key in cache if key not in _IN_GRAPHS]:
+            del cache[key]
 
 
 def _index_tensors(T: int, k: int, dev, d: int):
@@ -185,9 +193,10 @@ def _index_tensors(T: int, k: int, dev, d: int):
         ones = torch.ones(T, k + 1, device=dev, dtype=torch.float32)
         extra = torch.arange(T * k, T * k + T, dtype=torch.int32).to(dev)[:, None]
         hit = (one_seg, segs, nseg, ones, extra)
-        if len(_INDEX_CACHE) > 16:
-            _INDEX_CACHE.clear()
+        _make_room(_INDEX_CACHE)
         _INDEX_CACHE[key] = hit
+    if capturing(hit[0]):
+        _IN_GRAPHS.add(key)
     return hit
 
 
@@ -336,9 +345,10 @@ def _ones(T, fan, dev):
         t = torch.ones(T, fan, device=dev, dtype=torch.float32)
         if capturing(t):
             return t  # without contents before a replay
-        if len(_ONES) > 16:
-            _ONES.clear()
+        _make_room(_ONES)
         _ONES[key] = t
+    elif capturing(t):
+        _IN_GRAPHS.add(key)
     return t
 
 

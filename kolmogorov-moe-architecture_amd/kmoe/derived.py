@@ -5,6 +5,8 @@ is replaced, a .data that is assigned.  What it does not count is not: a write t
 a view of it, by a replayed graph, or by code outside of torch; `weights_changed` is for those.
 
 In a capture nothing runs, so what is made there is not kept: it has no contents before a replay.
+What was made before and is used in a capture lives as long as its module, since the replays
+read it, also when later calls have made another.
 """
 from __future__ import annotations
 
@@ -49,11 +51,26 @@ def capturing(t) -> bool:
     return t.is_cuda and torch.cuda.is_current_stream_capturing()
 
 
+class _Held(list):
+    """Values that graphs read; a module's copy has no such graphs."""
+
+    def __reduce__(self):
+        return _Held, ()
+
+    def __deepcopy__(self, memo):
+        return _Held()
+
+
 def derived(owner: dict, name: str, tensors, make, flags=()):
     """What make() made from the tensors (and the flags), kept in owner[name] (a module's __dict__)
     until one of them changes."""
     entry = owner.get(name)
     if entry is not None and isinstance(entry[0], Sources) and entry[0].same(tensors, flags):
+        if not capturing(tensors[0]):
+            return entry[1]
+        held = owner.setdefault("_held", _Held())
+        if not any(v is entry[1] for v in held):
+            held.append(entry[1])
         return entry[1]
     with torch.no_grad():
         value = make()

@@ -129,7 +129,7 @@ def test_freed_weights_are_not_held():
 
 
 def test_captures(packs, monkeypatch):
-    """What is made in a capture is not kept.  (A capture is a stand-in here.)"""
+    """What is made in a capture is not kept; what a capture uses outlives its replacement.  (A capture is a stand-in here.)"""
     from kmoe import backward, derived
     state = dict(capturing=False)
     for m in (derived, backward):
@@ -144,10 +144,21 @@ def test_captures(packs, monkeypatch):
     state["capturing"] = True
     assert ex.packed() is kept and ex.packed() is kept and len(packs) == 2
     state["capturing"] = False
+    with torch.no_grad():
+        ex.w1.add_(1.0)
+    assert ex.packed() is not kept and [v for v in ex._held if v is kept] == [kept]
+    other = copy.deepcopy(ex)
+    assert not other._held
     # constants of shapes
     monkeypatch.setattr(backward, "_ONES", {})
+    monkeypatch.setattr(backward, "_IN_GRAPHS", set())
     state["capturing"] = True
     assert backward._ones(3, 2, "cpu") is not backward._ones(3, 2, "cpu")
     state["capturing"] = False
     t = backward._ones(3, 2, "cpu")
+    state["capturing"] = True
     assert backward._ones(3, 2, "cpu") is t
+    state["capturing"] = False
+    for n in range(40):
+        backward._ones(4 + n, 2, "cpu")
+    assert backward._ones(3, 2, "cpu") is t and len(backward._ONES) < 20

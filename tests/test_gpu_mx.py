@@ -843,3 +843,25 @@ def test_a_captured_forward_packs_nothing_for_others(dev, mx):
             g.replay()
             torch.cuda.synchronize()
             assert torch.equal(y, want) and torch.equal(layer(x), want)
+
+
+@pytest.mark.parametrize("mx", [None, "w4a8"])
+def test_a_captured_forward_keeps_its_weights(dev, mx):
+    """Weights packed before the capture, then moved: the replays give what the weights at the capture
+    gave, whatever the memory of packed weights that nobody else needs is used for."""
+    cfg = kmoe.AdvancedMoEConfig(d_model=128, n_experts=4, moe_top_k=2, d_ff_expert=64, moe_mx=mx)
+    layer, x = kmoe.MoELayer(cfg).to(dev), rnd(dev, 1, 30, 128, dtype=torch.float32)
+    with torch.no_grad():
+        want = layer(x)
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            y = layer(x)
+        for i in range(3):
+            for p in layer.parameters():
+                p.mul_(1.5)
+            now = layer(x)
+            junk = [torch.full((n << 8,), 0x7f, dtype=torch.uint8, device=dev) for n in range(1, 600)]
+            g.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, want) and torch.equal(layer(x), now) and not torch.equal(now, want)
+            del junk
