@@ -6,7 +6,8 @@ a view of it, by a replayed graph, or by code outside of torch; `weights_changed
 
 In a capture nothing runs, so what is made there is not kept: it has no contents before a replay.
 What was made before and is used in a capture lives as long as its module, since the replays
-read it, also when later calls have made another.
+read it, also when later calls have made another.  A training step's replays make everything
+anew, as weights move between them.
 """
 from __future__ import annotations
 
@@ -61,17 +62,18 @@ class _Held(list):
         return _Held()
 
 
-def derived(owner: dict, name: str, tensors, make, flags=()):
+def derived(owner: dict, name: str, tensors, make, flags=(), training=False):
     """What make() made from the tensors (and the flags), kept in owner[name] (a module's __dict__)
-    until one of them changes."""
+    until one of them changes.  training: of a pass whose weights move, see above."""
     entry = owner.get(name)
     if entry is not None and isinstance(entry[0], Sources) and entry[0].same(tensors, flags):
         if not capturing(tensors[0]):
             return entry[1]
-        held = owner.setdefault("_held", _Held())
-        if not any(v is entry[1] for v in held):
-            held.append(entry[1])
-        return entry[1]
+        if not training:
+            held = owner.setdefault("_held", _Held())
+            if not any(v is entry[1] for v in held):
+                held.append(entry[1])
+            return entry[1]
     with torch.no_grad():
         value = make()
     if not capturing(tensors[0]):

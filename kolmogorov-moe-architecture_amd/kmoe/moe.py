@@ -81,17 +81,19 @@ class _RouterMLP(nn.Module):
     def _bwd_weights(self):
         """Backward packed w_in (rebuilt only when it changed)."""
         w_in = self.router[0].weight
-        return derived(self.__dict__, "_bwd_cache", (w_in,), lambda: _bwd.pack_bwd_weights(None, None, None, w_in))
+        return derived(self.__dict__, "_bwd_cache", (w_in,), lambda: _bwd.pack_bwd_weights(None, None, None, w_in),
+                       training=True)
 
     def _trainable(self, x) -> bool:
         return torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters()))
 
-    def _kernel_weights(self):
+    def _kernel_weights(self, training=False):
+        """The two weights in bf16; training: for a pass that records a backward."""
         w_in, w_out = self.router[0].weight, self.router[2].weight
         if w_in.dtype == torch.bfloat16:
             return w_in.detach(), w_out.detach()
         return derived(self.__dict__, "_bf16_cache", (w_in, w_out),
-                       lambda: tuple(w.detach().to(torch.bfloat16).contiguous() for w in (w_in, w_out)))
+                       lambda: tuple(w.detach().to(torch.bfloat16).contiguous() for w in (w_in, w_out)), training=training)
 
 
 def _route_spec(config) -> Optional[ops.RouteSpec]:
@@ -157,7 +159,7 @@ class Router(_RouterMLP):
         """Kernel-level routing of flattened tokens: fp32 logits, int64 idx, f32 weights.
         With moe_balanced_routing the picks are the capacity-balanced assignment
         (moe.py:443-451) over all the tokens of the call."""
-        w_in, w_out = self._kernel_weights()
+        w_in, w_out = self._kernel_weights(training=save_hidden)
         bias = self.device_bias(x2d)
         if self.balanced_routing:
             r = ops.router(x2d, w_in, w_out, 0, bias=bias, row_index=row_index, T=T, save_hidden=save_hidden)
@@ -198,7 +200,7 @@ class ExpertChoiceRouter(_RouterMLP):
     def route(self, hidden_states: torch.Tensor, descending: bool = True, save_hidden: bool = False):
         B, S, d = hidden_states.shape
         C = min(self.capacity(S), S)
-        w_in, w_out = self._kernel_weights()
+        w_in, w_out = self._kernel_weights(training=save_hidden)
         r = ops.router(hidden_states.reshape(B * S, d), w_in, w_out, 0, save_hidden=save_hidden)
         sel = ops.ec_select(r.logits, B, S, self.n_experts, C, descending=descending)
         return r, sel, C
@@ -274,7 +276,7 @@ class _PackedExperts(nn.Module):
         x w1 is always returned); fp8: from the e4m3 rows xperm with row scales xscale,
         with save h and the input rows dequantised (bf16, the values the fp8 GEMMs
         took: the straight-through backward's operands) and the descaled gate/up values."""
-        pw = self.packed()
+        pw = self.packed(training=save)
         if self.mx is not None:
             # row_token[r] of x2d, quantised once per token; the operands come back dequantised
             xq = ops.quant_rows_mx(x2d, self.mx_act)
@@ -324,7 +326,7 @@ class _PackedExperts(nn.Module):
     def bwd_packed(self) -> _bwd.BwdWeights:
         """Backward packed weights (no router part), rebuilt only when a parameter changed."""
         return derived(self.__dict__, "_bwd_cache", self._weights(),
-                       lambda: _bwd.pack_bwd_weights(*self.bwd_source_weights(), None), (self.use_fp8, self.mx))
+                       lambda: _bwd.pack_bwd_weights(*self.bwd_source_weights(), None), (self.use_fp8, self.mx), training=True)
 
     def _trainable(self, *inputs) -> bool:
         """Whether a direct call records a backward through the HIP kernels."""
@@ -344,9 +346,10 @@ class _PackedExperts(nn.Module):
             return ops.pack_weights_plain(self.w1.detach(), self.w2.detach())
         return ops.pack_weights(self.w1.detach(), self.w2.detach(), self.w3.detach(), fp8=self.use_fp8)
 
-    def packed(self) -> ops.PackedWeights:
-        """Packed weights, rebuilt only when a parameter changed (see `derived`)."""
-        return derived(self.__dict__, "_packed", self._weights(), self._pack, (self.use_fp8, self.mx))
+    def packed(self, training=False) -> ops.PackedWeights:
+        """Packed weights, rebuilt only when a parameter changed (see `derived`); training: for a pass
+        that records a backward."""
+        return derived(self.__dict__, "_packed", self._weights(), self._pack, (self.use_fp8, self.mx), training=training)
 
 
 class GroupedExperts(_PackedExperts):
@@ -822,7 +825,7 @@ class MoELayer(nn.Module):
         ge = self.grouped_experts if self.grouped_experts is not None else self.grouped_experts_ec
         w_in = self.router.router[0].weight
         return derived(self.__dict__, "_bwd_cache", ge._weights() + (w_in,),
-                       lambda: _bwd.pack_bwd_weights(*ge.bwd_source_weights(), w_in), (ge.use_fp8, ge.mx))
+                       lambda: _bwd.pack_bwd_weights(*ge.bwd_source_weights(), w_in), (ge.use_fp8, ge.mx), training=True)
 
     def _train_forward(self, x2d, T, out_dtype, out_map=None, scale=None, residual=None, T_out=None,
                        keep_mask=None, keep_scale=1.0):

@@ -129,7 +129,8 @@ def test_freed_weights_are_not_held():
 
 
 def test_captures(packs, monkeypatch):
-    """What is made in a capture is not kept; what a capture uses outlives its replacement.  (A capture is a stand-in here.)"""
+    """What is made in a capture is not kept; what a capture uses outlives its replacement; a training
+    pass in a capture makes it anew.  (A capture is a stand-in here.)"""
     from kmoe import backward, derived
     state = dict(capturing=False)
     for m in (derived, backward):
@@ -143,6 +144,8 @@ def test_captures(packs, monkeypatch):
     assert ex._packed[1] is kept and len(packs) == 2
     state["capturing"] = True
     assert ex.packed() is kept and ex.packed() is kept and len(packs) == 2
+    ex.packed(training=True), ex.bwd_packed()
+    assert len(packs) == 4 and ex._packed[1] is kept
     state["capturing"] = False
     with torch.no_grad():
         ex.w1.add_(1.0)

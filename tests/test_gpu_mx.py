@@ -865,3 +865,35 @@ def test_a_captured_forward_keeps_its_weights(dev, mx):
             torch.cuda.synchronize()
             assert torch.equal(y, want) and torch.equal(layer(x), now) and not torch.equal(now, want)
             del junk
+
+
+@pytest.mark.parametrize("mx", [None, "w4a8"])
+def test_a_captured_training_step_follows_its_weights(dev, mx):
+    """Forward and gradients captured after an eager pass has packed the weights, which then move between the
+    replays: each replay is the eager pass at the weights of its time."""
+    cfg = kmoe.AdvancedMoEConfig(d_model=128, n_experts=4, moe_top_k=2, d_ff_expert=64, moe_mx=mx)
+    layer, other = kmoe.MoELayer(cfg).to(dev), kmoe.MoELayer(cfg).to(dev)
+    x, dy = rnd(dev, 1, 30, 128, dtype=torch.float32), rnd(dev, 1, 30, 128, seed=1, dtype=torch.float32)
+
+    def step(m):
+        xg = x.detach().requires_grad_(True)
+        y = m(xg)
+        return [y.detach()] + list(torch.autograd.grad(y, [xg] + list(m.parameters()), dy))
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(layer)
+    torch.cuda.current_stream().wait_stream(side)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step(layer)
+    for i in range(4):
+        if i:
+            with torch.no_grad():
+                for p in layer.parameters():
+                    p.add_(rnd(dev, *p.shape, seed=i, std=0.02, dtype=p.dtype))
+        g.replay()
+        torch.cuda.synchronize()
+        other.load_state_dict(layer.state_dict())
+        for u, v in zip(out, step(other)):
+            assert torch.equal(u, v)
