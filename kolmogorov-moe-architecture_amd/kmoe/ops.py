@@ -24,6 +24,15 @@ def _need_gpu(*ts):
             raise ValueError("kmoe: tensors must be on a GPU (the HIP kernels are the only implementation)")
 
 
+def _one_gpu(who, first, *ts):
+    """All on one GPU, the first one's."""
+    _need_gpu(first)
+    dev = first.device
+    for t in ts:
+        if t is not None and t.device != dev:
+            raise ValueError(f"kmoe.{who}: tensors must be on one GPU, got {dev} and {t.device}")
+
+
 def _contig(t, dtype=None):
     if t is None:
         return None
@@ -789,7 +798,7 @@ def route_topk_bwd(logits, idx, dw, scores="softmax", renorm=True, scale=1.0, dl
     sc = _scores(scores)
     logits = _route_logits(logits, "route_topk_bwd")
     T, E = logits.shape
-    _need_gpu(idx, dw)
+    _one_gpu("route_topk_bwd", logits, idx, dw, dlogits)
     k = idx.shape[-1]
     if idx.shape != (T, k) or dw.shape != (T, k):
         raise ValueError(f"kmoe.route_topk_bwd: idx and dw must be ({T}, k), got {tuple(idx.shape)}, {tuple(dw.shape)}")
@@ -856,7 +865,9 @@ def quant_rows_mx(m, fmt="e4m3", row_index=None, n_rows_dev=None) -> MXRows:
     """Microscaled codes of the bf16 rows of m (n, K), K a multiple of 32, or of its rows
     row_index (int32; -1: zeros).  Rows past *n_rows_dev (int32, on the GPU) are left unwritten."""
     code = _mx_fmt(fmt)
-    _need_gpu(m, row_index, n_rows_dev)
+    if n_rows_dev is not None:
+        _table(n_rows_dev, 1, "quant_rows_mx", "n_rows_dev")
+    _one_gpu("quant_rows_mx", m, row_index, n_rows_dev)
     if m.dim() != 2:
         raise ValueError(f"kmoe.quant_rows_mx: a matrix is needed, got {tuple(m.shape)}")
     m = _contig(m, _BF16)
@@ -873,7 +884,9 @@ def quant_rows_mx(m, fmt="e4m3", row_index=None, n_rows_dev=None) -> MXRows:
 def dequant_rows_mx(r: MXRows, row_index=None, n_rows_dev=None):
     """The values (n, K) bf16 of coded rows, or of rows row_index (int32; -1: zeros)."""
     code = _coded(r, "dequant_rows_mx")
-    _need_gpu(r.q, r.scale, row_index, n_rows_dev)
+    if n_rows_dev is not None:
+        _table(n_rows_dev, 1, "dequant_rows_mx", "n_rows_dev")
+    _one_gpu("dequant_rows_mx", r.q, row_index, n_rows_dev)
     if row_index is not None:
         row_index = _contig(row_index, torch.int32)
     rows = r.q.shape[0] if row_index is None else row_index.numel()
@@ -912,7 +925,7 @@ class PackedWeightsMX(NamedTuple):
 
 def pack_weights_mx(w1, w2, w3) -> PackedWeightsMX:
     """e2m1 blocks along K of the expert weights w1, w2 (E,d,F), w3 (E,F,d), packed."""
-    _need_gpu(w1, w2, w3)
+    _one_gpu("pack_weights_mx", w1, w2, w3)
     E, d, F = w1.shape
     if w2.shape != (E, d, F) or w3.shape != (E, F, d):
         raise ValueError("kmoe.pack_weights_mx: w1/w2 must be (E,d,F) and w3 (E,F,d)")
@@ -936,7 +949,7 @@ def gemm_gate_up_mx(x: MXRows, row_token, offsets, pw: PackedWeightsMX, max_rows
     _table(offsets, pw.E + 1, "gemm_gate_up_mx", "offsets")
     if row_token is not None:
         _table(row_token, max_rows, "gemm_gate_up_mx", "row_token")
-    _need_gpu(x.q, row_token, offsets)
+    _one_gpu("gemm_gate_up_mx", x.q, row_token, offsets, pw.w13)
     if x.K != pw.d:
         raise ValueError(f"kmoe.gemm_gate_up_mx: rows of {x.K} values for weights of d={pw.d}")
     if row_token is None and x.q.shape[0] < max_rows:
@@ -955,7 +968,7 @@ def gemm_down_mx(h: MXRows, offsets, pw: PackedWeightsMX, max_rows):
     """y (max_rows, d) bf16 = h w3 of the coded rows of each expert."""
     code = _coded(h, "gemm_down_mx")
     _table(offsets, pw.E + 1, "gemm_down_mx", "offsets")
-    _need_gpu(h.q, offsets)
+    _one_gpu("gemm_down_mx", h.q, offsets, pw.w3)
     if h.K != pw.F or h.q.shape[0] < max_rows:
         raise ValueError(f"kmoe.gemm_down_mx: rows {tuple(h.q.shape)} of {h.K} values, F={pw.F}, max_rows {max_rows}")
     y = torch.empty(max(max_rows, 1), pw.d, device=h.q.device, dtype=_BF16)
@@ -983,7 +996,8 @@ def mx_experts(x2d, idx, w, pw: PackedWeightsMX, fmt, capacity=0, row_index=None
     (3,) f32 or None).  fmt: element type of the activations; coded: their codes, if the
     caller has them; aux = (partials, w_lb, w_z): as for dispatch."""
     code = _mx_fmt(fmt)
-    _need_gpu(x2d, idx, w, row_index, residual)
+    _one_gpu("mx_experts", x2d, idx, w, row_index, residual, out_map, scale, block_counts, pw.w13,
+             None if coded is None else coded.q)
     x2d = _contig(x2d, _BF16)
     idx = _contig(idx, torch.int64)
     if w.dtype not in (torch.float32, _BF16):
@@ -1027,8 +1041,9 @@ def mx_experts(x2d, idx, w, pw: PackedWeightsMX, fmt, capacity=0, row_index=None
         aux_out = torch.empty(3, device=dev, dtype=torch.float32)
     lib = _lib._LIB or _lib.load()
     with _device(dev):
-        if block_counts is not None and block_counts.numel() != -(-T // lib.kmoe_router_block_tokens(T)) * pw.E:
-            raise ValueError("kmoe.mx_experts: block_counts must be the router's per-block histograms")
+        if block_counts is not None and (block_counts.dtype != torch.int32 or not block_counts.is_contiguous() or
+                                         block_counts.numel() != -(-T // lib.kmoe_router_block_tokens(T)) * pw.E):
+            raise ValueError("kmoe.mx_experts: block_counts must be the router's per-block histograms (int32)")
         wsb = _mx_workspace(T, d, pw.E, k, pw.F, code, coded is not None)
         ws = torch.empty(max(wsb, 4), device=dev, dtype=torch.uint8)
         _lib.call("kmoe_mx_experts", ptr(x2d), ptr(row_index), T, d, code, ptr(xq), ptr(xs), ptr(idx), ptr(w),
@@ -1053,7 +1068,7 @@ def add_rmsnorm(x2d, delta, weight, eps, quant=None) -> AddNormOut:
     microscaled rows (those of quant_rows_mx(n)).  x2d, delta (T, d) bf16 or f32; an f32
     delta makes h f32.  Not differentiable: kmoe.add_rms_norm is."""
     code = _lib.DTYPE_BF16 if quant is None else _mx_fmt(quant)
-    _need_gpu(x2d, delta, weight)
+    _one_gpu("add_rmsnorm", x2d, delta, weight)
     T, d = x2d.shape
     if weight.shape != (d,) or (delta is not None and delta.shape != (T, d)):
         raise ValueError(f"kmoe.add_rmsnorm: x {(T, d)}, delta {None if delta is None else tuple(delta.shape)}, weight "
@@ -1085,12 +1100,14 @@ def add_rmsnorm_bwd(dn, h, weight, rrms, dh=None, bf16=False, dw_dtype=None):
     """Backward of add_rmsnorm from dn and dh (None: zero), the gradients of n and h (T, d):
     (dx in h's type, dx rounded to bf16 or None, dweight).  dx is the gradient of x and of
     delta; bf16 asks for the rounding of an f32 one, for the input that is bf16."""
-    _need_gpu(dn, h, weight, rrms, dh)
     T, d = h.shape
-    if dn.shape != (T, d) or (dh is not None and dh.shape != (T, d)):
+    if dn.shape != (T, d) or (dh is not None and dh.shape != (T, d)) or weight.shape != (d,) or rrms.shape != (T,):
         raise ValueError(f"kmoe.add_rmsnorm_bwd: h {(T, d)}, dn {tuple(dn.shape)}, dh "
-                         f"{None if dh is None else tuple(dh.shape)}")
-    dn, h = _contig(dn, _BF16), h.contiguous()
+                         f"{None if dh is None else tuple(dh.shape)}, weight {tuple(weight.shape)}, rrms {tuple(rrms.shape)}")
+    if rrms.dtype != torch.float32:
+        raise ValueError(f"kmoe.add_rmsnorm_bwd: rrms must be the forward's f32, got {rrms.dtype}")
+    _one_gpu("add_rmsnorm_bwd", h, dn, weight, rrms, dh)
+    dn, h, rrms = _contig(dn, _BF16), h.contiguous(), rrms.contiguous()
     weight = weight.detach()
     dw_dtype = weight.dtype if dw_dtype is None else dw_dtype
     weight = _contig(weight, weight.dtype if weight.dtype in (torch.float32, _BF16) else torch.float32)

@@ -897,3 +897,27 @@ def test_a_captured_training_step_follows_its_weights(dev, mx):
         other.load_state_dict(layer.state_dict())
         for u, v in zip(out, step(other)):
             assert torch.equal(u, v)
+
+
+def test_misplaced_arguments_are_refused(dev):
+    """Tables and outputs in host memory, histograms of another type: refused before a launch."""
+    E, d, F, T, k = 4, 64, 64, 3000, 2
+    pw = ops.pack_weights_mx(*weights(dev, E, d, F))
+    x, w = rnd(dev, T, d), torch.ones(T, k, device=dev)
+    lg = rnd(dev, T, E, dtype=torch.float32)
+    r = ops.route_topk(lg, k, hist=True)
+    ops.mx_experts(x, r.idx, w, pw, "e4m3", block_counts=r.block_counts)
+    bad = [dict(block_counts=r.block_counts.long()), dict(block_counts=r.block_counts.float()),
+           dict(block_counts=r.block_counts.cpu()), dict(block_counts=r.block_counts.t()),
+           dict(out_map=torch.arange(T, dtype=torch.int32), T_out=T), dict(scale=torch.ones(T)), dict(residual=x.cpu())]
+    for kw in bad:
+        with pytest.raises(ValueError):
+            ops.mx_experts(x, r.idx, w, pw, "e4m3", **kw)
+    cpu = pw._replace(w13=pw.w13.cpu(), w3=pw.w3.cpu())
+    off = torch.zeros(E + 1, device=dev, dtype=torch.int32)
+    rows = ops.quant_rows_mx(x)
+    for call in (lambda: ops.mx_experts(x, r.idx, w, cpu, "e4m3"), lambda: ops.gemm_gate_up_mx(rows, None, off, cpu, T),
+                 lambda: ops.gemm_down_mx(rows, off, cpu, T),
+                 lambda: ops.route_topk_bwd(lg, r.idx, w, dlogits=torch.zeros(T, E))):
+        with pytest.raises(ValueError, match="one GPU"):
+            call()

@@ -251,3 +251,36 @@ def test_route_restatement_against_torch():
     best = s.amax(-1).argmax(-1)
     v, i = s[torch.arange(50), best].topk(2)
     assert torch.equal(idx, best[:, None] * 3 + i) and torch.allclose(w, 2 * v, rtol=1e-12)
+
+
+def test_shapes_types_and_places_of_arguments():
+    """What the kernels would read past or misread is refused before anything else, on any device."""
+    h, w = torch.zeros(4, 64, dtype=torch.bfloat16), torch.ones(64)
+    r = torch.ones(4)
+    for kw in (dict(weight=torch.ones(32)), dict(rrms=torch.ones(3)), dict(rrms=torch.ones(4, 1)), dict(rrms=r.double()),
+               dict(dn=h[:2]), dict(dh=h[:, :32])):
+        a = {**dict(dn=h, h=h, weight=w, rrms=r), **kw}
+        with pytest.raises(ValueError, match="add_rmsnorm_bwd"):
+            ops.add_rmsnorm_bwd(**a)
+    rows = ops.MXRows(torch.zeros(4, 128, dtype=torch.uint8), torch.zeros(4, 16, dtype=torch.uint8), 64, "e4m3")
+    for n in (torch.zeros(1, dtype=torch.int64), torch.zeros(0, dtype=torch.int32)):
+        with pytest.raises(ValueError, match="n_rows_dev"):
+            ops.quant_rows_mx(h, n_rows_dev=n)
+        with pytest.raises(ValueError, match="n_rows_dev"):
+            ops.dequant_rows_mx(rows, n_rows_dev=n)
+
+
+class _On:
+    """A tensor's stand-in on a device of that name."""
+
+    def __init__(self, name):
+        self.device, self.is_cuda = torch.device(name), name != "cpu"
+
+
+def test_tensors_of_one_call_are_on_one_gpu():
+    ops._one_gpu("f", _On("cuda:0"), None, _On("cuda:0"))
+    for other in ("cpu", "cuda:1"):
+        with pytest.raises(ValueError, match="one GPU"):
+            ops._one_gpu("f", _On("cuda:0"), None, _On(other))
+    with pytest.raises(ValueError, match="GPU"):
+        ops._one_gpu("f", _On("cpu"), _On("cuda:0"))
