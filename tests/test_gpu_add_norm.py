@@ -189,3 +189,29 @@ def test_refusals(dev):
         ops.add_rmsnorm(y, y, torch.ones(40, device=dev), EPS, quant="e4m3")
     with pytest.raises(kmoe.KmoeError):
         ops.add_rmsnorm(y, y, torch.ones(40, device=dev), -1.0)
+
+
+@pytest.mark.parametrize("xd,dd", [(BF, BF), (F32, BF), (F32, F32), (BF, F32)])
+@pytest.mark.parametrize("T,d", [(3, 2112), (300, 4160), (33, 6144), (301, 8192)])
+def test_backward_of_wide_rows(dev, xd, dd, T, d):
+    """Rows of more than 2048 values, in each pair of types, with a bf16 gradient next to an f32
+    one: against the formula in 64 bits."""
+    x, delta = rnd(dev, T, d, seed=1, dtype=xd).requires_grad_(True), rnd(dev, T, d, seed=2, dtype=dd).requires_grad_(True)
+    w = (1 + 0.1 * rnd(dev, d, seed=3, dtype=F32)).requires_grad_(True)
+    h, n = kmoe.add_rms_norm(x, delta, w, EPS)
+    dh, dn = rnd(dev, T, d, seed=4, dtype=h.dtype), rnd(dev, T, d, seed=5)
+    dx, dd_, dg = torch.autograd.grad((h, n), (x, delta, w), (dh, dn))
+    h64, w64, dn64 = h.detach().double(), w.detach().double(), dn.double()
+    r = (h64.square().mean(1, keepdim=True) + EPS).rsqrt()
+    dot = w64 * dn64 * h64
+    want = dh.double() + r * w64 * dn64 - r ** 3 * h64 * dot.mean(1, keepdim=True)
+    terms = dh.double().abs() + r * (w64 * dn64).abs() + r ** 3 * h64.abs() * dot.abs().mean(1, keepdim=True)
+    # f32: a lane's sum of d / 64 terms and six additions over the wave, in r and in the dot product; a
+    # dozen operations; the stream's and the input's rounding
+    steps = (2 * (d // 64 + 6) + 12) * 2.0 ** -24
+    for got, dt in ((dx, xd), (dd_, dd)):
+        rounding = (torch.finfo(h.dtype).eps / 2 + torch.finfo(dt).eps / 2) * (1 + steps)
+        assert got.dtype == dt
+        assert bool(((got.double() - want).abs() <= rounding * want.abs() + (1 + rounding) * steps * terms).all())
+    gt = dn64 * h64 * r
+    assert bool(((dg.double() - gt.sum(0)).abs() <= (T + d // 64 + 16) * 2.0 ** -24 * gt.abs().sum(0)).all())

@@ -314,3 +314,118 @@ def test_gradients_that_nearly_vanish(dev, scores, renorm, k, same, std):
     assert float((l.amax(1, keepdim=True) - l).max()) < far
     steps = 3 * (far + E + 4) + E + k + 10
     assert bool(((got - scale * want).abs() <= steps * HALF_F32 * scale * terms.abs() + 1e-37).all())
+
+
+ROUTED = [
+    dict(moe_router_scores="sigmoid", moe_router_groups=4, moe_router_topk_groups=2, moe_router_scale=2.5, moe_balance_bias=True),
+    dict(moe_router_scores="softmax", moe_router_renorm=False, moe_router_scale=1.5),
+    dict(moe_router_scores="sigmoid", moe_router_renorm=False, moe_balance_bias=True),
+]
+
+
+def layer64(x, w_in, w_out, w1, w2, w3, idx, cfg, mx):
+    """(y, aux) of the layer in 64 bits at the choice idx, differentiable."""
+    T, k = idx.shape
+    E = w1.shape[0]
+    lg = torch.nn.functional.silu(x @ w_in.t()) @ w_out.t()
+    w = M.route_weights(lg, idx, cfg.moe_router_scores, cfg.moe_router_renorm, cfg.moe_router_scale)
+    if mx:
+        y = M.experts(x, idx, w, w1, w2, w3, mx)
+    else:
+        y = torch.zeros(T, x.shape[1], dtype=torch.float64)
+        for e in range(E):
+            t, j = (idx == e).nonzero(as_tuple=True)
+            y = y.index_add(0, t, (torch.nn.functional.silu(x[t] @ w1[e]) * (x[t] @ w2[e])) @ w3[e] * w[t, j][:, None])
+    f = torch.bincount(idx.reshape(-1), minlength=E).double() / (T * k)
+    aux = (cfg.moe_load_balance_loss_weight * E * (f * torch.softmax(lg, -1).mean(0)).sum()
+           + cfg.moe_router_z_loss_weight * torch.logsumexp(lg, -1).square().mean())
+    return y, aux
+
+
+# Gradients through the experts have the bf16 roundings of their backward: w dy, the two
+# pre-activations, dh, dgate / dup, a row's dx, the sum (seven); through the router those of the expert rows (the
+# weights' gradient is their product with dy), of the hidden gradient and the result (three); 4-bit
+# experts: elements of h on the other side of a border, 2e-3 of the norm.
+ROUTED_TOL = 10 * torch.finfo(torch.bfloat16).eps / 2
+
+
+@pytest.mark.parametrize("case", ROUTED)
+@pytest.mark.parametrize("mx", [None, "w4a8"])
+@pytest.mark.parametrize("with_y,with_aux", [(1.0, 0.0), (0.0, 1.0), (1.0, 1.0)])
+def test_layer_gradients_against_64_bits(dev, case, mx, with_y, with_aux):
+    """Every gradient of a layer with its own routing, of its output, of its aux losses, and of both (scaled
+    so that both count), at the kernel's choice of experts."""
+    torch.manual_seed(3)
+    cfg = kmoe.AdvancedMoEConfig(d_model=128, n_experts=16, moe_top_k=4, d_ff_expert=64, moe_mx=mx, **case)
+    layer = kmoe.MoELayer(cfg).to(dev).to(torch.bfloat16).train()
+    with torch.no_grad():
+        layer.router.router[2].weight.mul_(4.0)  # logits that differ
+        if layer.router.balance_bias is not None:
+            layer.router.balance_bias.copy_(bias_of("cpu", 16))
+    x = torch.randn(1, 150, 128, device=dev, dtype=torch.bfloat16)
+    dy = torch.randn_like(x)
+    with torch.no_grad():
+        idx = layer.router.route(x[0]).idx.cpu()
+    ge = layer.grouped_experts
+    xg = x.clone().requires_grad_(True)
+    leaves = [xg, layer.router.router[0].weight, layer.router.router[2].weight, ge.w1, ge.w2, ge.w3]
+    l64 = [v.detach().double().cpu().requires_grad_(True) for v in leaves]
+    y64, aux64 = layer64(l64[0][0], *l64[1:], idx, cfg, mx)
+    dy64 = dy.double().cpu()[0]
+    # the aux losses' share of the router's gradient is made as large as the output's
+    ga, = torch.autograd.grad(aux64, l64[2], retain_graph=True)
+    gy, = torch.autograd.grad((y64 * dy64).sum(), l64[2], retain_graph=True)
+    c = with_aux * float(gy.norm() / ga.norm())
+    want = torch.autograd.grad(with_y * (y64 * dy64).sum() + c * aux64, l64, allow_unused=True)
+    y = layer(xg)
+    assert abs(float(layer.aux_loss.detach()) - float(aux64)) <= 1e-4 * float(aux64)
+    assert float((y.detach().double().cpu()[0] - y64).norm() / y64.norm()) <= 4 * torch.finfo(torch.bfloat16).eps / 2
+    got = torch.autograd.grad((y.float() * dy.float()).sum() * with_y + c * layer.aux_loss, leaves)
+    for name, a, b in zip(("dx", "dw_in", "dw_out", "dw1", "dw2", "dw3"), got, want):
+        if not with_y and name[:3] in ("dw1", "dw2", "dw3"):
+            assert not a.any()
+            continue
+        err = float((a.double().cpu() - b).norm() / b.norm())
+        assert err <= ROUTED_TOL + (2e-3 if mx else 0.0), (name, err)
+
+
+@pytest.mark.parametrize("case", ROUTED)
+def test_block_gradients_against_64_bits(dev, case):
+    """The block of an f32 stream and a delta not yet added: h and delta get the same gradient, that of the
+    formula, next to the norm's, the router's and the experts'."""
+    torch.manual_seed(4)
+    cfg = kmoe.AdvancedMoEConfig(d_model=128, n_experts=16, moe_top_k=4, d_ff_expert=64, mod_enabled=False,
+                                 residual_dropout=0.0, **case)
+    blk = kmoe.MoEFFNBlock(cfg).to(dev).train()
+    r = blk.ffn.router
+    with torch.no_grad():
+        r.router[2].weight.mul_(4.0)
+        blk.ffn_norm.weight.add_(0.1 * torch.randn_like(blk.ffn_norm.weight))
+        if r.balance_bias is not None:
+            r.balance_bias.copy_(bias_of("cpu", 16))
+        for p in blk.parameters():  # values that bf16 holds: the kernels cast them
+            p.copy_(p.to(torch.bfloat16))
+    h, delta, dout = (torch.randn(1, 150, 128, device=dev) for _ in range(3))
+    with torch.no_grad():
+        idx = r.route(ops.rmsnorm((h + delta)[0], blk.ffn_norm.weight, cfg.norm_eps).n).idx.cpu()
+    ge = blk.ffn.grouped_experts
+    hg, dg = h.clone().requires_grad_(True), delta.clone().requires_grad_(True)
+    leaves = [hg, blk.ffn_norm.weight, r.router[0].weight, r.router[2].weight, ge.w1, ge.w2, ge.w3]
+    l64 = [v.detach().double().cpu().requires_grad_(True) for v in leaves]
+    s64 = l64[0][0] + delta.double().cpu()[0]
+    n64 = M.add_norm(s64, None, l64[1], cfg.norm_eps)[1]
+    y64, aux64 = layer64(n64, *l64[2:], idx, cfg, None)
+    d64 = dout.double().cpu()[0]
+    ga, = torch.autograd.grad(aux64, l64[3], retain_graph=True)
+    gy, = torch.autograd.grad((y64 * d64).sum(), l64[3], retain_graph=True)
+    c = float(gy.norm() / ga.norm())
+    want = list(torch.autograd.grad((y64 * d64).sum() + c * aux64, l64))  # without the residual's dout
+    out = blk(hg, dg)
+    assert blk.last_path == "fused_train"
+    g = torch.autograd.grad((out * dout).sum() + c * blk.aux_loss, leaves + [dg])
+    assert torch.equal(g[0], g[-1])
+    got = [(g[0] - dout).double().cpu()] + [v.double().cpu() for v in g[1:-1]]
+    for name, a, b in zip(("dh", "dg", "dw_in", "dw_out", "dw1", "dw2", "dw3"), got, want):
+        # (and the normalised rows are rounded to bf16 first, their gradient too: two more)
+        err = float((a - b).norm() / b.norm())
+        assert err <= ROUTED_TOL * 1.2, (name, err)
