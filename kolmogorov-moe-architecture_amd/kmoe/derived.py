@@ -15,26 +15,27 @@ import torch
 from torch.multiprocessing.reductions import StorageWeakRef
 
 
+def _state(tensors, flags):
+    s = [flags]  # (one list and one comparison: this runs in every call)
+    for t in tensors:
+        s += (t._version, t.data_ptr(), t.untyped_storage()._cdata)
+    return s
+
+
 class Sources:
     """The tensors that a value was made from: their addresses, version counters and storages.  An
     address and a counter alone say nothing, as the allocator gives a freed weight's place to
     the next one and counters start at zero; the weak references hold on to no memory, but to the
     storages' identities.  Equal to nothing once copied or pickled with its module, whose
     copy has other weights."""
-    __slots__ = ("_flags", "_at", "_refs")
+    __slots__ = ("_at", "_refs")
 
     def __init__(self, tensors, flags=()):
-        self._flags = flags
+        self._at = _state(tensors, flags)
         self._refs = tuple(StorageWeakRef(t.untyped_storage()) for t in tensors)
-        self._at = tuple((t.data_ptr(), t._version, r.cdata) for t, r in zip(tensors, self._refs))
 
     def same(self, tensors, flags=()) -> bool:
-        if flags != self._flags or len(tensors) != len(self._at):
-            return False
-        for t, (ptr, version, storage) in zip(tensors, self._at):
-            if t._version != version or t.data_ptr() != ptr or t.untyped_storage()._cdata != storage:
-                return False
-        return True
+        return _state(tensors, flags) == self._at
 
     def __reduce__(self):
         return _gone, ()
@@ -48,8 +49,10 @@ def _gone() -> Sources:
 
 
 def capturing(t) -> bool:
-    """Whether work on t's device is being captured into a graph."""
-    return t.is_cuda and torch.cuda.is_current_stream_capturing()
+    """Whether work on t's device is being captured into a graph (the default stream, 0, never is, and costs
+    less to tell)."""
+    i = t.get_device()
+    return i >= 0 and torch._C._cuda_getCurrentRawStream(i) != 0 and torch.cuda.is_current_stream_capturing()
 
 
 class _Held(list):

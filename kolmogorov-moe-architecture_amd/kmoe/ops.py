@@ -27,10 +27,10 @@ def _need_gpu(*ts):
 def _one_gpu(who, first, *ts):
     """All on one GPU, the first one's."""
     _need_gpu(first)
-    dev = first.device
+    dev = first.get_device()  # (an index: cheaper than a device, once a tensor and call)
     for t in ts:
-        if t is not None and t.device != dev:
-            raise ValueError(f"kmoe.{who}: tensors must be on one GPU, got {dev} and {t.device}")
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"kmoe.{who}: tensors must be on one GPU, got {first.device} and {t.device}")
 
 
 def _contig(t, dtype=None):

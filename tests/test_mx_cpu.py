@@ -276,6 +276,9 @@ class _On:
     def __init__(self, name):
         self.device, self.is_cuda = torch.device(name), name != "cpu"
 
+    def get_device(self):
+        return self.device.index if self.is_cuda else -1
+
 
 def test_tensors_of_one_call_are_on_one_gpu():
     ops._one_gpu("f", _On("cuda:0"), None, _On("cuda:0"))
