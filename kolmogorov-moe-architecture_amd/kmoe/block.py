@@ -99,6 +99,10 @@ def add_rms_norm(x: torch.Tensor, delta: torch.Tensor, weight: torch.Tensor, eps
     and weight (bf16 or f32; the residual stream h has x's type, or f32 with an f32 delta)."""
     if x.shape != delta.shape:
         raise ValueError(f"kmoe.add_rms_norm: x {tuple(x.shape)}, delta {tuple(delta.shape)}")
+    if not torch.is_grad_enabled():  # no graph: nothing that a capture could meet
+        d = x.shape[-1]
+        r = ops.add_rmsnorm(x.reshape(-1, d), delta.reshape(-1, d), weight, eps)
+        return r.h.view(x.shape), r.n.view(x.shape)
     return _AddNormFn.apply(x, delta, weight, eps)
 
 

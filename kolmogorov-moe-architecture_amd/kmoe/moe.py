@@ -485,7 +485,11 @@ class _RouteFn(torch.autograd.Function):
 def route_topk(logits, k, scores="softmax", bias=None, groups=1, topk_groups=1, group_top=2, renorm=True, scale=1.0):
     """(w (T, k) f32, idx (T, k) int64) of ops.route_topk, differentiable in the logits (the
     choice is piecewise constant: the bias gets no gradient)."""
-    return _RouteFn.apply(logits, k, bias, ops.RouteSpec(scores, groups, topk_groups, group_top, renorm, scale))
+    spec = ops.RouteSpec(scores, groups, topk_groups, group_top, renorm, scale)
+    if not torch.is_grad_enabled():  # no graph: nothing that a capture could meet
+        r = ops.route_topk(logits, k, bias=bias, **spec._asdict())
+        return r.w, r.idx
+    return _RouteFn.apply(logits, k, bias, spec)
 
 
 class _MoETrainFn(torch.autograd.Function):

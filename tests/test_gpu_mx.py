@@ -921,3 +921,26 @@ def test_misplaced_arguments_are_refused(dev):
                  lambda: ops.route_topk_bwd(lg, r.idx, w, dlogits=torch.zeros(T, E))):
         with pytest.raises(ValueError, match="one GPU"):
             call()
+
+
+def test_captured_forward_beside_an_eager_graph(dev):
+    """Without gradients a capture takes the same leaves while an eager graph of them lives, and that
+    graph's backward is as it was."""
+    x = rnd(dev, 8, 64)
+    gain = torch.ones(64, device=dev, dtype=BF).requires_grad_(True)
+    logits = rnd(dev, 8, 4, dtype=torch.float32).requires_grad_(True)
+    for call, leaf in ((lambda: kmoe.add_rms_norm(x, x, gain), gain), (lambda: kmoe.route_topk(logits, 2), logits)):
+        alive, again = call(), call()
+        i = 0 if alive[0].requires_grad and alive[0].dtype == torch.float32 else 1
+        g = torch.cuda.CUDAGraph()
+        with torch.no_grad(), torch.cuda.graph(g):
+            out = call()
+        assert not any(o.requires_grad for o in out)
+        for _ in range(3):
+            for o in out:
+                o.zero_()
+            g.replay()
+            torch.cuda.synchronize()
+            assert all(torch.equal(u, v) for u, v in zip(out, alive))
+        a, b = (torch.autograd.grad(v[i].float().square().sum(), leaf)[0] for v in (alive, again))
+        assert torch.equal(a, b) and bool(a.any())
