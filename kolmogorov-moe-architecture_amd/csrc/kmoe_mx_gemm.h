@@ -56,7 +56,7 @@ struct MxGemmArgs {
   int n_ct;                // small-row kernel: column tiles of an expert
   uint8_t* q;              // gate_up: h's codes, scales, and (training) gate / up values
   uint8_t* q_scale;
-  uint16_t* gu;
+  uint16_t* gu;            // (rounded to bf16, as the other experts' backward reads them: half of f32's bytes)
   uint16_t* c;             // down: output
   int64_t ldc;             // gate_up: padded columns of h; down: columns of c
   int n_valid;             // down: columns to store

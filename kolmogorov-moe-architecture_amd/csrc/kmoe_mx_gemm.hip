@@ -19,7 +19,8 @@ namespace {
 // (12) 115 / 97 / 99; e2m1: down, 500 (0.8) 17.4 / 15.3 / 17.5; 777 (1) 21.5 / 22 / 18; 2042 33 /
 // 31 / 32; gate/up, 777 (2.8) 34 / 32 / 27; 2042 55 / 51 / 45.  Top-6 of 64, d 1024, F 704,
 // gate/up: e4m3, 400 (1.6) 17.6 / 15.3 / 19.6; 2000 (5.1) 34 / 31 / 31; e2m1, 400 15.5 / 14.7 /
-// 17.1; 1000 (93 rows an expert, 2.9) 19.1 / 19.2 / 18.8.
+// 17.1; 1000 (93 rows an expert, 2.9) 19.1 / 19.2 / 18.8.  The 1.5 is e4m3's: the e2m1 product of
+// 500 tokens (0.8) loses 12 % by it.
 MxTileSize tile_size(bool fp4, int64_t max_rows, int E, int b_tiles) {
   const int64_t used = std::min<int64_t>(max_rows, E), tiles = std::max(used, max_rows / 64 + used / 2) * b_tiles;
   const int64_t cu = kmoe::cu_count();
@@ -32,7 +33,8 @@ MxTileSize tile_size(bool fp4, int64_t max_rows, int E, int b_tiles) {
 // kernel / 64 x 128 tiles, e4m3, weights from HBM (workgroups): top-2 of 16 experts, d 2048, F
 // 2816, down, 1 token (128) 4.9 / 9.8, 4 (512) 8.0 / 10.0, 16 (1088) 14.9 / 13.3; gate/up, 1
 // (176) 6.5 / 9.0, 2 (352) 9.7 / 9.1, 4 (704) 14.1 / 12.6, 48 (1672) 31 / 22; top-2 of 8, d 4096,
-// F 1408, gate/up, 4 (352) 9.5 / 18.3, 48 (484) 18.0 / 20.1, 100 (616) 23.5 / 20.1: each
+// F 1408, gate/up, 4 (352) 9.5 / 18.3, 48 (484) 18.0 / 20.1, 100 (616) 23.5 / 20.1; of the first shape 2 tokens
+// lose 6 % by the limit: each
 // workgroup looks its slot up and reduces, which the tiles do once for four times the weights.
 bool small_product(bool gate_up, int64_t max_rows, int E, int b_tiles) {
   const int64_t slots = max_rows / SMALL_ROWS + std::min<int64_t>(max_rows, E);

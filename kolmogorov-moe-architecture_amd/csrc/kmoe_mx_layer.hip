@@ -128,7 +128,9 @@ __global__ __launch_bounds__(FEW) void tables_kernel(const int64_t* __restrict__
   }
 }
 
-// Buffers of one call in the workspace, 256-byte aligned.
+// Buffers of one call in the workspace, 256-byte aligned.  yperm, the experts' rows of y, is bf16 as the
+// other experts' is: 2 bytes a value written and read (at 16384 tokens, top-2, d 2048 f32 rows
+// would add 256 MiB, about 55 us of 523) for one rounding more, 0.0024 relative to 64 bits in place of 0.0017.
 struct Buffers {
   size_t offsets, row_token, slot_row, slot_w, dispatch, xq, xs, hq, hs, yperm, total;
 };

@@ -157,8 +157,8 @@ __device__ __forceinline__ void unpack_raw(const Raw8<F32>& r, float (&v)[8]) {
 // norm being fused.  Sums as in rmsnorm_kernel, so n is that of a torch addition followed by
 // kmoe_rmsnorm, bit for bit.  One wave per row.  Memory bounds it, at few rows its latency: a
 // row's loads (up to d 2048 the weight's too) go out before the first is waited for.  bf16 with
-// e4m3 rows, d 2048: 16384 rows 56 us, 5.4 TB/s (each
-// vector waited for on its own 65), 48 rows 7.4 (8.7).
+// e4m3 rows, d 2048: 16384 rows 56 us, 5.4 TB/s (each vector waited for on its own 65), 48 rows 7.4
+// (8.7), one wave's walk over a whole row.  Without codes, d 4096 / 8192: bf16 4.4 / 2.8 TB/s, f32 5.7 / 4.2.
 template <int NV, bool XF32, int Q>
 __global__ __launch_bounds__(64 * NORM_FWD_WAVES) void add_rmsnorm_kernel(
     const void* __restrict__ x, const void* __restrict__ delta, bool delta_f32, const void* __restrict__ g, bool g_f32,
@@ -266,7 +266,9 @@ struct NormRow {
 // over the rows [seg * seg_rows, ...) of its segment, wave w taking every NORM_WAVES-th
 // row (its x, dn and dres loads issued together); the waves' dg sums are then added in
 // wave order through LDS and written as partial[seg][:] (reduced over segments afterwards
-// in a fixed order).
+// in a fixed order).  HBM bounds it up to d 2048: bf16 / f32 rows with dres 4.7 / 5.6 TB/s.  Wider rows do
+// not fit a lane's 256 registers: NV 8 spills 73 / 192 of them (d 4096: 2.5 / 2.8 TB/s), NV 16 793 / 919
+// (d 8192: 0.7 / 1.2 TB/s).
 template <int NV, bool XF32>
 __global__ __launch_bounds__(64 * NORM_WAVES) void rmsnorm_bwd_kernel(
     const uint16_t* __restrict__ dn, const void* __restrict__ x, const void* __restrict__ g, bool g_f32,

@@ -11,7 +11,9 @@
 //
 // Two choices may be closer than 32-bit rounding, and the experts picked are those of the
 // definition: a token is ranked in f32, and again in 64 bits where two neighbours of that
-// order (or the last kept and the first dropped group) are closer than the f32 error.
+// order (or the last kept and the first dropped group) are closer than the f32 error.  That error
+// is the largest of the token's choices, so the wider the logits spread the more tokens need 64
+// bits: of softmax scores of 64 experts, top-8, 0.1 % at a standard deviation of 1.5, 7 % at 5, 34 % at 8.
 #include <type_traits>
 
 #include "kmoe_common.h"
@@ -243,7 +245,8 @@ __device__ __forceinline__ int rank64(const RouteArgs& a, RouteLds& s, float l, 
 // 11.9 us (64 lanes a token, four tokens a wave one after the other: 27), 64 tokens 5.5; with
 // choices so far apart that no token needs the 64-bit order 8.6 and 5.5.  That order takes the
 // whole wave for one token (with its 16 lanes, the wave's four tokens together, 12.9; where every
-// token needs it, all logits alike, 29 against 17).
+// token needs it, all logits alike, 29 against 17).  At standard deviations of the logits of
+// 1.5 / 5 / 8 sigmoid 10 / 17 / 27 in a replayed graph, softmax 12 / 19 / 27.
 template <int EPL>
 __global__ __launch_bounds__(1024) void route_kernel(RouteArgs a) {
   __shared__ RouteLds lds[64];
