@@ -159,7 +159,7 @@ def _codes_m(m):
     """(e4m3 codes (n,) uint8, scales f32 per 256) of the first moment."""
     b = _blocks(m)
     scale = b.abs().amax(1) * (1.0 / TOP_M)
-    q = b / torch.where(scale > 0, scale, 1.0)[:, None]
+    q = b * (1.0 / torch.where(scale > 0, scale, 1.0))[:, None]
     return q.clamp(-TOP_M, TOP_M).to(torch.float8_e4m3fn).view(torch.uint8).view(-1)[: m.numel()].contiguous(), scale
 
 
@@ -169,8 +169,8 @@ def _codes_v(v):
     root = torch.sqrt(v)
     b = _blocks(root)
     scale = b.amax(1) * (1.0 / TOP_V)
-    q = (b / torch.where(scale > 0, scale, 1.0)[:, None]).clamp(max=TOP_V)
-    e = (torch.frexp(q).exponent - 1).clamp(min=-14)
+    q = (b * (1.0 / torch.where(scale > 0, scale, 1.0))[:, None]).clamp(max=TOP_V)
+    e = torch.where(q > 0, torch.frexp(q).exponent - 1, -14).clamp(min=-14)
     code = torch.round(torch.ldexp(q, 4 - e)).int() + (e + 14) * 16
     code = torch.where((code == 0) & (b > 0), 1, code)
     return code.to(torch.uint8).view(-1)[: v.numel()].contiguous(), scale
