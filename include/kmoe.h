@@ -636,6 +636,36 @@ int kmoe_mx_experts(const void* x, const int32_t* row_index, int64_t T, int d, i
                     const void* residual, int64_t T_out, void* y, int y_dtype, int32_t* counts, void* workspace,
                     size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------ */
+/* AdamW over many tensors in one launch (of up to 256 tensors).
+ *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g^2,  t = *step + 1
+ *   p = p - lr wd p - lr / (1 - b1^t) m / (sqrt(v / (1 - b2^t)) + eps),  *step = t
+ * table (n_tensors, KMOE_ADAMW_FIELDS) int64, on the device, a tensor in a row: the addresses
+ * of p, m, v, the scales of m and of v (8 bits), the f32 copy of p (has_master) and step (int32),
+ * and the number of values n.  Its workgroups ("chunks") are ceil(n / KMOE_ADAMW_CHUNK):
+ * chunk_base (n_tensors + 1) int32 their running sum, on the device and on the host,
+ * chunk_tensor the tensor of each chunk.  grads (host array): the gradients' device addresses,
+ * of p's type; NULL: the tensor is left as it is, its step too.  tickets (n_tensors) int32:
+ * zeros, and zeros again after the call; calls that overlap need other ones.
+ * dtype: BF16 or F32, of p and its gradient.  has_master (BF16): p is the rounding of its f32
+ * copy, which the step reads and writes.  lr_dev, when set, is the learning rate, on the device.
+ * bits 32: m and v in f32.  bits 8: codes, one byte a value, and one f32 scale per
+ * KMOE_ADAMW_BLOCK values: m in e4m3 (scale = largest |m| / 448), the root of v in unsigned
+ * codes of 4 exponent and 4 mantissa bits, c >= 16 for (16 + c % 16) 2^(c / 16 - 19), else
+ * c 2^-18 (scale = largest / 1.9375); a positive root gets no code 0.  A block with a value that
+ * is not finite gets the scale NaN.  Vectors of 16 bytes are used where p, its gradient and its
+ * copy, and where the states, are aligned for them.                                  */
+#define KMOE_ADAMW_FIELDS 8
+#define KMOE_ADAMW_CHUNK 8192
+#define KMOE_ADAMW_BLOCK 256
+int kmoe_adamw(const int64_t* table, const int32_t* chunk_tensor, const int32_t* chunk_base,
+               const int32_t* chunk_base_host, int n_tensors, const void* const* grads, int dtype, int bits,
+               int has_master, float lr, const float* lr_dev, double beta1, double beta2, float eps, float wd,
+               int32_t* tickets, void* stream);
+/* The values (n) of type `dtype` that 8-bit states of kmoe_adamw stand for: m, and the root of v. */
+int kmoe_adamw_values(const void* m_codes, const float* m_scale, const void* v_codes, const float* v_scale,
+                      int64_t n, int dtype, void* m, void* root, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -6,11 +6,12 @@ from .moe import (ExpertChoiceRouter, GroupedExperts, GroupedExpertsExpertChoice
 from .mod import MoDMoE, MoDRouter
 from .block import MoEFFNBlock, RMSNorm, add_rms_norm
 from .derived import weights_changed
+from .optim import AdamW
 from . import ops, kernels, checkpoint
 
 __all__ = [
     "AdvancedMoEConfig", "get_5b_config", "get_test_config", "MoELayer", "Router", "ExpertChoiceRouter",
     "GroupedExperts", "GroupedExpertsExpertChoice", "MoDRouter", "MoDMoE", "ops", "kernels", "KmoeError",
     "load_library", "MoEFFNBlock", "RMSNorm", "checkpoint", "add_rms_norm", "route_topk",
-    "weights_changed",
+    "weights_changed", "AdamW",
 ]
