@@ -52,9 +52,16 @@ extern "C" {
 #define KMOE_SCORES_SOFTMAX 0
 #define KMOE_SCORES_SIGMOID 1
 
+/* activations of the gated feed-forward block */
+#define KMOE_ACT_SILU 0
+#define KMOE_ACT_GELU 1      /* g Phi(g) */
+#define KMOE_ACT_GELU_TANH 2 /* g (1 + tanh(sqrt(2 / pi) (g + 0.044715 g^3))) / 2 */
+#define KMOE_ACT_RELU 3
+
 /* limits */
 #define KMOE_MAX_EXPERTS 64
 #define KMOE_ROUTER_HIDDEN 128 /* the reference router MLP width, moe.py:346 */
+#define KMOE_MAX_RANK 128 /* of the adapters beside a shared projection */
 
 const char* kmoe_last_error(void);
 int kmoe_abi_version(void);
@@ -665,6 +672,60 @@ int kmoe_adamw(const int64_t* table, const int32_t* chunk_tensor, const int32_t*
 /* The values (n) of type `dtype` that 8-bit states of kmoe_adamw stand for: m, and the root of v. */
 int kmoe_adamw_values(const void* m_codes, const float* m_scale, const void* v_codes, const float* v_scale,
                       int64_t n, int dtype, void* m, void* root, void* stream);
+
+/* ------------------------------------------------------------------------ */
+/* Dense products beside the routed experts, on weights as torch.nn.Linear holds them (rows of
+ * the output, K-contiguous), bf16, f32 sums.  Sizes other than the rows' are multiples of 8, the
+ * rows any number below 2^31, buffers contiguous and aligned to 16 bytes.
+ *
+ * Adapters: row t of a projection x w^T gets scale[i] (x a[i]^T) b[i]^T on top, i = ids[t]
+ * (device int32; outside [0, n_adapters): no adapter); a (n, rank, K), b (n, N, rank) bf16, scale (n)
+ * f32 or NULL for 1; rank a multiple of 8, at most KMOE_MAX_RANK.  The inner products are
+ * rounded to bf16 with their scale.  One row's adapter does not reach another row.       */
+typedef struct {
+  const void* a;
+  const void* b;
+  const float* scale;
+  int rank;
+} kmoe_adapter;
+
+/* y (T, d) = (act(x w_gate^T) * (x w_up^T)) w_down^T with adapters (each nullable; the gate's and
+ * the up projection's of one rank), act a KMOE_ACT_*; w_gate, w_up (F, d), w_down (d, F).
+ * The hidden values are rounded to bf16.                                            */
+size_t kmoe_gated_ffn_workspace_bytes(int64_t T, int F, int rank_gate_up, int rank_down);
+int kmoe_gated_ffn(const void* x, int64_t T, int d, int F, const void* w_gate, const void* w_up, const void* w_down,
+                   int act, const int32_t* ids, int n_adapters, const kmoe_adapter* gate, const kmoe_adapter* up,
+                   const kmoe_adapter* down, void* y, void* workspace, size_t workspace_bytes, void* stream);
+/* y (T, N) = x w^T with an adapter (nullable).                                      */
+size_t kmoe_adapted_linear_workspace_bytes(int64_t T, int rank);
+int kmoe_adapted_linear(const void* x, int64_t T, int K, const void* w, int N, const int32_t* ids, int n_adapters,
+                        const kmoe_adapter* adapter, void* y, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Their parts, for training.  v (T, rank) bf16 = the scaled inner products of x with a (and v2
+ * with a2, of one rank); rows without an adapter are left.                          */
+int kmoe_adapter_inner(const void* x, int64_t T, int K, const int32_t* ids, int n, int rank, const void* a,
+                       const float* scale, void* v, const void* a2, const float* scale2, void* v2, void* stream);
+/* h (T, F) = act(x w_gate^T) * (x w_up^T); with p and q (T, F) also what the backward needs, up
+ * act'(gate) and act(gate), bf16 (then no adapters).  ids NULL: no adapters.        */
+int kmoe_dense_gate_up(const void* x, int64_t T, int d, const void* w_gate, const void* w_up, int F, int act,
+                       const int32_t* ids, int n_adapters, int rank, const void* v_gate, const void* b_gate,
+                       const void* v_up, const void* b_up, void* h, void* p, void* q, void* stream);
+int kmoe_dense_linear(const void* x, int64_t T, int K, const void* w, int N, const int32_t* ids, int n_adapters,
+                      int rank, const void* v, const void* b, void* y, void* stream);
+/* dgate, dup (T, F) = (dy w_down) p, (dy w_down) q.                                 */
+int kmoe_dense_dh(const void* dy, int64_t T, int d, const void* w_down, int F, const void* p, const void* q,
+                  void* dgate, void* dup, void* stream);
+/* dx (T, K) = dy w (+ dy2 w2), w (N, K); with adapters (of one product) + u at[i]^T, u (T, rank) the
+ * scaled inner products of dy with the transposed b, at (n, K, rank) the transposed a. */
+int kmoe_dense_dx(const void* dy, const void* dy2, int64_t T, int N, const void* w, const void* w2, int K,
+                  const int32_t* ids, int n_adapters, int rank, const void* u, const void* at, void* dx, void* stream);
+/* c (M, N) bf16 or f32 = a^T b, a (T, M), b (T, N), any T.                          */
+int kmoe_dense_wgrad(const void* a, const void* b, int64_t T, int M, int N, void* c, int c_dtype, void* stream);
+/* out[i] = sum over the rows t of adapter i of l[t]^T m[t], l (T, rank), m (T, C): (rank, C), or with
+ * outer (C, rank), bf16; zeros for an adapter without rows.                         */
+size_t kmoe_adapter_grad_workspace_bytes(int64_t T, int n, int rank, int C);
+int kmoe_adapter_grad(const void* l, const void* m, int64_t T, const int32_t* ids, int n, int rank, int C, int outer,
+                      void* out, void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

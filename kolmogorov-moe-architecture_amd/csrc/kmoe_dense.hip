@@ -1,0 +1,108 @@
+// Entry points of the dense products (kmoe_dense.h): host checks and the choice of a tile.
+#include <initializer_list>
+
+#include "kmoe_dense_launch.h"
+
+using namespace kmoe_dense;
+
+namespace {
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
+
+}  // namespace
+
+#define KMOE_DENSE_SIZES(who, M, N, K)                                                                                   \
+  KMOE_REQUIRE((M) >= 0 && (N) > 0 && (K) > 0 && (N) % 8 == 0 && (K) % 8 == 0 && (M) < ((int64_t)1 << 31), KMOE_ERR_SHAPE, \
+               who ": %lld rows of %d and %d values (positive multiples of 8)", (long long)(M), (int)(K), (int)(N))
+#define KMOE_DENSE_ALIGNED(who, ...)                                            \
+  for (const void* p_ : std::initializer_list<const void*>{__VA_ARGS__})                                        \
+  KMOE_REQUIRE(aligned(p_), KMOE_ERR_SHAPE, who ": buffers are aligned to 16 bytes")
+#define KMOE_DENSE_ADAPTERS(who, n, r)                                                                          \
+  KMOE_REQUIRE((n) > 0 && (r) > 0 && (r) <= KMOE_MAX_RANK && (r) % 8 == 0, KMOE_ERR_SHAPE,                      \
+               who ": %d adapters of rank %d (a multiple of 8, at most %d)", (int)(n), (int)(r), KMOE_MAX_RANK)
+
+extern "C" int kmoe_dense_gate_up(const void* x, int64_t T, int d, const void* w_gate, const void* w_up, int F, int act,
+                                  const int32_t* ids, int n_adapters, int rank, const void* v_gate, const void* b_gate,
+                                  const void* v_up, const void* b_up, void* h, void* p, void* q, void* stream) {
+  KMOE_DENSE_SIZES("kmoe_dense_gate_up", T, F, d);
+  KMOE_REQUIRE(act >= KMOE_ACT_SILU && act <= KMOE_ACT_RELU, KMOE_ERR_UNSUPPORTED, "kmoe_dense_gate_up: activation %d", act);
+  if (T == 0) return KMOE_OK;
+  KMOE_REQUIRE(x && w_gate && w_up && h && !p == !q, KMOE_ERR_NULL, "kmoe_dense_gate_up: null buffer");
+  KMOE_DENSE_ALIGNED("kmoe_dense_gate_up", x, w_gate, w_up, h, p, q, v_gate, b_gate, v_up, b_up);
+  Args g{};
+  g.a[0] = static_cast<const uint16_t*>(x);
+  g.b[0] = static_cast<const uint16_t*>(w_gate), g.b[1] = static_cast<const uint16_t*>(w_up);
+  g.parts = 1, g.K = d, g.lda = d, g.ldb = d, g.M = T, g.N = F, g.ldc = F, g.c = h, g.act = act;
+  g.p = static_cast<uint16_t*>(p), g.q = static_cast<uint16_t*>(q);
+  if (ids) {
+    KMOE_DENSE_ADAPTERS("kmoe_dense_gate_up", n_adapters, rank);
+    KMOE_REQUIRE(!v_gate == !b_gate && !v_up == !b_up && !p, KMOE_ERR_NULL,
+                 "kmoe_dense_gate_up: adapters come with their inner products, and without values for a backward");
+    g.ad = {ids, {static_cast<const uint16_t*>(v_gate), static_cast<const uint16_t*>(v_up)},
+            {static_cast<const uint16_t*>(b_gate), static_cast<const uint16_t*>(b_up)}, n_adapters, rank};
+  }
+  return ids ? launch_gated_adapt(g, kmoe::as_stream(stream)) : launch_gated(g, kmoe::as_stream(stream));
+}
+
+extern "C" int kmoe_dense_linear(const void* x, int64_t T, int K, const void* w, int N, const int32_t* ids, int n_adapters,
+                                 int rank, const void* v, const void* b, void* y, void* stream) {
+  KMOE_DENSE_SIZES("kmoe_dense_linear", T, N, K);
+  if (T == 0) return KMOE_OK;
+  KMOE_REQUIRE(x && w && y, KMOE_ERR_NULL, "kmoe_dense_linear: null buffer");
+  KMOE_DENSE_ALIGNED("kmoe_dense_linear", x, w, y, v, b);
+  Args g{};
+  g.a[0] = static_cast<const uint16_t*>(x), g.b[0] = static_cast<const uint16_t*>(w);
+  g.parts = 1, g.K = K, g.lda = K, g.ldb = K, g.M = T, g.N = N, g.ldc = N, g.c = y;
+  if (ids) {
+    KMOE_DENSE_ADAPTERS("kmoe_dense_linear", n_adapters, rank);
+    KMOE_REQUIRE(v && b, KMOE_ERR_NULL, "kmoe_dense_linear: null adapter buffer");
+    g.ad = {ids, {static_cast<const uint16_t*>(v), nullptr}, {static_cast<const uint16_t*>(b), nullptr}, n_adapters, rank};
+  }
+  return ids ? launch_linear_adapt(g, kmoe::as_stream(stream)) : launch_linear(g, kmoe::as_stream(stream));
+}
+
+extern "C" int kmoe_dense_dh(const void* dy, int64_t T, int d, const void* w_down, int F, const void* p, const void* q,
+                             void* dgate, void* dup, void* stream) {
+  KMOE_DENSE_SIZES("kmoe_dense_dh", T, F, d);
+  if (T == 0) return KMOE_OK;
+  KMOE_REQUIRE(dy && w_down && p && q && dgate && dup, KMOE_ERR_NULL, "kmoe_dense_dh: null buffer");
+  KMOE_DENSE_ALIGNED("kmoe_dense_dh", dy, w_down, p, q, dgate, dup);
+  Args g{};
+  g.a[0] = static_cast<const uint16_t*>(dy), g.b[0] = static_cast<const uint16_t*>(w_down);
+  g.parts = 1, g.K = d, g.lda = d, g.ldb = F, g.M = T, g.N = F, g.ldc = F, g.c = dgate;
+  g.c2 = static_cast<uint16_t*>(dup);
+  g.p = static_cast<uint16_t*>(const_cast<void*>(p)), g.q = static_cast<uint16_t*>(const_cast<void*>(q));
+  return launch_dh(g, kmoe::as_stream(stream));
+}
+
+extern "C" int kmoe_dense_dx(const void* dy, const void* dy2, int64_t T, int N, const void* w, const void* w2, int K,
+                             const int32_t* ids, int n_adapters, int rank, const void* u, const void* at, void* dx,
+                             void* stream) {
+  KMOE_DENSE_SIZES("kmoe_dense_dx", T, N, K);
+  if (T == 0) return KMOE_OK;
+  KMOE_REQUIRE(dy && w && dx && !dy2 == !w2, KMOE_ERR_NULL, "kmoe_dense_dx: null buffer");
+  KMOE_DENSE_ALIGNED("kmoe_dense_dx", dy, dy2, w, w2, u, at, dx);
+  Args g{};
+  g.a[0] = static_cast<const uint16_t*>(dy), g.b[0] = static_cast<const uint16_t*>(w);
+  g.a[1] = static_cast<const uint16_t*>(dy2), g.b[1] = static_cast<const uint16_t*>(w2);
+  g.parts = dy2 ? 2 : 1, g.K = N, g.lda = N, g.ldb = K, g.M = T, g.N = K, g.ldc = K, g.c = dx;
+  if (ids) {
+    KMOE_DENSE_ADAPTERS("kmoe_dense_dx", n_adapters, rank);
+    KMOE_REQUIRE(u && at && !dy2, KMOE_ERR_NULL, "kmoe_dense_dx: adapters belong to one product, with both their buffers");
+    g.ad = {ids, {static_cast<const uint16_t*>(u), nullptr}, {static_cast<const uint16_t*>(at), nullptr}, n_adapters, rank};
+  }
+  return ids ? launch_dx_adapt(g, kmoe::as_stream(stream)) : launch_dx(g, kmoe::as_stream(stream));
+}
+
+extern "C" int kmoe_dense_wgrad(const void* a, const void* b, int64_t T, int M, int N, void* c, int c_dtype, void* stream) {
+  KMOE_REQUIRE(T >= 0 && T < ((int64_t)1 << 31) && M > 0 && N > 0 && M % 8 == 0 && N % 8 == 0, KMOE_ERR_SHAPE,
+               "kmoe_dense_wgrad: %lld rows of %d and %d values (positive multiples of 8)", (long long)T, M, N);
+  KMOE_REQUIRE(c_dtype == KMOE_DTYPE_BF16 || c_dtype == KMOE_DTYPE_F32, KMOE_ERR_DTYPE, "kmoe_dense_wgrad: dtype %d", c_dtype);
+  KMOE_REQUIRE(((a && b) || T == 0) && c, KMOE_ERR_NULL, "kmoe_dense_wgrad: null buffer");
+  KMOE_DENSE_ALIGNED("kmoe_dense_wgrad", a, b, c);
+  Args g{};
+  g.a[0] = static_cast<const uint16_t*>(a), g.b[0] = static_cast<const uint16_t*>(b);
+  g.parts = 1, g.K = (int)T, g.lda = M, g.ldb = N, g.M = M, g.N = N, g.ldc = N, g.c = c;
+  g.c_f32 = c_dtype == KMOE_DTYPE_F32;
+  return launch_wgrad(g, kmoe::as_stream(stream));
+}

@@ -1,0 +1,8 @@
+// The backward's products with a Linear weight as it lies.
+#include "kmoe_dense_launch.h"
+
+namespace kmoe_dense {
+int launch_dh(const Args& g, hipStream_t s) { return launch_any<false, true, EPI_DH>(g, s); }
+int launch_dx(const Args& g, hipStream_t s) { return launch_any<false, true, EPI_PLAIN>(g, s); }
+int launch_dx_adapt(const Args& g, hipStream_t s) { return launch_any<false, true, EPI_PLAIN, true>(g, s); }
+}  // namespace kmoe_dense

@@ -21,7 +21,9 @@ DTYPE_F32 = 1
 DTYPE_FP8_E4M3 = 2
 DTYPE_FP4_E2M1 = 3
 SCORES = {"softmax": 0, "sigmoid": 1}
+ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
 MAX_EXPERTS = 64
+MAX_RANK = 128
 ROUTER_HIDDEN = 128
 
 _vp = ctypes.c_void_p
@@ -127,10 +129,29 @@ _SIGNATURES = {
     "kmoe_mx_experts": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _vp, _vp, _vp, _i32, _i32, _i32, _i64, _vp, _vp, _f32, _f32,
                                _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _i32, _vp, _vp, _sz, _vp]),
     "kmoe_gemm_down_mx": (_i32, [_vp, _vp, _i32, _vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp, _vp]),
+    # dense products: the gated block, adapters, their backward
+    "kmoe_gated_ffn_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
+    "kmoe_gated_ffn": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
+    "kmoe_adapted_linear_workspace_bytes": (_sz, [_i64, _i32]),
+    "kmoe_adapted_linear": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _sz, _vp]),
+    "kmoe_adapter_inner": (_i32, [_vp, _i64, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "kmoe_dense_gate_up": (_i32, [_vp, _i64, _i32, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
+                                  _vp]),
+    "kmoe_dense_linear": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "kmoe_dense_dh": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "kmoe_dense_dx": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp]),
+    "kmoe_dense_wgrad": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _i32, _vp]),
+    "kmoe_adapter_grad_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
+    "kmoe_adapter_grad": (_i32, [_vp, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _sz, _vp]),
     # the optimizer step
     "kmoe_adamw": (_i32, [_vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _f32, _vp, _f64, _f64, _f32, _f32, _vp, _vp]),
     "kmoe_adamw_values": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _vp]),
 }
+
+
+class Adapter(ctypes.Structure):
+    """kmoe_adapter of include/kmoe.h."""
+    _fields_ = [("a", _vp), ("b", _vp), ("scale", _vp), ("rank", _i32)]
 
 
 class KmoeError(RuntimeError):

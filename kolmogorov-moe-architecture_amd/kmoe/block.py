@@ -31,7 +31,7 @@ which also adds the residual's gradient.
 With residual dropout active (training, p > 0) the keep mask is one Bernoulli(1-p)
 draw per call (the block's keep_mask_fn) and is applied in the combine, before the
 residual add; its backward scales the MoE's output gradient by the same mask.
-Other configurations (layernorm, expert choice, fp8) run the unfused composition:
+Other configurations (layernorm, expert choice, fp8, a shared expert) run the unfused composition:
 the reference's RMSNorm / LayerNorm in torch, the kmoe MoE layer (MoD-gated in training mode, with its HIP backward where it has one) and a
 torch add.  In training mode the MoD router's auxiliary BCE loss (mod.py:114-171) is
 added to aux_loss on the fused path as on the unfused one (MoDRouter.aux).
@@ -145,7 +145,7 @@ class MoEFFNBlock(nn.Module):
 
     def _fusable(self, h: torch.Tensor) -> bool:
         ffn = self.ffn
-        if not isinstance(self.ffn_norm, RMSNorm) or ffn.routing_type == "expert_choice":
+        if not isinstance(self.ffn_norm, RMSNorm) or ffn.routing_type == "expert_choice" or ffn.shared is not None:
             return False
         if ffn.grouped_experts.use_fp8 or ffn.router.balanced_routing or not ffn.grouped_experts.gated:
             return False
@@ -159,6 +159,8 @@ class MoEFFNBlock(nn.Module):
         """Whether the forward without gradients takes the norm's microscaled rows."""
         ffn = self.ffn
         if not isinstance(self.ffn_norm, RMSNorm) or ffn.routing_type == "expert_choice" or ffn.grouped_experts.mx is None:
+            return False
+        if ffn.shared is not None:
             return False
         if torch.is_grad_enabled() and (h.requires_grad or any(p.requires_grad for p in self.parameters())):
             return False
@@ -201,7 +203,7 @@ class MoEFFNBlock(nn.Module):
         params = tuple(self.parameters())
         if not (h.requires_grad or any(p.requires_grad for p in params)):
             return False
-        if not isinstance(self.ffn_norm, RMSNorm) or ffn.routing_type == "expert_choice":
+        if not isinstance(self.ffn_norm, RMSNorm) or ffn.routing_type == "expert_choice" or ffn.shared is not None:
             return False
         if not ffn._trainable_experts():
             return False

@@ -65,6 +65,9 @@ class AdvancedMoEConfig:
     # A bias for balance: Router.balance_bias (E f32, a buffer that starts at zero and that the
     # training program moves) is added to the scores for the choice of experts only.
     moe_balance_bias: bool = False
+    # Width of a dense gated block that every token takes beside its routed experts (a multiple of 8; 0:
+    # none): MoELayer.shared_expert.
+    moe_shared_d_ff: int = 0
     # Optional per-expert logit bias added before the softmax (E floats).
     moe_router_bias: Optional[Sequence[float]] = None
 

@@ -1,0 +1,387 @@
+"""Dense operators beside the routed experts, on weights as torch.nn.Linear holds them.
+
+* gated_ffn: the gated feed-forward block (act(x Wg^T) * (x Wu^T)) Wd^T (SwiGLU of
+  moe_arch/model/ffn.py:17-64 with act = silu), the layers without experts and the expert that all
+  tokens share (MoELayer's moe_shared_d_ff); without gradients in one native call, with its
+  backward on the HIP kernels.  No packed copies: a step's new weights cost nothing.
+* adapted_linear: a shared projection with low-rank adapters of many requests in one batch,
+  row t with the adapter ids[t]; also on all three projections of the block.
+
+Numerics: bf16 operands, f32 sums.  What is rounded to bf16 between the products: the block's
+hidden values h = act(g) u (an operand of the down product); for the backward u act'(g) and act(g),
+which take the pre-activations' place; an adapter's inner products with their scale.
+"""
+from __future__ import annotations
+
+import ctypes
+import functools
+from typing import NamedTuple, Optional
+
+import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from . import backward as _bwd
+from ._lib import ptr
+from .derived import derived
+from .ops import _BF16, _contig, _device, _one_gpu, _Stage, _stream
+
+
+class Adapters(NamedTuple):
+    """n low-rank adapters of one projection (N, K): row t gets scale[i] (x a[i]^T) b[i]^T, i = ids[t].
+    a (n, r, K), b (n, N, r); scale (n,) f32, None for 1.  Ranks up to 128; one that is not a
+    multiple of 8 is filled up with zeros in every call, so a program that serves keeps it filled."""
+    a: torch.Tensor
+    b: torch.Tensor
+    scale: Optional[torch.Tensor] = None
+
+
+class FFNAdapters(NamedTuple):
+    """Adapters of a gated block's projections, None where there are none; the gate's and the up
+    projection's have one rank."""
+    gate: Optional[Adapters] = None
+    up: Optional[Adapters] = None
+    down: Optional[Adapters] = None
+
+
+# ---------------------------------------------------------------- checks
+def _act(activation) -> int:
+    try:
+        return _lib.ACTIVATIONS[activation]
+    except (KeyError, TypeError):
+        raise ValueError(f"kmoe.gated_ffn: activation {activation!r} is none of {sorted(_lib.ACTIVATIONS)}") from None
+
+
+def _weight(w, rows, cols, who, name):
+    if w.dim() != 2 or (rows is not None and w.shape[0] != rows) or (cols is not None and w.shape[1] != cols):
+        raise ValueError(f"kmoe.{who}: {name} must be ({'N' if rows is None else rows}, {'K' if cols is None else cols}), got "
+                         f"{tuple(w.shape)}")
+    if w.dtype not in (_BF16, torch.float32):
+        raise ValueError(f"kmoe.{who}: {name} is bf16 or f32, got {w.dtype}")
+    if w.shape[0] % 8 or w.shape[1] % 8 or not w.numel():
+        raise ValueError(f"kmoe.{who}: {name} {tuple(w.shape)}: sizes are positive multiples of 8")
+
+
+def _rows(x, K, who):
+    if x.dim() < 1 or x.shape[-1] != K:
+        raise ValueError(f"kmoe.{who}: x {tuple(x.shape)} has rows of {K} values for these weights")
+    if not x.dtype.is_floating_point:
+        raise ValueError(f"kmoe.{who}: x is floating point, got {x.dtype}")
+
+
+def _adapters(ad, K, N, who, name):
+    """The adapters checked, in bf16, ranks filled up to a multiple of 8 (differentiable)."""
+    a, b, scale = ad
+    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or a.shape[2] != K or \
+            b.shape[1] != N or not 1 <= a.shape[1] <= _lib.MAX_RANK or not 1 <= a.shape[0] <= 65535:
+        raise ValueError(f"kmoe.{who}: {name}a must be (n, r, {K}) and b (n, {N}, r), n up to 65535 and r up to "
+                         f"{_lib.MAX_RANK}, got {tuple(a.shape)}, {tuple(b.shape)}")
+    if scale is not None:
+        if scale.shape != (a.shape[0],):
+            raise ValueError(f"kmoe.{who}: {name}scale must be ({a.shape[0]},), got {tuple(scale.shape)}")
+        if scale.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"kmoe.{who}: {name}scale has no gradient here: pass it detached")
+        scale = _contig(scale.detach(), torch.float32)
+    fill = -a.shape[1] % 8
+    if fill:
+        a, b = nn.functional.pad(a, (0, 0, 0, fill)), nn.functional.pad(b, (0, fill))
+    return Adapters(a, b, scale)
+
+
+def _ids(ids, x, n, who):
+    if ids is None:
+        raise ValueError(f"kmoe.{who}: adapters need ids, the adapter of each row (-1: none)")
+    if ids.shape != x.shape[:-1]:
+        raise ValueError(f"kmoe.{who}: ids {tuple(ids.shape)} are not one for each row of x {tuple(x.shape)}")
+    if ids.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"kmoe.{who}: ids are int32 or int64, got {ids.dtype}")
+    if ids.dtype == torch.int64:  # (an id past 32 bits is no adapter, not another one's)
+        ids = ids.clamp(-1, n).to(torch.int32)
+    return ids.reshape(-1).contiguous()
+
+
+def _struct(ad):
+    """kmoe_adapter of bf16 contiguous adapters (the caller keeps the tensors)."""
+    return None if ad is None else ctypes.byref(_lib.Adapter(ptr(ad.a), ptr(ad.b), ptr(ad.scale), ad.a.shape[1]))
+
+
+def _held(ad):
+    return None if ad is None else Adapters(_aligned(ad.a.detach()), _aligned(ad.b.detach()), ad.scale)
+
+
+def _aligned(t):
+    """t in bf16, contiguous, at a multiple of 16 bytes."""
+    t = _contig(t, _BF16)
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+@functools.lru_cache(maxsize=1024)
+def _ffn_workspace(T, F, rgu, rd) -> int:
+    return _lib.load().kmoe_gated_ffn_workspace_bytes(T, F, rgu, rd)
+
+
+# ---------------------------------------------------------------- without gradients
+def _ffn_forward(x2d, wg, wu, wd, act, ads, ids):
+    T, d = x2d.shape
+    F = wg.shape[0]
+    dev = x2d.device
+    y = torch.empty(T, d, device=dev, dtype=_BF16)
+    gate, up, down = ads if ads is not None else (None, None, None)
+    some = gate or up or down
+    rgu = gate.a.shape[1] if gate is not None else up.a.shape[1] if up is not None else 0
+    with _device(dev), _Stage("gated_ffn"):
+        wsb = _ffn_workspace(T, F, rgu, down.a.shape[1] if down is not None else 0)
+        ws = torch.empty(max(wsb, 16), device=dev, dtype=torch.uint8)
+        _lib.call("kmoe_gated_ffn", ptr(x2d), T, d, F, ptr(wg), ptr(wu), ptr(wd), act, ptr(ids),
+                  some.a.shape[0] if some else 0, _struct(gate), _struct(up), _struct(down), ptr(y), ptr(ws), wsb,
+                  _stream(x2d))
+    return y
+
+
+def _linear_forward(x2d, w, ad, ids):
+    T, K = x2d.shape
+    dev = x2d.device
+    y = torch.empty(T, w.shape[0], device=dev, dtype=_BF16)
+    with _device(dev), _Stage("adapted_linear"):
+        wsb = _lib.load().kmoe_adapted_linear_workspace_bytes(T, ad.a.shape[1]) if ad is not None else 0
+        ws = torch.empty(max(wsb, 16), device=dev, dtype=torch.uint8)
+        _lib.call("kmoe_adapted_linear", ptr(x2d), T, K, ptr(w), w.shape[0], ptr(ids), ad.a.shape[0] if ad is not None else 0,
+                  _struct(ad), ptr(y), ptr(ws), wsb, _stream(x2d))
+    return y
+
+
+# ---------------------------------------------------------------- parts of the backward
+def _inner(x2d, ids, a, scale):
+    """(T, r) bf16 scaled inner products; rows without an adapter are not written."""
+    v = torch.empty(x2d.shape[0], a.shape[1], device=x2d.device, dtype=_BF16)
+    _lib.call("kmoe_adapter_inner", ptr(x2d), x2d.shape[0], x2d.shape[1], ptr(ids), a.shape[0], a.shape[1], ptr(a), ptr(scale),
+              ptr(v), None, None, None, _stream(x2d))
+    return v
+
+
+def _factor_grad(l, m, ids, n, outer):
+    T, r = l.shape
+    C = m.shape[1]
+    out = torch.empty((n, C, r) if outer else (n, r, C), device=m.device, dtype=_BF16)
+    wsb = _lib.load().kmoe_adapter_grad_workspace_bytes(T, n, r, C)
+    ws = torch.empty(max(wsb, 16), device=m.device, dtype=torch.uint8)
+    _lib.call("kmoe_adapter_grad", ptr(l), ptr(m), T, ptr(ids), n, r, C, int(outer), ptr(out), ptr(ws), wsb, _stream(m))
+    return out
+
+
+def _dense_dx(dy, w, dy2=None, w2=None, ids=None, n=0, u=None, at=None):
+    T, N = dy.shape
+    K = w.shape[1]
+    dx = torch.empty(T, K, device=dy.device, dtype=_BF16)
+    _lib.call("kmoe_dense_dx", ptr(dy), ptr(dy2), T, N, ptr(w), ptr(w2), K, ptr(ids), n, 0 if u is None else u.shape[1],
+              ptr(u), ptr(at), ptr(dx), _stream(dy))
+    return dx
+
+
+def _dense_wgrad(a, b, dtype):
+    """a^T b, (M, N), in the weight's type."""
+    T, M = a.shape
+    N = b.shape[1]
+    dt = torch.float32 if dtype == torch.float32 else _BF16
+    c = torch.empty(M, N, device=a.device, dtype=dt)
+    _lib.call("kmoe_dense_wgrad", ptr(a), ptr(b), T, M, N, ptr(c), _lib.DTYPE_F32 if dt == torch.float32 else _lib.DTYPE_BF16,
+              _stream(a))
+    return c
+
+
+# ---------------------------------------------------------------- the gated block
+class _GatedFFNFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wg, wu, wd, act):
+        _bwd.leaves_of(ctx, x, wg, wu, wd)
+        x2d = _aligned(x.detach().reshape(-1, x.shape[-1]))
+        bg, bu, bd = (_aligned(w.detach()) for w in (wg, wu, wd))
+        T, d = x2d.shape
+        F = bg.shape[0]
+        h, p, q = (torch.empty(T, F, device=x.device, dtype=_BF16) for _ in range(3))
+        y = torch.empty(T, d, device=x.device, dtype=_BF16)
+        with _device(x.device):
+            with _Stage("ffn_gate_up"):
+                _lib.call("kmoe_dense_gate_up", ptr(x2d), T, d, ptr(bg), ptr(bu), F, act, None, 0, 0, None, None, None, None,
+                          ptr(h), ptr(p), ptr(q), _stream(x))
+            with _Stage("ffn_down"):
+                _lib.call("kmoe_dense_linear", ptr(h), T, F, ptr(bd), d, None, 0, 0, None, None, ptr(y), _stream(x))
+        # the weights themselves are saved too: a write to one before the backward is refused
+        ctx.save_for_backward(x2d, h, p, q, bg, bu, bd, wg, wu, wd)
+        ctx.meta = (x.shape, x.dtype)
+        return y.view(x.shape).to(x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x2d, h, p, q, bg, bu, bd, wg, wu, wd = ctx.saved_tensors
+        shape, dtype = ctx.meta
+        T, F = h.shape
+        d = x2d.shape[1]
+        need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
+        dy2 = _aligned(dy.reshape(T, d))
+        dx = dg = du = dwg = dwu = dwd = None
+        with _device(x2d.device):
+            if need_x or need_g or need_u:
+                dg, du = (torch.empty(T, F, device=x2d.device, dtype=_BF16) for _ in range(2))
+                with _Stage("bwd_ffn_dh"):
+                    _lib.call("kmoe_dense_dh", ptr(dy2), T, d, ptr(bd), F, ptr(p), ptr(q), ptr(dg), ptr(du), _stream(x2d))
+            if need_x:
+                with _Stage("bwd_ffn_dx"):
+                    dx = _dense_dx(dg, bg, du, bu).view(shape).to(dtype)
+            with _Stage("bwd_ffn_wgrad"):
+                if need_g:
+                    dwg = _dense_wgrad(dg, x2d, wg.dtype)
+                if need_u:
+                    dwu = _dense_wgrad(du, x2d, wu.dtype)
+                if need_d:
+                    dwd = _dense_wgrad(dy2, h, wd.dtype)
+        return dx, dwg, dwu, dwd, None
+
+
+_ACT_FN = {"silu": nn.functional.silu, "gelu": nn.functional.gelu,
+           "gelu_tanh": functools.partial(nn.functional.gelu, approximate="tanh"), "relu": torch.relu}
+
+
+def _wants_grad(*ts) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts)
+
+
+def gated_ffn(x, w_gate, w_up, w_down, activation="silu", adapters: Optional[FFNAdapters] = None, ids=None):
+    """(act(x w_gate^T) * (x w_up^T)) w_down^T for rows x (..., d): w_gate, w_up (F, d), w_down (d, F), bf16
+    or f32 (cast to bf16 in the call), d and F multiples of 8; activation "silu", "gelu",
+    "gelu_tanh" or "relu".  The result has x's type.  adapters with ids (..., int32 or int64): each row's
+    own low-rank adapter on the three projections, -1 (or any id that is no adapter) for none.
+
+    Differentiable in x, the weights and the adapters; with adapters the projections then run one by
+    one and the activation between them is torch's."""
+    act = _act(activation)
+    _weight(w_gate, None, None, "gated_ffn", "w_gate")
+    F, d = w_gate.shape
+    _weight(w_up, F, d, "gated_ffn", "w_up")
+    _weight(w_down, d, F, "gated_ffn", "w_down")
+    _rows(x, d, "gated_ffn")
+    if adapters is not None and not any(a is not None for a in adapters):
+        adapters = None
+    if adapters is None:
+        _one_gpu("gated_ffn", x, w_gate, w_up, w_down)
+        if _wants_grad(x, w_gate, w_up, w_down):
+            return _GatedFFNFn.apply(x, w_gate, w_up, w_down, act)
+        i32 = None
+    else:
+        sizes = dict(gate=(d, F), up=(d, F), down=(F, d))
+        adapters = FFNAdapters(*(None if a is None else _adapters(a, *sizes[k], "gated_ffn", f"{k} adapters: ")
+                                 for k, a in zip(sizes, adapters)))
+        some = [a for a in adapters if a is not None]
+        _one_gpu("gated_ffn", x, w_gate, w_up, w_down, ids, *(t for a in some for t in a))
+        if len({a.a.shape[0] for a in some}) > 1:
+            raise ValueError(f"kmoe.gated_ffn: the projections have as many adapters each, got {[a.a.shape[0] for a in some]}")
+        if adapters.gate is not None and adapters.up is not None and adapters.gate.a.shape[1] != adapters.up.a.shape[1]:
+            raise ValueError(f"kmoe.gated_ffn: the gate's and the up projection's adapters have one rank, got "
+                             f"{adapters.gate.a.shape[1]} and {adapters.up.a.shape[1]}")
+        i32 = _ids(ids, x, some[0].a.shape[0], "gated_ffn")
+        if _wants_grad(x, w_gate, w_up, w_down, *(t for a in some for t in a[:2])):
+            g, u = (_adapted(x, w, a, i32) for w, a in ((w_gate, adapters.gate), (w_up, adapters.up)))
+            return _adapted((_ACT_FN[activation](g.float()) * u.float()).to(_BF16), w_down, adapters.down, i32).to(x.dtype)
+        adapters = FFNAdapters(*(_held(a) for a in adapters))
+    x2d = _aligned(x.detach().reshape(-1, d))
+    y = _ffn_forward(x2d, *(_aligned(w.detach()) for w in (w_gate, w_up, w_down)), act, adapters, i32)
+    return y.view(x.shape).to(x.dtype)
+
+
+# ---------------------------------------------------------------- adapted projections
+class _AdaptedFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, a, b, scale, ids):
+        _bwd.leaves_of(ctx, x, w, a, b)
+        x2d = _aligned(x.detach().reshape(-1, x.shape[-1]))
+        bw = _aligned(w.detach())
+        ba, bb = (None, None) if a is None else (_aligned(a.detach()), _aligned(b.detach()))
+        T, K = x2d.shape
+        N = bw.shape[0]
+        y = torch.empty(T, N, device=x.device, dtype=_BF16)
+        v = None
+        with _device(x.device), _Stage("adapted_linear"):
+            if a is not None:
+                v = _inner(x2d, ids, ba, scale)
+            _lib.call("kmoe_dense_linear", ptr(x2d), T, K, ptr(bw), N, None if a is None else ptr(ids),
+                      0 if a is None else ba.shape[0], 0 if a is None else ba.shape[1], ptr(v), ptr(bb), ptr(y), _stream(x))
+        ctx.save_for_backward(x2d, bw, ba, bb, scale, ids if a is not None else None, v, w, a, b)
+        ctx.meta = (x.shape, x.dtype)
+        return y.view(*x.shape[:-1], N).to(x.dtype)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x2d, bw, ba, bb, scale, ids, v, w, a, b = ctx.saved_tensors
+        shape, dtype = ctx.meta
+        T, N = x2d.shape[0], bw.shape[0]
+        need_x, need_w, need_a, need_b = ctx.needs_input_grad[:4]
+        dy2 = _aligned(dy.reshape(T, N))
+        dx = dw = da = db = u = None
+        with _device(x2d.device), _Stage("bwd_adapted_linear"):
+            if ba is not None and (need_x or need_a):
+                u = _inner(dy2, ids, bb.transpose(1, 2).contiguous(), scale)
+            if need_x:
+                dx = (_dense_dx(dy2, bw) if ba is None else
+                      _dense_dx(dy2, bw, ids=ids, n=ba.shape[0], u=u, at=ba.transpose(1, 2).contiguous()))
+                dx = dx.view(shape).to(dtype)
+            if need_w:
+                dw = _dense_wgrad(dy2, x2d, w.dtype)
+            if need_a:
+                da = _factor_grad(u, x2d, ids, ba.shape[0], False).to(a.dtype)
+            if need_b:
+                db = _factor_grad(v, dy2, ids, ba.shape[0], True).to(b.dtype)
+        return dx, dw, da, db, None, None
+
+
+def _adapted(x, w, ad, i32):
+    """adapted_linear of checked arguments, with gradients."""
+    a, b, scale = ad if ad is not None else (None, None, None)
+    return _AdaptedFn.apply(x, w, a, b, scale, i32)
+
+
+def adapted_linear(x, weight, adapters: Optional[Adapters] = None, ids=None):
+    """x weight^T for rows x (..., K), weight (N, K) bf16 or f32 (cast to bf16 in the call), plus each
+    row's low-rank adapter: row t gets scale[i] (x a[i]^T) b[i]^T, i = ids[t] (ids (...,) int32 or int64;
+    -1, or any id that is no adapter: nothing).  K and N multiples of 8.  The result has x's
+    type.  Differentiable in x, the weight and the adapters' a and b."""
+    _weight(weight, None, None, "adapted_linear", "weight")
+    N, K = weight.shape
+    _rows(x, K, "adapted_linear")
+    i32 = None
+    if adapters is not None:
+        adapters = _adapters(adapters, K, N, "adapted_linear", "")
+        _one_gpu("adapted_linear", x, weight, ids, *adapters)
+        i32 = _ids(ids, x, adapters.a.shape[0], "adapted_linear")
+    else:
+        _one_gpu("adapted_linear", x, weight)
+    if _wants_grad(x, weight, *(adapters[:2] if adapters is not None else ())):
+        return _adapted(x, weight, adapters, i32)
+    y = _linear_forward(_aligned(x.detach().reshape(-1, K)), _aligned(weight.detach()), _held(adapters), i32)
+    return y.view(*x.shape[:-1], N).to(x.dtype)
+
+
+# ---------------------------------------------------------------- module
+class GatedFFN(nn.Module):
+    """The reference's gated block (SwiGLU, moe_arch/model/ffn.py:17-64: w1 gate, w2 up, w3 down, no
+    biases) on the HIP kernels, for the layers without experts and for a shared expert."""
+
+    def __init__(self, d_model: int, d_ff: int, activation: str = "silu"):
+        super().__init__()
+        _act(activation)
+        if d_model <= 0 or d_ff <= 0 or d_model % 8 or d_ff % 8:
+            raise ValueError(f"kmoe.GatedFFN: d_model={d_model}, d_ff={d_ff}: positive multiples of 8")
+        self.d_model, self.d_ff, self.activation = d_model, d_ff, activation
+        self.w1 = nn.Linear(d_model, d_ff, bias=False)
+        self.w2 = nn.Linear(d_model, d_ff, bias=False)
+        self.w3 = nn.Linear(d_ff, d_model, bias=False)
+        self._bf16_cache = None
+
+    def forward(self, x: torch.Tensor, adapters: Optional[FFNAdapters] = None, ids=None) -> torch.Tensor:
+        ws = (self.w1.weight, self.w2.weight, self.w3.weight)
+        if ws[0].dtype != _BF16 and not _wants_grad(x, *ws):
+            # f32 weights: their casts are kept until one changes
+            ws = derived(self.__dict__, "_bf16_cache", ws, lambda: tuple(w.detach().to(_BF16) for w in ws))
+        return gated_ffn(x, *ws, self.activation, adapters, ids)

@@ -185,8 +185,8 @@ def _mod_ffn(ffn: MoELayer, mod_router: MoDRouter, hidden_states: torch.Tensor,
     x = hidden_states.detach().to(torch.bfloat16).contiguous()
     sel = mod_router.select(x)
     mod_router.aux(x.view(B * S, d), sel.token_rows)
-    if ffn.routing_type == "expert_choice":
-        return _mod_expert_choice(ffn, mod_router, hidden_states, residual, sel)
+    if ffn.routing_type == "expert_choice" or ffn.shared is not None:
+        return _mod_composed(ffn, mod_router, hidden_states, residual, sel)
     if mod_trainable(ffn, mod_router, hidden_states, residual):
         ge = ffn.grouped_experts
         y, aux = _MoDTrainFn.apply(hidden_states, residual, mod_router.router.weight, ffn.router.router[0].weight,
@@ -205,10 +205,10 @@ def _mod_ffn(ffn: MoELayer, mod_router: MoDRouter, hidden_states: torch.Tensor,
                          *mod_router.parameters())
 
 
-def _mod_expert_choice(ffn: MoELayer, mod_router: MoDRouter, hidden_states: torch.Tensor,
-                       residual: torch.Tensor, sel: ops.ModSelectOut) -> torch.Tensor:
+def _mod_composed(ffn: MoELayer, mod_router: MoDRouter, hidden_states: torch.Tensor,
+                  residual: torch.Tensor, sel: ops.ModSelectOut) -> torch.Tensor:
     """MoD around an expert-choice MoELayer (layers.py:148-187 with moe_routing
-    "expert_choice"): at the MoD selection sel, the kept rows (B, keep, d) through
+    "expert_choice") or one with a shared expert: at the MoD selection sel, the kept rows (B, keep, d) through
     the expert-choice layer (its capacity from the kept length, moe.py:494-530; it trains
     through its own HIP backward and sets ffn.aux_loss), then the rows weighted by the
     softmax over the kept logits (mod.py:112) and scattered back (layers.py:175-184).

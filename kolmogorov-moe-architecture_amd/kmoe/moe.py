@@ -34,6 +34,7 @@ from . import _lib
 from . import backward as _bwd
 from . import ops
 from .config import AdvancedMoEConfig
+from .dense import GatedFFN
 from .derived import Sources, derived
 
 ROUTER_HIDDEN = 128  # moe.py:346
@@ -790,6 +791,11 @@ class MoELayer(nn.Module):
                                                  config.ffn_activation)
             self.grouped_experts.use_fp8 = use_fp8
             self.grouped_experts.mx = mx
+        shared = int(getattr(config, "moe_shared_d_ff", 0) or 0)
+        if shared and getattr(config, "ffn_activation", "swiglu") != "swiglu":
+            raise NotImplementedError("kmoe: a shared expert is implemented for swiglu only")
+        # a dense block that every token takes: y = routed experts + shared_expert(h)
+        self.shared_expert = GatedFFN(config.d_model, shared) if shared else None
         self.experts = None
         self.load_balance_loss_weight = config.moe_load_balance_loss_weight
         self.router_z_loss_weight = config.moe_router_z_loss_weight
@@ -803,7 +809,14 @@ class MoELayer(nn.Module):
             y = self._forward_expert_choice(hidden_states)
         else:
             y = self._forward_token_choice(hidden_states)
+        if self.shared is not None:
+            y = y + self.shared(hidden_states)
         return (y, self.aux_loss) if return_aux else y
+
+    @property
+    def shared(self) -> Optional[GatedFFN]:
+        """The shared expert, None without one (also in a layer pickled before there were any)."""
+        return self._modules.get("shared_expert")
 
     def _out_dtype(self, x):
         return torch.float32 if x.dtype == torch.float32 else torch.bfloat16

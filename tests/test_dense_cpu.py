@@ -1,0 +1,167 @@
+"""The dense operators without a GPU: refusals of arguments, in Python and at the C ABI."""
+import ctypes
+
+import pytest
+import torch
+
+import kmoe
+from kmoe import _lib
+
+BF = torch.bfloat16
+FAKE = ctypes.c_void_p(0x1000)  # never dereferenced: validation fails first
+ODD = ctypes.c_void_p(0x1008)
+
+
+def z(*s, dtype=BF):
+    return torch.zeros(*s, dtype=dtype)
+
+
+def ad(n=2, r=8, K=64, N=72):
+    return kmoe.Adapters(z(n, r, K), z(n, N, r), torch.ones(n))
+
+
+IDS = torch.zeros(4, dtype=torch.int32)
+
+
+@pytest.mark.parametrize("args,kw,match", [
+    ((z(4, 64), z(72, 64), z(72, 64), z(64, 72), "swish"), {}, "activation"),
+    ((z(4, 64), z(72, 64), z(72, 64), z(64, 72), ["silu"]), {}, "activation"),
+    ((z(4, 64), z(72, 64), z(72, 56), z(64, 72)), {}, "w_up"),
+    ((z(4, 64), z(72, 64), z(72, 64), z(72, 64)), {}, "w_down"),
+    ((z(4, 56), z(72, 64), z(72, 64), z(64, 72)), {}, "x "),
+    ((z(4, 64).int(), z(72, 64), z(72, 64), z(64, 72)), {}, "floating point"),
+    ((z(4, 60), z(72, 60), z(72, 60), z(60, 72)), {}, "multiples of 8"),
+    ((z(4, 64), z(70, 64), z(70, 64), z(64, 70)), {}, "multiples of 8"),
+    ((z(4, 64), z(72, 64, dtype=torch.float16), z(72, 64), z(64, 72)), {}, "bf16 or f32"),
+    ((z(4, 64), z(72, 64), z(72, 64), z(64, 72)), {}, "on a GPU"),
+    ((z(4, 64), z(72, 64), z(72, 64), z(64, 72)), dict(adapters=kmoe.FFNAdapters(gate=ad(N=64)), ids=IDS), "gate adapters"),
+    ((z(4, 64), z(72, 64), z(72, 64), z(64, 72)), dict(adapters=kmoe.FFNAdapters(gate=ad()), ids=IDS), "on a GPU"),
+])
+def test_ffn_refusals(args, kw, match):
+    with pytest.raises(ValueError, match=match):
+        kmoe.gated_ffn(*args, **kw)
+
+
+def test_adapter_refusals():
+    x, w = z(4, 64), z(72, 64)
+    bad = [ad()._replace(a=z(2, 8, 72)), ad()._replace(b=z(2, 64, 8)), ad()._replace(b=z(3, 72, 8)), ad()._replace(b=z(2, 72, 16)),
+           ad(r=136), ad(r=0), ad(n=0), ad()._replace(a=z(8, 64))]
+    for a in bad:
+        with pytest.raises(ValueError, match="adapted_linear: a must be"):
+            kmoe.adapted_linear(x, w, a, IDS)
+    with pytest.raises(ValueError, match="scale must be"):
+        kmoe.adapted_linear(x, w, ad()._replace(scale=torch.ones(3)), IDS)
+    with pytest.raises(ValueError, match="no gradient"):
+        kmoe.adapted_linear(x, w, ad()._replace(scale=torch.ones(2, requires_grad=True)), IDS)
+    with pytest.raises(ValueError, match="on a GPU"):
+        kmoe.adapted_linear(x, w, ad(), IDS)
+    from kmoe.dense import _ids
+    with pytest.raises(ValueError, match="need ids"):
+        _ids(None, x, 2, "adapted_linear")
+    with pytest.raises(ValueError, match="one for each row"):
+        _ids(IDS[:3], x, 2, "adapted_linear")
+    with pytest.raises(ValueError, match="int32 or int64"):
+        _ids(IDS.float(), x, 2, "adapted_linear")
+    assert _ids(torch.tensor([1 << 32, -5, 0, 1]), x, 2, "adapted_linear").tolist() == [2, -1, 0, 1]
+
+
+def test_module():
+    with pytest.raises(ValueError, match="multiples of 8"):
+        kmoe.GatedFFN(60, 72)
+    with pytest.raises(ValueError, match="activation"):
+        kmoe.GatedFFN(64, 72, "tanh")
+    m = kmoe.GatedFFN(64, 72)
+    assert [tuple(p.shape) for p in m.parameters()] == [(72, 64), (72, 64), (64, 72)]
+    c = kmoe.get_test_config()
+    assert kmoe.MoELayer(c).shared is None
+    c.moe_shared_d_ff = 704
+    layer = kmoe.MoELayer(c)
+    assert layer.shared is layer.shared_expert and layer.shared.d_ff == 704
+    import pickle
+    old = kmoe.MoELayer(kmoe.get_test_config())
+    del old.__dict__["shared_expert"]  # as a layer pickled before there were any
+    assert pickle.loads(pickle.dumps(old)).shared is None
+    c.ffn_activation = "silu"
+    with pytest.raises(NotImplementedError, match="swiglu"):
+        kmoe.MoELayer(c)
+
+
+def _call(name, good):
+    fn = getattr(_lib.load(), name)
+
+    def call(**at):
+        a = list(good)
+        for k, v in at.items():
+            a[int(k[1:])] = v
+        return fn(*a)
+    return call
+
+
+def test_abi_gated_ffn():
+    a = _lib.Adapter(0x1000, 0x1000, None, 8)
+    ws = _lib.load().kmoe_gated_ffn_workspace_bytes(100, 72, 8, 8)
+    assert ws >= 100 * 72 * 2 + 3 * 100 * 8 * 2
+    call = _call("kmoe_gated_ffn", [FAKE, 100, 64, 72, FAKE, FAKE, FAKE, 0, FAKE, 2, ctypes.byref(a), ctypes.byref(a),
+                                    ctypes.byref(a), FAKE, FAKE, ws, None])
+    assert call(a1=0) == 0
+    for i in (0, 4, 5, 6, 8, 13, 14):
+        assert call(**{f"a{i}": None}) == -1, i
+    for i in (0, 4, 5, 6, 13, 14):
+        assert call(**{f"a{i}": ODD}) == -2, i
+    assert call(a1=-1) == -2 and call(a1=1 << 31) == -2 and call(a2=60) == -2 and call(a3=0) == -2
+    assert call(a7=4) == -6 and call(a7=-1) == -6
+    assert call(a9=0) == -2 and call(a15=ws - 1) == -4
+    for r in (0, 4, 136):
+        assert call(a10=ctypes.byref(_lib.Adapter(0x1000, 0x1000, None, r))) == -2
+    assert call(a11=ctypes.byref(_lib.Adapter(0x1000, 0x1000, None, 16))) == -2  # not the gate's rank
+    assert call(a12=ctypes.byref(_lib.Adapter(None, 0x1000, None, 8))) == -1
+    assert call(a12=ctypes.byref(_lib.Adapter(0x1008, 0x1000, None, 8))) == -2
+
+
+def test_abi_adapted_linear():
+    a = _lib.Adapter(0x1000, 0x1000, None, 8)
+    ws = _lib.load().kmoe_adapted_linear_workspace_bytes(100, 8)
+    call = _call("kmoe_adapted_linear", [FAKE, 100, 64, FAKE, 72, FAKE, 2, ctypes.byref(a), FAKE, FAKE, ws, None])
+    assert call(a1=0) == 0 and call(a10=ws - 1) == -4 and call(a9=None) == -4
+    for i in (0, 3, 5, 8):
+        assert call(**{f"a{i}": None}) == -1, i
+    assert call(a2=4) == -2 and call(a4=-8) == -2 and call(a6=0) == -2 and call(a8=ODD) == -2
+
+
+def test_abi_parts():
+    call = _call("kmoe_adapter_inner", [FAKE, 100, 64, FAKE, 2, 8, FAKE, FAKE, FAKE, None, None, None, None])
+    assert call(a1=0) == 0
+    for i in (0, 3, 6, 8):
+        assert call(**{f"a{i}": None}) == -1, i
+    assert call(a9=FAKE) == -1 and call(a2=60) == -2 and call(a4=0) == -2 and call(a5=12) == -2 and call(a6=ODD) == -2
+    call = _call("kmoe_dense_gate_up", [FAKE, 100, 64, FAKE, FAKE, 72, 0, FAKE, 2, 8, FAKE, FAKE, FAKE, FAKE, FAKE, None, None,
+                                        None])
+    assert call(a1=0) == 0
+    for i in (0, 3, 4, 10, 13, 14):
+        assert call(**{f"a{i}": None}) == -1, i
+    assert call(a15=FAKE, a16=FAKE) == -1 and call(a15=FAKE) == -1  # adapters and values for a backward; p without q
+    assert call(a6=9) == -6 and call(a2=63) == -2 and call(a14=ODD) == -2 and call(a9=7) == -2
+    call = _call("kmoe_dense_linear", [FAKE, 100, 64, FAKE, 72, FAKE, 2, 8, FAKE, FAKE, FAKE, None])
+    assert call(a1=0) == 0
+    for i in (0, 3, 8, 9, 10):
+        assert call(**{f"a{i}": None}) == -1, i
+    assert call(a2=0) == -2 and call(a4=71) == -2 and call(a10=ODD) == -2
+    call = _call("kmoe_dense_dh", [FAKE, 100, 64, FAKE, 72, FAKE, FAKE, FAKE, FAKE, None])
+    assert call(a1=0) == 0
+    for i in (0, 3, 5, 6, 7, 8):
+        assert call(**{f"a{i}": None}) == -1, i
+    call = _call("kmoe_dense_dx", [FAKE, None, 100, 72, FAKE, None, 64, FAKE, 2, 8, FAKE, FAKE, FAKE, None])
+    assert call(a2=0) == 0
+    for i in (0, 4, 10, 11, 12):
+        assert call(**{f"a{i}": None}) == -1, i
+    assert call(a1=FAKE) == -1 and call(a1=FAKE, a5=FAKE) == -1  # two products and adapters
+    call = _call("kmoe_dense_wgrad", [FAKE, FAKE, 101, 72, 64, FAKE, 0, None])
+    for i in (0, 1, 5):
+        assert call(**{f"a{i}": None}) == -1, i
+    assert call(a2=-1) == -2 and call(a3=4) == -2 and call(a4=0) == -2 and call(a6=2) == -3 and call(a5=ODD) == -2
+    n = _lib.load().kmoe_adapter_grad_workspace_bytes(4096, 1, 8, 64)
+    assert n > 0
+    call = _call("kmoe_adapter_grad", [FAKE, FAKE, 4096, FAKE, 1, 8, 64, 0, FAKE, FAKE, n, None])
+    for i in (0, 1, 3, 8):
+        assert call(**{f"a{i}": None}) == -1, i
+    assert call(a10=n - 1) == -4 and call(a4=65536) == -2 and call(a5=136) == -2 and call(a6=4) == -2 and call(a2=-1) == -2

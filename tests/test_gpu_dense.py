@@ -1,0 +1,445 @@
+"""The gated block and adapted projections on the GPU against their formulas in 64 bits, within
+bounds that carry every rounding (dense_bounds.py)."""
+import os
+import sys
+
+import pytest
+import torch
+
+import kmoe
+
+sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
+import dense_bounds as B  # noqa: E402
+
+pytestmark = pytest.mark.gpu
+
+BF = torch.bfloat16
+ACTS = ("silu", "gelu", "gelu_tanh", "relu")
+
+
+def rnd(dev, *shape, std=1.0, dtype=BF, seed=[0]):
+    seed[0] += 1
+    g = torch.Generator().manual_seed(seed[0])
+    return torch.randn(*shape, generator=g).mul(std).to(dtype).to(dev)
+
+
+def make_ffn(dev, T, d, F):
+    return rnd(dev, T, d), rnd(dev, F, d, std=d ** -0.5), rnd(dev, F, d, std=d ** -0.5), rnd(dev, d, F, std=F ** -0.5)
+
+
+def make_ad(dev, n, r, K, N, scale=True):
+    return kmoe.Adapters(rnd(dev, n, r, K, std=K ** -0.5), rnd(dev, n, N, r, std=0.3),
+                         torch.linspace(0.5, 2.0, n).to(dev) if scale else None)
+
+
+# rows from one to many (few-row kernels up to 64, the three tiles beyond), widths of odd eighths
+SIZES = [(1, 64, 72), (2, 8, 8), (5, 136, 128), (16, 200, 24), (17, 72, 264), (33, 256, 136), (64, 520, 200), (65, 64, 72),
+         (127, 200, 136), (130, 136, 392), (300, 520, 264), (777, 64, 1032), (2042, 72, 1544), (16379, 136, 1096)]
+
+
+@pytest.mark.parametrize("T,d,F", SIZES)
+def test_ffn(dev, T, d, F):
+    x, wg, wu, wd = make_ffn(dev, T, d, F)
+    for act in ACTS if T in (5, 130) else ("silu",):
+        with torch.no_grad():
+            y = kmoe.gated_ffn(x, wg, wu, wd, act)
+        B.check(act, y, B.ffn(x, wg, wu, wd, act)[0])
+
+
+@pytest.mark.parametrize("T,d,F", SIZES)
+def test_ffn_backward(dev, T, d, F):
+    x, wg, wu, wd = make_ffn(dev, T, d, F)
+    dy = rnd(dev, T, d)
+    for act in ACTS if T in (5, 130) else ("silu",):
+        leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+        y = kmoe.gated_ffn(*leaves, act)
+        grads = torch.autograd.grad(y, leaves, dy)
+        want, h, p, q = B.ffn(x, wg, wu, wd, act)
+        B.check(act, y.detach(), want)
+        for name, g, w in zip(("dx", "dwg", "dwu", "dwd"), grads, B.ffn_grads(x, wg, wu, wd, dy, h, p, q)):
+            B.check((act, name), g, w)
+
+
+def test_ffn_gradient_is_the_difference(dev):
+    """The gradients against differences of the block itself, in a direction of every input."""
+    x, wg, wu, wd = make_ffn(dev, 40, 64, 72)
+    dy = rnd(dev, 40, 64)
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    grads = torch.autograd.grad(kmoe.gated_ffn(*leaves, "gelu"), leaves, dy)
+
+    def f(ts):  # the block in f64, so that the difference quotient is exact to about 1e-9
+        x, wg, wu, wd = ts
+        return float(((torch.nn.functional.gelu(x @ wg.t()) * (x @ wu.t())) @ wd.t() * dy.double()).sum())
+    base = [t.double() for t in (x, wg, wu, wd)]
+    for i, g in enumerate(grads):
+        way = torch.randn_like(base[i])
+        eps = 1e-5
+        up, down = list(base), list(base)
+        up[i], down[i] = base[i] + eps * way, base[i] - eps * way
+        slope = (f(up) - f(down)) / (2 * eps)
+        # each element is off by a few roundings of bf16 of its terms, of either sign: their sum in
+        # a random direction stays within 8 of the root of their squares
+        bound = 8 * 4 * 2.0 ** -8 * float((g.double() * way).norm())
+        assert abs(float((g.double() * way).sum()) - slope) <= bound
+
+
+@pytest.mark.parametrize("need", [(1, 0, 0, 0), (0, 1, 0, 0), (0, 0, 1, 0), (0, 0, 0, 1), (1, 0, 0, 1)])
+def test_ffn_some_gradients(dev, need):
+    x, wg, wu, wd = make_ffn(dev, 70, 64, 136)
+    dy = rnd(dev, 70, 64)
+    full = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    all_g = torch.autograd.grad(kmoe.gated_ffn(*full), full, dy)
+    part = [t.clone().requires_grad_(bool(k)) for t, k in zip((x, wg, wu, wd), need)]
+    kmoe.gated_ffn(*part).backward(dy)
+    for t, g, k in zip(part, all_g, need):
+        assert (t.grad is None) if not k else torch.equal(t.grad, g)
+
+
+def test_ffn_f32_weights_and_rows(dev):
+    """f32 masters: products of their bf16 casts, gradients of the weights in f32, of x in x's type."""
+    x, wg, wu, wd = (t.float() for t in make_ffn(dev, 100, 64, 72))
+    wg = wg + 1e-4
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = kmoe.gated_ffn(*leaves)
+    dy = rnd(dev, 100, 64, dtype=torch.float32)
+    grads = torch.autograd.grad(y, leaves, dy)
+    cast = [t.to(BF) for t in (x, wg, wu, wd)]
+    want, h, p, q = B.ffn(*cast, "silu")
+    assert y.dtype == torch.float32
+    B.check("y", y.detach().to(BF), want)
+    assert torch.equal(y.detach().to(BF).float(), y.detach())
+    bw = B.ffn_grads(*cast, dy.to(BF), h, p, q)
+    B.check("dx", grads[0].to(BF), bw[0])
+    for g, w in zip(grads[1:], bw[1:]):
+        B.check("dw", g, w, torch.float32)
+
+
+def test_ffn_layouts(dev):
+    """Leading dimensions, strided and misaligned inputs, no rows."""
+    x, wg, wu, wd = make_ffn(dev, 96, 64, 72)
+    y = kmoe.gated_ffn(x, wg, wu, wd)
+    assert torch.equal(kmoe.gated_ffn(x.view(2, 4, 12, 64), wg, wu, wd), y.view(2, 4, 12, 64))
+    wide = torch.randn(96, 128, device=dev).to(BF)
+    wide[:, :64] = x
+    assert torch.equal(kmoe.gated_ffn(wide[:, :64], wg, wu, wd), y)
+    buf = torch.empty(96 * 64 + 1, device=dev, dtype=BF)
+    buf[1:] = x.view(-1)
+    assert torch.equal(kmoe.gated_ffn(buf[1:].view(96, 64), wg, wu, wd), y)
+    assert torch.equal(kmoe.gated_ffn(x, wg.t().contiguous().t(), wu, wd), y)
+    assert torch.equal(kmoe.gated_ffn(x[5], wg, wu, wd), kmoe.gated_ffn(x[5:6], wg, wu, wd)[0])
+    e = x[:0].clone().requires_grad_(True)
+    w = wg.clone().requires_grad_(True)
+    out = kmoe.gated_ffn(e, w, wu, wd)
+    out.sum().backward()
+    assert out.shape == (0, 64) and e.grad.shape == (0, 64) and bool((w.grad == 0).all())
+
+
+def test_rows_stay_apart(dev):
+    """A row of NaN or infinities leaves the others as they were, and what lies past the rows too."""
+    for T in (33, 200, 700):
+        x, wg, wu, wd = make_ffn(dev, T, 136, 200)
+        y = kmoe.gated_ffn(x, wg, wu, wd)
+        z = x.clone()
+        z[7] = float("nan")
+        z[20, 3] = float("inf")
+        got = kmoe.gated_ffn(z, wg, wu, wd)
+        keep = torch.ones(T, dtype=torch.bool, device=dev)
+        keep[[7, 20]] = False
+        assert torch.equal(got[keep], y[keep]) and bool(got[7].isnan().all())
+
+
+# ---------------------------------------------------------------- adapters
+LINEAR = [(1, 64, 72, 3, 8), (3, 8, 8, 1, 8), (16, 72, 200, 5, 16), (48, 136, 136, 48, 16), (64, 264, 72, 2, 64), (65, 72, 136, 4, 32),
+          (130, 200, 264, 7, 8), (700, 136, 520, 300, 16), (2042, 72, 392, 4, 128), (4099, 136, 1096, 11, 40),
+          (16379, 72, 1032, 3, 64)]
+
+
+def make_ids(dev, T, n, how):
+    g = torch.Generator().manual_seed(T + n)
+    if how == "mixed":
+        ids = torch.randint(-1, n, (T,), generator=g)
+    elif how == "runs":
+        ids = torch.sort(torch.randint(0, n, (T,), generator=g)).values
+        ids[T // 2: T // 2 + 3] = -1
+    elif how == "none":
+        ids = torch.full((T,), -1)
+    else:  # ids that are no adapter's
+        ids = torch.randint(0, n, (T,), generator=g)
+        ids[::3] = n
+        ids[1::3] = -7
+    return ids.to(dev)
+
+
+@pytest.mark.parametrize("how", ["mixed", "runs", "none", "outside"])
+@pytest.mark.parametrize("T,K,N,n,r", LINEAR)
+def test_linear(dev, T, K, N, n, r, how):
+    x, w, ad = rnd(dev, T, K), rnd(dev, N, K, std=K ** -0.5), make_ad(dev, n, r, K, N)
+    ids = make_ids(dev, T, n, how)
+    y = kmoe.adapted_linear(x, w, ad, ids)
+    B.check("y", y, B.adapted(B.V(x), B.V(w), ad, ids))
+    assert torch.equal(kmoe.adapted_linear(x, w, ad, ids.to(torch.int32)), y)
+    if how == "none":
+        assert torch.equal(kmoe.adapted_linear(x, w), y)
+
+
+@pytest.mark.parametrize("how", ["mixed", "runs", "none", "outside"])
+@pytest.mark.parametrize("T,K,N,n,r", LINEAR)
+def test_linear_backward(dev, T, K, N, n, r, how):
+    x, w, ad = rnd(dev, T, K), rnd(dev, N, K, std=K ** -0.5), make_ad(dev, n, r, K, N)
+    ids, dy = make_ids(dev, T, n, how), rnd(dev, T, N)
+    lx, lw, la, lb = (t.clone().requires_grad_(True) for t in (x, w, ad.a, ad.b))
+    y = kmoe.adapted_linear(lx, lw, kmoe.Adapters(la, lb, ad.scale), ids)
+    dx, dw, da, db = torch.autograd.grad(y, (lx, lw, la, lb), dy)
+    B.check("y", y.detach(), B.adapted(B.V(x), B.V(w), ad, ids))
+    # dx is the adapted projection of dy by the transposed factors
+    back = kmoe.Adapters(ad.b.transpose(1, 2), ad.a.transpose(1, 2), ad.scale)
+    B.check("dx", dx, B.adapted(B.V(dy), B.V(w.t()), back, ids))
+    B.check("dw", dw, B.mm(B.V(dy).t(), B.V(x)))
+    for i in range(n) if n < 20 else (0, 1, n - 1):
+        t = (ids == i).nonzero().squeeze(1)
+        if t.numel() == 0:
+            assert not bool(da[i].any()) and not bool(db[i].any())
+            continue
+        s = float(ad.scale[i])
+        u = (B.mm(B.V(dy[t]), B.V(ad.b[i])) * s).bf16()
+        v = (B.mm(B.V(x[t]), B.V(ad.a[i]).t()) * s).bf16()
+        B.check(("da", i), da[i], B.mm(u.t(), B.V(x[t])))
+        B.check(("db", i), db[i], B.mm(B.V(dy[t]).t(), v))
+
+
+@pytest.mark.parametrize("T", [3, 50, 300])
+@pytest.mark.parametrize("which", [(1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1), (1, 1, 0), (0, 1, 1)])
+def test_ffn_adapters(dev, T, which):
+    d, F, n = 136, 200, 5
+    x, wg, wu, wd = make_ffn(dev, T, d, F)
+    ads = [make_ad(dev, n, r, *kn) if k else None for k, kn, r in zip(which, ((d, F), (d, F), (F, d)), (16, 16, 24))]
+    ids = make_ids(dev, T, n, "mixed")
+    with torch.no_grad():
+        y = kmoe.gated_ffn(x, wg, wu, wd, "silu", kmoe.FFNAdapters(*ads), ids)
+    B.check("y", y, B.ffn(x, wg, wu, wd, "silu", ads, ids)[0])
+    # the composed pass that trains is the same function
+    lead = [t.clone().requires_grad_(True) for t in (x, *(a.a for a in ads if a))]
+    it = iter(lead[1:])
+    z = kmoe.gated_ffn(lead[0], wg, wu, wd, "silu", kmoe.FFNAdapters(*(a and a._replace(a=next(it)) for a in ads)), ids)
+    # (it rounds the pre-activations to bf16, half a step of each, on top)
+    g, u = (B.adapted(B.V(x), B.V(w), a, ids).bf16() for w, a in ((wg, ads[0]), (wu, ads[1])))
+    a_, _ = B.act("silu", g)
+    B.check("z", z.detach(), B.adapted((a_ * u).bf16(), B.V(wd), ads[2], ids).bf16())
+    grads = torch.autograd.grad(z.float().square().sum(), lead)
+    assert all(bool(torch.isfinite(t).all()) and float(t.float().abs().max()) > 0 for t in grads)
+
+
+@pytest.mark.parametrize("T", [40, 300])
+def test_adapters_stay_apart(dev, T):
+    """An adapter of NaN reaches the rows that have it, and no others: forward and backward."""
+    K, N, n, r = 72, 136, 4, 16
+    x, w, ad = rnd(dev, T, K), rnd(dev, N, K, std=0.1), make_ad(dev, n, r, K, N)
+    ids, dy = make_ids(dev, T, n, "mixed"), rnd(dev, T, N)
+    bad = kmoe.Adapters(ad.a.clone(), ad.b.clone(), ad.scale)
+    bad.a[2], bad.b[2, 5] = float("nan"), float("inf")
+    xb = x.clone()
+    xb[(ids == 2).nonzero()[0, 0]] = float("nan")
+
+    def run(x, ad):
+        lx, la, lb = (t.clone().requires_grad_(True) for t in (x, ad.a, ad.b))
+        y = kmoe.adapted_linear(lx, w, kmoe.Adapters(la, lb, ad.scale), ids)
+        return (y.detach(), *torch.autograd.grad(y, (lx, la, lb), dy), kmoe.adapted_linear(x, w, ad, ids))
+    good, got = run(x, ad), run(xb, bad)
+    rows, others = ids != 2, torch.tensor([0, 1, 3], device=dev)
+    for k in (0, 1, 4):
+        assert torch.equal(got[k][rows], good[k][rows]) and bool(got[k][~rows].isnan().any())
+    for k in (2, 3):
+        assert torch.equal(got[k][others], good[k][others])
+
+
+def test_rank_is_filled_up(dev):
+    """A rank that is not a multiple of 8, with its gradients."""
+    T, K, N, n, r = 70, 72, 136, 3, 5
+    x, w, ad = rnd(dev, T, K), rnd(dev, N, K, std=0.1), make_ad(dev, n, r, K, N, scale=False)
+    ids, dy = make_ids(dev, T, n, "mixed"), rnd(dev, T, N)
+    la, lb = (t.clone().requires_grad_(True) for t in (ad.a, ad.b))
+    y = kmoe.adapted_linear(x, w, kmoe.Adapters(la, lb), ids)
+    B.check("y", y.detach(), B.adapted(B.V(x), B.V(w), ad, ids))
+    da, db = torch.autograd.grad(y, (la, lb), dy)
+    assert da.shape == ad.a.shape and db.shape == ad.b.shape
+    for i in range(n):
+        t = ids == i
+        u = B.mm(B.V(dy[t]), B.V(ad.b[i])).bf16()
+        B.check("da", da[i], B.mm(u.t(), B.V(x[t])))
+
+
+def test_ids_past_32_bits(dev):
+    x, w, ad = rnd(dev, 4, 64), rnd(dev, 72, 64), make_ad(dev, 2, 8, 64, 72)
+    ids = torch.tensor([1 << 32, -(1 << 40), (1 << 32) + 1, 0], device=dev)
+    y = kmoe.adapted_linear(x, w, ad, ids)
+    plain = kmoe.adapted_linear(x, w)
+    assert torch.equal(y[:3], plain[:3]) and not torch.equal(y[3], plain[3])
+
+
+# ---------------------------------------------------------------- graphs, streams, use together
+def test_captured_block(dev):
+    """Replays of a captured forward, with eager calls between them, and of a training step."""
+    x, wg, wu, wd = make_ffn(dev, 40, 64, 136)
+    ads = kmoe.FFNAdapters(make_ad(dev, 3, 8, 64, 136), None, make_ad(dev, 3, 8, 136, 64))
+    ids = make_ids(dev, 40, 3, "mixed").to(torch.int32)
+    with torch.no_grad():
+        kmoe.gated_ffn(x, wg, wu, wd, "silu", ads, ids)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            y = kmoe.gated_ffn(x, wg, wu, wd, "silu", ads, ids)
+        for k in range(4):
+            x.copy_(rnd(dev, 40, 64))
+            ids.copy_(ids.roll(1))
+            wg.mul_(-1.0)
+            eager = kmoe.gated_ffn(x, wg, wu, wd, "silu", ads, ids)
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(y, eager)
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    dy = rnd(dev, 40, 64)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(kmoe.gated_ffn(*leaves), leaves, dy)
+    for k in range(3):
+        with torch.no_grad():
+            leaves[0].copy_(rnd(dev, 40, 64))
+            leaves[3].mul_(0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        other = [t.detach().clone().requires_grad_(True) for t in leaves]
+        want = torch.autograd.grad(kmoe.gated_ffn(*other), other, dy)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_capture_beside_a_live_graph_is_refused(dev):
+    leaves = [t.requires_grad_(True) for t in make_ffn(dev, 8, 64, 72)]
+    live = kmoe.gated_ffn(*leaves)
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            kmoe.gated_ffn(*leaves)
+    del live
+
+
+def test_two_streams(dev):
+    x, wg, wu, wd = make_ffn(dev, 300, 136, 264)
+    ad, ids = make_ad(dev, 4, 16, 136, 264), make_ids(dev, 300, 4, "mixed")
+    y, z = kmoe.gated_ffn(x, wg, wu, wd), kmoe.adapted_linear(x, wg, ad, ids)
+    torch.cuda.synchronize()
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    outs = []
+    for _ in range(5):
+        for s in (a, b):
+            with torch.cuda.stream(s):
+                outs.append((kmoe.gated_ffn(x, wg, wu, wd), kmoe.adapted_linear(x, wg, ad, ids)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(p, y) and torch.equal(q, z) for p, q in outs)
+
+
+def test_a_written_weight_is_noticed(dev):
+    leaves = [t.requires_grad_(True) for t in make_ffn(dev, 8, 64, 72)]
+    y = kmoe.gated_ffn(*leaves)
+    with torch.no_grad():
+        leaves[1].mul_(2.0)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+def _layer(dev, **kw):
+    c = kmoe.AdvancedMoEConfig(d_model=128, d_ff_expert=136, n_experts=4, moe_shared_d_ff=264, mod_enabled=False,
+                               residual_dropout=0.0, **kw)
+    torch.manual_seed(5)
+    return c, kmoe.MoELayer(c).to(dev).to(BF)
+
+
+def test_shared_expert(dev):
+    """The layer with a shared expert is the layer without plus the block, in every kind of pass."""
+    for routing in ("token_choice", "expert_choice"):
+        c, layer = _layer(dev, moe_routing=routing)
+        x = rnd(dev, 2, 40, 128)
+        shared = layer.shared_expert
+        for mode in (True, False):
+            layer.train(mode)
+            with torch.no_grad():
+                y = layer(x)
+                layer._modules["shared_expert"] = None
+                base = layer(x)
+                layer._modules["shared_expert"] = shared
+                assert torch.equal(y, base + shared(x))
+        xg = x.clone().requires_grad_(True)
+        layer.train()(xg).float().square().sum().backward()
+        assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for p in layer.parameters())
+        sd = layer.state_dict()
+        assert {k for k in sd if k.startswith("shared")} == {f"shared_expert.w{i}.weight" for i in (1, 2, 3)}
+
+
+@pytest.mark.parametrize("mod", [False, True])
+def test_shared_expert_in_a_block(dev, mod):
+    c = kmoe.AdvancedMoEConfig(d_model=128, d_ff_expert=136, n_experts=4, moe_shared_d_ff=264, mod_enabled=mod,
+                               residual_dropout=0.0)
+    torch.manual_seed(6)
+    blk = kmoe.MoEFFNBlock(c).to(dev).to(BF).train()
+    x = rnd(dev, 2, 64, 128).requires_grad_(True)
+    out = blk(x)
+    (out.float().square().sum() + blk.aux_loss).backward()
+    assert blk.last_path == "unfused"
+    assert all(p.grad is not None and bool(torch.isfinite(p.grad).all()) for n, p in blk.named_parameters()
+               if "aux_router" not in n)
+    with torch.no_grad():
+        blk.eval()
+        y = blk(x)
+        want = x + (lambda n: blk.ffn(n))(blk.ffn_norm(x))
+        assert torch.equal(y, want)
+
+
+def test_train_and_serve_together(dev):
+    """A layer with a shared expert trained by AdamW for some steps, then adapters of its block trained
+    over the frozen weights, then served: each step's weights are what the next pass takes."""
+    c, layer = _layer(dev)
+    layer.train()
+    opt = kmoe.AdamW(layer.parameters(), lr=1e-2, state_bits=8, master_weights=True)
+    x = rnd(dev, 2, 40, 128)
+    for step in range(3):
+        opt.zero_grad()
+        y = layer(x)
+        (y.float().square().mean() + layer.aux_loss).backward()
+        before = {n: p.detach().clone() for n, p in layer.named_parameters()}
+        opt.step()
+        assert all(not torch.equal(p, before[n]) for n, p in layer.named_parameters())
+        fresh = kmoe.MoELayer(c).to(dev).to(BF).train()
+        fresh.load_state_dict(layer.state_dict())
+        with torch.no_grad():
+            assert torch.equal(layer(x), fresh(x))  # no packed copy of an old weight is left
+    layer.eval().requires_grad_(False)
+    ffn = layer.shared_expert
+    n, r = 3, 8
+    ps = [torch.nn.Parameter(rnd(dev, n, r, 128, std=0.1)), torch.nn.Parameter(torch.zeros(n, 264, r, device=dev, dtype=BF)),
+          torch.nn.Parameter(rnd(dev, n, r, 264, std=0.1)), torch.nn.Parameter(torch.zeros(n, 128, r, device=dev, dtype=BF))]
+    ads = kmoe.FFNAdapters(kmoe.Adapters(ps[0], ps[1]), None, kmoe.Adapters(ps[2], ps[3]))
+    ids = make_ids(dev, 80, n, "mixed").view(2, 40)
+    with torch.no_grad():
+        assert torch.equal(ffn(x, ads, ids), ffn(x))  # outer factors of zero
+    opt = kmoe.AdamW(ps, lr=1e-2)
+    for step in range(2):
+        opt.zero_grad()
+        ffn(x, ads, ids).float().square().mean().backward()
+        opt.step()
+    with torch.no_grad():
+        y = ffn(x, ads, ids)
+        plain = ffn(x)
+        assert torch.equal(y[ids < 0], plain[ids < 0]) and not torch.equal(y[ids >= 0], plain[ids >= 0])
+        ws = [w.weight for w in (ffn.w1, ffn.w2, ffn.w3)]
+        B.check("served", y.view(80, 128), B.ffn(x.view(80, 128), *ws, "silu", ads, ids.view(-1))[0])
+
+
+def test_f32_module_follows_its_weights(dev):
+    """Casts of f32 weights are kept between calls, until a weight changes."""
+    ffn = kmoe.GatedFFN(64, 72).to(dev).requires_grad_(False)
+    x = rnd(dev, 9, 64)
+    y = ffn(x)
+    assert ffn._bf16_cache is not None and torch.equal(ffn(x), y)
+    ffn.w2.weight.mul_(2.0)
+    z = ffn(x)
+    assert torch.equal(z, kmoe.gated_ffn(x, ffn.w1.weight, ffn.w2.weight, ffn.w3.weight)) and not torch.equal(z, y)
+    ffn.w1.weight.data.mul_(2.0)
+    kmoe.weights_changed(ffn)
+    assert not torch.equal(ffn(x), z)
