@@ -676,7 +676,8 @@ int kmoe_adamw_values(const void* m_codes, const float* m_scale, const void* v_c
 /* ------------------------------------------------------------------------ */
 /* Dense products beside the routed experts, on weights as torch.nn.Linear holds them (rows of
  * the output, K-contiguous), bf16, f32 sums.  Sizes other than the rows' are multiples of 8, the
- * rows any number below 2^31, buffers contiguous and aligned to 16 bytes.
+ * rows any number below 2^31, rows of fewer than 2^22 values, buffers contiguous and aligned to
+ * 16 bytes.
  *
  * Adapters: row t of a projection x w^T gets scale[i] (x a[i]^T) b[i]^T on top, i = ids[t]
  * (device int32; outside [0, n_adapters): no adapter); a (n, rank, K), b (n, N, rank) bf16, scale (n)
@@ -705,16 +706,18 @@ int kmoe_adapted_linear(const void* x, int64_t T, int K, const void* w, int N, c
  * with a2, of one rank); rows without an adapter are left.                          */
 int kmoe_adapter_inner(const void* x, int64_t T, int K, const int32_t* ids, int n, int rank, const void* a,
                        const float* scale, void* v, const void* a2, const float* scale2, void* v2, void* stream);
-/* h (T, F) = act(x w_gate^T) * (x w_up^T); with p and q (T, F) also what the backward needs, up
- * act'(gate) and act(gate), bf16 (then no adapters).  ids NULL: no adapters.        */
+/* h (T, F) = act(x w_gate^T) * (x w_up^T); with `saved` also what the backward needs, up act'(gate)
+ * and act(gate) in 24 bits, in an order of its own, kmoe_dense_saved_bytes(T, F) bytes (then no
+ * adapters).  ids NULL: no adapters.                                                */
+size_t kmoe_dense_saved_bytes(int64_t T, int F);
 int kmoe_dense_gate_up(const void* x, int64_t T, int d, const void* w_gate, const void* w_up, int F, int act,
                        const int32_t* ids, int n_adapters, int rank, const void* v_gate, const void* b_gate,
-                       const void* v_up, const void* b_up, void* h, void* p, void* q, void* stream);
+                       const void* v_up, const void* b_up, void* h, void* saved, void* stream);
 int kmoe_dense_linear(const void* x, int64_t T, int K, const void* w, int N, const int32_t* ids, int n_adapters,
                       int rank, const void* v, const void* b, void* y, void* stream);
-/* dgate, dup (T, F) = (dy w_down) p, (dy w_down) q.                                 */
-int kmoe_dense_dh(const void* dy, int64_t T, int d, const void* w_down, int F, const void* p, const void* q,
-                  void* dgate, void* dup, void* stream);
+/* dgate, dup (T, F): dy w_down times the first and the second of the saved values.   */
+int kmoe_dense_dh(const void* dy, int64_t T, int d, const void* w_down, int F, const void* saved, void* dgate,
+                  void* dup, void* stream);
 /* dx (T, K) = dy w (+ dy2 w2), w (N, K); with adapters (of one product) + u at[i]^T, u (T, rank) the
  * scaled inner products of dy with the transposed b, at (n, K, rank) the transposed a. */
 int kmoe_dense_dx(const void* dy, const void* dy2, int64_t T, int N, const void* w, const void* w2, int K,

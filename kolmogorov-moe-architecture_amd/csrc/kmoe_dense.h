@@ -7,22 +7,28 @@
 // the forward) or K-strided (its rows run along K: a Linear weight in the backward, the rows of
 // both operands of a weight gradient).
 //
-// A workgroup of 8 waves owns a BM x BN tile; waves form 2 (rows) x 4 (columns).  The tile is
-// split into halves along both sides and a wave holds the same place of each of the four
-// quadrants, so that the two column halves may come from two matrices: the gate and up rows of
-// the same f, whose values then meet in one lane.  K advances 64 per step; a step's 16-byte
-// pieces go from memory to LDS without passing registers, each lane picking the piece that belongs
-// where the hardware puts it, so the swizzle costs nothing.  NST stages, loads NST - 1 steps ahead,
-// one barrier a step.
-//   K-contiguous tiles: rows of 128 bytes, 16-byte chunks XOR-ed by (row / 2) % 8; a fragment is
-//   one ds_read_b128.
-//   K-strided tiles: 64 rows of the tile's columns, 32-byte slots XOR-ed by bits 0, 1 and 3 of the
+// A workgroup of four waves, one on a SIMD, owns a BM x BN tile.  The tile is split into halves along
+// both sides and a wave of the 2 x 2 holds the same place of each of the four quadrants, so that
+// the two column halves may come from two matrices: the gate and up rows of the same f, whose
+// values then meet in one lane.  Four waves and not more: LDS moves 128 bytes a cycle, every fragment
+// has to feed as many MFMAs as a wave can hold (256 x 256 with eight waves of 128 x 64: reads and
+// loads took longer than the MFMAs, 16384 rows, d 2048, F 5632, down 352 us; the MFMAs alone 189).
+// K advances 32 or 64 (32 KS) per step.  A step's 16-byte pieces go from memory to LDS without passing registers,
+// each lane picking the piece that belongs where the hardware puts it, so the swizzle costs nothing:
+//   K-contiguous tiles: rows of 64 KS bytes, 16-byte chunks XOR-ed by (row / 2) modulo their number;
+//   a fragment is one ds_read_b128.
+//   K-strided tiles: 32 KS rows of the tile's columns, 32-byte slots XOR-ed by bits 0, 1 and 3 of the
 //   row; a fragment is two ds_read_b64_tr_b16 (in each 16-lane group, lane i receives element
 //   i % 4 of the 8-byte chunks addressed by lanes 4 p + i / 4), whose 16 rows spread over all
 //   banks twice, the least for 512 bytes.
-// The MFMAs take the B fragment first, so a lane holds four consecutive columns of one row.
-// Rows and columns past the end read the last row's or zeros and are not stored; K past the end
-// reads zeros in both operands (a NaN next to a row's end must not meet a zero).
+// The MFMAs of 32 of K (16x16x32, the B fragment first: a lane holds four consecutive columns of a
+// row) are issued in program order, with the reads of the next 32's fragments, into another set of
+// registers, between them, and in a step's last 32 the loads of the step STAGES on.  These go
+// into the step's own stage: every wave has all of its fragments, as it passed the barrier before
+// its last 32, the step's only one.  A load has STAGES - 1 steps to land.  Past the last step zeros
+// are loaded, so that the counts of loads in flight stay the same.
+// Rows and columns past the end repeat others and are not stored; K past the end reads zeros in
+// both operands (a NaN next to a row's end must not meet a zero).
 #pragma once
 
 #include <type_traits>
@@ -31,12 +37,7 @@
 
 namespace kmoe_dense {
 
-constexpr int THREADS = 512;
-constexpr int BK = 64;      // K per step
-constexpr int KROWB = 128;  // bytes of a K-contiguous tile row
-
-// 16 zero bytes that lanes without data load
-__device__ __attribute__((aligned(16))) const uint32_t kZeros[4] = {0, 0, 0, 0};
+constexpr int THREADS = 256;
 
 // Low-rank adapters on top of a product: row m gets v[m] . b[ids[m]]^T, v (M, r) bf16 with the scale
 // in it, b (n, N, r); an id outside [0, n) is no adapter.  GATED: [1] are the up half's.
@@ -48,10 +49,9 @@ struct Adapt {
 };
 
 struct Args {
-  // the product's parts along K: A and B of each (GATED: one part, b[0] and b[1] the two halves)
+  // A and B, and of a product in two parts along K the second ones (GATED: b[0] and b[1] are the halves)
   const uint16_t* a[2];
   const uint16_t* b[2];
-  int parts;
   int K;              // of each part, a multiple of 8
   int64_t lda, ldb;   // elements
   int64_t M;
@@ -60,47 +60,60 @@ struct Args {
   void* c;            // bf16, or f32 with c_f32
   int c_f32;
   int act;            // GATED
-  uint16_t* p;        // GATED: up act'(gate), and q: act(gate), for the backward (nullable); DH: the same, read
-  uint16_t* q;
+  uint8_t* saved;     // GATED: up act'(gate) and act(gate) for the backward (nullable); DH: the same, read
   uint16_t* c2;       // DH: the up half's gradient
   Adapt ad;
 };
 
-enum { EPI_PLAIN = 0, EPI_GATED = 1, EPI_DH = 2 };
+// EPI_TWO: as EPI_PLAIN, of a product in two parts along K
+enum { EPI_PLAIN = 0, EPI_GATED = 1, EPI_DH = 2, EPI_TWO = 3 };
+
+template <int I0, int N, class Fn>
+__device__ __forceinline__ void static_for(Fn&& f) {
+  if constexpr (I0 < N) {
+    f(std::integral_constant<int, I0>{});
+    static_for<I0 + 1, N>(f);
+  }
+}
 
 typedef short tr4_t __attribute__((ext_vector_type(4)));
 
+// What the 32-byte slots of a K-strided tile's row r are XOR-ed by.
 template <int ROWB>
 __device__ __forceinline__ int strided_swz(int r) {
   return ROWB >= 256 ? ((r & 3) | (((r >> 3) & 1) << 2)) : (((r >> 1) & 1) | (((r >> 3) & 1) << 1));
 }
 
 // Activation and its derivative at g.
-__device__ __forceinline__ void act_f32(int act, float g, float& a, float& da) {
+template <int ACT>
+__device__ __forceinline__ void act_at(float g, float& a, float& da) {
+  if constexpr (ACT == KMOE_ACT_SILU) {
+    const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));
+    a = g * s;
+    da = s * (1.0f + g * (1.0f - s));
+  } else if constexpr (ACT == KMOE_ACT_GELU) {
+    const float c = 0.5f * (1.0f + erff(g * 0.70710678f));
+    a = g * c;
+    da = c + g * __expf(-0.5f * g * g) * 0.39894228f;
+  } else if constexpr (ACT == KMOE_ACT_GELU_TANH) {
+    const float g2 = g * g, in = 0.79788456f * g * (1.0f + 0.044715f * g2);
+    // tanh(z) = 1 - 2 / (1 + e^(2z)): 1 and -1 at its ends
+    const float t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __expf(2.0f * in));
+    a = 0.5f * g * (1.0f + t);
+    da = 0.5f * (1.0f + t) + 0.5f * g * (1.0f - t * t) * 0.79788456f * (1.0f + 0.134145f * g2);
+  } else {
+    a = g > 0.0f ? g : 0.0f;
+    da = g > 0.0f ? 1.0f : 0.0f;
+  }
+}
+// f(tag of the activation): the choice is made once, not at every value.
+template <class Fn>
+__device__ __forceinline__ void with_act(int act, Fn&& f) {
   switch (act) {
-    case KMOE_ACT_SILU: {
-      const float s = __builtin_amdgcn_rcpf(1.0f + __expf(-g));
-      a = g * s;
-      da = s * (1.0f + g * (1.0f - s));
-      break;
-    }
-    case KMOE_ACT_GELU: {
-      const float c = 0.5f * (1.0f + erff(g * 0.70710678f));
-      a = g * c;
-      da = c + g * __expf(-0.5f * g * g) * 0.39894228f;
-      break;
-    }
-    case KMOE_ACT_GELU_TANH: {
-      const float g2 = g * g, in = 0.79788456f * g * (1.0f + 0.044715f * g2);
-      // tanh(z) = 1 - 2 / (1 + e^(2z)): 1 and -1 at its ends
-      const float t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __expf(2.0f * in));
-      a = 0.5f * g * (1.0f + t);
-      da = 0.5f * (1.0f + t) + 0.5f * g * (1.0f - t * t) * 0.79788456f * (1.0f + 0.134145f * g2);
-      break;
-    }
-    default:
-      a = g > 0.0f ? g : 0.0f;
-      da = g > 0.0f ? 1.0f : 0.0f;
+    case KMOE_ACT_SILU: f(std::integral_constant<int, KMOE_ACT_SILU>{}); break;
+    case KMOE_ACT_GELU: f(std::integral_constant<int, KMOE_ACT_GELU>{}); break;
+    case KMOE_ACT_GELU_TANH: f(std::integral_constant<int, KMOE_ACT_GELU_TANH>{}); break;
+    default: f(std::integral_constant<int, KMOE_ACT_RELU>{});
   }
 }
 
@@ -109,9 +122,31 @@ __device__ __forceinline__ i32x2_t pack4(float a, float b, float c, float d) {
   const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{c, d}, bf16x2_t));
   return i32x2_t{(int)lo, (int)hi};
 }
-__device__ __forceinline__ void unpack4(i32x2_t v, float* o) {
-  o[0] = __uint_as_float((uint32_t)v[0] << 16), o[1] = __uint_as_float((uint32_t)v[0] & 0xffff0000u);
-  o[2] = __uint_as_float((uint32_t)v[1] << 16), o[3] = __uint_as_float((uint32_t)v[1] & 0xffff0000u);
+// What the backward multiplies by, up act'(gate) and act(gate), is held in 24 bits, the top of its f32:
+// in bf16 its rounding would add to those of the products' operands and results, a third of one
+// size (gradients of the weights and of x: 1.73 roundings off, so 1.41).  It lies as the MFMAs
+// leave it, by 16 x 16 blocks, a lane's four values in 12 bytes: in one access of 768 bytes a wave.
+constexpr int SAVED_BLOCK = 2 * 768;  // bytes of a block: both values
+struct Three {  // (12 bytes: a vector of three would be stored as four)
+  uint32_t a, b, c;
+};
+__device__ __forceinline__ uint8_t* saved_block(uint8_t* p, int N, int64_t m, int n) {
+  return p + ((m >> 4) * ((N + 15) >> 4) + (n >> 4)) * SAVED_BLOCK;
+}
+__device__ __forceinline__ void store24(uint8_t* block, int lane, const float* v) {
+  uint32_t u[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) u[t] = __float_as_uint(v[t]);
+  *reinterpret_cast<Three*>(block + lane * 12) = {(u[0] >> 8) | (u[1] << 16 & 0xff000000u),
+                                                  (u[1] >> 16) | (u[2] << 8 & 0xffff0000u),
+                                                  (u[2] >> 24) | (u[3] & 0xffffff00u)};
+}
+__device__ __forceinline__ void load24(const uint8_t* block, int lane, float* v) {
+  const Three w = *reinterpret_cast<const Three*>(block + lane * 12);
+  v[0] = __uint_as_float(w.a << 8);
+  v[1] = __uint_as_float((w.a >> 24 << 8) | (w.b << 16));
+  v[2] = __uint_as_float((w.b >> 16 << 8) | (w.c << 24));
+  v[3] = __uint_as_float(w.c & 0xffffff00u);
 }
 
 // Workgroup -> tile: ids go round-robin over the 8 XCDs, so each XCD gets a run of consecutive
@@ -125,75 +160,6 @@ __device__ __forceinline__ void tile_of(int id, int n_mt, int n_nt, int& mt, int
   const int g = t / (G * n_nt), r = t - g * G * n_nt, gm = n_mt - g * G < G ? n_mt - g * G : G;
   nt = r / gm;
   mt = g * G + (r - nt * gm);
-}
-
-// Loads of one operand's stage tile (R rows or columns of the product).
-template <int R, bool STRIDED, bool SPLIT>
-struct Loader {
-  static constexpr int BYTES = R * KROWB;      // of a stage tile, either layout
-  static constexpr int NB = BYTES / 1024 / 8;  // 1 KiB pieces of a wave
-  static constexpr int ROWB = STRIDED ? R * 2 : KROWB;
-  static constexpr int BROWS = 1024 / ROWB;    // tile rows of a piece
-  const uint16_t* src[NB];
-  int kpos[NB];   // first K of this lane's chunk (row, for strided tiles)
-  bool in[NB];    // strided: the chunk's columns exist
-
-  // Rows (columns) [r0, r0 + R) of an operand with `rows` of them; SPLIT: the second half of the
-  // tile is the same rows of another matrix.
-  __device__ __forceinline__ void init(const uint16_t* base, const uint16_t* base2, int64_t ld, int64_t r0, int64_t rows,
-                                       int wave, int lane) {
-#pragma unroll
-    for (int q = 0; q < NB; ++q) {
-      const int blk = wave + 8 * q;
-      if constexpr (!STRIDED) {
-        const int row = blk * BROWS + (lane >> 3), chunk = (lane & 7) ^ ((row >> 1) & 7);
-        const bool second = SPLIT && row >= R / 2;
-        int64_t g = r0 + (second ? row - R / 2 : row);
-        g = g < rows ? g : rows - 1;
-        src[q] = (second ? base2 : base) + g * ld + chunk * 8;
-        kpos[q] = chunk * 8;
-        in[q] = true;
-      } else {
-        constexpr int CPR = ROWB / 16;
-        const int row = blk * BROWS + lane / CPR, chunk = (lane % CPR) ^ (strided_swz<ROWB>(row) << 1);
-        in[q] = r0 + chunk * 8 < rows;
-        src[q] = base + (int64_t)row * ld + (in[q] ? r0 + chunk * 8 : 0);
-        kpos[q] = row;
-      }
-    }
-  }
-  // the next part's matrix, from K = 0
-  __device__ __forceinline__ void rebase(int64_t delta) {
-#pragma unroll
-    for (int q = 0; q < NB; ++q) src[q] += delta;
-  }
-  // K-step with `left` of K to go into the stage tile at lds; moves on to the next step
-  __device__ __forceinline__ void load(int left, int64_t step, KMOE_LDS uint8_t* lds, int wave) {
-#pragma unroll
-    for (int q = 0; q < NB; ++q) {
-      const uint16_t* s = src[q];
-      if ((STRIDED && !in[q]) || (left < BK && kpos[q] >= left)) s = reinterpret_cast<const uint16_t*>(kZeros);
-      dma16_to_lds(s, lds + (wave + 8 * q) * 1024);
-      src[q] += step;
-    }
-  }
-};
-
-// Fragment of 16 rows (columns) at tile row `r`, K-substep i.
-template <int R, bool STRIDED>
-__device__ __forceinline__ bf16x8_t frag(const uint8_t* l, int r, int i, int lane) {
-  if constexpr (!STRIDED) {
-    const int row = r + (lane & 15), chunk = 4 * i + (lane >> 4);
-    return *reinterpret_cast<const bf16x8_t*>(l + row * KROWB + ((chunk ^ ((row >> 1) & 7)) << 4));
-  } else {
-    constexpr int ROWB = R * 2;
-    const int i16 = lane & 15, row = 32 * i + 8 * (lane >> 4) + (i16 >> 2), col = r + 4 * (i16 & 3);
-    const uint8_t* p = l + row * ROWB + (((col >> 3) ^ (strided_swz<ROWB>(row) << 1)) << 4) + (col & 4) * 2;
-    const tr4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((KMOE_LDS tr4_t*)p);
-    const tr4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((KMOE_LDS tr4_t*)(p + 4 * ROWB));
-    return __builtin_bit_cast(bf16x8_t, (short __attribute__((ext_vector_type(8)))){lo[0], lo[1], lo[2], lo[3], hi[0], hi[1],
-                                                                                   hi[2], hi[3]});
-  }
 }
 
 // Distinct adapters of the tile's rows: list[0 .. *count), in no order (a row has one adapter, so the
@@ -217,44 +183,303 @@ __device__ __forceinline__ void list_adapters(const Adapt& ad, int64_t m0, int64
   __syncthreads();
 }
 
-template <int BM, int BN, bool SA, bool SB, int EPI, int NST, bool ADAPT = false>
-__global__ __launch_bounds__(THREADS, 2) void dense_kernel(Args g, int n_mt, int n_nt) {
+// Adapters and epilogue of a tile: acc[x][y][i][j][t] is row m0 + x BM / 2 + wm BM / 4 + 16 i + l % 16, column
+// n0 + y BN / 2 + wn BN / 4 + 16 j + 4 (l / 16) + t.
+template <int BM, int BN, int EPI, bool ADAPT>
+__device__ __forceinline__ void finish(const Args& g, f32x4_t (&acc)[2][2][BM / 64][BN / 64], int64_t m0, int n0, int wm,
+                                       int wn, int lane, const int* sid, const int* list, int n_list) {
+  constexpr bool GATED = EPI == EPI_GATED;
+  constexpr int QA = BM / 64, QB = BN / 64, WC = BN / 4;
+  const int l16 = lane & 15, lq = lane >> 4;
+  if constexpr (ADAPT) {
+    // Each adapter of the tile: its product with the rows that have it, 32 ranks at a time.  Where all
+    // 16 rows of a block have it, the sums go on; in a block of several it is computed for all and
+    // added, by selection, to the rows that have it: a sum over masked operands would carry a NaN or
+    // an infinity of one request's adapter into the others' rows.
+#pragma unroll 1
+    for (int a = 0; a < n_list; ++a) {
+      const int id = __builtin_amdgcn_readfirstlane(list[a]);
+      uint32_t some = 0, all = 0;  // blocks x QA + i with a row of it, with no other
+#pragma unroll
+      for (int b = 0; b < 2 * QA; ++b) {
+        const uint64_t mine = __ballot(sid[(b / QA) * (BM / 2) + wm * (BM / 4) + (b % QA) * 16 + l16] == id);
+        some |= (mine != 0) << b, all |= (mine == ~0ull) << b;
+      }
+      some = __builtin_amdgcn_readfirstlane(some), all = __builtin_amdgcn_readfirstlane(all);
+      if (!some) continue;
+#pragma unroll 1
+      for (int s = 0; s < g.ad.r; s += 32) {
+        const int k = s + 8 * lq;
+        const bool in = k < g.ad.r;
+        static_for<0, 2>([&](auto yt) {
+          constexpr int y = decltype(yt)::value, h = GATED ? y : 0;
+          const uint16_t *b = g.ad.b[h], *v = g.ad.v[h];
+          if (!b) return;
+          bf16x8_t fb[QB];
+#pragma unroll
+          for (int j = 0; j < QB; ++j) {
+            const int n = n0 + (GATED ? 0 : y * (BN / 2)) + wn * WC + j * 16 + l16;
+            fb[j] = bf16x8_t{};
+            if (in && n < g.N) fb[j] = *reinterpret_cast<const bf16x8_t*>(b + ((int64_t)id * g.N + n) * g.ad.r + k);
+          }
+          static_for<0, 2 * QA>([&](auto xt) {
+            constexpr int blk = decltype(xt)::value, x = blk / QA, i = blk % QA;
+            const int tr = x * (BM / 2) + wm * (BM / 4) + i * 16 + l16;
+            const bool mine = sid[tr] == id;
+            bf16x8_t fv = {};
+            if (in && mine) fv = *reinterpret_cast<const bf16x8_t*>(v + (m0 + tr) * g.ad.r + k);
+            // (after each branch the sums are back in their accumulation registers, block by block)
+            if (all >> blk & 1) {
+#pragma unroll
+              for (int j = 0; j < QB; ++j)
+                acc[x][y][i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fv, acc[x][y][i][j], 0, 0, 0);
+            }
+#pragma unroll
+            for (int j = 0; j < QB; ++j) asm volatile("" : "+a"(acc[x][y][i][j]));
+            if ((some & ~all) >> blk & 1) {
+#pragma unroll
+              for (int j = 0; j < QB; ++j) {
+                const f32x4_t d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fv, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+                for (int t = 0; t < 4; ++t) acc[x][y][i][j][t] += mine ? d[t] : 0.0f;
+              }
+            }
+#pragma unroll
+            for (int j = 0; j < QB; ++j) asm volatile("" : "+a"(acc[x][y][i][j]));
+          });
+        });
+      }
+    }
+  }
+  auto rows = [&](auto&& f) {  // f(x, i, m) for this lane's rows
+#pragma unroll
+    for (int x = 0; x < 2; ++x)
+#pragma unroll
+      for (int i = 0; i < QA; ++i) {
+        const int64_t m = m0 + x * (BM / 2) + wm * (BM / 4) + i * 16;
+        if (m < g.M) f(x, i, m + l16);
+      }
+  };
+  if constexpr (GATED) {
+    with_act(g.act, [&](auto tag) {
+      rows([&](int x, int i, int64_t m) {
+#pragma unroll
+        for (int j = 0; j < QB; ++j) {
+          const int n16 = n0 + wn * WC + j * 16, n = n16 + 4 * lq;
+          if (n16 >= g.N) continue;
+          float h[4], p[4], q[4];
+#pragma unroll
+          for (int t = 0; t < 4; ++t) {
+            float a, da;
+            const float up = acc[x][1][i][j][t];
+            act_at<decltype(tag)::value>(acc[x][0][i][j][t], a, da);
+            h[t] = a * up, p[t] = da * up, q[t] = a;
+          }
+          if (m < g.M && n < g.N)
+            *reinterpret_cast<i32x2_t*>(static_cast<uint16_t*>(g.c) + m * g.ldc + n) = pack4(h[0], h[1], h[2], h[3]);
+          if (g.saved) {  // (whole blocks: the buffer has them)
+            uint8_t* const block = saved_block(g.saved, g.N, m, n16);
+            store24(block, lane, p);
+            store24(block + SAVED_BLOCK / 2, lane, q);
+          }
+        }
+      });
+    });
+  } else {
+    rows([&](int x, int i, int64_t m) {
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int j = 0; j < QB; ++j) {
+          const int n16 = n0 + y * (BN / 2) + wn * WC + j * 16, n = n16 + 4 * lq;
+          if (n16 >= g.N) continue;
+          const f32x4_t v = acc[x][y][i][j];
+          const int64_t at = m * g.ldc + n;
+          if constexpr (EPI == EPI_DH) {
+            float p[4], q[4];
+            const uint8_t* const block = saved_block(g.saved, g.N, m, n16);
+            load24(block, lane, p);
+            load24(block + SAVED_BLOCK / 2, lane, q);
+            if (m < g.M && n < g.N) {
+              *reinterpret_cast<i32x2_t*>(static_cast<uint16_t*>(g.c) + at) =
+                  pack4(v[0] * p[0], v[1] * p[1], v[2] * p[2], v[3] * p[3]);
+              *reinterpret_cast<i32x2_t*>(g.c2 + at) = pack4(v[0] * q[0], v[1] * q[1], v[2] * q[2], v[3] * q[3]);
+            }
+          } else if (m < g.M && n < g.N) {
+            if (g.c_f32)
+              *reinterpret_cast<f32x4_t*>(static_cast<float*>(g.c) + at) = v;
+            else
+              *reinterpret_cast<i32x2_t*>(static_cast<uint16_t*>(g.c) + at) = pack4(v[0], v[1], v[2], v[3]);
+          }
+        }
+    });
+  }
+}
+
+// ---------------------------------------------------------------- the tile kernel
+template <int R, bool STRIDED, int KS>
+struct Loads {  // of one operand's stage tile (R rows or columns, 32 KS of K): this lane's pieces
+  static constexpr int BYTES = R * 64 * KS;  // of the stage tile, either layout
+  static constexpr int N = BYTES / 4096;     // 1 KiB pieces of a wave
+  static constexpr int CPR = STRIDED ? R / 8 : 4 * KS;  // 16-byte chunks of a row
+  uint32_t off[N];  // bytes from the first row (column) of the tile, or for split of its half
+  int kpos;         // first K of the first piece's chunk
+
+  // rows: how many of the tile's R exist, at least one (what is past them repeats others: it is not
+  // stored); split: its halves are the same R / 2 rows of two matrices
+  __device__ __forceinline__ void init(int64_t ld, int64_t rows, bool split, int wave, int lane) {
+#pragma unroll
+    for (int q = 0; q < N; ++q) {
+      const int row = (wave + 4 * q) * (64 / CPR) + lane / CPR;
+      if constexpr (!STRIDED) {
+        // (rows of a lane's pieces are multiples of 32 apart: the same chunk of K)
+        const int chunk = (lane % CPR) ^ ((row >> 1) & (CPR - 1));
+        const int64_t want = split ? row & (R / 2 - 1) : row, r = want < rows ? want : rows - 1;
+        off[q] = (uint32_t)(r * ld * 2) + chunk * 16;
+        if (q == 0) kpos = chunk * 8;
+      } else {
+        const int chunk = (lane % CPR) ^ (strided_swz<2 * R>(row) << 1);
+        off[q] = (uint32_t)(row * ld * 2) + (chunk * 8 < rows ? chunk * 16 : 0);
+        if (q == 0) kpos = row;
+      }
+    }
+  }
+  // with `left` of K to go, what is past its end gets an offset that reads as zero: a bit that the
+  // others do not have
+  __device__ __forceinline__ void cut(int left) {
+#pragma unroll
+    for (int q = 0; q < N; ++q)
+      if (kpos + (STRIDED ? 4 * q * (64 / CPR) : 0) >= left) off[q] |= 0x80000000u;
+  }
+  __device__ __forceinline__ void uncut() {
+#pragma unroll
+    for (int q = 0; q < N; ++q) off[q] &= 0x7fffffffu;
+  }
+};
+
+// Direct global -> LDS load of 16 bytes a lane (see dma16_to_lds) at a uniform address plus a 32-bit
+// offset, in two parts with an MFMA between them: M0, the LDS address, needs a cycle before its
+// use, and the wave's SIMD issues nothing else meanwhile.  Nothing else in the loop writes M0.
+// A buffer load, whose window of 2 GiB turns larger offsets into zeros without an access.
+__device__ __forceinline__ void dma16_where(KMOE_LDS void* lds) {
+  const uint32_t la = (uint32_t)(uintptr_t)lds;
+  asm volatile("s_mov_b32 m0, %0" ::"s"(__builtin_amdgcn_readfirstlane(la)) : "m0");
+}
+__device__ __forceinline__ void dma16_at(const void* base, uint32_t off) {
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  const i32x4_t window = {(int)(uint32_t)b, (int)(uint32_t)(b >> 32), 0x7fffffff, 0x00020000};
+  asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(window));
+}
+
+// Where a lane reads a wave's fragments of an R-row stage tile: the wave's 16-row blocks are
+// r = half R / 2 + w R / 4 + 16 i, Q = R / 64 of them in a half.
+template <int R, bool STRIDED, int KS>
+struct Frags {
+  static constexpr int Q = R / 64;
+  // K-contiguous: the swizzle repeats every 16 rows, a block only adds to the address.  Strided: a
+  // block's number is XOR-ed into bits from 5 on, which in a 512-byte row is for the halves an addition.
+  static constexpr int PLACES = !STRIDED ? 1 : R == 256 ? Q : 2 * Q;
+  uint32_t place[PLACES];
+
+  __device__ __forceinline__ void init(int w, int lane) {
+    if constexpr (!STRIDED) {
+      const int row = w * (R / 4) + (lane & 15);
+      place[0] = row * 64 * KS + (((lane >> 4) ^ ((row >> 1) & (4 * KS - 1))) << 4);
+    } else {
+      const int i16 = lane & 15, row = 8 * (lane >> 4) + (i16 >> 2);
+      const uint32_t first = row * 2 * R + (((w * (R / 64)) ^ strided_swz<2 * R>(row)) << 5) + (i16 & 3) * 8;
+#pragma unroll
+      for (int i = 0; i < PLACES; ++i) {
+        const int block = R == 256 ? i : (i / Q) * (R / 32) + i % Q;
+        place[i] = first ^ (block << 5);
+      }
+    }
+  }
+  // block b (b / Q the half) of K from 32 ks on, of a stage tile.  (One addition for a tile and place: the
+  // rest goes into the instructions' offsets.)
+  __device__ __forceinline__ bf16x8_t read(const KMOE_LDS uint8_t* tile, int b, int ks) const {
+    if constexpr (!STRIDED) {
+      // (the second 32 of K are chunks 4 .. 7: bit 6 of the place, whatever the swizzle makes of it)
+      const KMOE_LDS uint8_t* at = tile + (ks ? place[0] ^ 64u : place[0]);
+      return *(const KMOE_LDS bf16x8_t*)(at + ((b / Q) * (R / 2) + (b % Q) * 16) * 64 * KS);
+    } else {
+      const KMOE_LDS uint8_t* at = tile + (R == 256 ? place[b % Q] : place[b]);
+      const int c = (R == 256 ? (b / Q) * 256 : 0) + ks * 64 * R;
+      const tr4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((KMOE_LDS tr4_t*)(at + c));
+      const tr4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((KMOE_LDS tr4_t*)(at + c + 8 * R));
+      return __builtin_bit_cast(bf16x8_t, (short __attribute__((ext_vector_type(8)))){lo[0], lo[1], lo[2], lo[3], hi[0],
+                                                                                     hi[1], hi[2], hi[3]});
+    }
+  }
+};
+
+// Waves of a SIMD that the tile leaves room for.
+template <int BM, int BN, int KS, int STAGES>
+constexpr int side_by_side = (BM * BN == 256 * 256 || (BM + BN) * 64 * KS * STAGES > 78 * 1024) ? 1 : 2;
+
+template <int BM, int BN, int KS, int STAGES, bool SA, bool SB, int EPI, bool ADAPT>
+__global__ __launch_bounds__(THREADS, (side_by_side<BM, BN, KS, STAGES>)) __attribute__((
+    amdgpu_waves_per_eu(side_by_side<BM, BN, KS, STAGES>, side_by_side<BM, BN, KS, STAGES>))) void dense_kernel(Args g, int n_mt,
+                                                                                                       int n_nt) {
   constexpr bool GATED = EPI == EPI_GATED;
   static_assert(!GATED || !SB, "gate and up rows are K-contiguous");
-  constexpr int QA = BM / 64, QB = BN / 128;  // 16 x 16 blocks of a wave and quadrant
-  using LoadA = Loader<BM, SA, false>;
-  using LoadB = Loader<BN, SB, GATED>;
-  constexpr int STAGE = LoadA::BYTES + LoadB::BYTES;
-  constexpr int NL = LoadA::NB + LoadB::NB;  // loads of a wave and step
-  __shared__ __attribute__((aligned(1024))) uint8_t lds[NST * STAGE];
-
+  static_assert(KS == 1 || KS == 2, "K per step");
+  constexpr int PARTS = EPI == EPI_TWO ? 2 : 1;
+  constexpr int SK = 32 * KS;
+  using LoadA = Loads<BM, SA, KS>;
+  using LoadB = Loads<BN, SB, KS>;
+  constexpr int QA = BM / 64, QB = BN / 64;          // 16 x 16 blocks of a wave in a half
+  constexpr int TILE = LoadA::BYTES, STAGE = TILE + LoadB::BYTES;
+  constexpr int NP = LoadA::N + LoadB::N;            // loads of a wave and step
+  constexpr int NR = 2 * (QA + QB), NM = 4 * QA * QB;  // fragments and MFMAs of a wave and 32 of K
+  __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * STAGE];
+  __shared__ int sid[ADAPT ? BM : 1], list[ADAPT ? BM : 1], n_list;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave >> 2, wn = wave & 3;
+  const int wm = wave >> 1, wn = wave & 1;
   int mt, nt;
   tile_of(blockIdx.x, n_mt, n_nt, mt, nt);
   const int64_t m0 = (int64_t)mt * BM;
   const int n0 = nt * (GATED ? BN / 2 : BN);
+  KMOE_LDS uint8_t* const ldsp = (KMOE_LDS uint8_t*)lds;
 
+  // where the step to load lies, and how much of K is left from it on
+  const int64_t row_a = SA ? 1 : g.lda, row_b = SB ? 1 : g.ldb;
+  const int64_t step_a = SA ? (int64_t)SK * g.lda : SK, step_b = SB ? (int64_t)SK * g.ldb : SK;
   LoadA la;
   LoadB lb;
-  la.init(g.a[0], nullptr, g.lda, m0, g.M, wave, lane);
-  lb.init(g.b[0], g.b[1], g.ldb, n0, g.N, wave, lane);
-  const int per = (g.K + BK - 1) / BK, nk = per * g.parts;
-  const int64_t step_a = SA ? (int64_t)BK * g.lda : BK, step_b = SB ? (int64_t)BK * g.ldb : BK;
-  KMOE_LDS uint8_t* const ldsp = (KMOE_LDS uint8_t*)lds;
-  int issued = 0, pos = 0;  // steps asked for; the next one's place in its part
-  auto issue = [&]() {
-    const int st = issued % NST;
-    la.load(g.K - pos * BK, step_a, ldsp + st * STAGE, wave);
-    lb.load(g.K - pos * BK, step_b, ldsp + st * STAGE + LoadA::BYTES, wave);
-    ++issued;
-    if (++pos == per && !GATED && issued < nk) {
-      pos = 0;
-      la.rebase((g.a[1] - g.a[0]) - per * step_a);
-      lb.rebase((g.b[1] - g.b[0]) - per * step_b);
+  la.init(g.lda, g.M - m0, false, wave, lane);
+  lb.init(g.ldb, g.N - n0, GATED, wave, lane);
+  const uint16_t* pa = g.a[0] + m0 * row_a;
+  const uint16_t* pb = g.b[0] + n0 * row_b;
+  const int64_t second = GATED ? g.b[1] - g.b[0] : 0;  // from the gate's to the up projection's rows
+  int left = g.K, part = 1, to = 0;
+  // piece q of the step to load, A's before B's
+  auto place_piece = [&](int q) {
+    return ldsp + to * STAGE + (q < LoadA::N ? wave + 4 * q : TILE / 1024 + wave + 4 * (q - LoadA::N)) * 1024;
+  };
+  auto load_piece = [&](int q) {
+    const int c = q < LoadA::N ? q : q - LoadA::N;
+    // (the second half of B's pieces are the second half of its rows)
+    if (q < LoadA::N)
+      dma16_at(pa, la.off[c]);
+    else
+      dma16_at(pb + (GATED && c >= LoadB::N / 2 ? second : 0), lb.off[c]);
+  };
+  auto next_step = [&]() {
+    left -= SK, to = to + 1 == STAGES ? 0 : to + 1;
+    pa += step_a, pb += step_b;
+    if (left < SK) {  // the last step of a part and those past it
+      if (PARTS == 2 && left <= 0 && part == 1) {
+        left = g.K, part = 2;
+        pa = g.a[1] + m0 * row_a;
+        pb = g.b[1] + n0 * row_b;
+        la.uncut(), lb.uncut();
+      }
+      if (left < SK) la.cut(left), lb.cut(left);
     }
   };
+  if (left < SK) la.cut(left), lb.cut(left);
 
   f32x4_t acc[2][2][QA][QB];
 #pragma unroll
@@ -265,150 +490,93 @@ __global__ __launch_bounds__(THREADS, 2) void dense_kernel(Args g, int n_mt, int
       for (int i = 0; i < QA; ++i)
 #pragma unroll
         for (int j = 0; j < QB; ++j) acc[x][y][i][j] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-
-  for (int s = 0; s < NST - 1 && s < nk; ++s) issue();
-  __shared__ int sid[ADAPT ? BM : 1], list[ADAPT ? BM : 1], n_list;
-  if constexpr (ADAPT) list_adapters<BM>(g.ad, m0, g.M, tid, sid, list, &n_list);
-  for (int kt = 0; kt < nk; ++kt) {
-    // step kt has landed when at most the loads of the steps behind it are in flight; past the
-    // barrier every wave's part of it has, and every wave is done with step kt - 1
-    if (issued - kt - 1 >= NST - 2 && NST > 2)
-      wait_vmcnt<(NST - 2) * NL>();
+  bf16x8_t fa[2][2 * QA], fb[2][2 * QB];
+  Frags<BM, SA, KS> ra;
+  Frags<BN, SB, KS> rb;
+  ra.init(wm, lane);
+  rb.init(wn, lane);
+  // fragment r of 32 of a stage's K, B's before A's
+  auto read_frag = [&](int set, int r, const KMOE_LDS uint8_t* st, int ks) {
+    if (r < 2 * QB)
+      fb[set][r] = rb.read(st + TILE, r, ks);
     else
-      wait_vmcnt<0>();
-    wait_lgkmcnt0();
-    barrier_nofence();
-    if (issued < nk) issue();
-    const uint8_t* const pa = lds + (kt % NST) * STAGE;
-    const uint8_t* const pb = pa + LoadA::BYTES;
-    bf16x8_t fa[2][QA][2], fb[2][QB][2];
+      fa[set][r - 2 * QB] = ra.read(st, r - 2 * QB, ks);
+  };
+  const int nk = (g.K + SK - 1) / SK * PARTS;
+#pragma unroll 1
+  for (int s = 0; s < STAGES; ++s) {
 #pragma unroll
-    for (int x = 0; x < 2; ++x) {
-#pragma unroll
-      for (int i = 0; i < QA; ++i)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) fa[x][i][s] = frag<BM, SA>(pa, x * (BM / 2) + wm * (BM / 4) + i * 16, s, lane);
-#pragma unroll
-      for (int j = 0; j < QB; ++j)
-#pragma unroll
-        for (int s = 0; s < 2; ++s) fb[x][j][s] = frag<BN, SB>(pb, x * (BN / 2) + wn * (BN / 8) + j * 16, s, lane);
+    for (int q = 0; q < NP; ++q) {
+      dma16_where(place_piece(q));
+      asm volatile("s_nop 1");
+      load_piece(q);
     }
+    next_step();
+  }
+  if constexpr (ADAPT) list_adapters<BM>(g.ad, m0, g.M, tid, sid, list, &n_list);
+  wait_vmcnt<(STAGES - 1) * NP>();
+  barrier_nofence();
+#pragma unroll
+  for (int r = 0; r < NR; ++r) read_frag(0, r, ldsp, 0);
+  constexpr int RS = NM >= 3 * NR + 8 ? 3 : NM >= 2 * NR ? 2 : 1;  // MFMAs from read to read: the last has time to land
+  constexpr int PS = NM / NP;                                      // and from load to load
+  static_assert(RS * (NR - 1) < NM && NP <= NM, "reads and loads find their places");
+  int at = 0;  // where the step's stage begins
+  // 32 of K of a step: its fragments are in set SET, those of the next 32 are read into the other;
+  // LAST of a step: from the next stage, which has landed past the barrier, and the step STAGES on is
+  // loaded into this one, of which every wave then has all fragments.
+  auto sub = [&](auto ks_tag, auto set_tag) {
+    constexpr int ks = decltype(ks_tag)::value, SET = decltype(set_tag)::value;
+    constexpr bool LAST = ks == KS - 1;
+    if constexpr (LAST) {
+      wait_lgkmcnt0();
+      wait_vmcnt<(STAGES - 2) * NP>();
+      barrier_nofence();
+      __builtin_amdgcn_sched_barrier(0);
+      at = at == (STAGES - 1) * STAGE ? 0 : at + STAGE;
+    }
+    static_for<0, NM>([&](auto gt) {
+      constexpr int G = decltype(gt)::value, a = G / (2 * QB), b = G % (2 * QB);
+      f32x4_t& c = acc[a / QA][b / QB][a % QA][b % QB];
+      c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[SET][b], fa[SET][a], c, 0, 0, 0);
+      __builtin_amdgcn_sched_barrier(0);
+      constexpr bool reads = G % RS == 0 && G / RS < NR;
+      constexpr bool points = LAST && G % PS == 0 && G / PS < NP;
+      constexpr bool loads = LAST && G % PS == (PS > 1) && G / PS < NP;
+      if constexpr (reads) read_frag(SET ^ 1, G / RS, ldsp + at, LAST ? 0 : ks + 1);
+      if constexpr (points) dma16_where(place_piece(G / PS));
+      if constexpr (points && loads) asm volatile("s_nop 1");  // (no MFMA between the two)
+      if constexpr (loads) load_piece(G / PS);
+      if constexpr (reads || points || loads) __builtin_amdgcn_sched_barrier(0);
+    });
+    if constexpr (LAST) next_step();
+  };
+  using Zero = std::integral_constant<int, 0>;
+  using One = std::integral_constant<int, 1>;
+  // (two times 32 of K, two steps or one of 64: the fragments' sets take turns.  An odd last step of 32
+  // is followed by one of zeros.)
+  // The accumulators stay in accumulation registers over the loop: left to itself the compiler keeps some
+  // in others and copies them there and back in every step.
+  auto hold = [&]() {
 #pragma unroll
     for (int x = 0; x < 2; ++x)
 #pragma unroll
-      for (int yy = 0; yy < 2; ++yy) {
-        const int y = x ? 1 - yy : yy;
+      for (int y = 0; y < 2; ++y)
 #pragma unroll
-        for (int s = 0; s < 2; ++s)
+        for (int i = 0; i < QA; ++i)
 #pragma unroll
-          for (int i = 0; i < QA; ++i)
-#pragma unroll
-            for (int j = 0; j < QB; ++j)
-              acc[x][y][i][j] =
-                  __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[y][j][s], fa[x][i][s], acc[x][y][i][j], 0, 0, 0);
-      }
-  }
-
-  const int l16 = lane & 15, lq = lane >> 4;
-  if constexpr (ADAPT) {
-    // Each adapter of the tile: its product with the rows that have it, 32 ranks at a time.  A
-    // wave computes it for whole blocks of 16 rows and adds it, by selection, to the rows that have
-    // the adapter: a sum over masked operands would carry a NaN or an infinity of one request's
-    // adapter into the others' rows.
-    for (int a = 0; a < n_list; ++a) {
-      const int id = __builtin_amdgcn_readfirstlane(list[a]);
-      for (int s = 0; s < g.ad.r; s += 32) {
-        const int k = s + 8 * lq;
-        const bool in = k < g.ad.r;
-        bf16x8_t fb[2][QB];
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-          for (int j = 0; j < QB; ++j) {
-            const int n = n0 + (GATED ? 0 : y * (BN / 2)) + wn * (BN / 8) + j * 16 + l16;
-            const uint16_t* b = g.ad.b[GATED ? y : 0];
-            fb[y][j] = bf16x8_t{};
-            if (in && n < g.N && b)
-              fb[y][j] = *reinterpret_cast<const bf16x8_t*>(b + ((int64_t)id * g.N + n) * g.ad.r + k);
-          }
-#pragma unroll
-        for (int x = 0; x < 2; ++x)
-#pragma unroll
-          for (int i = 0; i < QA; ++i) {
-            const int tr = x * (BM / 2) + wm * (BM / 4) + i * 16 + l16;
-            const bool mine = sid[tr] == id;
-            if (!__any(mine)) continue;
-            bf16x8_t fv[2];
-#pragma unroll
-            for (int y = 0; y < (GATED ? 2 : 1); ++y) {
-              const uint16_t* v = g.ad.v[y];
-              fv[y] = bf16x8_t{};
-              if (in && mine && v) fv[y] = *reinterpret_cast<const bf16x8_t*>(v + (m0 + tr) * g.ad.r + k);
-            }
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-#pragma unroll
-              for (int j = 0; j < QB; ++j) {
-                const f32x4_t d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[y][j], fv[GATED ? y : 0],
-                                                                         f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-#pragma unroll
-                for (int t = 0; t < 4; ++t) acc[x][y][i][j][t] += mine ? d[t] : 0.0f;
-              }
-          }
-      }
-    }
-  }
-  // ---- epilogue: acc[x][y][i][j][t] is row m, column n + t
-#pragma unroll
-  for (int x = 0; x < 2; ++x)
-#pragma unroll
-    for (int i = 0; i < QA; ++i) {
-      const int64_t m = m0 + x * (BM / 2) + wm * (BM / 4) + i * 16 + l16;
-      if (m >= g.M) continue;
-      if constexpr (GATED) {
-#pragma unroll
-        for (int j = 0; j < QB; ++j) {
-          const int n = n0 + wn * (BN / 8) + j * 16 + 4 * lq;
-          if (n >= g.N) continue;
-          float h[4], p[4], q[4];
-#pragma unroll
-          for (int t = 0; t < 4; ++t) {
-            float a, da;
-            const float up = acc[x][1][i][j][t];
-            act_f32(g.act, acc[x][0][i][j][t], a, da);
-            h[t] = a * up, p[t] = da * up, q[t] = a;
-          }
-          const int64_t at = m * g.ldc + n;
-          *reinterpret_cast<i32x2_t*>(static_cast<uint16_t*>(g.c) + at) = pack4(h[0], h[1], h[2], h[3]);
-          if (g.p) {
-            *reinterpret_cast<i32x2_t*>(g.p + at) = pack4(p[0], p[1], p[2], p[3]);
-            *reinterpret_cast<i32x2_t*>(g.q + at) = pack4(q[0], q[1], q[2], q[3]);
-          }
-        }
-      } else {
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-          for (int j = 0; j < QB; ++j) {
-            const int n = n0 + y * (BN / 2) + wn * (BN / 8) + j * 16 + 4 * lq;
-            if (n >= g.N) continue;
-            const f32x4_t v = acc[x][y][i][j];
-            const int64_t at = m * g.ldc + n;
-            if constexpr (EPI == EPI_DH) {
-              float p[4], q[4];
-              unpack4(*reinterpret_cast<const i32x2_t*>(g.p + at), p);
-              unpack4(*reinterpret_cast<const i32x2_t*>(g.q + at), q);
-              *reinterpret_cast<i32x2_t*>(static_cast<uint16_t*>(g.c) + at) =
-                  pack4(v[0] * p[0], v[1] * p[1], v[2] * p[2], v[3] * p[3]);
-              *reinterpret_cast<i32x2_t*>(g.c2 + at) = pack4(v[0] * q[0], v[1] * q[1], v[2] * q[2], v[3] * q[3]);
-            } else if (g.c_f32) {
-              *reinterpret_cast<f32x4_t*>(static_cast<float*>(g.c) + at) = v;
-            } else {
-              *reinterpret_cast<i32x2_t*>(static_cast<uint16_t*>(g.c) + at) = pack4(v[0], v[1], v[2], v[3]);
-            }
-          }
-      }
-    }
+          for (int j = 0; j < QB; ++j) asm volatile("" : "+a"(acc[x][y][i][j]));
+  };
+  hold();
+  int n = 0;
+#pragma unroll 1
+  do {
+    sub(Zero{}, Zero{});
+    sub(std::integral_constant<int, KS - 1>{}, One{});
+  } while ((n += 2) < nk * KS);
+  hold();
+  wait_vmcnt<0>();  // (the zeros past the end are on their way into this workgroup's LDS)
+  finish<BM, BN, EPI, ADAPT>(g, acc, m0, n0, wm, wn, lane, sid, list, n_list);
 }
 
 }  // namespace kmoe_dense

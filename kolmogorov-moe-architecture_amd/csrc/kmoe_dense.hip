@@ -21,22 +21,26 @@ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
   KMOE_REQUIRE((n) > 0 && (r) > 0 && (r) <= KMOE_MAX_RANK && (r) % 8 == 0, KMOE_ERR_SHAPE,                      \
                who ": %d adapters of rank %d (a multiple of 8, at most %d)", (int)(n), (int)(r), KMOE_MAX_RANK)
 
+extern "C" size_t kmoe_dense_saved_bytes(int64_t T, int F) {
+  return T <= 0 || F <= 0 ? 0 : (size_t)kmoe::ceil_div<int64_t>(T, 16) * kmoe::ceil_div(F, 16) * SAVED_BLOCK;
+}
+
 extern "C" int kmoe_dense_gate_up(const void* x, int64_t T, int d, const void* w_gate, const void* w_up, int F, int act,
                                   const int32_t* ids, int n_adapters, int rank, const void* v_gate, const void* b_gate,
-                                  const void* v_up, const void* b_up, void* h, void* p, void* q, void* stream) {
+                                  const void* v_up, const void* b_up, void* h, void* saved, void* stream) {
   KMOE_DENSE_SIZES("kmoe_dense_gate_up", T, F, d);
   KMOE_REQUIRE(act >= KMOE_ACT_SILU && act <= KMOE_ACT_RELU, KMOE_ERR_UNSUPPORTED, "kmoe_dense_gate_up: activation %d", act);
   if (T == 0) return KMOE_OK;
-  KMOE_REQUIRE(x && w_gate && w_up && h && !p == !q, KMOE_ERR_NULL, "kmoe_dense_gate_up: null buffer");
-  KMOE_DENSE_ALIGNED("kmoe_dense_gate_up", x, w_gate, w_up, h, p, q, v_gate, b_gate, v_up, b_up);
+  KMOE_REQUIRE(x && w_gate && w_up && h, KMOE_ERR_NULL, "kmoe_dense_gate_up: null buffer");
+  KMOE_DENSE_ALIGNED("kmoe_dense_gate_up", x, w_gate, w_up, h, saved, v_gate, b_gate, v_up, b_up);
   Args g{};
   g.a[0] = static_cast<const uint16_t*>(x);
   g.b[0] = static_cast<const uint16_t*>(w_gate), g.b[1] = static_cast<const uint16_t*>(w_up);
-  g.parts = 1, g.K = d, g.lda = d, g.ldb = d, g.M = T, g.N = F, g.ldc = F, g.c = h, g.act = act;
-  g.p = static_cast<uint16_t*>(p), g.q = static_cast<uint16_t*>(q);
+  g.K = d, g.lda = d, g.ldb = d, g.M = T, g.N = F, g.ldc = F, g.c = h, g.act = act;
+  g.saved = static_cast<uint8_t*>(saved);
   if (ids) {
     KMOE_DENSE_ADAPTERS("kmoe_dense_gate_up", n_adapters, rank);
-    KMOE_REQUIRE(!v_gate == !b_gate && !v_up == !b_up && !p, KMOE_ERR_NULL,
+    KMOE_REQUIRE(!v_gate == !b_gate && !v_up == !b_up && !saved, KMOE_ERR_NULL,
                  "kmoe_dense_gate_up: adapters come with their inner products, and without values for a backward");
     g.ad = {ids, {static_cast<const uint16_t*>(v_gate), static_cast<const uint16_t*>(v_up)},
             {static_cast<const uint16_t*>(b_gate), static_cast<const uint16_t*>(b_up)}, n_adapters, rank};
@@ -52,7 +56,7 @@ extern "C" int kmoe_dense_linear(const void* x, int64_t T, int K, const void* w,
   KMOE_DENSE_ALIGNED("kmoe_dense_linear", x, w, y, v, b);
   Args g{};
   g.a[0] = static_cast<const uint16_t*>(x), g.b[0] = static_cast<const uint16_t*>(w);
-  g.parts = 1, g.K = K, g.lda = K, g.ldb = K, g.M = T, g.N = N, g.ldc = N, g.c = y;
+  g.K = K, g.lda = K, g.ldb = K, g.M = T, g.N = N, g.ldc = N, g.c = y;
   if (ids) {
     KMOE_DENSE_ADAPTERS("kmoe_dense_linear", n_adapters, rank);
     KMOE_REQUIRE(v && b, KMOE_ERR_NULL, "kmoe_dense_linear: null adapter buffer");
@@ -61,17 +65,17 @@ extern "C" int kmoe_dense_linear(const void* x, int64_t T, int K, const void* w,
   return ids ? launch_linear_adapt(g, kmoe::as_stream(stream)) : launch_linear(g, kmoe::as_stream(stream));
 }
 
-extern "C" int kmoe_dense_dh(const void* dy, int64_t T, int d, const void* w_down, int F, const void* p, const void* q,
-                             void* dgate, void* dup, void* stream) {
+extern "C" int kmoe_dense_dh(const void* dy, int64_t T, int d, const void* w_down, int F, const void* saved, void* dgate,
+                             void* dup, void* stream) {
   KMOE_DENSE_SIZES("kmoe_dense_dh", T, F, d);
   if (T == 0) return KMOE_OK;
-  KMOE_REQUIRE(dy && w_down && p && q && dgate && dup, KMOE_ERR_NULL, "kmoe_dense_dh: null buffer");
-  KMOE_DENSE_ALIGNED("kmoe_dense_dh", dy, w_down, p, q, dgate, dup);
+  KMOE_REQUIRE(dy && w_down && saved && dgate && dup, KMOE_ERR_NULL, "kmoe_dense_dh: null buffer");
+  KMOE_DENSE_ALIGNED("kmoe_dense_dh", dy, w_down, saved, dgate, dup);
   Args g{};
   g.a[0] = static_cast<const uint16_t*>(dy), g.b[0] = static_cast<const uint16_t*>(w_down);
-  g.parts = 1, g.K = d, g.lda = d, g.ldb = F, g.M = T, g.N = F, g.ldc = F, g.c = dgate;
+  g.K = d, g.lda = d, g.ldb = F, g.M = T, g.N = F, g.ldc = F, g.c = dgate;
   g.c2 = static_cast<uint16_t*>(dup);
-  g.p = static_cast<uint16_t*>(const_cast<void*>(p)), g.q = static_cast<uint16_t*>(const_cast<void*>(q));
+  g.saved = static_cast<uint8_t*>(const_cast<void*>(saved));
   return launch_dh(g, kmoe::as_stream(stream));
 }
 
@@ -85,13 +89,14 @@ extern "C" int kmoe_dense_dx(const void* dy, const void* dy2, int64_t T, int N, 
   Args g{};
   g.a[0] = static_cast<const uint16_t*>(dy), g.b[0] = static_cast<const uint16_t*>(w);
   g.a[1] = static_cast<const uint16_t*>(dy2), g.b[1] = static_cast<const uint16_t*>(w2);
-  g.parts = dy2 ? 2 : 1, g.K = N, g.lda = N, g.ldb = K, g.M = T, g.N = K, g.ldc = K, g.c = dx;
+  g.K = N, g.lda = N, g.ldb = K, g.M = T, g.N = K, g.ldc = K, g.c = dx;
   if (ids) {
     KMOE_DENSE_ADAPTERS("kmoe_dense_dx", n_adapters, rank);
     KMOE_REQUIRE(u && at && !dy2, KMOE_ERR_NULL, "kmoe_dense_dx: adapters belong to one product, with both their buffers");
     g.ad = {ids, {static_cast<const uint16_t*>(u), nullptr}, {static_cast<const uint16_t*>(at), nullptr}, n_adapters, rank};
   }
-  return ids ? launch_dx_adapt(g, kmoe::as_stream(stream)) : launch_dx(g, kmoe::as_stream(stream));
+  hipStream_t s = kmoe::as_stream(stream);
+  return ids ? launch_dx_adapt(g, s) : dy2 ? launch_dx_two(g, s) : launch_dx(g, s);
 }
 
 extern "C" int kmoe_dense_wgrad(const void* a, const void* b, int64_t T, int M, int N, void* c, int c_dtype, void* stream) {
@@ -102,7 +107,7 @@ extern "C" int kmoe_dense_wgrad(const void* a, const void* b, int64_t T, int M, 
   KMOE_DENSE_ALIGNED("kmoe_dense_wgrad", a, b, c);
   Args g{};
   g.a[0] = static_cast<const uint16_t*>(a), g.b[0] = static_cast<const uint16_t*>(b);
-  g.parts = 1, g.K = (int)T, g.lda = M, g.ldb = N, g.M = M, g.N = N, g.ldc = N, g.c = c;
+  g.K = (int)T, g.lda = M, g.ldb = N, g.M = M, g.N = N, g.ldc = N, g.c = c;
   g.c_f32 = c_dtype == KMOE_DTYPE_F32;
   return launch_wgrad(g, kmoe::as_stream(stream));
 }

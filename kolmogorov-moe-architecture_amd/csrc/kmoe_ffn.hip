@@ -107,15 +107,18 @@ __global__ __launch_bounds__(W * 64) void few_kernel(Args g) {
     }
   }
   float o[4];
+  if constexpr (GATED) {
+    with_act(g.act, [&](auto tag) {
 #pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    if constexpr (GATED) {
-      float a, da;
-      act_f32(g.act, s[0][c], a, da);
-      o[c] = a * s[G - 1][c];
-    } else {
-      o[c] = s[0][c];
-    }
+      for (int c = 0; c < 4; ++c) {
+        float a, da;
+        act_at<decltype(tag)::value>(s[0][c], a, da);
+        o[c] = a * s[G - 1][c];
+      }
+    });
+  } else {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[c] = s[0][c];
   }
   *reinterpret_cast<i32x2_t*>(static_cast<uint16_t*>(g.c) + t * g.ldc + n) = pack4(o[0], o[1], o[2], o[3]);
 }
@@ -152,7 +155,7 @@ int project(const void* x, int64_t T, int K, const void* w, int N, const int32_t
   if (T > FEW)
     return kmoe_dense_linear(x, T, K, w, N, ad ? ids : nullptr, n, ad ? ad->rank : 0, v, ad ? ad->b : nullptr, y, s);
   Args g{};
-  g.a[0] = bf(x), g.b[0] = bf(w), g.parts = 1, g.K = K, g.lda = K, g.ldb = K, g.M = T, g.N = N, g.ldc = N, g.c = y;
+  g.a[0] = bf(x), g.b[0] = bf(w), g.K = K, g.lda = K, g.ldb = K, g.M = T, g.N = N, g.ldc = N, g.c = y;
   if (!ad) return launch_few<false, false>(g, s);
   g.ad = {ids, {bf(v), nullptr}, {bf(ad->b), nullptr}, n, ad->rank};
   return launch_few<false, true>(g, s);
@@ -224,10 +227,10 @@ extern "C" int kmoe_gated_ffn(const void* x, int64_t T, int d, int F, const void
   }
   if (T > FEW) {
     rc = kmoe_dense_gate_up(x, T, d, w_gate, w_up, F, act, rgu ? ids : nullptr, n_adapters, rgu, gate ? vg : nullptr,
-                            gate ? gate->b : nullptr, up ? vu : nullptr, up ? up->b : nullptr, h, nullptr, nullptr, stream);
+                            gate ? gate->b : nullptr, up ? vu : nullptr, up ? up->b : nullptr, h, nullptr, stream);
   } else {
     Args g{};
-    g.a[0] = bf(x), g.b[0] = bf(w_gate), g.b[1] = bf(w_up), g.parts = 1, g.K = d, g.lda = d, g.ldb = d, g.M = T, g.N = F;
+    g.a[0] = bf(x), g.b[0] = bf(w_gate), g.b[1] = bf(w_up), g.K = d, g.lda = d, g.ldb = d, g.M = T, g.N = F;
     g.ldc = F, g.c = h, g.act = act;
     if (rgu)
       g.ad = {ids, {gate ? bf(vg) : nullptr, up ? bf(vu) : nullptr}, {gate ? bf(gate->b) : nullptr, up ? bf(up->b) : nullptr},

@@ -135,10 +135,10 @@ _SIGNATURES = {
     "kmoe_adapted_linear_workspace_bytes": (_sz, [_i64, _i32]),
     "kmoe_adapted_linear": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _sz, _vp]),
     "kmoe_adapter_inner": (_i32, [_vp, _i64, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
-    "kmoe_dense_gate_up": (_i32, [_vp, _i64, _i32, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp,
-                                  _vp]),
+    "kmoe_dense_saved_bytes": (_sz, [_i64, _i32]),
+    "kmoe_dense_gate_up": (_i32, [_vp, _i64, _i32, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "kmoe_dense_linear": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp]),
-    "kmoe_dense_dh": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp]),
+    "kmoe_dense_dh": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _vp]),
     "kmoe_dense_dx": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp]),
     "kmoe_dense_wgrad": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _i32, _vp]),
     "kmoe_adapter_grad_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),

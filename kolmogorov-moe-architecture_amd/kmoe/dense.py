@@ -8,8 +8,9 @@
   row t with the adapter ids[t]; also on all three projections of the block.
 
 Numerics: bf16 operands, f32 sums.  What is rounded to bf16 between the products: the block's
-hidden values h = act(g) u (an operand of the down product); for the backward u act'(g) and act(g),
-which take the pre-activations' place; an adapter's inner products with their scale.
+hidden values h = act(g) u (an operand of the down product), the gradients of its pre-activations, and an
+adapter's inner products with their scale.  What the backward keeps of the pre-activations, u act'(g)
+and act(g), has 16 bits of precision.
 """
 from __future__ import annotations
 
@@ -199,23 +200,24 @@ class _GatedFFNFn(torch.autograd.Function):
         bg, bu, bd = (_aligned(w.detach()) for w in (wg, wu, wd))
         T, d = x2d.shape
         F = bg.shape[0]
-        h, p, q = (torch.empty(T, F, device=x.device, dtype=_BF16) for _ in range(3))
+        h = torch.empty(T, F, device=x.device, dtype=_BF16)
+        saved = torch.empty(max(_lib.load().kmoe_dense_saved_bytes(T, F), 16), device=x.device, dtype=torch.uint8)
         y = torch.empty(T, d, device=x.device, dtype=_BF16)
         with _device(x.device):
             with _Stage("ffn_gate_up"):
                 _lib.call("kmoe_dense_gate_up", ptr(x2d), T, d, ptr(bg), ptr(bu), F, act, None, 0, 0, None, None, None, None,
-                          ptr(h), ptr(p), ptr(q), _stream(x))
+                          ptr(h), ptr(saved), _stream(x))
             with _Stage("ffn_down"):
                 _lib.call("kmoe_dense_linear", ptr(h), T, F, ptr(bd), d, None, 0, 0, None, None, ptr(y), _stream(x))
         # the weights themselves are saved too: a write to one before the backward is refused
-        ctx.save_for_backward(x2d, h, p, q, bg, bu, bd, wg, wu, wd)
+        ctx.save_for_backward(x2d, h, saved, bg, bu, bd, wg, wu, wd)
         ctx.meta = (x.shape, x.dtype)
         return y.view(x.shape).to(x.dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x2d, h, p, q, bg, bu, bd, wg, wu, wd = ctx.saved_tensors
+        x2d, h, saved, bg, bu, bd, wg, wu, wd = ctx.saved_tensors
         shape, dtype = ctx.meta
         T, F = h.shape
         d = x2d.shape[1]
@@ -226,7 +228,7 @@ class _GatedFFNFn(torch.autograd.Function):
             if need_x or need_g or need_u:
                 dg, du = (torch.empty(T, F, device=x2d.device, dtype=_BF16) for _ in range(2))
                 with _Stage("bwd_ffn_dh"):
-                    _lib.call("kmoe_dense_dh", ptr(dy2), T, d, ptr(bd), F, ptr(p), ptr(q), ptr(dg), ptr(du), _stream(x2d))
+                    _lib.call("kmoe_dense_dh", ptr(dy2), T, d, ptr(bd), F, ptr(saved), ptr(dg), ptr(du), _stream(x2d))
             if need_x:
                 with _Stage("bwd_ffn_dx"):
                     dx = _dense_dx(dg, bg, du, bu).view(shape).to(dtype)

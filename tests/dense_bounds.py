@@ -79,13 +79,18 @@ def adapted(x, w, ad, ids):
     return V(v, e)
 
 
+def cut24(a):
+    """A value cut to the top 24 bits of its f32: up to 2^-15 of it lost."""
+    return V(a.v, a.e + 2.0 ** -15 * (a.v.abs() + a.e) + 1e-40)
+
+
 def ffn(x, wg, wu, wd, name, ads=(None, None, None), ids=None):
     """(y, and for the backward h, p, q) of the gated block."""
     x, wg, wu, wd = V(x), V(wg), V(wu), V(wd)
     g, u = adapted(x, wg, ads[0], ids), adapted(x, wu, ads[1], ids)
     a, d = act(name, g)
     h = (a * u).bf16()
-    return adapted(h, wd, ads[2], ids).bf16(), h, (d * u).bf16(), a.bf16()
+    return adapted(h, wd, ads[2], ids).bf16(), h, cut24(d * u), cut24(a)
 
 
 def ffn_grads(x, wg, wu, wd, dy, h, p, q):

@@ -134,21 +134,22 @@ def test_abi_parts():
     for i in (0, 3, 6, 8):
         assert call(**{f"a{i}": None}) == -1, i
     assert call(a9=FAKE) == -1 and call(a2=60) == -2 and call(a4=0) == -2 and call(a5=12) == -2 and call(a6=ODD) == -2
-    call = _call("kmoe_dense_gate_up", [FAKE, 100, 64, FAKE, FAKE, 72, 0, FAKE, 2, 8, FAKE, FAKE, FAKE, FAKE, FAKE, None, None,
-                                        None])
+    call = _call("kmoe_dense_gate_up", [FAKE, 100, 64, FAKE, FAKE, 72, 0, FAKE, 2, 8, FAKE, FAKE, FAKE, FAKE, FAKE, None, None])
     assert call(a1=0) == 0
     for i in (0, 3, 4, 10, 13, 14):
         assert call(**{f"a{i}": None}) == -1, i
-    assert call(a15=FAKE, a16=FAKE) == -1 and call(a15=FAKE) == -1  # adapters and values for a backward; p without q
+    assert call(a15=FAKE) == -1  # adapters and values for a backward
+    assert _lib.load().kmoe_dense_saved_bytes(17, 24) == 2 * 2 * 1536 and _lib.load().kmoe_dense_saved_bytes(0, 24) == 0
     assert call(a6=9) == -6 and call(a2=63) == -2 and call(a14=ODD) == -2 and call(a9=7) == -2
     call = _call("kmoe_dense_linear", [FAKE, 100, 64, FAKE, 72, FAKE, 2, 8, FAKE, FAKE, FAKE, None])
     assert call(a1=0) == 0
     for i in (0, 3, 8, 9, 10):
         assert call(**{f"a{i}": None}) == -1, i
     assert call(a2=0) == -2 and call(a4=71) == -2 and call(a10=ODD) == -2
-    call = _call("kmoe_dense_dh", [FAKE, 100, 64, FAKE, 72, FAKE, FAKE, FAKE, FAKE, None])
+    assert call(a2=1 << 22) == -2  # a tile's offsets are 32 bits
+    call = _call("kmoe_dense_dh", [FAKE, 100, 64, FAKE, 72, FAKE, FAKE, FAKE, None])
     assert call(a1=0) == 0
-    for i in (0, 3, 5, 6, 7, 8):
+    for i in (0, 3, 5, 6, 7):
         assert call(**{f"a{i}": None}) == -1, i
     call = _call("kmoe_dense_dx", [FAKE, None, 100, 72, FAKE, None, 64, FAKE, 2, 8, FAKE, FAKE, FAKE, None])
     assert call(a2=0) == 0
