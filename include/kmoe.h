@@ -693,12 +693,12 @@ typedef struct {
 /* y (T, d) = (act(x w_gate^T) * (x w_up^T)) w_down^T with adapters (each nullable; the gate's and
  * the up projection's of one rank), act a KMOE_ACT_*; w_gate, w_up (F, d), w_down (d, F).
  * The hidden values are rounded to bf16.                                            */
-size_t kmoe_gated_ffn_workspace_bytes(int64_t T, int F, int rank_gate_up, int rank_down);
+size_t kmoe_gated_ffn_workspace_bytes(int64_t T, int d, int F, int rank_gate_up, int rank_down);
 int kmoe_gated_ffn(const void* x, int64_t T, int d, int F, const void* w_gate, const void* w_up, const void* w_down,
                    int act, const int32_t* ids, int n_adapters, const kmoe_adapter* gate, const kmoe_adapter* up,
                    const kmoe_adapter* down, void* y, void* workspace, size_t workspace_bytes, void* stream);
 /* y (T, N) = x w^T with an adapter (nullable).                                      */
-size_t kmoe_adapted_linear_workspace_bytes(int64_t T, int rank);
+size_t kmoe_adapted_linear_workspace_bytes(int64_t T, int K, int N, int rank);
 int kmoe_adapted_linear(const void* x, int64_t T, int K, const void* w, int N, const int32_t* ids, int n_adapters,
                         const kmoe_adapter* adapter, void* y, void* workspace, size_t workspace_bytes, void* stream);
 

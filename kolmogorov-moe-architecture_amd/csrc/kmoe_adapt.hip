@@ -1,7 +1,10 @@
 // Low-rank adapters of many requests: the inner products, and the gradients of both factors.
-#include "kmoe_dense.h"
+#include "kmoe_dense_launch.h"
+#include "kmoe_few.h"
 
+using kmoe_dense::NOWHERE;
 using kmoe_dense::pack4;
+using kmoe_dense::stream16;
 using kmoe_dense::tr4_t;
 
 namespace {
@@ -9,10 +12,11 @@ namespace {
 // ---------------------------------------------------------------- inner products
 // v[t, j] = scale[i] sum_k x[t, k] a[i, j, k], i = ids[t], rounded to bf16: an operand of the outer
 // product's MFMAs, one rounding (half a step of 2^-8) of a term that adds to the projection's.
-// A workgroup takes 16 rows and every gridDim.y-th of the adapters that they have (few rows with
-// an adapter each: a workgroup an adapter); its 8 waves share K, 64 at a time.  Each adapter's
-// product is computed for all 16 rows and kept for those that have it: bound by reading x and the
-// adapters, not by the products, and no row's values meet another's adapter.
+// A workgroup takes 16 rows, RB blocks of 16 ranks and every gridDim.y-th of the adapters that the rows
+// have (few rows with an adapter each: a workgroup an adapter); its 8 waves share K.  Each
+// adapter's product is computed for all 16 rows and kept for those that have it: bound by reading
+// x and the adapters, not by the products, and no row's values meet another's adapter.  Few
+// rows take a workgroup a block of ranks: latency counts and x is small.
 constexpr int SW = 8;  // waves
 
 struct Shrink {
@@ -21,18 +25,19 @@ struct Shrink {
   int K;
   const int32_t* ids;
   int n, r;
+  int sides;      // 1 or 2 sets of adapters; blockIdx.z = the first of its RB blocks of ranks * sides + set
   const uint16_t* a[2];
   const float* scale[2];
   uint16_t* v[2];
 };
 
-template <int RB>
+template <int RB, int D>
 __global__ __launch_bounds__(SW * 64) void shrink_kernel(Shrink g) {
   __shared__ f32x4_t part[SW][RB][64];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, lq = lane >> 4;
   const int64_t t0 = (int64_t)blockIdx.x * 16;
-  const int z = blockIdx.z;
+  const int z = blockIdx.z % g.sides, j0 = blockIdx.z / g.sides * (RB * 16);
   int id = t0 + l16 < g.T ? g.ids[t0 + l16] : -1;
   if ((unsigned)id >= (unsigned)g.n) id = -1;
   bool first = lane < 16 && id >= 0;
@@ -42,40 +47,27 @@ __global__ __launch_bounds__(SW * 64) void shrink_kernel(Shrink g) {
     if (t < lane && o == id) first = false;
   }
   uint64_t todo = __ballot(first);
-  const int64_t row = t0 + l16 < g.T ? t0 + l16 : g.T - 1;
-  const uint16_t* const xr = g.x + row * g.K;
+  const uint16_t* const x = g.x + t0 * g.K;
+  const uint32_t xoff = t0 + l16 < g.T ? (uint32_t)(l16 * g.K) * 2 : NOWHERE;
+  uint32_t aoff[RB];
+#pragma unroll
+  for (int b = 0; b < RB; ++b) {
+    const int j = j0 + b * 16 + l16;
+    aoff[b] = j < g.r ? (uint32_t)(j * g.K) * 2 : NOWHERE;
+  }
   for (int c = 0; todo; ++c, todo &= todo - 1) {
     if (c % (int)gridDim.y != (int)blockIdx.y) continue;
     const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
-    const uint16_t* ar[RB];
-#pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const int j = b * 16 + l16 < g.r ? b * 16 + l16 : g.r - 1;
-      ar[b] = g.a[z] + ((int64_t)cur * g.r + j) * g.K;
-    }
+    const void* a[RB];
     f32x4_t acc[RB];
 #pragma unroll
-    for (int b = 0; b < RB; ++b) acc[b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-    auto step = [&](int k, bool in) {
-      bf16x8_t fx = *reinterpret_cast<const bf16x8_t*>(xr + (in ? k : 0));
-      if (!in) fx = bf16x8_t{};
-#pragma unroll
-      for (int b = 0; b < RB; ++b) {
-        bf16x8_t fa = *reinterpret_cast<const bf16x8_t*>(ar[b] + (in ? k : 0));
-        if (!in) fa = bf16x8_t{};
-        acc[b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fa, fx, acc[b], 0, 0, 0);
-      }
-    };
-    const int full = g.K & ~63;
-#pragma unroll 4
-    for (int k0 = wave * 64; k0 < full; k0 += SW * 64) {
-      step(k0 + 8 * lq, true);
-      step(k0 + 32 + 8 * lq, true);
+    for (int b = 0; b < RB; ++b) {
+      a[b] = g.a[z] + (int64_t)cur * g.r * g.K;
+      acc[b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    if (full < g.K && (full / 64) % SW == wave) {
-      step(full + 8 * lq, full + 8 * lq < g.K);
-      step(full + 32 + 8 * lq, full + 32 + 8 * lq < g.K);
-    }
+    bf16x8_t fa[D][2][RB], fx[D][2];
+    stream16<RB, SW, D>(a, aoff, x, xoff, g.K, wave, lane, acc, false, fa, fx);
+    stream16<RB, SW, D>(a, aoff, x, xoff, g.K, wave, lane, acc, true, fa, fx);
 #pragma unroll
     for (int b = 0; b < RB; ++b) part[wave][b][lane] = acc[b];
     __syncthreads();
@@ -84,7 +76,7 @@ __global__ __launch_bounds__(SW * 64) void shrink_kernel(Shrink g) {
       f32x4_t s = part[0][wave][lane];
 #pragma unroll
       for (int w = 1; w < SW; ++w) s += part[w][wave][lane];
-      const int j = wave * 16 + 4 * lq;
+      const int j = j0 + wave * 16 + 4 * lq;
       if (id == cur && j < g.r) {
         const float f = g.scale[z] ? g.scale[z][cur] : 1.0f;
         *reinterpret_cast<i32x2_t*>(g.v[z] + (t0 + l16) * g.r + j) = pack4(f * s[0], f * s[1], f * s[2], f * s[3]);
@@ -226,6 +218,12 @@ bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0;
 
 }  // namespace
 
+int kmoe_dense::launch_sum_runs(const float* part, int runs, int64_t total, uint16_t* out, hipStream_t s) {
+  hipLaunchKernelGGL(sum_runs_kernel, dim3((unsigned)kmoe::ceil_div<int64_t>(total, 1024)), dim3(256), 0, s, part, runs, total,
+                     out);
+  return kmoe::check_launch("kmoe sum of runs");
+}
+
 extern "C" int kmoe_adapter_inner(const void* x, int64_t T, int K, const int32_t* ids, int n, int rank, const void* a,
                                   const float* scale, void* v, const void* a2, const float* scale2, void* v2,
                                   void* stream) {
@@ -237,24 +235,25 @@ extern "C" int kmoe_adapter_inner(const void* x, int64_t T, int K, const int32_t
   KMOE_REQUIRE(x && ids && a && v && !a2 == !v2, KMOE_ERR_NULL, "kmoe_adapter_inner: null buffer");
   KMOE_REQUIRE(aligned(x) && aligned(a) && aligned(v) && aligned(a2) && aligned(v2), KMOE_ERR_SHAPE,
                "kmoe_adapter_inner: buffers are aligned to 16 bytes");
-  Shrink g{static_cast<const uint16_t*>(x), T, K, ids, n, rank,
+  KMOE_REQUIRE(K < 1 << 22, KMOE_ERR_SHAPE, "kmoe_adapter_inner: rows of %d values (below 2^22)", K);
+  Shrink g{static_cast<const uint16_t*>(x), T, K, ids, n, rank, a2 ? 2 : 1,
            {static_cast<const uint16_t*>(a), static_cast<const uint16_t*>(a2)}, {scale, scale2},
            {static_cast<uint16_t*>(v), static_cast<uint16_t*>(v2)}};
   const int64_t tiles = kmoe::ceil_div<int64_t>(T, 16);
   int64_t y = kmoe::ceil_div<int64_t>(1024, tiles);
   y = y < 16 ? y : 16;
   y = y < n ? y : n;
-  const dim3 grid((unsigned)tiles, (unsigned)y, a2 ? 2 : 1), block(SW * 64);
+  const int blocks = kmoe::ceil_div(rank, 16);
+  // (blocks of ranks side by side read x again each: up to a place for every workgroup)
+  const int rb = tiles * y * blocks * g.sides <= 2 * kmoe::cu_count() || blocks == 1 ? 1 : blocks == 2 ? 2 : 4;
+  const dim3 grid((unsigned)tiles, (unsigned)y, kmoe::ceil_div(blocks, rb) * g.sides), block(SW * 64);
   hipStream_t s = kmoe::as_stream(stream);
-  const int rb = kmoe::ceil_div(rank, 16);
   if (rb == 1)
-    hipLaunchKernelGGL(shrink_kernel<1>, grid, block, 0, s, g);
+    hipLaunchKernelGGL((shrink_kernel<1, 4>), grid, block, 0, s, g);
   else if (rb == 2)
-    hipLaunchKernelGGL(shrink_kernel<2>, grid, block, 0, s, g);
-  else if (rb <= 4)
-    hipLaunchKernelGGL(shrink_kernel<4>, grid, block, 0, s, g);
+    hipLaunchKernelGGL((shrink_kernel<2, 4>), grid, block, 0, s, g);
   else
-    hipLaunchKernelGGL(shrink_kernel<8>, grid, block, 0, s, g);
+    hipLaunchKernelGGL((shrink_kernel<4, 2>), grid, block, 0, s, g);
   return kmoe::check_launch("kmoe_adapter_inner");
 }
 
@@ -305,7 +304,5 @@ extern "C" int kmoe_adapter_grad(const void* l, const void* m, int64_t T, const 
   int rc = kmoe::check_launch("kmoe_adapter_grad");
   if (rc != KMOE_OK || runs == 1) return rc;
   const int64_t total = (int64_t)n * rank * C;
-  hipLaunchKernelGGL(sum_runs_kernel, dim3((unsigned)kmoe::ceil_div<int64_t>(total, 1024)), dim3(256), 0, s, g.part, (int)runs,
-                     total, g.out);
-  return kmoe::check_launch("kmoe_adapter_grad");
+  return kmoe_dense::launch_sum_runs(g.part, (int)runs, total, g.out, s);
 }

@@ -17,7 +17,7 @@
 // each lane picking the piece that belongs where the hardware puts it, so the swizzle costs nothing:
 //   K-contiguous tiles: rows of 64 KS bytes, 16-byte chunks XOR-ed by (row / 2) modulo their number;
 //   a fragment is one ds_read_b128.
-//   K-strided tiles: 32 KS rows of the tile's columns, 32-byte slots XOR-ed by bits 0, 1 and 3 of the
+//   K-strided tiles: 32 KS rows of the tile's columns (192 lie as 256), 32-byte slots XOR-ed by bits 0, 1 and 3 of the
 //   row; a fragment is two ds_read_b64_tr_b16 (in each 16-lane group, lane i receives element
 //   i % 4 of the 8-byte chunks addressed by lanes 4 p + i / 4), whose 16 rows spread over all
 //   banks twice, the least for 512 bytes.
@@ -27,8 +27,8 @@
 // into the step's own stage: every wave has all of its fragments, as it passed the barrier before
 // its last 32, the step's only one.  A load has STAGES - 1 steps to land.  Past the last step zeros
 // are loaded, so that the counts of loads in flight stay the same.
-// Rows and columns past the end repeat others and are not stored; K past the end reads zeros in
-// both operands (a NaN next to a row's end must not meet a zero).
+// Rows, columns and K past the end read as zeros (K's in both operands: a NaN next to a row's end must
+// not meet a zero); what they give is not stored.
 #pragma once
 
 #include <type_traits>
@@ -53,12 +53,13 @@ struct Args {
   const uint16_t* a[2];
   const uint16_t* b[2];
   int K;              // of each part, a multiple of 8
+  int k_run;          // of a run of K (a multiple of 64), one for each y of the grid; 0: K
   int64_t lda, ldb;   // elements
   int64_t M;
   int N;              // columns (GATED: of each half)
   int64_t ldc;
   void* c;            // bf16, or f32 with c_f32
-  int c_f32;
+  int c_f32;          // (with runs of K: 1, their sums one after the other, M ldc apart)
   int act;            // GATED
   uint8_t* saved;     // GATED: up act'(gate) and act(gate) for the backward (nullable); DH: the same, read
   uint16_t* c2;       // DH: the up half's gradient
@@ -74,6 +75,15 @@ __device__ __forceinline__ void static_for(Fn&& f) {
     f(std::integral_constant<int, I0>{});
     static_for<I0 + 1, N>(f);
   }
+}
+
+// 16 bytes at a uniform address plus a 32-bit offset, zeros without an access where the offset has
+// bit 31: no branch around the load, so that later ones need not wait for it.
+constexpr uint32_t NOWHERE = 0x80000000u;
+__device__ __forceinline__ bf16x8_t load16(const void* base, uint32_t off) {
+  return __builtin_bit_cast(bf16x8_t, __builtin_amdgcn_raw_buffer_load_b128(
+                                          __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), 0, 0x7fffffff, 0x00020000),
+                                          off, 0, 0));
 }
 
 typedef short tr4_t __attribute__((ext_vector_type(4)));
@@ -192,63 +202,84 @@ __device__ __forceinline__ void finish(const Args& g, f32x4_t (&acc)[2][2][BM / 
   constexpr int QA = BM / 64, QB = BN / 64, WC = BN / 4;
   const int l16 = lane & 15, lq = lane >> 4;
   if constexpr (ADAPT) {
-    // Each adapter of the tile: its product with the rows that have it, 32 ranks at a time.  Where all
+    // Each adapter of the tile: its product with the rows' inner products, 32 ranks at a time.  Where all
     // 16 rows of a block have it, the sums go on; in a block of several it is computed for all and
     // added, by selection, to the rows that have it: a sum over masked operands would carry a NaN or
-    // an infinity of one request's adapter into the others' rows.
-#pragma unroll 1
-    for (int a = 0; a < n_list; ++a) {
-      const int id = __builtin_amdgcn_readfirstlane(list[a]);
-      uint32_t some = 0, all = 0;  // blocks x QA + i with a row of it, with no other
+    // an infinity of one request's adapter into the others' rows.  Bound by the latency of the
+    // factors' reads, so they run D adapters ahead (64 to 512 rows with 16 adapters in turn, rank 16,
+    // F 5632: one at a time 25 to 50 us more than without adapters).
+    constexpr int H = GATED ? 2 : 1, D = QB >= 4 ? 2 : 4;
+    int own[2 * QA];
 #pragma unroll
-      for (int b = 0; b < 2 * QA; ++b) {
-        const uint64_t mine = __ballot(sid[(b / QA) * (BM / 2) + wm * (BM / 4) + (b % QA) * 16 + l16] == id);
-        some |= (mine != 0) << b, all |= (mine == ~0ull) << b;
-      }
-      some = __builtin_amdgcn_readfirstlane(some), all = __builtin_amdgcn_readfirstlane(all);
-      if (!some) continue;
+    for (int b = 0; b < 2 * QA; ++b) own[b] = sid[(b / QA) * (BM / 2) + wm * (BM / 4) + (b % QA) * 16 + l16];
+    const bool has[2] = {g.ad.b[0] != nullptr, !GATED || g.ad.b[1] != nullptr};
+    if (n_list)
 #pragma unroll 1
-      for (int s = 0; s < g.ad.r; s += 32) {
-        const int k = s + 8 * lq;
-        const bool in = k < g.ad.r;
-        static_for<0, 2>([&](auto yt) {
-          constexpr int y = decltype(yt)::value, h = GATED ? y : 0;
-          const uint16_t *b = g.ad.b[h], *v = g.ad.v[h];
-          if (!b) return;
-          bf16x8_t fb[QB];
+    for (int s = 0; s < g.ad.r; s += 32) {
+      const int k = s + 8 * lq;
+      const bool in = k < g.ad.r;
+      bf16x8_t fv[H][2 * QA], fb[D][2][QB];
+      auto load = [&](int set, int a) {
+        const int id = __builtin_amdgcn_readfirstlane(list[a < n_list ? a : n_list - 1]);
+#pragma unroll
+        for (int y = 0; y < 2; ++y)
 #pragma unroll
           for (int j = 0; j < QB; ++j) {
+            // (columns past the end are not stored)
             const int n = n0 + (GATED ? 0 : y * (BN / 2)) + wn * WC + j * 16 + l16;
-            fb[j] = bf16x8_t{};
-            if (in && n < g.N) fb[j] = *reinterpret_cast<const bf16x8_t*>(b + ((int64_t)id * g.N + n) * g.ad.r + k);
+            fb[set][y][j] = load16(g.ad.b[GATED ? y : 0] + (int64_t)id * g.N * g.ad.r,
+                                   in && n < g.N && has[y] ? (uint32_t)(n * g.ad.r + k) * 2 : NOWHERE);
           }
-          static_for<0, 2 * QA>([&](auto xt) {
-            constexpr int blk = decltype(xt)::value, x = blk / QA, i = blk % QA;
-            const int tr = x * (BM / 2) + wm * (BM / 4) + i * 16 + l16;
-            const bool mine = sid[tr] == id;
-            bf16x8_t fv = {};
-            if (in && mine) fv = *reinterpret_cast<const bf16x8_t*>(v + (m0 + tr) * g.ad.r + k);
+      };
+#pragma unroll
+      for (int d = 0; d < D; ++d) load(d, d);
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int b = 0; b < 2 * QA; ++b) {
+          const int tr = (b / QA) * (BM / 2) + wm * (BM / 4) + (b % QA) * 16 + l16;
+          fv[h][b] = load16(g.ad.v[h] + m0 * g.ad.r, in && own[b] >= 0 && has[h] ? (uint32_t)(tr * g.ad.r + k) * 2 : NOWHERE);
+        }
+#pragma unroll 1
+      for (int a0 = 0; a0 < n_list; a0 += D)
+        static_for<0, D>([&](auto dt) {
+          constexpr int d = decltype(dt)::value;
+          const int id = a0 + d < n_list ? list[a0 + d] : -2;
+          static_for<0, 2 * QA>([&](auto bt) {
+            constexpr int blk = decltype(bt)::value, x = blk / QA, i = blk % QA;
+            const bool mine = own[blk] == id;
+            const uint64_t rows = __ballot(mine);
             // (after each branch the sums are back in their accumulation registers, block by block)
-            if (all >> blk & 1) {
+            if (rows == ~0ull) {
 #pragma unroll
-              for (int j = 0; j < QB; ++j)
-                acc[x][y][i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fv, acc[x][y][i][j], 0, 0, 0);
+              for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int j = 0; j < QB; ++j)
+                  acc[x][y][i][j] =
+                      __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[d][y][j], fv[GATED ? y : 0][blk], acc[x][y][i][j], 0, 0, 0);
             }
 #pragma unroll
-            for (int j = 0; j < QB; ++j) asm volatile("" : "+a"(acc[x][y][i][j]));
-            if ((some & ~all) >> blk & 1) {
+            for (int y = 0; y < 2; ++y)
 #pragma unroll
-              for (int j = 0; j < QB; ++j) {
-                const f32x4_t d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fv, f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+              for (int j = 0; j < QB; ++j) asm volatile("" : "+a"(acc[x][y][i][j]));
+            if (rows != 0 && rows != ~0ull) {
 #pragma unroll
-                for (int t = 0; t < 4; ++t) acc[x][y][i][j][t] += mine ? d[t] : 0.0f;
-              }
+              for (int y = 0; y < 2; ++y)
+#pragma unroll
+                for (int j = 0; j < QB; ++j) {
+                  const f32x4_t p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[d][y][j], fv[GATED ? y : 0][blk],
+                                                                           f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
+#pragma unroll
+                  for (int t = 0; t < 4; ++t) acc[x][y][i][j][t] += mine ? p[t] : 0.0f;
+                }
             }
 #pragma unroll
-            for (int j = 0; j < QB; ++j) asm volatile("" : "+a"(acc[x][y][i][j]));
+            for (int y = 0; y < 2; ++y)
+#pragma unroll
+              for (int j = 0; j < QB; ++j) asm volatile("" : "+a"(acc[x][y][i][j]));
           });
+          load(d, a0 + d + D);
         });
-      }
     }
   }
   auto rows = [&](auto&& f) {  // f(x, i, m) for this lane's rows
@@ -319,14 +350,15 @@ __device__ __forceinline__ void finish(const Args& g, f32x4_t (&acc)[2][2][BM / 
 // ---------------------------------------------------------------- the tile kernel
 template <int R, bool STRIDED, int KS>
 struct Loads {  // of one operand's stage tile (R rows or columns, 32 KS of K): this lane's pieces
-  static constexpr int BYTES = R * 64 * KS;  // of the stage tile, either layout
+  static constexpr int P = STRIDED && R == 192 ? 256 : R;  // (rows of 384 bytes take 512: the swizzle is for powers of two)
+  static constexpr int BYTES = P * 64 * KS;  // of the stage tile, either layout
   static constexpr int N = BYTES / 4096;     // 1 KiB pieces of a wave
-  static constexpr int CPR = STRIDED ? R / 8 : 4 * KS;  // 16-byte chunks of a row
+  static constexpr int CPR = STRIDED ? P / 8 : 4 * KS;  // 16-byte chunks of a row
   uint32_t off[N];  // bytes from the first row (column) of the tile, or for split of its half
   int kpos;         // first K of the first piece's chunk
 
-  // rows: how many of the tile's R exist, at least one (what is past them repeats others: it is not
-  // stored); split: its halves are the same R / 2 rows of two matrices
+  // rows: how many of the tile's R exist (what is past them reads as zeros, for nothing: a tile of few
+  // rows costs the other operand's bytes); split: its halves are the same R / 2 rows of two matrices
   __device__ __forceinline__ void init(int64_t ld, int64_t rows, bool split, int wave, int lane) {
 #pragma unroll
     for (int q = 0; q < N; ++q) {
@@ -334,26 +366,21 @@ struct Loads {  // of one operand's stage tile (R rows or columns, 32 KS of K): 
       if constexpr (!STRIDED) {
         // (rows of a lane's pieces are multiples of 32 apart: the same chunk of K)
         const int chunk = (lane % CPR) ^ ((row >> 1) & (CPR - 1));
-        const int64_t want = split ? row & (R / 2 - 1) : row, r = want < rows ? want : rows - 1;
-        off[q] = (uint32_t)(r * ld * 2) + chunk * 16;
+        const int r = split ? row % (R / 2) : row;
+        off[q] = r < rows ? (uint32_t)(r * ld * 2) + chunk * 16 : NOWHERE;
         if (q == 0) kpos = chunk * 8;
       } else {
-        const int chunk = (lane % CPR) ^ (strided_swz<2 * R>(row) << 1);
-        off[q] = (uint32_t)(row * ld * 2) + (chunk * 8 < rows ? chunk * 16 : 0);
+        const int chunk = (lane % CPR) ^ (strided_swz<2 * P>(row) << 1);
+        off[q] = chunk * 8 < (rows < R ? rows : R) ? (uint32_t)(row * ld * 2) + chunk * 16 : NOWHERE;
         if (q == 0) kpos = row;
       }
     }
   }
-  // with `left` of K to go, what is past its end gets an offset that reads as zero: a bit that the
-  // others do not have
+  // with `left` of K to go, what is past its end reads as zeros
   __device__ __forceinline__ void cut(int left) {
 #pragma unroll
     for (int q = 0; q < N; ++q)
-      if (kpos + (STRIDED ? 4 * q * (64 / CPR) : 0) >= left) off[q] |= 0x80000000u;
-  }
-  __device__ __forceinline__ void uncut() {
-#pragma unroll
-    for (int q = 0; q < N; ++q) off[q] &= 0x7fffffffu;
+      if (kpos + (STRIDED ? 4 * q * (64 / CPR) : 0) >= left) off[q] |= NOWHERE;
   }
 };
 
@@ -376,8 +403,9 @@ __device__ __forceinline__ void dma16_at(const void* base, uint32_t off) {
 template <int R, bool STRIDED, int KS>
 struct Frags {
   static constexpr int Q = R / 64;
+  static constexpr int P = Loads<R, STRIDED, KS>::P;
   // K-contiguous: the swizzle repeats every 16 rows, a block only adds to the address.  Strided: a
-  // block's number is XOR-ed into bits from 5 on, which in a 512-byte row is for the halves an addition.
+  // block's number is XOR-ed into bits from 5 on, which for the halves of 256 columns is an addition.
   static constexpr int PLACES = !STRIDED ? 1 : R == 256 ? Q : 2 * Q;
   uint32_t place[PLACES];
 
@@ -387,11 +415,10 @@ struct Frags {
       place[0] = row * 64 * KS + (((lane >> 4) ^ ((row >> 1) & (4 * KS - 1))) << 4);
     } else {
       const int i16 = lane & 15, row = 8 * (lane >> 4) + (i16 >> 2);
-      const uint32_t first = row * 2 * R + (((w * (R / 64)) ^ strided_swz<2 * R>(row)) << 5) + (i16 & 3) * 8;
 #pragma unroll
       for (int i = 0; i < PLACES; ++i) {
-        const int block = R == 256 ? i : (i / Q) * (R / 32) + i % Q;
-        place[i] = first ^ (block << 5);
+        const int block = (i / Q) * (R / 32) + w * Q + i % Q;
+        place[i] = row * 2 * P + ((block ^ strided_swz<2 * P>(row)) << 5) + (i16 & 3) * 8;
       }
     }
   }
@@ -404,9 +431,9 @@ struct Frags {
       return *(const KMOE_LDS bf16x8_t*)(at + ((b / Q) * (R / 2) + (b % Q) * 16) * 64 * KS);
     } else {
       const KMOE_LDS uint8_t* at = tile + (R == 256 ? place[b % Q] : place[b]);
-      const int c = (R == 256 ? (b / Q) * 256 : 0) + ks * 64 * R;
+      const int c = (R == 256 ? (b / Q) * 256 : 0) + ks * 64 * P;
       const tr4_t lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((KMOE_LDS tr4_t*)(at + c));
-      const tr4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((KMOE_LDS tr4_t*)(at + c + 8 * R));
+      const tr4_t hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((KMOE_LDS tr4_t*)(at + c + 8 * P));
       return __builtin_bit_cast(bf16x8_t, (short __attribute__((ext_vector_type(8)))){lo[0], lo[1], lo[2], lo[3], hi[0],
                                                                                      hi[1], hi[2], hi[3]});
     }
@@ -415,7 +442,7 @@ struct Frags {
 
 // Waves of a SIMD that the tile leaves room for.
 template <int BM, int BN, int KS, int STAGES>
-constexpr int side_by_side = (BM * BN == 256 * 256 || (BM + BN) * 64 * KS * STAGES > 78 * 1024) ? 1 : 2;
+constexpr int side_by_side = (BM * BN > 128 * 256 || (BM + BN) * 64 * KS * STAGES > 78 * 1024) ? 1 : 2;
 
 template <int BM, int BN, int KS, int STAGES, bool SA, bool SB, int EPI, bool ADAPT>
 __global__ __launch_bounds__(THREADS, (side_by_side<BM, BN, KS, STAGES>)) __attribute__((
@@ -428,6 +455,7 @@ __global__ __launch_bounds__(THREADS, (side_by_side<BM, BN, KS, STAGES>)) __attr
   constexpr int SK = 32 * KS;
   using LoadA = Loads<BM, SA, KS>;
   using LoadB = Loads<BN, SB, KS>;
+  static_assert(!GATED || LoadB::N % 2 == 0, "a wave's loads are of one half");
   constexpr int QA = BM / 64, QB = BN / 64;          // 16 x 16 blocks of a wave in a half
   constexpr int TILE = LoadA::BYTES, STAGE = TILE + LoadB::BYTES;
   constexpr int NP = LoadA::N + LoadB::N;            // loads of a wave and step
@@ -454,6 +482,13 @@ __global__ __launch_bounds__(THREADS, (side_by_side<BM, BN, KS, STAGES>)) __attr
   const uint16_t* pb = g.b[0] + n0 * row_b;
   const int64_t second = GATED ? g.b[1] - g.b[0] : 0;  // from the gate's to the up projection's rows
   int left = g.K, part = 1, to = 0;
+  if (g.k_run) {
+    const int k0 = blockIdx.y * g.k_run;
+    left = g.K - k0 < g.k_run ? g.K - k0 : g.k_run;
+    pa += SA ? k0 * g.lda : k0, pb += SB ? k0 * g.ldb : k0;
+    g.c = static_cast<float*>(g.c) + blockIdx.y * g.M * g.ldc;
+    if (blockIdx.y) g.ad.n = 0;  // (adapters: the first run's)
+  }
   // piece q of the step to load, A's before B's
   auto place_piece = [&](int q) {
     return ldsp + to * STAGE + (q < LoadA::N ? wave + 4 * q : TILE / 1024 + wave + 4 * (q - LoadA::N)) * 1024;
@@ -474,11 +509,13 @@ __global__ __launch_bounds__(THREADS, (side_by_side<BM, BN, KS, STAGES>)) __attr
         left = g.K, part = 2;
         pa = g.a[1] + m0 * row_a;
         pb = g.b[1] + n0 * row_b;
-        la.uncut(), lb.uncut();
+        la.init(g.lda, g.M - m0, false, wave, lane);
+        lb.init(g.ldb, g.N - n0, GATED, wave, lane);
       }
       if (left < SK) la.cut(left), lb.cut(left);
     }
   };
+  const int nk = (left + SK - 1) / SK * PARTS;
   if (left < SK) la.cut(left), lb.cut(left);
 
   f32x4_t acc[2][2][QA][QB];
@@ -502,7 +539,7 @@ __global__ __launch_bounds__(THREADS, (side_by_side<BM, BN, KS, STAGES>)) __attr
     else
       fa[set][r - 2 * QB] = ra.read(st, r - 2 * QB, ks);
   };
-  const int nk = (g.K + SK - 1) / SK * PARTS;
+
 #pragma unroll 1
   for (int s = 0; s < STAGES; ++s) {
 #pragma unroll

@@ -14,6 +14,51 @@ int launch_dx(const Args& g, hipStream_t s);            // a b
 int launch_dx_two(const Args& g, hipStream_t s);        // a0 b0 + a1 b1
 int launch_dx_adapt(const Args& g, hipStream_t s);
 int launch_wgrad(const Args& g, hipStream_t s);         // a^T b
+// a b^T of few rows in runs of K (kmoe_ffn.hip)
+int launch_linear_runs(const Args& g, hipStream_t s);
+int launch_linear_runs_adapt(const Args& g, hipStream_t s);
+// out = the sum of `runs` arrays of `total` f32 in their order, as bf16
+int launch_sum_runs(const float* part, int runs, int64_t total, uint16_t* out, hipStream_t s);
+
+// The tile, by the time that each would take: rounds of workgroups over the compute units, a round's
+// time for 64 of K with every place taken and with one workgroup a unit, and what a round costs
+// besides (us; from the down product of 16384 to 48 rows, d 2048, F 5632, and the others of these sizes).
+// 256 x 256 and 192 x 256 lie alone on a unit, a fuller chip clocks lower; 128 x 128 two side by side, or
+// one with twice the stages; 64 x 128 and 64 x 64 two side by side.  Measured, us:
+//                        256x256 192x256 128x128 128x128/4  64x128  64x64
+//   16384 rows, gate up    664     690     784       886      981
+//   16384 rows, down       291     350     358       421      494
+//    2042 rows, gate up    100      89     100       117      127
+//    2042 rows, down       103      89      67        49       59
+//     777 rows, gate up     49      41      53        55       53
+//     777 rows, down        99      85      56        40       31
+//     128 rows, gate up     39      33      23        23       19       21
+//      48 rows, gate up     37      31      22        18       18       13
+enum Tile { T256, T192, T128, T128_DEEP, T64X128, T64 };
+inline Tile choose_tile(int64_t M, int64_t cols, double steps, double* us = nullptr) {
+  struct Rate {
+    int bm, bn, side;
+    double full, few, besides;
+  };
+  constexpr Rate rates[] = {{256, 256, 1, 1.63, 1.25, 7.0}, {192, 256, 1, 1.27, 1.05, 6.0}, {128, 128, 2, 1.08, 0.62, 3.0},
+                            {128, 128, 1, 0.57, 0.57, 3.0}, {64, 128, 2, 0.72, 0.42, 2.5},  {64, 64, 2, 0.50, 0.33, 2.0}};
+  const int64_t cus = kmoe::cu_count();
+  int best = 0;
+  double least = 0;
+  for (int i = 0; i < 6; ++i) {
+    const Rate& r = rates[i];
+    const int64_t tiles = kmoe::ceil_div<int64_t>(M, r.bm) * kmoe::ceil_div<int64_t>(cols, r.bn);
+    const int64_t rounds = tiles / (cus * r.side), rest = tiles - rounds * cus * r.side;
+    double t = rounds * (r.full * steps + r.besides);
+    if (rest > cus)
+      t += r.full * steps + r.besides;
+    else if (rest > 0)
+      t += (r.side == 1 ? r.few + (r.full - r.few) * rest / cus : r.few) * steps + r.besides;
+    if (i == 0 || t < least) best = i, least = t;
+  }
+  if (us) *us = least;
+  return (Tile)best;
+}
 
 template <int BM, int BN, int KS, int STAGES, bool SA, bool SB, int EPI, bool ADAPT>
 int launch_tile(const Args& g, hipStream_t s) {
@@ -21,43 +66,29 @@ int launch_tile(const Args& g, hipStream_t s) {
   const int64_t n_mt = kmoe::ceil_div<int64_t>(g.M, BM), n_nt = kmoe::ceil_div(g.N, CN);
   KMOE_REQUIRE(n_mt * n_nt < (int64_t)1 << 31, KMOE_ERR_SHAPE, "kmoe dense product: %lld x %d results in one call",
                (long long)g.M, g.N);
-  // (a tile's 32-bit offsets: 256 rows of a K-contiguous operand, 64 of a K-strided one)
+  // (a tile's 32-bit offsets: 256 rows of a K-contiguous operand, 64 of a K-strided one, an adapter's rows)
   KMOE_REQUIRE(g.lda < (int64_t)1 << 22 && g.ldb < (int64_t)1 << 22, KMOE_ERR_SHAPE,
                "kmoe dense product: rows of %lld and %lld values (below 2^22)", (long long)g.lda, (long long)g.ldb);
-  hipLaunchKernelGGL((dense_kernel<BM, BN, KS, STAGES, SA, SB, EPI, ADAPT>), dim3((unsigned)(n_mt * n_nt)), dim3(THREADS), 0,
-                     s, g, (int)n_mt, (int)n_nt);
+  KMOE_REQUIRE(!ADAPT || (int64_t)g.N * g.ad.r < (int64_t)1 << 30, KMOE_ERR_SHAPE,
+               "kmoe dense product: adapters of %d x %d values (below 2^30)", g.N, g.ad.r);
+  const int runs = g.k_run ? kmoe::ceil_div(g.K, g.k_run) : 1;
+  hipLaunchKernelGGL((dense_kernel<BM, BN, KS, STAGES, SA, SB, EPI, ADAPT>), dim3((unsigned)(n_mt * n_nt), runs),
+                     dim3(THREADS), 0, s, g, (int)n_mt, (int)n_nt);
   return kmoe::check_launch("kmoe dense product");
 }
 
-// The tile, by the time that each would take: rounds of workgroups over the compute units, a round's
-// time for 64 of K with every place taken and with one workgroup a unit, and what a round costs
-// besides (us, down product of 16384 to 200 rows, d 2048, F 5632: 256 x 256 alone on a unit 1.69, 1.15 where
-// few are and the chip clocks higher; 128 x 128 two side by side 1.08, one 0.65; the same with
-// twice the stages, alone, 0.59; 64 x 128 two side by side 0.70, one 0.36).  So 16384 rows take the
-// large tile (297 us; 381, 414, 495 with the others), 2042 the third (51; 103, 66, 59), 777 the fourth
-// (30; 98, 55, 40).
 template <bool SA, bool SB, int EPI, bool ADAPT = false>
 int launch_any(const Args& g, hipStream_t s) {
-  const int cus = kmoe::cu_count();
-  const int64_t cols = (int64_t)g.N * (EPI == EPI_GATED ? 2 : 1);
   const double steps = (double)kmoe::ceil_div(g.K, 64) * (EPI == EPI_TWO ? 2 : 1);
-  auto cost = [&](int bm, int bn, int side, double full, double few, double besides) {
-    const int64_t tiles = kmoe::ceil_div<int64_t>(g.M, bm) * kmoe::ceil_div<int64_t>(cols, bn);
-    const int64_t rounds = tiles / (cus * side), rest = tiles - rounds * cus * side;
-    double t = rounds * (full * steps + besides);
-    if (rest > cus)
-      t += full * steps + besides;
-    else if (rest > 0)
-      t += (side == 1 ? few + (full - few) * rest / cus : few) * steps + besides;
-    return t;
-  };
-  const double big = cost(256, 256, 1, 1.69, 1.15, 7.0), two = cost(128, 128, 2, 1.08, 0.65, 3.0);
-  const double deep = cost(128, 128, 1, 0.59, 0.44, 3.0), small = cost(64, 128, 2, 0.70, 0.36, 2.5);
-  if (big <= two && big <= deep && big <= small) return launch_tile<256, 256, 2, 2, SA, SB, EPI, ADAPT>(g, s);
-  // (weight gradients: steps of 32 of K lie as well, and two more stages fit; 2042 rows 57 against 61 us)
-  if (two <= deep && two <= small) return launch_tile<128, 128, SA ? 1 : 2, SA ? 4 : 2, SA, SB, EPI, ADAPT>(g, s);
-  if (deep <= small) return launch_tile<128, 128, 2, 4, SA, SB, EPI, ADAPT>(g, s);
-  return launch_tile<64, 128, 2, 3, SA, SB, EPI, ADAPT>(g, s);
+  switch (choose_tile(g.M, (int64_t)g.N * (EPI == EPI_GATED ? 2 : 1), steps)) {
+    case T256: return launch_tile<256, 256, 2, 2, SA, SB, EPI, ADAPT>(g, s);
+    case T192: return launch_tile<192, 256, 2, 2, SA, SB, EPI, ADAPT>(g, s);
+    // (weight gradients: steps of 32 of K lie as well, and two more stages fit; 2042 rows 57 against 61 us)
+    case T128: return launch_tile<128, 128, SA ? 1 : 2, SA ? 4 : 2, SA, SB, EPI, ADAPT>(g, s);
+    case T128_DEEP: return launch_tile<128, 128, 2, 4, SA, SB, EPI, ADAPT>(g, s);
+    case T64X128: return launch_tile<64, 128, 2, 3, SA, SB, EPI, ADAPT>(g, s);
+    default: return launch_tile<64, 64, 2, 4, SA, SB, EPI, ADAPT>(g, s);
+  }
 }
 
 }  // namespace kmoe_dense

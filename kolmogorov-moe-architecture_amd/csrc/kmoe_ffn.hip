@@ -1,140 +1,110 @@
 // The gated feed-forward block and adapted projections without gradients in one native call, and
-// the products of few rows, which stream the weights once.
+// the projection of few rows, which streams the weights once.
 #include "kmoe_dense_launch.h"
+#include "kmoe_few.h"
 
 using namespace kmoe_dense;
 
 namespace {
 
 // ---------------------------------------------------------------- few rows
-// A workgroup takes 16 weight rows (GATED: 16 gate and the same 16 up rows) and all T <= 64 rows of
-// x; its waves share K, 64 at a time, each lane reading 16 bytes of a weight row and of an x row
-// straight into the MFMA's operands: every weight byte is read once, by one wave, two 64-byte
-// halves of a line one after the other.  The waves' sums meet in LDS.  Bound by the weights'
-// bytes, and below some 10 MB by latency.  Adapters are added by the lanes that hold the results,
-// rank by rank in f32 (few rows: their factors are read once, like the weights).
-constexpr int FEW = 64;
+// y = x w^T of T <= 16 rows.  A workgroup takes ROWS weight rows and all of x; its W waves share K and
+// their sums meet in LDS.  Bound by the weights' bytes, and below some 10 MB by latency (one row,
+// weights from HBM: 5632 x 2048 9.7 us, 2048 x 5632 8.2; the gate and up rows of the block are
+// enough for the tiles of 64 x 64, 11.7 against 14.1 us).  An adapter is added in f32: a thread sums
+// all ranks of one result, its factors on their way with the first weights.
+constexpr int FEW = 16;
 
-template <int TB, int W, bool GATED, bool ADAPT>
-__global__ __launch_bounds__(W * 64) void few_kernel(Args g) {
-  constexpr int G = GATED ? 2 : 1;
-  __shared__ f32x4_t part[W][G][TB][64];
+template <int ROWS, bool ADAPT>
+__global__ __launch_bounds__(512) void few_kernel(Args g) {
+  constexpr int W = 8, D = 4;
+  __shared__ f32x4_t part[W][64];
+  __shared__ float extra[16][ADAPT ? 17 : 1];  // [row of x][weight row]
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, lq = lane >> 4;
-  const int n0 = blockIdx.x * 16;
-  const int wrow = n0 + l16 < g.N ? n0 + l16 : g.N - 1;
-  const uint16_t* wp[G];
-#pragma unroll
-  for (int y = 0; y < G; ++y) wp[y] = g.b[y] + (int64_t)wrow * g.ldb;
-  const uint16_t* xp[TB];
-#pragma unroll
-  for (int b = 0; b < TB; ++b) {
-    const int64_t t = b * 16 + l16 < g.M ? b * 16 + l16 : g.M - 1;
-    xp[b] = g.a[0] + t * g.lda;
-  }
-  f32x4_t acc[G][TB];
-#pragma unroll
-  for (int y = 0; y < G; ++y)
-#pragma unroll
-    for (int b = 0; b < TB; ++b) acc[y][b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
-  auto step = [&](int k, bool in) {
-    bf16x8_t fw[G], fx[TB];
-#pragma unroll
-    for (int y = 0; y < G; ++y) {
-      fw[y] = *reinterpret_cast<const bf16x8_t*>(wp[y] + (in ? k : 0));
-      if (!in) fw[y] = bf16x8_t{};
-    }
-#pragma unroll
-    for (int b = 0; b < TB; ++b) {
-      fx[b] = *reinterpret_cast<const bf16x8_t*>(xp[b] + (in ? k : 0));
-      if (!in) fx[b] = bf16x8_t{};
-    }
-#pragma unroll
-    for (int y = 0; y < G; ++y)
-#pragma unroll
-      for (int b = 0; b < TB; ++b) acc[y][b] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fw[y], fx[b], acc[y][b], 0, 0, 0);
-  };
-  const int full = g.K & ~63;
-#pragma unroll 4
-  for (int k0 = wave * 64; k0 < full; k0 += W * 64) {
-    step(k0 + 8 * lq, true);
-    step(k0 + 32 + 8 * lq, true);
-  }
-  if (full < g.K && (full / 64) % W == wave) {
-    step(full + 8 * lq, full + 8 * lq < g.K);
-    step(full + 32 + 8 * lq, full + 32 + 8 * lq < g.K);
-  }
-#pragma unroll
-  for (int y = 0; y < G; ++y)
-#pragma unroll
-    for (int b = 0; b < TB; ++b) part[wave][y][b][lane] = acc[y][b];
-  __syncthreads();
-  // thread: row 16 (tid / 64) + l % 16, columns n0 + 4 (l / 16) .. + 3
-  if (tid >= TB * 64) return;
-  const int64_t t = wave * 16 + l16;
-  const int n = n0 + 4 * lq;
-  if (t >= g.M || n >= g.N) return;
-  f32x4_t s[G];
-#pragma unroll
-  for (int y = 0; y < G; ++y) {
-    s[y] = part[0][y][wave][lane];
-#pragma unroll
-    for (int w = 1; w < W; ++w) s[y] += part[w][y][wave][lane];
-  }
+  const int n0 = blockIdx.x * ROWS;
+  const int at = tid & 15, an = tid >> 4;
+  int id = -1;
+  if (ADAPT && at < g.M && an < ROWS && n0 + an < g.N) id = g.ad.ids[at];
+  const void* const w[1] = {g.b[0] + (int64_t)n0 * g.ldb};
+  const uint32_t woff[1] = {l16 < ROWS && n0 + l16 < g.N ? (uint32_t)(l16 * g.ldb) * 2 : NOWHERE};
+  const uint32_t xoff = l16 < g.M ? (uint32_t)(l16 * g.lda) * 2 : NOWHERE;
+  f32x4_t acc[1] = {f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
+  bf16x8_t fw[D][2][1], fx[D][2];
+  stream16<1, W, D>(w, woff, g.a[0], xoff, g.K, wave, lane, acc, false, fw, fx);
   if constexpr (ADAPT) {
-    const int id = g.ad.ids[t];
+    float sum = 0.0f;
     if ((unsigned)id < (unsigned)g.ad.n) {
+      const uint16_t* const b = g.ad.b[0] + ((int64_t)id * g.N + n0 + an) * g.ad.r;
+      const uint16_t* const v = g.ad.v[0] + at * g.ad.r;
+      for (int s = 0; s < g.ad.r; s += 32) {
+        i32x4_t bv[4], vv[4];
 #pragma unroll
-      for (int y = 0; y < G; ++y) {
-        if (!g.ad.b[y]) continue;
-        const uint16_t* const b = g.ad.b[y] + ((int64_t)id * g.N + n) * g.ad.r;
-        const uint16_t* const v = g.ad.v[y] + t * g.ad.r;
-        float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-        for (int j = 0; j < g.ad.r; j += 8) {
-          const i32x4_t vv = *reinterpret_cast<const i32x4_t*>(v + j);
-#pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            const i32x4_t bv = *reinterpret_cast<const i32x4_t*>(b + c * g.ad.r + j);
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              d[c] += __uint_as_float((uint32_t)vv[q] << 16) * __uint_as_float((uint32_t)bv[q] << 16) +
-                      __uint_as_float((uint32_t)vv[q] & 0xffff0000u) * __uint_as_float((uint32_t)bv[q] & 0xffff0000u);
-          }
+        for (int q = 0; q < 4; ++q) {
+          const int j = s + 8 * q < g.ad.r ? s + 8 * q : s;
+          bv[q] = *reinterpret_cast<const i32x4_t*>(b + j);
+          vv[q] = *reinterpret_cast<const i32x4_t*>(v + j);
         }
 #pragma unroll
-        for (int c = 0; c < 4; ++c) s[y][c] += d[c];
+        for (int q = 0; q < 4; ++q) {
+          if (s + 8 * q >= g.ad.r) break;
+#pragma unroll
+          for (int c = 0; c < 4; ++c)
+            sum += __uint_as_float((uint32_t)bv[q][c] << 16) * __uint_as_float((uint32_t)vv[q][c] << 16) +
+                   __uint_as_float((uint32_t)bv[q][c] & 0xffff0000u) * __uint_as_float((uint32_t)vv[q][c] & 0xffff0000u);
+        }
       }
     }
+    if (an < 16) extra[at][an] = sum;
   }
-  float o[4];
-  if constexpr (GATED) {
-    with_act(g.act, [&](auto tag) {
+  stream16<1, W, D>(w, woff, g.a[0], xoff, g.K, wave, lane, acc, true, fw, fx);
+  part[wave][lane] = acc[0];
+  __syncthreads();
+  // row l % 16, columns n0 + 4 (l / 16) .. + 3
+  const int n = n0 + 4 * lq;
+  if (wave || l16 >= g.M || 4 * lq >= ROWS || n >= g.N) return;
+  f32x4_t s = part[0][lane];
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float a, da;
-        act_at<decltype(tag)::value>(s[0][c], a, da);
-        o[c] = a * s[G - 1][c];
-      }
-    });
-  } else {
+  for (int k = 1; k < W; ++k) s += part[k][lane];
+  if constexpr (ADAPT) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) o[c] = s[0][c];
+    for (int c = 0; c < 4; ++c) s[c] += extra[l16][4 * lq + c];
   }
-  *reinterpret_cast<i32x2_t*>(static_cast<uint16_t*>(g.c) + t * g.ldc + n) = pack4(o[0], o[1], o[2], o[3]);
+  *reinterpret_cast<i32x2_t*>(static_cast<uint16_t*>(g.c) + l16 * g.ldc + n) = pack4(s[0], s[1], s[2], s[3]);
 }
 
-template <bool GATED, bool ADAPT>
+template <bool ADAPT>
 int launch_few(const Args& g, hipStream_t s) {
-  const dim3 grid((unsigned)kmoe::ceil_div(g.N, 16));
-  constexpr int W = 8;
-  switch (kmoe::ceil_div<int64_t>(g.M, 16)) {
-    case 1: hipLaunchKernelGGL((few_kernel<1, W, GATED, ADAPT>), grid, dim3(W * 64), 0, s, g); break;
-    case 2: hipLaunchKernelGGL((few_kernel<2, W, GATED, ADAPT>), grid, dim3(W * 64), 0, s, g); break;
-    case 3: hipLaunchKernelGGL((few_kernel<3, W, GATED, ADAPT>), grid, dim3(W * 64), 0, s, g); break;
-    default: hipLaunchKernelGGL((few_kernel<4, W, GATED, ADAPT>), grid, dim3(W * 64), 0, s, g);
-  }
+  KMOE_REQUIRE(g.K < 1 << 22, KMOE_ERR_SHAPE, "kmoe product of few rows: rows of %d values (below 2^22)", g.K);
+  // (8 weight rows a workgroup where 16 would leave units idle: 2048 x 5632 8.2 against 9.4 us, 5632 x
+  // 2048 10.6 against 9.7)
+  if (kmoe::ceil_div(g.N, 16) < kmoe::cu_count())
+    hipLaunchKernelGGL((few_kernel<8, ADAPT>), dim3((unsigned)kmoe::ceil_div(g.N, 8)), dim3(512), 0, s, g);
+  else
+    hipLaunchKernelGGL((few_kernel<16, ADAPT>), dim3((unsigned)kmoe::ceil_div(g.N, 16)), dim3(512), 0, s, g);
   return kmoe::check_launch("kmoe product of few rows");
 }
+
+// Runs of K in which a projection of more rows is computed, where its tiles leave units idle: partial
+// sums in f32, summed by a second launch (some 5 us with the partial sums' way).  1: in one.
+int linear_runs(int64_t T, int K, int N) {
+  if (T <= FEW) return 1;
+  const int64_t tiles = kmoe::ceil_div<int64_t>(T, 64) * kmoe::ceil_div(N, 64), cus = kmoe::cu_count();
+  const int steps = kmoe::ceil_div(K, 64);
+  double least;
+  choose_tile(T, N, steps, &least);
+  int64_t best = 1;
+  for (int side = 1; side <= 2; ++side) {
+    int64_t runs = side * cus / tiles;
+    runs = runs < 16 ? runs : 16;
+    runs = runs < steps / 4 ? runs : steps / 4;
+    if (runs < 2) continue;
+    const double us = (tiles * runs > cus ? 0.50 : 0.33) * kmoe::ceil_div<int64_t>(steps, runs) + 2.0 + 5.0;
+    if (us < least) least = us, best = runs;
+  }
+  return (int)best;
+}
+int64_t run_of(int K, int runs) { return kmoe::ceil_div(kmoe::ceil_div(K, 64), runs) * 64; }
 
 const uint16_t* bf(const void* p) { return static_cast<const uint16_t*>(p); }
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -149,21 +119,31 @@ int check_adapter(const char* who, const kmoe_adapter* a, int n) {
   return KMOE_OK;
 }
 
-// y = x w^T with the adapter's outer product, whose inner products v are there.
+size_t runs_bytes(int64_t T, int K, int N) {
+  const int runs = T > 0 && K > 0 && N > 0 ? linear_runs(T, K, N) : 1;
+  return runs > 1 ? piece((int64_t)runs * T * N * 4) : 0;
+}
+
+// y = x w^T with the adapter's outer product, whose inner products v are there; part: runs_bytes.
 int project(const void* x, int64_t T, int K, const void* w, int N, const int32_t* ids, int n, const kmoe_adapter* ad,
-            const void* v, void* y, hipStream_t s) {
-  if (T > FEW)
-    return kmoe_dense_linear(x, T, K, w, N, ad ? ids : nullptr, n, ad ? ad->rank : 0, v, ad ? ad->b : nullptr, y, s);
+            const void* v, void* y, void* part, hipStream_t s) {
   Args g{};
   g.a[0] = bf(x), g.b[0] = bf(w), g.K = K, g.lda = K, g.ldb = K, g.M = T, g.N = N, g.ldc = N, g.c = y;
-  if (!ad) return launch_few<false, false>(g, s);
-  g.ad = {ids, {bf(v), nullptr}, {bf(ad->b), nullptr}, n, ad->rank};
-  return launch_few<false, true>(g, s);
+  if (ad) g.ad = {ids, {bf(v), nullptr}, {bf(ad->b), nullptr}, n, ad->rank};
+  if (T <= FEW) return ad ? launch_few<true>(g, s) : launch_few<false>(g, s);
+  const int runs = linear_runs(T, K, N);
+  if (runs == 1) return ad ? launch_linear_adapt(g, s) : launch_linear(g, s);
+  g.k_run = (int)run_of(K, runs), g.c = part, g.c_f32 = 1;
+  if (const int rc = ad ? launch_linear_runs_adapt(g, s) : launch_linear_runs(g, s)) return rc;
+  return launch_sum_runs(static_cast<const float*>(part), kmoe::ceil_div(K, g.k_run), T * N, static_cast<uint16_t*>(y), s);
 }
 
 }  // namespace
 
-extern "C" size_t kmoe_adapted_linear_workspace_bytes(int64_t T, int rank) { return piece(T * (rank > 0 ? rank : 0) * 2); }
+extern "C" size_t kmoe_adapted_linear_workspace_bytes(int64_t T, int K, int N, int rank) {
+  if (T <= 0) return 0;
+  return piece(T * (rank > 0 ? rank : 0) * 2) + runs_bytes(T, K, N);
+}
 
 extern "C" int kmoe_adapted_linear(const void* x, int64_t T, int K, const void* w, int N, const int32_t* ids, int n_adapters,
                                    const kmoe_adapter* adapter, void* y, void* workspace, size_t workspace_bytes,
@@ -175,19 +155,21 @@ extern "C" int kmoe_adapted_linear(const void* x, int64_t T, int K, const void* 
   KMOE_REQUIRE(x && w && y && (ids || !adapter), KMOE_ERR_NULL, "kmoe_adapted_linear: null buffer");
   KMOE_REQUIRE(aligned(x) && aligned(w) && aligned(y) && aligned(workspace), KMOE_ERR_SHAPE,
                "kmoe_adapted_linear: buffers are aligned to 16 bytes");
+  const size_t need = kmoe_adapted_linear_workspace_bytes(T, K, N, adapter ? adapter->rank : 0);
+  KMOE_REQUIRE((workspace || !need) && workspace_bytes >= need, KMOE_ERR_WORKSPACE,
+               "kmoe_adapted_linear: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
   if (adapter) {
-    KMOE_REQUIRE(workspace && workspace_bytes >= kmoe_adapted_linear_workspace_bytes(T, adapter->rank), KMOE_ERR_WORKSPACE,
-                 "kmoe_adapted_linear: workspace of %zu bytes, %zu are needed", workspace_bytes,
-                 kmoe_adapted_linear_workspace_bytes(T, adapter->rank));
     const int rc = kmoe_adapter_inner(x, T, K, ids, n_adapters, adapter->rank, adapter->a, adapter->scale, workspace, nullptr,
                                       nullptr, nullptr, stream);
     if (rc) return rc;
   }
-  return project(x, T, K, w, N, ids, n_adapters, adapter, workspace, y, kmoe::as_stream(stream));
+  return project(x, T, K, w, N, ids, n_adapters, adapter, workspace, y,
+                 static_cast<uint8_t*>(workspace) + piece(T * (adapter ? adapter->rank : 0) * 2), kmoe::as_stream(stream));
 }
 
-extern "C" size_t kmoe_gated_ffn_workspace_bytes(int64_t T, int F, int rank_gate_up, int rank_down) {
-  return piece(T * F * 2) + 2 * piece(T * rank_gate_up * 2) + piece(T * rank_down * 2);
+extern "C" size_t kmoe_gated_ffn_workspace_bytes(int64_t T, int d, int F, int rank_gate_up, int rank_down) {
+  if (T <= 0) return 0;
+  return piece(T * F * 2) + 2 * piece(T * rank_gate_up * 2) + piece(T * rank_down * 2) + runs_bytes(T, F, d);
 }
 
 extern "C" int kmoe_gated_ffn(const void* x, int64_t T, int d, int F, const void* w_gate, const void* w_up,
@@ -207,14 +189,15 @@ extern "C" int kmoe_gated_ffn(const void* x, int64_t T, int d, int F, const void
   KMOE_REQUIRE(aligned(x) && aligned(w_gate) && aligned(w_up) && aligned(w_down) && aligned(y) && aligned(workspace),
                KMOE_ERR_SHAPE, "kmoe_gated_ffn: buffers are aligned to 16 bytes");
   const int rgu = gate ? gate->rank : up ? up->rank : 0, rd = down ? down->rank : 0;
-  KMOE_REQUIRE(workspace_bytes >= kmoe_gated_ffn_workspace_bytes(T, F, rgu, rd), KMOE_ERR_WORKSPACE,
+  KMOE_REQUIRE(workspace_bytes >= kmoe_gated_ffn_workspace_bytes(T, d, F, rgu, rd), KMOE_ERR_WORKSPACE,
                "kmoe_gated_ffn: workspace of %zu bytes, %zu are needed", workspace_bytes,
-               kmoe_gated_ffn_workspace_bytes(T, F, rgu, rd));
+               kmoe_gated_ffn_workspace_bytes(T, d, F, rgu, rd));
   uint8_t* w = static_cast<uint8_t*>(workspace);
   void* const h = w;
   void* const vg = w += piece(T * F * 2);
   void* const vu = w += piece(T * rgu * 2);
   void* const vd = w += piece(T * rgu * 2);
+  void* const part = w += piece(T * rd * 2);
   hipStream_t s = kmoe::as_stream(stream);
   int rc = KMOE_OK;
   if (rgu) {
@@ -225,22 +208,12 @@ extern "C" int kmoe_gated_ffn(const void* x, int64_t T, int d, int F, const void
                               nullptr, nullptr, nullptr, stream);
     if (rc) return rc;
   }
-  if (T > FEW) {
-    rc = kmoe_dense_gate_up(x, T, d, w_gate, w_up, F, act, rgu ? ids : nullptr, n_adapters, rgu, gate ? vg : nullptr,
-                            gate ? gate->b : nullptr, up ? vu : nullptr, up ? up->b : nullptr, h, nullptr, stream);
-  } else {
-    Args g{};
-    g.a[0] = bf(x), g.b[0] = bf(w_gate), g.b[1] = bf(w_up), g.K = d, g.lda = d, g.ldb = d, g.M = T, g.N = F;
-    g.ldc = F, g.c = h, g.act = act;
-    if (rgu)
-      g.ad = {ids, {gate ? bf(vg) : nullptr, up ? bf(vu) : nullptr}, {gate ? bf(gate->b) : nullptr, up ? bf(up->b) : nullptr},
-              n_adapters, rgu};
-    rc = rgu ? launch_few<true, true>(g, s) : launch_few<true, false>(g, s);
-  }
+  rc = kmoe_dense_gate_up(x, T, d, w_gate, w_up, F, act, rgu ? ids : nullptr, n_adapters, rgu, gate ? vg : nullptr,
+                          gate ? gate->b : nullptr, up ? vu : nullptr, up ? up->b : nullptr, h, nullptr, stream);
   if (rc) return rc;
   if (down) {
     rc = kmoe_adapter_inner(h, T, F, ids, n_adapters, rd, down->a, down->scale, vd, nullptr, nullptr, nullptr, stream);
     if (rc) return rc;
   }
-  return project(h, T, F, w_down, d, ids, n_adapters, down, vd, y, s);
+  return project(h, T, F, w_down, d, ids, n_adapters, down, vd, y, part, s);
 }

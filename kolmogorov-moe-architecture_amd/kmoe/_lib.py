@@ -130,9 +130,9 @@ _SIGNATURES = {
                                _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp, _i32, _vp, _vp, _sz, _vp]),
     "kmoe_gemm_down_mx": (_i32, [_vp, _vp, _i32, _vp, _i32, _i32, _i32, _i64, _vp, _vp, _vp, _vp]),
     # dense products: the gated block, adapters, their backward
-    "kmoe_gated_ffn_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
+    "kmoe_gated_ffn_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32]),
     "kmoe_gated_ffn": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
-    "kmoe_adapted_linear_workspace_bytes": (_sz, [_i64, _i32]),
+    "kmoe_adapted_linear_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
     "kmoe_adapted_linear": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _sz, _vp]),
     "kmoe_adapter_inner": (_i32, [_vp, _i64, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "kmoe_dense_saved_bytes": (_sz, [_i64, _i32]),

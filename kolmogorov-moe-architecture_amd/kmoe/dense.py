@@ -118,8 +118,13 @@ def _aligned(t):
 
 
 @functools.lru_cache(maxsize=1024)
-def _ffn_workspace(T, F, rgu, rd) -> int:
-    return _lib.load().kmoe_gated_ffn_workspace_bytes(T, F, rgu, rd)
+def _ffn_workspace(device, T, d, F, rgu, rd) -> int:
+    return _lib.load().kmoe_gated_ffn_workspace_bytes(T, d, F, rgu, rd)
+
+
+@functools.lru_cache(maxsize=1024)
+def _linear_workspace(device, T, K, N, r) -> int:
+    return _lib.load().kmoe_adapted_linear_workspace_bytes(T, K, N, r)
 
 
 # ---------------------------------------------------------------- without gradients
@@ -132,7 +137,7 @@ def _ffn_forward(x2d, wg, wu, wd, act, ads, ids):
     some = gate or up or down
     rgu = gate.a.shape[1] if gate is not None else up.a.shape[1] if up is not None else 0
     with _device(dev), _Stage("gated_ffn"):
-        wsb = _ffn_workspace(T, F, rgu, down.a.shape[1] if down is not None else 0)
+        wsb = _ffn_workspace(dev.index, T, d, F, rgu, down.a.shape[1] if down is not None else 0)
         ws = torch.empty(max(wsb, 16), device=dev, dtype=torch.uint8)
         _lib.call("kmoe_gated_ffn", ptr(x2d), T, d, F, ptr(wg), ptr(wu), ptr(wd), act, ptr(ids),
                   some.a.shape[0] if some else 0, _struct(gate), _struct(up), _struct(down), ptr(y), ptr(ws), wsb,
@@ -145,7 +150,7 @@ def _linear_forward(x2d, w, ad, ids):
     dev = x2d.device
     y = torch.empty(T, w.shape[0], device=dev, dtype=_BF16)
     with _device(dev), _Stage("adapted_linear"):
-        wsb = _lib.load().kmoe_adapted_linear_workspace_bytes(T, ad.a.shape[1]) if ad is not None else 0
+        wsb = _linear_workspace(dev.index, T, K, w.shape[0], ad.a.shape[1] if ad is not None else 0)
         ws = torch.empty(max(wsb, 16), device=dev, dtype=torch.uint8)
         _lib.call("kmoe_adapted_linear", ptr(x2d), T, K, ptr(w), w.shape[0], ptr(ids), ad.a.shape[0] if ad is not None else 0,
                   _struct(ad), ptr(y), ptr(ws), wsb, _stream(x2d))

@@ -99,7 +99,7 @@ def _call(name, good):
 
 def test_abi_gated_ffn():
     a = _lib.Adapter(0x1000, 0x1000, None, 8)
-    ws = _lib.load().kmoe_gated_ffn_workspace_bytes(100, 72, 8, 8)
+    ws = _lib.load().kmoe_gated_ffn_workspace_bytes(100, 64, 72, 8, 8)
     assert ws >= 100 * 72 * 2 + 3 * 100 * 8 * 2
     call = _call("kmoe_gated_ffn", [FAKE, 100, 64, 72, FAKE, FAKE, FAKE, 0, FAKE, 2, ctypes.byref(a), ctypes.byref(a),
                                     ctypes.byref(a), FAKE, FAKE, ws, None])
@@ -120,7 +120,7 @@ def test_abi_gated_ffn():
 
 def test_abi_adapted_linear():
     a = _lib.Adapter(0x1000, 0x1000, None, 8)
-    ws = _lib.load().kmoe_adapted_linear_workspace_bytes(100, 8)
+    ws = _lib.load().kmoe_adapted_linear_workspace_bytes(100, 64, 72, 8)
     call = _call("kmoe_adapted_linear", [FAKE, 100, 64, FAKE, 72, FAKE, 2, ctypes.byref(a), FAKE, FAKE, ws, None])
     assert call(a1=0) == 0 and call(a10=ws - 1) == -4 and call(a9=None) == -4
     for i in (0, 3, 5, 8):
