@@ -4,7 +4,7 @@
 
 using kmoe_dense::NOWHERE;
 using kmoe_dense::pack4;
-using kmoe_dense::stream16;
+using kmoe_dense::Stream16;
 using kmoe_dense::tr4_t;
 
 namespace {
@@ -43,31 +43,29 @@ __global__ __launch_bounds__(SW * 64) void shrink_kernel(Shrink g) {
   bool first = lane < 16 && id >= 0;
 #pragma unroll
   for (int t = 0; t < 15; ++t) {
-    const int o = __shfl(id, t, 64);
+    const int o = __builtin_amdgcn_readlane(id, t);
     if (t < lane && o == id) first = false;
   }
   uint64_t todo = __ballot(first);
-  const uint16_t* const x = g.x + t0 * g.K;
-  const uint32_t xoff = t0 + l16 < g.T ? (uint32_t)(l16 * g.K) * 2 : NOWHERE;
-  uint32_t aoff[RB];
+  Stream16<RB, SW, D> st;
+  st.x = g.x + t0 * g.K, st.K = g.K;
+  st.xoff = t0 + l16 < g.T ? (uint32_t)(l16 * g.K) * 2 : NOWHERE;
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
     const int j = j0 + b * 16 + l16;
-    aoff[b] = j < g.r ? (uint32_t)(j * g.K) * 2 : NOWHERE;
+    st.woff[b] = j < g.r ? (uint32_t)(j * g.K) * 2 : NOWHERE;
   }
   for (int c = 0; todo; ++c, todo &= todo - 1) {
     if (c % (int)gridDim.y != (int)blockIdx.y) continue;
     const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
-    const void* a[RB];
     f32x4_t acc[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
-      a[b] = g.a[z] + (int64_t)cur * g.r * g.K;
+      st.w[b] = g.a[z] + (int64_t)cur * g.r * g.K;
       acc[b] = f32x4_t{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    bf16x8_t fa[D][2][RB], fx[D][2];
-    stream16<RB, SW, D>(a, aoff, x, xoff, g.K, wave, lane, acc, false, fa, fx);
-    stream16<RB, SW, D>(a, aoff, x, xoff, g.K, wave, lane, acc, true, fa, fx);
+    st.start(wave, lane);
+    st.run(wave, lane, acc);
 #pragma unroll
     for (int b = 0; b < RB; ++b) part[wave][b][lane] = acc[b];
     __syncthreads();

@@ -173,115 +173,199 @@ __device__ __forceinline__ void tile_of(int id, int n_mt, int n_nt, int& mt, int
 }
 
 // Distinct adapters of the tile's rows: list[0 .. *count), in no order (a row has one adapter, so the
-// order does not reach the results).  sid: the rows' ids, -1 without one.
+// order does not reach the results).  sid: the rows' ids, of which those that are no adapter's become
+// -1.  A wave takes 64 rows, one adapter after the other, and leaves out those of the waves before it.
 template <int BM>
-__device__ __forceinline__ void list_adapters(const Adapt& ad, int64_t m0, int64_t M, int tid, int* sid, int* list,
-                                              int* count) {
+__device__ __forceinline__ void list_adapters(int n_adapters, int rows, int tid, int* sid, int* list, int* count) {
   int id = -1;
   if (tid < BM) {
-    if (m0 + tid < M) id = ad.ids[m0 + tid];
-    if ((unsigned)id >= (unsigned)ad.n) id = -1;
+    if (tid < rows) id = sid[tid];
+    if ((unsigned)id >= (unsigned)n_adapters) id = -1;
     sid[tid] = id;
   }
   if (tid == 0) *count = 0;
-  __syncthreads();
-  if (tid < BM && id >= 0 && !(tid > 0 && sid[tid - 1] == id)) {
-    bool first = true;
-    for (int t = 0; t + 1 < tid && first; ++t) first = sid[t] != id;
-    if (first) list[atomicAdd(count, 1)] = id;
+  wait_lgkmcnt0();
+  barrier_nofence();
+  if (tid < BM) {
+    const int wave = tid >> 6, lane = tid & 63;
+    int before[BM / 64];
+#pragma unroll
+    for (int w = 0; w < BM / 64; ++w) before[w] = w < wave ? sid[w * 64 + lane] : -1;
+    int mine = -1, n = 0;  // this wave's n-th adapter is held by lane n
+    for (uint64_t todo = __ballot(id >= 0); todo;) {
+      const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
+      todo &= ~__ballot(id == cur);
+      bool known = false;
+#pragma unroll
+      for (int w = 0; w + 1 < BM / 64; ++w) known |= before[w] == cur;
+      if (__ballot(known)) continue;
+      if (lane == n) mine = cur;
+      ++n;
+    }
+    int at = 0;
+    if (lane == 0 && n) at = atomicAdd(count, n);
+    at = __builtin_amdgcn_readfirstlane(at);
+    if (lane < n) list[at + lane] = mine;
   }
-  __syncthreads();
+  wait_lgkmcnt0();
+  barrier_nofence();
 }
 
-// Adapters and epilogue of a tile: acc[x][y][i][j][t] is row m0 + x BM / 2 + wm BM / 4 + 16 i + l % 16, column
+// The adapters' outer products of a tile.  A turn is an MFMA's 32 of K: 32 ranks of an adapter of the tile's
+// list, or two adapters of 16, or four of 8, each with the rows' inner products where they have it
+// and zeros where not, so the sums go on in their registers.  A zero times an infinity or a NaN of
+// another request's adapter would be a NaN: a turn with such factors is computed one adapter at a
+// time and kept, by selection, for the rows that have it.  Bound by the latency of the factors' reads:
+// those of the next C turns run during these (16 adapters of rank 16 in turn, 48 rows, F 5632, gate
+// and up: 4 us; read and selected turn by turn 25).
+template <int BM, int BN, bool GATED>
+struct Outer {
+  static constexpr int QA = BM / 64, QB = BN / 64, H = GATED ? 2 : 1, C = QB == 1 ? 8 : 1;
+  const Adapt& ad;
+  const int *sid, *list;
+  int n_list;
+  int64_t m0;
+  int n0, N, wm, wn, lane;
+  int per;       // adapters of a turn
+  int slot, k0;  // this lane's adapter of them, and its first rank
+  int turns;     // of 32 ranks
+  int own[2 * QA];
+  bf16x8_t fv[H][2 * QA];
+  bf16x8_t next[C][2 * QB];
+  int next_id[C];
+
+  __device__ __forceinline__ Outer(const Adapt& ad, const int* sid, const int* list, int n_list, int64_t m0, int n0, int N,
+                                   int wm, int wn, int lane)
+      : ad(ad), sid(sid), list(list), n_list(n_list), m0(m0), n0(n0), N(N), wm(wm), wn(wn), lane(lane) {
+    const int lq = lane >> 4;
+    per = ad.r <= 8 ? 4 : ad.r <= 16 ? 2 : 1;
+    slot = per == 4 ? lq : per == 2 ? lq >> 1 : 0;
+    k0 = per == 4 ? 0 : per == 2 ? (lq & 1) * 8 : lq * 8;
+    turns = (n_list + per - 1) / per;
+#pragma unroll
+    for (int b = 0; b < 2 * QA; ++b) own[b] = sid[row(b)];
+  }
+  __device__ __forceinline__ int row(int blk) const {  // of the tile
+    return (blk / QA) * (BM / 2) + wm * (BM / 4) + (blk % QA) * 16 + (lane & 15);
+  }
+  // the factors of turns t .. t + C - 1 from rank s on.  Every address is some adapter's: a lane without
+  // one, or past the ranks, meets zeros of the rows, and columns past the end are not stored.
+  __device__ __forceinline__ void load(int s, int t) {
+    const int k = s + k0 < ad.r ? s + k0 : 0;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+      if (t + c >= turns) break;
+      const int a = (t + c) * per + slot;
+      const int id = list[a < n_list ? a : 0];
+      next_id[c] = a < n_list ? id : -2;
+#pragma unroll
+      for (int yj = 0; yj < 2 * QB; ++yj) {
+        const int n = n0 + (GATED ? 0 : yj / QB * (BN / 2)) + wn * (BN / 4) + yj % QB * 16 + (lane & 15);
+        const uint16_t* const b = GATED && yj >= QB ? ad.b[1] : ad.b[0];
+        next[c][yj] = bf16x8_t{};
+        if (b) next[c][yj] = *reinterpret_cast<const bf16x8_t*>(b + ((int64_t)id * N + (n < N ? n : N - 1)) * ad.r + k);
+      }
+    }
+  }
+  __device__ __forceinline__ void load_rows(int s) {
+#pragma unroll
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int b = 0; b < 2 * QA; ++b) {
+        fv[h][b] = bf16x8_t{};
+        if (s + k0 < ad.r && own[b] >= 0 && ad.b[h])
+          fv[h][b] = *reinterpret_cast<const bf16x8_t*>(ad.v[h] + (m0 + row(b)) * ad.r + s + k0);
+      }
+  }
+  __device__ __forceinline__ void add(f32x4_t (&acc)[2][2][QA][QB]) {
+    load(0, 0);
+#pragma unroll 1
+    for (int s = 0; s < ad.r; s += 32) {
+      load_rows(s);
+#pragma unroll 1
+      for (int t = 0; t < turns; t += C) {
+        bf16x8_t fb[C][2 * QB];
+        int id[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+          id[c] = next_id[c];
+#pragma unroll
+          for (int yj = 0; yj < 2 * QB; ++yj) fb[c][yj] = next[c][yj];
+        }
+        if (t + C < turns)
+          load(s, t + C);
+        else if (s + 32 < ad.r)
+          load(s + 32, 0);
+        static_for<0, C>([&](auto ct) {
+          constexpr int c = decltype(ct)::value;
+          if (C == 1 || t + c < turns) {
+            uint32_t odd = 0;  // a half with all exponent bits, where adding one to them reaches the sign
+#pragma unroll
+            for (int yj = 0; yj < 2 * QB; ++yj) {
+              const i32x4_t w = __builtin_bit_cast(i32x4_t, fb[c][yj]);
+#pragma unroll
+              for (int q = 0; q < 4; ++q) odd |= ((uint32_t)w[q] & 0x7f807f80u) + 0x00800080u;
+            }
+            const bool split = __ballot((odd & 0x80008000u) != 0) != 0;
+            static_for<0, 2 * QA>([&](auto bt) {
+              constexpr int blk = decltype(bt)::value;
+              const bool mine = own[blk] == id[c] && !split;
+              const bf16x8_t zero = {};
+              bf16x8_t v[H];
+#pragma unroll
+              for (int h = 0; h < H; ++h) v[h] = mine ? fv[h][blk] : zero;
+#pragma unroll
+              for (int yj = 0; yj < 2 * QB; ++yj) {
+                f32x4_t& a = acc[blk / QA][yj / QB][blk % QA][yj % QB];
+                a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(split ? zero : fb[c][yj], v[GATED ? yj / QB : 0], a, 0, 0, 0);
+              }
+              __builtin_amdgcn_sched_barrier(0);
+            });
+            hold(acc);
+            if (split) apart(acc, fb[c], id[c]);
+            hold(acc);
+          }
+        });
+      }
+    }
+  }
+  // (after each branch the sums are back in their accumulation registers)
+  __device__ __forceinline__ static void hold(f32x4_t (&acc)[2][2][QA][QB]) {
+#pragma unroll
+    for (int i = 0; i < 4 * QA * QB; ++i) asm volatile("" : "+a"(acc[i / (2 * QA * QB)][i / (QA * QB) % 2][i / QB % QA][i % QB]));
+    __builtin_amdgcn_sched_barrier(0);
+  }
+  // a turn's products, one adapter at a time
+  __device__ __forceinline__ void apart(f32x4_t (&acc)[2][2][QA][QB], const bf16x8_t (&fb)[2 * QB], int id) {
+#pragma unroll 1
+    for (int p = 0; p < per; ++p) {
+      const int cur = __builtin_amdgcn_readlane(id, per == 4 ? p * 16 : p * 32);
+      static_for<0, 2 * QA>([&](auto bt) {
+        constexpr int blk = decltype(bt)::value;
+        const bf16x8_t zero = {};
+        static_for<0, 2 * QB>([&](auto yt) {
+          constexpr int yj = decltype(yt)::value;
+          // (from the sums on, as the others: a row's result does not depend on whom it is computed with)
+          f32x4_t& a = acc[blk / QA][yj / QB][blk % QA][yj % QB];
+          const f32x4_t d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              slot == p ? fb[yj] : zero, slot == p && own[blk] == cur ? fv[GATED ? yj / QB : 0][blk] : zero, a, 0, 0, 0);
+#pragma unroll
+          for (int q = 0; q < 4; ++q) a[q] = own[blk] == cur ? d[q] : a[q];
+          asm volatile("" : "+a"(a));
+        });
+      });
+    }
+  }
+};
+
+// Epilogue of a tile: acc[x][y][i][j][t] is row m0 + x BM / 2 + wm BM / 4 + 16 i + l % 16, column
 // n0 + y BN / 2 + wn BN / 4 + 16 j + 4 (l / 16) + t.
-template <int BM, int BN, int EPI, bool ADAPT>
-__device__ __forceinline__ void finish(const Args& g, f32x4_t (&acc)[2][2][BM / 64][BN / 64], int64_t m0, int n0, int wm,
-                                       int wn, int lane, const int* sid, const int* list, int n_list) {
+template <int BM, int BN, int EPI>
+__device__ __forceinline__ void finish(const Args& g, const f32x4_t (&acc)[2][2][BM / 64][BN / 64], int64_t m0, int n0, int wm,
+                                       int wn, int lane) {
   constexpr bool GATED = EPI == EPI_GATED;
   constexpr int QA = BM / 64, QB = BN / 64, WC = BN / 4;
   const int l16 = lane & 15, lq = lane >> 4;
-  if constexpr (ADAPT) {
-    // Each adapter of the tile: its product with the rows' inner products, 32 ranks at a time.  Where all
-    // 16 rows of a block have it, the sums go on; in a block of several it is computed for all and
-    // added, by selection, to the rows that have it: a sum over masked operands would carry a NaN or
-    // an infinity of one request's adapter into the others' rows.  Bound by the latency of the
-    // factors' reads, so they run D adapters ahead (64 to 512 rows with 16 adapters in turn, rank 16,
-    // F 5632: one at a time 25 to 50 us more than without adapters).
-    constexpr int H = GATED ? 2 : 1, D = QB >= 4 ? 2 : 4;
-    int own[2 * QA];
-#pragma unroll
-    for (int b = 0; b < 2 * QA; ++b) own[b] = sid[(b / QA) * (BM / 2) + wm * (BM / 4) + (b % QA) * 16 + l16];
-    const bool has[2] = {g.ad.b[0] != nullptr, !GATED || g.ad.b[1] != nullptr};
-    if (n_list)
-#pragma unroll 1
-    for (int s = 0; s < g.ad.r; s += 32) {
-      const int k = s + 8 * lq;
-      const bool in = k < g.ad.r;
-      bf16x8_t fv[H][2 * QA], fb[D][2][QB];
-      auto load = [&](int set, int a) {
-        const int id = __builtin_amdgcn_readfirstlane(list[a < n_list ? a : n_list - 1]);
-#pragma unroll
-        for (int y = 0; y < 2; ++y)
-#pragma unroll
-          for (int j = 0; j < QB; ++j) {
-            // (columns past the end are not stored)
-            const int n = n0 + (GATED ? 0 : y * (BN / 2)) + wn * WC + j * 16 + l16;
-            fb[set][y][j] = load16(g.ad.b[GATED ? y : 0] + (int64_t)id * g.N * g.ad.r,
-                                   in && n < g.N && has[y] ? (uint32_t)(n * g.ad.r + k) * 2 : NOWHERE);
-          }
-      };
-#pragma unroll
-      for (int d = 0; d < D; ++d) load(d, d);
-#pragma unroll
-      for (int h = 0; h < H; ++h)
-#pragma unroll
-        for (int b = 0; b < 2 * QA; ++b) {
-          const int tr = (b / QA) * (BM / 2) + wm * (BM / 4) + (b % QA) * 16 + l16;
-          fv[h][b] = load16(g.ad.v[h] + m0 * g.ad.r, in && own[b] >= 0 && has[h] ? (uint32_t)(tr * g.ad.r + k) * 2 : NOWHERE);
-        }
-#pragma unroll 1
-      for (int a0 = 0; a0 < n_list; a0 += D)
-        static_for<0, D>([&](auto dt) {
-          constexpr int d = decltype(dt)::value;
-          const int id = a0 + d < n_list ? list[a0 + d] : -2;
-          static_for<0, 2 * QA>([&](auto bt) {
-            constexpr int blk = decltype(bt)::value, x = blk / QA, i = blk % QA;
-            const bool mine = own[blk] == id;
-            const uint64_t rows = __ballot(mine);
-            // (after each branch the sums are back in their accumulation registers, block by block)
-            if (rows == ~0ull) {
-#pragma unroll
-              for (int y = 0; y < 2; ++y)
-#pragma unroll
-                for (int j = 0; j < QB; ++j)
-                  acc[x][y][i][j] =
-                      __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[d][y][j], fv[GATED ? y : 0][blk], acc[x][y][i][j], 0, 0, 0);
-            }
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-#pragma unroll
-              for (int j = 0; j < QB; ++j) asm volatile("" : "+a"(acc[x][y][i][j]));
-            if (rows != 0 && rows != ~0ull) {
-#pragma unroll
-              for (int y = 0; y < 2; ++y)
-#pragma unroll
-                for (int j = 0; j < QB; ++j) {
-                  const f32x4_t p = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[d][y][j], fv[GATED ? y : 0][blk],
-                                                                           f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}, 0, 0, 0);
-#pragma unroll
-                  for (int t = 0; t < 4; ++t) acc[x][y][i][j][t] += mine ? p[t] : 0.0f;
-                }
-            }
-#pragma unroll
-            for (int y = 0; y < 2; ++y)
-#pragma unroll
-              for (int j = 0; j < QB; ++j) asm volatile("" : "+a"(acc[x][y][i][j]));
-          });
-          load(d, a0 + d + D);
-        });
-    }
-  }
   auto rows = [&](auto&& f) {  // f(x, i, m) for this lane's rows
 #pragma unroll
     for (int x = 0; x < 2; ++x)
@@ -397,6 +481,11 @@ __device__ __forceinline__ void dma16_at(const void* base, uint32_t off) {
   const i32x4_t window = {(int)(uint32_t)b, (int)(uint32_t)(b >> 32), 0x7fffffff, 0x00020000};
   asm volatile("buffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(off), "s"(window));
 }
+__device__ __forceinline__ void dma4_at(const void* base, uint32_t off) {
+  const uint64_t b = reinterpret_cast<uint64_t>(base);
+  const i32x4_t window = {(int)(uint32_t)b, (int)(uint32_t)(b >> 32), 0x7fffffff, 0x00020000};
+  asm volatile("buffer_load_dword %0, %1, 0 offen lds" ::"v"(off), "s"(window));
+}
 
 // Where a lane reads a wave's fragments of an R-row stage tile: the wave's 16-row blocks are
 // r = half R / 2 + w R / 4 + 16 i, Q = R / 64 of them in a half.
@@ -461,7 +550,8 @@ __global__ __launch_bounds__(THREADS, (side_by_side<BM, BN, KS, STAGES>)) __attr
   constexpr int NP = LoadA::N + LoadB::N;            // loads of a wave and step
   constexpr int NR = 2 * (QA + QB), NM = 4 * QA * QB;  // fragments and MFMAs of a wave and 32 of K
   __shared__ __attribute__((aligned(1024))) uint8_t lds[STAGES * STAGE];
-  __shared__ int sid[ADAPT ? BM : 1], list[ADAPT ? BM : 1], n_list;
+  __shared__ __attribute__((aligned(256))) int sid[ADAPT ? BM : 1];
+  __shared__ int list[ADAPT ? BM : 1], n_list;
   const int tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int wm = wave >> 1, wn = wave & 1;
@@ -540,6 +630,14 @@ __global__ __launch_bounds__(THREADS, (side_by_side<BM, BN, KS, STAGES>)) __attr
       fa[set][r - 2 * QB] = ra.read(st, r - 2 * QB, ks);
   };
 
+  if constexpr (ADAPT) {  // (ids past the tile's rows: zeros, which list_adapters does not look at)
+    if (wave < BM / 64) {
+      const int64_t m = m0 + tid;
+      dma16_where((KMOE_LDS uint8_t*)sid + wave * 256);
+      asm volatile("s_nop 1");
+      dma4_at(g.ad.ids + m0, m < g.M ? (uint32_t)tid * 4 : NOWHERE);
+    }
+  }
 #pragma unroll 1
   for (int s = 0; s < STAGES; ++s) {
 #pragma unroll
@@ -550,7 +648,12 @@ __global__ __launch_bounds__(THREADS, (side_by_side<BM, BN, KS, STAGES>)) __attr
     }
     next_step();
   }
-  if constexpr (ADAPT) list_adapters<BM>(g.ad, m0, g.M, tid, sid, list, &n_list);
+  if constexpr (ADAPT) {
+    // (the ids have landed before the first step's operands)
+    wait_vmcnt<STAGES * NP>();
+    barrier_nofence();
+    list_adapters<BM>(g.ad.n, g.M - m0 < BM ? (int)(g.M - m0) : BM, tid, sid, list, &n_list);
+  }
   wait_vmcnt<(STAGES - 1) * NP>();
   barrier_nofence();
 #pragma unroll
@@ -613,7 +716,14 @@ __global__ __launch_bounds__(THREADS, (side_by_side<BM, BN, KS, STAGES>)) __attr
   } while ((n += 2) < nk * KS);
   hold();
   wait_vmcnt<0>();  // (the zeros past the end are on their way into this workgroup's LDS)
-  finish<BM, BN, EPI, ADAPT>(g, acc, m0, n0, wm, wn, lane, sid, list, n_list);
+  if constexpr (ADAPT) {
+    if (n_list) {
+      Outer<BM, BN, GATED> outer(g.ad, sid, list, n_list, m0, n0, g.N, wm, wn, lane);
+      outer.add(acc);
+    }
+    hold();
+  }
+  finish<BM, BN, EPI>(g, acc, m0, n0, wm, wn, lane);
 }
 
 }  // namespace kmoe_dense

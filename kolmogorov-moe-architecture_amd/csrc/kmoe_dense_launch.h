@@ -35,7 +35,7 @@ int launch_sum_runs(const float* part, int runs, int64_t total, uint16_t* out, h
 //     128 rows, gate up     39      33      23        23       19       21
 //      48 rows, gate up     37      31      22        18       18       13
 enum Tile { T256, T192, T128, T128_DEEP, T64X128, T64 };
-inline Tile choose_tile(int64_t M, int64_t cols, double steps, double* us = nullptr) {
+inline Tile choose_tile(int64_t M, int64_t cols, double steps, int from = T256, double* us = nullptr) {
   struct Rate {
     int bm, bn, side;
     double full, few, besides;
@@ -43,9 +43,9 @@ inline Tile choose_tile(int64_t M, int64_t cols, double steps, double* us = null
   constexpr Rate rates[] = {{256, 256, 1, 1.63, 1.25, 7.0}, {192, 256, 1, 1.27, 1.05, 6.0}, {128, 128, 2, 1.08, 0.62, 3.0},
                             {128, 128, 1, 0.57, 0.57, 3.0}, {64, 128, 2, 0.72, 0.42, 2.5},  {64, 64, 2, 0.50, 0.33, 2.0}};
   const int64_t cus = kmoe::cu_count();
-  int best = 0;
+  int best = from;
   double least = 0;
-  for (int i = 0; i < 6; ++i) {
+  for (int i = from; i < 6; ++i) {
     const Rate& r = rates[i];
     const int64_t tiles = kmoe::ceil_div<int64_t>(M, r.bm) * kmoe::ceil_div<int64_t>(cols, r.bn);
     const int64_t rounds = tiles / (cus * r.side), rest = tiles - rounds * cus * r.side;
@@ -54,7 +54,7 @@ inline Tile choose_tile(int64_t M, int64_t cols, double steps, double* us = null
       t += r.full * steps + r.besides;
     else if (rest > 0)
       t += (r.side == 1 ? r.few + (r.full - r.few) * rest / cus : r.few) * steps + r.besides;
-    if (i == 0 || t < least) best = i, least = t;
+    if (i == from || t < least) best = i, least = t;
   }
   if (us) *us = least;
   return (Tile)best;
@@ -80,8 +80,11 @@ int launch_tile(const Args& g, hipStream_t s) {
 template <bool SA, bool SB, int EPI, bool ADAPT = false>
 int launch_any(const Args& g, hipStream_t s) {
   const double steps = (double)kmoe::ceil_div(g.K, 64) * (EPI == EPI_TWO ? 2 : 1);
-  switch (choose_tile(g.M, (int64_t)g.N * (EPI == EPI_GATED ? 2 : 1), steps)) {
-    case T256: return launch_tile<256, 256, 2, 2, SA, SB, EPI, ADAPT>(g, s);
+  // (with adapters not the largest tile: its sums fill the registers)
+  switch (choose_tile(g.M, (int64_t)g.N * (EPI == EPI_GATED ? 2 : 1), steps, ADAPT ? T192 : T256)) {
+    case T256:
+      if constexpr (!ADAPT) return launch_tile<256, 256, 2, 2, SA, SB, EPI, ADAPT>(g, s);
+      [[fallthrough]];
     case T192: return launch_tile<192, 256, 2, 2, SA, SB, EPI, ADAPT>(g, s);
     // (weight gradients: steps of 32 of K lie as well, and two more stages fit; 2042 rows 57 against 61 us)
     case T128: return launch_tile<128, 128, SA ? 1 : 2, SA ? 4 : 2, SA, SB, EPI, ADAPT>(g, s);

@@ -26,12 +26,12 @@ __global__ __launch_bounds__(512) void few_kernel(Args g) {
   const int at = tid & 15, an = tid >> 4;
   int id = -1;
   if (ADAPT && at < g.M && an < ROWS && n0 + an < g.N) id = g.ad.ids[at];
-  const void* const w[1] = {g.b[0] + (int64_t)n0 * g.ldb};
-  const uint32_t woff[1] = {l16 < ROWS && n0 + l16 < g.N ? (uint32_t)(l16 * g.ldb) * 2 : NOWHERE};
-  const uint32_t xoff = l16 < g.M ? (uint32_t)(l16 * g.lda) * 2 : NOWHERE;
+  Stream16<1, W, D> st;
+  st.w[0] = g.b[0] + (int64_t)n0 * g.ldb, st.x = g.a[0], st.K = g.K;
+  st.woff[0] = l16 < ROWS && n0 + l16 < g.N ? (uint32_t)(l16 * g.ldb) * 2 : NOWHERE;
+  st.xoff = l16 < g.M ? (uint32_t)(l16 * g.lda) * 2 : NOWHERE;
   f32x4_t acc[1] = {f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
-  bf16x8_t fw[D][2][1], fx[D][2];
-  stream16<1, W, D>(w, woff, g.a[0], xoff, g.K, wave, lane, acc, false, fw, fx);
+  st.start(wave, lane);
   if constexpr (ADAPT) {
     float sum = 0.0f;
     if ((unsigned)id < (unsigned)g.ad.n) {
@@ -57,7 +57,7 @@ __global__ __launch_bounds__(512) void few_kernel(Args g) {
     }
     if (an < 16) extra[at][an] = sum;
   }
-  stream16<1, W, D>(w, woff, g.a[0], xoff, g.K, wave, lane, acc, true, fw, fx);
+  st.run(wave, lane, acc);
   part[wave][lane] = acc[0];
   __syncthreads();
   // row l % 16, columns n0 + 4 (l / 16) .. + 3
@@ -92,7 +92,7 @@ int linear_runs(int64_t T, int K, int N) {
   const int64_t tiles = kmoe::ceil_div<int64_t>(T, 64) * kmoe::ceil_div(N, 64), cus = kmoe::cu_count();
   const int steps = kmoe::ceil_div(K, 64);
   double least;
-  choose_tile(T, N, steps, &least);
+  choose_tile(T, N, steps, T256, &least);
   int64_t best = 1;
   for (int side = 1; side <= 2; ++side) {
     int64_t runs = side * cus / tiles;
