@@ -692,12 +692,13 @@ typedef struct {
 
 /* y (T, d) = (act(x w_gate^T) * (x w_up^T)) w_down^T with adapters (each nullable; the gate's and
  * the up projection's of one rank), act a KMOE_ACT_*; w_gate, w_up (F, d), w_down (d, F).
- * The hidden values are rounded to bf16.                                            */
+ * The hidden values are rounded to bf16 (of at most 8 rows to twice its bits).       */
 size_t kmoe_gated_ffn_workspace_bytes(int64_t T, int d, int F, int rank_gate_up, int rank_down);
 int kmoe_gated_ffn(const void* x, int64_t T, int d, int F, const void* w_gate, const void* w_up, const void* w_down,
                    int act, const int32_t* ids, int n_adapters, const kmoe_adapter* gate, const kmoe_adapter* up,
                    const kmoe_adapter* down, void* y, void* workspace, size_t workspace_bytes, void* stream);
-/* y (T, N) = x w^T with an adapter (nullable).                                      */
+/* y (T, N) = x w^T with an adapter (nullable): then the workspace begins with the scaled inner
+ * products (T, rank) bf16, those of kmoe_adapter_inner.                             */
 size_t kmoe_adapted_linear_workspace_bytes(int64_t T, int K, int N, int rank);
 int kmoe_adapted_linear(const void* x, int64_t T, int K, const void* w, int N, const int32_t* ids, int n_adapters,
                         const kmoe_adapter* adapter, void* y, void* workspace, size_t workspace_bytes, void* stream);
@@ -724,6 +725,13 @@ int kmoe_dense_dx(const void* dy, const void* dy2, int64_t T, int N, const void*
                   const int32_t* ids, int n_adapters, int rank, const void* u, const void* at, void* dx, void* stream);
 /* c (M, N) bf16 or f32 = a^T b, a (T, M), b (T, N), any T.                          */
 int kmoe_dense_wgrad(const void* a, const void* b, int64_t T, int M, int N, void* c, int c_dtype, void* stream);
+/* The backward of kmoe_adapted_linear with an adapter and without a gradient of w (kmoe_dense_wgrad is
+ * that one's): dx (T, K), da (n, r, K) and db (n, N, r) from dy (T, N), each where it is not NULL.
+ * v (T, r): the forward's scaled inner products, for db.  At most 32767 adapters.  */
+size_t kmoe_adapted_linear_backward_workspace_bytes(int64_t T, int K, int N, int n_adapters, int rank);
+int kmoe_adapted_linear_backward(const void* dy, const void* x, int64_t T, int K, const void* w, int N,
+                                 const int32_t* ids, int n_adapters, const kmoe_adapter* adapter, const void* v,
+                                 void* dx, void* da, void* db, void* workspace, size_t workspace_bytes, void* stream);
 /* out[i] = sum over the rows t of adapter i of l[t]^T m[t], l (T, rank), m (T, C): (rank, C), or with
  * outer (C, rank), bf16; zeros for an adapter without rows.                         */
 size_t kmoe_adapter_grad_workspace_bytes(int64_t T, int n, int rank, int C);

@@ -62,7 +62,7 @@ struct Args {
   int c_f32;          // (with runs of K: 1, their sums one after the other, M ldc apart)
   int act;            // GATED
   uint8_t* saved;     // GATED: up act'(gate) and act(gate) for the backward (nullable); DH: the same, read
-  uint16_t* c2;       // DH: the up half's gradient
+  uint16_t* c2;       // DH: the up half's gradient; GATED: what the values in c lost by their rounding (nullable)
   Adapt ad;
 };
 
@@ -390,8 +390,18 @@ __device__ __forceinline__ void finish(const Args& g, const f32x4_t (&acc)[2][2]
             act_at<decltype(tag)::value>(acc[x][0][i][j][t], a, da);
             h[t] = a * up, p[t] = da * up, q[t] = a;
           }
-          if (m < g.M && n < g.N)
-            *reinterpret_cast<i32x2_t*>(static_cast<uint16_t*>(g.c) + m * g.ldc + n) = pack4(h[0], h[1], h[2], h[3]);
+          if (m < g.M && n < g.N) {
+            const i32x2_t w = pack4(h[0], h[1], h[2], h[3]);
+            *reinterpret_cast<i32x2_t*>(static_cast<uint16_t*>(g.c) + m * g.ldc + n) = w;
+            if (g.c2) {
+              const auto lost = [&](int t) {
+                const uint32_t u = (uint32_t)w[t / 2];
+                const float r = h[t] - __uint_as_float(t % 2 ? u & 0xffff0000u : u << 16);
+                return r - r == 0.0f ? r : 0.0f;  // (of an infinity nothing)
+              };
+              *reinterpret_cast<i32x2_t*>(g.c2 + m * g.ldc + n) = pack4(lost(0), lost(1), lost(2), lost(3));
+            }
+          }
           if (g.saved) {  // (whole blocks: the buffer has them)
             uint8_t* const block = saved_block(g.saved, g.N, m, n16);
             store24(block, lane, p);

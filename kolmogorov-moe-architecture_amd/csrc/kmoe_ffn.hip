@@ -13,7 +13,9 @@ namespace {
 // weights from HBM: 5632 x 2048 9.7 us, 2048 x 5632 8.2; the gate and up rows of the block are
 // enough for the tiles of 64 x 64, 11.7 against 14.1 us).  An adapter is added in f32: a thread sums
 // all ranks of one result, its factors on their way with the first weights.
-constexpr int FEW = 16;
+// Of at most 8 rows the upper 8 of the MFMA's 16 are free: there go what the block's hidden values lost by
+// their rounding to bf16, for nothing, and so the block's result is rounded once and not twice.
+constexpr int FEW = 16, FEW_EXACT = 8;
 
 template <int ROWS, bool ADAPT>
 __global__ __launch_bounds__(512) void few_kernel(Args g) {
@@ -29,7 +31,10 @@ __global__ __launch_bounds__(512) void few_kernel(Args g) {
   Stream16<1, W, D> st;
   st.w[0] = g.b[0] + (int64_t)n0 * g.ldb, st.x = g.a[0], st.K = g.K;
   st.woff[0] = l16 < ROWS && n0 + l16 < g.N ? (uint32_t)(l16 * g.ldb) * 2 : NOWHERE;
-  st.xoff = l16 < g.M ? (uint32_t)(l16 * g.lda) * 2 : NOWHERE;
+  const int lost = g.a[1] ? l16 - 8 : -1;  // (the second rows lie less than 2^27 bytes behind the first ones)
+  st.xoff = l16 < g.M                  ? (uint32_t)(l16 * g.lda) * 2
+            : lost >= 0 && lost < g.M  ? (uint32_t)(g.a[1] - g.a[0] + lost * g.lda) * 2
+                                       : NOWHERE;
   f32x4_t acc[1] = {f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
   st.start(wave, lane);
   if constexpr (ADAPT) {
@@ -62,10 +67,15 @@ __global__ __launch_bounds__(512) void few_kernel(Args g) {
   __syncthreads();
   // row l % 16, columns n0 + 4 (l / 16) .. + 3
   const int n = n0 + 4 * lq;
-  if (wave || l16 >= g.M || 4 * lq >= ROWS || n >= g.N) return;
+  if (wave) return;
   f32x4_t s = part[0][lane];
 #pragma unroll
   for (int k = 1; k < W; ++k) s += part[k][lane];
+  if (g.a[1]) {
+#pragma unroll
+    for (int c = 0; c < 4; ++c) s[c] += __shfl(s[c], lane | 8, 64);
+  }
+  if (l16 >= g.M || 4 * lq >= ROWS || n >= g.N) return;
   if constexpr (ADAPT) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) s[c] += extra[l16][4 * lq + c];
@@ -125,10 +135,11 @@ size_t runs_bytes(int64_t T, int K, int N) {
 }
 
 // y = x w^T with the adapter's outer product, whose inner products v are there; part: runs_bytes.
-int project(const void* x, int64_t T, int K, const void* w, int N, const int32_t* ids, int n, const kmoe_adapter* ad,
-            const void* v, void* y, void* part, hipStream_t s) {
+// lost: of T <= FEW_EXACT rows what x lost by its rounding, behind x (nullable).
+int project(const void* x, const void* lost, int64_t T, int K, const void* w, int N, const int32_t* ids, int n,
+            const kmoe_adapter* ad, const void* v, void* y, void* part, hipStream_t s) {
   Args g{};
-  g.a[0] = bf(x), g.b[0] = bf(w), g.K = K, g.lda = K, g.ldb = K, g.M = T, g.N = N, g.ldc = N, g.c = y;
+  g.a[0] = bf(x), g.a[1] = bf(lost), g.b[0] = bf(w), g.K = K, g.lda = K, g.ldb = K, g.M = T, g.N = N, g.ldc = N, g.c = y;
   if (ad) g.ad = {ids, {bf(v), nullptr}, {bf(ad->b), nullptr}, n, ad->rank};
   if (T <= FEW) return ad ? launch_few<true>(g, s) : launch_few<false>(g, s);
   const int runs = linear_runs(T, K, N);
@@ -163,13 +174,13 @@ extern "C" int kmoe_adapted_linear(const void* x, int64_t T, int K, const void* 
                                       nullptr, nullptr, stream);
     if (rc) return rc;
   }
-  return project(x, T, K, w, N, ids, n_adapters, adapter, workspace, y,
+  return project(x, nullptr, T, K, w, N, ids, n_adapters, adapter, workspace, y,
                  static_cast<uint8_t*>(workspace) + piece(T * (adapter ? adapter->rank : 0) * 2), kmoe::as_stream(stream));
 }
 
 extern "C" size_t kmoe_gated_ffn_workspace_bytes(int64_t T, int d, int F, int rank_gate_up, int rank_down) {
   if (T <= 0) return 0;
-  return piece(T * F * 2) + 2 * piece(T * rank_gate_up * 2) + piece(T * rank_down * 2) + runs_bytes(T, F, d);
+  return piece(T * F * (T <= FEW_EXACT ? 4 : 2)) + 2 * piece(T * rank_gate_up * 2) + piece(T * rank_down * 2) + runs_bytes(T, F, d);
 }
 
 extern "C" int kmoe_gated_ffn(const void* x, int64_t T, int d, int F, const void* w_gate, const void* w_up,
@@ -194,7 +205,8 @@ extern "C" int kmoe_gated_ffn(const void* x, int64_t T, int d, int F, const void
                kmoe_gated_ffn_workspace_bytes(T, d, F, rgu, rd));
   uint8_t* w = static_cast<uint8_t*>(workspace);
   void* const h = w;
-  void* const vg = w += piece(T * F * 2);
+  void* const lost = T <= FEW_EXACT ? w + T * F * 2 : nullptr;
+  void* const vg = w += piece(T * F * (lost ? 4 : 2));
   void* const vu = w += piece(T * rgu * 2);
   void* const vd = w += piece(T * rgu * 2);
   void* const part = w += piece(T * rd * 2);
@@ -208,12 +220,17 @@ extern "C" int kmoe_gated_ffn(const void* x, int64_t T, int d, int F, const void
                               nullptr, nullptr, nullptr, stream);
     if (rc) return rc;
   }
-  rc = kmoe_dense_gate_up(x, T, d, w_gate, w_up, F, act, rgu ? ids : nullptr, n_adapters, rgu, gate ? vg : nullptr,
-                          gate ? gate->b : nullptr, up ? vu : nullptr, up ? up->b : nullptr, h, nullptr, stream);
+  Args g{};
+  g.a[0] = bf(x), g.b[0] = bf(w_gate), g.b[1] = bf(w_up), g.K = d, g.lda = d, g.ldb = d, g.M = T, g.N = F;
+  g.ldc = F, g.c = h, g.c2 = static_cast<uint16_t*>(lost), g.act = act;
+  if (rgu)
+    g.ad = {ids, {gate ? bf(vg) : nullptr, up ? bf(vu) : nullptr}, {gate ? bf(gate->b) : nullptr, up ? bf(up->b) : nullptr},
+            n_adapters, rgu};
+  rc = rgu ? launch_gated_adapt(g, s) : launch_gated(g, s);
   if (rc) return rc;
   if (down) {
     rc = kmoe_adapter_inner(h, T, F, ids, n_adapters, rd, down->a, down->scale, vd, nullptr, nullptr, nullptr, stream);
     if (rc) return rc;
   }
-  return project(h, T, F, w_down, d, ids, n_adapters, down, vd, y, part, s);
+  return project(h, lost, T, F, w_down, d, ids, n_adapters, down, vd, y, part, s);
 }

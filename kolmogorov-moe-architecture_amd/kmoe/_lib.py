@@ -141,6 +141,8 @@ _SIGNATURES = {
     "kmoe_dense_dh": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _vp]),
     "kmoe_dense_dx": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp]),
     "kmoe_dense_wgrad": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _i32, _vp]),
+    "kmoe_adapted_linear_backward_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32]),
+    "kmoe_adapted_linear_backward": (_i32, [_vp, _vp, _i64, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "kmoe_adapter_grad_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
     "kmoe_adapter_grad": (_i32, [_vp, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _sz, _vp]),
     # the optimizer step

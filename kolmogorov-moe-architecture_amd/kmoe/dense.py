@@ -8,7 +8,8 @@
   row t with the adapter ids[t]; also on all three projections of the block.
 
 Numerics: bf16 operands, f32 sums.  What is rounded to bf16 between the products: the block's
-hidden values h = act(g) u (an operand of the down product), the gradients of its pre-activations, and an
+hidden values h = act(g) u (an operand of the down product; of up to 8 rows in a call without
+gradients they keep 16 bits), the gradients of its pre-activations, and an
 adapter's inner products with their scale.  What the backward keeps of the pre-activations, u act'(g)
 and act(g), has 16 bits of precision.
 """
@@ -74,17 +75,17 @@ def _rows(x, K, who):
 def _adapters(ad, K, N, who, name):
     """The adapters checked, in bf16, ranks filled up to a multiple of 8 (differentiable)."""
     a, b, scale = ad
-    if a.dim() != 3 or b.dim() != 3 or a.shape[0] != b.shape[0] or a.shape[1] != b.shape[2] or a.shape[2] != K or \
-            b.shape[1] != N or not 1 <= a.shape[1] <= _lib.MAX_RANK or not 1 <= a.shape[0] <= 65535:
-        raise ValueError(f"kmoe.{who}: {name}a must be (n, r, {K}) and b (n, {N}, r), n up to 65535 and r up to "
+    n, r = a.shape[:2] if a.dim() == 3 else (0, 0)
+    if not 1 <= r <= _lib.MAX_RANK or not 1 <= n <= 32767 or a.shape[2] != K or b.shape != (n, N, r):
+        raise ValueError(f"kmoe.{who}: {name}a must be (n, r, {K}) and b (n, {N}, r), n up to 32767 and r up to "
                          f"{_lib.MAX_RANK}, got {tuple(a.shape)}, {tuple(b.shape)}")
     if scale is not None:
-        if scale.shape != (a.shape[0],):
-            raise ValueError(f"kmoe.{who}: {name}scale must be ({a.shape[0]},), got {tuple(scale.shape)}")
+        if scale.shape != (n,):
+            raise ValueError(f"kmoe.{who}: {name}scale must be ({n},), got {tuple(scale.shape)}")
         if scale.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"kmoe.{who}: {name}scale has no gradient here: pass it detached")
         scale = _contig(scale.detach(), torch.float32)
-    fill = -a.shape[1] % 8
+    fill = -r % 8
     if fill:
         a, b = nn.functional.pad(a, (0, 0, 0, fill)), nn.functional.pad(b, (0, fill))
     return Adapters(a, b, scale)
@@ -104,16 +105,18 @@ def _ids(ids, x, n, who):
 
 def _struct(ad):
     """kmoe_adapter of bf16 contiguous adapters (the caller keeps the tensors)."""
-    return None if ad is None else ctypes.byref(_lib.Adapter(ptr(ad.a), ptr(ad.b), ptr(ad.scale), ad.a.shape[1]))
+    return None if ad is None else ctypes.byref(_lib.Adapter(ad.a.data_ptr(), ad.b.data_ptr(), ptr(ad.scale), ad.a.shape[1]))
 
 
 def _held(ad):
-    return None if ad is None else Adapters(_aligned(ad.a.detach()), _aligned(ad.b.detach()), ad.scale)
+    return None if ad is None else Adapters(_ready(ad.a), _ready(ad.b), ad.scale)
 
 
-def _aligned(t):
-    """t in bf16, contiguous, at a multiple of 16 bytes."""
-    t = _contig(t, _BF16)
+def _ready(t):
+    """t's values in bf16, contiguous, at a multiple of 16 bytes: t itself where it is so already."""
+    if t.dtype is _BF16 and t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
+    t = _contig(t.detach(), _BF16)
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -127,61 +130,49 @@ def _linear_workspace(device, T, K, N, r) -> int:
     return _lib.load().kmoe_adapted_linear_workspace_bytes(T, K, N, r)
 
 
+@functools.lru_cache(maxsize=1024)
+def _linear_backward_workspace(device, T, K, N, n, r) -> int:
+    return _lib.load().kmoe_adapted_linear_backward_workspace_bytes(T, K, N, n, r)
+
+
 # ---------------------------------------------------------------- without gradients
-def _ffn_forward(x2d, wg, wu, wd, act, ads, ids):
-    T, d = x2d.shape
-    F = wg.shape[0]
-    dev = x2d.device
-    y = torch.empty(T, d, device=dev, dtype=_BF16)
+def _ffn_forward(x, wg, wu, wd, act, ads, ids):
+    F, d = wg.shape
+    T = x.numel() // d
+    dev = x.device
+    y = torch.empty_like(x)
     gate, up, down = ads if ads is not None else (None, None, None)
     some = gate or up or down
     rgu = gate.a.shape[1] if gate is not None else up.a.shape[1] if up is not None else 0
     with _device(dev), _Stage("gated_ffn"):
         wsb = _ffn_workspace(dev.index, T, d, F, rgu, down.a.shape[1] if down is not None else 0)
-        ws = torch.empty(max(wsb, 16), device=dev, dtype=torch.uint8)
-        _lib.call("kmoe_gated_ffn", ptr(x2d), T, d, F, ptr(wg), ptr(wu), ptr(wd), act, ptr(ids),
-                  some.a.shape[0] if some else 0, _struct(gate), _struct(up), _struct(down), ptr(y), ptr(ws), wsb,
-                  _stream(x2d))
+        ws = torch.empty(wsb, device=dev, dtype=torch.uint8)
+        _lib.call("kmoe_gated_ffn", x.data_ptr(), T, d, F, wg.data_ptr(), wu.data_ptr(), wd.data_ptr(), act, ptr(ids),
+                  some.a.shape[0] if some else 0, _struct(gate), _struct(up), _struct(down), y.data_ptr(), ws.data_ptr(), wsb,
+                  _stream(x))
     return y
 
 
-def _linear_forward(x2d, w, ad, ids):
-    T, K = x2d.shape
-    dev = x2d.device
-    y = torch.empty(T, w.shape[0], device=dev, dtype=_BF16)
+def _linear_forward(x, w, ad, ids):
+    N, K = w.shape
+    T = x.numel() // K
+    dev = x.device
+    y = x.new_empty(x.shape[:-1] + (N,))
+    n, r = ad.a.shape[:2] if ad is not None else (0, 0)
     with _device(dev), _Stage("adapted_linear"):
-        wsb = _linear_workspace(dev.index, T, K, w.shape[0], ad.a.shape[1] if ad is not None else 0)
-        ws = torch.empty(max(wsb, 16), device=dev, dtype=torch.uint8)
-        _lib.call("kmoe_adapted_linear", ptr(x2d), T, K, ptr(w), w.shape[0], ptr(ids), ad.a.shape[0] if ad is not None else 0,
-                  _struct(ad), ptr(y), ptr(ws), wsb, _stream(x2d))
-    return y
+        wsb = _linear_workspace(dev.index, T, K, N, r)
+        ws = torch.empty(wsb, device=dev, dtype=torch.uint8) if wsb else None
+        _lib.call("kmoe_adapted_linear", x.data_ptr(), T, K, w.data_ptr(), N, ptr(ids), n, _struct(ad), y.data_ptr(), ptr(ws),
+                  wsb, _stream(x))
+    return y, ws
 
 
 # ---------------------------------------------------------------- parts of the backward
-def _inner(x2d, ids, a, scale):
-    """(T, r) bf16 scaled inner products; rows without an adapter are not written."""
-    v = torch.empty(x2d.shape[0], a.shape[1], device=x2d.device, dtype=_BF16)
-    _lib.call("kmoe_adapter_inner", ptr(x2d), x2d.shape[0], x2d.shape[1], ptr(ids), a.shape[0], a.shape[1], ptr(a), ptr(scale),
-              ptr(v), None, None, None, _stream(x2d))
-    return v
-
-
-def _factor_grad(l, m, ids, n, outer):
-    T, r = l.shape
-    C = m.shape[1]
-    out = torch.empty((n, C, r) if outer else (n, r, C), device=m.device, dtype=_BF16)
-    wsb = _lib.load().kmoe_adapter_grad_workspace_bytes(T, n, r, C)
-    ws = torch.empty(max(wsb, 16), device=m.device, dtype=torch.uint8)
-    _lib.call("kmoe_adapter_grad", ptr(l), ptr(m), T, ptr(ids), n, r, C, int(outer), ptr(out), ptr(ws), wsb, _stream(m))
-    return out
-
-
-def _dense_dx(dy, w, dy2=None, w2=None, ids=None, n=0, u=None, at=None):
+def _dense_dx(dy, w, dy2=None, w2=None):
     T, N = dy.shape
     K = w.shape[1]
     dx = torch.empty(T, K, device=dy.device, dtype=_BF16)
-    _lib.call("kmoe_dense_dx", ptr(dy), ptr(dy2), T, N, ptr(w), ptr(w2), K, ptr(ids), n, 0 if u is None else u.shape[1],
-              ptr(u), ptr(at), ptr(dx), _stream(dy))
+    _lib.call("kmoe_dense_dx", ptr(dy), ptr(dy2), T, N, ptr(w), ptr(w2), K, None, 0, 0, None, None, ptr(dx), _stream(dy))
     return dx
 
 
@@ -197,53 +188,57 @@ def _dense_wgrad(a, b, dtype):
 
 
 # ---------------------------------------------------------------- the gated block
+def _copied(*pairs):
+    """The tensors whose values in bf16 are copies.  They are saved too, so that a write to one before the
+    backward is refused; of the others the saved values are the tensor itself."""
+    return tuple(t for t, held in pairs if t is not None and held is not t)
+
+
 class _GatedFFNFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, wg, wu, wd, act):
         _bwd.leaves_of(ctx, x, wg, wu, wd)
-        x2d = _aligned(x.detach().reshape(-1, x.shape[-1]))
-        bg, bu, bd = (_aligned(w.detach()) for w in (wg, wu, wd))
-        T, d = x2d.shape
-        F = bg.shape[0]
-        h = torch.empty(T, F, device=x.device, dtype=_BF16)
+        xr, bg, bu, bd = _ready(x), _ready(wg), _ready(wu), _ready(wd)
+        F, d = bg.shape
+        T = xr.numel() // d
+        h = xr.new_empty((T, F))
         saved = torch.empty(max(_lib.load().kmoe_dense_saved_bytes(T, F), 16), device=x.device, dtype=torch.uint8)
-        y = torch.empty(T, d, device=x.device, dtype=_BF16)
+        y = xr.new_empty(x.shape)
         with _device(x.device):
             with _Stage("ffn_gate_up"):
-                _lib.call("kmoe_dense_gate_up", ptr(x2d), T, d, ptr(bg), ptr(bu), F, act, None, 0, 0, None, None, None, None,
+                _lib.call("kmoe_dense_gate_up", ptr(xr), T, d, ptr(bg), ptr(bu), F, act, None, 0, 0, None, None, None, None,
                           ptr(h), ptr(saved), _stream(x))
             with _Stage("ffn_down"):
                 _lib.call("kmoe_dense_linear", ptr(h), T, F, ptr(bd), d, None, 0, 0, None, None, ptr(y), _stream(x))
-        # the weights themselves are saved too: a write to one before the backward is refused
-        ctx.save_for_backward(x2d, h, saved, bg, bu, bd, wg, wu, wd)
-        ctx.meta = (x.shape, x.dtype)
-        return y.view(x.shape).to(x.dtype)
+        ctx.save_for_backward(xr, h, saved, bg, bu, bd, *_copied((x, xr), (wg, bg), (wu, bu), (wd, bd)))
+        ctx.meta = (x.dtype, wg.dtype, wu.dtype, wd.dtype)
+        return y if x.dtype is _BF16 else y.to(x.dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x2d, h, saved, bg, bu, bd, wg, wu, wd = ctx.saved_tensors
-        shape, dtype = ctx.meta
-        T, F = h.shape
-        d = x2d.shape[1]
+        xr, h, saved, bg, bu, bd = ctx.saved_tensors[:6]
+        dtypes = ctx.meta
+        F, d = bg.shape
+        T = h.shape[0]
         need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
-        dy2 = _aligned(dy.reshape(T, d))
+        dy2, x2d = _ready(dy).view(T, d), xr.view(T, d)
         dx = dg = du = dwg = dwu = dwd = None
-        with _device(x2d.device):
+        with _device(xr.device):
             if need_x or need_g or need_u:
-                dg, du = (torch.empty(T, F, device=x2d.device, dtype=_BF16) for _ in range(2))
+                dg, du = torch.empty_like(h), torch.empty_like(h)
                 with _Stage("bwd_ffn_dh"):
-                    _lib.call("kmoe_dense_dh", ptr(dy2), T, d, ptr(bd), F, ptr(saved), ptr(dg), ptr(du), _stream(x2d))
+                    _lib.call("kmoe_dense_dh", ptr(dy2), T, d, ptr(bd), F, ptr(saved), ptr(dg), ptr(du), _stream(xr))
             if need_x:
                 with _Stage("bwd_ffn_dx"):
-                    dx = _dense_dx(dg, bg, du, bu).view(shape).to(dtype)
+                    dx = _dense_dx(dg, bg, du, bu).view(xr.shape).to(dtypes[0])
             with _Stage("bwd_ffn_wgrad"):
                 if need_g:
-                    dwg = _dense_wgrad(dg, x2d, wg.dtype)
+                    dwg = _dense_wgrad(dg, x2d, dtypes[1])
                 if need_u:
-                    dwu = _dense_wgrad(du, x2d, wu.dtype)
+                    dwu = _dense_wgrad(du, x2d, dtypes[2])
                 if need_d:
-                    dwd = _dense_wgrad(dy2, h, wd.dtype)
+                    dwd = _dense_wgrad(dy2, h, dtypes[3])
         return dx, dwg, dwu, dwd, None
 
 
@@ -292,9 +287,8 @@ def gated_ffn(x, w_gate, w_up, w_down, activation="silu", adapters: Optional[FFN
             g, u = (_adapted(x, w, a, i32) for w, a in ((w_gate, adapters.gate), (w_up, adapters.up)))
             return _adapted((_ACT_FN[activation](g.float()) * u.float()).to(_BF16), w_down, adapters.down, i32).to(x.dtype)
         adapters = FFNAdapters(*(_held(a) for a in adapters))
-    x2d = _aligned(x.detach().reshape(-1, d))
-    y = _ffn_forward(x2d, *(_aligned(w.detach()) for w in (w_gate, w_up, w_down)), act, adapters, i32)
-    return y.view(x.shape).to(x.dtype)
+    y = _ffn_forward(_ready(x), _ready(w_gate), _ready(w_up), _ready(w_down), act, adapters, i32)
+    return y if x.dtype is _BF16 else y.to(x.dtype)
 
 
 # ---------------------------------------------------------------- adapted projections
@@ -302,45 +296,40 @@ class _AdaptedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, a, b, scale, ids):
         _bwd.leaves_of(ctx, x, w, a, b)
-        x2d = _aligned(x.detach().reshape(-1, x.shape[-1]))
-        bw = _aligned(w.detach())
-        ba, bb = (None, None) if a is None else (_aligned(a.detach()), _aligned(b.detach()))
-        T, K = x2d.shape
-        N = bw.shape[0]
-        y = torch.empty(T, N, device=x.device, dtype=_BF16)
-        v = None
-        with _device(x.device), _Stage("adapted_linear"):
-            if a is not None:
-                v = _inner(x2d, ids, ba, scale)
-            _lib.call("kmoe_dense_linear", ptr(x2d), T, K, ptr(bw), N, None if a is None else ptr(ids),
-                      0 if a is None else ba.shape[0], 0 if a is None else ba.shape[1], ptr(v), ptr(bb), ptr(y), _stream(x))
-        ctx.save_for_backward(x2d, bw, ba, bb, scale, ids if a is not None else None, v, w, a, b)
-        ctx.meta = (x.shape, x.dtype)
-        return y.view(*x.shape[:-1], N).to(x.dtype)
+        xr, bw = _ready(x), _ready(w)
+        ad = None if a is None else Adapters(_ready(a), _ready(b), scale)
+        y, ws = _linear_forward(xr, bw, ad, ids)
+        # (with an adapter the workspace begins with the scaled inner products)
+        ba, bb, kept = (None, None, None) if a is None else (ad.a, ad.b, ws)
+        ctx.save_for_backward(xr, bw, ba, bb, scale, ids, kept, *_copied((x, xr), (w, bw), (a, ba), (b, bb)))
+        ctx.meta = (x.dtype, w.dtype, None if a is None else a.dtype, None if b is None else b.dtype)
+        return y if x.dtype is _BF16 else y.to(x.dtype)
 
     @staticmethod
     @once_differentiable
     def backward(ctx, dy):
-        x2d, bw, ba, bb, scale, ids, v, w, a, b = ctx.saved_tensors
-        shape, dtype = ctx.meta
-        T, N = x2d.shape[0], bw.shape[0]
+        xr, bw, ba, bb, scale, ids, v = ctx.saved_tensors[:7]
+        dtypes = ctx.meta
+        N, K = bw.shape
+        T = xr.numel() // K
         need_x, need_w, need_a, need_b = ctx.needs_input_grad[:4]
-        dy2 = _aligned(dy.reshape(T, N))
-        dx = dw = da = db = u = None
-        with _device(x2d.device), _Stage("bwd_adapted_linear"):
-            if ba is not None and (need_x or need_a):
-                u = _inner(dy2, ids, bb.transpose(1, 2).contiguous(), scale)
-            if need_x:
-                dx = (_dense_dx(dy2, bw) if ba is None else
-                      _dense_dx(dy2, bw, ids=ids, n=ba.shape[0], u=u, at=ba.transpose(1, 2).contiguous()))
-                dx = dx.view(shape).to(dtype)
+        dy2 = _ready(dy)
+        dx = dw = da = db = None
+        with _device(xr.device), _Stage("bwd_adapted_linear"):
+            if ba is not None and (need_x or need_a or need_b):
+                n, r = ba.shape[:2]
+                dx = torch.empty_like(xr) if need_x else None
+                da = torch.empty_like(ba) if need_a else None
+                db = torch.empty_like(bb) if need_b else None
+                wsb = _linear_backward_workspace(xr.device.index, T, K, N, n, r)
+                ws = torch.empty(max(wsb, 16), device=xr.device, dtype=torch.uint8)
+                _lib.call("kmoe_adapted_linear_backward", ptr(dy2), ptr(xr), T, K, ptr(bw), N, ptr(ids), n,
+                          _struct(Adapters(ba, bb, scale)), ptr(v), ptr(dx), ptr(da), ptr(db), ptr(ws), wsb, _stream(xr))
+            elif need_x:
+                dx = _dense_dx(dy2.view(T, N), bw).view(xr.shape)
             if need_w:
-                dw = _dense_wgrad(dy2, x2d, w.dtype)
-            if need_a:
-                da = _factor_grad(u, x2d, ids, ba.shape[0], False).to(a.dtype)
-            if need_b:
-                db = _factor_grad(v, dy2, ids, ba.shape[0], True).to(b.dtype)
-        return dx, dw, da, db, None, None
+                dw = _dense_wgrad(dy2.view(T, N), xr.view(T, K), dtypes[1])
+        return tuple(g if g is None or g.dtype is t else g.to(t) for g, t in zip((dx, dw, da, db), dtypes)) + (None, None)
 
 
 def _adapted(x, w, ad, i32):
@@ -366,8 +355,8 @@ def adapted_linear(x, weight, adapters: Optional[Adapters] = None, ids=None):
         _one_gpu("adapted_linear", x, weight)
     if _wants_grad(x, weight, *(adapters[:2] if adapters is not None else ())):
         return _adapted(x, weight, adapters, i32)
-    y = _linear_forward(_aligned(x.detach().reshape(-1, K)), _aligned(weight.detach()), _held(adapters), i32)
-    return y.view(*x.shape[:-1], N).to(x.dtype)
+    y, _ = _linear_forward(_ready(x), _ready(weight), _held(adapters), i32)
+    return y if x.dtype is _BF16 else y.to(x.dtype)
 
 
 # ---------------------------------------------------------------- module

@@ -118,6 +118,24 @@ def test_abi_gated_ffn():
     assert call(a12=ctypes.byref(_lib.Adapter(0x1008, 0x1000, None, 8))) == -2
 
 
+def test_abi_adapted_linear_backward():
+    a = _lib.Adapter(0x1000, 0x1000, None, 8)
+    ws = _lib.load().kmoe_adapted_linear_backward_workspace_bytes(100, 64, 72, 2, 8)
+    assert ws >= 2 * (100 * 8 + 2 * 8 * 64 + 2 * 8 * 72)
+    call = _call("kmoe_adapted_linear_backward", [FAKE, FAKE, 100, 64, FAKE, 72, FAKE, 2, ctypes.byref(a), FAKE, FAKE, FAKE,
+                                                  FAKE, FAKE, ws, None])
+    assert call(a2=0, a10=None, a11=None, a12=None) == 0
+    for i in (0, 1, 4, 6, 8, 9):
+        assert call(**{f"a{i}": None}) == -1, i
+    for i in (0, 1, 4, 9, 10, 11, 12, 13):
+        assert call(**{f"a{i}": ODD}) == -2, i
+    assert call(a2=-1) == -2 and call(a3=4) == -2 and call(a5=0) == -2 and call(a7=0) == -2 and call(a7=32768) == -2
+    assert call(a14=ws - 1) == -4 and call(a13=None) == -4
+    for r in (0, 4, 136):
+        assert call(a8=ctypes.byref(_lib.Adapter(0x1000, 0x1000, None, r))) == -2
+    assert call(a8=ctypes.byref(_lib.Adapter(None, 0x1000, None, 8))) == -1
+
+
 def test_abi_adapted_linear():
     a = _lib.Adapter(0x1000, 0x1000, None, 8)
     ws = _lib.load().kmoe_adapted_linear_workspace_bytes(100, 64, 72, 8)
