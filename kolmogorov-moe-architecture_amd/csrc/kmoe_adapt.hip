@@ -324,7 +324,7 @@ extern "C" int kmoe_adapter_inner(const void* x, int64_t T, int K, const int32_t
   if (rb == 1)
     hipLaunchKernelGGL((shrink_kernel<1, 8, 4>), grid, dim3(512), 0, s, g);
   else if (rb == 2)
-    hipLaunchKernelGGL((shrink_kernel<2, 8, 4>), grid, dim3(512), 0, s, g);
+    hipLaunchKernelGGL((shrink_kernel<2, 8, 2>), grid, dim3(512), 0, s, g);
   else
     hipLaunchKernelGGL((shrink_kernel<4, 8, 2>), grid, dim3(512), 0, s, g);
   return kmoe::check_launch("kmoe_adapter_inner");
