@@ -692,52 +692,44 @@ typedef struct {
 
 /* y (T, d) = (act(x w_gate^T) * (x w_up^T)) w_down^T with adapters (each nullable; the gate's and
  * the up projection's of one rank), act a KMOE_ACT_*; w_gate, w_up (F, d), w_down (d, F).
- * The hidden values are rounded to bf16 (of at most 8 rows to twice its bits).       */
+ * The hidden values are rounded to bf16 (of at most KMOE_DENSE_LOST_ROWS rows to twice its bits). */
 size_t kmoe_gated_ffn_workspace_bytes(int64_t T, int d, int F, int rank_gate_up, int rank_down);
 int kmoe_gated_ffn(const void* x, int64_t T, int d, int F, const void* w_gate, const void* w_up, const void* w_down,
                    int act, const int32_t* ids, int n_adapters, const kmoe_adapter* gate, const kmoe_adapter* up,
                    const kmoe_adapter* down, void* y, void* workspace, size_t workspace_bytes, void* stream);
-/* y (T, N) = x w^T with an adapter (nullable): then the workspace begins with the scaled inner
- * products (T, rank) bf16, those of kmoe_adapter_inner.                             */
+/* y (T, N) = x w^T with an adapter (nullable): then the workspace begins with v (2, T, rank) bf16, the
+ * scaled inner products x a^T and what these lost by their rounding (rows without an adapter are left). */
 size_t kmoe_adapted_linear_workspace_bytes(int64_t T, int K, int N, int rank);
 int kmoe_adapted_linear(const void* x, int64_t T, int K, const void* w, int N, const int32_t* ids, int n_adapters,
                         const kmoe_adapter* adapter, void* y, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Their parts, for training.  v (T, rank) bf16 = the scaled inner products of x with a (and v2
- * with a2, of one rank); rows without an adapter are left.                          */
-int kmoe_adapter_inner(const void* x, int64_t T, int K, const int32_t* ids, int n, int rank, const void* a,
-                       const float* scale, void* v, const void* a2, const float* scale2, void* v2, void* stream);
+/* Their parts, for training.  Of T <= KMOE_DENSE_LOST_ROWS rows with `lost`, h, dgate and dup are
+ * (2, T, F), the second T rows what the first lost by their rounding (x, dy, dy2 where they are
+ * operands).                                                                        */
+#define KMOE_DENSE_LOST_ROWS 32
 /* h (T, F) = act(x w_gate^T) * (x w_up^T); with `saved` also what the backward needs, up act'(gate)
- * and act(gate) in 24 bits, in an order of its own, kmoe_dense_saved_bytes(T, F) bytes (then no
- * adapters).  ids NULL: no adapters.                                                */
+ * and act(gate) in 24 bits, in an order of its own, kmoe_dense_saved_bytes(T, F) bytes. */
 size_t kmoe_dense_saved_bytes(int64_t T, int F);
-int kmoe_dense_gate_up(const void* x, int64_t T, int d, const void* w_gate, const void* w_up, int F, int act,
-                       const int32_t* ids, int n_adapters, int rank, const void* v_gate, const void* b_gate,
-                       const void* v_up, const void* b_up, void* h, void* saved, void* stream);
-int kmoe_dense_linear(const void* x, int64_t T, int K, const void* w, int N, const int32_t* ids, int n_adapters,
-                      int rank, const void* v, const void* b, void* y, void* stream);
+int kmoe_dense_gate_up(const void* x, int64_t T, int d, const void* w_gate, const void* w_up, int F, int act, void* h,
+                       int lost, void* saved, void* stream);
+/* y (T, N) = x w^T.                                                                 */
+int kmoe_dense_linear(const void* x, int lost, int64_t T, int K, const void* w, int N, void* y, void* stream);
 /* dgate, dup (T, F): dy w_down times the first and the second of the saved values.   */
 int kmoe_dense_dh(const void* dy, int64_t T, int d, const void* w_down, int F, const void* saved, void* dgate,
-                  void* dup, void* stream);
-/* dx (T, K) = dy w (+ dy2 w2), w (N, K); with adapters (of one product) + u at[i]^T, u (T, rank) the
- * scaled inner products of dy with the transposed b, at (n, K, rank) the transposed a. */
-int kmoe_dense_dx(const void* dy, const void* dy2, int64_t T, int N, const void* w, const void* w2, int K,
-                  const int32_t* ids, int n_adapters, int rank, const void* u, const void* at, void* dx, void* stream);
-/* c (M, N) bf16 or f32 = a^T b, a (T, M), b (T, N), any T.                          */
-int kmoe_dense_wgrad(const void* a, const void* b, int64_t T, int M, int N, void* c, int c_dtype, void* stream);
+                  void* dup, int lost, void* stream);
+/* dx (T, K) = dy w (+ dy2 w2), w (N, K).                                            */
+int kmoe_dense_dx(const void* dy, const void* dy2, int lost, int64_t T, int N, const void* w, const void* w2, int K,
+                  void* dx, void* stream);
+/* c (M, N) bf16 or f32 = a^T b (+ a2^T b2), a (T, M), b (T, N), any T.              */
+int kmoe_dense_wgrad(const void* a, const void* b, const void* a2, const void* b2, int64_t T, int M, int N, void* c,
+                     int c_dtype, void* stream);
 /* The backward of kmoe_adapted_linear with an adapter and without a gradient of w (kmoe_dense_wgrad is
  * that one's): dx (T, K), da (n, r, K) and db (n, N, r) from dy (T, N), each where it is not NULL.
- * v (T, r): the forward's scaled inner products, for db.  At most 32767 adapters.  */
+ * v (2, T, r): the forward's, for db.  At most 32767 adapters.  */
 size_t kmoe_adapted_linear_backward_workspace_bytes(int64_t T, int K, int N, int n_adapters, int rank);
 int kmoe_adapted_linear_backward(const void* dy, const void* x, int64_t T, int K, const void* w, int N,
                                  const int32_t* ids, int n_adapters, const kmoe_adapter* adapter, const void* v,
                                  void* dx, void* da, void* db, void* workspace, size_t workspace_bytes, void* stream);
-/* out[i] = sum over the rows t of adapter i of l[t]^T m[t], l (T, rank), m (T, C): (rank, C), or with
- * outer (C, rank), bf16; zeros for an adapter without rows.                         */
-size_t kmoe_adapter_grad_workspace_bytes(int64_t T, int n, int rank, int C);
-int kmoe_adapter_grad(const void* l, const void* m, int64_t T, const int32_t* ids, int n, int rank, int C, int outer,
-                      void* out, void* workspace, size_t workspace_bytes, void* stream);
-
 #ifdef __cplusplus
 }
 #endif

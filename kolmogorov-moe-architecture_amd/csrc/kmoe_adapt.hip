@@ -11,7 +11,8 @@ namespace {
 
 // ---------------------------------------------------------------- inner products
 // v[t, j] = scale[i] sum_k x[t, k] a[i, j, k], i = ids[t], rounded to bf16: an operand of the outer
-// product's MFMAs, one rounding (half a step of 2^-8) of a term that adds to the projection's.
+// product's MFMAs, one rounding (half a step of 2^-8) of a term that adds to the projection's.  What
+// it loses is kept behind, for the factors' gradients, of which it is the whole operand.
 // A workgroup takes 16 rows, RB blocks of 16 ranks and every gridDim.y-th of the adapters that the rows
 // have (few rows with an adapter each: a workgroup an adapter); its W waves share K.  Each
 // adapter's product is computed for all 16 rows and kept for those that have it: bound by reading
@@ -75,7 +76,11 @@ __global__ __launch_bounds__(W * 64) void shrink_kernel(Shrink g) {
       const int j = j0 + wave * 16 + 4 * lq;
       if (id == cur && j < g.r) {
         const float f = g.scale[z] ? g.scale[z][cur] : 1.0f;
-        *reinterpret_cast<i32x2_t*>(g.v[z] + (t0 + l16) * g.r + j) = pack4(f * s[0], f * s[1], f * s[2], f * s[3]);
+        const float o[4] = {f * s[0], f * s[1], f * s[2], f * s[3]};
+        const i32x2_t w = pack4(o[0], o[1], o[2], o[3]);
+        uint16_t* const to = g.v[z] + (t0 + l16) * g.r + j;
+        *reinterpret_cast<i32x2_t*>(to) = w;
+        kmoe_dense::store_lost(to + g.T * g.r, o, w);
       }
     }
     __syncthreads();
@@ -83,7 +88,8 @@ __global__ __launch_bounds__(W * 64) void shrink_kernel(Shrink g) {
 }
 
 // ---------------------------------------------------------------- gradients of the factors
-// out[i][j, c] = sum over rows t with ids[t] = i of l[t, j] m[t, c], l (T, r), m (T, C), f32 sums.
+// out[i][j, c] = sum over rows t with ids[t] = i of l[t, j] m[t, c], l (2, T, r) (the second T rows what the
+// first lost by their rounding), m (T, C), f32 sums.
 // A workgroup takes an adapter, 128 columns (32 a wave) and a run of rows; of the run it visits the
 // groups of 32 rows in which the adapter occurs, other rows in them read as zeros in both
 // operands.  Operands along t come from LDS by transposing reads, a group's while the next one's rows
@@ -124,8 +130,8 @@ __device__ __forceinline__ bf16x8_t gfrag(const uint8_t* p, int col0, int lane) 
 
 template <int RB, bool OUTER>
 __device__ __forceinline__ void factor_grad(const FactorGrad& g, const FactorJob& job, int block, uint8_t* lds, uint32_t* occurs) {
-  constexpr int LROWB = RB * 32, MROWB = GC * 2, LT = GR * LROWB, STAGE = LT + GR * MROWB;
-  constexpr int NL = RB > 4 ? RB / 4 : 1;  // 16-byte pieces of l a thread holds (of m: 2)
+  constexpr int LROWB = RB * 32, MROWB = GC * 2, LT = GR * LROWB, STAGE = 2 * LT + GR * MROWB;
+  constexpr int NL = RB > 2 ? RB / 2 : 1;  // 16-byte pieces of l a thread holds (of m: 2)
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int l16 = lane & 15, lq = lane >> 4;
   const int c0 = block * GC, me = blockIdx.y;
@@ -156,7 +162,7 @@ __device__ __forceinline__ void factor_grad(const FactorGrad& g, const FactorJob
   i32x4_t mv[2], lv[NL];
   int mid[2], lid[NL];
   auto row_at = [&](int64_t t) { return t < r1 ? t : r1 - 1; };
-  auto fetch = [&](int64_t t0) {  // 32 rows x 16 pieces of m, 32 x 2 RB of l (those not to be used are some row's)
+  auto fetch = [&](int64_t t0) {  // 32 rows x 16 pieces of m, 64 x 2 RB of l (those not to be used are some row's)
 #pragma unroll
     for (int q = 0; q < 2; ++q) {
       const int64_t t = t0 + (tid >> 4) + 16 * q, at = row_at(t);
@@ -167,16 +173,16 @@ __device__ __forceinline__ void factor_grad(const FactorGrad& g, const FactorJob
 #pragma unroll
     for (int q = 0; q < NL; ++q) {
       const int e = tid + 256 * q, j = e % (2 * RB) * 8;
-      const int64_t t = t0 + e / (2 * RB), at = row_at(t);
+      const int64_t t = t0 + e / (2 * RB) % GR, at = row_at(t);
       lid[q] = t < r1 && j < g.r ? g.ids[at] : -1;
-      lv[q] = *reinterpret_cast<const i32x4_t*>(job.l + at * g.r + (j < g.r ? j : 0));
+      lv[q] = *reinterpret_cast<const i32x4_t*>(job.l + (at + (e < GR * 2 * RB ? 0 : g.T)) * g.r + (j < g.r ? j : 0));
     }
   };
   int64_t t0 = next_group();
   if (t0 >= 0) fetch(t0);
   for (int stage = 0; t0 >= 0; stage ^= 1) {
     uint8_t* const lt = lds + stage * STAGE;
-    uint8_t* const mt = lt + LT;
+    uint8_t* const mt = lt + 2 * LT;
     const i32x4_t zero{0, 0, 0, 0};
 #pragma unroll
     for (int q = 0; q < 2; ++q)
@@ -184,7 +190,9 @@ __device__ __forceinline__ void factor_grad(const FactorGrad& g, const FactorJob
 #pragma unroll
     for (int q = 0; q < NL; ++q) {
       const int e = tid + 256 * q;
-      if (e < GR * 2 * RB) *reinterpret_cast<i32x4_t*>(lt + gpos<LROWB>(e / (2 * RB), e % (2 * RB) * 8)) = lid[q] == me ? lv[q] : zero;
+      if (e < 2 * GR * 2 * RB)
+        *reinterpret_cast<i32x4_t*>(lt + e / (GR * 2 * RB) * LT + gpos<LROWB>(e / (2 * RB) % GR, e % (2 * RB) * 8)) =
+            lid[q] == me ? lv[q] : zero;
     }
     t0 = next_group();
     if (t0 >= 0) fetch(t0);
@@ -193,12 +201,14 @@ __device__ __forceinline__ void factor_grad(const FactorGrad& g, const FactorJob
 #pragma unroll
     for (int y = 0; y < 2; ++y) fm[y] = gfrag<MROWB>(mt, wave * 32 + y * 16, lane);
 #pragma unroll
-    for (int b = 0; b < RB; ++b) {
-      const bf16x8_t fl = gfrag<LROWB>(lt, b * 16, lane);
+    for (int b = 0; b < 2 * RB; ++b) {
+      const bf16x8_t fl = gfrag<LROWB>(lt + b / RB * LT, b % RB * 16, lane);
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
-        acc[b][y] = OUTER ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fl, fm[y], acc[b][y], 0, 0, 0)
-                          : __builtin_amdgcn_mfma_f32_16x16x32_bf16(fm[y], fl, acc[b][y], 0, 0, 0);
+      for (int y = 0; y < 2; ++y) {
+        f32x4_t& a = acc[b % RB][y];
+        a = OUTER ? __builtin_amdgcn_mfma_f32_16x16x32_bf16(fl, fm[y], a, 0, 0, 0)
+                  : __builtin_amdgcn_mfma_f32_16x16x32_bf16(fm[y], fl, a, 0, 0, 0);
+      }
     }
   }
   // OUTER: a lane holds column l % 16, ranks 4 (l / 16) .. + 3; else rank l % 16, four columns
@@ -220,7 +230,7 @@ __device__ __forceinline__ void factor_grad(const FactorGrad& g, const FactorJob
 
 template <int RB>
 __global__ __launch_bounds__(256) void factor_grad_kernel(FactorGrad g) {
-  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * GR * (RB * 32 + GC * 2)];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[2 * GR * (2 * RB * 32 + GC * 2)];
   __shared__ uint32_t occurs[GMAXRUN / GR / 32];
   const bool second = (int)blockIdx.x >= g.job[0].blocks;
   const FactorJob& job = g.job[second];
@@ -297,18 +307,9 @@ int kmoe_dense::launch_sum_runs(const float* part, int runs, int64_t total, uint
   return kmoe::check_launch("kmoe sum of runs");
 }
 
-extern "C" int kmoe_adapter_inner(const void* x, int64_t T, int K, const int32_t* ids, int n, int rank, const void* a,
-                                  const float* scale, void* v, const void* a2, const float* scale2, void* v2,
-                                  void* stream) {
-  KMOE_REQUIRE(T >= 0 && T < ((int64_t)1 << 31) && K > 0 && K % 8 == 0, KMOE_ERR_SHAPE,
-               "kmoe_adapter_inner: %lld rows of %d values (a positive multiple of 8)", (long long)T, K);
-  KMOE_REQUIRE(n > 0 && rank > 0 && rank <= KMOE_MAX_RANK && rank % 8 == 0, KMOE_ERR_SHAPE,
-               "kmoe_adapter_inner: %d adapters of rank %d (a multiple of 8, at most %d)", n, rank, KMOE_MAX_RANK);
-  if (T == 0) return KMOE_OK;
-  KMOE_REQUIRE(x && ids && a && v && !a2 == !v2, KMOE_ERR_NULL, "kmoe_adapter_inner: null buffer");
-  KMOE_REQUIRE(aligned(x) && aligned(a) && aligned(v) && aligned(a2) && aligned(v2), KMOE_ERR_SHAPE,
-               "kmoe_adapter_inner: buffers are aligned to 16 bytes");
-  KMOE_REQUIRE(K < 1 << 22, KMOE_ERR_SHAPE, "kmoe_adapter_inner: rows of %d values (below 2^22)", K);
+int kmoe_dense::adapter_inner(const void* x, int64_t T, int K, const int32_t* ids, int n, int rank, const void* a,
+                              const float* scale, void* v, const void* a2, const float* scale2, void* v2, void* stream) {
+  KMOE_REQUIRE(K < 1 << 22, KMOE_ERR_SHAPE, "kmoe adapters: rows of %d values (below 2^22)", K);
   Shrink g{static_cast<const uint16_t*>(x), T, K, ids, n, rank, a2 ? 2 : 1,
            {static_cast<const uint16_t*>(a), static_cast<const uint16_t*>(a2)}, {scale, scale2},
            {static_cast<uint16_t*>(v), static_cast<uint16_t*>(v2)}};
@@ -327,7 +328,7 @@ extern "C" int kmoe_adapter_inner(const void* x, int64_t T, int K, const int32_t
     hipLaunchKernelGGL((shrink_kernel<2, 8, 2>), grid, dim3(512), 0, s, g);
   else
     hipLaunchKernelGGL((shrink_kernel<4, 8, 2>), grid, dim3(512), 0, s, g);
-  return kmoe::check_launch("kmoe_adapter_inner");
+  return kmoe::check_launch("kmoe adapters");
 }
 
 namespace {
@@ -342,7 +343,7 @@ size_t grads_bytes(int64_t T, int n, int rank, int C, int C2) {
 // The gradients of up to two factors (C2 = 0: one) of adapters with rows ids.
 int factor_grads(FactorGrad g, int C, int C2, void* workspace, hipStream_t s) {
   const int64_t runs = g.T > 0 ? runs_of(g.T, g.n, C, C2) : 1;
-  KMOE_REQUIRE(runs <= 65535, KMOE_ERR_SHAPE, "kmoe_adapter_grad: %lld rows", (long long)g.T);
+  KMOE_REQUIRE(runs <= 65535, KMOE_ERR_SHAPE, "kmoe_adapted_linear_backward: %lld rows", (long long)g.T);
   // (a run is whole groups: a wave looks at two of them at a time)
   g.run = kmoe::ceil_div<int64_t>(kmoe::ceil_div<int64_t>(g.T, runs), 64) * 64;
   g.runs = (int)runs, g.part = static_cast<float*>(workspace);
@@ -360,43 +361,18 @@ int factor_grads(FactorGrad g, int C, int C2, void* workspace, hipStream_t s) {
     hipLaunchKernelGGL(factor_grad_kernel<4>, grid, block, 0, s, g);
   else
     hipLaunchKernelGGL(factor_grad_kernel<8>, grid, block, 0, s, g);
-  const int rc = kmoe::check_launch("kmoe_adapter_grad");
+  const int rc = kmoe::check_launch("kmoe_adapted_linear_backward");
   if (rc != KMOE_OK || runs == 1) return rc;
   hipLaunchKernelGGL(sum_runs_kernel, dim3((unsigned)kmoe::ceil_div<int64_t>(g.total, 1024)), dim3(256), 0, s, g.part, (int)runs,
                      g.total, first, g.job[0].out, g.job[1].out);
-  return kmoe::check_launch("kmoe_adapter_grad");
+  return kmoe::check_launch("kmoe_adapted_linear_backward");
 }
 
 }  // namespace
 
-extern "C" size_t kmoe_adapter_grad_workspace_bytes(int64_t T, int n, int rank, int C) {
-  if (T <= 0 || n <= 0 || rank <= 0 || C <= 0) return 0;
-  return grads_bytes(T, n, rank, C, 0);
-}
-
-extern "C" int kmoe_adapter_grad(const void* l, const void* m, int64_t T, const int32_t* ids, int n, int rank, int C,
-                                 int outer, void* out, void* workspace, size_t workspace_bytes, void* stream) {
-  KMOE_REQUIRE(T >= 0 && T < ((int64_t)1 << 31) && C > 0 && C % 8 == 0, KMOE_ERR_SHAPE,
-               "kmoe_adapter_grad: %lld rows of %d values (a positive multiple of 8)", (long long)T, C);
-  KMOE_REQUIRE(n > 0 && n <= 65535 && rank > 0 && rank <= KMOE_MAX_RANK && rank % 8 == 0, KMOE_ERR_SHAPE,
-               "kmoe_adapter_grad: %d adapters (at most 65535) of rank %d (a multiple of 8, at most %d)", n, rank,
-               KMOE_MAX_RANK);
-  KMOE_REQUIRE(out && (T == 0 || (l && m && ids)), KMOE_ERR_NULL, "kmoe_adapter_grad: null buffer");
-  KMOE_REQUIRE(aligned(l) && aligned(m) && aligned(out) && aligned(workspace), KMOE_ERR_SHAPE,
-               "kmoe_adapter_grad: buffers are aligned to 16 bytes");
-  const size_t need = kmoe_adapter_grad_workspace_bytes(T, n, rank, C);
-  KMOE_REQUIRE((workspace || !need) && workspace_bytes >= need, KMOE_ERR_WORKSPACE,
-               "kmoe_adapter_grad: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
-  FactorGrad g{};
-  g.job[0].l = static_cast<const uint16_t*>(l), g.job[0].m = static_cast<const uint16_t*>(m);
-  g.job[0].out = static_cast<uint16_t*>(out), g.job[0].outer = outer;
-  g.ids = ids, g.T = T, g.n = n, g.r = rank;
-  return factor_grads(g, C, 0, workspace, kmoe::as_stream(stream));
-}
-
 extern "C" size_t kmoe_adapted_linear_backward_workspace_bytes(int64_t T, int K, int N, int n_adapters, int rank) {
   if (T < 0 || K <= 0 || N <= 0 || n_adapters <= 0 || rank <= 0) return 0;
-  return piece(T * rank * 2) + piece((int64_t)n_adapters * rank * K * 2) + piece((int64_t)n_adapters * rank * N * 2) +
+  return piece(T * rank * 4) + piece((int64_t)n_adapters * rank * K * 2) + piece((int64_t)n_adapters * rank * N * 2) +
          grads_bytes(T, n_adapters, rank, K, N);
 }
 
@@ -420,7 +396,7 @@ extern "C" int kmoe_adapted_linear_backward(const void* dy, const void* x, int64
                "kmoe_adapted_linear_backward: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
   uint8_t* at = static_cast<uint8_t*>(workspace);
   uint16_t* const u = reinterpret_cast<uint16_t*>(at);
-  uint16_t* const bt = reinterpret_cast<uint16_t*>(at += piece(T * r * 2));
+  uint16_t* const bt = reinterpret_cast<uint16_t*>(at += piece(T * r * 4));
   uint16_t* const a_t = reinterpret_cast<uint16_t*>(at += piece((int64_t)n_adapters * r * N * 2));
   void* const part = at + piece((int64_t)n_adapters * r * K * 2);
   hipStream_t s = kmoe::as_stream(stream);
@@ -430,11 +406,16 @@ extern "C" int kmoe_adapted_linear_backward(const void* dy, const void* x, int64
     const int nr = kmoe::ceil_div(r, 64), blocks = nr * kmoe::ceil_div(N > K ? N : K, 64);
     hipLaunchKernelGGL(turn_kernel, dim3((unsigned)blocks, (unsigned)(dx ? 2 * n_adapters : n_adapters)), dim3(256), 0, s, g);
     if (const int rc = kmoe::check_launch("kmoe_adapted_linear_backward")) return rc;
-    if (const int rc = kmoe_adapter_inner(dy, T, N, ids, n_adapters, r, bt, adapter->scale, u, nullptr, nullptr, nullptr, stream))
+    if (const int rc = kmoe_dense::adapter_inner(dy, T, N, ids, n_adapters, r, bt, adapter->scale, u, nullptr, nullptr, nullptr, stream))
       return rc;
   }
-  if (T > 0 && dx)
-    if (const int rc = kmoe_dense_dx(dy, nullptr, T, N, w, nullptr, K, ids, n_adapters, r, u, a_t, dx, stream)) return rc;
+  if (T > 0 && dx) {
+    kmoe_dense::Args g{};
+    g.a[0] = static_cast<const uint16_t*>(dy), g.b[0] = static_cast<const uint16_t*>(w);
+    g.K = N, g.lda = N, g.ldb = K, g.M = T, g.N = K, g.ldc = K, g.c = dx;
+    g.ad = {ids, {u, nullptr}, {a_t, nullptr}, n_adapters, r};
+    if (const int rc = kmoe_dense::launch_dx_adapt(g, s)) return rc;
+  }
   if (!da && !db) return KMOE_OK;
   FactorGrad g{};
   FactorJob inner{u, static_cast<const uint16_t*>(x), static_cast<uint16_t*>(da), 0, 0, 0, 0};

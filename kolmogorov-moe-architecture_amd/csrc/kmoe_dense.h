@@ -38,9 +38,12 @@
 namespace kmoe_dense {
 
 constexpr int THREADS = 256;
+constexpr int LOST_ROWS = KMOE_DENSE_LOST_ROWS;  // half a tile of 64
+static_assert(LOST_ROWS == 32, "half a tile of 64 rows");
 
-// Low-rank adapters on top of a product: row m gets v[m] . b[ids[m]]^T, v (M, r) bf16 with the scale
-// in it, b (n, N, r); an id outside [0, n) is no adapter.  GATED: [1] are the up half's.
+// Low-rank adapters on top of a product: row m gets v[m] . b[ids[m]]^T, v (2, M, r) bf16 with the scale
+// in it and then what it lost by its rounding, b (n, N, r); an id outside [0, n) is no adapter.  GATED:
+// [1] are the up half's.
 struct Adapt {
   const int32_t* ids;
   const uint16_t* v[2];
@@ -62,7 +65,9 @@ struct Args {
   int c_f32;          // (with runs of K: 1, their sums one after the other, M ldc apart)
   int act;            // GATED
   uint8_t* saved;     // GATED: up act'(gate) and act(gate) for the backward (nullable); DH: the same, read
-  uint16_t* c2;       // DH: the up half's gradient; GATED: what the values in c lost by their rounding (nullable)
+  uint16_t* c2;       // DH: the up half's gradient
+  int64_t lost;       // GATED, DH: elements from a value of c (c2) to what it lost by its rounding; 0: not kept
+  int64_t fold;       // of M <= 32 rows (tiles of 64 rows): elements from A to what it lost; 0: nothing
   Adapt ad;
 };
 
@@ -131,6 +136,19 @@ __device__ __forceinline__ i32x2_t pack4(float a, float b, float c, float d) {
   const uint32_t lo = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{a, b}, bf16x2_t));
   const uint32_t hi = __builtin_bit_cast(uint32_t, __builtin_convertvector(f32x2_t{c, d}, bf16x2_t));
   return i32x2_t{(int)lo, (int)hi};
+}
+// What four values lost by their rounding to w.  Of up to 32 rows the products take that too, at the
+// cost of rows that a tile has anyway: there a rounding is seen in few results, and does not average
+// out.
+__device__ __forceinline__ void store_lost(uint16_t* to, const float* v, i32x2_t w) {
+  float r[4];
+#pragma unroll
+  for (int t = 0; t < 4; ++t) {
+    const uint32_t u = (uint32_t)w[t / 2];
+    r[t] = v[t] - __uint_as_float(t % 2 ? u & 0xffff0000u : u << 16);
+    if (!(r[t] - r[t] == 0.0f)) r[t] = 0.0f;  // (of an infinity nothing)
+  }
+  *reinterpret_cast<i32x2_t*>(to) = pack4(r[0], r[1], r[2], r[3]);
 }
 // What the backward multiplies by, up act'(gate) and act(gate), is held in 24 bits, the top of its f32:
 // in bf16 its rounding would add to those of the products' operands and results, a third of one
@@ -216,11 +234,16 @@ __device__ __forceinline__ void list_adapters(int n_adapters, int rows, int tid,
 // and zeros where not, so the sums go on in their registers.  A zero times an infinity or a NaN of
 // another request's adapter would be a NaN: a turn with such factors is computed one adapter at a
 // time and kept, by selection, for the rows that have it.  Bound by the latency of the factors' reads:
-// those of the next C turns run during these (16 adapters of rank 16 in turn, 48 rows, F 5632, gate
+// those of the next C turns run during these.  What the inner products lost by their rounding takes
+// part too where it costs little (tiles of 64 rows) and where such an error, which reaches a whole
+// row, adds to those of the hidden values' rounding (GATED; the block's result was 1.7 times as far
+// off as with one rounding, now 1.4).
+// (16 adapters of rank 16 in turn, 48 rows, F 5632, gate
 // and up: 4 us; read and selected turn by turn 25).
 template <int BM, int BN, bool GATED>
 struct Outer {
   static constexpr int QA = BM / 64, QB = BN / 64, H = GATED ? 2 : 1, C = QB == 1 ? 8 : 1;
+  static constexpr int HELD = QA == 1 ? 2 : 1, PASSES = GATED && QA > 1 ? 2 : 1;  // both at once where registers are
   const Adapt& ad;
   const int *sid, *list;
   int n_list;
@@ -230,13 +253,14 @@ struct Outer {
   int slot, k0;  // this lane's adapter of them, and its first rank
   int turns;     // of 32 ranks
   int own[2 * QA];
-  bf16x8_t fv[H][2 * QA];
+  bf16x8_t fv[H][HELD][2 * QA];
+  int64_t behind;  // from an inner product to what it lost
   bf16x8_t next[C][2 * QB];
   int next_id[C];
 
-  __device__ __forceinline__ Outer(const Adapt& ad, const int* sid, const int* list, int n_list, int64_t m0, int n0, int N,
-                                   int wm, int wn, int lane)
-      : ad(ad), sid(sid), list(list), n_list(n_list), m0(m0), n0(n0), N(N), wm(wm), wn(wn), lane(lane) {
+  __device__ __forceinline__ Outer(const Adapt& ad, const int* sid, const int* list, int n_list, int64_t m0, int64_t M, int n0,
+                                   int N, int wm, int wn, int lane)
+      : ad(ad), sid(sid), list(list), n_list(n_list), m0(m0), n0(n0), N(N), wm(wm), wn(wn), lane(lane), behind(M * ad.r) {
     const int lq = lane >> 4;
     per = ad.r <= 8 ? 4 : ad.r <= 16 ? 2 : 1;
     slot = per == 4 ? lq : per == 2 ? lq >> 1 : 0;
@@ -267,21 +291,23 @@ struct Outer {
       }
     }
   }
-  __device__ __forceinline__ void load_rows(int s) {
+  __device__ __forceinline__ void load_rows(int pass, int s) {
 #pragma unroll
     for (int h = 0; h < H; ++h)
 #pragma unroll
-      for (int b = 0; b < 2 * QA; ++b) {
-        fv[h][b] = bf16x8_t{};
-        if (s + k0 < ad.r && own[b] >= 0 && ad.b[h])
-          fv[h][b] = *reinterpret_cast<const bf16x8_t*>(ad.v[h] + (m0 + row(b)) * ad.r + s + k0);
-      }
+      for (int p = 0; p < HELD; ++p)
+#pragma unroll
+        for (int b = 0; b < 2 * QA; ++b) {
+          fv[h][p][b] = bf16x8_t{};
+          if (s + k0 < ad.r && own[b] >= 0 && ad.b[h])
+            fv[h][p][b] = *reinterpret_cast<const bf16x8_t*>(ad.v[h] + (m0 + row(b)) * ad.r + s + k0 + (pass + p) * behind);
+        }
   }
   __device__ __forceinline__ void add(f32x4_t (&acc)[2][2][QA][QB]) {
     load(0, 0);
 #pragma unroll 1
-    for (int s = 0; s < ad.r; s += 32) {
-      load_rows(s);
+    for (int pass = 0, s = 0; pass < PASSES; s + 32 < ad.r ? s += 32 : (s = 0, ++pass)) {
+      load_rows(pass, s);
 #pragma unroll 1
       for (int t = 0; t < turns; t += C) {
         bf16x8_t fb[C][2 * QB];
@@ -294,8 +320,8 @@ struct Outer {
         }
         if (t + C < turns)
           load(s, t + C);
-        else if (s + 32 < ad.r)
-          load(s + 32, 0);
+        else if (s + 32 < ad.r || pass + 1 < PASSES)
+          load(s + 32 < ad.r ? s + 32 : 0, 0);
         static_for<0, C>([&](auto ct) {
           constexpr int c = decltype(ct)::value;
           if (C == 1 || t + c < turns) {
@@ -311,13 +337,16 @@ struct Outer {
               constexpr int blk = decltype(bt)::value;
               const bool mine = own[blk] == id[c] && !split;
               const bf16x8_t zero = {};
-              bf16x8_t v[H];
 #pragma unroll
-              for (int h = 0; h < H; ++h) v[h] = mine ? fv[h][blk] : zero;
+              for (int p = 0; p < HELD; ++p) {
+                bf16x8_t v[H];
 #pragma unroll
-              for (int yj = 0; yj < 2 * QB; ++yj) {
-                f32x4_t& a = acc[blk / QA][yj / QB][blk % QA][yj % QB];
-                a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(split ? zero : fb[c][yj], v[GATED ? yj / QB : 0], a, 0, 0, 0);
+                for (int h = 0; h < H; ++h) v[h] = mine ? fv[h][p][blk] : zero;
+#pragma unroll
+                for (int yj = 0; yj < 2 * QB; ++yj) {
+                  f32x4_t& a = acc[blk / QA][yj / QB][blk % QA][yj % QB];
+                  a = __builtin_amdgcn_mfma_f32_16x16x32_bf16(split ? zero : fb[c][yj], v[GATED ? yj / QB : 0], a, 0, 0, 0);
+                }
               }
               __builtin_amdgcn_sched_barrier(0);
             });
@@ -347,8 +376,11 @@ struct Outer {
           constexpr int yj = decltype(yt)::value;
           // (from the sums on, as the others: a row's result does not depend on whom it is computed with)
           f32x4_t& a = acc[blk / QA][yj / QB][blk % QA][yj % QB];
-          const f32x4_t d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-              slot == p ? fb[yj] : zero, slot == p && own[blk] == cur ? fv[GATED ? yj / QB : 0][blk] : zero, a, 0, 0, 0);
+          f32x4_t d = a;
+#pragma unroll
+          for (int q = 0; q < HELD; ++q)
+            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+                slot == p ? fb[yj] : zero, slot == p && own[blk] == cur ? fv[GATED ? yj / QB : 0][q][blk] : zero, d, 0, 0, 0);
 #pragma unroll
           for (int q = 0; q < 4; ++q) a[q] = own[blk] == cur ? d[q] : a[q];
           asm volatile("" : "+a"(a));
@@ -393,14 +425,7 @@ __device__ __forceinline__ void finish(const Args& g, const f32x4_t (&acc)[2][2]
           if (m < g.M && n < g.N) {
             const i32x2_t w = pack4(h[0], h[1], h[2], h[3]);
             *reinterpret_cast<i32x2_t*>(static_cast<uint16_t*>(g.c) + m * g.ldc + n) = w;
-            if (g.c2) {
-              const auto lost = [&](int t) {
-                const uint32_t u = (uint32_t)w[t / 2];
-                const float r = h[t] - __uint_as_float(t % 2 ? u & 0xffff0000u : u << 16);
-                return r - r == 0.0f ? r : 0.0f;  // (of an infinity nothing)
-              };
-              *reinterpret_cast<i32x2_t*>(g.c2 + m * g.ldc + n) = pack4(lost(0), lost(1), lost(2), lost(3));
-            }
+            if (g.lost) store_lost(static_cast<uint16_t*>(g.c) + g.lost + m * g.ldc + n, h, w);
           }
           if (g.saved) {  // (whole blocks: the buffer has them)
             uint8_t* const block = saved_block(g.saved, g.N, m, n16);
@@ -426,9 +451,13 @@ __device__ __forceinline__ void finish(const Args& g, const f32x4_t (&acc)[2][2]
             load24(block, lane, p);
             load24(block + SAVED_BLOCK / 2, lane, q);
             if (m < g.M && n < g.N) {
-              *reinterpret_cast<i32x2_t*>(static_cast<uint16_t*>(g.c) + at) =
-                  pack4(v[0] * p[0], v[1] * p[1], v[2] * p[2], v[3] * p[3]);
-              *reinterpret_cast<i32x2_t*>(g.c2 + at) = pack4(v[0] * q[0], v[1] * q[1], v[2] * q[2], v[3] * q[3]);
+#pragma unroll
+              for (int t = 0; t < 4; ++t) p[t] *= v[t], q[t] *= v[t];
+              const i32x2_t dg = pack4(p[0], p[1], p[2], p[3]), du = pack4(q[0], q[1], q[2], q[3]);
+              uint16_t* const c = static_cast<uint16_t*>(g.c);
+              *reinterpret_cast<i32x2_t*>(c + at) = dg;
+              *reinterpret_cast<i32x2_t*>(g.c2 + at) = du;
+              if (g.lost) store_lost(c + g.lost + at, p, dg), store_lost(g.c2 + g.lost + at, q, du);
             }
           } else if (m < g.M && n < g.N) {
             if (g.c_f32)
@@ -452,16 +481,17 @@ struct Loads {  // of one operand's stage tile (R rows or columns, 32 KS of K): 
   int kpos;         // first K of the first piece's chunk
 
   // rows: how many of the tile's R exist (what is past them reads as zeros, for nothing: a tile of few
-  // rows costs the other operand's bytes); split: its halves are the same R / 2 rows of two matrices
-  __device__ __forceinline__ void init(int64_t ld, int64_t rows, bool split, int wave, int lane) {
+  // rows costs the other operand's bytes); split: its halves are the same R / 2 rows of two matrices;
+  // fold: the second half is the same rows, that many elements behind
+  __device__ __forceinline__ void init(int64_t ld, int64_t rows, bool split, int64_t fold, int wave, int lane) {
 #pragma unroll
     for (int q = 0; q < N; ++q) {
       const int row = (wave + 4 * q) * (64 / CPR) + lane / CPR;
       if constexpr (!STRIDED) {
         // (rows of a lane's pieces are multiples of 32 apart: the same chunk of K)
         const int chunk = (lane % CPR) ^ ((row >> 1) & (CPR - 1));
-        const int r = split ? row % (R / 2) : row;
-        off[q] = r < rows ? (uint32_t)(r * ld * 2) + chunk * 16 : NOWHERE;
+        const int r = split || fold ? row % (R / 2) : row;
+        off[q] = r < rows ? (uint32_t)((r * ld + (row >= R / 2 ? fold : 0)) * 2) + chunk * 16 : NOWHERE;
         if (q == 0) kpos = chunk * 8;
       } else {
         const int chunk = (lane % CPR) ^ (strided_swz<2 * P>(row) << 1);
@@ -574,10 +604,11 @@ __global__ __launch_bounds__(THREADS, (side_by_side<BM, BN, KS, STAGES>)) __attr
   // where the step to load lies, and how much of K is left from it on
   const int64_t row_a = SA ? 1 : g.lda, row_b = SB ? 1 : g.ldb;
   const int64_t step_a = SA ? (int64_t)SK * g.lda : SK, step_b = SB ? (int64_t)SK * g.ldb : SK;
+  const int64_t fold = BM == 64 && !SA && !GATED ? g.fold : 0;
   LoadA la;
   LoadB lb;
-  la.init(g.lda, g.M - m0, false, wave, lane);
-  lb.init(g.ldb, g.N - n0, GATED, wave, lane);
+  la.init(g.lda, g.M - m0, false, fold, wave, lane);
+  lb.init(g.ldb, g.N - n0, GATED, 0, wave, lane);
   const uint16_t* pa = g.a[0] + m0 * row_a;
   const uint16_t* pb = g.b[0] + n0 * row_b;
   const int64_t second = GATED ? g.b[1] - g.b[0] : 0;  // from the gate's to the up projection's rows
@@ -609,8 +640,8 @@ __global__ __launch_bounds__(THREADS, (side_by_side<BM, BN, KS, STAGES>)) __attr
         left = g.K, part = 2;
         pa = g.a[1] + m0 * row_a;
         pb = g.b[1] + n0 * row_b;
-        la.init(g.lda, g.M - m0, false, wave, lane);
-        lb.init(g.ldb, g.N - n0, GATED, wave, lane);
+        la.init(g.lda, g.M - m0, false, fold, wave, lane);
+        lb.init(g.ldb, g.N - n0, GATED, 0, wave, lane);
       }
       if (left < SK) la.cut(left), lb.cut(left);
     }
@@ -726,9 +757,18 @@ __global__ __launch_bounds__(THREADS, (side_by_side<BM, BN, KS, STAGES>)) __attr
   } while ((n += 2) < nk * KS);
   hold();
   wait_vmcnt<0>();  // (the zeros past the end are on their way into this workgroup's LDS)
+  if constexpr (BM == 64 && !SA && !GATED) {
+    if (fold) {  // (both halves' rows lie in one lane; the second half's are past M)
+#pragma unroll
+      for (int y = 0; y < 2; ++y)
+#pragma unroll
+        for (int j = 0; j < QB; ++j) acc[0][y][0][j] += acc[1][y][0][j];
+      hold();
+    }
+  }
   if constexpr (ADAPT) {
     if (n_list) {
-      Outer<BM, BN, GATED> outer(g.ad, sid, list, n_list, m0, n0, g.N, wm, wn, lane);
+      Outer<BM, BN, GATED> outer(g.ad, sid, list, n_list, m0, g.M, n0, g.N, wm, wn, lane);
       outer.add(acc);
     }
     hold();

@@ -14,9 +14,14 @@ int launch_dx(const Args& g, hipStream_t s);            // a b
 int launch_dx_two(const Args& g, hipStream_t s);        // a0 b0 + a1 b1
 int launch_dx_adapt(const Args& g, hipStream_t s);
 int launch_wgrad(const Args& g, hipStream_t s);         // a^T b
+int launch_wgrad_two(const Args& g, hipStream_t s);     // a0^T b0 + a1^T b1
 // a b^T of few rows in runs of K (kmoe_ffn.hip)
 int launch_linear_runs(const Args& g, hipStream_t s);
 int launch_linear_runs_adapt(const Args& g, hipStream_t s);
+// v (2, T, rank): the scaled inner products of x with a, then what these lost by their rounding (and v2 with a2, of
+// one rank); rows without an adapter are left.  The caller has checked the sizes.
+int adapter_inner(const void* x, int64_t T, int K, const int32_t* ids, int n, int rank, const void* a, const float* scale,
+                  void* v, const void* a2, const float* scale2, void* v2, void* stream);
 // out = the sum of `runs` arrays of `total` f32 in their order, as bf16
 int launch_sum_runs(const float* part, int runs, int64_t total, uint16_t* out, hipStream_t s);
 
@@ -79,6 +84,11 @@ int launch_tile(const Args& g, hipStream_t s) {
 
 template <bool SA, bool SB, int EPI, bool ADAPT = false>
 int launch_any(const Args& g, hipStream_t s) {
+  if (g.fold) {
+    KMOE_REQUIRE(g.M <= LOST_ROWS, KMOE_ERR_SHAPE, "kmoe dense product: %lld rows with what they lost (at most %d)",
+                 (long long)g.M, LOST_ROWS);
+    return launch_tile<64, 64, 2, 4, SA, SB, EPI, ADAPT>(g, s);
+  }
   const double steps = (double)kmoe::ceil_div(g.K, 64) * (EPI == EPI_TWO ? 2 : 1);
   // (with adapters not the largest tile: its sums fill the registers)
   switch (choose_tile(g.M, (int64_t)g.N * (EPI == EPI_GATED ? 2 : 1), steps, ADAPT ? T192 : T256)) {

@@ -13,9 +13,8 @@ namespace {
 // weights from HBM: 5632 x 2048 9.7 us, 2048 x 5632 8.2; the gate and up rows of the block are
 // enough for the tiles of 64 x 64, 11.7 against 14.1 us).  An adapter is added in f32: a thread sums
 // all ranks of one result, its factors on their way with the first weights.
-// Of at most 8 rows the upper 8 of the MFMA's 16 are free: there go what the block's hidden values lost by
-// their rounding to bf16, for nothing, and so the block's result is rounded once and not twice.
-constexpr int FEW = 16, FEW_EXACT = 8;
+// Of at most 8 rows what they lost by their rounding goes into the upper 8 of the MFMA's 16.
+constexpr int FEW = 16, FEW_LOST = 8;
 
 template <int ROWS, bool ADAPT>
 __global__ __launch_bounds__(512) void few_kernel(Args g) {
@@ -31,9 +30,9 @@ __global__ __launch_bounds__(512) void few_kernel(Args g) {
   Stream16<1, W, D> st;
   st.w[0] = g.b[0] + (int64_t)n0 * g.ldb, st.x = g.a[0], st.K = g.K;
   st.woff[0] = l16 < ROWS && n0 + l16 < g.N ? (uint32_t)(l16 * g.ldb) * 2 : NOWHERE;
-  const int lost = g.a[1] ? l16 - 8 : -1;  // (the second rows lie less than 2^27 bytes behind the first ones)
+  const int lost = g.fold ? l16 - 8 : -1;  // (less than 2^27 bytes behind)
   st.xoff = l16 < g.M                  ? (uint32_t)(l16 * g.lda) * 2
-            : lost >= 0 && lost < g.M  ? (uint32_t)(g.a[1] - g.a[0] + lost * g.lda) * 2
+            : lost >= 0 && lost < g.M  ? (uint32_t)(g.fold + lost * g.lda) * 2
                                        : NOWHERE;
   f32x4_t acc[1] = {f32x4_t{0.0f, 0.0f, 0.0f, 0.0f}};
   st.start(wave, lane);
@@ -43,20 +42,24 @@ __global__ __launch_bounds__(512) void few_kernel(Args g) {
       const uint16_t* const b = g.ad.b[0] + ((int64_t)id * g.N + n0 + an) * g.ad.r;
       const uint16_t* const v = g.ad.v[0] + at * g.ad.r;
       for (int s = 0; s < g.ad.r; s += 32) {
-        i32x4_t bv[4], vv[4];
+        i32x4_t bv[4], vv[4], lv[4];
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           const int j = s + 8 * q < g.ad.r ? s + 8 * q : s;
           bv[q] = *reinterpret_cast<const i32x4_t*>(b + j);
           vv[q] = *reinterpret_cast<const i32x4_t*>(v + j);
+          lv[q] = *reinterpret_cast<const i32x4_t*>(v + g.M * g.ad.r + j);
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
           if (s + 8 * q >= g.ad.r) break;
 #pragma unroll
-          for (int c = 0; c < 4; ++c)
-            sum += __uint_as_float((uint32_t)bv[q][c] << 16) * __uint_as_float((uint32_t)vv[q][c] << 16) +
-                   __uint_as_float((uint32_t)bv[q][c] & 0xffff0000u) * __uint_as_float((uint32_t)vv[q][c] & 0xffff0000u);
+          for (int c = 0; c < 4; ++c) {
+            auto half = [&](const i32x4_t& w, int i) {
+              return __uint_as_float(i ? (uint32_t)w[c] & 0xffff0000u : (uint32_t)w[c] << 16);
+            };
+            sum += half(bv[q], 0) * (half(vv[q], 0) + half(lv[q], 0)) + half(bv[q], 1) * (half(vv[q], 1) + half(lv[q], 1));
+          }
         }
       }
     }
@@ -71,7 +74,7 @@ __global__ __launch_bounds__(512) void few_kernel(Args g) {
   f32x4_t s = part[0][lane];
 #pragma unroll
   for (int k = 1; k < W; ++k) s += part[k][lane];
-  if (g.a[1]) {
+  if (g.fold) {
 #pragma unroll
     for (int c = 0; c < 4; ++c) s[c] += __shfl(s[c], lane | 8, 64);
   }
@@ -97,8 +100,8 @@ int launch_few(const Args& g, hipStream_t s) {
 
 // Runs of K in which a projection of more rows is computed, where its tiles leave units idle: partial
 // sums in f32, summed by a second launch (some 5 us with the partial sums' way).  1: in one.
-int linear_runs(int64_t T, int K, int N) {
-  if (T <= FEW) return 1;
+int linear_runs(int64_t T, int K, int N, bool lost) {
+  if (T <= (lost ? FEW_LOST : FEW)) return 1;
   const int64_t tiles = kmoe::ceil_div<int64_t>(T, 64) * kmoe::ceil_div(N, 64), cus = kmoe::cu_count();
   const int steps = kmoe::ceil_div(K, 64);
   double least;
@@ -129,20 +132,21 @@ int check_adapter(const char* who, const kmoe_adapter* a, int n) {
   return KMOE_OK;
 }
 
-size_t runs_bytes(int64_t T, int K, int N) {
-  const int runs = T > 0 && K > 0 && N > 0 ? linear_runs(T, K, N) : 1;
+size_t runs_bytes(int64_t T, int K, int N, bool lost) {
+  const int runs = T > 0 && K > 0 && N > 0 ? linear_runs(T, K, N, lost) : 1;
   return runs > 1 ? piece((int64_t)runs * T * N * 4) : 0;
 }
 
 // y = x w^T with the adapter's outer product, whose inner products v are there; part: runs_bytes.
-// lost: of T <= FEW_EXACT rows what x lost by its rounding, behind x (nullable).
-int project(const void* x, const void* lost, int64_t T, int K, const void* w, int N, const int32_t* ids, int n,
+// lost: x is (2, T, K), the second T rows what the first ones lost.
+int project(const void* x, bool lost, int64_t T, int K, const void* w, int N, const int32_t* ids, int n,
             const kmoe_adapter* ad, const void* v, void* y, void* part, hipStream_t s) {
   Args g{};
-  g.a[0] = bf(x), g.a[1] = bf(lost), g.b[0] = bf(w), g.K = K, g.lda = K, g.ldb = K, g.M = T, g.N = N, g.ldc = N, g.c = y;
+  g.a[0] = bf(x), g.b[0] = bf(w), g.K = K, g.lda = K, g.ldb = K, g.M = T, g.N = N, g.ldc = N, g.c = y;
+  g.fold = lost ? T * K : 0;
   if (ad) g.ad = {ids, {bf(v), nullptr}, {bf(ad->b), nullptr}, n, ad->rank};
-  if (T <= FEW) return ad ? launch_few<true>(g, s) : launch_few<false>(g, s);
-  const int runs = linear_runs(T, K, N);
+  if (T <= (lost ? FEW_LOST : FEW)) return ad ? launch_few<true>(g, s) : launch_few<false>(g, s);
+  const int runs = linear_runs(T, K, N, lost);
   if (runs == 1) return ad ? launch_linear_adapt(g, s) : launch_linear(g, s);
   g.k_run = (int)run_of(K, runs), g.c = part, g.c_f32 = 1;
   if (const int rc = ad ? launch_linear_runs_adapt(g, s) : launch_linear_runs(g, s)) return rc;
@@ -153,7 +157,7 @@ int project(const void* x, const void* lost, int64_t T, int K, const void* w, in
 
 extern "C" size_t kmoe_adapted_linear_workspace_bytes(int64_t T, int K, int N, int rank) {
   if (T <= 0) return 0;
-  return piece(T * (rank > 0 ? rank : 0) * 2) + runs_bytes(T, K, N);
+  return piece(T * (rank > 0 ? rank : 0) * 4) + runs_bytes(T, K, N, false);
 }
 
 extern "C" int kmoe_adapted_linear(const void* x, int64_t T, int K, const void* w, int N, const int32_t* ids, int n_adapters,
@@ -170,17 +174,18 @@ extern "C" int kmoe_adapted_linear(const void* x, int64_t T, int K, const void* 
   KMOE_REQUIRE((workspace || !need) && workspace_bytes >= need, KMOE_ERR_WORKSPACE,
                "kmoe_adapted_linear: workspace of %zu bytes, %zu are needed", workspace_bytes, need);
   if (adapter) {
-    const int rc = kmoe_adapter_inner(x, T, K, ids, n_adapters, adapter->rank, adapter->a, adapter->scale, workspace, nullptr,
-                                      nullptr, nullptr, stream);
+    const int rc = adapter_inner(x, T, K, ids, n_adapters, adapter->rank, adapter->a, adapter->scale, workspace, nullptr,
+                                 nullptr, nullptr, stream);
     if (rc) return rc;
   }
-  return project(x, nullptr, T, K, w, N, ids, n_adapters, adapter, workspace, y,
-                 static_cast<uint8_t*>(workspace) + piece(T * (adapter ? adapter->rank : 0) * 2), kmoe::as_stream(stream));
+  return project(x, false, T, K, w, N, ids, n_adapters, adapter, workspace, y,
+                 static_cast<uint8_t*>(workspace) + piece(T * (adapter ? adapter->rank : 0) * 4), kmoe::as_stream(stream));
 }
 
 extern "C" size_t kmoe_gated_ffn_workspace_bytes(int64_t T, int d, int F, int rank_gate_up, int rank_down) {
   if (T <= 0) return 0;
-  return piece(T * F * (T <= FEW_EXACT ? 4 : 2)) + 2 * piece(T * rank_gate_up * 2) + piece(T * rank_down * 2) + runs_bytes(T, F, d);
+  const bool lost = T <= LOST_ROWS;
+  return piece(T * F * (lost ? 4 : 2)) + 2 * piece(T * rank_gate_up * 4) + piece(T * rank_down * 4) + runs_bytes(T, F, d, lost);
 }
 
 extern "C" int kmoe_gated_ffn(const void* x, int64_t T, int d, int F, const void* w_gate, const void* w_up,
@@ -205,31 +210,31 @@ extern "C" int kmoe_gated_ffn(const void* x, int64_t T, int d, int F, const void
                kmoe_gated_ffn_workspace_bytes(T, d, F, rgu, rd));
   uint8_t* w = static_cast<uint8_t*>(workspace);
   void* const h = w;
-  void* const lost = T <= FEW_EXACT ? w + T * F * 2 : nullptr;
+  const bool lost = T <= LOST_ROWS;
   void* const vg = w += piece(T * F * (lost ? 4 : 2));
-  void* const vu = w += piece(T * rgu * 2);
-  void* const vd = w += piece(T * rgu * 2);
-  void* const part = w += piece(T * rd * 2);
+  void* const vu = w += piece(T * rgu * 4);
+  void* const vd = w += piece(T * rgu * 4);
+  void* const part = w += piece(T * rd * 4);
   hipStream_t s = kmoe::as_stream(stream);
   int rc = KMOE_OK;
   if (rgu) {
     if (gate && up)
-      rc = kmoe_adapter_inner(x, T, d, ids, n_adapters, rgu, gate->a, gate->scale, vg, up->a, up->scale, vu, stream);
+      rc = adapter_inner(x, T, d, ids, n_adapters, rgu, gate->a, gate->scale, vg, up->a, up->scale, vu, stream);
     else
-      rc = kmoe_adapter_inner(x, T, d, ids, n_adapters, rgu, (gate ? gate : up)->a, (gate ? gate : up)->scale, gate ? vg : vu,
+      rc = adapter_inner(x, T, d, ids, n_adapters, rgu, (gate ? gate : up)->a, (gate ? gate : up)->scale, gate ? vg : vu,
                               nullptr, nullptr, nullptr, stream);
     if (rc) return rc;
   }
   Args g{};
   g.a[0] = bf(x), g.b[0] = bf(w_gate), g.b[1] = bf(w_up), g.K = d, g.lda = d, g.ldb = d, g.M = T, g.N = F;
-  g.ldc = F, g.c = h, g.c2 = static_cast<uint16_t*>(lost), g.act = act;
+  g.ldc = F, g.c = h, g.lost = lost ? T * F : 0, g.act = act;
   if (rgu)
     g.ad = {ids, {gate ? bf(vg) : nullptr, up ? bf(vu) : nullptr}, {gate ? bf(gate->b) : nullptr, up ? bf(up->b) : nullptr},
             n_adapters, rgu};
   rc = rgu ? launch_gated_adapt(g, s) : launch_gated(g, s);
   if (rc) return rc;
   if (down) {
-    rc = kmoe_adapter_inner(h, T, F, ids, n_adapters, rd, down->a, down->scale, vd, nullptr, nullptr, nullptr, stream);
+    rc = adapter_inner(h, T, F, ids, n_adapters, rd, down->a, down->scale, vd, nullptr, nullptr, nullptr, stream);
     if (rc) return rc;
   }
   return project(h, lost, T, F, w_down, d, ids, n_adapters, down, vd, y, part, s);

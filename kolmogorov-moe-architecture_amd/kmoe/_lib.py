@@ -24,6 +24,7 @@ SCORES = {"softmax": 0, "sigmoid": 1}
 ACTIVATIONS = {"silu": 0, "gelu": 1, "gelu_tanh": 2, "relu": 3}
 MAX_EXPERTS = 64
 MAX_RANK = 128
+LOST_ROWS = 32
 ROUTER_HIDDEN = 128
 
 _vp = ctypes.c_void_p
@@ -134,17 +135,14 @@ _SIGNATURES = {
     "kmoe_gated_ffn": (_i32, [_vp, _i64, _i32, _i32, _vp, _vp, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "kmoe_adapted_linear_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
     "kmoe_adapted_linear": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _sz, _vp]),
-    "kmoe_adapter_inner": (_i32, [_vp, _i64, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
     "kmoe_dense_saved_bytes": (_sz, [_i64, _i32]),
-    "kmoe_dense_gate_up": (_i32, [_vp, _i64, _i32, _vp, _vp, _i32, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
-    "kmoe_dense_linear": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp]),
-    "kmoe_dense_dh": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _vp]),
-    "kmoe_dense_dx": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _i32, _vp, _i32, _i32, _vp, _vp, _vp, _vp]),
-    "kmoe_dense_wgrad": (_i32, [_vp, _vp, _i64, _i32, _i32, _vp, _i32, _vp]),
+    "kmoe_dense_gate_up": (_i32, [_vp, _i64, _i32, _vp, _vp, _i32, _i32, _vp, _i32, _vp, _vp]),
+    "kmoe_dense_linear": (_i32, [_vp, _i32, _i64, _i32, _vp, _i32, _vp, _vp]),
+    "kmoe_dense_dh": (_i32, [_vp, _i64, _i32, _vp, _i32, _vp, _vp, _vp, _i32, _vp]),
+    "kmoe_dense_dx": (_i32, [_vp, _vp, _i32, _i64, _i32, _vp, _vp, _i32, _vp, _vp]),
+    "kmoe_dense_wgrad": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _i32, _vp, _i32, _vp]),
     "kmoe_adapted_linear_backward_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32, _i32]),
     "kmoe_adapted_linear_backward": (_i32, [_vp, _vp, _i64, _i32, _vp, _i32, _vp, _i32, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
-    "kmoe_adapter_grad_workspace_bytes": (_sz, [_i64, _i32, _i32, _i32]),
-    "kmoe_adapter_grad": (_i32, [_vp, _vp, _i64, _vp, _i32, _i32, _i32, _i32, _vp, _vp, _sz, _vp]),
     # the optimizer step
     "kmoe_adamw": (_i32, [_vp, _vp, _vp, _vp, _i32, _vp, _i32, _i32, _i32, _f32, _vp, _f64, _f64, _f32, _f32, _vp, _vp]),
     "kmoe_adamw_values": (_i32, [_vp, _vp, _vp, _vp, _i64, _i32, _vp, _vp, _vp]),

@@ -7,11 +7,11 @@
 * adapted_linear: a shared projection with low-rank adapters of many requests in one batch,
   row t with the adapter ids[t]; also on all three projections of the block.
 
-Numerics: bf16 operands, f32 sums.  What is rounded to bf16 between the products: the block's
-hidden values h = act(g) u (an operand of the down product; of up to 8 rows in a call without
-gradients they keep 16 bits), the gradients of its pre-activations, and an
-adapter's inner products with their scale.  What the backward keeps of the pre-activations, u act'(g)
-and act(g), has 16 bits of precision.
+Numerics: bf16 operands, f32 sums.  What is rounded to bf16 between the products: the block's hidden
+values h = act(g) u and the gradients of its pre-activations (of up to 32 rows both keep 16 bits, as
+two bf16: in few results a rounding does not average out), and an adapter's inner products with
+their scale (16 bits for the factors' gradients).  What the backward keeps of the pre-activations,
+u act'(g) and act(g), has 16 bits of precision.
 """
 from __future__ import annotations
 
@@ -168,22 +168,23 @@ def _linear_forward(x, w, ad, ids):
 
 
 # ---------------------------------------------------------------- parts of the backward
-def _dense_dx(dy, w, dy2=None, w2=None):
-    T, N = dy.shape
-    K = w.shape[1]
+def _dense_dx(dy, w, T, dy2=None, w2=None):
+    """dy w (+ dy2 w2) of T rows; rows behind those are what they lost by their rounding."""
+    N, K = w.shape
     dx = torch.empty(T, K, device=dy.device, dtype=_BF16)
-    _lib.call("kmoe_dense_dx", ptr(dy), ptr(dy2), T, N, ptr(w), ptr(w2), K, None, 0, 0, None, None, ptr(dx), _stream(dy))
+    _lib.call("kmoe_dense_dx", ptr(dy), ptr(dy2), int(dy.shape[0] > T), T, N, ptr(w), ptr(w2), K, ptr(dx), _stream(dy))
     return dx
 
 
-def _dense_wgrad(a, b, dtype):
-    """a^T b, (M, N), in the weight's type."""
-    T, M = a.shape
-    N = b.shape[1]
+def _dense_wgrad(a, b, T, dtype):
+    """a^T b of T rows, (M, N), in the weight's type; rows behind those (of one of the two) are what they
+    lost by their rounding."""
+    M, N = a.shape[1], b.shape[1]
     dt = torch.float32 if dtype == torch.float32 else _BF16
     c = torch.empty(M, N, device=a.device, dtype=dt)
-    _lib.call("kmoe_dense_wgrad", ptr(a), ptr(b), T, M, N, ptr(c), _lib.DTYPE_F32 if dt == torch.float32 else _lib.DTYPE_BF16,
-              _stream(a))
+    a2, b2 = (a[-T:], b[-T:]) if T and max(a.shape[0], b.shape[0]) > T else (None, None)
+    _lib.call("kmoe_dense_wgrad", ptr(a), ptr(b), ptr(a2), ptr(b2), T, M, N, ptr(c),
+              _lib.DTYPE_F32 if dt == torch.float32 else _lib.DTYPE_BF16, _stream(a))
     return c
 
 
@@ -201,15 +202,15 @@ class _GatedFFNFn(torch.autograd.Function):
         xr, bg, bu, bd = _ready(x), _ready(wg), _ready(wu), _ready(wd)
         F, d = bg.shape
         T = xr.numel() // d
-        h = xr.new_empty((T, F))
+        lost = int(T <= _lib.LOST_ROWS)
+        h = xr.new_empty((T + T * lost, F))
         saved = torch.empty(max(_lib.load().kmoe_dense_saved_bytes(T, F), 16), device=x.device, dtype=torch.uint8)
         y = xr.new_empty(x.shape)
         with _device(x.device):
             with _Stage("ffn_gate_up"):
-                _lib.call("kmoe_dense_gate_up", ptr(xr), T, d, ptr(bg), ptr(bu), F, act, None, 0, 0, None, None, None, None,
-                          ptr(h), ptr(saved), _stream(x))
+                _lib.call("kmoe_dense_gate_up", ptr(xr), T, d, ptr(bg), ptr(bu), F, act, ptr(h), lost, ptr(saved), _stream(x))
             with _Stage("ffn_down"):
-                _lib.call("kmoe_dense_linear", ptr(h), T, F, ptr(bd), d, None, 0, 0, None, None, ptr(y), _stream(x))
+                _lib.call("kmoe_dense_linear", ptr(h), lost, T, F, ptr(bd), d, ptr(y), _stream(x))
         ctx.save_for_backward(xr, h, saved, bg, bu, bd, *_copied((x, xr), (wg, bg), (wu, bu), (wd, bd)))
         ctx.meta = (x.dtype, wg.dtype, wu.dtype, wd.dtype)
         return y if x.dtype is _BF16 else y.to(x.dtype)
@@ -220,7 +221,7 @@ class _GatedFFNFn(torch.autograd.Function):
         xr, h, saved, bg, bu, bd = ctx.saved_tensors[:6]
         dtypes = ctx.meta
         F, d = bg.shape
-        T = h.shape[0]
+        T = xr.numel() // d
         need_x, need_g, need_u, need_d = ctx.needs_input_grad[:4]
         dy2, x2d = _ready(dy).view(T, d), xr.view(T, d)
         dx = dg = du = dwg = dwu = dwd = None
@@ -228,17 +229,18 @@ class _GatedFFNFn(torch.autograd.Function):
             if need_x or need_g or need_u:
                 dg, du = torch.empty_like(h), torch.empty_like(h)
                 with _Stage("bwd_ffn_dh"):
-                    _lib.call("kmoe_dense_dh", ptr(dy2), T, d, ptr(bd), F, ptr(saved), ptr(dg), ptr(du), _stream(xr))
+                    _lib.call("kmoe_dense_dh", ptr(dy2), T, d, ptr(bd), F, ptr(saved), ptr(dg), ptr(du),
+                              int(h.shape[0] > T), _stream(xr))
             if need_x:
                 with _Stage("bwd_ffn_dx"):
-                    dx = _dense_dx(dg, bg, du, bu).view(xr.shape).to(dtypes[0])
+                    dx = _dense_dx(dg, bg, T, du, bu).view(xr.shape).to(dtypes[0])
             with _Stage("bwd_ffn_wgrad"):
                 if need_g:
-                    dwg = _dense_wgrad(dg, x2d, dtypes[1])
+                    dwg = _dense_wgrad(dg, x2d, T, dtypes[1])
                 if need_u:
-                    dwu = _dense_wgrad(du, x2d, dtypes[2])
+                    dwu = _dense_wgrad(du, x2d, T, dtypes[2])
                 if need_d:
-                    dwd = _dense_wgrad(dy2, h, dtypes[3])
+                    dwd = _dense_wgrad(dy2, h, T, dtypes[3])
         return dx, dwg, dwu, dwd, None
 
 
@@ -326,9 +328,9 @@ class _AdaptedFn(torch.autograd.Function):
                 _lib.call("kmoe_adapted_linear_backward", ptr(dy2), ptr(xr), T, K, ptr(bw), N, ptr(ids), n,
                           _struct(Adapters(ba, bb, scale)), ptr(v), ptr(dx), ptr(da), ptr(db), ptr(ws), wsb, _stream(xr))
             elif need_x:
-                dx = _dense_dx(dy2.view(T, N), bw).view(xr.shape)
+                dx = _dense_dx(dy2.view(T, N), bw, T).view(xr.shape)
             if need_w:
-                dw = _dense_wgrad(dy2.view(T, N), xr.view(T, K), dtypes[1])
+                dw = _dense_wgrad(dy2.view(T, N), xr.view(T, K), T, dtypes[1])
         return tuple(g if g is None or g.dtype is t else g.to(t) for g, t in zip((dx, dw, da, db), dtypes)) + (None, None)
 
 

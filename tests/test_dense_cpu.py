@@ -147,40 +147,31 @@ def test_abi_adapted_linear():
 
 
 def test_abi_parts():
-    call = _call("kmoe_adapter_inner", [FAKE, 100, 64, FAKE, 2, 8, FAKE, FAKE, FAKE, None, None, None, None])
+    call = _call("kmoe_dense_gate_up", [FAKE, 100, 64, FAKE, FAKE, 72, 0, FAKE, 0, FAKE, None])
     assert call(a1=0) == 0
-    for i in (0, 3, 6, 8):
+    for i in (0, 3, 4, 7):
         assert call(**{f"a{i}": None}) == -1, i
-    assert call(a9=FAKE) == -1 and call(a2=60) == -2 and call(a4=0) == -2 and call(a5=12) == -2 and call(a6=ODD) == -2
-    call = _call("kmoe_dense_gate_up", [FAKE, 100, 64, FAKE, FAKE, 72, 0, FAKE, 2, 8, FAKE, FAKE, FAKE, FAKE, FAKE, None, None])
-    assert call(a1=0) == 0
-    for i in (0, 3, 4, 10, 13, 14):
-        assert call(**{f"a{i}": None}) == -1, i
-    assert call(a15=FAKE) == -1  # adapters and values for a backward
     assert _lib.load().kmoe_dense_saved_bytes(17, 24) == 2 * 2 * 1536 and _lib.load().kmoe_dense_saved_bytes(0, 24) == 0
-    assert call(a6=9) == -6 and call(a2=63) == -2 and call(a14=ODD) == -2 and call(a9=7) == -2
-    call = _call("kmoe_dense_linear", [FAKE, 100, 64, FAKE, 72, FAKE, 2, 8, FAKE, FAKE, FAKE, None])
-    assert call(a1=0) == 0
-    for i in (0, 3, 8, 9, 10):
+    assert call(a6=9) == -6 and call(a2=63) == -2 and call(a7=ODD) == -2 and call(a9=ODD) == -2 and call(a8=1) == -2
+    call = _call("kmoe_dense_linear", [FAKE, 0, 100, 64, FAKE, 72, FAKE, None])
+    assert call(a2=0) == 0
+    for i in (0, 4, 6):
         assert call(**{f"a{i}": None}) == -1, i
-    assert call(a2=0) == -2 and call(a4=71) == -2 and call(a10=ODD) == -2
-    assert call(a2=1 << 22) == -2  # a tile's offsets are 32 bits
-    call = _call("kmoe_dense_dh", [FAKE, 100, 64, FAKE, 72, FAKE, FAKE, FAKE, None])
+    assert call(a3=0) == -2 and call(a5=71) == -2 and call(a6=ODD) == -2
+    assert call(a3=1 << 22) == -2  # a tile's offsets are 32 bits
+    assert call(a1=1, a2=_lib.LOST_ROWS + 1) == -2
+    call = _call("kmoe_dense_dh", [FAKE, 100, 64, FAKE, 72, FAKE, FAKE, FAKE, 0, None])
     assert call(a1=0) == 0
     for i in (0, 3, 5, 6, 7):
         assert call(**{f"a{i}": None}) == -1, i
-    call = _call("kmoe_dense_dx", [FAKE, None, 100, 72, FAKE, None, 64, FAKE, 2, 8, FAKE, FAKE, FAKE, None])
-    assert call(a2=0) == 0
-    for i in (0, 4, 10, 11, 12):
+    assert call(a8=1) == -2
+    call = _call("kmoe_dense_dx", [FAKE, None, 0, 100, 72, FAKE, None, 64, FAKE, None])
+    assert call(a3=0) == 0
+    for i in (0, 5, 8):
         assert call(**{f"a{i}": None}) == -1, i
-    assert call(a1=FAKE) == -1 and call(a1=FAKE, a5=FAKE) == -1  # two products and adapters
-    call = _call("kmoe_dense_wgrad", [FAKE, FAKE, 101, 72, 64, FAKE, 0, None])
-    for i in (0, 1, 5):
+    assert call(a1=FAKE) == -1 and call(a2=1) == -2
+    call = _call("kmoe_dense_wgrad", [FAKE, FAKE, None, None, 101, 72, 64, FAKE, 0, None])
+    for i in (0, 1, 7):
         assert call(**{f"a{i}": None}) == -1, i
-    assert call(a2=-1) == -2 and call(a3=4) == -2 and call(a4=0) == -2 and call(a6=2) == -3 and call(a5=ODD) == -2
-    n = _lib.load().kmoe_adapter_grad_workspace_bytes(4096, 1, 8, 64)
-    assert n > 0
-    call = _call("kmoe_adapter_grad", [FAKE, FAKE, 4096, FAKE, 1, 8, 64, 0, FAKE, FAKE, n, None])
-    for i in (0, 1, 3, 8):
-        assert call(**{f"a{i}": None}) == -1, i
-    assert call(a10=n - 1) == -4 and call(a4=65536) == -2 and call(a5=136) == -2 and call(a6=4) == -2 and call(a2=-1) == -2
+    assert call(a2=FAKE) == -1 and call(a2=FAKE, a3=ODD) == -2
+    assert call(a4=-1) == -2 and call(a5=4) == -2 and call(a6=0) == -2 and call(a8=2) == -3 and call(a7=ODD) == -2
