@@ -30,6 +30,9 @@ class V:
     def bf16(self):
         return V(self.v, self.e + H * (self.v.abs() + self.e) + 1e-40)
 
+    def twice(self):  # as two bf16, the second what the first lost
+        return V(self.v, self.e + H * H * (self.v.abs() + self.e) + 1e-40)
+
 
 def mm(a, b):
     """A matrix product with f32 sums of K terms: products of bf16 numbers are exact, each sum
@@ -61,7 +64,7 @@ def act(name, g):
     return V(a, 1.13 * g.e + off * a.abs() + 2.0 ** -21 * x.abs()), V(d, 0.8 * g.e + off * (1 + d.abs()))
 
 
-def adapted(x, w, ad, ids):
+def adapted(x, w, ad, ids, to=V.bf16):
     """x w^T + scale (x a^T) b^T of each row's adapter, before its last rounding."""
     y = mm(x, w.t())
     if ad is None:
@@ -72,7 +75,7 @@ def adapted(x, w, ad, ids):
         t = (ids == i).nonzero().squeeze(1)
         if t.numel():
             s = 1.0 if scale is None else float(scale[i])
-            inner = (mm(V(x.v[t], x.e[t]), V(a[i]).t()) * s).bf16()
+            inner = to(mm(V(x.v[t], x.e[t]), V(a[i]).t()) * s)
             d = mm(inner, V(b[i]).t())
             v[t] += d.v
             e[t] += d.e + U * v[t].abs()
@@ -84,22 +87,23 @@ def cut24(a):
     return V(a.v, a.e + 2.0 ** -15 * (a.v.abs() + a.e) + 1e-40)
 
 
-def ffn(x, wg, wu, wd, name, ads=(None, None, None), ids=None):
-    """(y, and for the backward h, p, q) of the gated block."""
+def ffn(x, wg, wu, wd, name, ads=(None, None, None), ids=None, to=V.bf16):
+    """(y before its last rounding, and for the backward h, p, q) of the gated block; to: how h and the
+    adapters' inner products are held."""
     x, wg, wu, wd = V(x), V(wg), V(wu), V(wd)
-    g, u = adapted(x, wg, ads[0], ids), adapted(x, wu, ads[1], ids)
+    g, u = adapted(x, wg, ads[0], ids, to), adapted(x, wu, ads[1], ids, to)
     a, d = act(name, g)
-    h = (a * u).bf16()
-    return adapted(h, wd, ads[2], ids).bf16(), h, cut24(d * u), cut24(a)
+    h = to(a * u)
+    return adapted(h, wd, ads[2], ids, to), h, cut24(d * u), cut24(a)
 
 
-def ffn_grads(x, wg, wu, wd, dy, h, p, q):
-    """Bounded gradients of x, wg, wu, wd."""
+def ffn_grads(x, wg, wu, wd, dy, h, p, q, to=V.bf16):
+    """Bounded gradients of x, wg, wu, wd before their last rounding; to: how dgate and dup are held."""
     dh = mm(V(dy), V(wd))
-    dg, du = (dh * p).bf16(), (dh * q).bf16()
+    dg, du = to(dh * p), to(dh * q)
     # (one sum over both parts)
     cat = lambda a, b, k: V(torch.cat((a.v, b.v), k), torch.cat((a.e, b.e), k))
-    dx = mm(cat(dg, du, 1), cat(V(wg), V(wu), 0)).bf16()
+    dx = mm(cat(dg, du, 1), cat(V(wg), V(wu), 0))
     return dx, mm(dg.t(), V(x)), mm(du.t(), V(x)), mm(V(dy).t(), h)
 
 

@@ -32,9 +32,11 @@ def make_ad(dev, n, r, K, N, scale=True):
                          torch.linspace(0.5, 2.0, n).to(dev) if scale else None)
 
 
-# rows from one to many (few-row kernels up to 64, the three tiles beyond), widths of odd eighths
+# rows from one to many (the kernel of few rows up to 16, runs of K, the tiles), widths of odd eighths
 SIZES = [(1, 64, 72), (2, 8, 8), (5, 136, 128), (16, 200, 24), (17, 72, 264), (33, 256, 136), (64, 520, 200), (65, 64, 72),
          (127, 200, 136), (130, 136, 392), (300, 520, 264), (777, 64, 1032), (2042, 72, 1544), (16379, 136, 1096)]
+# sizes that take each of the large tiles in each kind of product
+LARGE = [(10001, 1032, 2056), (8195, 1032, 1096), (1030, 2056, 5640)]
 
 
 @pytest.mark.parametrize("T,d,F", SIZES)
@@ -46,7 +48,7 @@ def test_ffn(dev, T, d, F):
         B.check(act, y, B.ffn(x, wg, wu, wd, act)[0])
 
 
-@pytest.mark.parametrize("T,d,F", SIZES)
+@pytest.mark.parametrize("T,d,F", SIZES + LARGE)
 def test_ffn_backward(dev, T, d, F):
     x, wg, wu, wd = make_ffn(dev, T, d, F)
     dy = rnd(dev, T, d)
@@ -58,6 +60,35 @@ def test_ffn_backward(dev, T, d, F):
         B.check(act, y.detach(), want)
         for name, g, w in zip(("dx", "dwg", "dwu", "dwd"), grads, B.ffn_grads(x, wg, wu, wd, dy, h, p, q)):
             B.check((act, name), g, w)
+
+
+@pytest.mark.parametrize("T,d,F", [(1, 64, 72), (8, 136, 200), (9, 200, 136), (17, 72, 1096), (32, 1032, 264)])
+def test_few_rows_are_rounded_once(dev, T, d, F):
+    """Of up to 32 rows h, dgate, dup and the adapters' inner products are two bf16 each."""
+    x, wg, wu, wd = make_ffn(dev, T, d, F)
+    dy, ids = rnd(dev, T, d), make_ids(dev, T, 3, "mixed")
+    ads = [make_ad(dev, 3, r, *kn) for kn, r in (((d, F), 16), ((d, F), 16), ((F, d), 8))]
+    with torch.no_grad():
+        B.check("y", kmoe.gated_ffn(x, wg, wu, wd), B.ffn(x, wg, wu, wd, "silu", to=B.V.twice)[0])
+        B.check("adapters", kmoe.gated_ffn(x, wg, wu, wd, "silu", kmoe.FFNAdapters(*ads), ids),
+                B.ffn(x, wg, wu, wd, "silu", ads, ids, B.V.twice)[0])
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = kmoe.gated_ffn(*leaves)
+    want, h, p, q = B.ffn(x, wg, wu, wd, "silu", to=B.V.twice)
+    B.check("train", y.detach(), want)
+    for name, g, w in zip(("dx", "dwg", "dwu", "dwd"), torch.autograd.grad(y, leaves, dy),
+                          B.ffn_grads(x, wg, wu, wd, dy, h, p, q, B.V.twice)):
+        B.check(name, g, w)
+
+
+def test_overflowing_rows(dev):
+    """Values that bf16 holds no more become infinite, as of one rounding, and reach their own rows only."""
+    x, wg, wu, wd = make_ffn(dev, 8, 64, 72)
+    x[3] *= 1e20
+    good = torch.arange(8, device=dev) != 3
+    with torch.no_grad():
+        y, z = kmoe.gated_ffn(x, wg, wu, wd), kmoe.gated_ffn(x[good], wg, wu, wd)
+    assert torch.equal(y[good], z) and not bool(torch.isfinite(y[3]).any())
 
 
 def test_ffn_gradient_is_the_difference(dev):
@@ -252,6 +283,34 @@ def test_adapters_stay_apart(dev, T):
         assert torch.equal(got[k][others], good[k][others])
 
 
+@pytest.mark.parametrize("r", [8, 16, 40])
+@pytest.mark.parametrize("T", [5, 20, 60, 300, 2042])
+def test_block_adapters_stay_apart(dev, T, r):
+    """The same of the block's three adapters, for each number of them that share a matrix instruction."""
+    d, F, n = 72, 264, 4
+    x, wg, wu, wd = make_ffn(dev, T, d, F)
+    ids = make_ids(dev, T, n, "mixed")
+    ads = [make_ad(dev, n, k, *kn) for kn, k in (((d, F), r), ((d, F), r), ((F, d), 8))]
+    bad = [a._replace(a=a.a.clone(), b=a.b.clone()) for a in ads]
+    bad[0].b[2, 5], bad[1].b[2, 7, 0], bad[2].b[1, 3] = float("inf"), float("nan"), float("-inf")
+    with torch.no_grad():
+        y, z = (kmoe.gated_ffn(x, wg, wu, wd, "silu", kmoe.FFNAdapters(*a), ids) for a in (ads, bad))
+    rows = (ids != 2) & (ids != 1)
+    assert torch.equal(y[rows], z[rows])
+    assert not bool(torch.isfinite(z[ids == 2]).any()) and not bool(torch.isfinite(z[ids == 1][:, 3]).any())
+    assert torch.equal(y[ids == 1][:, 4:], z[ids == 1][:, 4:])
+
+
+@pytest.mark.parametrize("T,K,N", [(8195, 1032, 1096), (2042, 1032, 5640), (48, 2056, 520), (1030, 2056, 2056)])
+def test_linear_large(dev, T, K, N):
+    """The large tiles with adapters, and runs of K."""
+    x, w, ad = rnd(dev, T, K), rnd(dev, N, K, std=K ** -0.5), make_ad(dev, 5, 24, K, N)
+    ids = make_ids(dev, T, 5, "runs")
+    with torch.no_grad():
+        B.check("y", kmoe.adapted_linear(x, w, ad, ids), B.adapted(B.V(x), B.V(w), ad, ids))
+        B.check("without", kmoe.adapted_linear(x, w), B.mm(B.V(x), B.V(w).t()))
+
+
 def test_rank_is_filled_up(dev):
     """A rank that is not a multiple of 8, with its gradients."""
     T, K, N, n, r = 70, 72, 136, 3, 5
@@ -309,6 +368,39 @@ def test_captured_block(dev):
         other = [t.detach().clone().requires_grad_(True) for t in leaves]
         want = torch.autograd.grad(kmoe.gated_ffn(*other), other, dy)
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+def test_captured_projection(dev):
+    """Replays of a projection in runs of K with adapters, and of its backward; two graphs in turn."""
+    x, w, ad = rnd(dev, 48, 1032), rnd(dev, 264, 1032, std=0.03), make_ad(dev, 3, 16, 1032, 264)
+    ids, dy = make_ids(dev, 48, 3, "mixed").to(torch.int32), rnd(dev, 48, 264)
+    with torch.no_grad():
+        kmoe.adapted_linear(x, w, ad, ids)
+        graphs, outs = [torch.cuda.CUDAGraph() for _ in range(2)], []
+        for k, graph in enumerate(graphs):
+            with torch.cuda.graph(graph):
+                outs.append(kmoe.adapted_linear(x[: 48 - 16 * k], w, ad, ids[: 48 - 16 * k]))
+        for _ in range(3):
+            x.copy_(rnd(dev, 48, 1032))
+            ids.copy_(ids.roll(1))
+            for graph in graphs:
+                graph.replay()
+            eager = kmoe.adapted_linear(x, w, ad, ids), kmoe.adapted_linear(x[:32], w, ad, ids[:32])
+            torch.cuda.synchronize()
+            assert torch.equal(outs[0], eager[0]) and torch.equal(outs[1], eager[1])
+    leaves = [t.clone().requires_grad_(True) for t in (x, ad.a, ad.b)]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = kmoe.adapted_linear(leaves[0], w, kmoe.Adapters(leaves[1], leaves[2], ad.scale), ids)
+        got = torch.autograd.grad(y, leaves, dy)
+    for _ in range(3):
+        with torch.no_grad():
+            leaves[0].copy_(rnd(dev, 48, 1032))
+        graph.replay()
+        torch.cuda.synchronize()
+        other = [t.detach().clone().requires_grad_(True) for t in leaves]
+        z = kmoe.adapted_linear(other[0], w, kmoe.Adapters(other[1], other[2], ad.scale), ids)
+        assert torch.equal(y, z) and all(torch.equal(a, b) for a, b in zip(got, torch.autograd.grad(z, other, dy)))
 
 
 def test_capture_beside_a_live_graph_is_refused(dev):
