@@ -311,6 +311,22 @@ def test_linear_large(dev, T, K, N):
         B.check("without", kmoe.adapted_linear(x, w), B.mm(B.V(x), B.V(w).t()))
 
 
+@pytest.mark.parametrize("r", [8, 16, 32])
+def test_results_repeat(dev, r):
+    """Which adapters share a matrix instruction is not told by the input; the results are, bit for bit."""
+    T, K, N, n = 2042, 136, 2056, 200
+    x, w, ad, dy = rnd(dev, T, K), rnd(dev, N, K, std=0.1), make_ad(dev, n, r, K, N), rnd(dev, T, N)
+    ids = make_ids(dev, T, n, "mixed")
+
+    def run():
+        leaves = [t.clone().requires_grad_(True) for t in (x, ad.a, ad.b)]
+        y = kmoe.adapted_linear(leaves[0], w, kmoe.Adapters(leaves[1], leaves[2], ad.scale), ids)
+        return (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    first = run()
+    for _ in range(4):
+        assert all(torch.equal(a, b) for a, b in zip(first, run()))
+
+
 def test_rank_is_filled_up(dev):
     """A rank that is not a multiple of 8, with its gradients."""
     T, K, N, n, r = 70, 72, 136, 3, 5
