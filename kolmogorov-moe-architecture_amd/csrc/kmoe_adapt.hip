@@ -14,11 +14,11 @@ namespace {
 // product's MFMAs, one rounding (half a step of 2^-8) of a term that adds to the projection's.  What
 // it loses is kept behind, for the factors' gradients, of which it is the whole operand.
 // A workgroup takes 16 rows, RB blocks of 16 ranks and every gridDim.y-th of the adapters that the rows
-// have (few rows with an adapter each: a workgroup an adapter); its W waves share K.  Each
-// adapter's product is computed for all 16 rows and kept for those that have it: bound by reading
-// x and the adapters, not by the products, and no row's values meet another's adapter.  Few
-// rows take a workgroup a block of ranks: latency counts and x is small.  K 2048, rank 16: one row 5 us,
-// 48 rows with an adapter each 8; 4099 rows of prompts, rank 32, 14.5 (x alone 3.5 at HBM's rate).
+// have (few rows with an adapter each: a workgroup an adapter); its W waves share K.  Rows that have
+// another adapter than the one in turn read as zeros, for nothing (512 rows with 16 adapters in
+// turn, rank 16: 13.8 us; read and not kept 20).  Bound by reading x and the adapters and by latency, not
+// by the products; few rows take a workgroup a block of ranks.  K 2048, rank 16: one row 5 us, 48
+// rows with an adapter each 7; 4099 rows of prompts, rank 32, 14.5 (x alone 3.5 at HBM's rate).
 struct Shrink {
   const uint16_t* x;
   int64_t T;
@@ -49,7 +49,6 @@ __global__ __launch_bounds__(W * 64) void shrink_kernel(Shrink g) {
   uint64_t todo = __ballot(first);
   Stream16<RB, W, D> st;
   st.x = g.x + t0 * g.K, st.K = g.K;
-  st.xoff = t0 + l16 < g.T ? (uint32_t)(l16 * g.K) * 2 : NOWHERE;
 #pragma unroll
   for (int b = 0; b < RB; ++b) {
     const int j = j0 + b * 16 + l16;
@@ -58,6 +57,7 @@ __global__ __launch_bounds__(W * 64) void shrink_kernel(Shrink g) {
   for (int c = 0; todo; ++c, todo &= todo - 1) {
     if (c % (int)gridDim.y != (int)blockIdx.y) continue;
     const int cur = __builtin_amdgcn_readlane(id, __builtin_ctzll(todo));
+    st.xoff = id == cur ? (uint32_t)(l16 * g.K) * 2 : NOWHERE;
     f32x4_t acc[RB];
 #pragma unroll
     for (int b = 0; b < RB; ++b) {
