@@ -290,13 +290,21 @@ __global__ __launch_bounds__(256) void turn_kernel(Turn g) {
   }
 }
 
-// Runs of rows: as many as give every compute unit two workgroups, of at least 256 rows.
-int64_t runs_of(int64_t T, int n, int C, int C2) {
+// The runs of rows in which a launch computes the gradients of factors of C and C2 columns (C2 = 0: of
+// one factor), and the bytes of their partial sums: as many runs as give every compute unit two
+// workgroups, of at least 256 rows.  One factor alone has fewer blocks, so it may take more runs than both.
+struct Runs {
+  int64_t n;
+  size_t bytes;
+};
+Runs runs_of(int64_t T, int n, int rank, int C, int C2) {
+  if (T <= 0) return {1, 0};
   const int64_t blocks = (int64_t)n * (kmoe::ceil_div(C, GC) + kmoe::ceil_div(C2, GC));
   int64_t runs = kmoe::ceil_div<int64_t>(512, blocks);
   runs = runs < kmoe::ceil_div<int64_t>(T, 256) ? runs : kmoe::ceil_div<int64_t>(T, 256);
   const int64_t least = kmoe::ceil_div<int64_t>(T, GMAXRUN);
-  return runs > least ? runs : (least > 1 ? least : 1);
+  runs = runs > least ? runs : (least > 1 ? least : 1);
+  return {runs, runs > 1 ? (size_t)runs * n * rank * ((size_t)C + C2) * sizeof(float) : 0};
 }
 
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
@@ -337,14 +345,18 @@ namespace {
 
 size_t piece(int64_t bytes) { return (size_t)((bytes + 255) / 256 * 256); }
 
-size_t grads_bytes(int64_t T, int n, int rank, int C, int C2) {
-  const int64_t runs = T > 0 ? runs_of(T, n, C, C2) : 1;
-  return runs > 1 ? (size_t)runs * n * rank * ((size_t)C + C2) * sizeof(float) : 0;
+// Of both factors or of either one alone, whichever takes most.
+size_t grads_bytes(int64_t T, int n, int rank, int K, int N) {
+  const size_t both = runs_of(T, n, rank, K, N).bytes, inner = runs_of(T, n, rank, K, 0).bytes,
+               outer = runs_of(T, n, rank, N, 0).bytes, one = inner > outer ? inner : outer;
+  return both > one ? both : one;
 }
 
 // The gradients of up to two factors (C2 = 0: one) of adapters with rows ids.
-int factor_grads(FactorGrad g, int C, int C2, void* workspace, hipStream_t s) {
-  const int64_t runs = g.T > 0 ? runs_of(g.T, g.n, C, C2) : 1;
+int factor_grads(FactorGrad g, int C, int C2, void* workspace, size_t workspace_bytes, hipStream_t s) {
+  const auto [runs, bytes] = runs_of(g.T, g.n, g.r, C, C2);
+  KMOE_REQUIRE(bytes <= workspace_bytes, KMOE_ERR_WORKSPACE,
+               "kmoe_adapted_linear_backward: %zu bytes are left for partial sums, %zu are needed", workspace_bytes, bytes);
   KMOE_REQUIRE(runs <= 65535, KMOE_ERR_SHAPE, "kmoe_adapted_linear_backward: %lld rows", (long long)g.T);
   // (a run is whole groups: a wave looks at two of them at a time)
   g.run = kmoe::ceil_div<int64_t>(kmoe::ceil_div<int64_t>(g.T, runs), 64) * 64;
@@ -424,5 +436,6 @@ extern "C" int kmoe_adapted_linear_backward(const void* dy, const void* x, int64
   FactorJob outer{static_cast<const uint16_t*>(v), static_cast<const uint16_t*>(dy), static_cast<uint16_t*>(db), 0, 0, 0, 1};
   g.ids = ids, g.T = T, g.n = n_adapters, g.r = r;
   g.job[0] = da ? inner : outer, g.job[1] = outer;
-  return factor_grads(g, da ? K : N, da && db ? N : 0, part, s);
+  return factor_grads(g, da ? K : N, da && db ? N : 0, part,
+                      workspace_bytes - (static_cast<uint8_t*>(part) - static_cast<uint8_t*>(workspace)), s);
 }

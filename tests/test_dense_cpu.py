@@ -175,3 +175,28 @@ def test_abi_parts():
         assert call(**{f"a{i}": None}) == -1, i
     assert call(a2=FAKE) == -1 and call(a2=FAKE, a3=ODD) == -2
     assert call(a4=-1) == -2 and call(a5=4) == -2 and call(a6=0) == -2 and call(a8=2) == -3 and call(a7=ODD) == -2
+
+
+def _partial_bytes(T, n, r, C, C2):
+    """Bytes of the partial sums of a launch over the gradients of factors of C and C2 columns (0: none):
+    columns in blocks of 128 an adapter, runs of rows up to 512 workgroups, of 256 to 65536 rows."""
+    up = lambda a, b: -(-a // b)
+    runs = min(up(512, n * (up(C, 128) + up(C2, 128))), up(T, 256))
+    runs = max(runs, up(T, 65536), 1)
+    return runs * n * r * (C + C2) * 4 if runs > 1 else 0
+
+
+def test_adapter_gradients_fit_their_workspace():
+    """With the gradients of both factors, or of either one alone, which may take more runs of rows."""
+    import random
+    lib, rng = _lib.load(), random.Random(3)
+    piece = lambda b: -(-b // 256) * 256
+    cases = [(257, 2048, 2048, 16, 16), (513, 2048, 5632, 5, 16), (2042, 2048, 2048, 16, 16), (4099, 2048, 5632, 16, 32),
+             (1, 8, 8, 1, 8), (70000, 64, 72, 2, 8)]
+    cases += [(rng.randint(1, 1 << rng.randint(1, 18)), 8 * rng.randint(1, 704), 8 * rng.randint(1, 704), rng.randint(1, 40),
+               8 * rng.randint(1, 16)) for _ in range(5000)]
+    for T, K, N, n, r in cases:
+        have = lib.kmoe_adapted_linear_backward_workspace_bytes(T, K, N, n, r)
+        have -= piece(4 * T * r) + piece(2 * n * r * K) + piece(2 * n * r * N)
+        for C, C2 in ((K, N), (K, 0), (N, 0)):
+            assert _partial_bytes(T, n, r, C, C2) <= have, (T, K, N, n, r, C, C2)

@@ -1,5 +1,6 @@
 """The gated block and adapted projections on the GPU against their formulas in 64 bits, within
 bounds that carry every rounding (dense_bounds.py)."""
+import ctypes
 import os
 import sys
 
@@ -7,6 +8,7 @@ import pytest
 import torch
 
 import kmoe
+from kmoe import _lib
 
 sys.path.insert(0, os.path.dirname(os.path.abspath(__file__)))
 import dense_bounds as B  # noqa: E402
@@ -236,6 +238,61 @@ def test_linear_backward(dev, T, K, N, n, r, how):
         v = (B.mm(B.V(x[t]), B.V(ad.a[i]).t()) * s).bf16()
         B.check(("da", i), da[i], B.mm(u.t(), B.V(x[t])))
         B.check(("db", i), db[i], B.mm(B.V(dy[t]).t(), v))
+
+
+FACTORS = [(300, 72, 136, 3, 16), (257, 1032, 1032, 16, 8), (513, 264, 1544, 5, 16), (2042, 2048, 2048, 16, 16), (4099, 136, 264, 2, 40)]
+
+
+@pytest.mark.parametrize("need", [(0, 0, 1, 0), (0, 0, 0, 1), (1, 0, 0, 0), (0, 1, 0, 0), (1, 0, 0, 1), (0, 1, 1, 0), (1, 1, 1, 1)])
+@pytest.mark.parametrize("T,K,N,n,r", FACTORS)
+def test_linear_some_gradients(dev, T, K, N, n, r, need):
+    """Frozen factors, weights and inputs, at sizes where one factor's gradient takes more runs of rows
+    than both."""
+    x, w, ad = rnd(dev, T, K), rnd(dev, N, K, std=K ** -0.5), make_ad(dev, n, r, K, N)
+    ids, dy = make_ids(dev, T, n, "mixed"), rnd(dev, T, N)
+    lx, lw, la, lb = (t.clone().requires_grad_(bool(k)) for t, k in zip((x, w, ad.a, ad.b), need))
+    kmoe.adapted_linear(lx, lw, kmoe.Adapters(la, lb, ad.scale), ids).backward(dy)
+    for t, k in zip((lx, lw, la, lb), need):
+        assert (t.grad is not None) == bool(k)
+    if need[0]:
+        back = kmoe.Adapters(ad.b.transpose(1, 2), ad.a.transpose(1, 2), ad.scale)
+        B.check("dx", lx.grad, B.adapted(B.V(dy), B.V(w.t()), back, ids))
+    if need[1]:
+        B.check("dw", lw.grad, B.mm(B.V(dy).t(), B.V(x)))
+    for i in range(n):
+        t, s = (ids == i).nonzero().squeeze(1), float(ad.scale[i])
+        if need[2]:
+            B.check(("da", i), la.grad[i], B.mm((B.mm(B.V(dy[t]), B.V(ad.b[i])) * s).bf16().t(), B.V(x[t])))
+        if need[3]:
+            B.check(("db", i), lb.grad[i], B.mm(B.V(dy[t]).t(), (B.mm(B.V(x[t]), B.V(ad.a[i]).t()) * s).bf16()))
+
+
+@pytest.mark.parametrize("which", ["da", "db", "both"])
+@pytest.mark.parametrize("T,K,N,n,r", FACTORS)
+def test_adapter_gradients_stay_in_their_workspace(dev, T, K, N, n, r, which):
+    """The C entry with exactly the workspace that it asks for, and bytes of a pattern behind it."""
+    x, w, ad, dy = rnd(dev, T, K), rnd(dev, N, K, std=K ** -0.5), make_ad(dev, n, r, K, N), rnd(dev, T, N)
+    ids = make_ids(dev, T, n, "mixed").to(torch.int32)
+    ws1 = _lib.load().kmoe_adapted_linear_workspace_bytes(T, K, N, r)
+    fwd, y = torch.empty(ws1, device=dev, dtype=torch.uint8), torch.empty_like(dy)
+    need = _lib.load().kmoe_adapted_linear_backward_workspace_bytes(T, K, N, n, r)
+    buf = torch.full((need + (16 << 20),), 0xA5, device=dev, dtype=torch.uint8)
+    da = torch.empty_like(ad.a) if which != "db" else None
+    db = torch.empty_like(ad.b) if which != "da" else None
+    a = _lib.Adapter(ad.a.data_ptr(), ad.b.data_ptr(), ad.scale.data_ptr(), r)
+    s = _lib.stream_ptr(dev)
+    _lib.call("kmoe_adapted_linear", x.data_ptr(), T, K, w.data_ptr(), N, ids.data_ptr(), n, ctypes.byref(a), y.data_ptr(),
+              fwd.data_ptr(), ws1, s)
+    _lib.call("kmoe_adapted_linear_backward", dy.data_ptr(), x.data_ptr(), T, K, w.data_ptr(), N, ids.data_ptr(), n,
+              ctypes.byref(a), fwd.data_ptr(), None, _lib.ptr(da), _lib.ptr(db), buf.data_ptr(), need, s)
+    torch.cuda.synchronize()
+    assert bool((buf[need:] == 0xA5).all())
+    for i in (0, n - 1):
+        t, f = (ids == i).nonzero().squeeze(1), float(ad.scale[i])
+        if da is not None:
+            B.check("da", da[i], B.mm((B.mm(B.V(dy[t]), B.V(ad.b[i])) * f).bf16().t(), B.V(x[t])))
+        if db is not None:
+            B.check("db", db[i], B.mm(B.V(dy[t]).t(), (B.mm(B.V(x[t]), B.V(ad.a[i]).t()) * f).bf16()))
 
 
 @pytest.mark.parametrize("T", [3, 50, 300])
