@@ -8,6 +8,7 @@ outside of torch's operations and counts the change, so what the modules keep fr
 from __future__ import annotations
 
 import ctypes
+import operator
 from typing import Optional
 
 import torch
@@ -45,15 +46,23 @@ class _Plan:
         self.bits = 8 if "exp_avg_scale" in states[0] else 32
         self.dtype = _lib.DTYPE_F32 if params[0].dtype == torch.float32 else _lib.DTYPE_BF16
         self.device = dev
-        self.at = [r[:-1] for r in rows]
+        self.at = [(p.data_ptr(), p.numel(), p.dtype) for p in params]
+        self.held = [[(k, t, t.data_ptr()) for k, t in st.items()] for st in states]
 
     @staticmethod
     def _where(p, st):
         return [p.data_ptr(), *(st[k].data_ptr() if k in st else 0 for k in _FIELDS)]
 
-    def current(self) -> bool:
-        """Whether every tensor is where it was."""
-        return all(self._where(p, st) == a for p, st, a in zip(self.params, self.states, self.at))
+    def current(self, state) -> bool:
+        """Whether the tensors are those of the optimizer's `state`, each of them where it was and the
+        parameters what they were."""
+        for p, st, at, held in zip(self.params, self.states, self.at, self.held):
+            if state.get(p) is not st or len(st) != len(held) or (p.data_ptr(), p.numel(), p.dtype) != at or not p.is_contiguous():
+                return False
+            for k, t, a in held:
+                if st.get(k) is not t or t.data_ptr() != a:
+                    return False
+        return True
 
 
 class AdamW(torch.optim.Optimizer):
@@ -76,7 +85,7 @@ class AdamW(torch.optim.Optimizer):
         if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
             raise ValueError(f"kmoe.AdamW: lr={lr}")
         self._check(dict(betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
-        self._plans, self._held, self._seen = None, [], {}
+        self._plans, self._stepped, self._held, self._seen = None, [], [], {}
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=bool(master_weights)))
 
@@ -104,14 +113,14 @@ class AdamW(torch.optim.Optimizer):
         if not p.is_contiguous():
             raise ValueError(f"kmoe.AdamW: parameters are contiguous, got strides {p.stride()} of {tuple(p.shape)}")
 
-    # _plans: the tables of the last step; _held: those that captured steps read; _seen: version of
-    # each parameter with an f32 copy after its last step
+    # _plans: the tables of the last step, _stepped: each group's parameters in them; _held: tables that
+    # captured steps read; _seen: version of each parameter with an f32 copy after its last step
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._plans, self._held, self._seen = None, [], {}
+        self._plans, self._stepped, self._held, self._seen = None, [], [], {}
 
     def __getstate__(self):
-        return {k: v for k, v in super().__getstate__().items() if k not in ("_plans", "_held", "_seen")}
+        return {k: v for k, v in super().__getstate__().items() if k not in ("_plans", "_stepped", "_held", "_seen")}
 
     # ---------------------------------------------------------------- states
     def _new_state(self, p, group):
@@ -189,14 +198,17 @@ class AdamW(torch.optim.Optimizer):
         self._plans = None
 
     # ---------------------------------------------------------------- the step
-    def _plan(self):
-        """[(group, plan)] of the parameters that have had a gradient."""
-        plans = []
+    def _to_step(self, group):
+        """The group's parameters that have had a gradient."""
+        return [p for p in group["params"] if p.grad is not None or p in self.state]
+
+    def _plan(self) -> None:
+        """The tables of the parameters that have had a gradient."""
+        plans, stepped = [], []
         for group in self.param_groups:
             kinds = {}
-            for p in group["params"]:
-                if p.grad is None and p not in self.state:
-                    continue
+            stepped.append((group, self._to_step(group)))
+            for p in stepped[-1][1]:
                 if not p.is_cuda:
                     raise ValueError("kmoe.AdamW: parameters must be on a GPU (the HIP kernel is the only implementation)")
                 self._check_param(p)
@@ -209,13 +221,16 @@ class AdamW(torch.optim.Optimizer):
                 # (a state of another form than the group's has been refused)
             for (_, _, master), ps in kinds.items():
                 plans.append((group, _Plan(ps, [self.state[p] for p in ps], master)))
-        return plans
+        self._plans, self._stepped = plans, stepped
 
     def _stale(self) -> bool:
-        if self._plans is None or not all(plan.current() for _, plan in self._plans):
+        if self._plans is None or len(self._stepped) != len(self.param_groups):
             return True
-        known = sum(len(plan.params) for _, plan in self._plans)
-        return sum(p.grad is not None or p in self.state for g in self.param_groups for p in g["params"]) != known
+        for group, (known, ps) in zip(self.param_groups, self._stepped):
+            now = self._to_step(group)
+            if group is not known or len(now) != len(ps) or not all(map(operator.is_, now, ps)):
+                return True
+        return not all(plan.current(self.state) for _, plan in self._plans)
 
     @torch.no_grad()
     def step(self, closure=None) -> Optional[torch.Tensor]:
@@ -228,7 +243,7 @@ class AdamW(torch.optim.Optimizer):
             if capturing:
                 raise RuntimeError("kmoe.AdamW: a capture needs the states and tables of an eager step before it: take one, "
                                    "and keep the parameters where they are")
-            self._plans = self._plan()
+            self._plan()
         for group, plan in self._plans:
             lr, (b1, b2) = group["lr"], group["betas"]
             lr_dev, kept, moved = None, [], []

@@ -110,3 +110,115 @@ def test_abi_refuses():
     assert call(a11=1.0) == -2 and call(a12=-0.5) == -2 and call(a13=-1.0) == -2 and call(a14=-1.0) == -2
     assert call(a3=(ctypes.c_int32 * 2)(2, 1)) == -2
     assert call(a5=(ctypes.c_void_p * 1)(None)) == 0  # nothing has a gradient: nothing runs
+
+
+# ---------------------------------------------------------------- what a step is given
+class OnGpu(torch.nn.Parameter):
+    """A parameter that says it is on a GPU, for the host's part of a step."""
+    is_cuda = True
+
+
+@pytest.fixture
+def steps(monkeypatch):
+    """The tensors that each native call of a step gets: [(address of p, of its first moment, values, of its
+    gradient), ...] of those with a gradient.  Nothing runs."""
+    import contextlib
+
+    from kmoe import optim
+    calls = []
+
+    def call(name, table, owner, base, base_host, n, grads, *rest):
+        rows = torch.frombuffer((ctypes.c_int64 * (8 * n)).from_address(table), dtype=torch.int64).view(n, 8).tolist()
+        calls.append([(r[0], r[1], r[7], g) for r, g in zip(rows, list(grads)[:n]) if g])
+    monkeypatch.setattr(optim._lib, "call", call)
+    monkeypatch.setattr(optim._lib, "stream_ptr", lambda d=None: 0)
+    monkeypatch.setattr(optim, "_device", lambda d: contextlib.nullcontext())
+    return calls
+
+
+def _on_gpu(*sizes, dtype=torch.float32):
+    ps = [OnGpu(torch.randn(n).to(dtype)) for n in sizes]
+    for p in ps:
+        p.grad = torch.ones_like(p.detach())
+    return ps
+
+
+def _want(opt, *ps):
+    return [(p.data_ptr(), opt.state[p]["exp_avg"].data_ptr(), p.numel(), p.grad.data_ptr()) for p in ps]
+
+
+def test_a_step_takes_the_present_states(steps):
+    """States that a program clears or replaces, whole or a tensor of them."""
+    a, b = _on_gpu(5, 300)
+    opt = kmoe.AdamW([a, b])
+    opt.step()
+    plans = opt._plans
+    opt.step()
+    assert opt._plans is plans and steps[0] == steps[1] == _want(opt, a, b)  # made once
+    old = opt.state[a]
+    opt.state.clear()
+    opt.step()
+    assert opt.state[a] is not old and steps[-1] == _want(opt, a, b) and set(opt.state_dict()["state"]) == {0, 1}
+    import collections
+    opt.state = collections.defaultdict(dict)
+    opt.step()
+    assert steps[-1] == _want(opt, a, b)
+    opt.state[b] = {k: v.clone() for k, v in opt.state[b].items()}
+    opt.step()
+    assert steps[-1] == _want(opt, a, b)
+    opt.state[b]["exp_avg"] = torch.ones(300)
+    opt.step()
+    assert steps[-1] == _want(opt, a, b)
+    opt.state[b]["exp_avg"] = torch.ones(299)
+    with pytest.raises(ValueError, match="the state exp_avg"):
+        opt.step()
+
+
+def test_a_step_takes_the_present_parameters(steps):
+    """Parameters that a program replaces in their group, or gives other memory."""
+    a, b, c = _on_gpu(5, 300, 300)
+    opt = kmoe.AdamW([a, b])
+    opt.step()
+    opt.param_groups[0]["params"][1] = c
+    opt.step()
+    assert steps[-1] == _want(opt, a, c)
+    opt.param_groups[0]["params"] = [c, a]
+    opt.step()
+    assert steps[-1] == _want(opt, c, a)
+    n = len(steps)
+    for shorter in (lambda t: t[:3], lambda t: t.view(15, 20).t()):
+        (q,) = _on_gpu(300)
+        opt = kmoe.AdamW([q])
+        opt.step()
+        q.grad = None
+        q.data = shorter(q.data)  # the same address
+        q.grad = torch.ones_like(q.detach())
+        with pytest.raises(ValueError, match="kmoe.AdamW"):
+            opt.step()
+    assert len(steps) == n + 2  # (the first step of each)
+
+
+def test_a_parameter_without_a_state_or_gradient_is_left(steps):
+    a, b = _on_gpu(5, 300)
+    opt = kmoe.AdamW([a, b])
+    opt.step()
+    del opt.state[b]
+    b.grad = None
+    opt.step()
+    assert steps[-1] == _want(opt, a) and b not in opt.state
+    b.grad = torch.ones(300)
+    opt.step()
+    assert steps[-1] == _want(opt, a, b)
+
+
+def test_a_refused_parameter_stays_refused(steps):
+    a, b = _on_gpu(5, 300)
+    b.grad = None
+    opt = kmoe.AdamW([a, b])
+    opt.step()
+    b.is_cuda = False
+    b.grad = torch.ones(300)
+    for _ in range(2):
+        with pytest.raises(ValueError, match="on a GPU"):
+            opt.step()
+    assert len(steps) == 1

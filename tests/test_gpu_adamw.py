@@ -311,3 +311,36 @@ def test_refusals(dev):
     q.grad = torch.zeros(4, device=dev, dtype=torch.bfloat16).to_sparse()
     with pytest.raises(ValueError, match="dense"):
         opt.step()
+
+
+def test_replaced_states_and_parameters(dev):
+    """A cleared state starts anew, a replaced parameter is stepped, a parameter of fewer values in the same
+    place is refused."""
+    ps, gs = _tensors(dev, [(300,), (1000,), (1000,)], torch.float32)
+    p, q, r = ps
+    for t, g in zip(ps, gs):
+        t.grad = g
+    start = [t.detach().clone() for t in ps]
+    opt = kmoe.AdamW([p, q], **HYPER)
+    opt.step()
+    first = [t.detach().clone() for t in ps]
+    opt.step()
+    opt.state.clear()
+    with torch.no_grad():
+        for t, s in zip(ps, start):
+            t.copy_(s)
+    opt.step()
+    assert torch.equal(p, first[0]) and torch.equal(q, first[1]) and int(opt.state[p]["step"]) == 1
+    opt.param_groups[0]["params"][1] = r
+    with torch.no_grad():
+        r.copy_(start[1])
+    r.grad = q.grad
+    opt.step()
+    assert torch.equal(r, first[1]) and torch.equal(q, first[1]) and int(opt.state[p]["step"]) == 2
+    guard = r.detach().clone()
+    r.grad = None
+    r.data = r.data[:400]
+    r.grad = gs[0].new_ones(400)
+    with pytest.raises(ValueError, match="the state"):
+        opt.step()
+    assert torch.equal(r.data.as_strided((1000,), (1,)), guard)
