@@ -72,8 +72,9 @@ class AdamW(torch.optim.Optimizer):
     scale per 256 values; the first moment in e4m3, the second as the square root in unsigned
     codes of 4 exponent and 4 mantissa bits, a positive one never as zero.  master_weights (bf16
     parameters): the step works on an f32 copy of the weights, kept in the state, and the
-    parameters are its rounding; without it, changes below half a bf16 step are lost.  The copy
-    is made anew when something else has written the parameter (as torch counts it).
+    parameters are its rounding; without it, changes below half a bf16 step are lost.  When
+    something else has written the parameter (as torch counts it), the copy is made anew where it
+    does not round to it; a copied or unpickled optimizer keeps its copies' bits.
 
     lr may be a one-element f32 tensor on the parameters' GPU, read when the step runs: a captured
     step follows it.  The step count is on the GPU too, one per parameter; a parameter without a
@@ -271,7 +272,9 @@ class AdamW(torch.optim.Optimizer):
                     if capturing:
                         raise RuntimeError("kmoe.AdamW: a parameter was written since the last step; take an eager step, which "
                                            "makes its f32 copy anew, before the capture")
-                    plan.states[i]["master"].copy_(p)
+                    # (anew where it does not round to the parameter: what was not written keeps its bits)
+                    master = plan.states[i]["master"]
+                    master.copy_(torch.where(master.to(p.dtype) == p, master, p.float()))
             if not moved:
                 continue
             if capturing and not any(h is plan for h in self._held):

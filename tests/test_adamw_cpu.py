@@ -222,3 +222,52 @@ def test_a_refused_parameter_stays_refused(steps):
         with pytest.raises(ValueError, match="on a GPU"):
             opt.step()
     assert len(steps) == 1
+
+
+@pytest.mark.parametrize("how", ["deepcopy", "pickle", "state_dict", "weights_after"])
+def test_master_weights_outlive_a_copy(steps, how):
+    """The f32 copies of a copied, unpickled or reloaded optimizer keep the bits that bf16 lacks; what was
+    written since is taken over."""
+    import copy
+    import io
+    (p,) = _on_gpu(5, dtype=torch.bfloat16)
+    opt = kmoe.AdamW([p], master_weights=True)
+    opt.step()
+    fine = torch.tensor([1.0010, -2.003, 0.5, 3.01, 0.0])
+    opt.state[p]["master"].copy_(fine)
+    with torch.no_grad():
+        p.copy_(fine)
+    opt._seen[p] = p._version  # as after a step
+    if how == "deepcopy":
+        opt = copy.deepcopy(opt)
+    elif how == "pickle":
+        buf = io.BytesIO()
+        torch.save(opt, buf)
+        buf.seek(0)
+        opt = torch.load(buf, weights_only=False)
+    else:
+        (q,) = _on_gpu(5, dtype=torch.bfloat16)
+        other = kmoe.AdamW([q], master_weights=True)
+        with torch.no_grad():
+            if how == "state_dict":
+                q.copy_(p)
+                other.load_state_dict(opt.state_dict())
+            else:  # the weights after the states
+                other.load_state_dict(opt.state_dict())
+                q.copy_(p)
+        opt = other
+    (q,) = opt.param_groups[0]["params"]
+    if not getattr(q, "is_cuda"):
+        q = OnGpu(q.detach())
+        st = opt.state.pop(opt.param_groups[0]["params"][0])
+        opt.param_groups[0]["params"][0] = q
+        opt.state[q] = st
+    q.grad = torch.ones_like(q.detach())
+    opt.step()
+    assert torch.equal(opt.state[q]["master"], fine)
+    with torch.no_grad():
+        q[3] = 7.0
+        q[4] = float("nan")
+    opt.step()
+    got = opt.state[q]["master"]
+    assert torch.equal(got[:3], fine[:3]) and float(got[3]) == 7.0 and bool(got[4].isnan())

@@ -344,3 +344,24 @@ def test_replaced_states_and_parameters(dev):
     with pytest.raises(ValueError, match="the state"):
         opt.step()
     assert torch.equal(r.data.as_strided((1000,), (1,)), guard)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_copied_optimizer_goes_on(dev, bits):
+    """Steps of a copy with f32 weights are the original's, bit for bit."""
+    ps, gs = _tensors(dev, [(300,), (40, 25)], torch.bfloat16)
+    opt = kmoe.AdamW(ps, state_bits=bits, master_weights=True, **HYPER)
+    for t in range(3):
+        for p, g in zip(ps, gs):
+            p.grad = g * (t + 1)
+        opt.step()
+    qs, other = copy.deepcopy((ps, opt))
+    assert all(a is b for a, b in zip(qs, other.param_groups[0]["params"]))
+    for t in range(3):
+        for p, q, g in zip(ps, qs, gs):
+            p.grad, q.grad = g * -t, g * -t
+        opt.step()
+        other.step()
+        for p, q in zip(ps, qs):
+            assert torch.equal(p, q) and torch.equal(opt.state[p]["master"], other.state[q]["master"])
+            assert not torch.equal(opt.state[p]["master"], p.detach().float())
