@@ -119,8 +119,8 @@ __device__ __forceinline__ void act_at(float g, float& a, float& da) {
     a = 0.5f * g * (1.0f + t);
     da = 0.5f * (1.0f + t) + 0.5f * g * (1.0f - t * t) * 0.79788456f * (1.0f + 0.134145f * g2);
   } else {
-    a = g > 0.0f ? g : 0.0f;
-    da = g > 0.0f ? 1.0f : 0.0f;
+    a = g <= 0.0f ? 0.0f : g;  // (a NaN stays one)
+    da = g <= 0.0f ? 0.0f : 1.0f;
   }
 }
 // f(tag of the activation): the choice is made once, not at every value.

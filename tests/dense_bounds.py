@@ -8,6 +8,10 @@ U = 2.0 ** -24   # half a step of f32
 H = 2.0 ** -8    # half a step of bf16
 
 
+TORCH_ACT = {"silu": torch.nn.functional.silu, "gelu": torch.nn.functional.gelu,
+             "gelu_tanh": lambda t: torch.nn.functional.gelu(t, approximate="tanh"), "relu": torch.relu}
+
+
 class V:
     """A value and a bound on the distance of the kernel's from it."""
 

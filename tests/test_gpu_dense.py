@@ -608,3 +608,28 @@ def test_f32_module_follows_its_weights(dev):
     ffn.w1.weight.data.mul_(2.0)
     kmoe.weights_changed(ffn)
     assert not torch.equal(ffn(x), z)
+
+
+# ---------------------------------------------------------------- values that are not finite
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("T", [5, 40, 300])
+def test_a_nan_of_the_gate_shows(dev, T, act):
+    """In the result and in the gradients where the formula (torch's, in 64 bits) has it; of one row's
+    adapter in that row."""
+    x, wg, wu, wd = make_ffn(dev, T, 72, 136)
+    dy = rnd(dev, T, 72)
+    wg[9, 3] = float("nan")
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = kmoe.gated_ffn(*leaves, act)
+    got = (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    lx, lg, lu, ld = ref = [t.double().requires_grad_(True) for t in (x, wg, wu, wd)]
+    z = (B.TORCH_ACT[act](lx @ lg.t()) * (lx @ lu.t())) @ ld.t()
+    for g, w in zip(got, (z.detach(), *torch.autograd.grad(z, ref, dy.double()))):
+        assert torch.equal(g.isnan(), w.isnan())
+    x, wg, wu, wd = make_ffn(dev, T, 72, 136)
+    ad, ids = make_ad(dev, 3, 8, 72, 136), make_ids(dev, T, 3, "mixed")
+    ids[2] = 1
+    ad.b[1, 17] = float("nan")
+    with torch.no_grad():
+        y = kmoe.gated_ffn(x, wg, wu, wd, act, kmoe.FFNAdapters(gate=ad), ids)
+    assert torch.equal(y.isnan(), (ids == 1)[:, None].expand_as(y))
