@@ -353,7 +353,7 @@ struct Outer {
               __builtin_amdgcn_sched_barrier(0);
             });
             hold(acc);
-            if (split) apart(acc, fb[c], id[c]);
+            if (split) apart(acc, fb[c], id[c], s, pass);
             hold(acc);
           }
         });
@@ -366,11 +366,15 @@ struct Outer {
     for (int i = 0; i < 4 * QA * QB; ++i) asm volatile("" : "+a"(acc[i / (2 * QA * QB)][i / (QA * QB) % 2][i / QB % QA][i % QB]));
     __builtin_amdgcn_sched_barrier(0);
   }
-  // a turn's products, one adapter at a time
-  __device__ __forceinline__ void apart(f32x4_t (&acc)[2][2][QA][QB], const bf16x8_t (&fb)[2 * QB], int id) {
+  // a turn's products, one adapter at a time.  A lane past the ranks holds some rank's factor again, which
+  // must not meet its zeros; and what the inner products lost meets the finite factors only: an infinity
+  // has what it makes of the inner product itself.
+  __device__ __forceinline__ void apart(f32x4_t (&acc)[2][2][QA][QB], const bf16x8_t (&fb)[2 * QB], int id, int s, int pass) {
+    const bool past = s + k0 >= ad.r;
 #pragma unroll 1
     for (int p = 0; p < per; ++p) {
       const int cur = __builtin_amdgcn_readlane(id, per == 4 ? p * 16 : p * 32);
+      const bool here = slot == p && !past;
       static_for<0, 2 * QA>([&](auto bt) {
         constexpr int blk = decltype(bt)::value;
         const bf16x8_t zero = {};
@@ -380,15 +384,29 @@ struct Outer {
           f32x4_t& a = acc[blk / QA][yj / QB][blk % QA][yj % QB];
           f32x4_t d = a;
 #pragma unroll
-          for (int q = 0; q < HELD; ++q)
+          for (int q = 0; q < HELD; ++q) {
+            const bool lost = HELD > 1 ? q > 0 : pass > 0;
             d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                slot == p ? fb[yj] : zero, slot == p && own[blk] == cur ? fv[GATED ? yj / QB : 0][q][blk] : zero, d, 0, 0, 0);
+                here ? (lost ? finite(fb[yj]) : fb[yj]) : zero,
+                here && own[blk] == cur ? fv[GATED ? yj / QB : 0][q][blk] : zero, d, 0, 0, 0);
+          }
 #pragma unroll
           for (int q = 0; q < 4; ++q) a[q] = own[blk] == cur ? d[q] : a[q];
           asm volatile("" : "+a"(a));
         });
       });
     }
+  }
+  // f with zeros for infinities and NaN
+  __device__ __forceinline__ static bf16x8_t finite(bf16x8_t f) {
+    i32x4_t w = __builtin_bit_cast(i32x4_t, f);
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const uint32_t u = (uint32_t)w[q];
+      const uint32_t lo = (u & 0x7f80u) == 0x7f80u ? 0u : u & 0xffffu;
+      w[q] = (int)((u & 0x7f800000u) == 0x7f800000u ? lo : lo | (u & 0xffff0000u));
+    }
+    return __builtin_bit_cast(bf16x8_t, w);
   }
 };
 

@@ -633,3 +633,45 @@ def test_a_nan_of_the_gate_shows(dev, T, act):
     with torch.no_grad():
         y = kmoe.gated_ffn(x, wg, wu, wd, act, kmoe.FFNAdapters(gate=ad), ids)
     assert torch.equal(y.isnan(), (ids == 1)[:, None].expand_as(y))
+
+
+def same_infinities(got, want):
+    """Infinite where the formula is, of its sign, and finite elsewhere."""
+    inf = want.isinf()
+    assert not bool(want.isnan().any()) and bool(inf.any())
+    assert torch.equal(got.isinf(), inf) and torch.equal(got[inf].double(), want[inf]) and not bool(got.isnan().any())
+
+
+@pytest.mark.parametrize("r,j", [(8, 0), (16, 9), (24, 0), (32, 0), (40, 0), (40, 33), (56, 7)])
+@pytest.mark.parametrize("T", [5, 20, 60, 300, 2042])
+def test_infinite_factors(dev, T, r, j):
+    """An infinity of an adapter's factor makes one of its sign in the rows that have the adapter: ranks past
+    the last one and what the inner products lost add nothing to it."""
+    d, F, n = 72, 264, 4
+    x, wg, wu, wd = make_ffn(dev, T, d, F)
+    ids = make_ids(dev, T, n, "mixed")
+    ids[1] = 2
+    ad, up = make_ad(dev, n, r, d, F), make_ad(dev, n, r, d, F)
+    delta = lambda t, ad, i: float(ad.scale[i]) * (t @ ad.a[i].double().t()) @ ad.b[i].double().t()
+
+    def formula(t, w, ad):
+        y = t @ w.double().t()
+        for i in range(n):
+            y[ids == i] += delta(t[ids == i], ad, i)
+        return y
+    ad.b[2, 130, j] = float("inf")
+    with torch.no_grad():
+        y = kmoe.adapted_linear(x, wu, ad, ids)
+        same_infinities(y, formula(x.double(), wu, ad))
+        up.b[2, 130, j] = float("-inf")
+        y = kmoe.gated_ffn(x, wg, wu, wd, "silu", kmoe.FFNAdapters(up=up), ids)
+        h = torch.nn.functional.silu(x.double() @ wg.double().t()) * formula(x.double(), wu, up)
+        same_infinities(y, h @ wd.double().t())
+    # backward: the other factor's
+    ad = make_ad(dev, n, r, d, F)
+    ad.a[2, j, 40] = float("inf")
+    w, dy = rnd(dev, F, d, std=0.1), rnd(dev, T, F)
+    lx = rnd(dev, T, d).requires_grad_(True)
+    (dx,) = torch.autograd.grad(kmoe.adapted_linear(lx, w, ad, ids), lx, dy)
+    back = kmoe.Adapters(ad.b.transpose(1, 2), ad.a.transpose(1, 2), ad.scale)
+    same_infinities(dx, formula(dy.double(), w.t(), back))
