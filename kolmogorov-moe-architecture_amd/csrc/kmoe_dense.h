@@ -324,6 +324,7 @@ struct Outer {
           load(s, t + C);
         else if (s + 32 < ad.r || pass + 1 < PASSES)
           load(s + 32 < ad.r ? s + 32 : 0, 0);
+        uint32_t splits = 0;
         static_for<0, C>([&](auto ct) {
           constexpr int c = decltype(ct)::value;
           if (C == 1 || t + c < turns) {
@@ -353,10 +354,25 @@ struct Outer {
               __builtin_amdgcn_sched_barrier(0);
             });
             hold(acc);
-            if (split) apart(acc, fb[c], id[c], s, pass);
-            hold(acc);
+            splits |= split ? 1u << c : 0u;
           }
         });
+        // (a row has terms in one turn only, so those taken apart may come last, in one copy of the code)
+        for (; splits; splits &= splits - 1) {
+          const int at = __builtin_ctz(splits);
+          bf16x8_t f[2 * QB];
+          int who = 0;
+          static_for<0, C>([&](auto ct) {
+            constexpr int c = decltype(ct)::value;
+            if (at == c) {
+#pragma unroll
+              for (int yj = 0; yj < 2 * QB; ++yj) f[yj] = fb[c][yj];
+              who = id[c];
+            }
+          });
+          apart(acc, f, who, s, pass);
+          hold(acc);
+        }
       }
     }
   }
@@ -369,29 +385,30 @@ struct Outer {
   // a turn's products, one adapter at a time.  A lane past the ranks holds some rank's factor again, which
   // must not meet its zeros; and what the inner products lost meets the finite factors only: an infinity
   // has what it makes of the inner product itself.
-  __device__ __forceinline__ void apart(f32x4_t (&acc)[2][2][QA][QB], const bf16x8_t (&fb)[2 * QB], int id, int s, int pass) {
-    const bool past = s + k0 >= ad.r;
+  __device__ __forceinline__ void apart(f32x4_t (&acc)[2][2][QA][QB], bf16x8_t (&fb)[2 * QB], int id, int s, int pass) {
+    const bf16x8_t zero = {};
+#pragma unroll
+    for (int yj = 0; yj < 2 * QB; ++yj) fb[yj] = s + k0 < ad.r ? fb[yj] : zero;
 #pragma unroll 1
-    for (int p = 0; p < per; ++p) {
+    for (int i = 0; i < HELD * per; ++i) {  // (one body for both parts: the instruction cache holds more of the turns)
+      const int p = HELD > 1 && i >= per ? i - per : i;
+      const bool lost = HELD > 1 ? i >= per : pass > 0;
+      if (p == 0 && lost) {
+#pragma unroll
+        for (int yj = 0; yj < 2 * QB; ++yj) fb[yj] = finite(fb[yj]);
+      }
       const int cur = __builtin_amdgcn_readlane(id, per == 4 ? p * 16 : p * 32);
-      const bool here = slot == p && !past;
       static_for<0, 2 * QA>([&](auto bt) {
         constexpr int blk = decltype(bt)::value;
-        const bf16x8_t zero = {};
         static_for<0, 2 * QB>([&](auto yt) {
-          constexpr int yj = decltype(yt)::value;
+          constexpr int yj = decltype(yt)::value, h = GATED ? yj / QB : 0;
           // (from the sums on, as the others: a row's result does not depend on whom it is computed with)
           f32x4_t& a = acc[blk / QA][yj / QB][blk % QA][yj % QB];
-          f32x4_t d = a;
+          const bf16x8_t v = HELD > 1 && lost ? fv[h][HELD - 1][blk] : fv[h][0][blk];
+          const f32x4_t d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              slot == p ? fb[yj] : zero, slot == p && own[blk] == cur ? v : zero, a, 0, 0, 0);
 #pragma unroll
-          for (int q = 0; q < HELD; ++q) {
-            const bool lost = HELD > 1 ? q > 0 : pass > 0;
-            d = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-                here ? (lost ? finite(fb[yj]) : fb[yj]) : zero,
-                here && own[blk] == cur ? fv[GATED ? yj / QB : 0][q][blk] : zero, d, 0, 0, 0);
-          }
-#pragma unroll
-          for (int q = 0; q < 4; ++q) a[q] = own[blk] == cur ? d[q] : a[q];
+          for (int c = 0; c < 4; ++c) a[c] = own[blk] == cur ? d[c] : a[c];
           asm volatile("" : "+a"(a));
         });
       });
