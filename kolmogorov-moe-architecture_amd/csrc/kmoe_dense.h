@@ -152,6 +152,9 @@ __device__ __forceinline__ void store_lost(uint16_t* to, const float* v, i32x2_t
   }
   *reinterpret_cast<i32x2_t*>(to) = pack4(r[0], r[1], r[2], r[3]);
 }
+// A product's result with what its operand lost by the rounding.  An infinity of the other operand has made
+// its infinity of the operand itself; what that lost would make a second one of any sign, or a NaN.
+__device__ __forceinline__ float with_lost(float v, float lost) { return v - v == 0.0f ? v + lost : v; }
 // What the backward multiplies by, up act'(gate) and act(gate), is held in 24 bits, the top of its f32:
 // in bf16 its rounding would add to those of the products' operands and results, a third of one
 // size (gradients of the weights and of x: 1.73 roundings off, so 1.41).  It lies as the MFMAs
@@ -799,7 +802,9 @@ __global__ __launch_bounds__(THREADS, (side_by_side<BM, BN, KS, STAGES>)) __attr
 #pragma unroll
       for (int y = 0; y < 2; ++y)
 #pragma unroll
-        for (int j = 0; j < QB; ++j) acc[0][y][0][j] += acc[1][y][0][j];
+        for (int j = 0; j < QB; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) acc[0][y][0][j][c] = with_lost(acc[0][y][0][j][c], acc[1][y][0][j][c]);
       hold();
     }
   }

@@ -76,7 +76,7 @@ __global__ __launch_bounds__(512) void few_kernel(Args g) {
   for (int k = 1; k < W; ++k) s += part[k][lane];
   if (g.fold) {
 #pragma unroll
-    for (int c = 0; c < 4; ++c) s[c] += __shfl(s[c], lane | 8, 64);
+    for (int c = 0; c < 4; ++c) s[c] = with_lost(s[c], __shfl(s[c], lane | 8, 64));
   }
   if (l16 >= g.M || 4 * lq >= ROWS || n >= g.N) return;
   if constexpr (ADAPT) {

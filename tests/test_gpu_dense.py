@@ -675,3 +675,18 @@ def test_infinite_factors(dev, T, r, j):
     (dx,) = torch.autograd.grad(kmoe.adapted_linear(lx, w, ad, ids), lx, dy)
     back = kmoe.Adapters(ad.b.transpose(1, 2), ad.a.transpose(1, 2), ad.scale)
     same_infinities(dx, formula(dy.double(), w.t(), back))
+
+
+@pytest.mark.parametrize("T", [1, 5, 8, 9, 20, 32, 40])
+def test_infinite_weights(dev, T):
+    """An infinity of the down projection meets the hidden values, not what these lost by their rounding."""
+    for d, F in ((72, 136), (72, 2056)):
+        x, wg, wu, wd = make_ffn(dev, T, d, F)
+        wd[5, 77], wd[60, 3] = float("inf"), float("-inf")
+        with torch.no_grad():
+            y = kmoe.gated_ffn(x, wg, wu, wd)
+        z = kmoe.gated_ffn(x.clone().requires_grad_(True), wg, wu, wd).detach()
+        xs = x.double()
+        want = (torch.nn.functional.silu(xs @ wg.double().t()) * (xs @ wu.double().t())) @ wd.double().t()
+        same_infinities(y, want)
+        same_infinities(z, want)
