@@ -117,7 +117,9 @@ __device__ __forceinline__ void act_at(float g, float& a, float& da) {
     // tanh(z) = 1 - 2 / (1 + e^(2z)): 1 and -1 at its ends
     const float t = 1.0f - 2.0f * __builtin_amdgcn_rcpf(1.0f + __expf(2.0f * in));
     a = 0.5f * g * (1.0f + t);
-    da = 0.5f * (1.0f + t) + 0.5f * g * (1.0f - t * t) * 0.79788456f * (1.0f + 0.134145f * g2);
+    // (where tanh is 1 or -1 its slope is 0, also against a square past f32's range)
+    const float slope = 1.0f - t * t;
+    da = 0.5f * (1.0f + t) + (slope == 0.0f ? 0.0f : 0.5f * g * slope * 0.79788456f * (1.0f + 0.134145f * g2));
   } else {
     a = g <= 0.0f ? 0.0f : g;  // (a NaN stays one)
     da = g <= 0.0f ? 0.0f : 1.0f;

@@ -690,3 +690,24 @@ def test_infinite_weights(dev, T):
         want = (torch.nn.functional.silu(xs @ wg.double().t()) * (xs @ wu.double().t())) @ wd.double().t()
         same_infinities(y, want)
         same_infinities(z, want)
+
+
+@pytest.mark.parametrize("act", ACTS)
+@pytest.mark.parametrize("T", [5, 40])
+def test_huge_gates(dev, T, act):
+    """Pre-activations whose square f32 does not hold: the activations are 0 or the gate, their slopes 0 or 1."""
+    x, wg, wu, wd = make_ffn(dev, T, 72, 136)
+    dy = rnd(dev, T, 72)
+    wg[9] *= 1e25
+    wu[9] *= 1e-25
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = kmoe.gated_ffn(*leaves, act)
+    got = (y.detach(), *torch.autograd.grad(y, leaves, dy))
+    assert all(bool(torch.isfinite(g).all()) for g in got)
+    # row 9 of dwg: each term is off by the rounding of dgate and little else, the sum by its own
+    xs, gate, up = x.double(), x.double() @ wg[9].double(), x.double() @ wu[9].double()
+    on = (gate > 0).double() * up
+    want = (dy.double() @ wd[:, 9].double() * on) @ xs
+    terms = (dy.double().abs() @ wd[:, 9].double().abs() * on.abs()) @ xs.abs()
+    assert bool((gate.abs() > 2e19).all())
+    assert bool(((got[2][9].double() - want).abs() <= 4 * B.H * terms).all())
