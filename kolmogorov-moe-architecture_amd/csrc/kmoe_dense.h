@@ -157,10 +157,12 @@ __device__ __forceinline__ void store_lost(uint16_t* to, const float* v, i32x2_t
 // A product's result with what its operand lost by the rounding.  An infinity of the other operand has made
 // its infinity of the operand itself; what that lost would make a second one of any sign, or a NaN.
 __device__ __forceinline__ float with_lost(float v, float lost) { return v - v == 0.0f ? v + lost : v; }
-// What the backward multiplies by, up act'(gate) and act(gate), is held in 24 bits, the top of its f32:
-// in bf16 its rounding would add to those of the products' operands and results, a third of one
-// size (gradients of the weights and of x: 1.73 roundings off, so 1.41).  It lies as the MFMAs
-// leave it, by 16 x 16 blocks, a lane's four values in 12 bytes: in one access of 768 bytes a wave.
+// What the backward multiplies by, up act'(gate) and act(gate), is held in 24 bits, the top of its f32
+// rounded to the nearest, ties to even (cut, it would lose up to twice as much, always towards zero;
+// 2042 rows, forward and backward 427.7 us, cut 426.6): in bf16 its rounding would add to those of the
+// products' operands and results, a third of one size (gradients of the weights and of x: 1.73
+// roundings off, so 1.41).  It lies as the MFMAs leave it, by 16 x 16 blocks, a lane's four values
+// in 12 bytes: in one access of 768 bytes a wave.
 constexpr int SAVED_BLOCK = 2 * 768;  // bytes of a block: both values
 struct Three {  // (12 bytes: a vector of three would be stored as four)
   uint32_t a, b, c;
@@ -171,7 +173,11 @@ __device__ __forceinline__ uint8_t* saved_block(uint8_t* p, int N, int64_t m, in
 __device__ __forceinline__ void store24(uint8_t* block, int lane, const float* v) {
   uint32_t u[4];
 #pragma unroll
-  for (int t = 0; t < 4; ++t) u[t] = __float_as_uint(v[t]);
+  // (a NaN is a bf16 number's or an operation's own: its low bits are zeros and do not carry)
+  for (int t = 0; t < 4; ++t) {
+    u[t] = __float_as_uint(v[t]);
+    u[t] += 0x7fu + ((u[t] >> 8) & 1u);
+  }
   *reinterpret_cast<Three*>(block + lane * 12) = {(u[0] >> 8) | (u[1] << 16 & 0xff000000u),
                                                   (u[1] >> 16) | (u[2] << 8 & 0xffff0000u),
                                                   (u[2] >> 24) | (u[3] & 0xffffff00u)};

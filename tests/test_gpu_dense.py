@@ -711,3 +711,38 @@ def test_huge_gates(dev, T, act):
     terms = (dy.double().abs() @ wd[:, 9].double().abs() * on.abs()) @ xs.abs()
     assert bool((gate.abs() > 2e19).all())
     assert bool(((got[2][9].double() - want).abs() <= 4 * B.H * terms).all())
+
+
+@pytest.mark.parametrize("T,F", [(5, 24), (33, 264)])
+def test_saved_values_are_rounded(dev, T, F):
+    """act(gate), kept in 24 bits for the backward: half a step (2^-16) off at most, to either side."""
+    d = 8
+    g = torch.Generator().manual_seed(T)
+    x, wg, wu = torch.zeros(T, d), torch.zeros(F, d), torch.zeros(F, d)
+    x[:, 0], x[:, 1] = 1.0, torch.randint(1, 3, (T,), generator=g).float()
+    # gates of up to 18 bits, exact in f32
+    wg[:, 0] = torch.randint(128, 256, (F,), generator=g) / 128
+    wg[:, 1] = torch.randint(128, 256, (F,), generator=g) * 2.0 ** -18
+    wu[:, 0] = 1.0
+    want = x.double() @ wg.double().t()
+    assert torch.equal(want.float().double(), want)
+    wg[3, 0], wg[4, 0], wg[5, 0] = float("nan"), float("inf"), 3.3e38
+    x, wg, wu = (t.to(BF).to(dev) for t in (x, wg, wu))
+    wg.view(torch.int16)[6:8, 0] = torch.tensor([0x7fff, -1], dtype=torch.int16, device=dev)  # other NaN
+    h = torch.empty(T, F, device=dev, dtype=BF)
+    saved = torch.zeros(_lib.load().kmoe_dense_saved_bytes(T, F), device=dev, dtype=torch.uint8)
+    _lib.call("kmoe_dense_gate_up", x.data_ptr(), T, d, wg.data_ptr(), wu.data_ptr(), F, _lib.ACTIVATIONS["relu"], h.data_ptr(), 0,
+              saved.data_ptr(), _lib.stream_ptr(dev))
+    # blocks of 16 x 16: both values, 64 lanes (4 columns / row), 4 columns, 3 bytes
+    b = saved.cpu().long().view(-(-T // 16), -(-F // 16), 2, 4, 16, 4, 3)
+    bits = (b[..., 0] << 8) | (b[..., 1] << 16) | (b[..., 2] << 24)
+    v = bits.to(torch.int64).where(bits < 1 << 31, bits - (1 << 32)).to(torch.int32).view(torch.float32)
+    v = v.permute(2, 0, 4, 1, 3, 5).reshape(2, b.shape[0] * 16, b.shape[1] * 16)[:, :T, :F]
+    up, a = v[0], v[1].double()
+    plain = [f for f in range(F) if f not in (3, 4, 5, 6, 7)]
+    assert bool((up[:, plain] == 1).all()) and bool(a[:, [3, 6, 7]].isnan().all()) and bool((a[:, 4] == float("inf")).all())
+    assert bool((a[:, 5] >= 3.2e38).all())
+    off = (a - want)[:, plain] / want[:, plain]
+    assert float(off.abs().max()) <= 2.0 ** -16
+    # (of n values, each within half a step to either side: 5 deviations of their mean)
+    assert abs(float(off.mean())) <= 5 * 2.0 ** -16 / (3 * off.numel()) ** 0.5
