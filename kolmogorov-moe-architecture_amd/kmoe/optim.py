@@ -83,16 +83,16 @@ class AdamW(torch.optim.Optimizer):
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
                  master_weights=False):
-        if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
-            raise ValueError(f"kmoe.AdamW: lr={lr}")
-        self._check(dict(betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
+        self._check(dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
         self._plans, self._stepped, self._held, self._seen = None, [], [], {}
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=bool(master_weights)))
 
     @staticmethod
     def _check(group):
-        b1, b2 = group["betas"]
+        lr, (b1, b2) = group["lr"], group["betas"]
+        if not isinstance(lr, torch.Tensor) and not lr >= 0.0:
+            raise ValueError(f"kmoe.AdamW: lr={lr}")
         if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0 and group["eps"] >= 0.0 and group["weight_decay"] >= 0.0):
             raise ValueError(f"kmoe.AdamW: betas {group['betas']} lie in [0, 1), eps {group['eps']} and weight_decay "
                              f"{group['weight_decay']} are not negative")
@@ -102,9 +102,13 @@ class AdamW(torch.optim.Optimizer):
     def add_param_group(self, group):
         super().add_param_group(group)
         group = self.param_groups[-1]
-        self._check(group)
-        for p in group["params"]:
-            self._check_param(p)
+        try:
+            self._check(group)
+            for p in group["params"]:
+                self._check_param(p)
+        except Exception:
+            self.param_groups.pop()
+            raise
         self._plans = None
 
     @staticmethod

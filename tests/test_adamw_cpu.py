@@ -271,3 +271,18 @@ def test_master_weights_outlive_a_copy(steps, how):
     opt.step()
     got = opt.state[q]["master"]
     assert torch.equal(got[:3], fine[:3]) and float(got[3]) == 7.0 and bool(got[4].isnan())
+
+
+@pytest.mark.parametrize("group,match", [
+    (dict(params=[_param(4, dtype=torch.float16)]), "bf16 or f32"), (dict(params=[_param(4), torch.nn.Parameter(torch.zeros(4, 6).t())]), "contiguous"),
+    (dict(params=[_param(4)], state_bits=4), "state_bits"), (dict(params=[_param(4)], betas=(0.9, 1.0)), "betas"),
+    (dict(params=[_param(4)], lr=-1.0), "lr=-1"), (dict(params=[_param(4)], lr=float("nan")), "lr=nan")])
+def test_a_refused_group_does_not_join(group, match):
+    opt = kmoe.AdamW([_param(4)])
+    good = opt.param_groups[0]
+    for _ in range(2):
+        with pytest.raises(ValueError, match=match):
+            opt.add_param_group(dict(group))
+        assert len(opt.param_groups) == 1 and opt.param_groups[0] is good
+    opt.add_param_group({"params": [_param(4)], "lr": torch.tensor(0.1)})
+    assert len(opt.param_groups) == 2
