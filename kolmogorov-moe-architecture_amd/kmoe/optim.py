@@ -27,6 +27,7 @@ class _Plan:
 
     def __init__(self, params, states, has_master):
         dev = params[0].device
+        self._apart(params, states)
         rows, base, owner = [], [0], []
         for i, (p, st) in enumerate(zip(params, states)):
             rows.append([*self._where(p, st), p.numel()])
@@ -48,6 +49,15 @@ class _Plan:
         self.device = dev
         self.at = [(p.data_ptr(), p.numel(), p.dtype) for p in params]
         self.held = [[(k, t, t.data_ptr()) for k, t in st.items()] for st in states]
+
+    @staticmethod
+    def _apart(params, states):
+        """Refuses tensors that share memory: workgroups write them side by side."""
+        places = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), tuple(p.shape))
+                        for p, st in zip(params, states) for t in (p, *st.values()) if t.numel())
+        for (_, end, a), (start, _, b) in zip(places, places[1:]):
+            if start < end:
+                raise ValueError(f"kmoe.AdamW: parameters {a} and {b} of one group, or states of theirs, share memory")
 
     @staticmethod
     def _where(p, st):
@@ -106,6 +116,8 @@ class AdamW(torch.optim.Optimizer):
             self._check(group)
             for p in group["params"]:
                 self._check_param(p)
+            if len(set(map(id, group["params"]))) < len(group["params"]):
+                raise ValueError("kmoe.AdamW: a parameter stands twice in its group")
         except Exception:
             self.param_groups.pop()
             raise

@@ -286,3 +286,40 @@ def test_a_refused_group_does_not_join(group, match):
         assert len(opt.param_groups) == 1 and opt.param_groups[0] is good
     opt.add_param_group({"params": [_param(4)], "lr": torch.tensor(0.1)})
     assert len(opt.param_groups) == 2
+
+
+@pytest.mark.filterwarnings("ignore:optimizer contains")
+def test_parameters_that_share_memory_are_refused(steps):
+    """Their values would be stepped by two workgroups at once."""
+    p = _param(40)
+    with pytest.raises(ValueError, match="twice"):
+        kmoe.AdamW([p, p])
+    opt = kmoe.AdamW([_param(4)])
+    with pytest.raises(ValueError, match="twice"):
+        opt.add_param_group({"params": [p, _param(3), p]})
+    assert len(opt.param_groups) == 1
+    buf = torch.zeros(100)
+    for cut in ((0, 40, 39, 100), (0, 100, 40, 60), (50, 60, 0, 51)):
+        ps = [OnGpu(buf[cut[0]:cut[1]]), OnGpu(buf[cut[2]:cut[3]])]
+        for q in ps:
+            q.grad = torch.ones_like(q.detach())
+        opt = kmoe.AdamW(ps)
+        for _ in range(2):
+            with pytest.raises(ValueError, match="share memory"):
+                opt.step()
+        n = len(steps)
+        kmoe.AdamW([{"params": [q]} for q in ps]).step()  # groups are stepped one after the other
+        assert len(steps) == n + 2
+    a, b = _on_gpu(5, 300)
+    opt = kmoe.AdamW([a, b])
+    m = torch.zeros(305)
+    for q, at in ((a, m[:5]), (b, m[4:304])):
+        opt.set_state(q, 1, exp_avg=at, exp_avg_sq=torch.zeros(q.numel()))
+    with pytest.raises(ValueError, match="share memory"):
+        opt.step()
+    n = len(steps)
+    ps = [OnGpu(buf[:40]), OnGpu(buf[:0]), OnGpu(buf[40:]), OnGpu(torch.zeros(0))]
+    for q in ps:
+        q.grad = torch.ones_like(q.detach())
+    kmoe.AdamW(ps).step()
+    assert len(steps) == n + 1
