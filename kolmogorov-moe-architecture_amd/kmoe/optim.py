@@ -291,7 +291,7 @@ class AdamW(torch.optim.Optimizer):
                     # (anew where it does not round to the parameter: what was not written keeps its bits)
                     master = plan.states[i]["master"]
                     master.copy_(torch.where(master.to(p.dtype) == p, master, p.float()))
-            if not moved:
+            if not any(p.numel() for p in moved):
                 continue
             if capturing and not any(h is plan for h in self._held):
                 self._held.append(plan)  # the replays read its tables

@@ -365,3 +365,14 @@ def test_a_copied_optimizer_goes_on(dev, bits):
         for p, q in zip(ps, qs):
             assert torch.equal(p, q) and torch.equal(opt.state[p]["master"], other.state[q]["master"])
             assert not torch.equal(opt.state[p]["master"], p.detach().float())
+
+
+def test_groups_of_empty_parameters(dev):
+    """Nothing to step is no error."""
+    e, p = torch.nn.Parameter(torch.zeros(0, 5, device=dev)), torch.nn.Parameter(torch.ones(3, device=dev))
+    e.grad, p.grad = torch.zeros_like(e), torch.ones_like(p)
+    for bits in (32, 8):
+        opt = kmoe.AdamW([{"params": [e]}, {"params": [p]}], state_bits=bits, **HYPER)
+        opt.step()
+        opt.step()
+        assert int(opt.state[p]["step"]) == 2 and all(t.numel() == 0 for t in opt.state_values(e))
