@@ -130,7 +130,7 @@ class AdamW(torch.optim.Optimizer):
         if not p.is_contiguous():
             raise ValueError(f"kmoe.AdamW: parameters are contiguous, got strides {p.stride()} of {tuple(p.shape)}")
 
-    # _plans: the tables of the last step, _stepped: each group's parameters in them; _held: tables that
+    # _plans: the tables of the last step, _stepped: each group's parameters in them; _held: what
     # captured steps read; _seen: version of each parameter with an f32 copy after its last step
     def __setstate__(self, state):
         super().__setstate__(state)
@@ -293,8 +293,8 @@ class AdamW(torch.optim.Optimizer):
                     master.copy_(torch.where(master.to(p.dtype) == p, master, p.float()))
             if not any(p.numel() for p in moved):
                 continue
-            if capturing and not any(h is plan for h in self._held):
-                self._held.append(plan)  # the replays read its tables
+            if capturing and not any(a is plan and b is group["lr"] for a, b in self._held):
+                self._held.append((plan, group["lr"]))  # the replays read its tables, and a rate on the GPU
             with _device(plan.device):
                 _lib.call("kmoe_adamw", plan.table.data_ptr(), plan.owner.data_ptr(), plan.base.data_ptr(),
                           plan.base_host, len(plan.params), plan.grads, plan.dtype, plan.bits,

@@ -376,3 +376,25 @@ def test_groups_of_empty_parameters(dev):
         opt.step()
         opt.step()
         assert int(opt.state[p]["step"]) == 2 and all(t.numel() == 0 for t in opt.state_values(e))
+
+
+def test_a_captured_step_keeps_its_learning_rate(dev):
+    """A rate on the GPU that the program drops or replaces after the capture is not read from freed memory."""
+    (p,), (g,) = _tensors(dev, [(300,)], torch.float32)
+    q = torch.nn.Parameter(p.detach().clone())
+    p.grad, q.grad = g, g.clone()
+    hp = {k: v for k, v in HYPER.items() if k != "lr"}
+    opt = kmoe.AdamW([{"params": [p], "lr": torch.full((), 1e-2, device=dev)}], **hp)
+    eager = kmoe.AdamW([q], lr=1e-2, **hp)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    opt.param_groups[0]["lr"] = 1e-3
+    other = [torch.full((), 7.0, device=dev) for _ in range(64)]  # where the old one was, if it was freed
+    for _ in range(2):
+        graph.replay()
+    torch.cuda.synchronize()
+    for _ in range(3):
+        eager.step()
+    assert torch.equal(p, q) and len(other) == 64
