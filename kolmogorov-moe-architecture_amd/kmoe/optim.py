@@ -293,8 +293,9 @@ class AdamW(torch.optim.Optimizer):
                     master.copy_(torch.where(master.to(p.dtype) == p, master, p.float()))
             if not any(p.numel() for p in moved):
                 continue
-            if capturing and not any(a is plan and b is group["lr"] for a, b in self._held):
-                self._held.append((plan, group["lr"]))  # the replays read its tables, and a rate on the GPU
+            if capturing and not any(a is plan and b is group["lr"] for a, b, _ in self._held):
+                # the replays read its tables and a rate on the GPU, and write the parameters as they lie now
+                self._held.append((plan, group["lr"], [p.detach() for p in plan.params]))
             with _device(plan.device):
                 _lib.call("kmoe_adamw", plan.table.data_ptr(), plan.owner.data_ptr(), plan.base.data_ptr(),
                           plan.base_host, len(plan.params), plan.grads, plan.dtype, plan.bits,

@@ -398,3 +398,25 @@ def test_a_captured_step_keeps_its_learning_rate(dev):
     for _ in range(3):
         eager.step()
     assert torch.equal(p, q) and len(other) == 64
+
+
+def test_a_captured_step_keeps_its_memory(dev):
+    """Replays after a parameter or its states were given other memory write what they were captured with, not
+    what has come there since."""
+    (p,), (g,) = _tensors(dev, [(3000,)], torch.float32)
+    p.grad = g
+    opt = kmoe.AdamW([p], **HYPER)
+    opt.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    p.data = p.data.clone()
+    opt.state[p] = {k: v.clone() for k, v in opt.state[p].items()}
+    opt.step()  # with tables of its own
+    kept = p.detach().clone()
+    other = [torch.full((3000,), 7.0, device=dev) for _ in range(64)]
+    step = int(opt.state[p]["step"])
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(p, kept) and int(opt.state[p]["step"]) == step
+    assert all(bool((t == 7.0).all()) for t in other)
