@@ -134,7 +134,8 @@ class AdamW(torch.optim.Optimizer):
     # captured steps read; _seen: version of each parameter with an f32 copy after its last step
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._plans, self._stepped, self._held, self._seen = None, [], [], {}
+        self._plans, self._stepped, self._seen = None, [], {}
+        self.__dict__.setdefault("_held", [])  # (torch's load_state_dict comes here too: graphs stay)
 
     def __getstate__(self):
         return {k: v for k, v in super().__getstate__().items() if k not in ("_plans", "_stepped", "_held", "_seen")}

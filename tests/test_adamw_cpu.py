@@ -323,3 +323,21 @@ def test_parameters_that_share_memory_are_refused(steps):
         q.grad = torch.ones_like(q.detach())
     kmoe.AdamW(ps).step()
     assert len(steps) == n + 1
+
+
+def test_what_captured_steps_read_outlives_a_load(steps, monkeypatch):
+    """Loading a state dict takes states and tables away from later steps, not from the graphs of earlier ones."""
+    a, b = _on_gpu(5, 300)
+    opt = kmoe.AdamW([a, b])
+    opt.step()
+    with monkeypatch.context() as m:
+        m.setattr(torch.cuda, "is_available", lambda: True)
+        m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+        opt.step()
+    (plan,) = [p for _, p in opt._plans]
+    held = list(opt._held)
+    assert any(x is plan for x in held[0])
+    opt.load_state_dict(opt.state_dict())
+    assert len(opt._held) == len(held) and all(x is y for x, y in zip(opt._held, held))
+    opt.step()
+    assert all(p is not plan for _, p in opt._plans) and steps[-1] == _want(opt, a, b)

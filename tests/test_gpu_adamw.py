@@ -420,3 +420,23 @@ def test_a_captured_step_keeps_its_memory(dev):
     torch.cuda.synchronize()
     assert torch.equal(p, kept) and int(opt.state[p]["step"]) == step
     assert all(bool((t == 7.0).all()) for t in other)
+
+
+def test_replays_after_a_load(dev):
+    """A step captured before load_state_dict still writes the parameters, with the states that it was captured with."""
+    (p,), (g,) = _tensors(dev, [(3000,)], torch.float32)
+    q = torch.nn.Parameter(p.detach().clone())
+    p.grad, q.grad = g, g.clone()
+    opt, eager = kmoe.AdamW([p], **HYPER), kmoe.AdamW([q], **HYPER)
+    opt.step()
+    eager.step()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        opt.step()
+    opt.load_state_dict(opt.state_dict())
+    other = [torch.full((n,), 7.0, device=dev) for n in (1, 16, 3000) * 30]
+    for _ in range(2):
+        graph.replay()
+        eager.step()
+    torch.cuda.synchronize()
+    assert torch.equal(p, q) and all(bool((t == 7.0).all()) for t in other)
