@@ -163,10 +163,11 @@ class AdamW(torch.optim.Optimizer):
         want = self._new_state(torch.empty(p.shape, dtype=p.dtype, device="meta"), group)
         for k, v in want.items():
             t = st.get(k)
-            if (t is None or t.dtype != v.dtype or t.numel() != v.numel() or t.device != p.device or not t.is_contiguous()):
+            if (not isinstance(t, torch.Tensor) or t.dtype != v.dtype or t.numel() != v.numel() or t.device != p.device
+                    or not t.is_contiguous()):
                 raise ValueError(f"kmoe.AdamW: the state {k} of a parameter {tuple(p.shape)} is contiguous {v.dtype} of "
                                  f"{v.numel()} values on {p.device}, got "
-                                 f"{None if t is None else (t.dtype, tuple(t.shape), str(t.device))}")
+                                 f"{(t.dtype, tuple(t.shape), str(t.device)) if isinstance(t, torch.Tensor) else t}")
 
     def set_state(self, p, step: int, **tensors) -> None:
         """Takes `tensors` (exp_avg, exp_avg_sq; in 8 bits also exp_avg_scale, exp_avg_sq_scale; with
@@ -185,7 +186,10 @@ class AdamW(torch.optim.Optimizer):
     def state_values(self, p, dtype=torch.float32):
         """(first moment, square root of the second) of p as bf16 or f32: in 8 bits the values that the
         codes stand for."""
-        st = self.state[p]
+        self._group_of(p)
+        st = self.state.get(p)
+        if not st:
+            raise ValueError(f"kmoe.AdamW: a parameter {tuple(p.shape)} has no state before its first step")
         if dtype not in (torch.bfloat16, torch.float32):
             raise ValueError(f"kmoe.AdamW: state values are bf16 or f32, not {dtype}")
         if "exp_avg_scale" not in st:
@@ -202,18 +206,29 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """As torch's, but the states keep the types they were saved in (torch casts them to their
-        parameter's)."""
+        parameter's); what is refused leaves the optimizer as it was."""
+        before = self.state, self.param_groups, self._plans, self._stepped, self._seen
         super().load_state_dict(state_dict)
-        saved = state_dict["state"]
-        params = [p for g in self.param_groups for p in g["params"]]
-        names = [i for g in state_dict["param_groups"] for i in g["params"]]
-        for i, p in zip(names, params):
-            if i in saved:
-                st = {k: v.detach().to(p.device, copy=True).contiguous() for k, v in saved[i].items()}
-                self._check_state(p, self._group_of(p), st)
-                self.state[p] = st
-                self._seen[p] = p._version
-        self._plans = None
+        try:
+            saved, states = state_dict["state"], {}
+            params = [p for g in self.param_groups for p in g["params"]]
+            names = [i for g in state_dict["param_groups"] for i in g["params"]]
+            for group in self.param_groups:
+                lacks = [k for k in ("lr", "betas", "eps", "weight_decay", "state_bits", "master_weights") if k not in group]
+                if lacks:
+                    raise ValueError(f"kmoe.AdamW: a parameter group of the state dict has no {', '.join(lacks)}")
+                self._check(group)
+            for i, p in zip(names, params):
+                if i in saved:
+                    st = {k: v.detach().to(p.device, copy=True).contiguous() if isinstance(v, torch.Tensor) else v
+                          for k, v in saved[i].items()}
+                    self._check_state(p, self._group_of(p), st)
+                    states[p] = st
+        except Exception:
+            self.state, self.param_groups, self._plans, self._stepped, self._seen = before
+            raise
+        self.state.update(states)
+        self._seen.update((p, p._version) for p in states)
 
     # ---------------------------------------------------------------- the step
     def _to_step(self, group):

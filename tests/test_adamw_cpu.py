@@ -341,3 +341,44 @@ def test_what_captured_steps_read_outlives_a_load(steps, monkeypatch):
     assert len(opt._held) == len(held) and all(x is y for x, y in zip(opt._held, held))
     opt.step()
     assert all(p is not plan for _, p in opt._plans) and steps[-1] == _want(opt, a, b)
+
+
+@pytest.mark.parametrize("bits", [8, 32])
+def test_a_refused_state_dict_changes_nothing(bits):
+    """One of another form, or of torch's own AdamW."""
+    ps = [_param(3, 100), _param(7)]
+    opt = kmoe.AdamW(ps, lr=0.5, state_bits=bits)
+    for p in ps:
+        st = opt._new_state(p, opt.param_groups[0])
+        opt.set_state(p, 5, **{k: v for k, v in st.items() if k != "step"})
+    states, groups = [opt.state[p] for p in ps], opt.param_groups
+    qs = [torch.nn.Parameter(p.detach().float()) for p in ps]
+    other = torch.optim.AdamW(qs, lr=0.25)
+    for q in qs:
+        q.grad = torch.ones_like(q)
+    other.step()
+    wrong = kmoe.AdamW([_param(3, 100), _param(8)], state_bits=bits)
+    for p in wrong.param_groups[0]["params"]:
+        st = wrong._new_state(p, wrong.param_groups[0])
+        wrong.set_state(p, 5, **{k: v for k, v in st.items() if k != "step"})
+    bad = opt.state_dict()
+    bad["state"] = {0: bad["state"][0], 1: {**bad["state"][1], "exp_avg": None}}
+    number = opt.state_dict()
+    number["state"] = {**number["state"], 1: {**number["state"][1], "step": 5}}
+    for sd, match in ((other.state_dict(), "state_bits"), (wrong.state_dict(), "the state exp_avg"), (bad, "the state exp_avg"),
+                      (number, "the state step")):
+        with pytest.raises(ValueError, match=match):
+            opt.load_state_dict(sd)
+        assert opt.param_groups is groups and groups[0]["lr"] == 0.5 and set(opt.state) == set(ps)
+        assert all(opt.state[p] is st and st["exp_avg"].dtype == (torch.uint8 if bits == 8 else torch.float32)
+                   for p, st in zip(ps, states))
+
+
+def test_values_of_no_state():
+    p = _param(5)
+    opt = kmoe.AdamW([p])
+    with pytest.raises(ValueError, match="no state"):
+        opt.state_values(p)
+    with pytest.raises(ValueError, match="not a parameter"):
+        opt.state_values(_param(5))
+    assert not opt.state
