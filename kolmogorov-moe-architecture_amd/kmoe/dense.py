@@ -73,7 +73,7 @@ def _rows(x, K, who):
 
 
 def _adapters(ad, K, N, who, name):
-    """The adapters checked, in bf16, ranks filled up to a multiple of 8 (differentiable)."""
+    """The adapters checked."""
     a, b, scale = ad
     n, r = a.shape[:2] if a.dim() == 3 else (0, 0)
     if not 1 <= r <= _lib.MAX_RANK or not 1 <= n <= 32767 or a.shape[2] != K or b.shape != (n, N, r):
@@ -85,9 +85,6 @@ def _adapters(ad, K, N, who, name):
         if scale.requires_grad and torch.is_grad_enabled():
             raise ValueError(f"kmoe.{who}: {name}scale has no gradient here: pass it detached")
         scale = _contig(scale.detach(), torch.float32)
-    fill = -r % 8
-    if fill:
-        a, b = nn.functional.pad(a, (0, 0, 0, fill)), nn.functional.pad(b, (0, fill))
     return Adapters(a, b, scale)
 
 
@@ -109,7 +106,14 @@ def _struct(ad):
 
 
 def _held(ad):
-    return None if ad is None else Adapters(_ready(ad.a), _ready(ad.b), ad.scale)
+    """The adapters as the kernels take them: bf16, ranks filled up to a multiple of 8 with zeros."""
+    if ad is None:
+        return None
+    a, b = _ready(ad.a), _ready(ad.b)
+    fill = -a.shape[1] % 8
+    if fill:
+        a, b = nn.functional.pad(a, (0, 0, 0, fill)), nn.functional.pad(b, (0, fill))
+    return Adapters(a, b, ad.scale)
 
 
 def _ready(t):
@@ -281,7 +285,7 @@ def gated_ffn(x, w_gate, w_up, w_down, activation="silu", adapters: Optional[FFN
         _one_gpu("gated_ffn", x, w_gate, w_up, w_down, ids, *(t for a in some for t in a))
         if len({a.a.shape[0] for a in some}) > 1:
             raise ValueError(f"kmoe.gated_ffn: the projections have as many adapters each, got {[a.a.shape[0] for a in some]}")
-        if adapters.gate is not None and adapters.up is not None and adapters.gate.a.shape[1] != adapters.up.a.shape[1]:
+        if adapters.gate is not None and adapters.up is not None and len({-(-a.a.shape[1] // 8) for a in adapters[:2]}) > 1:
             raise ValueError(f"kmoe.gated_ffn: the gate's and the up projection's adapters have one rank, got "
                              f"{adapters.gate.a.shape[1]} and {adapters.up.a.shape[1]}")
         i32 = _ids(ids, x, some[0].a.shape[0], "gated_ffn")
@@ -299,12 +303,14 @@ class _AdaptedFn(torch.autograd.Function):
     def forward(ctx, x, w, a, b, scale, ids):
         _bwd.leaves_of(ctx, x, w, a, b)
         xr, bw = _ready(x), _ready(w)
-        ad = None if a is None else Adapters(_ready(a), _ready(b), scale)
+        # (odd ranks are filled up here: a node of torch's for it would be one more of the leaves')
+        ad = None if a is None else _held(Adapters(a, b, scale))
         y, ws = _linear_forward(xr, bw, ad, ids)
         # (with an adapter the workspace begins with the scaled inner products)
         ba, bb, kept = (None, None, None) if a is None else (ad.a, ad.b, ws)
         ctx.save_for_backward(xr, bw, ba, bb, scale, ids, kept, *_copied((x, xr), (w, bw), (a, ba), (b, bb)))
         ctx.meta = (x.dtype, w.dtype, None if a is None else a.dtype, None if b is None else b.dtype)
+        ctx.rank = 0 if a is None else a.shape[1]
         return y if x.dtype is _BF16 else y.to(x.dtype)
 
     @staticmethod
@@ -327,6 +333,9 @@ class _AdaptedFn(torch.autograd.Function):
                 ws = torch.empty(max(wsb, 16), device=xr.device, dtype=torch.uint8)
                 _lib.call("kmoe_adapted_linear_backward", ptr(dy2), ptr(xr), T, K, ptr(bw), N, ptr(ids), n,
                           _struct(Adapters(ba, bb, scale)), ptr(v), ptr(dx), ptr(da), ptr(db), ptr(ws), wsb, _stream(xr))
+                if r != ctx.rank:
+                    da = None if da is None else da[:, :ctx.rank].contiguous()
+                    db = None if db is None else db[..., :ctx.rank].contiguous()
             elif need_x:
                 dx = _dense_dx(dy2.view(T, N), bw, T).view(xr.shape)
             if need_w:

@@ -200,3 +200,17 @@ def test_adapter_gradients_fit_their_workspace():
         have -= piece(4 * T * r) + piece(2 * n * r * K) + piece(2 * n * r * N)
         for C, C2 in ((K, N), (K, 0), (N, 0)):
             assert _partial_bytes(T, n, r, C, C2) <= have, (T, K, N, n, r, C, C2)
+
+
+def test_odd_ranks_are_filled_up_inside_the_operator():
+    """The factors reach the operator's own graph node as they are: another node of theirs, outside of it, would
+    not be seen where a capture beside a live graph of the same leaves is refused."""
+    from kmoe import dense
+    given = kmoe.Adapters(z(2, 5, 64).requires_grad_(True), z(2, 72, 5).requires_grad_(True))
+    got = dense._adapters(given, 64, 72, "adapted_linear", "")
+    assert got.a is given.a and got.b is given.b
+    a, b = (t.detach().normal_() for t in given[:2])
+    held = dense._held(kmoe.Adapters(a, b))
+    assert held.a.shape == (2, 8, 64) and held.b.shape == (2, 72, 8)
+    assert torch.equal(held.a[:, :5], a) and torch.equal(held.b[..., :5], b)
+    assert not bool(held.a[:, 5:].any()) and not bool(held.b[..., 5:].any())

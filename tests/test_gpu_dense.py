@@ -746,3 +746,31 @@ def test_saved_values_are_rounded(dev, T, F):
     assert float(off.abs().max()) <= 2.0 ** -16
     # (of n values, each within half a step to either side: 5 deviations of their mean)
     assert abs(float(off.mean())) <= 5 * 2.0 ** -16 / (3 * off.numel()) ** 0.5
+
+
+@pytest.mark.parametrize("r", [5, 8])
+def test_captured_adapters_of_any_rank(dev, r):
+    """A training step of adapters is refused beside a live graph of theirs, and else replays as it runs."""
+    T, K, N, n = 70, 72, 136, 3
+    x, w, ids, dy = rnd(dev, T, K), rnd(dev, N, K, std=0.1), make_ids(dev, T, n, "mixed").to(torch.int32), rnd(dev, T, N)
+    a, b = rnd(dev, n, r, K, std=0.1).requires_grad_(True), rnd(dev, n, N, r, std=0.3).requires_grad_(True)
+    live = kmoe.adapted_linear(x, w, kmoe.Adapters(a, b), ids)
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            kmoe.adapted_linear(x, w, kmoe.Adapters(a, b), ids)
+    with pytest.raises(RuntimeError, match="still alive"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            kmoe.gated_ffn(x, w, w, w.t().contiguous(), "silu", kmoe.FFNAdapters(gate=kmoe.Adapters(a, b)), ids)
+    del live
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = torch.autograd.grad(kmoe.adapted_linear(x, w, kmoe.Adapters(a, b), ids), (a, b), dy)
+    for _ in range(3):
+        with torch.no_grad():
+            x.copy_(rnd(dev, T, K))
+            a.mul_(-0.5)
+        graph.replay()
+        torch.cuda.synchronize()
+        other = [t.detach().clone().requires_grad_(True) for t in (a, b)]
+        want = torch.autograd.grad(kmoe.adapted_linear(x, w, kmoe.Adapters(*other), ids), other, dy)
+        assert all(torch.equal(s, t) and s.shape == u.shape and s.is_contiguous() for s, t, u in zip(got, want, (a, b)))
