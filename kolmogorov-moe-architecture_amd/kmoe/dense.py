@@ -306,8 +306,11 @@ class _AdaptedFn(torch.autograd.Function):
         # (odd ranks are filled up here: a node of torch's for it would be one more of the leaves')
         ad = None if a is None else _held(Adapters(a, b, scale))
         y, ws = _linear_forward(xr, bw, ad, ids)
-        # (with an adapter the workspace begins with the scaled inner products)
-        ba, bb, kept = (None, None, None) if a is None else (ad.a, ad.b, ws)
+        ba, bb, kept = (None, None, None) if a is None else (ad.a, ad.b, None)
+        if a is not None and ctx.needs_input_grad[3] and ws is not None:
+            # the workspace begins with the scaled inner products; partial sums behind them are not kept
+            size = 4 * ids.numel() * ba.shape[1]
+            kept = ws if ws.numel() < size + 256 else ws[:size].clone()
         ctx.save_for_backward(xr, bw, ba, bb, scale, ids, kept, *_copied((x, xr), (w, bw), (a, ba), (b, bb)))
         ctx.meta = (x.dtype, w.dtype, None if a is None else a.dtype, None if b is None else b.dtype)
         ctx.rank = 0 if a is None else a.shape[1]

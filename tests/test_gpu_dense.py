@@ -774,3 +774,23 @@ def test_captured_adapters_of_any_rank(dev, r):
         other = [t.detach().clone().requires_grad_(True) for t in (a, b)]
         want = torch.autograd.grad(kmoe.adapted_linear(x, w, kmoe.Adapters(*other), ids), other, dy)
         assert all(torch.equal(s, t) and s.shape == u.shape and s.is_contiguous() for s, t, u in zip(got, want, (a, b)))
+
+
+def test_training_keeps_what_it_reads(dev):
+    """For the backward of a projection in runs of K: the inner products, not the runs' partial sums with them;
+    nothing of them where the outer factor is frozen."""
+    T, K, N, n, r = 64, 5632, 2048, 3, 16
+    x, w, ad = rnd(dev, T, K), rnd(dev, N, K, std=K ** -0.5), make_ad(dev, n, r, K, N)
+    ids, dy = make_ids(dev, T, n, "mixed"), rnd(dev, T, N)
+    assert _lib.load().kmoe_adapted_linear_workspace_bytes(T, K, N, r) > 8 * T * r  # (it has runs)
+    a, b = (t.clone().requires_grad_(True) for t in ad[:2])
+    y = kmoe.adapted_linear(x, w, kmoe.Adapters(a, b, ad.scale), ids)
+    assert sum(t.untyped_storage().nbytes() for t in y.grad_fn.saved_tensors if t is not None and t.dtype == torch.uint8) == 4 * T * r
+    da, db = torch.autograd.grad(y, (a, b), dy)
+    z = kmoe.adapted_linear(x, w, kmoe.Adapters(a, ad.b, ad.scale), ids)
+    assert all(t is None or t.dtype != torch.uint8 for t in z.grad_fn.saved_tensors)
+    assert torch.equal(torch.autograd.grad(z, a, dy)[0], da)
+    for i in range(n):
+        t = (ids == i).nonzero().squeeze(1)
+        v = (B.mm(B.V(x[t]), B.V(ad.a[i]).t()) * float(ad.scale[i])).bf16()
+        B.check("db", db[i], B.mm(B.V(dy[t]).t(), v))
