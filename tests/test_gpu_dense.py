@@ -794,3 +794,23 @@ def test_training_keeps_what_it_reads(dev):
         t = (ids == i).nonzero().squeeze(1)
         v = (B.mm(B.V(x[t]), B.V(ad.a[i]).t()) * float(ad.scale[i])).bf16()
         B.check("db", db[i], B.mm(B.V(dy[t]).t(), v))
+
+
+@pytest.mark.parametrize("routing", ["token_choice", "expert_choice"])
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float32, BF])
+def test_shared_expert_keeps_the_result_type(dev, dtype, routing):
+    """The layer's result with a shared expert has the rows' type, as without one."""
+    c, layer = _layer(dev, moe_routing=routing)
+    layer.eval()
+    x = rnd(dev, 2, 40, 128, std=200.0, dtype=dtype)
+    shared = layer.shared_expert
+    with torch.no_grad():
+        layer._modules["shared_expert"] = None
+        base = layer(x)
+        layer._modules["shared_expert"] = shared
+        y = layer(x)
+        assert y.dtype == base.dtype == dtype and torch.equal(y, base + shared(x))
+    layer.train()
+    z = layer(x.requires_grad_(True))
+    z.float().sum().backward()
+    assert z.dtype == y.dtype and x.grad.dtype == dtype
