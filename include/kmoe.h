@@ -676,8 +676,8 @@ int kmoe_adamw_values(const void* m_codes, const float* m_scale, const void* v_c
 /* ------------------------------------------------------------------------ */
 /* Dense products beside the routed experts, on weights as torch.nn.Linear holds them (rows of
  * the output, K-contiguous), bf16, f32 sums.  Sizes other than the rows' are multiples of 8, the
- * rows any number below 2^31, rows of fewer than 2^22 values, buffers contiguous and aligned to
- * 16 bytes.
+ * rows any number below 2^31 - 63 (with adapters below 2^27 - 15; a call whose launch would have 2^32
+ * threads is refused), rows of fewer than 2^22 values, buffers contiguous and aligned to 16 bytes.
  *
  * Adapters: row t of a projection x w^T gets scale[i] (x a[i]^T) b[i]^T on top, i = ids[t]
  * (device int32; outside [0, n_adapters): no adapter); a (n, rank, K), b (n, N, rank) bf16, scale (n)

@@ -358,6 +358,9 @@ extern "C" int kmoe_adamw(const int64_t* table, const int32_t* chunk_tensor, con
     for (int t = t0; t < t1; ++t) any |= (gr.g[t - t0] = grads[t]) != nullptr;
     const int c0 = chunk_base_host[t0], c1 = chunk_base_host[t1];
     if (!any || c1 == c0) continue;
+    // (a launch has fewer than 2^32 threads)
+    KMOE_REQUIRE(c1 - c0 < 1 << 24, KMOE_ERR_SHAPE, "kmoe_adamw: %d workgroups of %d values in a launch (below 2^24)", c1 - c0,
+                 KMOE_ADAMW_CHUNK);
 #define KMOE_ADAMW_CASE(PT, B, M) launch<PT, B, M>(table, chunk_tensor, chunk_base, t0, c0, c1, tickets, gr, hp, s)
     if (dtype == KMOE_DTYPE_F32)
       bits == 32 ? KMOE_ADAMW_CASE(float, 32, false) : KMOE_ADAMW_CASE(float, 8, false);
@@ -379,7 +382,7 @@ extern "C" int kmoe_adamw_values(const void* m_codes, const float* m_scale, cons
   if (n == 0) return KMOE_OK;
   KMOE_REQUIRE(m_codes && m_scale && v_codes && v_scale && m && root, KMOE_ERR_NULL, "kmoe_adamw_values: null buffer");
   const int64_t blocks = kmoe::ceil_div<int64_t>(n, STEP_VALS);
-  KMOE_REQUIRE(blocks < (int64_t)1 << 31, KMOE_ERR_SHAPE, "kmoe_adamw_values: %lld values", (long long)n);
+  KMOE_REQUIRE(blocks < (int64_t)1 << 24, KMOE_ERR_SHAPE, "kmoe_adamw_values: %lld values", (long long)n);
   const bool wide = ((reinterpret_cast<uintptr_t>(m_codes) | reinterpret_cast<uintptr_t>(v_codes) |
                       reinterpret_cast<uintptr_t>(m) | reinterpret_cast<uintptr_t>(root)) & 15) == 0;
   const auto *mc = static_cast<const uint8_t*>(m_codes), *vc = static_cast<const uint8_t*>(v_codes);

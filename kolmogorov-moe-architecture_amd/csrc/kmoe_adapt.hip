@@ -394,8 +394,9 @@ extern "C" int kmoe_adapted_linear_backward(const void* dy, const void* x, int64
                                             const int32_t* ids, int n_adapters, const kmoe_adapter* adapter, const void* v,
                                             void* dx, void* da, void* db, void* workspace, size_t workspace_bytes,
                                             void* stream) {
-  KMOE_REQUIRE(T >= 0 && T < ((int64_t)1 << 31) && K > 0 && N > 0 && K % 8 == 0 && N % 8 == 0, KMOE_ERR_SHAPE,
-               "kmoe_adapted_linear_backward: %lld rows of %d and %d values (positive multiples of 8)", (long long)T, K, N);
+  KMOE_REQUIRE(T >= 0 && T <= kmoe_dense::ADAPTED_ROWS && K > 0 && N > 0 && K % 8 == 0 && N % 8 == 0, KMOE_ERR_SHAPE,
+               "kmoe_adapted_linear_backward: %lld rows (at most %lld) of %d and %d values (positive multiples of 8)", (long long)T,
+               (long long)kmoe_dense::ADAPTED_ROWS, K, N);
   KMOE_REQUIRE(adapter && adapter->a && adapter->b, KMOE_ERR_NULL, "kmoe_adapted_linear_backward: null adapter buffer");
   const int r = adapter->rank;
   KMOE_REQUIRE(n_adapters > 0 && n_adapters <= 32767 && r > 0 && r <= KMOE_MAX_RANK && r % 8 == 0, KMOE_ERR_SHAPE,

@@ -90,8 +90,9 @@ extern "C" int kmoe_dense_dx(const void* dy, const void* dy2, int lost, int64_t 
 
 extern "C" int kmoe_dense_wgrad(const void* a, const void* b, const void* a2, const void* b2, int64_t T, int M, int N,
                                 void* c, int c_dtype, void* stream) {
-  KMOE_REQUIRE(T >= 0 && T < ((int64_t)1 << 31) && M > 0 && N > 0 && M % 8 == 0 && N % 8 == 0, KMOE_ERR_SHAPE,
-               "kmoe_dense_wgrad: %lld rows of %d and %d values (positive multiples of 8)", (long long)T, M, N);
+  // (the rows are the product's K: its steps of up to 64 are counted in 32 bits)
+  KMOE_REQUIRE(T >= 0 && T < ((int64_t)1 << 31) - 63 && M > 0 && N > 0 && M % 8 == 0 && N % 8 == 0, KMOE_ERR_SHAPE,
+               "kmoe_dense_wgrad: %lld rows (below 2^31 - 63) of %d and %d values (positive multiples of 8)", (long long)T, M, N);
   KMOE_REQUIRE(c_dtype == KMOE_DTYPE_BF16 || c_dtype == KMOE_DTYPE_F32, KMOE_ERR_DTYPE, "kmoe_dense_wgrad: dtype %d", c_dtype);
   KMOE_REQUIRE(((a && b) || T == 0) && c && !a2 == !b2, KMOE_ERR_NULL, "kmoe_dense_wgrad: null buffer");
   KMOE_DENSE_ALIGNED("kmoe_dense_wgrad", a, b, a2, b2, c);

@@ -18,6 +18,9 @@ int launch_wgrad_two(const Args& g, hipStream_t s);     // a0^T b0 + a1^T b1
 // a b^T of few rows in runs of K (kmoe_ffn.hip)
 int launch_linear_runs(const Args& g, hipStream_t s);
 int launch_linear_runs_adapt(const Args& g, hipStream_t s);
+// The adapters' rows of one call: a launch of the inner products (a workgroup of 512 a 16 rows) has fewer than
+// 2^32 threads.
+constexpr int64_t ADAPTED_ROWS = (((int64_t)1 << 32) / 512 - 1) * 16;
 // v (2, T, rank): the scaled inner products of x with a, then what these lost by their rounding (and v2 with a2, of
 // one rank); rows without an adapter are left.  The caller has checked the sizes.
 int adapter_inner(const void* x, int64_t T, int K, const int32_t* ids, int n, int rank, const void* a, const float* scale,
@@ -69,7 +72,8 @@ template <int BM, int BN, int KS, int STAGES, bool SA, bool SB, int EPI, bool AD
 int launch_tile(const Args& g, hipStream_t s) {
   constexpr int CN = EPI == EPI_GATED ? BN / 2 : BN;
   const int64_t n_mt = kmoe::ceil_div<int64_t>(g.M, BM), n_nt = kmoe::ceil_div(g.N, CN);
-  KMOE_REQUIRE(n_mt * n_nt < (int64_t)1 << 31, KMOE_ERR_SHAPE, "kmoe dense product: %lld x %d results in one call",
+  // (a launch has fewer than 2^32 threads)
+  KMOE_REQUIRE(n_mt * n_nt < ((int64_t)1 << 32) / THREADS, KMOE_ERR_SHAPE, "kmoe dense product: %lld x %d results in one call",
                (long long)g.M, g.N);
   // (a tile's 32-bit offsets: 256 rows of a K-contiguous operand, 64 of a K-strided one, an adapter's rows)
   KMOE_REQUIRE(g.lda < (int64_t)1 << 22 && g.ldb < (int64_t)1 << 22, KMOE_ERR_SHAPE,

@@ -123,8 +123,10 @@ const uint16_t* bf(const void* p) { return static_cast<const uint16_t*>(p); }
 bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15) == 0; }
 size_t piece(int64_t bytes) { return (size_t)((bytes + 255) / 256 * 256); }
 
-int check_adapter(const char* who, const kmoe_adapter* a, int n) {
+int check_adapter(const char* who, const kmoe_adapter* a, int n, int64_t T) {
   if (!a) return KMOE_OK;
+  KMOE_REQUIRE(T <= ADAPTED_ROWS, KMOE_ERR_SHAPE, "%s: %lld rows with adapters (at most %lld)", who, (long long)T,
+               (long long)ADAPTED_ROWS);
   KMOE_REQUIRE(a->a && a->b, KMOE_ERR_NULL, "%s: null adapter buffer", who);
   KMOE_REQUIRE(n > 0 && a->rank > 0 && a->rank <= KMOE_MAX_RANK && a->rank % 8 == 0, KMOE_ERR_SHAPE,
                "%s: %d adapters of rank %d (a multiple of 8, at most %d)", who, n, a->rank, KMOE_MAX_RANK);
@@ -165,7 +167,7 @@ extern "C" int kmoe_adapted_linear(const void* x, int64_t T, int K, const void* 
                                    void* stream) {
   KMOE_REQUIRE(T >= 0 && T < ((int64_t)1 << 31) && K > 0 && N > 0 && K % 8 == 0 && N % 8 == 0, KMOE_ERR_SHAPE,
                "kmoe_adapted_linear: %lld rows of %d and %d values (positive multiples of 8)", (long long)T, K, N);
-  if (const int rc = check_adapter("kmoe_adapted_linear", adapter, n_adapters)) return rc;
+  if (const int rc = check_adapter("kmoe_adapted_linear", adapter, n_adapters, T)) return rc;
   if (T == 0) return KMOE_OK;
   KMOE_REQUIRE(x && w && y && (ids || !adapter), KMOE_ERR_NULL, "kmoe_adapted_linear: null buffer");
   KMOE_REQUIRE(aligned(x) && aligned(w) && aligned(y) && aligned(workspace), KMOE_ERR_SHAPE,
@@ -196,7 +198,7 @@ extern "C" int kmoe_gated_ffn(const void* x, int64_t T, int d, int F, const void
                "kmoe_gated_ffn: %lld rows, d=%d, F=%d (positive multiples of 8)", (long long)T, d, F);
   KMOE_REQUIRE(act >= KMOE_ACT_SILU && act <= KMOE_ACT_RELU, KMOE_ERR_UNSUPPORTED, "kmoe_gated_ffn: activation %d", act);
   for (const kmoe_adapter* a : {gate, up, down})
-    if (const int rc = check_adapter("kmoe_gated_ffn", a, n_adapters)) return rc;
+    if (const int rc = check_adapter("kmoe_gated_ffn", a, n_adapters, T)) return rc;
   KMOE_REQUIRE(!gate || !up || gate->rank == up->rank, KMOE_ERR_SHAPE,
                "kmoe_gated_ffn: the gate's and the up projection's adapters have one rank, got %d and %d", gate->rank, up->rank);
   if (T == 0) return KMOE_OK;

@@ -214,3 +214,25 @@ def test_odd_ranks_are_filled_up_inside_the_operator():
     assert held.a.shape == (2, 8, 64) and held.b.shape == (2, 72, 8)
     assert torch.equal(held.a[:, :5], a) and torch.equal(held.b[..., :5], b)
     assert not bool(held.a[:, 5:].any()) and not bool(held.b[..., 5:].any())
+
+
+def test_abi_refuses_launches_past_32_bits():
+    """Grids of 2^32 threads and counters of 2^31 rows, before anything is launched."""
+    a, lib = _lib.Adapter(0x1000, 0x1000, None, 8), _lib.load()
+    big = 1 << 62
+    call = _call("kmoe_adapted_linear", [FAKE, 1 << 27, 8, FAKE, 8, FAKE, 2, ctypes.byref(a), FAKE, FAKE, big, None])
+    assert call() == -2 and call(a1=(1 << 31) - 1) == -2
+    call = _call("kmoe_adapted_linear_backward", [FAKE, FAKE, 1 << 27, 8, FAKE, 8, FAKE, 2, ctypes.byref(a), FAKE, FAKE, FAKE, FAKE, FAKE,
+                                                  big, None])
+    assert call() == -2
+    call = _call("kmoe_gated_ffn", [FAKE, 1 << 27, 8, 8, FAKE, FAKE, FAKE, 0, FAKE, 2, None, None, ctypes.byref(a), FAKE, FAKE, big, None])
+    assert call() == -2
+    call = _call("kmoe_dense_linear", [FAKE, 0, (1 << 31) - 1, 8, FAKE, 8, FAKE, None])
+    assert call() == -2
+    call = _call("kmoe_dense_wgrad", [FAKE, FAKE, None, None, (1 << 31) - 63, 8, 8, FAKE, 0, None])
+    assert call() == -2
+    n = 1 << 35
+    assert lib.kmoe_adamw_values(FAKE, FAKE, FAKE, FAKE, n, 0, FAKE, FAKE, None) == -2
+    base = (ctypes.c_int32 * 2)(0, 1 << 24)
+    assert lib.kmoe_adamw(FAKE, FAKE, FAKE, base, 1, (ctypes.c_void_p * 1)(0x1000), 0, 32, 0, 1e-3, None, 0.9, 0.99, 1e-8, 0.0,
+                          FAKE, None) == -2
