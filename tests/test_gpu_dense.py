@@ -814,3 +814,112 @@ def test_shared_expert_keeps_the_result_type(dev, dtype, routing):
     z = layer(x.requires_grad_(True))
     z.float().sum().backward()
     assert z.dtype == y.dtype and x.grad.dtype == dtype
+
+
+# ---------------------------------------------------------------- how far off, all values together
+def check_rms(name, got, want, most):
+    """The root mean square of got's distance from want, against that of one rounding to bf16 of want itself.
+    Where a value passes two roundings of one size on its way, as a sum's own and its terms', it is
+    2^0.5 times as much; terms that went missing show, which the worst cases of long sums would cover."""
+    w = want.v
+    one = (w.to(BF).double() - w).square().mean().sqrt()
+    off = (got.double() - w).square().mean().sqrt()
+    assert float(off) <= most * float(one), (name, float(off / one))
+
+
+@pytest.mark.parametrize("T,d,F", [(300, 520, 264), (2042, 136, 1544), (16379, 136, 1096)] + LARGE)
+def test_block_is_two_roundings_off(dev, T, d, F):
+    """Past 32 rows h, dgate and dup are rounded to bf16, and so is each result."""
+    x, wg, wu, wd = make_ffn(dev, T, d, F)
+    dy = rnd(dev, T, d)
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = kmoe.gated_ffn(*leaves)
+    want, h, p, q = B.ffn(x, wg, wu, wd, "silu")
+    for name, g, w in zip(("y", "dx", "dwg", "dwu", "dwd"), (y.detach(), *torch.autograd.grad(y, leaves, dy)),
+                          (want, *B.ffn_grads(x, wg, wu, wd, dy, h, p, q))):
+        check_rms(name, g, w, 1.5)
+
+
+@pytest.mark.parametrize("T,d,F", [(8, 520, 264), (24, 2056, 1096)])
+def test_few_rows_are_one_rounding_off(dev, T, d, F):
+    x, wg, wu, wd = make_ffn(dev, T, d, F)
+    dy = rnd(dev, T, d)
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = kmoe.gated_ffn(*leaves)
+    want, h, p, q = B.ffn(x, wg, wu, wd, "silu")
+    for name, g, w in zip(("y", "dx", "dwg", "dwu", "dwd"), (y.detach(), *torch.autograd.grad(y, leaves, dy)),
+                          (want, *B.ffn_grads(x, wg, wu, wd, dy, h, p, q))):
+        check_rms(name, g, w, 1.1)
+
+
+@pytest.mark.parametrize("T,K,N,n,r", [(300, 520, 264, 3, 16), (2042, 1032, 2056, 4, 16), (8195, 264, 1096, 11, 40)])
+def test_projection_is_two_roundings_off(dev, T, K, N, n, r):
+    """The result and dx have an adapter's inner products in bf16 at most; the factors' gradients those in two."""
+    x, w, ad = rnd(dev, T, K), rnd(dev, N, K, std=K ** -0.5), make_ad(dev, n, r, K, N)
+    ids, dy = make_ids(dev, T, n, "mixed"), rnd(dev, T, N)
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, ad.a, ad.b)]
+    y = kmoe.adapted_linear(leaves[0], leaves[1], kmoe.Adapters(leaves[2], leaves[3], ad.scale), ids)
+    dx, dw, da, db = torch.autograd.grad(y, leaves, dy)
+    back = kmoe.Adapters(ad.b.transpose(1, 2), ad.a.transpose(1, 2), ad.scale)
+    check_rms("y", y.detach(), B.adapted(B.V(x), B.V(w), ad, ids), 1.5)
+    check_rms("dx", dx, B.adapted(B.V(dy), B.V(w.t()), back, ids), 1.5)
+    check_rms("dw", dw, B.mm(B.V(dy).t(), B.V(x)), 1.1)
+    for i in range(n):
+        t, s = (ids == i).nonzero().squeeze(1), float(ad.scale[i])
+        check_rms("da", da[i], B.mm((B.mm(B.V(dy[t]), B.V(ad.b[i])) * s).t(), B.V(x[t])), 1.1)
+        check_rms("db", db[i], B.mm(B.V(dy[t]).t(), B.mm(B.V(x[t]), B.V(ad.a[i]).t()) * s), 1.1)
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu_tanh"])
+@pytest.mark.parametrize("T", [3, 50, 300])
+@pytest.mark.parametrize("which", [(1, 1, 1), (1, 0, 0), (0, 1, 0), (0, 0, 1)])
+def test_block_adapters_gradients(dev, T, which, act):
+    """Every gradient of the block with adapters against the formula's, with the roundings of its three
+    projections: pre-activations, h and the gradients between the projections are bf16."""
+    d, F, n = 136, 200, 4
+    x, wg, wu, wd = make_ffn(dev, T, d, F)
+    ads = [make_ad(dev, n, r, *kn) if k else None for k, kn, r in zip(which, ((d, F), (d, F), (F, d)), (16, 16, 24))]
+    ids, dy = make_ids(dev, T, n, "mixed"), rnd(dev, T, d)
+    leaves = [t.clone().requires_grad_(True) for t in (x, wg, wu, wd)]
+    factors = [tuple(t.clone().requires_grad_(True) for t in ad[:2]) if ad else None for ad in ads]
+    y = kmoe.gated_ffn(*leaves, act, kmoe.FFNAdapters(*(f and kmoe.Adapters(*f, ad.scale) for f, ad in zip(factors, ads))), ids)
+    every = leaves + [t for f in factors if f for t in f]
+    got = dict(zip(map(id, every), torch.autograd.grad(y, every, dy)))
+    V, turned = B.V, [ad and kmoe.Adapters(ad.b.transpose(1, 2), ad.a.transpose(1, 2), ad.scale) for ad in ads]
+    g, u = B.adapted(V(x), V(wg), ads[0], ids).bf16(), B.adapted(V(x), V(wu), ads[1], ids).bf16()
+    a, slope = B.act(act, g)
+    h = (a * u).bf16()
+    dh = B.adapted(V(dy), V(wd).t(), turned[2], ids).bf16()
+    dg, du = (dh * u * slope).bf16(), (dh * a).bf16()
+    dx = B.adapted(dg, V(wg).t(), turned[0], ids).bf16() + B.adapted(du, V(wu).t(), turned[1], ids).bf16()
+    # eight roundings to bf16 on the way to any of them, independent and each of 2^-8 3^-0.5 of its value at most
+    # in the root mean square; the pre-activations' reach h and the slopes by up to 1.13: 3 2^-8 in all
+    def close(name, a, b):
+        B.check(name, a, b)
+        assert float((a.double() - b.v).norm()) <= 3 * 2.0 ** -8 * float(b.v.norm()), name
+    close("dx", got[id(leaves[0])], dx)
+    for name, leaf, w in zip(("dwg", "dwu", "dwd"), leaves[1:], (B.mm(dg.t(), V(x)), B.mm(du.t(), V(x)), B.mm(V(dy).t(), h))):
+        close(name, got[id(leaf)], w)
+    for name, ad, f, rows, grad in zip(("gate", "up", "down"), ads, factors, (V(x), V(x), h), (dg, du, V(dy))):
+        for i in range(n) if ad else ():
+            t, s = (ids == i).nonzero().squeeze(1), float(ad.scale[i])
+            if t.numel() == 0:
+                assert not bool(got[id(f[0])][i].any()) and not bool(got[id(f[1])][i].any())
+                continue
+            rt, gt = V(rows.v[t], rows.e[t]), V(grad.v[t], grad.e[t])
+            close((name, "da"), got[id(f[0])][i], B.mm((B.mm(gt, V(ad.b[i])) * s).bf16().t(), rt))
+            close((name, "db"), got[id(f[1])][i], B.mm(gt.t(), (B.mm(rt, V(ad.a[i]).t()) * s).bf16()))
+    # the formula itself, by torch's gradients in 64 bits
+    ref = [t.detach().double().requires_grad_(True) for t in every]
+    it = iter(ref[4:])
+    pairs = [(next(it), next(it)) if f else None for f in factors]
+
+    def project(v, w, ad, f):
+        out = v @ w.t()
+        for i in range(n) if f else ():
+            out = out + (ids == i)[:, None] * (float(ad.scale[i]) * (v @ f[0][i].t()) @ f[1][i].t())
+        return out
+    gates = [project(ref[0], w, ad, f) for w, ad, f in zip(ref[1:3], ads, pairs)]
+    out = project(B.TORCH_ACT[act](gates[0]) * gates[1], ref[3], ads[2], pairs[2])
+    for leaf, w in zip(every, torch.autograd.grad(out, ref, dy.double())):
+        assert float((got[id(leaf)].double() - w).norm()) <= 3 * 2.0 ** -8 * float(w.norm())
