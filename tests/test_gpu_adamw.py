@@ -440,3 +440,25 @@ def test_replays_after_a_load(dev):
         eager.step()
     torch.cuda.synchronize()
     assert torch.equal(p, q) and all(bool((t == 7.0).all()) for t in other)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_tensor_past_32_bits(dev, bits):
+    """More than 2^31 values: the first, the middle and the last ones are stepped as a small tensor of theirs is."""
+    n, part = (1 << 31) + 1234 * 256 + 77, 256 * 40
+    gen = torch.Generator(device=dev).manual_seed(3)
+    p = torch.nn.Parameter(torch.empty(n, device=dev, dtype=torch.bfloat16).normal_(0.0, 0.02, generator=gen))
+    p.grad = torch.empty(n, device=dev, dtype=torch.bfloat16).normal_(0.0, 1e-3, generator=gen)
+    cuts = [slice(0, part), slice((1 << 31) - part, (1 << 31) + part), slice((n - part) // 256 * 256, n)]
+    qs = [torch.nn.Parameter(p.detach()[c].clone()) for c in cuts]
+    opt, small = kmoe.AdamW([p], state_bits=bits, **HYPER), kmoe.AdamW(qs, state_bits=bits, **HYPER)
+    for t in range(2):
+        for q, c in zip(qs, cuts):
+            q.grad = p.grad[c].clone()
+        opt.step()
+        small.step()
+    m, root = (opt.state_values(p, torch.bfloat16))
+    for q, c in zip(qs, cuts):
+        assert torch.equal(p.detach()[c], q.detach())
+        assert all(torch.equal(a[c], b) for a, b in zip((m, root), small.state_values(q, torch.bfloat16)))
+    assert int(opt.state[p]["step"]) == 2

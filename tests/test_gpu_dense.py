@@ -923,3 +923,122 @@ def test_block_adapters_gradients(dev, T, which, act):
     out = project(B.TORCH_ACT[act](gates[0]) * gates[1], ref[3], ads[2], pairs[2])
     for leaf, w in zip(every, torch.autograd.grad(out, ref, dy.double())):
         assert float((got[id(leaf)].double() - w).norm()) <= 3 * 2.0 ** -8 * float(w.norm())
+
+
+def test_shared_expert_under_mod_by_value(dev):
+    """With a shared expert the kept rows' outputs are those without it plus the block's, weighted alike."""
+    c = kmoe.AdvancedMoEConfig(d_model=128, d_ff_expert=136, n_experts=4, moe_shared_d_ff=264, mod_enabled=True,
+                               residual_dropout=0.0)
+    torch.manual_seed(8)
+    mod = kmoe.MoDMoE(c).to(dev).to(BF).train()
+    x, res = rnd(dev, 2, 64, 128), rnd(dev, 2, 64, 128)
+    shared = mod.ffn.shared_expert
+    with torch.no_grad():
+        y = mod(x, res)
+        mod.ffn._modules["shared_expert"] = None
+        base = mod(x, res)
+        mod.ffn._modules["shared_expert"] = shared
+        sel = mod.ffn_mod_router.select(x)
+        rows = sel.sel_idx.long()
+        s = shared(torch.stack([x[b, rows[b]] for b in range(2)])).double()
+    add = torch.zeros(2, 64, 128, device=dev, dtype=torch.float64)
+    for b in range(2):
+        add[b, rows[b]] = sel.sel_w[b].double()[:, None] * s[b]
+    want = base.double() + add
+    # half a step of bf16 each: base's and y's own rounding; the experts' rows twice (theirs and their sum with
+    # the block's) and the block's twice, with the rows' weights
+    off = B.H * (base.double().abs() + want.abs() + 2 * (base.double() - res.double()).abs() + 2 * add.abs())
+    assert bool(((y.double() - want).abs() <= 1.01 * off + 1e-6).all())
+    assert float(add.abs().max()) > 0.01
+
+
+def test_no_rows_with_adapters(dev):
+    """No tokens: results of no rows, zero gradients of the adapters."""
+    x, wg, wu, wd = make_ffn(dev, 3, 64, 72)
+    ads = [make_ad(dev, 2, 8, 64, 72), make_ad(dev, 2, 8, 64, 72), make_ad(dev, 2, 5, 72, 64)]
+    e, ids = x[:0].clone().requires_grad_(True), torch.zeros(0, device=dev, dtype=torch.int64)
+    with torch.no_grad():
+        assert kmoe.gated_ffn(e, wg, wu, wd, "silu", kmoe.FFNAdapters(*ads), ids).shape == (0, 64)
+        assert kmoe.adapted_linear(e, wg, ads[0], ids).shape == (0, 72)
+    f = [t.clone().requires_grad_(True) for a in ads for t in a[:2]]
+    y = kmoe.gated_ffn(e, wg, wu, wd, "silu", kmoe.FFNAdapters(*(kmoe.Adapters(*f[2 * i:2 * i + 2]) for i in range(3))), ids)
+    y.sum().backward()
+    assert e.grad.shape == (0, 64) and all(bool((t.grad == 0).all()) for t in f)
+
+
+# ---------------------------------------------------------------- offsets past 32 bits
+def test_rows_past_32_bits(dev):
+    """More than 2^31 values of x, of dy's gradient and of h."""
+    T, K, N, n, r = (1 << 20) + 5, 2056, 72, 3, 8
+    g = torch.Generator(device=dev).manual_seed(1)
+    x = torch.empty(T, K, device=dev, dtype=BF).normal_(generator=g)
+    w, ad, dy = rnd(dev, N, K, std=K ** -0.5), make_ad(dev, n, r, K, N), torch.empty(T, N, device=dev, dtype=BF).normal_(generator=g)
+    ids = torch.randint(-1, n, (T,), device=dev, generator=g)
+    leaves = [t.requires_grad_(True) for t in (x, ad.a, ad.b)]
+    y = kmoe.adapted_linear(x, w, kmoe.Adapters(leaves[1], leaves[2], ad.scale), ids)
+    dx, da, db = torch.autograd.grad(y, leaves, dy)
+    y, x, a, b = (t.detach() for t in (y, *leaves))
+    ad, back = kmoe.Adapters(a, b, ad.scale), kmoe.Adapters(b.transpose(1, 2), a.transpose(1, 2), ad.scale)
+    for rows in (slice(0, 300), slice(T // 2, T // 2 + 300), slice(T - 300, T)):
+        B.check("y", y[rows], B.adapted(B.V(x[rows]), B.V(w), ad, ids[rows]))
+        B.check("dx", dx[rows], B.adapted(B.V(dy[rows]), B.V(w.t()), back, ids[rows]))
+    wa, wb = torch.zeros(n, r, K, device=dev, dtype=torch.float64), torch.zeros(n, N, r, device=dev, dtype=torch.float64)
+    for t0 in range(0, T, 1 << 17):
+        xs, ds, own = x[t0:t0 + (1 << 17)].double(), dy[t0:t0 + (1 << 17)].double(), ids[t0:t0 + (1 << 17)]
+        for i in range(n):
+            on = (own == i)[:, None] * float(ad.scale[i])
+            wa[i] += (ds @ b[i].double() * on).t() @ xs
+            wb[i] += ds.t() @ (xs @ a[i].double().t() * on)
+    check_rms("da", da, B.V(wa), 1.1)
+    check_rms("db", db, B.V(wb), 1.1)
+
+
+def test_block_past_32_bits(dev):
+    T, d, F = (1 << 18) + 3, 72, 8200
+    x, wg, wu, wd = make_ffn(dev, T, d, F)
+    dy = rnd(dev, T, d)
+    leaves = [t.requires_grad_(True) for t in (x, wg, wu, wd)]
+    y = kmoe.gated_ffn(*leaves)
+    grads = torch.autograd.grad(y, leaves, dy)
+    y, x, wg, wu, wd = (t.detach() for t in (y, *leaves))
+    sums = [torch.zeros(F, d, device=dev, dtype=torch.float64), torch.zeros(F, d, device=dev, dtype=torch.float64),
+            torch.zeros(d, F, device=dev, dtype=torch.float64)]
+    for t0 in range(0, T, 1 << 14):
+        rows = slice(t0, t0 + (1 << 14))
+        xs, ds = x[rows].double(), dy[rows].double()
+        gate, up = xs @ wg.double().t(), xs @ wu.double().t()
+        s = torch.sigmoid(gate)
+        a, dh = gate * s, ds @ wd.double()
+        dg, du = dh * up * s * (1 + gate * (1 - s)), dh * a
+        check_rms("y", y[rows], B.V((a * up) @ wd.double().t()), 1.5)
+        check_rms("dx", grads[0][rows], B.V(dg @ wg.double() + du @ wu.double()), 1.5)
+        for total, part in zip(sums, (dg.t() @ xs, du.t() @ xs, ds.t() @ (a * up))):
+            total += part
+    for name, g, w in zip(("dwg", "dwu", "dwd"), grads[1:], sums):
+        check_rms(name, g, B.V(w), 1.5)
+
+
+def test_adapters_past_32_bits(dev):
+    """Factors of many adapters: more than 2^31 values each, the last ones used."""
+    T, K, N, n, r = 130, 1032, 1032, 16500, 128
+    x, w, dy = rnd(dev, T, K), rnd(dev, N, K, std=K ** -0.5), rnd(dev, T, N)
+    a, b = torch.zeros(n, r, K, device=dev, dtype=BF), torch.zeros(n, N, r, device=dev, dtype=BF)
+    used = (0, n // 2, n - 2, n - 1)
+    for i in used:
+        a[i], b[i] = rnd(dev, r, K, std=K ** -0.5), rnd(dev, N, r, std=0.3)
+    ids = torch.tensor(used, device=dev)[torch.arange(T, device=dev) % 4]
+    ad = kmoe.Adapters(a.requires_grad_(True), b.requires_grad_(True))
+    lx = x.clone().requires_grad_(True)
+    y = kmoe.adapted_linear(lx, w, ad, ids)
+    dx, da, db = torch.autograd.grad(y, (lx, a, b), dy)
+    few = kmoe.Adapters(a.detach()[list(used)], b.detach()[list(used)])
+    back, at = kmoe.Adapters(few.b.transpose(1, 2), few.a.transpose(1, 2)), torch.arange(T, device=dev) % 4
+    for rows in (slice(0, T), slice(0, 5)):
+        with torch.no_grad():
+            B.check("y", kmoe.adapted_linear(x[rows], w, ad, ids[rows]), B.adapted(B.V(x[rows]), B.V(w), few, at[rows]))
+    B.check("dx", dx, B.adapted(B.V(dy), B.V(w.t()), back, at))
+    for k, i in enumerate(used):
+        t = at == k
+        B.check("da", da[i], B.mm(B.mm(B.V(dy[t]), B.V(few.b[k])).bf16().t(), B.V(x[t])))
+        B.check("db", db[i], B.mm(B.V(dy[t]).t(), B.mm(B.V(x[t]), B.V(few.a[k]).t()).bf16()))
+    assert not bool(da[1:n // 2].any()) and not bool(db[n // 2 + 1:n - 2].any())
