@@ -8,7 +8,7 @@ outside of torch's operations and counts the change, so what the modules keep fr
 from __future__ import annotations
 
 import ctypes
-import operator
+from operator import is_ as _is
 from typing import Optional
 
 import torch
@@ -47,8 +47,10 @@ class _Plan:
         self.bits = 8 if "exp_avg_scale" in states[0] else 32
         self.dtype = _lib.DTYPE_F32 if params[0].dtype == torch.float32 else _lib.DTYPE_BF16
         self.device = dev
-        self.at = [(p.data_ptr(), p.numel(), p.dtype) for p in params]
-        self.held = [[(k, t, t.data_ptr()) for k, t in st.items()] for st in states]
+        self.kind = params[0].dtype
+        self.shapes = [p.shape for p in params]
+        self.at = [(p, p.data_ptr(), p.shape, st, list(st.values()), [t.data_ptr() for t in st.values()])
+                   for p, st in zip(params, states)]
 
     @staticmethod
     def _apart(params, states):
@@ -63,15 +65,15 @@ class _Plan:
     def _where(p, st):
         return [p.data_ptr(), *(st[k].data_ptr() if k in st else 0 for k in _FIELDS)]
 
-    def current(self, state) -> bool:
-        """Whether the tensors are those of the optimizer's `state`, each of them where it was and the
-        parameters what they were."""
-        for p, st, at, held in zip(self.params, self.states, self.at, self.held):
-            if state.get(p) is not st or len(st) != len(held) or (p.data_ptr(), p.numel(), p.dtype) != at or not p.is_contiguous():
+    def current(self) -> bool:
+        """Whether the states hold the same tensors, each tensor is where it was and the parameters are what
+        they were."""
+        kind = self.kind
+        for p, at, shape, st, tensors, places in self.at:
+            if p.data_ptr() != at or p.shape != shape or p.dtype is not kind or not p.is_contiguous():
                 return False
-            for k, t, a in held:
-                if st.get(k) is not t or t.data_ptr() != a:
-                    return False
+            if len(st) != len(tensors) or not all(map(_is, st.values(), tensors)) or [t.data_ptr() for t in tensors] != places:
+                return False
         return True
 
 
@@ -94,7 +96,7 @@ class AdamW(torch.optim.Optimizer):
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, state_bits=32,
                  master_weights=False):
         self._check(dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
-        self._plans, self._stepped, self._held, self._seen = None, [], [], {}
+        self._plans, self._stepped, self._states, self._held, self._seen = None, [], ([], []), [], {}
         super().__init__(params, dict(lr=lr, betas=tuple(betas), eps=eps, weight_decay=weight_decay, state_bits=state_bits,
                                       master_weights=bool(master_weights)))
 
@@ -130,15 +132,16 @@ class AdamW(torch.optim.Optimizer):
         if not p.is_contiguous():
             raise ValueError(f"kmoe.AdamW: parameters are contiguous, got strides {p.stride()} of {tuple(p.shape)}")
 
-    # _plans: the tables of the last step, _stepped: each group's parameters in them; _held: what
+    # _plans: the tables of the last step, _stepped: each group's parameters in them, _states: the state that
+    # they were made from; _held: what
     # captured steps read; _seen: version of each parameter with an f32 copy after its last step
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._plans, self._stepped, self._seen = None, [], {}
+        self._plans, self._stepped, self._states, self._seen = None, [], ([], []), {}
         self.__dict__.setdefault("_held", [])  # (torch's load_state_dict comes here too: graphs stay)
 
     def __getstate__(self):
-        return {k: v for k, v in super().__getstate__().items() if k not in ("_plans", "_stepped", "_held", "_seen")}
+        return {k: v for k, v in super().__getstate__().items() if k not in ("_plans", "_stepped", "_states", "_held", "_seen")}
 
     # ---------------------------------------------------------------- states
     def _new_state(self, p, group):
@@ -207,7 +210,7 @@ class AdamW(torch.optim.Optimizer):
     def load_state_dict(self, state_dict) -> None:
         """As torch's, but the states keep the types they were saved in (torch casts them to their
         parameter's); what is refused leaves the optimizer as it was."""
-        before = self.state, self.param_groups, self._plans, self._stepped, self._seen
+        before = self.state, self.param_groups, self._plans, self._stepped, self._states, self._seen
         super().load_state_dict(state_dict)
         try:
             saved, states = state_dict["state"], {}
@@ -225,7 +228,7 @@ class AdamW(torch.optim.Optimizer):
                     self._check_state(p, self._group_of(p), st)
                     states[p] = st
         except Exception:
-            self.state, self.param_groups, self._plans, self._stepped, self._seen = before
+            self.state, self.param_groups, self._plans, self._stepped, self._states, self._seen = before
             raise
         self.state.update(states)
         self._seen.update((p, p._version) for p in states)
@@ -254,16 +257,20 @@ class AdamW(torch.optim.Optimizer):
                 # (a state of another form than the group's has been refused)
             for (_, _, master), ps in kinds.items():
                 plans.append((group, _Plan(ps, [self.state[p] for p in ps], master)))
-        self._plans, self._stepped = plans, stepped
+        self._plans, self._stepped, self._states = plans, stepped, (list(self.state), list(self.state.values()))
 
     def _stale(self) -> bool:
         if self._plans is None or len(self._stepped) != len(self.param_groups):
             return True
         for group, (known, ps) in zip(self.param_groups, self._stepped):
             now = self._to_step(group)
-            if group is not known or len(now) != len(ps) or not all(map(operator.is_, now, ps)):
+            if group is not known or len(now) != len(ps) or not all(map(_is, now, ps)):
                 return True
-        return not all(plan.current(self.state) for _, plan in self._plans)
+        # (the whole state entry by entry: a parameter's own would be looked up by its hash, which costs more)
+        keys, states = self._states
+        if len(self.state) != len(keys) or not all(map(_is, self.state, keys)) or not all(map(_is, self.state.values(), states)):
+            return True
+        return not all(plan.current() for _, plan in self._plans)
 
     @torch.no_grad()
     def step(self, closure=None) -> Optional[torch.Tensor]:
@@ -287,12 +294,13 @@ class AdamW(torch.optim.Optimizer):
                     lr_dev, lr = lr.data_ptr(), 0.0
                 else:
                     lr = float(lr)
+            kind, dev, shapes = plan.kind, plan.device, plan.shapes
             for i, p in enumerate(plan.params):
                 g = p.grad
                 if g is None:
                     plan.grads[i] = None
                     continue
-                if g.is_sparse or g.dtype != p.dtype or g.device != p.device or g.shape != p.shape:
+                if g.dtype is not kind or g.shape != shapes[i] or g.device != dev or g.is_sparse:
                     raise ValueError(f"kmoe.AdamW: gradients are dense and of their parameter's type, device and shape, got "
                                      f"{g.dtype} {tuple(g.shape)} on {g.device}")
                 if not g.is_contiguous():
