@@ -13,8 +13,9 @@
 // values then meet in one lane.  Four waves and not more: LDS moves 128 bytes a cycle, every fragment
 // has to feed as many MFMAs as a wave can hold (256 x 256 with eight waves of 128 x 64: reads and
 // loads took longer than the MFMAs, 16384 rows, d 2048, F 5632, down 352 us; the MFMAs alone 189).
-// Measured, back to back: gate and up 558 us (1.36 PFLOP/s; a library product of the shape 552), down
-// 288 (304), dx 673, weight gradients 344 each (291).  Bound by the chip's power on such data.
+// Measured on normal numbers, 60 ms back to back: gate and up 563 us (1.34 PFLOP/s; a library product of
+// the shape 527), down 259 (243), dx 578 (567), weight gradients 311 each (349); in the first
+// milliseconds after a pause all take some 20% longer.  Bound by the chip's power on such data.
 // K advances 32 or 64 (32 KS) per step.  A step's 16-byte pieces go from memory to LDS without passing registers,
 // each lane picking the piece that belongs where the hardware puts it, so the swizzle costs nothing:
 //   K-contiguous tiles: rows of 64 KS bytes, 16-byte chunks XOR-ed by (row / 2) modulo their number;
@@ -251,8 +252,8 @@ __device__ __forceinline__ void list_adapters(int n_adapters, int rows, int tid,
 // part too where it costs little (tiles of 64 rows) and where such an error, which reaches a whole
 // row, adds to those of the hidden values' rounding (GATED; the block's result was 1.7 times as far
 // off as with one rounding, now 1.4).
-// (16 adapters of rank 16 in turn, 48 rows, F 5632, gate
-// and up: 4 us; read and selected turn by turn 25).
+// (48 rows, F 5632, gate and up: 10.7 us, with 16 adapters of rank 16 in turn 18.6; read and selected turn
+// by turn they took 25 us more).
 template <int BM, int BN, bool GATED>
 struct Outer {
   static constexpr int QA = BM / 64, QB = BN / 64, H = GATED ? 2 : 1, C = QB == 1 ? 8 : 1;

@@ -32,16 +32,17 @@ int launch_sum_runs(const float* part, int runs, int64_t total, uint16_t* out, h
 // time for 64 of K with every place taken and with one workgroup a unit, and what a round costs
 // besides (us; from the down product of 16384 to 48 rows, d 2048, F 5632, and the others of these sizes).
 // 256 x 256 and 192 x 256 lie alone on a unit, a fuller chip clocks lower; 128 x 128 two side by side, or
-// one with twice the stages; 64 x 128 and 64 x 64 two side by side.  Measured, us:
+// one with twice the stages; 64 x 128 and 64 x 64 two side by side.  The rates are those of the first
+// milliseconds after a pause; measured 60 ms back to back, at the clocks that the chip then holds, us:
 //                        256x256 192x256 128x128 128x128/4  64x128  64x64
-//   16384 rows, gate up    664     690     784       886      981
-//   16384 rows, down       291     350     358       421      494
-//    2042 rows, gate up    100      89     100       117      127
-//    2042 rows, down       103      89      67        49       59
-//     777 rows, gate up     49      41      53        55       53
-//     777 rows, down        99      85      56        40       31
-//     128 rows, gate up     39      33      23        23       19       21
-//      48 rows, gate up     37      31      22        18       18       13
+//   16384 rows, gate up    563     605     664       794      859     1071
+//   16384 rows, down       259     298     322       355      429      559
+//    2042 rows, gate up     92      82      90       108      110      137
+//    2042 rows, down        99      85      61        46       56       71
+//     777 rows, gate up     42      38      50        51       49       58
+//     777 rows, down        98      82      54        37       29       35
+//     128 rows, gate up     43      41      30        23       18       21
+//      48 rows, gate up     42      40      30        18       18       12
 enum Tile { T256, T192, T128, T128_DEEP, T64X128, T64 };
 inline Tile choose_tile(int64_t M, int64_t cols, double steps, int from = T256, double* us = nullptr) {
   struct Rate {

@@ -11,7 +11,8 @@ Numerics: bf16 operands, f32 sums.  What is rounded to bf16 between the products
 values h = act(g) u and the gradients of its pre-activations (of up to 32 rows both keep 16 bits, as
 two bf16: in few results a rounding does not average out), and an adapter's inner products with
 their scale (16 bits for the factors' gradients).  What the backward keeps of the pre-activations,
-u act'(g) and act(g), has 16 bits of precision.
+u act'(g) and act(g), has 16 bits of precision.  An infinite weight or factor gives the infinities of the
+formula in the results of its rows; gradients summed over a row with an infinity are not finite.
 """
 from __future__ import annotations
 
