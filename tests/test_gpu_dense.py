@@ -1042,3 +1042,76 @@ def test_adapters_past_32_bits(dev):
         B.check("da", da[i], B.mm(B.mm(B.V(dy[t]), B.V(few.b[k])).bf16().t(), B.V(x[t])))
         B.check("db", db[i], B.mm(B.V(dy[t]).t(), B.mm(B.V(x[t]), B.V(few.a[k]).t()).bf16()))
     assert not bool(da[1:n // 2].any()) and not bool(db[n // 2 + 1:n - 2].any())
+
+
+@pytest.mark.parametrize("r", [8, 16, 32])
+@pytest.mark.parametrize("T", [14, 30, 60, 300])
+def test_many_infinite_adapters_stay_apart(dev, T, r):
+    """Every second of many adapters with infinities: turns of the tile with and without them, in every place of
+    a group of turns; the others' rows are the same bit for bit, and theirs are the formula's."""
+    d, F, n = 72, 264, 150
+    x, wg, wu, wd = make_ffn(dev, T, d, F)
+    ads = [make_ad(dev, n, k, *kn) for kn, k in (((d, F), r), ((d, F), r), ((F, d), r))]
+    bad = [a._replace(b=a.b.clone()) for a in ads]
+    ids = torch.arange(T, device=dev) * 7 % n
+    for i in range(0, n, 3):
+        bad[1].b[i, i % F, i % r], bad[2].b[i, i % d, (i + 1) % r] = float("inf"), float("-inf")
+    clean = ids % 3 != 0
+    with torch.no_grad():
+        y, z = (kmoe.gated_ffn(x, wg, wu, wd, "silu", kmoe.FFNAdapters(*a), ids) for a in (ads, bad))
+        assert torch.equal(y[clean], z[clean]) and not bool(torch.isfinite(z[~clean]).all(dim=1).any())
+        p, q = (kmoe.adapted_linear(x, wu, a, ids) for a in (ads[1], bad[1]))
+    assert torch.equal(p[clean], q[clean])
+    finite = ~(torch.arange(F, device=dev)[None] == (ids % F)[:, None])
+    assert torch.equal(p[~clean][finite[~clean]], q[~clean][finite[~clean]])
+    want = x.double() @ wu.double().t()
+    for t in range(T):
+        i = int(ids[t])
+        want[t] += float(ads[1].scale[i]) * (x[t].double() @ ads[1].a[i].double().t()) @ bad[1].b[i].double().t()
+    same_infinities(q, want)
+
+
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("T", [12, 300])
+def test_captured_training_steps(dev, T, bits):
+    """Forward, backward and optimizer step of the block and of adapters on it in one graph: its replays are the
+    eager steps, bit for bit, with eager passes of the same weights between them."""
+    x, dy = rnd(dev, T, 72), rnd(dev, T, 72)
+    ids = make_ids(dev, T, 3, "mixed").to(torch.int32)
+    start = [*make_ffn(dev, T, 72, 136)[1:], *make_ad(dev, 3, 5, 72, 136)[:2], *make_ad(dev, 3, 8, 136, 72)[:2]]
+
+    def make():
+        ps = [torch.nn.Parameter(t.clone()) for t in start]
+        for p in ps:
+            p.grad = torch.zeros_like(p)
+        return ps, kmoe.AdamW(ps, lr=1e-2, state_bits=bits, master_weights=True)
+
+    def run(ps, opt):
+        ads = kmoe.FFNAdapters(kmoe.Adapters(ps[3], ps[4]), None, kmoe.Adapters(ps[5], ps[6]))
+        y = kmoe.gated_ffn(x, *ps[:3], "gelu", ads, ids)
+        for p, g in zip(ps, torch.autograd.grad(y, ps, dy)):
+            p.grad.copy_(g)
+        opt.step()
+        return y.detach()
+    (ps, opt), (qs, eager) = make(), make()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(ps, opt)
+        run(qs, eager)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        y = run(ps, opt)
+    for _ in range(4):
+        x.mul_(-1.0)
+        ids.copy_(ids.roll(1))
+        graph.replay()
+        with torch.no_grad():
+            kmoe.gated_ffn(x, *ps[:3], "gelu")
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.default_stream())
+            want = run(qs, eager)
+        torch.cuda.synchronize()
+        assert torch.equal(y, want) and all(torch.equal(p, q) for p, q in zip(ps, qs))
+        assert all(torch.equal(opt.state[p][k], eager.state[q][k]) for p, q in zip(ps, qs) for k in opt.state[p])
