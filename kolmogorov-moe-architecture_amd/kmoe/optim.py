@@ -25,7 +25,7 @@ _FIELDS = ("exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "master
 class _Plan:
     """The tensors of a group of one type on one device, as the kernel's table has them."""
 
-    def __init__(self, params, states, has_master):
+    def __init__(self, params, states, bits, has_master):
         dev = params[0].device
         self._apart(params, states)
         rows, base, owner = [], [0], []
@@ -44,19 +44,19 @@ class _Plan:
         self.grads = (ctypes.c_void_p * len(rows))()
         self.params, self.states = params, states
         self.has_master = has_master
-        self.bits = 8 if "exp_avg_scale" in states[0] else 32
+        self.bits = bits
         self.dtype = _lib.DTYPE_F32 if params[0].dtype == torch.float32 else _lib.DTYPE_BF16
         self.device = dev
         self.kind = params[0].dtype
         self.shapes = [p.shape for p in params]
-        self.at = [(p, p.data_ptr(), p.shape, st, list(st.values()), [t.data_ptr() for t in st.values()])
+        self.at = [(p, p.data_ptr(), p.shape, st, [(k, st[k], st[k].data_ptr()) for k in _FIELDS if k in st])
                    for p, st in zip(params, states)]
 
     @staticmethod
     def _apart(params, states):
         """Refuses tensors that share memory: workgroups write them side by side."""
         places = sorted((t.data_ptr(), t.data_ptr() + t.numel() * t.element_size(), tuple(p.shape))
-                        for p, st in zip(params, states) for t in (p, *st.values()) if t.numel())
+                        for p, st in zip(params, states) for t in (p, *(st[k] for k in _FIELDS if k in st)) if t.numel())
         for (_, end, a), (start, _, b) in zip(places, places[1:]):
             if start < end:
                 raise ValueError(f"kmoe.AdamW: parameters {a} and {b} of one group, or states of theirs, share memory")
@@ -69,11 +69,12 @@ class _Plan:
         """Whether the states hold the same tensors, each tensor is where it was and the parameters are what
         they were."""
         kind = self.kind
-        for p, at, shape, st, tensors, places in self.at:
+        for p, at, shape, st, held in self.at:
             if p.data_ptr() != at or p.shape != shape or p.dtype is not kind or not p.is_contiguous():
                 return False
-            if len(st) != len(tensors) or not all(map(_is, st.values(), tensors)) or [t.data_ptr() for t in tensors] != places:
-                return False
+            for k, t, place in held:
+                if st.get(k) is not t or t.data_ptr() != place:
+                    return False
         return True
 
 
@@ -132,9 +133,9 @@ class AdamW(torch.optim.Optimizer):
         if not p.is_contiguous():
             raise ValueError(f"kmoe.AdamW: parameters are contiguous, got strides {p.stride()} of {tuple(p.shape)}")
 
-    # _plans: the tables of the last step, _stepped: each group's parameters in them, _states: the state that
-    # they were made from; _held: what
-    # captured steps read; _seen: version of each parameter with an f32 copy after its last step
+    # _plans: the tables of the last step, _stepped: each group's parameters in them and the form of their
+    # states, _states: the states that they were made from; _held: what captured steps read; _seen: version
+    # of each parameter with an f32 copy after its last step
     def __setstate__(self, state):
         super().__setstate__(state)
         self._plans, self._stepped, self._states, self._seen = None, [], ([], []), {}
@@ -164,6 +165,10 @@ class AdamW(torch.optim.Optimizer):
 
     def _check_state(self, p, group, st):
         want = self._new_state(torch.empty(p.shape, dtype=p.dtype, device="meta"), group)
+        odd = [k for k in _FIELDS if k in st and k not in want]
+        if odd:
+            raise ValueError(f"kmoe.AdamW: the state {', '.join(odd)} of a parameter {tuple(p.shape)} has no place in a group with "
+                             f"state_bits {group['state_bits']} and master_weights {group['master_weights']}")
         for k, v in want.items():
             t = st.get(k)
             if (not isinstance(t, torch.Tensor) or t.dtype != v.dtype or t.numel() != v.numel() or t.device != p.device
@@ -243,7 +248,7 @@ class AdamW(torch.optim.Optimizer):
         plans, stepped = [], []
         for group in self.param_groups:
             kinds = {}
-            stepped.append((group, self._to_step(group)))
+            stepped.append((group, self._to_step(group), group["state_bits"], group["master_weights"]))
             for p in stepped[-1][1]:
                 if not p.is_cuda:
                     raise ValueError("kmoe.AdamW: parameters must be on a GPU (the HIP kernel is the only implementation)")
@@ -256,15 +261,16 @@ class AdamW(torch.optim.Optimizer):
                 kinds.setdefault((p.device, p.dtype, "master" in self.state[p]), []).append(p)
                 # (a state of another form than the group's has been refused)
             for (_, _, master), ps in kinds.items():
-                plans.append((group, _Plan(ps, [self.state[p] for p in ps], master)))
+                plans.append((group, _Plan(ps, [self.state[p] for p in ps], group["state_bits"], master)))
         self._plans, self._stepped, self._states = plans, stepped, (list(self.state), list(self.state.values()))
 
     def _stale(self) -> bool:
         if self._plans is None or len(self._stepped) != len(self.param_groups):
             return True
-        for group, (known, ps) in zip(self.param_groups, self._stepped):
+        for group, (known, ps, bits, master) in zip(self.param_groups, self._stepped):
             now = self._to_step(group)
-            if group is not known or len(now) != len(ps) or not all(map(_is, now, ps)):
+            if (group is not known or group["state_bits"] != bits or group["master_weights"] != master or len(now) != len(ps)
+                    or not all(map(_is, now, ps))):
                 return True
         # (the whole state entry by entry: a parameter's own would be looked up by its hash, which costs more)
         keys, states = self._states

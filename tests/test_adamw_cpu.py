@@ -382,3 +382,46 @@ def test_values_of_no_state():
     with pytest.raises(ValueError, match="not a parameter"):
         opt.state_values(_param(5))
     assert not opt.state
+
+
+def test_states_of_another_form_are_refused(steps):
+    """Entries that the kernel would take for another form of states than the group's; a program's own entries
+    are left alone."""
+    f32 = lambda n: torch.zeros(n)
+    for bits, extra in ((32, dict(exp_avg_scale=f32(1))), (32, dict(exp_avg_sq_scale=f32(2))), (32, dict(master=f32(300))),
+                        (8, dict(master=f32(300)))):
+        (p,) = _on_gpu(300, dtype=torch.bfloat16)
+        opt = kmoe.AdamW([p], state_bits=bits)
+        good = {k: v for k, v in opt._new_state(p, opt.param_groups[0]).items() if k != "step"}
+        with pytest.raises(ValueError, match="has no"):
+            opt.set_state(p, 1, **good, **extra)
+        assert p not in opt.state
+        opt.step()
+        opt.state[p] = {**opt.state[p], **extra}
+        with pytest.raises(ValueError, match="has no"):
+            opt.step()
+        sd = opt.state_dict()
+        other = kmoe.AdamW([_param(300)], state_bits=bits)
+        with pytest.raises(ValueError, match="has no"):
+            other.load_state_dict(sd)
+        assert not other.state
+    for key, value in (("state_bits", 8), ("master_weights", True)):
+        (p,) = _on_gpu(300, dtype=torch.bfloat16)
+        opt = kmoe.AdamW([p])
+        opt.step()
+        opt.param_groups[0][key] = value
+        with pytest.raises(ValueError, match="the state"):
+            opt.step()
+    a, b = _on_gpu(5, 300)
+    opt = kmoe.AdamW([a, b])
+    opt.step()
+    opt.state[a]["note"], opt.state[b]["mean"] = "mine", torch.ones(7)
+    opt.step()
+    plans = opt._plans
+    opt.state[b]["mean"] = torch.zeros(9)
+    opt.step()
+    assert opt._plans is plans and steps[-1] == _want(opt, a, b)
+    other = kmoe.AdamW(_on_gpu(5, 300))
+    other.load_state_dict(opt.state_dict())
+    q, r = other.param_groups[0]["params"]
+    assert other.state[q]["note"] == "mine" and torch.equal(other.state[r]["mean"], torch.zeros(9))
