@@ -725,7 +725,8 @@ int kmoe_dense_wgrad(const void* a, const void* b, const void* a2, const void* b
                      int c_dtype, void* stream);
 /* The backward of kmoe_adapted_linear with an adapter and without a gradient of w (kmoe_dense_wgrad is
  * that one's): dx (T, K), da (n, r, K) and db (n, N, r) from dy (T, N), each where it is not NULL.
- * v (2, T, r): the forward's, for db.  At most 32767 adapters.  */
+ * v (2, T, r): the forward's, for db.  The workspace does for da and db and for either alone.  At
+ * most 32767 adapters.  */
 size_t kmoe_adapted_linear_backward_workspace_bytes(int64_t T, int K, int N, int n_adapters, int rank);
 int kmoe_adapted_linear_backward(const void* dy, const void* x, int64_t T, int K, const void* w, int N,
                                  const int32_t* ids, int n_adapters, const kmoe_adapter* adapter, const void* v,
